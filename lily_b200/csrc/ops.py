@@ -97,6 +97,12 @@ _SIGNATURES = {
     "lily_moe_gather": [_vp, _i, _vp, _i, _vp, _i, _i, _vp, _vp],
     "lily_moe_activation": [_vp, _i, _i, _vp, _i, _f, _f, _vp, _vp, _i, _vp, _vp],
     "lily_moe_relu2": [_vp, _i, _i, _vp, _vp, _vp, _i, _vp, _vp],
+    "lily_axes_rope_write": [_vp, _i, _i, _sz, _i, _vp, _vp, _i, _f, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _vp,
+                             _i, _i, _i, _i, _i, _i, _vp],
+    "lily_attention_decode_weighed": [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
+    "lily_key_weights": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
+    "lily_select_keys": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
+    "lily_move_keys": [_vp, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp],
     "lily_argmax": [_vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_apply_penalties": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_top_logprobs": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
@@ -134,6 +140,10 @@ def library():
         lib.lily_top_logprobs_cap.restype = _i
         lib.lily_attention_decode_scratch_floats.argtypes = [_i, _i, _i, _i]
         lib.lily_attention_decode_scratch_floats.restype = _sz
+        lib.lily_attention_decode_weighed_floats.argtypes = [_i, _i, _i, _i, _i]
+        lib.lily_attention_decode_weighed_floats.restype = _sz
+        lib.lily_key_weights_floats.argtypes = [_i, _i, _i]
+        lib.lily_key_weights_floats.restype = _sz
         lib.lily_normed_mean_max.restype = _i
         lib.lily_row_cluster_threads.argtypes = [_i]
         lib.lily_row_cluster_threads.restype = _i
@@ -1185,6 +1195,204 @@ def attention_decode_fused(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_
           float(softcap or 0.0), ld, kv_layer.shape[0], DECODE_POLLS, _stream())
     if splits > 1 and (stages or requests * nkv * -(-(nq // nkv) // 16) > decode_clusters(d, splits, nq // nkv)):
         launches["count"] += 1                                       # the combine kernel, launched inside
+
+
+# ------------------------------------------------------------------------------ a cache held to a budget of places
+
+def pair_axes(sections: Sequence[int], device, in_turn: bool = False) -> torch.Tensor:
+    """The axis of each rotated pair, int32 [sum(sections)]: ``sections[a]`` pairs belong to axis a, in runs (16, 24, 24: sixteen
+    pairs by time, 24 by height, 24 by width) or, ``in_turn``, one after the other (0, 1, 2, 0, 1, 2, ...) while an axis has pairs left."""
+    if not sections or any(int(n) != n or n < 0 for n in sections):
+        raise KernelError(f"pair_axes: sections {tuple(sections)} are not numbers of pairs")
+    if in_turn:
+        axes = [a for i in range(max(sections)) for a, n in enumerate(sections) if i < n]
+    else:
+        axes = [a for a, n in enumerate(sections) for _ in range(n)]
+    return torch.tensor(axes, dtype=torch.int32, device=device)
+
+
+def _layer_and_weights(what: str, kv_layer: torch.Tensor, weights: torch.Tensor, nkv: int, page_size: int, d: int) -> None:
+    cache_layer_fits(kv_layer, nkv, page_size, d, d)
+    if weights.dtype != torch.float32 or tuple(weights.shape) != (kv_layer.shape[0], nkv, page_size):
+        raise KernelError(f"{what}: weights are float32 [{kv_layer.shape[0]}, {nkv}, {page_size}], got {weights.dtype} {tuple(weights.shape)}")
+
+
+def _table(what: str, table: torch.Tensor, requests: int, name: str = "block_table") -> int:
+    if table.dim() != 2 or table.shape[0] != requests or table.shape[1] < 1:
+        raise KernelError(f"{what}: {name} is int32 [{requests}, pages], got {tuple(table.shape)}")
+    return table.shape[1]
+
+
+def axes_rope_write(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_gain: Optional[torch.Tensor], eps: float, cos: torch.Tensor,
+                    sin: torch.Tensor, positions: torch.Tensor, pair_axis: torch.Tensor, places: torch.Tensor, token_req: torch.Tensor,
+                    block_table: torch.Tensor, kv_layer: torch.Tensor, nq: int, nkv: int, d: int, rotary_dim: int, page_size: int,
+                    q_out: Optional[torch.Tensor] = None, row: Optional[int] = None) -> torch.Tensor:
+    """``qk_norm_rope_write`` for positions with several axes and a cache in which a token's place is not its position: per-head
+    RMSNorm of q and k (when gains are given), pair j of the first ``rotary_dim`` features rotated by the tables' row
+    ``positions[pair_axis[j], token]`` (``positions`` int32 [axes, tokens], ``pair_axis`` int32 [rotary_dim / 2]: ``pair_axes``), q to
+    ``q_out`` [tokens, nq * d], k and v to ``places[token]`` of the pages of request ``token_req[token]``.  ``qkv`` is [tokens,
+    (nq + 2 nkv) d] in the cache's dtype or float32 partial sums [splits, tokens, ...], its rows ``row`` numbers apart.  A position outside the
+    tables gives NaN; a place outside the block table is not written."""
+    _dev(qkv, q_gain, k_gain, cos, sin, positions, pair_axis, places, token_req, block_table, kv_layer, q_out)
+    n = qkv.shape[-2]
+    ld = int(row or (nq + 2 * nkv) * d)
+    splits, stride = _summed(qkv, n, ld, "axes_rope_write qkv")
+    if qkv.dtype not in (kv_layer.dtype, torch.float32):
+        raise KernelError(f"axes_rope_write: cache dtype {kv_layer.dtype} differs from activations {qkv.dtype}")
+    cache_layer_fits(kv_layer, nkv, page_size, d, d)
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape[1] != rotary_dim // 2 or sin.shape != cos.shape:
+        raise KernelError("axes_rope_write: rotation tables are float32 [positions, rotary_dim / 2]")
+    if positions.dim() != 2 or positions.shape[1] != n or pair_axis.numel() != rotary_dim // 2:
+        raise KernelError(f"axes_rope_write: positions are [axes, {n}] and there is an axis for each of the {rotary_dim // 2} pairs; got {tuple(positions.shape)} "
+                          f"and {pair_axis.numel()}")
+    if places.numel() != n or token_req.numel() != n or block_table.dim() != 2 or block_table.shape[1] < 1:
+        raise KernelError(f"axes_rope_write: {n} tokens have a place and a request each")
+    if (q_gain is None) != (k_gain is None) or (q_gain is not None and (q_gain.dtype != k_gain.dtype or q_gain.numel() != d or k_gain.numel() != d)):
+        raise KernelError("axes_rope_write: q and k gains come together, with one dtype and head_dim numbers each")
+    if q_out is None:
+        q_out = torch.empty((n, nq * d), dtype=kv_layer.dtype, device=qkv.device)
+    elif q_out.dtype != kv_layer.dtype or q_out.numel() != n * nq * d:
+        raise KernelError("axes_rope_write: q_out is [tokens, nq * d] in the cache's dtype")
+    _call("lily_axes_rope_write", _p(qkv), _dt(qkv), splits, stride, ld, _p(q_gain), _p(k_gain), _dt(q_gain) if q_gain is not None else _F32,
+          float(eps), _p(cos), _p(sin), cos.shape[0], _i32(positions, "positions"), _i32(pair_axis, "pair_axis"), positions.shape[0], n,
+          _i32(places, "places"), _i32(token_req, "token_req"), _i32(block_table, "block_table"), block_table.shape[1], _p(kv_layer),
+          kv_layer.shape[0], _p(q_out), _dt(kv_layer), nq, nkv, d, rotary_dim, page_size, _stream())
+    return q_out
+
+
+def choose_weighed_splits(requests: int, kv_heads: int, max_seq_len: int, sm_count: int = 148) -> int:
+    """Ranges that the keys of a decode row are cut into for ``attention_decode_weighed``: about three blocks a SM, none under 128 keys."""
+    return max(1, min(-(-max_seq_len // 128), -(-3 * sm_count // max(1, requests * kv_heads)), 64))
+
+
+def decode_weighed_scratch_floats(requests: int, nq: int, nkv: int, d: int, max_seq_len: int) -> int:
+    """Float32 scratch that ``attention_decode_weighed`` needs for rows of up to ``max_seq_len`` places."""
+    splits = choose_weighed_splits(requests, nkv, max_seq_len, sm_count())
+    return int(library().lily_attention_decode_weighed_floats(requests, nq, d, splits, -(-max_seq_len // 4) * 4))
+
+
+def attention_decode_weighed(q: torch.Tensor, kv_layer: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                             max_seq_len: int, nq: int, nkv: int, d: int, page_size: int, scale: float,
+                             out: Optional[torch.Tensor] = None, scratch: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token a request (rows of ``q`` [requests, nq * d]) over its ``seq_lens`` cached places, none more than
+    ``max_seq_len``, that also adds up the weight every place was given: ``weights`` float32 [pages, nkv, page_size] lies beside the
+    layer's pages, a place's entry grows by the softmax weights that the query heads of its kv head gave it, and the newest place's (this
+    step's own, ``seq_lens - 1``) is set to them.  A request without places has a row of zeros.  A page belongs to one request.
+    ``scratch``: float32, ``decode_weighed_scratch_floats`` of them (allocated where not given)."""
+    _dev(q, kv_layer, weights, block_table, seq_lens, out, scratch)
+    requests = q.shape[0] if q.dim() else 0
+    if q.dtype != kv_layer.dtype or q.numel() != requests * nq * d:
+        raise KernelError(f"attention_decode_weighed: queries are [requests, {nq * d}] in the cache's dtype, got {q.dtype} {tuple(q.shape)}")
+    _layer_and_weights("attention_decode_weighed", kv_layer, weights, nkv, page_size, d)
+    width = _table("attention_decode_weighed", block_table, requests)
+    if seq_lens.numel() != requests or not 0 <= max_seq_len <= width * page_size:
+        raise KernelError(f"attention_decode_weighed: {requests} lengths of up to {max_seq_len} places; the block table holds {width * page_size}")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.dtype != q.dtype or out.numel() != q.numel():
+        raise KernelError("attention_decode_weighed: out has the shape and dtype of q")
+    splits = choose_weighed_splits(requests, nkv, max_seq_len, sm_count())
+    need = int(library().lily_attention_decode_weighed_floats(requests, nq, d, splits, -(-max_seq_len // 4) * 4))
+    if scratch is None:
+        scratch = torch.empty((need,), dtype=torch.float32, device=q.device)
+    elif scratch.dtype != torch.float32 or scratch.numel() < need:
+        raise KernelError(f"attention_decode_weighed: scratch of {need} float32 needed")
+    _call("lily_attention_decode_weighed", _p(q), _p(kv_layer), _p(weights), _p(out), _i32(block_table, "block_table"), width,
+          _i32(seq_lens, "seq_lens"), _p(scratch), requests, splits, int(max_seq_len), nq, nkv, d, page_size, float(scale), _dt(q), _stream())
+    launches["count"] += 1                                       # the kernel that joins the ranges
+    return out
+
+
+def _heard(new_lens: Sequence[int], observe: Optional[int]) -> int:
+    return max((min(int(n), int(observe)) if observe else int(n) for n in new_lens), default=0)
+
+
+def key_weights_scratch_floats(new_lens: Sequence[int], nq: int, observe: Optional[int] = None) -> int:
+    """Float32 scratch that ``attention_key_weights`` needs for portions of these lengths."""
+    return int(library().lily_key_weights_floats(len(new_lens), nq, _heard(new_lens, observe)))
+
+
+def attention_key_weights(q: torch.Tensor, kv_layer: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
+                          prefix_lens: torch.Tensor, h_prefix_lens: Sequence[int], h_new_lens: Sequence[int], nq: int, nkv: int, d: int,
+                          page_size: int, scale: float, observe: Optional[int] = None, scratch: Optional[torch.Tensor] = None) -> None:
+    """Adds to ``weights`` (as in ``attention_decode_weighed``) what the tokens of prompt portions give to every cached place: the
+    column sums of the causal softmax of each request's new tokens (rows ``cu_seqlens`` of ``q`` [tokens, nq * d]) over its cached
+    prefix and themselves, whose keys are in the cache already.  ``observe``: only the last that many tokens of each portion are heard (all where not
+    given).  The portion's own places are set, also where nobody who is heard sees them.  ``h_prefix_lens``, ``h_new_lens``:
+    the lengths on the host.  ``scratch``: float32, ``key_weights_scratch_floats`` of them (allocated where not given)."""
+    _dev(q, kv_layer, weights, block_table, cu_seqlens, prefix_lens, scratch)
+    requests = len(h_new_lens)
+    if q.dtype != kv_layer.dtype or q.dim() != 2 or q.shape[1] != nq * d or q.shape[0] < sum(h_new_lens):
+        raise KernelError(f"attention_key_weights: queries are [tokens, {nq * d}] in the cache's dtype, got {q.dtype} {tuple(q.shape)}")
+    _layer_and_weights("attention_key_weights", kv_layer, weights, nkv, page_size, d)
+    width = _table("attention_key_weights", block_table, requests)
+    if len(h_prefix_lens) != requests or cu_seqlens.numel() != requests + 1 or prefix_lens.numel() != requests:
+        raise KernelError(f"attention_key_weights: {requests} portions have a prefix each and {requests + 1} offsets")
+    if observe is not None and observe < 1:
+        raise KernelError(f"attention_key_weights: the last {observe} tokens cannot be heard")
+    longest = max((int(p) + int(n) for p, n in zip(h_prefix_lens, h_new_lens)), default=0)
+    if longest > width * page_size or any(n < 0 or p < 0 for p, n in zip(h_prefix_lens, h_new_lens)):
+        raise KernelError(f"attention_key_weights: {longest} places; the block table holds {width * page_size}")
+    heard = _heard(h_new_lens, observe)
+    if heard == 0:
+        return
+    need = int(library().lily_key_weights_floats(requests, nq, heard))
+    if scratch is None:
+        scratch = torch.empty((need,), dtype=torch.float32, device=q.device)
+    elif scratch.dtype != torch.float32 or scratch.numel() < need:
+        raise KernelError(f"attention_key_weights: scratch of {need} float32 needed")
+    _call("lily_key_weights", _p(q), _p(kv_layer), _p(weights), _i32(block_table, "block_table"), width, _i32(cu_seqlens, "cu_seqlens"),
+          _i32(prefix_lens, "prefix_lens"), _p(scratch), requests, int(observe or 0), heard, longest, nq, nkv, d, page_size, float(scale), _dt(q), _stream())
+    launches["count"] += 1                                       # the columns behind the rows
+
+
+def select_keys(weights: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, max_length: int, keep: int, first: int = 0,
+                recent: int = 0) -> torch.Tensor:
+    """The places each (layer, request, kv head) keeps, int32 [layers, requests, kv_heads, keep], ascending, -1 behind the last.  Of a
+    request of ``lengths`` places with more than ``keep``: the first ``first``, the last ``recent`` and the heaviest of the rest, ties to the
+    lower place; of a shorter one all.  ``weights`` float32 [layers, pages, kv_heads, page_size], or of one layer without the first axis; a
+    NaN counts as the heaviest.  ``max_length``: no request has more places."""
+    _dev(weights, block_table, lengths)
+    if weights.dim() == 3:
+        return select_keys(weights[None], block_table, lengths, max_length, keep, first, recent)
+    if weights.dtype != torch.float32 or weights.dim() != 4:
+        raise KernelError(f"select_keys: weights are float32 [layers, pages, kv_heads, page_size], got {weights.dtype} {tuple(weights.shape)}")
+    layers, pages, nkv, page_size = weights.shape
+    requests = lengths.numel()
+    width = _table("select_keys", block_table, requests)
+    if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
+        raise KernelError(f"select_keys: the first {first} and the last {recent} places do not fit into {keep}")
+    if not 0 <= max_length <= width * page_size:
+        raise KernelError(f"select_keys: {max_length} places; the block table holds {width * page_size}")
+    kept = torch.empty((layers, requests, nkv, keep), dtype=torch.int32, device=weights.device)
+    _call("lily_select_keys", _p(weights), _i32(block_table, "block_table"), width, _i32(lengths, "lengths"), _p(kept), layers, pages, requests, nkv,
+          page_size, int(keep), int(first), int(recent), _stream())
+    return kept
+
+
+def move_keys(kv: torch.Tensor, weights: Optional[torch.Tensor], block_table: torch.Tensor, kept: torch.Tensor,
+              to_table: Optional[torch.Tensor] = None) -> None:
+    """Moves keys, values and weights of the ``kept`` places (``select_keys``: ascending) to the front: place i of (layer, request, kv
+    head) becomes what was at ``kept[..., i]``.  ``kv`` [layers, pages, 2, kv_heads, page_size, d] and ``weights`` [layers, pages, kv_heads, page_size]
+    (or None), or those of one layer without the first axis.  In place, or, with ``to_table`` int32 [requests, pages], into those pages (a fork of the request; none of them
+    may be a page of ``block_table``).  Places outside their tables, and what lies behind the last kept place, stay as they are."""
+    _dev(kv, weights, block_table, kept, to_table)
+    if kv.dim() == 5:
+        return move_keys(kv[None], None if weights is None else weights[None], block_table, kept, to_table)
+    if kv.dim() != 6 or kv.shape[2] != 2 or kept.dim() != 4 or kept.dtype != torch.int32:
+        raise KernelError(f"move_keys: a cache [layers, pages, 2, kv_heads, page_size, d] and int32 places [layers, requests, kv_heads, keep], got {tuple(kv.shape)}, "
+                          f"{kept.dtype} {tuple(kept.shape)}")
+    layers, pages, _, nkv, page_size, d = kv.shape
+    requests, keep = kept.shape[1], kept.shape[3]
+    if kept.shape[0] != layers or kept.shape[2] != nkv:
+        raise KernelError(f"move_keys: places of {kept.shape[0]} layers and {kept.shape[2]} kv heads for a cache of {layers} and {nkv}")
+    if weights is not None and (weights.dtype != torch.float32 or tuple(weights.shape) != (layers, pages, nkv, page_size)):
+        raise KernelError(f"move_keys: weights are float32 [{layers}, {pages}, {nkv}, {page_size}], got {weights.dtype} {tuple(weights.shape)}")
+    _dt(kv)
+    width = _table("move_keys", block_table, requests)
+    to = block_table if to_table is None else to_table
+    _call("lily_move_keys", _p(kv), _p(weights), _i32(block_table, "block_table"), width, _i32(to, "to_table"), _table("move_keys", to, requests, "to_table"),
+          _p(kept), layers, pages, requests, nkv, page_size, d * kv.element_size(), keep, _stream())
 
 
 # ------------------------------------------------------------------------------ joining sublayers
