@@ -1076,6 +1076,10 @@ static int* lost_word() {
     return word;
 }
 
+namespace lily {
+int* decode_lost_word() { return lost_word(); }          // for the other decode kernels whose tiles come by TMA
+}
+
 static int decode_mma(AttnArgs& a, const void* q, const void* kv, void* out, const int* block_table, int bt_stride,
                       const int* seq_lens, float* scratch, int requests, int splits, int nq, int nkv, int d, int page_size,
                       int window, float scale, int stages, cudaStream_t stream) {

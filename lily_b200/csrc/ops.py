@@ -11,6 +11,7 @@ matrix mode can slip in.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from dataclasses import dataclass
 from typing import Callable, Optional, Sequence, Tuple
@@ -99,7 +100,7 @@ _SIGNATURES = {
     "lily_moe_relu2": [_vp, _i, _i, _vp, _vp, _vp, _i, _vp, _vp],
     "lily_axes_rope_write": [_vp, _i, _i, _sz, _i, _vp, _vp, _i, _f, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _vp,
                              _i, _i, _i, _i, _i, _i, _vp],
-    "lily_attention_decode_weighed": [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
+    "lily_attention_decode_weighed": [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp],
     "lily_key_weights": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
     "lily_select_keys": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
     "lily_move_keys": [_vp, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp],
@@ -140,7 +141,7 @@ def library():
         lib.lily_top_logprobs_cap.restype = _i
         lib.lily_attention_decode_scratch_floats.argtypes = [_i, _i, _i, _i]
         lib.lily_attention_decode_scratch_floats.restype = _sz
-        lib.lily_attention_decode_weighed_floats.argtypes = [_i, _i, _i, _i, _i]
+        lib.lily_attention_decode_weighed_floats.argtypes = [_i, _i, _i, _i, _i, _i, _i]
         lib.lily_attention_decode_weighed_floats.restype = _sz
         lib.lily_key_weights_floats.argtypes = [_i, _i, _i]
         lib.lily_key_weights_floats.restype = _sz
@@ -1260,15 +1261,10 @@ def axes_rope_write(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_gain: O
     return q_out
 
 
-def choose_weighed_splits(requests: int, kv_heads: int, max_seq_len: int, sm_count: int = 148) -> int:
-    """Ranges that the keys of a decode row are cut into for ``attention_decode_weighed``: about three blocks a SM, none under 128 keys."""
-    return max(1, min(-(-max_seq_len // 128), -(-3 * sm_count // max(1, requests * kv_heads)), 64))
-
-
-def decode_weighed_scratch_floats(requests: int, nq: int, nkv: int, d: int, max_seq_len: int) -> int:
+@functools.lru_cache(maxsize=1024)
+def decode_weighed_scratch_floats(requests: int, nq: int, nkv: int, d: int, max_seq_len: int, page_size: int, dtype: torch.dtype) -> int:
     """Float32 scratch that ``attention_decode_weighed`` needs for rows of up to ``max_seq_len`` places."""
-    splits = choose_weighed_splits(requests, nkv, max_seq_len, sm_count())
-    return int(library().lily_attention_decode_weighed_floats(requests, nq, d, splits, -(-max_seq_len // 4) * 4))
+    return int(library().lily_attention_decode_weighed_floats(requests, nq, nkv, d, max_seq_len, page_size, _BF16 if dtype == torch.bfloat16 else _F32))
 
 
 def attention_decode_weighed(q: torch.Tensor, kv_layer: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -1291,15 +1287,14 @@ def attention_decode_weighed(q: torch.Tensor, kv_layer: torch.Tensor, weights: t
         out = torch.empty_like(q)
     elif out.dtype != q.dtype or out.numel() != q.numel():
         raise KernelError("attention_decode_weighed: out has the shape and dtype of q")
-    splits = choose_weighed_splits(requests, nkv, max_seq_len, sm_count())
-    need = int(library().lily_attention_decode_weighed_floats(requests, nq, d, splits, -(-max_seq_len // 4) * 4))
+    need = decode_weighed_scratch_floats(requests, nq, nkv, d, max_seq_len, page_size, q.dtype)
     if scratch is None:
         scratch = torch.empty((need,), dtype=torch.float32, device=q.device)
     elif scratch.dtype != torch.float32 or scratch.numel() < need:
         raise KernelError(f"attention_decode_weighed: scratch of {need} float32 needed")
     _call("lily_attention_decode_weighed", _p(q), _p(kv_layer), _p(weights), _p(out), _i32(block_table, "block_table"), width,
-          _i32(seq_lens, "seq_lens"), _p(scratch), requests, splits, int(max_seq_len), nq, nkv, d, page_size, float(scale), _dt(q), _stream())
-    launches["count"] += 1                                       # the kernel that joins the ranges
+          _i32(seq_lens, "seq_lens"), _p(scratch), requests, int(max_seq_len), nq, nkv, d, page_size, kv_layer.shape[0], float(scale), _dt(q), DECODE_POLLS,
+          _stream())
     return out
 
 

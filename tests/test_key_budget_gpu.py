@@ -108,7 +108,7 @@ def test_decode_weighed_of_many_or_long_rows(dtype, nq, nkv, d, page, rows, long
     kv, w, table = pool(lengths, nkv, page, d, dtype, 11)
     q = torch.randn(rows, nq * d, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).to(dtype)
     want, want_w = decode_want(q, kv, w, table, lengths, nq, nkv, d, page, d ** -0.5)
-    scratch = torch.full((ops().decode_weighed_scratch_floats(rows, nq, nkv, d, longest + 13),), math.nan, device=DEV)
+    scratch = torch.full((ops().decode_weighed_scratch_floats(rows, nq, nkv, d, longest + 13, page, dtype),), math.nan, device=DEV)
     out = torch.full_like(q, math.nan)
     seq = torch.tensor(lengths, dtype=torch.int32, device=DEV)
     ops().attention_decode_weighed(q, kv, w, table, seq, min(longest + 13, table.shape[1] * page), nq, nkv, d, page, d ** -0.5, out=out, scratch=scratch)
