@@ -102,6 +102,7 @@ _SIGNATURES = {
                              _i, _i, _i, _i, _i, _i, _vp],
     "lily_attention_decode_weighed": [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp],
     "lily_key_weights": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
+    "lily_key_weights_tc": [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp],
     "lily_select_keys": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
     "lily_move_keys": [_vp, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp],
     "lily_argmax": [_vp, _vp, _vp, _vp, _i, _i, _vp],
@@ -145,6 +146,11 @@ def library():
         lib.lily_attention_decode_weighed_floats.restype = _sz
         lib.lily_key_weights_floats.argtypes = [_i, _i, _i]
         lib.lily_key_weights_floats.restype = _sz
+        lib.lily_key_weights_tc_floats.argtypes = [_i, _vp, _vp, _i, _i, _i]
+        lib.lily_key_weights_tc_floats.restype = _sz
+        lib.lily_key_weights_tc_takes.argtypes = [_i, _i, _i, _i, _f]
+        lib.lily_key_weights_tc_takes.restype = _i
+        lib.lily_key_weights_status.restype = _i
         lib.lily_normed_mean_max.restype = _i
         lib.lily_row_cluster_threads.argtypes = [_i]
         lib.lily_row_cluster_threads.restype = _i
@@ -1302,9 +1308,27 @@ def _heard(new_lens: Sequence[int], observe: Optional[int]) -> int:
     return max((min(int(n), int(observe)) if observe else int(n) for n in new_lens), default=0)
 
 
-def key_weights_scratch_floats(new_lens: Sequence[int], nq: int, observe: Optional[int] = None) -> int:
+@functools.lru_cache(maxsize=64)
+def _portions(h_prefix_lens: Tuple[int, ...], h_new_lens: Tuple[int, ...], nq: int, nkv: int, d: int, page_size: int, scale: float, dtype: torch.dtype,
+              observe: int):
+    """Of portions of these lengths: (whether the tcgen05 kernels take them, float32 scratch, the lengths as C arrays)."""
+    lib, n = library(), len(h_new_lens)
+    prefix, new = (ctypes.c_int * n)(*h_prefix_lens), (ctypes.c_int * n)(*h_new_lens)
+    if dtype == torch.bfloat16 and lib.lily_key_weights_tc_takes(nq, nkv, d, page_size, scale):
+        return True, int(lib.lily_key_weights_tc_floats(n, prefix, new, observe, nq, nkv)), prefix, new
+    return False, int(lib.lily_key_weights_floats(n, nq, _heard(h_new_lens, observe))), prefix, new
+
+
+def key_weights_scratch_floats(h_prefix_lens: Sequence[int], h_new_lens: Sequence[int], nq: int, nkv: int, d: int, page_size: int, scale: float,
+                               dtype: torch.dtype, observe: Optional[int] = None) -> int:
     """Float32 scratch that ``attention_key_weights`` needs for portions of these lengths."""
-    return int(library().lily_key_weights_floats(len(new_lens), nq, _heard(new_lens, observe)))
+    return _portions(tuple(h_prefix_lens), tuple(h_new_lens), nq, nkv, d, page_size, float(scale), dtype, int(observe or 0))[1]
+
+
+def key_weights_status() -> int:
+    """0, or a code of the first bounded wait that gave up in the tcgen05 kernels of ``attention_key_weights`` (its weights are NaN;
+    synchronises, and clears the code)."""
+    return int(library().lily_key_weights_status())
 
 
 def attention_key_weights(q: torch.Tensor, kv_layer: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -1331,13 +1355,19 @@ def attention_key_weights(q: torch.Tensor, kv_layer: torch.Tensor, weights: torc
     heard = _heard(h_new_lens, observe)
     if heard == 0:
         return
-    need = int(library().lily_key_weights_floats(requests, nq, heard))
+    tensor_cores, need, prefix, new = _portions(tuple(h_prefix_lens), tuple(h_new_lens), nq, nkv, d, page_size, float(scale), q.dtype, int(observe or 0))
     if scratch is None:
         scratch = torch.empty((need,), dtype=torch.float32, device=q.device)
     elif scratch.dtype != torch.float32 or scratch.numel() < need:
         raise KernelError(f"attention_key_weights: scratch of {need} float32 needed")
-    _call("lily_key_weights", _p(q), _p(kv_layer), _p(weights), _i32(block_table, "block_table"), width, _i32(cu_seqlens, "cu_seqlens"),
-          _i32(prefix_lens, "prefix_lens"), _p(scratch), requests, int(observe or 0), heard, longest, nq, nkv, d, page_size, float(scale), _dt(q), _stream())
+    _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens")
+    if tensor_cores:
+        _call("lily_key_weights_tc", _p(q), q.shape[0], _p(kv_layer), kv_layer.shape[0], _p(weights), _i32(block_table, "block_table"), width, _p(scratch),
+              requests, prefix, new, int(observe or 0), nq, nkv, d, page_size, float(scale), _stream())
+        launches["count"] += 2                                   # rows, their joining, columns
+        return
+    _call("lily_key_weights", _p(q), _p(kv_layer), _p(weights), _i32(block_table, "block_table"), width, _p(cu_seqlens),
+          _p(prefix_lens), _p(scratch), requests, int(observe or 0), heard, longest, nq, nkv, d, page_size, float(scale), _dt(q), _stream())
     launches["count"] += 1                                       # the columns behind the rows
 
 

@@ -193,12 +193,13 @@ def test_key_weights_of_long_portions(dtype, cached, new, observe):
     want = portion_want(q, kv, w, table, cached, new, nq, nkv, d, page, d ** -0.5, observe)
     cu = torch.tensor([0, *torch.tensor(new).cumsum(0).tolist()], dtype=torch.int32, device=DEV)
     pre = torch.tensor(cached, dtype=torch.int32, device=DEV)
-    scratch = torch.full((ops().key_weights_scratch_floats(new, nq, observe),), math.nan, device=DEV)
+    scratch = torch.full((ops().key_weights_scratch_floats(cached, new, nq, nkv, d, page, d ** -0.5, dtype, observe),), math.nan, device=DEV)
     again = w.clone()
     ops().attention_key_weights(q, kv, w, table, cu, pre, cached, new, nq, nkv, d, page, d ** -0.5, observe=observe, scratch=scratch)
     close(w, want, F32)
     ops().attention_key_weights(q, kv, again, table, cu, pre, cached, new, nq, nkv, d, page, d ** -0.5, observe=observe)
     assert same(w, again)                                         # to the bit: no sum depends on who comes first
+    assert ops().key_weights_status() == 0
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
