@@ -12,7 +12,7 @@
 // What bounds both is the exponential: 128 x 256 of them take the SM's 16 a cycle 2,048 cycles, the products 1,440.
 //
 // One block a SM, ten warps: a loader (TMA into two stages of 64 KB), one that issues tcgen05.mma into two accumulators of 256
-// columns (all of tensor memory), and two groups of four that read them in turn.  The steps of all (request, kv head, tile) are numbered
+// columns (all of tensor memory), and four groups of four that read them.  The steps of all (request, kv head, tile) are numbered
 // through and every block takes the same number of neighbouring ones, whatever the causal mask leaves of each tile; a tile that
 // several blocks share leaves a part in scratch for each, joined in their order (rows: by the join kernel; columns: by the block that
 // comes last), so the results do not depend on who is first.
@@ -30,7 +30,9 @@ using namespace tc5;
 constexpr int MAX_R = 40;                 // requests a launch
 constexpr int AR = 128, BR = 256;         // rows of the standing and of the streamed operand
 constexpr int STAGES = 2;
-constexpr int THREADS = 320;              // loader, mma, two groups of four warps
+constexpr int GROUPS = 4;                 // groups of four warps: two pairs that take steps in turn, each group half of a step's columns
+constexpr int COLS = BR / 2;
+constexpr int THREADS = 64 + GROUPS * 128;
 constexpr uint32_t SPIN_LIMIT = 1u << 24;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -42,19 +44,22 @@ struct Portion {
     int heard, place0, prefix, total;     // heard tokens, the place of the first, cached places before and after the portion
     int unit0, step1, per1;               // its first row tile; its first step of the row kernel, steps of one kv head
     int tile0, step2, per2;               // the same of the column kernel (tiles of 128 places)
+    int row_steps;                        // pieces of two row tiles
 };
 
 struct Params {
     const int* block_table;
     float* weights;                       // [pages, nkv, page_size]
     float2* parts;                        // rows: [unit + block][group][128] (max, sum)
-    float* lse;                           // [units][128]
+    float* lse;                           // [units][128], negative
     int2* info;                           // [units] first block, blocks
     int* done;                            // [tiles] parts that have arrived
     float* sums;                          // columns: [tile + block][group][128]
     int bt_stride, requests, nkv, group, tq, page_size, pages, units, tiles;
     int steps1, quota1, steps2, quota2;   // steps in all and of a block
     float c;                              // scale * log2 e
+    float per_step;                       // 1 / (2 tq)
+    int page_shift;
     Portion p[MAX_R];
 };
 
@@ -72,14 +77,17 @@ __host__ __device__ inline int steps2_of(const Portion& p, int tq, int i) { retu
 
 constexpr int a_bytes(int d) { return AR * d * 2; }
 constexpr int b_bytes(int d) { return BR * d * 2; }
-// shared memory: two standing tiles | stages | lse of the columns (twice 256) | token of each row of a tile | barriers
+constexpr int LSE = 4;                    // steps whose lse are held
+constexpr int SUMS = 8;                   // tiles whose groups' sums are
+// shared memory: two standing tiles | stages | lse of the columns | the groups' sums | token of each row of a tile | barriers
 constexpr int off_b(int d) { return 2 * a_bytes(d); }
 constexpr int off_lse(int d) { return off_b(d) + STAGES * b_bytes(d); }
-constexpr int off_tok(int d) { return off_lse(d) + 2 * BR * 4; }
+constexpr int off_sums(int d) { return off_lse(d) + LSE * BR * 4; }
+constexpr int off_tok(int d) { return off_sums(d) + SUMS * GROUPS * AR * 4; }
 constexpr int off_bars(int d) { return off_tok(d) + AR * 4; }
-constexpr int NUM_BARS = 4 + 2 * STAGES + 6;
+constexpr int NUM_BARS = 4 + 2 * STAGES + 4 + 2 * LSE + SUMS;
 constexpr int off_misc(int d) { return off_bars(d) + 8 * NUM_BARS; }
-constexpr int smem_bytes(int d) { return off_misc(d) + 64; }
+constexpr int smem_bytes(int d) { return off_misc(d) + 128; }
 
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
     for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
@@ -94,18 +102,88 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code));
 }
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void group_sync(int group) { asm volatile("bar.sync %0, 128;\n" ::"r"(group + 1) : "memory"); }
 
-// Where a role stands: tile `i` of (request r, kv head), step `s` of its `n`.
-struct Cursor { int r, kvh, i, s, n, unit; };
+// ---- pairs of floats in one register pair (fma.rn.f32x2: two IEEE operations an instruction) ----
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float a, float b) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void apart(Two v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 
-template <int PASS>
-__device__ __forceinline__ int steps_of(const Params& p, int r, int i) { return PASS == 1 ? steps1_of(p.p[r], p.tq, i) : steps2_of(p.p[r], p.tq, i); }
+__device__ __forceinline__ Two exp2_of(Two x) {
+    float a, b;
+    apart(x, a, b);
+    return two(ex2(a), ex2(b));
+}
+
+// Waits for the loads from tensor memory; what they bring is not used ahead of this.
+__device__ __forceinline__ void wait_loaded(float (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+                 : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]), "+f"(r[9]), "+f"(r[10]),
+                   "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]), "+f"(r[16]), "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]),
+                   "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]), "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]),
+                   "+f"(r[31])::"memory");
+}
+
+// Where a role stands: step `s` of the `n` of tile `i` of (request r, kv head), whose first step `f` is (columns), and the request's lengths.
+struct Cursor { int r, kvh, i, s, n, unit, f, tiles, first, heard, place0, prefix, total, unit0; };
+
+__device__ __forceinline__ void of_request(const Params& p, Cursor& c, int tiles) {
+    const Portion& q = p.p[c.r];
+    c.tiles = tiles;
+    c.first = q.first, c.heard = q.heard, c.place0 = q.place0, c.prefix = q.prefix, c.total = q.total, c.unit0 = q.unit0;
+}
 template <int PASS>
 __device__ __forceinline__ int tiles_of(const Params& p, int r) { return PASS == 1 ? row_tiles(p.p[r], p.tq) : key_tiles(p.p[r]); }
+
+// The steps of the cursor's tile (the same as steps1_of and steps2_of; the quotient by float, set right).
+template <int PASS>
+__device__ __forceinline__ void of_tile(const Params& p, Cursor& c) {
+    if (PASS == 1) {
+        const int from = c.i * p.tq, end = min(from + p.tq, c.heard);
+        c.n = from < c.heard ? (c.place0 + end + BR - 1) / BR : 0;
+    } else {
+        const int x = c.i * AR - c.place0, d = 2 * p.tq;
+        int f = 0;
+        if (x > 0) {
+            f = (int)((float)x * p.per_step);
+            const int rest = x - f * d;
+            f += rest >= d ? 1 : rest < 0 ? -1 : 0;
+        }
+        c.f = f;
+        c.n = p.p[c.r].row_steps - f;
+    }
+}
 
 // On to the next tile that has steps.
 template <int PASS>
@@ -113,14 +191,20 @@ __device__ __forceinline__ void next_tile(const Params& p, Cursor& c) {
     c.s = 0;
     do {
         ++c.i, ++c.unit;
-        if (c.i == tiles_of<PASS>(p, c.r)) {
+        if (c.i == c.tiles) {
             c.i = 0;
             if (++c.kvh == p.nkv) {
                 c.kvh = 0;
-                do ++c.r; while (c.r < p.requests && tiles_of<PASS>(p, c.r) == 0);
+                int tiles = 0;
+                do ++c.r; while (c.r < p.requests && (tiles = tiles_of<PASS>(p, c.r)) == 0);
+                if (c.r == p.requests) {
+                    c.n = 1;
+                    return;
+                }
+                of_request(p, c, tiles);
             }
         }
-        c.n = c.r < p.requests ? steps_of<PASS>(p, c.r, c.i) : 1;
+        of_tile<PASS>(p, c);
     } while (c.n == 0);
 }
 
@@ -133,11 +217,12 @@ __device__ Cursor find(const Params& p, int g) {
     const Portion& q = p.p[c.r];
     int off = g - (PASS == 1 ? q.step1 : q.step2);
     const int per = PASS == 1 ? q.per1 : q.per2, tiles = tiles_of<PASS>(p, c.r), lane = threadIdx.x & 31;
+    of_request(p, c, tiles);
     c.kvh = off / per;
     off -= c.kvh * per;
     c.i = 0;
     for (int i0 = 0; i0 < tiles; i0 += 32) {
-        const int i = i0 + lane, n = i < tiles ? steps_of<PASS>(p, c.r, i) : 0;
+        const int i = i0 + lane, n = i < tiles ? (PASS == 1 ? steps1_of(q, p.tq, i) : steps2_of(q, p.tq, i)) : 0;
         int sum = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -154,7 +239,7 @@ __device__ Cursor find(const Params& p, int g) {
         off -= __shfl_sync(0xffffffffu, sum, 31);
     }
     c.s = off;
-    c.n = steps_of<PASS>(p, c.r, c.i);
+    of_tile<PASS>(p, c);
     c.unit = (PASS == 1 ? q.unit0 : q.tile0) + c.kvh * tiles + c.i;
     return c;
 }
@@ -164,18 +249,19 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
                                                                     const __grid_constant__ Params p) {
     constexpr int DH = D / 64;
     extern __shared__ __align__(1024) unsigned char smem[];
-    float* lse_s = reinterpret_cast<float*>(smem + off_lse(D));       // [2][256]
+    float* lse_s = reinterpret_cast<float*>(smem + off_lse(D));       // [LSE][256]
+    float* sums_s = reinterpret_cast<float*>(smem + off_sums(D));     // [SUMS][GROUPS][128]
     int* tok_s = reinterpret_cast<int*>(smem + off_tok(D));           // [128] token of a tile's row
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + off_bars(D));
     uint32_t& tmem_base_s = *reinterpret_cast<uint32_t*>(smem + off_misc(D));
     int& abort_s = *reinterpret_cast<int*>(smem + off_misc(D) + 4);
-    int* last_s = reinterpret_cast<int*>(smem + off_misc(D) + 8);     // [2]
-    Cursor& start_s = *reinterpret_cast<Cursor*>(smem + off_misc(D) + 16);
+    int* last_s = reinterpret_cast<int*>(smem + off_misc(D) + 8);     // [GROUPS]
+    Cursor& start_s = *reinterpret_cast<Cursor*>(smem + off_misc(D) + 8 + 4 * GROUPS);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = smem_u32(smem);
     const uint32_t a_smem = base, b_smem = base + off_b(D);
     const uint32_t a_full = smem_u32(bars), a_empty = a_full + 16, b_full = a_empty + 16, b_empty = b_full + 8 * STAGES, s_full = b_empty + 8 * STAGES,
-                   s_empty = s_full + 16, l_full = s_empty + 16;
+                   s_empty = s_full + 16, l_full = s_empty + 16, l_empty = l_full + 8 * LSE, sums_full = l_empty + 8 * LSE;
     if (base & 1023u) {                                               // the swizzled tiles need it; never seen, but checked
         if (threadIdx.x == 0) atomicCAS(&g_status, 0, (11 << 24) | (int)(blockIdx.x & 0xFFFFFF));
         return;
@@ -186,9 +272,13 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
             mbar_init(a_full + 8 * s, 1);
             mbar_init(a_empty + 8 * s, 1);
             mbar_init(s_full + 8 * s, 1);
-            mbar_init(s_empty + 8 * s, 128);
-            mbar_init(l_full + 8 * s, 1);
+            mbar_init(s_empty + 8 * s, 8);
         }
+        for (int s = 0; s < LSE; ++s) {
+            mbar_init(l_full + 8 * s, 1);
+            mbar_init(l_empty + 8 * s, 8);
+        }
+        for (int s = 0; s < SUMS; ++s) mbar_init(sums_full + 8 * s, (GROUPS - 1) * 4);
         for (int s = 0; s < STAGES; ++s) {
             mbar_init(b_full + 8 * s, 1);
             mbar_init(b_empty + 8 * s, 1);
@@ -211,6 +301,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
         }
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     }
+    const int group_rows = p.group * p.tq;
     const int steps = PASS == 1 ? p.steps1 : p.steps2, quota = PASS == 1 ? p.quota1 : p.quota2;
     const int g0 = blockIdx.x * quota, mine = min(quota, steps - g0);
     if (warp == 1) {
@@ -227,36 +318,36 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
     const uint32_t tmem = tmem_base_s;
     volatile int* abort_flag = &abort_s;
     Cursor cur = start_s;
-    pdl_wait();
-    pdl_launch_dependents();
+    // The column kernel's loader, products and waits begin ahead of the wait for the join kernel: queries and keys were there before the row
+    // kernel began.  What reads the lse (the loader, further down) or writes waits.
+    if (PASS == 1 || warp >= 2) pdl_wait();
+    if (PASS == 1) pdl_launch_dependents();
 
     if (warp == 0) {
         // ---- loader ----
-        const int box = min(p.page_size, 64);                        // places a box of the cache
-        // the pages of `rows` places from `key` on, a box a lane and step; all lanes stay together
-        auto load_keys = [&](uint32_t dst, int rows, int pitch, int r, int kvh, int key, uint32_t bar) {
-            const int* table = p.block_table + (size_t)r * p.bt_stride;
-            const int boxes = rows / box;
-            for (int b0 = 0; b0 < boxes; b0 += 32) {
-                const int mine_key = key + (b0 + lane) * box;
-                const bool held = b0 + lane < boxes && mine_key < p.p[r].total;
-                const int page = held ? table[mine_key / p.page_size] : 0, at = held ? mine_key % p.page_size : 0;
-                for (int b = 0; b < min(32, boxes - b0); ++b) {
-                    const int pg = __shfl_sync(0xffffffffu, page, b), off = __shfl_sync(0xffffffffu, at, b);
-                    if (lane == 0)
-#pragma unroll
-                        for (int h = 0; h < DH; ++h) tma_load_4d(dst + h * pitch + (b0 + b) * box * 128, &map_kv, bar, h * 64, off, kvh, pg);
-                }
-            }
+        // Of a tile of keys lane b has box b (a page, or 64 places of one): it looks its page up a step ahead and asks for it itself.
+        const int box = min(p.page_size, 64), mask = p.page_size - 1;
+        int page = 0, page_a = 0;
+        auto look_up = [&](const Cursor& at, int key, int rows) {
+            const int mine_key = key + lane * box;
+            return lane * box < rows && mine_key < at.total ? p.block_table[(size_t)at.r * p.bt_stride + (mine_key >> p.page_shift)] : 0;
         };
-        auto load_rows = [&](uint32_t dst, int pitch, int r, int kvh, int tile, uint32_t bar) {
-            if (lane == 0)
+        auto load_keys = [&](uint32_t dst, int rows, int pitch, int kvh, int key, int pg, uint32_t bar) {
+            if (lane * box < rows)
 #pragma unroll
-                for (int h = 0; h < DH; ++h) tma_load_3d(dst + h * pitch, &map_q, bar, h * 64, kvh * p.group, p.p[r].first + tile * p.tq);
+                for (int h = 0; h < DH; ++h) tma_load_4d(dst + h * pitch + lane * box * 128, &map_kv, bar, h * 64, (key + lane * box) & mask, kvh, pg);
         };
-        const int q_bytes = p.group * p.tq * D * 2;
+        auto load_rows = [&](uint32_t dst, int pitch, int kvh, int token, uint32_t bar) {
+            if (lane < DH) tma_load_3d(dst + lane * pitch, &map_q, bar, lane * 64, kvh * p.group, token);
+        };
+        const int q_bytes = group_rows * D * 2;
         bool ok = true;
         int tile = 0, sent_a = 0, sent_b = 0, sent_l = 0;
+        auto look_ahead = [&](bool fresh) {
+            if (PASS == 1) page = look_up(cur, cur.s * BR, BR);
+            else if (fresh) page_a = look_up(cur, cur.i * AR, AR);
+        };
+        look_ahead(true);
         for (int k = 0; k < mine && ok; ++k) {
             if (k == 0 || cur.s == 0) {                               // a new standing tile
                 ok = warp_wait(a_empty + 8 * (tile & 1), ((tile >> 1) & 1) ^ 1, abort_flag, 1);
@@ -264,8 +355,8 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
                 const uint32_t bar = a_full + 8 * (tile & 1), dst = a_smem + (tile & 1) * a_bytes(D);
                 if (lane == 0) mbar_expect_tx(bar, PASS == 1 ? q_bytes : a_bytes(D));
                 __syncwarp();
-                if (PASS == 1) load_rows(dst, AR * 128, cur.r, cur.kvh, cur.i, bar);
-                else load_keys(dst, AR, AR * 128, cur.r, cur.kvh, cur.i * AR, bar);
+                if (PASS == 1) load_rows(dst, AR * 128, cur.kvh, cur.first + cur.i * p.tq, bar);
+                else load_keys(dst, AR, AR * 128, cur.kvh, cur.i * AR, page_a, bar);
                 ++tile;
                 ++sent_a;
             }
@@ -276,23 +367,26 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
             if (lane == 0) mbar_expect_tx(bar, PASS == 1 ? b_bytes(D) : 2 * q_bytes);
             __syncwarp();
             if (PASS == 1) {
-                load_keys(dst, BR, BR * 128, cur.r, cur.kvh, cur.s * BR, bar);
+                load_keys(dst, BR, BR * 128, cur.kvh, cur.s * BR, page, bar);
                 ++sent_b;
             } else {
-                const int t0 = 2 * (first2_of(p.p[cur.r], p.tq, cur.i) + cur.s);
-                load_rows(dst, BR * 128, cur.r, cur.kvh, t0, bar);
-                load_rows(dst + AR * 128, BR * 128, cur.r, cur.kvh, t0 + 1, bar);
+                const int t0 = 2 * (cur.f + cur.s);
+                load_rows(dst, BR * 128, cur.kvh, cur.first + t0 * p.tq, bar);
+                load_rows(dst + AR * 128, BR * 128, cur.kvh, cur.first + (t0 + 1) * p.tq, bar);
                 ++sent_b;
-                ok = warp_wait(s_empty + 8 * (k & 1), ((k >> 1) & 1) ^ 1, abort_flag, 3);        // the lse of step k - 2 have been read
+                if (k == 0) pdl_wait();
+                const int ls = k % LSE;
+                ok = warp_wait(l_empty + 8 * ls, ((k / LSE) & 1) ^ 1, abort_flag, 3);       // the lse of step k - LSE have been read
                 if (!ok) break;
                 if (lane == 0) {
-                    mbar_expect_tx(l_full + 8 * (k & 1), BR * 4);
-                    const int unit = p.p[cur.r].unit0 + cur.kvh * row_tiles(p.p[cur.r], p.tq) + t0;
-                    bulk_load(smem_u32(lse_s + (k & 1) * BR), p.lse + (size_t)unit * AR, BR * 4, l_full + 8 * (k & 1));
+                    mbar_expect_tx(l_full + 8 * ls, BR * 4);
+                    bulk_load(smem_u32(lse_s + ls * BR), p.lse + (size_t)(cur.unit0 + cur.kvh * 2 * p.p[cur.r].row_steps + t0) * AR, BR * 4, l_full + 8 * ls);
                 }
                 ++sent_l;
             }
-            if (++cur.s == cur.n) next_tile<PASS>(p, cur);
+            const bool fresh = ++cur.s == cur.n;
+            if (fresh) next_tile<PASS>(p, cur);
+            if (k + 1 < mine) look_ahead(fresh);
         }
         if (*abort_flag && lane == 0) {
             // copies already issued still land in this block's shared memory: give each a bounded wait
@@ -300,8 +394,8 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
                 for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(a_full + 8 * (j & 1), (j >> 1) & 1); ++i) {}
             for (int j = max(0, sent_b - STAGES); j < sent_b; ++j)
                 for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(b_full + 8 * (j % STAGES), (j / STAGES) & 1); ++i) {}
-            for (int j = max(0, sent_l - 2); j < sent_l; ++j)
-                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(l_full + 8 * (j & 1), (j >> 1) & 1); ++i) {}
+            for (int j = max(0, sent_l - LSE); j < sent_l; ++j)
+                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(l_full + 8 * (j % LSE), (j / LSE) & 1); ++i) {}
         }
     } else if (warp == 1) {
         // ---- products: accumulator k & 1 = standing tile x streamed tile of step k ----
@@ -333,115 +427,160 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
             if (++cur.s == cur.n) next_tile<PASS>(p, cur);
         }
     } else {
-        // ---- two groups of 128 threads, a lane of tensor memory each: group k & 1 takes step k ----
-        // (where a wait runs out they go on without it to the ends of the tiles, where they meet, and what they leave is NaN)
-        const int which = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
-        const uint32_t my = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)which * BR;
+        // ---- groups of 128 threads, a lane of tensor memory each: pair k & 1 takes step k, each of its groups 128 columns ----
+        // The pairs drift half a period apart, so that one's exponentials run under what the other does around its own.
+        // (Where a wait runs out the threads go on without it to the ends of the tiles, where they meet, and what they leave is NaN.)
+        const int which = (warp - 2) >> 2, pair = which >> 1, quarter = warp & 3, row = quarter * 32 + lane;
+        const int col0 = (which & 1) * COLS;
+        const uint32_t my = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(pair * BR + col0);
         const int tok = tok_s[row];
         const float c = p.c;
         float m = -INFINITY, l = 0.f;                                 // rows: running maximum (log2 units) and sum; columns: l is the sum
         bool ok = true;
-        int unit_first = g0;                                          // the step at which this block's share of the tile begins
+        int tile = 0;
+        float* at = nullptr;
+        float old = 0.f;
         for (int k = 0; k < mine; ++k) {
-            const Portion& q = p.p[cur.r];
-            if ((k & 1) == which && ok) {
-                ok = warp_wait(s_full + 8 * which, (k >> 1) & 1, abort_flag, 7);
-                if (PASS == 2 && ok) ok = warp_wait(l_full + 8 * which, (k >> 1) & 1, abort_flag, 8);
+            const int buf = k & 1, ls = k % LSE;
+            if (PASS == 2 && which == 0 && (k == 0 || cur.s == 0)) {
+                // where this thread's place has its weight, and what it is: asked for ahead of the tile's steps
+                const int place = cur.i * AR + row;
+                at = nullptr;
+                if (place < cur.total) {
+                    at = p.weights + (((size_t)p.block_table[(size_t)cur.r * p.bt_stride + (place >> p.page_shift)] * p.nkv + cur.kvh) << p.page_shift) +
+                         (place & (p.page_size - 1));
+                    old = place < cur.prefix ? *at : 0.f;
+                }
             }
+            if (buf == pair && ok) ok = warp_wait(s_full + 8 * buf, (k >> 1) & 1, abort_flag, 7);
+            if (PASS == 2 && buf == pair && ok) ok = warp_wait(l_full + 8 * ls, (k / LSE) & 1, abort_flag, 8);
             if (!ok) l = __int_as_float(0x7fffffff);
-            if ((k & 1) == which && ok) {
+            else if (buf == pair) {
                 tc_fence_after();
-                if (PASS == 1) {
-                    const int key0 = cur.s * BR, first = q.place0 + cur.i * p.tq, own = q.place0 + cur.i * p.tq + tok;      // the last place this row sees
-                    const bool masked = key0 + BR - 1 > first;
-#pragma unroll 1
-                    for (int c0 = 0; c0 < BR; c0 += 64) {
-                        float s[64];
-                        tmem_ld32(my + (uint32_t)c0, s);
-                        tmem_ld32(my + (uint32_t)c0 + 32, s + 32);
-                        tmem_wait_ld();
+                const int key0 = cur.s * BR + col0, own = cur.place0 + cur.i * p.tq + tok;              // rows: the last place this one sees
+                // columns: the first token of their row tile
+                const int t0 = PASS == 2 ? ((cur.f + cur.s) * 2 + col0 / AR) * p.tq : 0, key = cur.i * AR + row;
+                const bool masked = PASS == 1 ? key0 + COLS - 1 > own - tok : cur.i * AR + AR - 1 > cur.place0 + t0 || t0 + p.tq > cur.heard;
+                Two sum[4] = {two(l, 0.f), 0, 0, 0};
+#pragma unroll
+                for (int c0 = 0; c0 < COLS; c0 += 32) {
+                    float s[32];
+                    tmem_ld32(my + (uint32_t)c0, s);
+                    wait_loaded(s);
+                    if (c0 + 32 == COLS) {                            // the last has come: the accumulator goes back to the products
+                        tc_fence_before();
+                        warp_arrive(s_empty + 8 * buf);
+                    }
+                    if (PASS == 1) {
                         if (masked) {
 #pragma unroll
-                            for (int e = 0; e < 64; ++e) s[e] = key0 + c0 + e <= own ? s[e] : -INFINITY;
+                            for (int e = 0; e < 32; ++e) s[e] = key0 + c0 + e <= own ? s[e] : -INFINITY;
                         }
                         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                        for (int e = 4; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
-                        const float now = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c), off = now == -INFINITY ? 0.f : now;
-                        float sum[4] = {l * ex2(m - off), 0.f, 0.f, 0.f};
-                        m = now;
+                        for (int e = 4; e < 28; e += 8)
 #pragma unroll
-                        for (int e = 0; e < 64; ++e) sum[e & 3] += ex2(fmaf(s[e], c, -off));
-                        l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    }
-                } else {
-                    const int step = first2_of(q, p.tq, cur.i) + cur.s, t0 = step * 2 * p.tq, key = cur.i * AR + row;
-                    const bool masked = cur.i * AR + AR - 1 > q.place0 + t0 || t0 + 2 * p.tq > q.heard;
-                    const float4* lse4 = reinterpret_cast<const float4*>(lse_s + which * BR);
-                    float sum[4] = {l, 0.f, 0.f, 0.f};
-#pragma unroll 1
-                    for (int c0 = 0; c0 < BR; c0 += 64) {
-                        float s[64];
-                        tmem_ld32(my + (uint32_t)c0, s);
-                        tmem_ld32(my + (uint32_t)c0 + 32, s + 32);
-                        tmem_wait_ld();
+                            for (int j = 0; j < 4; ++j) mx[j] = max3(mx[j], s[e + 2 * j], s[e + 2 * j + 1]);
+                        mx[0] = max3(mx[0], s[28], s[29]);
+                        mx[1] = max3(mx[1], s[30], s[31]);
+                        const float now = fmaxf(m, fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * c);
+                        if (__any_sync(0xffffffffu, now > m)) {
+                            const float f = now > m ? ex2(m - now) : 1.f;             // (0 where m is -inf)
 #pragma unroll
-                        for (int e = 0; e < 64; e += 4) {
-                            const float4 z = lse4[(c0 + e) >> 2];
-                            s[e] = ex2(fmaf(s[e], c, -z.x));
-                            s[e + 1] = ex2(fmaf(s[e + 1], c, -z.y));
-                            s[e + 2] = ex2(fmaf(s[e + 2], c, -z.z));
-                            s[e + 3] = ex2(fmaf(s[e + 3], c, -z.w));
+                            for (int j = 0; j < 4; ++j) sum[j] = mul2(sum[j], two(f, f));
+                            m = now;
+                        }
+                        const float off = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const Two x = fma2(two(s[2 * e], s[2 * e + 1]), two(c, c), two(off, off));
+                            sum[e & 3] = add2(sum[e & 3], exp2_of(x));
+                        }
+                    } else {
+                        const ulonglong2* minus_lse = reinterpret_cast<const ulonglong2*>(lse_s + ls * BR + col0 + c0);
+                        Two v[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e += 2) {
+                            const ulonglong2 z = minus_lse[e >> 1];
+                            const Two x = fma2(two(s[2 * e], s[2 * e + 1]), two(c, c), z.x), y = fma2(two(s[2 * e + 2], s[2 * e + 3]), two(c, c), z.y);
+                            v[e] = exp2_of(x);
+                            v[e + 1] = exp2_of(y);
                         }
                         if (masked) {
-                            const int t = t0 + (c0 >= AR ? p.tq : 0);
+                            // the columns' tokens that are heard and see this place: [from, heard), in tokens of the row tile
+                            const int from = max(key - cur.place0 - t0, 0);
+                            const uint32_t some = max(cur.heard - t0 - from, 0);
+                            const int4* tok4 = reinterpret_cast<const int4*>(tok_s + c0);
 #pragma unroll
-                            for (int e = 0; e < 64; ++e) {
-                                const int tc = t + tok_s[(c0 & (AR - 1)) + e];
-                                s[e] = tc < q.heard && key <= q.place0 + tc ? s[e] : 0.f;
+                            for (int e = 0; e < 16; e += 2) {
+                                const int4 t = tok4[e >> 1];
+                                float a, b;
+                                apart(v[e], a, b);
+                                v[e] = two((uint32_t)(t.x - from) < some ? a : 0.f, (uint32_t)(t.y - from) < some ? b : 0.f);
+                                apart(v[e + 1], a, b);
+                                v[e + 1] = two((uint32_t)(t.z - from) < some ? a : 0.f, (uint32_t)(t.w - from) < some ? b : 0.f);
                             }
                         }
 #pragma unroll
-                        for (int e = 0; e < 64; ++e) sum[e & 3] += s[e];
+                        for (int e = 0; e < 16; ++e) sum[e & 3] = add2(sum[e & 3], v[e]);
                     }
-                    l = (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 }
-                tc_fence_before();
-                mbar_arrive(s_empty + 8 * which);
+                float a, b;
+                apart(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, b);
+                l = a + b;
+                if (PASS == 2) warp_arrive(l_empty + 8 * ls);
             }
             if (cur.s + 1 == cur.n || k + 1 == mine) {
-                // the end of this block's share of the tile
-                const int at = g0 + k - cur.s, blocks_first = at / quota, blocks = (at + cur.n - 1) / quota - blocks_first + 1;
-                const size_t slot = ((size_t)(cur.unit + (int)blockIdx.x) * 2 + which) * AR + row;
+                // the end of this block's share of the tile, whose first step is `begin`
+                const int begin = g0 + k - cur.s, end = begin + cur.n;
+                const bool alone = begin >= g0 && end <= g0 + quota;
+                const size_t slot = ((size_t)(cur.unit + (int)blockIdx.x) * GROUPS + which) * AR + row;
                 if (PASS == 1) {
                     p.parts[slot] = make_float2(m, l);
-                    if (unit_first == at && which == 0 && row == 0) p.info[cur.unit] = make_int2(blocks_first, blocks);
+                    if (begin >= g0 && which == 0 && row == 0) p.info[cur.unit] = make_int2(blockIdx.x, alone ? 1 : (end - 1) / quota - (int)blockIdx.x + 1);
+                } else if (alone) {
+                    // The groups' sums through shared memory, joined by the first group; the others go on.  (SUMS tiles of room: a group is at most five
+                    // tiles ahead of the first, whose accumulators the products behind wait for.)
+                    float* sums = sums_s + (size_t)(tile % SUMS) * GROUPS * AR;
+                    sums[which * AR + row] = l;
+                    if (which) warp_arrive(sums_full + 8 * (tile % SUMS));
+                    else {
+                        ok = warp_wait(sums_full + 8 * (tile % SUMS), (tile / SUMS) & 1, abort_flag, 9) && ok;
+                        float w = old;
+#pragma unroll
+                        for (int j = 0; j < GROUPS; ++j) w += sums[j * AR + row];
+                        if (at) *at = ok ? w : __int_as_float(0x7fffffff);
+                    }
+                    ++tile;
                 } else {
+                    // several blocks: the one that comes last joins what all have left in scratch
+                    const int blocks_first = begin / quota, parts = GROUPS * ((end - 1) / quota - blocks_first + 1);
                     __stcg(p.sums + slot, l);
                     __threadfence();
                     group_sync(which);
-                    if (row == 0) last_s[which] = atomicAdd(p.done + cur.unit, 1) == 2 * blocks - 1;
+                    if (row == 0) last_s[which] = atomicAdd(p.done + cur.unit, 1) == parts - 1;
                     group_sync(which);
                     if (last_s[which]) {
                         __threadfence();
                         float w = 0.f;
-                        for (int b = 0; b < 2 * blocks; ++b) w += __ldcg(p.sums + ((size_t)(cur.unit + blocks_first) * 2 + b) * AR + row);
+                        for (int b = 0; b < parts; ++b) w += __ldcg(p.sums + ((size_t)(cur.unit + blocks_first) * GROUPS + b) * AR + row);
                         const int place = cur.i * AR + row;
-                        if (place < q.total) {
-                            float* to = p.weights + ((size_t)p.block_table[(size_t)cur.r * p.bt_stride + place / p.page_size] * p.nkv + cur.kvh) * p.page_size +
-                                        place % p.page_size;
-                            *to = (place < q.prefix ? *to : 0.f) + w;
+                        if (place < cur.total) {
+                            float* to = p.weights + (((size_t)p.block_table[(size_t)cur.r * p.bt_stride + (place >> p.page_shift)] * p.nkv + cur.kvh) << p.page_shift) +
+                                        (place & (p.page_size - 1));
+                            *to = (place < cur.prefix ? *to : 0.f) + w;
                         }
                     }
                     group_sync(which);                                // (the word is read before the next tile's)
                 }
                 m = -INFINITY;
                 l = 0.f;
-                unit_first = g0 + k + 1;
             }
             if (++cur.s == cur.n) next_tile<PASS>(p, cur);
         }
     }
+    if (PASS == 2 && warp < 2) pdl_wait();                            // (a block ends behind the kernels ahead)
+    if (PASS == 2) pdl_launch_dependents();
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
@@ -460,17 +599,17 @@ __global__ void __launch_bounds__(AR) key_weights_join_kernel(const __grid_const
     while (r + 1 < p.requests && p.p[r + 1].unit0 <= unit) ++r;
     const Portion& q = p.p[r];
     const int i = (unit - q.unit0) % row_tiles(q, p.tq);
-    float lse = INFINITY;
+    float lse = -INFINITY;                                            // negative
     if (row < p.group * p.tq && i * p.tq + row / p.group < q.heard) {
         const int2 in = p.info[unit];
-        const float2* part = p.parts + (size_t)(unit + in.x) * 2 * AR + row;
+        const float2* part = p.parts + (size_t)(unit + in.x) * GROUPS * AR + row;
         float m = -INFINITY, l = 0.f;
-        for (int b = 0; b < 2 * in.y; ++b) m = fmaxf(m, part[b * AR].x);
-        for (int b = 0; b < 2 * in.y; ++b) {
+        for (int b = 0; b < GROUPS * in.y; ++b) m = fmaxf(m, part[b * AR].x);
+        for (int b = 0; b < GROUPS * in.y; ++b) {
             const float2 v = part[b * AR];
             if (v.x > -INFINITY || v.y != 0.f) l = fmaf(v.y, exp2f(v.x - m), l);      // (a NaN is no maximum, but makes the sum one)
         }
-        lse = m + log2f(l);
+        lse = -(m + log2f(l));
     }
     p.lse[(size_t)unit * AR + row] = lse;
 }
@@ -514,6 +653,7 @@ static size_t plan(Params& p, int requests, const int* prefix, const int* fresh,
         q.step2 = (int)s2;
         q.per1 = q.per2 = 0;
         const int rows = row_tiles(q, p.tq), keys = key_tiles(q);
+        q.row_steps = rows / 2;
         for (int i = 0; i < rows; ++i) q.per1 += steps1_of(q, p.tq, i);
         for (int i = 0; i < keys; ++i) q.per2 += steps2_of(q, p.tq, i);
         s1 += (long long)q.per1 * nkv;
@@ -532,7 +672,7 @@ static size_t plan(Params& p, int requests, const int* prefix, const int* fresh,
     p.quota2 = s2 > 0 ? (int)((s2 + sms - 1) / sms) : 1;
     const int b1 = (p.steps1 + p.quota1 - 1) / p.quota1, b2 = (p.steps2 + p.quota2 - 1) / p.quota2;
     // parts | lse | info | counters | sums, each on 16 bytes
-    return (size_t)(unit + b1) * 4 * AR + (size_t)unit * AR + (size_t)unit * 2 + ((size_t)tile + 3) / 4 * 4 + (size_t)(tile + b2) * 2 * AR + 16;
+    return (size_t)(unit + b1) * 2 * GROUPS * AR + (size_t)unit * AR + (size_t)unit * 2 + ((size_t)tile + 3) / 4 * 4 + (size_t)(tile + b2) * GROUPS * AR + 16;
 }
 
 }  // namespace keyw5
@@ -604,10 +744,12 @@ LILY_API int lily_key_weights_tc(const void* q, int tokens, const void* kv, int 
             p.page_size = page_size;
             p.pages = pages;
             p.c = scale * keyw5::LOG2E;
+            p.per_step = 1.f / (float)(2 * tq);
+            for (p.page_shift = 0; 1 << p.page_shift < page_size;) ++p.page_shift;
             const int b1 = (p.steps1 + p.quota1 - 1) / p.quota1;
             float* at = scratch;
             p.parts = reinterpret_cast<float2*>(at);
-            at += (size_t)(p.units + b1) * 4 * keyw5::AR;
+            at += (size_t)(p.units + b1) * 2 * keyw5::GROUPS * keyw5::AR;
             p.lse = at;
             at += (size_t)p.units * keyw5::AR;
             p.info = reinterpret_cast<int2*>(at);
