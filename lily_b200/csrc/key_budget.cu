@@ -21,69 +21,88 @@ struct SelectArgs {
     const int* block_table;          // [requests, bt_stride]
     const int* lengths;              // [requests]
     int* kept;                       // [layers, requests, nkv, keep]
-    int bt_stride, requests, nkv, page_size, pages, keep, first, recent;
+    int bt_stride, requests, nkv, page_size, page_shift, pages, max_length, keep, first, recent;
 };
 
-constexpr int SELECT_THREADS = 512;
+constexpr int SELECT_MOST = 1024;          // threads of a block at most
+constexpr int SELECT_HELD = 48 * 1024;     // places whose ranks a block holds in shared memory; of longer rows they are worked out again a pass
 
-// Sums two counts over the block in thread order: `before` what lies ahead of this thread; `total` of the block.
-__device__ __forceinline__ void scan2(int a, int b, int& before_a, int& before_b, int& total_a, int& total_b, int2* warp_s) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    int ia = a, ib = b;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int ua = __shfl_up_sync(0xffffffffu, ia, o), ub = __shfl_up_sync(0xffffffffu, ib, o);
-        if (lane >= o) ia += ua, ib += ub;
-    }
-    __syncthreads();
-    if (lane == 31) warp_s[warp] = make_int2(ia, ib);
-    __syncthreads();
-    before_a = ia - a, before_b = ib - b, total_a = 0, total_b = 0;
-    for (int w = 0; w < warps; ++w) {
-        const int2 v = warp_s[w];
-        if (w < warp) before_a += v.x, before_b += v.y;
-        total_a += v.x, total_b += v.y;
-    }
-}
-
-// One block a (layer, request, kv head): the rank that the last kept weight has, eight bits a pass over the row, then the kept places in order.
-__global__ void __launch_bounds__(SELECT_THREADS) select_keys_kernel(const SelectArgs a) {
-    __shared__ int hist[256];
-    __shared__ int2 warp_s[SELECT_THREADS / 32];
+// One block a (layer, request, kv head).  The weights are read once, as ranks; the rank that the last kept weight has comes out eight bits a
+// pass (a histogram of the competing ranks that share the bits found so far; lanes with the same eight bits count as one, since
+// weights are alike in their exponents and would queue for a counter); then every warp counts what it keeps of its stretch of the row, and
+// writes it behind what the warps ahead keep.  What bounds it is the chain of passes, 5 us for 4,096 places, not the bytes.
+__global__ void __launch_bounds__(SELECT_MOST) select_keys_kernel(const SelectArgs a) {
+    extern __shared__ uint32_t rank_s[];                             // [min(max_length, SELECT_HELD)]
+    __shared__ __align__(16) int hist[256];
+    __shared__ int2 warp_s[32];
     __shared__ uint32_t prefix_s;
     __shared__ int need_s;
     pdl_enter_small();
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
     const int kvh = blockIdx.x % a.nkv, req = blockIdx.x / a.nkv % a.requests, layer = blockIdx.x / a.nkv / a.requests;
-    const int n = min(max(a.lengths[req], 0), a.bt_stride * a.page_size);
+    const int n = min(max(a.lengths[req], 0), a.max_length);
     int* out = a.kept + (size_t)blockIdx.x * a.keep;
     if (n <= a.keep) {
-        for (int i = tid; i < a.keep; i += SELECT_THREADS) out[i] = i < n ? i : -1;
+        for (int i = tid; i < a.keep; i += threads) out[i] = i < n ? i : -1;
         return;
     }
     const int* table = a.block_table + (size_t)req * a.bt_stride;
-    const float* base = a.weights + (size_t)layer * a.pages * a.nkv * a.page_size;
-    auto weight = [&](int j) {
-        const int page = table[j / a.page_size];
-        return page >= 0 && page < a.pages ? rank_of(base[((size_t)page * a.nkv + kvh) * a.page_size + j % a.page_size]) : 0u;
+    const float* base = a.weights + ((size_t)layer * a.pages * a.nkv + kvh) * a.page_size;
+    const size_t page_stride = (size_t)a.nkv * a.page_size;
+    auto look = [&](int j) {
+        const int page = table[j >> a.page_shift];
+        return page >= 0 && page < a.pages ? rank_of(base[page * page_stride + (j & (a.page_size - 1))]) : 0u;
     };
-    const int lo = a.first, hi = n - a.recent;                   // the places that compete; more than `need` of them
-    int need = a.keep - a.first - a.recent;
+    const int wanted = a.keep - a.first - a.recent, lo = a.first, hi = n - a.recent;      // more than `wanted` places compete, [lo, hi)
+    const bool held = n <= SELECT_HELD;
+    if (held && wanted > 0) {
+#pragma unroll 4
+        for (int j = lo + tid; j < hi; j += threads) rank_s[j] = look(j);
+    }
+    auto rank = [&](int j) { return held ? rank_s[j] : look(j); };
     uint32_t prefix = 0;
-    if (need > 0) {
+    int need = wanted;
+    if (wanted > 0) {
         for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += SELECT_THREADS) hist[i] = 0;
             __syncthreads();
-            for (int j = lo + tid; j < hi; j += SELECT_THREADS) {
-                const uint32_t r = weight(j);
-                if (shift == 24 || r >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&hist[r >> shift & 255], 1);
+            for (int i = tid; i < 256; i += threads) hist[i] = 0;
+            __syncthreads();
+            for (int j0 = lo + warp * 32; j0 < hi; j0 += threads) {
+                const int j = j0 + lane;
+                const uint32_t r = j < hi ? rank(j) : 0u;
+                const bool in = j < hi && (shift == 24 || r >> ((shift + 8) & 31) == prefix >> ((shift + 8) & 31));
+                if (!__any_sync(0xffffffffu, in)) continue;
+                const int digit = in ? (int)(r >> shift & 255u) : 256;
+                const uint32_t alike = __match_any_sync(0xffffffffu, digit);
+                if (in && (alike & ((1u << lane) - 1u)) == 0) atomicAdd(&hist[digit], __popc(alike));
             }
             __syncthreads();
-            if (tid == 0) {
-                int b = 255, above = 0;
-                while (above + hist[b] < need) above += hist[b--];
-                prefix_s = prefix | (uint32_t)b << shift;
-                need_s = need - above;
+            if (warp == 0) {
+                // eight bins a lane, the highest with the first: the bin in which the count from above reaches what is needed
+                const int top = 248 - 8 * lane;
+                const int4 u = *reinterpret_cast<const int4*>(hist + top + 4), v = *reinterpret_cast<const int4*>(hist + top);
+                const int c[8] = {u.w, u.z, u.y, u.x, v.w, v.z, v.y, v.x};
+                int sum = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum += c[i];
+                int upto = sum;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int t = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += t;
+                }
+                int above = upto - sum;
+                if (above < need && need <= upto) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (above < need && need <= above + c[i]) {
+                            prefix_s = prefix | (uint32_t)(top + 7 - i) << shift;
+                            need_s = need - above;
+                            break;
+                        }
+                        above += c[i];
+                    }
+                }
             }
             __syncthreads();
             prefix = prefix_s;
@@ -91,27 +110,42 @@ __global__ void __launch_bounds__(SELECT_THREADS) select_keys_kernel(const Selec
         }
     }
     // now `prefix` is the rank of the last kept weight and `need` how many of that rank are kept, the lowest places first
-    int done_kept = 0, done_ties = 0;
-    const int wanted = a.keep - a.first - a.recent;
-    for (int j0 = 0; j0 < n; j0 += SELECT_THREADS) {
-        const int j = j0 + tid;
-        int sure = 0, tie = 0;
-        if (j < n) {
-            if (j < lo || j >= hi) sure = 1;
+    const int per = (n + threads - 1) / threads * 32, beg = warp * per, end = min(n, beg + per);
+    auto kinds = [&](int j0, uint32_t& sure, uint32_t& tie) {
+        const int j = j0 + lane;
+        bool s = false, t = false;
+        if (j < end) {
+            if (j < lo || j >= hi) s = true;
             else if (wanted > 0) {
-                const uint32_t r = weight(j);
-                sure = r > prefix;
-                tie = r == prefix;
+                const uint32_t r = rank(j);
+                s = r > prefix;
+                t = r == prefix;
             }
         }
-        int bs, bt, ts, tt;
-        scan2(sure, tie, bs, bt, ts, tt, warp_s);
-        const int ties_before = done_ties + bt;
-        const bool mine = sure || (tie && ties_before < need);
-        const int at = done_kept + bs + min(ties_before, need);
-        if (mine && at < a.keep) out[at] = j;
-        done_kept += ts;
-        done_ties += tt;
+        sure = __ballot_sync(0xffffffffu, s);
+        tie = __ballot_sync(0xffffffffu, t);
+    };
+    int sures = 0, ties = 0;
+    for (int j0 = beg; j0 < end; j0 += 32) {
+        uint32_t s, t;
+        kinds(j0, s, t);
+        sures += __popc(s);
+        ties += __popc(t);
+    }
+    if (lane == 0) warp_s[warp] = make_int2(sures, ties);
+    __syncthreads();
+    int2 before = lane < warps && lane < warp ? warp_s[lane] : make_int2(0, 0);
+    int at_sure = __reduce_add_sync(0xffffffffu, before.x), at_tie = __reduce_add_sync(0xffffffffu, before.y);
+    const uint32_t ahead = (1u << lane) - 1u;
+    for (int j0 = beg; j0 < end; j0 += 32) {
+        uint32_t s, t;
+        kinds(j0, s, t);
+        const int tb = at_tie + __popc(t & ahead);
+        const bool mine = (s >> lane & 1u) || ((t >> lane & 1u) && tb < need);
+        const int at = at_sure + __popc(s & ahead) + min(tb, need);
+        if (mine && at < a.keep) out[at] = j0 + lane;
+        at_sure += __popc(s);
+        at_tie += __popc(t);
     }
 }
 
@@ -121,45 +155,89 @@ struct MoveArgs {
     const int* block_table;
     const int* to_table;
     const int* kept;                 // [layers, requests, nkv, keep], ascending, -1 behind the last
-    int bt_stride, to_stride, requests, nkv, page_size, pages, keep, row_bytes;
+    int bt_stride, to_stride, requests, nkv, page_size, page_shift, pages, keep, row_bytes;
 };
 
-constexpr int MOVE_THREADS = 256;
+constexpr int MOVE_THREADS = 256, MOVE_AHEAD = 4;        // pieces a thread has on their way
+constexpr int MOVE_CLUSTER = 8;
 
-// One block a (layer, request, kv head, keys | values | weights) goes through the kept places in order.  In place the target i is at most
-// its source and the sources ascend, so nothing that a later tile reads lies where an earlier one writes, and a tile reads all it moves before it writes.
-template <typename V>
+// A block moves MOVE_THREADS * MOVE_AHEAD pieces of the rows of one (layer, request, kv head) and of its keys, values or weights (grid y).
+// Into other pages every block works for itself.  In place (IN_PLACE) the eight blocks of a cluster go through the list together, a
+// round of eight blocks' pieces at a time: all read before any writes, for which the cluster's barrier is enough, since the target i is at
+// most its source and the sources ascend, so nothing that a later round reads lies where an earlier one writes.  What bounds it are the
+// bytes; a piece is a chain of three reads (place, page, row), so many are kept on their way: 1,024 of 4,096 rows of 256 bytes, eight heads, eight
+// layers (67 MB) take 19 us into other pages.
+template <typename V, bool IN_PLACE>
 __global__ void __launch_bounds__(MOVE_THREADS) move_keys_kernel(const MoveArgs a) {
-    pdl_enter_small();
-    const int kvh = blockIdx.x % a.nkv, req = blockIdx.x / a.nkv % a.requests, layer = blockIdx.x / a.nkv / a.requests, part = blockIdx.y;
-    const int* kept = a.kept + (size_t)blockIdx.x * a.keep;
+    // (no launch_dependents: the kernel behind may read keys ahead of its wait)
+    pdl_wait();
+    const int part = blockIdx.z, list = blockIdx.y;
+    const int kvh = list % a.nkv, req = list / a.nkv % a.requests, layer = list / a.nkv / a.requests;
+    const int* kept = a.kept + (size_t)list * a.keep;
     const int* from = a.block_table + (size_t)req * a.bt_stride;
     const int* to = a.to_table + (size_t)req * a.to_stride;
     const int per = part == 2 ? 1 : a.row_bytes / (int)sizeof(V);          // pieces of a row
     const size_t heads = part == 2 ? a.nkv : 2 * a.nkv, head = part == 2 ? kvh : part * a.nkv + kvh;
     auto offset = [&](const int* table, int width, int place) -> long long {
-        if (place < 0 || place / a.page_size >= width) return -1;
-        const int page = table[place / a.page_size];
+        const int at = place >> a.page_shift;
+        if (place < 0 || at >= width) return -1;
+        const int page = table[at];
         if (page < 0 || page >= a.pages) return -1;
-        return (long long)((((size_t)layer * a.pages + page) * heads + head) * a.page_size + place % a.page_size);
+        return (long long)(((((size_t)layer * a.pages + page) * heads + head) << a.page_shift) + (place & (a.page_size - 1)));
     };
-    const int pieces = a.keep * per;
-    for (int p0 = 0; p0 < pieces; p0 += MOVE_THREADS) {
-        const int p = p0 + threadIdx.x, i = p / per, c = p % per;
-        const int place = p < pieces ? kept[i] : -1;
-        const long long src = offset(from, a.bt_stride, place), dst = src >= 0 ? offset(to, a.to_stride, i) : -1;
-        V v;
-        float w;
-        if (dst >= 0) {
-            if (part == 2) w = a.weights[src];
-            else v = reinterpret_cast<const V*>(a.kv)[(size_t)src * per + c];
+    const int pieces = a.keep * per, step = MOVE_THREADS * MOVE_AHEAD, rounds = IN_PLACE ? (pieces + gridDim.x * step - 1) / (gridDim.x * step) : 1;
+    for (int round = 0; round < rounds; ++round) {
+        const int p0 = (round * gridDim.x + blockIdx.x) * step + threadIdx.x;
+        V v[MOVE_AHEAD];
+        float w[MOVE_AHEAD];
+        long long dst[MOVE_AHEAD];
+#pragma unroll
+        for (int u = 0; u < MOVE_AHEAD; ++u) {
+            const int p = p0 + u * MOVE_THREADS, i = p / per, c = p - i * per;
+            const int place = p < pieces ? kept[i] : -1;
+            const long long src = place == i && IN_PLACE ? -1 : offset(from, a.bt_stride, place);          // (a row that stays where it is)
+            dst[u] = src >= 0 ? offset(to, a.to_stride, i) : -1;
+            if (dst[u] >= 0) {
+                dst[u] = dst[u] * per + c;
+                if (part == 2) w[u] = a.weights[src];
+                else v[u] = reinterpret_cast<const V*>(a.kv)[src * per + c];
+            }
         }
-        __syncthreads();
-        if (dst >= 0) {
-            if (part == 2) a.weights[dst] = w;
-            else reinterpret_cast<V*>(a.kv)[(size_t)dst * per + c] = v;
-        }
+        if (IN_PLACE) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+#pragma unroll
+        for (int u = 0; u < MOVE_AHEAD; ++u)
+            if (dst[u] >= 0) {
+                if (part == 2) a.weights[dst[u]] = w[u];
+                else reinterpret_cast<V*>(a.kv)[dst[u]] = v[u];
+            }
     }
+}
+
+template <typename V>
+static void launch_move(const MoveArgs& a, long long rows, bool in_place, cudaStream_t stream) {
+    const int step = MOVE_THREADS * MOVE_AHEAD;
+    const long long pieces = (long long)a.keep * a.row_bytes / (long long)sizeof(V);
+    const unsigned blocks = (unsigned)((pieces + step - 1) / step);
+    const unsigned parts = a.weights ? 3 : 2;
+    if (!in_place) {
+        launch_pdl(move_keys_kernel<V, false>, dim3(blocks, (unsigned)rows, parts), dim3(MOVE_THREADS), 0, stream, a);
+        return;
+    }
+    const unsigned cluster = blocks < (unsigned)MOVE_CLUSTER ? blocks : MOVE_CLUSTER;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cluster, (unsigned)rows, parts);
+    cfg.blockDim = dim3(MOVE_THREADS);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, move_keys_kernel<V, true>, a);
 }
 
 }  // namespace budget
@@ -168,29 +246,52 @@ __global__ void __launch_bounds__(MOVE_THREADS) move_keys_kernel(const MoveArgs 
 using namespace lily;
 
 LILY_API int lily_select_keys(const float* weights, const int* block_table, int bt_stride, const int* lengths, int* kept, int layers, int pages,
-                              int requests, int nkv, int page_size, int keep, int first, int recent, cudaStream_t stream) {
+                              int requests, int nkv, int page_size, int max_length, int keep, int first, int recent, cudaStream_t stream) {
     const long long rows = (long long)layers * requests * nkv;
     if (rows == 0 || keep == 0) return 0;
     LILY_REQUIRE(keep > 0 && first >= 0 && recent >= 0 && (long long)first + recent <= keep, "select_keys: the first %d and the last %d do not fit %d places",
                  first, recent, keep);
-    LILY_REQUIRE(page_size > 0 && bt_stride > 0 && rows <= 0x7fffffff && (long long)bt_stride * page_size <= 0x7fffffff, "select_keys: %lld rows, tables of %d pages", rows, bt_stride);
-    const budget::SelectArgs a{weights, block_table, lengths, kept, bt_stride, requests, nkv, page_size, pages, keep, first, recent};
-    launch_pdl(budget::select_keys_kernel, dim3((unsigned)rows), dim3(budget::SELECT_THREADS), 0, stream, a);
+    LILY_REQUIRE(page_size > 0 && (page_size & (page_size - 1)) == 0, "select_keys: page_size %d is not a power of two", page_size);
+    LILY_REQUIRE(bt_stride > 0 && max_length >= 0 && max_length <= (long long)bt_stride * page_size && rows <= 0x7fffffff, "select_keys: %lld rows of up to %d places, tables of %d pages",
+                 rows, max_length, bt_stride);
+    budget::SelectArgs a{weights, block_table, lengths, kept, bt_stride, requests, nkv, page_size, 0, pages, max_length, keep, first, recent};
+    while (1 << a.page_shift < page_size) ++a.page_shift;
+    static bool configured = false;
+    if (!configured) {
+        const cudaError_t e = cudaFuncSetAttribute(budget::select_keys_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, budget::SELECT_HELD * 4);
+        LILY_REQUIRE(e == cudaSuccess, "select_keys: cannot get %d bytes of shared memory: %s", budget::SELECT_HELD * 4, cudaGetErrorString(e));
+        configured = true;
+    }
+    int threads = 128;                                       // four places a thread
+    while (threads < budget::SELECT_MOST && threads * 4 < max_length) threads *= 2;
+    const size_t smem = (size_t)(max_length < budget::SELECT_HELD ? max_length : budget::SELECT_HELD) * 4;
+    launch_pdl(budget::select_keys_kernel, dim3((unsigned)rows), dim3(threads), smem, stream, a);
     LILY_CHECK_LAUNCH("select_keys");
     return 0;
 }
 
 LILY_API int lily_move_keys(void* kv, float* weights, const int* block_table, int bt_stride, const int* to_table, int to_stride, const int* kept,
-                            int layers, int pages, int requests, int nkv, int page_size, int row_bytes, int keep, cudaStream_t stream) {
+                            int layers, int pages, int requests, int nkv, int page_size, int row_bytes, int keep, int in_place, cudaStream_t stream) {
     const long long rows = (long long)layers * requests * nkv;
     if (rows == 0 || keep == 0) return 0;
-    LILY_REQUIRE(page_size > 0 && bt_stride > 0 && to_stride > 0 && rows <= 0x7fffffff && row_bytes > 0 && row_bytes % 2 == 0, "move_keys: %lld rows of %d bytes", rows, row_bytes);
-    const budget::MoveArgs a{(unsigned char*)kv, weights, block_table, to_table, kept, bt_stride, to_stride, requests, nkv, page_size, pages, keep, row_bytes};
-    const dim3 grid((unsigned)rows, weights ? 3 : 2);
-    LILY_REQUIRE((long long)keep * row_bytes <= 0x7fffffff, "move_keys: %d places of %d bytes", keep, row_bytes);
-    if (row_bytes % 16 == 0 && (uintptr_t)kv % 16 == 0) launch_pdl(budget::move_keys_kernel<uint4>, grid, dim3(budget::MOVE_THREADS), 0, stream, a);
-    else if (row_bytes % 4 == 0 && (uintptr_t)kv % 4 == 0) launch_pdl(budget::move_keys_kernel<uint32_t>, grid, dim3(budget::MOVE_THREADS), 0, stream, a);
-    else launch_pdl(budget::move_keys_kernel<uint16_t>, grid, dim3(budget::MOVE_THREADS), 0, stream, a);
+    LILY_REQUIRE(page_size > 0 && (page_size & (page_size - 1)) == 0, "move_keys: page_size %d is not a power of two", page_size);
+    LILY_REQUIRE(bt_stride > 0 && to_stride > 0 && row_bytes > 0 && row_bytes % 2 == 0 && (long long)keep * row_bytes <= 0x7fff0000, "move_keys: %d places of %d bytes", keep, row_bytes);
+    const int vec = row_bytes % 16 == 0 && (uintptr_t)kv % 16 == 0 ? 16 : row_bytes % 4 == 0 && (uintptr_t)kv % 4 == 0 ? 4 : 2;
+    for (long long at = 0; at < rows;) {
+        // (a grid has 65,535 lists at most: whole layers of them)
+        const long long layer_rows = (long long)requests * nkv, some = layer_rows > 65535 ? 0 : 65535 / layer_rows < layers ? 65535 / layer_rows : layers;
+        LILY_REQUIRE(some > 0, "move_keys: %d requests of %d kv heads", requests, nkv);
+        const long long first_layer = at / layer_rows, now = first_layer + some <= layers ? some : layers - first_layer;
+        budget::MoveArgs a{(unsigned char*)kv + (size_t)first_layer * pages * 2 * nkv * page_size * row_bytes,
+                           weights ? weights + (size_t)first_layer * pages * nkv * page_size : nullptr, block_table, to_table,
+                           kept + (size_t)at * keep, bt_stride, to_stride, requests, nkv, page_size, 0, pages, keep, row_bytes};
+        while (1 << a.page_shift < page_size) ++a.page_shift;
+        const long long lists = now * layer_rows;
+        if (vec == 16) budget::launch_move<uint4>(a, lists, in_place, stream);
+        else if (vec == 4) budget::launch_move<uint32_t>(a, lists, in_place, stream);
+        else budget::launch_move<uint16_t>(a, lists, in_place, stream);
+        at += lists;
+    }
     LILY_CHECK_LAUNCH("move_keys");
     return 0;
 }

@@ -103,8 +103,8 @@ _SIGNATURES = {
     "lily_attention_decode_weighed": [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp],
     "lily_key_weights": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
     "lily_key_weights_tc": [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp],
-    "lily_select_keys": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
-    "lily_move_keys": [_vp, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp],
+    "lily_select_keys": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
+    "lily_move_keys": [_vp, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
     "lily_argmax": [_vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_apply_penalties": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_top_logprobs": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
@@ -1391,7 +1391,7 @@ def select_keys(weights: torch.Tensor, block_table: torch.Tensor, lengths: torch
         raise KernelError(f"select_keys: {max_length} places; the block table holds {width * page_size}")
     kept = torch.empty((layers, requests, nkv, keep), dtype=torch.int32, device=weights.device)
     _call("lily_select_keys", _p(weights), _i32(block_table, "block_table"), width, _i32(lengths, "lengths"), _p(kept), layers, pages, requests, nkv,
-          page_size, int(keep), int(first), int(recent), _stream())
+          page_size, int(max_length), int(keep), int(first), int(recent), _stream())
     return kept
 
 
@@ -1417,7 +1417,8 @@ def move_keys(kv: torch.Tensor, weights: Optional[torch.Tensor], block_table: to
     width = _table("move_keys", block_table, requests)
     to = block_table if to_table is None else to_table
     _call("lily_move_keys", _p(kv), _p(weights), _i32(block_table, "block_table"), width, _i32(to, "to_table"), _table("move_keys", to, requests, "to_table"),
-          _p(kept), layers, pages, requests, nkv, page_size, d * kv.element_size(), keep, _stream())
+          _p(kept), layers, pages, requests, nkv, page_size, d * kv.element_size(), keep,
+          int(to_table is None or to_table.data_ptr() == block_table.data_ptr()), _stream())
 
 
 # ------------------------------------------------------------------------------ joining sublayers
