@@ -33,7 +33,7 @@ constexpr int SELECT_HELD = 48 * 1024;     // places whose ranks a block holds i
 // writes it behind what the warps ahead keep.  What bounds it is the chain of passes, 5 us for 4,096 places, not the bytes.
 __global__ void __launch_bounds__(SELECT_MOST) select_keys_kernel(const SelectArgs a) {
     extern __shared__ uint32_t rank_s[];                             // [min(max_length, SELECT_HELD)]
-    __shared__ __align__(16) int hist[256];
+    __shared__ __align__(16) int hists[4][256];
     __shared__ int2 warp_s[32];
     __shared__ uint32_t prefix_s;
     __shared__ int need_s;
@@ -55,6 +55,7 @@ __global__ void __launch_bounds__(SELECT_MOST) select_keys_kernel(const SelectAr
     };
     const int wanted = a.keep - a.first - a.recent, lo = a.first, hi = n - a.recent;      // more than `wanted` places compete, [lo, hi)
     const bool held = n <= SELECT_HELD;
+    for (int i = tid; i < 1024; i += threads) hists[0][i] = 0;
     if (held && wanted > 0) {
 #pragma unroll 4
         for (int j = lo + tid; j < hi; j += threads) rank_s[j] = look(j);
@@ -64,9 +65,8 @@ __global__ void __launch_bounds__(SELECT_MOST) select_keys_kernel(const SelectAr
     int need = wanted;
     if (wanted > 0) {
         for (int shift = 24; shift >= 0; shift -= 8) {
-            __syncthreads();
-            for (int i = tid; i < 256; i += threads) hist[i] = 0;
-            __syncthreads();
+            int* hist = hists[shift >> 3];
+            if (shift == 24) __syncthreads();
             for (int j0 = lo + warp * 32; j0 < hi; j0 += threads) {
                 const int j = j0 + lane;
                 const uint32_t r = j < hi ? rank(j) : 0u;
@@ -96,8 +96,10 @@ __global__ void __launch_bounds__(SELECT_MOST) select_keys_kernel(const SelectAr
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         if (above < need && need <= above + c[i]) {
-                            prefix_s = prefix | (uint32_t)(top + 7 - i) << shift;
-                            need_s = need - above;
+                            // all of a bin: whatever its ranks are beyond these bits, they are above the bin below it
+                            const bool whole = need == above + c[i];
+                            prefix_s = (prefix | (uint32_t)(top + 7 - i) << shift) - (whole ? 1u : 0u);
+                            need_s = whole ? 0 : need - above;
                             break;
                         }
                         above += c[i];
@@ -107,9 +109,10 @@ __global__ void __launch_bounds__(SELECT_MOST) select_keys_kernel(const SelectAr
             __syncthreads();
             prefix = prefix_s;
             need = need_s;
+            if (need == 0) break;
         }
     }
-    // now `prefix` is the rank of the last kept weight and `need` how many of that rank are kept, the lowest places first
+    // now `prefix` is the rank of the last kept weight and `need` how many of that rank are kept, the lowest places first (none: what is above it is kept)
     const int per = (n + threads - 1) / threads * 32, beg = warp * per, end = min(n, beg + per);
     auto kinds = [&](int j0, uint32_t& sure, uint32_t& tie) {
         const int j = j0 + lane;
@@ -156,76 +159,88 @@ struct MoveArgs {
     const int* to_table;
     const int* kept;                 // [layers, requests, nkv, keep], ascending, -1 behind the last
     int bt_stride, to_stride, requests, nkv, page_size, page_shift, pages, keep, row_bytes;
+    int block_rows;                  // rows a block moves at a time
 };
 
-constexpr int MOVE_THREADS = 256, MOVE_AHEAD = 4;        // pieces a thread has on their way
-constexpr int MOVE_CLUSTER = 8;
+constexpr int MOVE_THREADS = 256, MOVE_AHEAD = 8;        // pieces a thread has on their way
+constexpr int MOVE_CLUSTER = 8, MOVE_ROWS = 128;         // rows a block moves at most
 
-// A block moves MOVE_THREADS * MOVE_AHEAD pieces of the rows of one (layer, request, kv head) and of its keys, values or weights (grid y).
-// Into other pages every block works for itself.  In place (IN_PLACE) the eight blocks of a cluster go through the list together, a
-// round of eight blocks' pieces at a time: all read before any writes, for which the cluster's barrier is enough, since the target i is at
-// most its source and the sources ascend, so nothing that a later round reads lies where an earlier one writes.  What bounds it are the
-// bytes; a piece is a chain of three reads (place, page, row), so many are kept on their way: 1,024 of 4,096 rows of 256 bytes, eight heads, eight
-// layers (67 MB) take 19 us into other pages.
+// A block moves the keys, values and weights of some rows of one (layer, request, kv head): the rows' places and pages are looked up once, by a
+// thread a row, then every thread has eight pieces on their way.  Into other pages every block works for itself.  In place (IN_PLACE) the
+// eight blocks of a cluster go through the list together, a round of eight blocks' rows at a time: all read before any writes, for which the cluster's barrier
+// is enough, since the target i is at most its source and the sources ascend, so nothing that a later round reads lies where an earlier
+// one writes.  What bounds it are the bytes.
 template <typename V, bool IN_PLACE>
 __global__ void __launch_bounds__(MOVE_THREADS) move_keys_kernel(const MoveArgs a) {
+    __shared__ long long src_s[MOVE_ROWS], dst_s[MOVE_ROWS];         // rows of the cache; -1: not moved
     // (no launch_dependents: the kernel behind may read keys ahead of its wait)
     pdl_wait();
-    const int part = blockIdx.z, list = blockIdx.y;
+    const int tid = threadIdx.x, list = blockIdx.y;
     const int kvh = list % a.nkv, req = list / a.nkv % a.requests, layer = list / a.nkv / a.requests;
     const int* kept = a.kept + (size_t)list * a.keep;
     const int* from = a.block_table + (size_t)req * a.bt_stride;
     const int* to = a.to_table + (size_t)req * a.to_stride;
-    const int per = part == 2 ? 1 : a.row_bytes / (int)sizeof(V);          // pieces of a row
-    const size_t heads = part == 2 ? a.nkv : 2 * a.nkv, head = part == 2 ? kvh : part * a.nkv + kvh;
-    auto offset = [&](const int* table, int width, int place) -> long long {
-        const int at = place >> a.page_shift;
-        if (place < 0 || at >= width) return -1;
-        const int page = table[at];
-        if (page < 0 || page >= a.pages) return -1;
-        return (long long)(((((size_t)layer * a.pages + page) * heads + head) << a.page_shift) + (place & (a.page_size - 1)));
-    };
-    const int pieces = a.keep * per, step = MOVE_THREADS * MOVE_AHEAD, rounds = IN_PLACE ? (pieces + gridDim.x * step - 1) / (gridDim.x * step) : 1;
+    const int per = a.row_bytes / (int)sizeof(V), both = 2 * per;          // pieces of a key, of key and value
+    const long long to_value = (long long)a.nkv * a.page_size;             // rows from a key to its value
+    const int rounds = IN_PLACE ? (a.keep + gridDim.x * a.block_rows - 1) / (gridDim.x * a.block_rows) : 1;
     for (int round = 0; round < rounds; ++round) {
-        const int p0 = (round * gridDim.x + blockIdx.x) * step + threadIdx.x;
+        const int row0 = (round * gridDim.x + blockIdx.x) * a.block_rows;
+        float w = 0.f;
+        long long w_to = -1;
+        if (tid < a.block_rows) {
+            const int i = row0 + tid, place = i < a.keep ? kept[i] : -1, at = place >> a.page_shift, to_at = i >> a.page_shift;
+            long long src = -1, dst = -1;
+            // (a row that stays where it is need not move)
+            if (place >= 0 && at < a.bt_stride && to_at < a.to_stride && !(IN_PLACE && place == i)) {
+                const int page = from[at], to_page = to[to_at];
+                if (page >= 0 && page < a.pages && to_page >= 0 && to_page < a.pages) {
+                    const size_t r = (size_t)layer * a.pages + page, t = (size_t)layer * a.pages + to_page;
+                    const int off = place & (a.page_size - 1), to_off = i & (a.page_size - 1);
+                    src = (long long)(((r * 2 * a.nkv + kvh) << a.page_shift) + off);
+                    dst = (long long)(((t * 2 * a.nkv + kvh) << a.page_shift) + to_off);
+                    if (a.weights) {
+                        w = a.weights[((r * a.nkv + kvh) << a.page_shift) + off];
+                        w_to = (long long)(((t * a.nkv + kvh) << a.page_shift) + to_off);
+                    }
+                }
+            }
+            src_s[tid] = src;
+            dst_s[tid] = dst;
+        }
+        __syncthreads();
         V v[MOVE_AHEAD];
-        float w[MOVE_AHEAD];
         long long dst[MOVE_AHEAD];
 #pragma unroll
         for (int u = 0; u < MOVE_AHEAD; ++u) {
-            const int p = p0 + u * MOVE_THREADS, i = p / per, c = p - i * per;
-            const int place = p < pieces ? kept[i] : -1;
-            const long long src = place == i && IN_PLACE ? -1 : offset(from, a.bt_stride, place);          // (a row that stays where it is)
-            dst[u] = src >= 0 ? offset(to, a.to_stride, i) : -1;
-            if (dst[u] >= 0) {
-                dst[u] = dst[u] * per + c;
-                if (part == 2) w[u] = a.weights[src];
-                else v[u] = reinterpret_cast<const V*>(a.kv)[src * per + c];
+            const int p = tid + u * MOVE_THREADS, i = p / both, in = p - i * both;
+            dst[u] = -1;
+            if (i < a.block_rows && src_s[i] >= 0) {
+                const long long more = in < per ? (long long)in : to_value * per + (in - per);
+                dst[u] = dst_s[i] * per + more;
+                v[u] = reinterpret_cast<const V*>(a.kv)[src_s[i] * per + more];
             }
         }
         if (IN_PLACE) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 #pragma unroll
         for (int u = 0; u < MOVE_AHEAD; ++u)
-            if (dst[u] >= 0) {
-                if (part == 2) a.weights[dst[u]] = w[u];
-                else reinterpret_cast<V*>(a.kv)[dst[u]] = v[u];
-            }
+            if (dst[u] >= 0) reinterpret_cast<V*>(a.kv)[dst[u]] = v[u];
+        if (w_to >= 0) a.weights[w_to] = w;
+        if (IN_PLACE) __syncthreads();                                     // the rows have been read before the next round's are put there
     }
 }
 
 template <typename V>
-static void launch_move(const MoveArgs& a, long long rows, bool in_place, cudaStream_t stream) {
-    const int step = MOVE_THREADS * MOVE_AHEAD;
-    const long long pieces = (long long)a.keep * a.row_bytes / (long long)sizeof(V);
-    const unsigned blocks = (unsigned)((pieces + step - 1) / step);
-    const unsigned parts = a.weights ? 3 : 2;
+static void launch_move(MoveArgs a, long long rows, bool in_place, cudaStream_t stream) {
+    const int most = MOVE_THREADS * MOVE_AHEAD / (2 * (a.row_bytes / (int)sizeof(V)));
+    a.block_rows = most < MOVE_ROWS ? most : MOVE_ROWS;
+    const unsigned blocks = (unsigned)((a.keep + a.block_rows - 1) / a.block_rows);
     if (!in_place) {
-        launch_pdl(move_keys_kernel<V, false>, dim3(blocks, (unsigned)rows, parts), dim3(MOVE_THREADS), 0, stream, a);
+        launch_pdl(move_keys_kernel<V, false>, dim3(blocks, (unsigned)rows), dim3(MOVE_THREADS), 0, stream, a);
         return;
     }
     const unsigned cluster = blocks < (unsigned)MOVE_CLUSTER ? blocks : MOVE_CLUSTER;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cluster, (unsigned)rows, parts);
+    cfg.gridDim = dim3(cluster, (unsigned)rows);
     cfg.blockDim = dim3(MOVE_THREADS);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -262,8 +277,9 @@ LILY_API int lily_select_keys(const float* weights, const int* block_table, int 
         LILY_REQUIRE(e == cudaSuccess, "select_keys: cannot get %d bytes of shared memory: %s", budget::SELECT_HELD * 4, cudaGetErrorString(e));
         configured = true;
     }
-    int threads = 128;                                       // four places a thread
-    while (threads < budget::SELECT_MOST && threads * 4 < max_length) threads *= 2;
+    // four places a thread, more where the rows would not all run at once (2,048 threads a SM)
+    int threads = 128;
+    while (threads < budget::SELECT_MOST && threads * 4 < max_length && rows * threads * 2 <= 2048LL * sm_count()) threads *= 2;
     const size_t smem = (size_t)(max_length < budget::SELECT_HELD ? max_length : budget::SELECT_HELD) * 4;
     launch_pdl(budget::select_keys_kernel, dim3((unsigned)rows), dim3(threads), smem, stream, a);
     LILY_CHECK_LAUNCH("select_keys");
@@ -277,6 +293,7 @@ LILY_API int lily_move_keys(void* kv, float* weights, const int* block_table, in
     LILY_REQUIRE(page_size > 0 && (page_size & (page_size - 1)) == 0, "move_keys: page_size %d is not a power of two", page_size);
     LILY_REQUIRE(bt_stride > 0 && to_stride > 0 && row_bytes > 0 && row_bytes % 2 == 0 && (long long)keep * row_bytes <= 0x7fff0000, "move_keys: %d places of %d bytes", keep, row_bytes);
     const int vec = row_bytes % 16 == 0 && (uintptr_t)kv % 16 == 0 ? 16 : row_bytes % 4 == 0 && (uintptr_t)kv % 4 == 0 ? 4 : 2;
+    LILY_REQUIRE(row_bytes / vec <= budget::MOVE_THREADS * budget::MOVE_AHEAD / 2, "move_keys: rows of %d bytes in pieces of %d", row_bytes, vec);
     for (long long at = 0; at < rows;) {
         // (a grid has 65,535 lists at most: whole layers of them)
         const long long layer_rows = (long long)requests * nkv, some = layer_rows > 65535 ? 0 : 65535 / layer_rows < layers ? 65535 / layer_rows : layers;
@@ -284,7 +301,7 @@ LILY_API int lily_move_keys(void* kv, float* weights, const int* block_table, in
         const long long first_layer = at / layer_rows, now = first_layer + some <= layers ? some : layers - first_layer;
         budget::MoveArgs a{(unsigned char*)kv + (size_t)first_layer * pages * 2 * nkv * page_size * row_bytes,
                            weights ? weights + (size_t)first_layer * pages * nkv * page_size : nullptr, block_table, to_table,
-                           kept + (size_t)at * keep, bt_stride, to_stride, requests, nkv, page_size, 0, pages, keep, row_bytes};
+                           kept + (size_t)at * keep, bt_stride, to_stride, requests, nkv, page_size, 0, pages, keep, row_bytes, 0};
         while (1 << a.page_shift < page_size) ++a.page_shift;
         const long long lists = now * layer_rows;
         if (vec == 16) budget::launch_move<uint4>(a, lists, in_place, stream);
