@@ -28,9 +28,9 @@ constexpr int SELECT_MOST = 1024;          // threads of a block at most
 constexpr int SELECT_HELD = 48 * 1024;     // places whose ranks a block holds in shared memory; of longer rows they are worked out again a pass
 
 // One block a (layer, request, kv head).  The weights are read once, as ranks; the rank that the last kept weight has comes out eight bits a
-// pass (a histogram of the competing ranks that share the bits found so far; lanes with the same eight bits count as one, since
-// weights are alike in their exponents and would queue for a counter); then every warp counts what it keeps of its stretch of the row, and
-// writes it behind what the warps ahead keep.  What bounds it is the chain of passes, 5 us for 4,096 places, not the bytes.
+// pass (a histogram of the competing ranks that share the bits found so far, in shared memory; lanes that meet in a counter are added up by the
+// hardware, gathering them ahead with match costs more: 8.2 against 13.6 us for 64 rows of 4,096); then every warp counts what it keeps of its stretch
+// of the row, and writes it behind what the warps ahead keep.  What bounds it is the chain of passes, not the bytes.
 __global__ void __launch_bounds__(SELECT_MOST) select_keys_kernel(const SelectArgs a) {
     extern __shared__ uint32_t rank_s[];                             // [min(max_length, SELECT_HELD)]
     __shared__ __align__(16) int hists[4][256];
@@ -57,8 +57,18 @@ __global__ void __launch_bounds__(SELECT_MOST) select_keys_kernel(const SelectAr
     const bool held = n <= SELECT_HELD;
     for (int i = tid; i < 1024; i += threads) hists[0][i] = 0;
     if (held && wanted > 0) {
-#pragma unroll 4
-        for (int j = lo + tid; j < hi; j += threads) rank_s[j] = look(j);
+        for (int j0 = lo + tid; j0 < hi; j0 += 4 * threads) {
+            int page[4];
+            float w[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) page[u] = j0 + u * threads < hi ? table[(j0 + u * threads) >> a.page_shift] : -1;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                w[u] = page[u] >= 0 && page[u] < a.pages ? base[page[u] * page_stride + ((j0 + u * threads) & (a.page_size - 1))] : -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (j0 + u * threads < hi) rank_s[j0 + u * threads] = rank_of(w[u]);
+        }
     }
     auto rank = [&](int j) { return held ? rank_s[j] : look(j); };
     uint32_t prefix = 0;
@@ -71,10 +81,7 @@ __global__ void __launch_bounds__(SELECT_MOST) select_keys_kernel(const SelectAr
                 const int j = j0 + lane;
                 const uint32_t r = j < hi ? rank(j) : 0u;
                 const bool in = j < hi && (shift == 24 || r >> ((shift + 8) & 31) == prefix >> ((shift + 8) & 31));
-                if (!__any_sync(0xffffffffu, in)) continue;
-                const int digit = in ? (int)(r >> shift & 255u) : 256;
-                const uint32_t alike = __match_any_sync(0xffffffffu, digit);
-                if (in && (alike & ((1u << lane) - 1u)) == 0) atomicAdd(&hist[digit], __popc(alike));
+                if (in) atomicAdd(&hist[r >> shift & 255u], 1);
             }
             __syncthreads();
             if (warp == 0) {

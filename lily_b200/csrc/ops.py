@@ -144,7 +144,7 @@ def library():
         lib.lily_attention_decode_scratch_floats.restype = _sz
         lib.lily_attention_decode_weighed_floats.argtypes = [_i, _i, _i, _i, _i, _i, _i]
         lib.lily_attention_decode_weighed_floats.restype = _sz
-        lib.lily_key_weights_floats.argtypes = [_i, _i, _i]
+        lib.lily_key_weights_floats.argtypes = [_i, _i, _i, _i, _i]
         lib.lily_key_weights_floats.restype = _sz
         lib.lily_key_weights_tc_floats.argtypes = [_i, _vp, _vp, _i, _i, _i]
         lib.lily_key_weights_tc_floats.restype = _sz
@@ -1316,7 +1316,8 @@ def _portions(h_prefix_lens: Tuple[int, ...], h_new_lens: Tuple[int, ...], nq: i
     prefix, new = (ctypes.c_int * n)(*h_prefix_lens), (ctypes.c_int * n)(*h_new_lens)
     if dtype == torch.bfloat16 and lib.lily_key_weights_tc_takes(nq, nkv, d, page_size, scale):
         return True, int(lib.lily_key_weights_tc_floats(n, prefix, new, observe, nq, nkv)), prefix, new
-    return False, int(lib.lily_key_weights_floats(n, nq, _heard(h_new_lens, observe))), prefix, new
+    longest = max((p + m for p, m in zip(h_prefix_lens, h_new_lens)), default=0)
+    return False, int(lib.lily_key_weights_floats(n, nq, nkv, _heard(h_new_lens, observe), longest)), prefix, new
 
 
 def key_weights_scratch_floats(h_prefix_lens: Sequence[int], h_new_lens: Sequence[int], nq: int, nkv: int, d: int, page_size: int, scale: float,
@@ -1368,7 +1369,7 @@ def attention_key_weights(q: torch.Tensor, kv_layer: torch.Tensor, weights: torc
         return
     _call("lily_key_weights", _p(q), _p(kv_layer), _p(weights), _i32(block_table, "block_table"), width, _p(cu_seqlens),
           _p(prefix_lens), _p(scratch), requests, int(observe or 0), heard, longest, nq, nkv, d, page_size, float(scale), _dt(q), _stream())
-    launches["count"] += 1                                       # the columns behind the rows
+    launches["count"] += 2                                       # scores, the rows' lse, columns
 
 
 def select_keys(weights: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, max_length: int, keep: int, first: int = 0,
