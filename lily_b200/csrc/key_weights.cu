@@ -11,34 +11,47 @@
 // instead of formed twice; long portions come in runs of rows whose scores fit the scratch, each adding to the weights of the one before.
 #include "common.cuh"
 
+#include <cooperative_groups.h>
+
 namespace lily {
 namespace keyw {
 
+namespace cg = cooperative_groups;
+
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int TM = 64, TN = 64, KC = 32, LD = KC + 4, THREADS = 256;
+
+constexpr int MAX_R = 48;                 // requests a launch
+
+// One request of a launch, for the heard tokens of this run.
+struct Portion {
+    int request;                  // row of the block table
+    int first, rows;              // row of q of the run's first token; rows
+    int place0, prefix, total;    // that token's place, cached places before and after the portion
+    int row_tiles, key_tiles;
+    int tile0, rows0, cols0;      // its first tile of scores, tile of rows, tile of keys (of its first kv head)
+};
 
 struct Args {
     const void* q;                // [tokens, nq * d]
     const void* kv;               // layer base: [pages, 2, nkv, page_size, d]
     float* weights;               // [pages, nkv, page_size]
-    float* scores;                // [requests, nkv, row tiles, key tiles][64][64], log2 units; -inf where a row does not see a place
-    float2* parts;                // [requests, nkv, row tiles, key tiles][64] (max, sum)
-    float* lse;                   // [requests, nkv, row tiles][64]
+    float* scores;                // [tiles][64][64], log2 units; -inf where a row does not see a place
+    float2* parts;                // [tiles][64] (max, sum)
+    float* lse;                   // [tiles of rows][64]
     const int* block_table;
-    int bt_stride;
-    const int* cu_seqlens;        // [requests + 1]
-    const int* prefix_lens;       // [requests]
-    int observe, from, some;      // heard tokens: the last `observe` (0: all); of those [from, from + some) in this run
-    int max_total, nq, nkv, d, page_size, row_tiles, key_tiles;
+    int bt_stride, requests, again, nq, nkv, d, page_size, page_shift;      // again: not the first run, which sets the portions' own weights
     float scale;
+    Portion p[MAX_R];
 };
 
-struct Span { int first, rows, place0, prefix, total; };       // first token of the run (row of q), rows, the first one's place, places before and after
-
-__device__ __forceinline__ Span span_of(const Args& a, int req) {
-    const int t0 = a.cu_seqlens[req], n = a.cu_seqlens[req + 1] - t0, prefix = a.prefix_lens[req], total = min(prefix + n, a.max_total);
-    const int heard = a.observe > 0 ? min(n, a.observe) : n, some = max(0, min(a.some, heard - a.from)), first = n - heard + a.from;
-    return {t0 + first, some * (a.nq / a.nkv), prefix + first, prefix, total};
+// The request of tile `at` of a kernel that numbers its tiles by `OFF`, and the tile within it.
+template <int Portion::*OFF>
+__device__ __forceinline__ const Portion& request_of(const Args& a, int& at) {
+    int r = 0;
+    while (r + 1 < a.requests && a.p[r + 1].*OFF <= at) ++r;
+    at -= a.p[r].*OFF;
+    return a.p[r];
 }
 
 __device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
@@ -73,19 +86,21 @@ __device__ __forceinline__ float4 four(const T* row, int c, int d) {
     return v;
 }
 
-// grid (key tiles, row tiles, requests * kv heads): a tile of scores.  A thread has the 4 x 4 of rows ty + 16 i and keys tx + 16 j, so that the
+// A tile of scores a block (kv heads, row tiles, key tiles of each request, numbered through).  A thread has the 4 x 4 of rows ty + 16 i and keys tx + 16 j, so that the
 // rows of both tiles lie in shared memory as they come (36 numbers a row of 32: no two lanes meet in a bank) and products are packed pairs along the
 // head; the 32 products of a chunk are added up by themselves, which quarters the error of a long sum of like terms.  The next chunk is on its way
 // while one is multiplied.  What bounds it are the multiply-adds.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(THREADS) key_weights_scores_kernel(const Args a) {
+__global__ void __launch_bounds__(THREADS, 2) key_weights_scores_kernel(const __grid_constant__ Args a) {
     __shared__ __align__(16) float q_s[TM][LD], k_s[TN][LD];
     pdl_enter_small();
-    const int req = blockIdx.z / a.nkv, kvh = blockIdx.z % a.nkv, group = a.nq / a.nkv, row0 = blockIdx.y * TM, k0 = blockIdx.x * TN;
-    const Span sp = span_of(a, req);
-    if (row0 >= sp.rows || k0 > sp.place0 + (min(row0 + TM, sp.rows) - 1) / group) return;
+    int at = blockIdx.x;
+    const Portion& sp = request_of<&Portion::tile0>(a, at);
+    const int kt = at % sp.key_tiles, rt = at / sp.key_tiles % sp.row_tiles, kvh = at / sp.key_tiles / sp.row_tiles;
+    const int group = a.nq / a.nkv, row0 = rt * TM, k0 = kt * TN;
+    if (k0 > sp.place0 + (min(row0 + TM, sp.rows) - 1) / group) return;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int* table = a.block_table + (size_t)req * a.bt_stride;
+    const int* table = a.block_table + (size_t)sp.request * a.bt_stride;
     // a thread brings columns 4 (tid % 8) of rows tid / 8 and tid / 8 + 32 of either tile
     const T *q_row[2], *k_row[2];
     const int c4 = (tid & 7) * 4;
@@ -93,7 +108,7 @@ __global__ void __launch_bounds__(THREADS) key_weights_scores_kernel(const Args 
     for (int u = 0; u < 2; ++u) {
         const int r = (tid >> 3) + 32 * u, row = row0 + r, place = k0 + r;
         q_row[u] = row < sp.rows ? (const T*)a.q + ((size_t)(sp.first + row / group) * a.nq + kvh * group + row % group) * a.d : nullptr;
-        k_row[u] = place < sp.total ? (const T*)a.kv + (((size_t)table[place / a.page_size] * 2 * a.nkv + kvh) * a.page_size + place % a.page_size) * a.d : nullptr;
+        k_row[u] = place < sp.total ? (const T*)a.kv + ((((size_t)table[place >> a.page_shift] * 2 * a.nkv + kvh) << a.page_shift) + (place & (a.page_size - 1))) * a.d : nullptr;
     }
     float4 q_next[2], k_next[2];
     auto fetch = [&](int c0) {
@@ -134,7 +149,7 @@ __global__ void __launch_bounds__(THREADS) key_weights_scores_kernel(const Args 
             for (int j = 0; j < 4; ++j) s[i][j] += halves(part[i][j]);
     }
     const float c = a.scale * LOG2E;
-    const size_t tile = ((size_t)blockIdx.z * a.row_tiles + blockIdx.y) * a.key_tiles + blockIdx.x;
+    const size_t tile = blockIdx.x;
     float* to = a.scores + tile * (TM * TN);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -157,83 +172,149 @@ __global__ void __launch_bounds__(THREADS) key_weights_scores_kernel(const Args 
     }
 }
 
-// grid (row tiles, requests * kv heads): a row's tiles joined in their order.
-__global__ void __launch_bounds__(TM) key_weights_lse_kernel(const Args a) {
+// A tile of rows a block: the parts of each row joined in their order.
+__global__ void __launch_bounds__(TM) key_weights_lse_kernel(const __grid_constant__ Args a) {
     pdl_enter_small();
-    const int req = blockIdx.y / a.nkv, group = a.nq / a.nkv, row = blockIdx.x * TM + threadIdx.x;
-    const Span sp = span_of(a, req);
-    if (blockIdx.x * TM >= sp.rows) return;
+    int at = blockIdx.x;
+    const Portion& sp = request_of<&Portion::rows0>(a, at);
+    const int rt = at % sp.row_tiles, kvh = at / sp.row_tiles, group = a.nq / a.nkv, row = rt * TM + threadIdx.x;
     // the tiles that were made for this tile of rows
-    const int tiles = (sp.place0 + (min((int)(blockIdx.x + 1) * TM, sp.rows) - 1) / group) / TN + 1;
-    const size_t tile = (size_t)blockIdx.y * a.row_tiles + blockIdx.x;
-    const float2* part = a.parts + tile * a.key_tiles * TM + threadIdx.x;
+    const int tiles = (sp.place0 + (min((rt + 1) * TM, sp.rows) - 1) / group) / TN + 1;
+    const float2* part = a.parts + ((size_t)sp.tile0 + ((size_t)kvh * sp.row_tiles + rt) * sp.key_tiles) * TM + threadIdx.x;
     float m = -INFINITY, l = 0.f;
     for (int t = 0; t < tiles; ++t) m = fmaxf(m, part[(size_t)t * TM].x);
     for (int t = 0; t < tiles; ++t) {
         const float2 v = part[(size_t)t * TM];
         if (v.x > -INFINITY || v.y != 0.f) l = fmaf(v.y, exp2f(v.x - m), l);              // (a NaN is no maximum, but makes the sum one)
     }
-    a.lse[tile * TM + threadIdx.x] = row < sp.rows ? m + log2f(l) : 0.f;
+    a.lse[(size_t)blockIdx.x * TM + threadIdx.x] = row < sp.rows ? m + log2f(l) : 0.f;
 }
 
-// grid (key tiles, requests * kv heads): the sums of a tile's columns, four a thread over every sixteenth row.
-__global__ void __launch_bounds__(THREADS) key_weights_columns_kernel(const Args a) {
-    __shared__ __align__(16) float sum_s[16][TN];
+// grid (tiles of keys, parts): the sums of a tile's columns, four a thread over every 32nd row.  What bounds it is the chain of
+// reads: the parts, a cluster of up to eight blocks, take turns at the tiles of rows, eight rows a thread on their way, and the first adds up what all have
+// found, in their order.
+constexpr int COL_THREADS = 512, COL_PARTS = 8;
+__global__ void __launch_bounds__(COL_THREADS) key_weights_columns_kernel(const __grid_constant__ Args a) {
+    __shared__ __align__(16) float sum_s[32][TN];
+    __shared__ float parts_s[COL_PARTS][TN];
+    if (gridDim.y > 1) cluster_arrive_started();
     pdl_enter_small();
-    const int req = blockIdx.y / a.nkv, kvh = blockIdx.y % a.nkv, group = a.nq / a.nkv, k0 = blockIdx.x * TN;
-    const Span sp = span_of(a, req);
-    if (k0 >= sp.total) return;
+    int tile_at = blockIdx.x;
+    const Portion& sp = request_of<&Portion::cols0>(a, tile_at);
+    const int kt = tile_at % sp.key_tiles, kvh = tile_at / sp.key_tiles, group = a.nq / a.nkv, k0 = kt * TN, part = blockIdx.y, parts = gridDim.y;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     // the weights' places, asked for ahead
     float* at = nullptr;
     float sum = 0.f;
-    if (tid < TN && k0 + tid < sp.total) {
+    if (part == 0 && tid < TN && k0 + tid < sp.total) {
         const int place = k0 + tid;
-        at = a.weights + ((size_t)a.block_table[(size_t)req * a.bt_stride + place / a.page_size] * a.nkv + kvh) * a.page_size + place % a.page_size;
-        sum = place < sp.prefix || a.from > 0 ? *at : 0.f;
+        at = a.weights + (((size_t)a.block_table[(size_t)sp.request * a.bt_stride + (place >> a.page_shift)] * a.nkv + kvh) << a.page_shift) + (place & (a.page_size - 1));
+        sum = place < sp.prefix || a.again ? *at : 0.f;
     }
     float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int first = max(0, k0 - sp.place0) * group / TM;           // the first tile of rows that sees any of these places
-    for (int t = first; t * TM < sp.rows; ++t) {
-        const size_t tile = (size_t)blockIdx.y * a.row_tiles + t;
-        const float4* scores = reinterpret_cast<const float4*>(a.scores + (tile * a.key_tiles + blockIdx.x) * (TM * TN));
-        const float* lse = a.lse + tile * TM;
+    const int first = max(0, k0 - sp.place0) * group / TM, tiles = sp.row_tiles;      // the tiles of rows that see any of these places
+    for (int t0 = first + part; t0 < tiles; t0 += 4 * parts) {
+        float4 s[8];
+        float e[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 s = scores[(ty + 16 * i) * (TN / 4) + tx];
-            const float e = lse[ty + 16 * i];
-            w.x += exp2f(s.x - e);
-            w.y += exp2f(s.y - e);
-            w.z += exp2f(s.z - e);
-            w.w += exp2f(s.w - e);
+        for (int u = 0; u < 8; ++u) {
+            const int t = t0 + (u >> 1) * parts, r = ty + 32 * (u & 1);
+            s[u] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            e[u] = 0.f;
+            if (t < tiles) {
+                const size_t rows = (size_t)kvh * sp.row_tiles + t;
+                s[u] = reinterpret_cast<const float4*>(a.scores + ((size_t)sp.tile0 + rows * sp.key_tiles + kt) * (TM * TN))[r * (TN / 4) + tx];
+                e[u] = a.lse[((size_t)sp.rows0 + rows) * TM + r];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            w.x += exp2f(s[u].x - e[u]);
+            w.y += exp2f(s[u].y - e[u]);
+            w.z += exp2f(s[u].z - e[u]);
+            w.w += exp2f(s[u].w - e[u]);
         }
     }
     *reinterpret_cast<float4*>(&sum_s[ty][4 * tx]) = w;
     __syncthreads();
-    if (at) {
+    if (tid < TN) {
+        float mine = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum += sum_s[i][tid];
-        *at = sum;
+        for (int i = 0; i < 32; ++i) mine += sum_s[i][tid];
+        if (parts == 1) sum += mine;
+        else {
+            cluster_wait_started();                                  // (the warps of these threads; the others below)
+            *cg::this_cluster().map_shared_rank(&parts_s[part][tid], 0) = mine;
+        }
     }
+    if (parts > 1) {
+        if (tid >= TN) cluster_wait_started();
+        cg::this_cluster().sync();
+        if (tid < TN)
+            for (int i = 0; i < parts; ++i) sum += parts_s[i][tid];
+    }
+    if (at) *at = sum;
 }
 
-// Heard tokens of a run, so that its scores fit about a gigabyte, and the floats of scratch it takes.
-struct Runs { int some, row_tiles, key_tiles; size_t tiles, floats; };
-static Runs runs_of(int requests, int nq, int nkv, int max_heard, int max_total) {
-    Runs r{};
-    const int group = nq / nkv;
-    r.key_tiles = (max_total + TN - 1) / TN;
-    const size_t row_tile = (size_t)requests * nkv * r.key_tiles * TM * TN;          // floats of one tile of rows of every request and head
-    const size_t most = (size_t)1 << 28;
-    size_t tiles = most / (row_tile ? row_tile : 1);
-    if (tiles < 1) tiles = 1;
-    const size_t need = ((size_t)max_heard * group + TM - 1) / TM;
-    if (tiles >= need) r.some = max_heard;
-    else r.some = (int)(tiles * TM / group > 0 ? tiles * TM / group : 1);
-    r.row_tiles = (int)(((size_t)r.some * group + TM - 1) / TM);
-    r.tiles = (size_t)requests * nkv * r.row_tiles;
-    r.floats = r.tiles * r.key_tiles * (TM * TN + 2 * TM) + r.tiles * TM;
-    return r;
+// The tiles of a launch: heard tokens [from, from + some) of up to MAX_R requests (host lengths).  Requests without such tokens are left out.
+struct Tiles { long long scores, rows, keys; };
+static Tiles plan(Args& a, int requests, int request0, int token0, const int* prefix, const int* fresh, int observe, int from, int some) {
+    Tiles t{};
+    const int group = a.nq / a.nkv;
+    a.requests = 0;
+    for (int r = 0; r < requests; ++r) {
+        const int heard = observe > 0 && observe < fresh[r] ? observe : fresh[r], mine = heard - from < some ? heard - from : some;
+        if (mine > 0) {
+            Portion& p = a.p[a.requests++];
+            p.request = request0 + r;
+            p.first = token0 + fresh[r] - heard + from;
+            p.rows = mine * group;
+            p.place0 = prefix[r] + fresh[r] - heard + from;
+            p.prefix = prefix[r];
+            p.total = prefix[r] + fresh[r];
+            p.row_tiles = (p.rows + TM - 1) / TM;
+            p.key_tiles = (p.total + TN - 1) / TN;
+            p.tile0 = (int)t.scores;
+            p.rows0 = (int)t.rows;
+            p.cols0 = (int)t.keys;
+            t.scores += (long long)a.nkv * p.row_tiles * p.key_tiles;
+            t.rows += (long long)a.nkv * p.row_tiles;
+            t.keys += (long long)a.nkv * p.key_tiles;
+        }
+        token0 += fresh[r];
+    }
+    return t;
+}
+static size_t floats_of(const Tiles& t) { return (size_t)t.scores * (TM * TN + 2 * TM) + (size_t)t.rows * TM; }
+
+// Heard tokens of a run: as many as keep the scores of MAX_R requests within about a gigabyte, a tile of rows at least.
+static int run_of(const Args& a, int requests, const int* prefix, const int* fresh) {
+    long long places = 0;
+    for (int r = 0; r < requests; ++r) places += prefix[r] + fresh[r] + TN;
+    const int group = a.nq / a.nkv, least = (TM + group - 1) / group;
+    const long long most = ((long long)1 << 28) / (places * a.nq > 0 ? places * a.nq : 1);
+    return most < least ? least : most > 0x7fffff ? 0x7fffff : (int)most;
+}
+
+template <typename F>
+static int each_run(Args& a, int requests, const int* prefix, const int* fresh, int observe, F&& use) {
+    int token0 = 0;
+    for (int r = 0; r < requests; r += MAX_R) {
+        const int now = requests - r < MAX_R ? requests - r : MAX_R, some = run_of(a, now, prefix + r, fresh + r);
+        int heard = 0, tokens = 0;
+        for (int i = r; i < r + now; ++i) {
+            const int h = observe > 0 && observe < fresh[i] ? observe : fresh[i];
+            heard = h > heard ? h : heard;
+            tokens += fresh[i];
+        }
+        for (int from = 0; from < heard; from += some) {
+            const Tiles t = plan(a, now, r, token0, prefix + r, fresh + r, observe, from, some);
+            a.again = from > 0;
+            if (int rc = use(t)) return rc;
+        }
+        token0 += tokens;
+    }
+    return 0;
 }
 
 }  // namespace keyw
@@ -241,34 +322,64 @@ static Runs runs_of(int requests, int nq, int nkv, int max_heard, int max_total)
 
 using namespace lily;
 
-// Floats of scratch: scores, the rows' parts, their lse.
-LILY_API size_t lily_key_weights_floats(int requests, int nq, int nkv, int max_heard, int max_total) {
-    return requests > 0 && nkv > 0 && max_heard > 0 && max_total > 0 ? keyw::runs_of(requests, nq, nkv, max_heard, max_total).floats : 0;
+// Floats of scratch for portions of `fresh` tokens behind `prefix` places (host arrays): scores, the rows' parts, their lse.
+LILY_API size_t lily_key_weights_floats(int requests, const int* prefix, const int* fresh, int observe, int nq, int nkv) {
+    static thread_local keyw::Args a;
+    a.nq = nq;
+    a.nkv = nkv;
+    size_t most = 0;
+    keyw::each_run(a, requests, prefix, fresh, observe, [&](const keyw::Tiles& t) {
+        const size_t n = keyw::floats_of(t);
+        most = n > most ? n : most;
+        return 0;
+    });
+    return most;
 }
 
-LILY_API int lily_key_weights(const void* q, const void* kv, float* weights, const int* block_table, int bt_stride, const int* cu_seqlens,
-                              const int* prefix_lens, float* scratch, int requests, int observe, int max_heard, int max_total, int nq, int nkv,
-                              int d, int page_size, float scale, int dtype, cudaStream_t stream) {
-    if (requests == 0 || max_total == 0) return 0;
+LILY_API int lily_key_weights(const void* q, const void* kv, float* weights, const int* block_table, int bt_stride, float* scratch, int requests,
+                              const int* prefix, const int* fresh, int observe, int nq, int nkv, int d, int page_size, float scale, int dtype,
+                              cudaStream_t stream) {
     LILY_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "attention_key_weights: %d query heads over %d kv heads", nq, nkv);
-    LILY_REQUIRE(d >= 1 && page_size > 0 && observe >= 0 && max_heard >= 1, "attention_key_weights: head size %d, pages of %d, the last %d heard", d, page_size, observe);
-    LILY_REQUIRE((long long)requests * nkv <= 65535, "attention_key_weights: %d requests of %d kv heads", requests, nkv);
+    LILY_REQUIRE(d >= 1 && page_size > 0 && (page_size & (page_size - 1)) == 0 && observe >= 0, "attention_key_weights: head size %d, pages of %d, the last %d heard", d, page_size,
+                 observe);
     LILY_REQUIRE(dtype == kF32 || dtype == kBF16, "attention_key_weights: dtype %d", dtype);
-    const keyw::Runs run = keyw::runs_of(requests, nq, nkv, max_heard, max_total);
-    LILY_REQUIRE(run.row_tiles <= 65535, "attention_key_weights: %d tiles of rows", run.row_tiles);
-    float* parts = scratch + run.tiles * run.key_tiles * (keyw::TM * keyw::TN);
-    keyw::Args a{q, kv, weights, scratch, (float2*)parts, parts + run.tiles * run.key_tiles * 2 * keyw::TM, block_table, bt_stride, cu_seqlens, prefix_lens, observe, 0, run.some,
-                 max_total, nq, nkv, d, page_size, run.row_tiles, run.key_tiles, scale};
+    keyw::Args a{};
+    a.q = q; a.kv = kv; a.weights = weights; a.scores = scratch; a.block_table = block_table; a.bt_stride = bt_stride; a.nq = nq; a.nkv = nkv; a.d = d;
+    a.page_size = page_size; a.scale = scale;
+    while (1 << a.page_shift < page_size) ++a.page_shift;
     const bool vec = d % 4 == 0 && (((uintptr_t)q | (uintptr_t)kv) & 15) == 0;
-    for (; a.from < max_heard; a.from += a.some) {
-        const dim3 grid(run.key_tiles, run.row_tiles, requests * nkv);
+    const int rc = keyw::each_run(a, requests, prefix, fresh, observe, [&](const keyw::Tiles& t) {
+        LILY_REQUIRE(t.scores <= 0x7fffffff, "attention_key_weights: %lld tiles", t.scores);
+        a.parts = (float2*)(a.scores + (size_t)t.scores * (keyw::TM * keyw::TN));
+        a.lse = (float*)(a.parts + (size_t)t.scores * keyw::TM);
+        const dim3 grid((unsigned)t.scores);
 #define LAUNCH(T, V) launch_pdl(keyw::key_weights_scores_kernel<T, V>, grid, dim3(keyw::THREADS), 0, stream, a)
         if (dtype == kF32) { if (vec) LAUNCH(float, true); else LAUNCH(float, false); }
         else { if (vec) LAUNCH(__nv_bfloat16, true); else LAUNCH(__nv_bfloat16, false); }
 #undef LAUNCH
-        launch_pdl(keyw::key_weights_lse_kernel, dim3(run.row_tiles, requests * nkv), dim3(keyw::TM), 0, stream, a);
-        launch_pdl(keyw::key_weights_columns_kernel, dim3(run.key_tiles, requests * nkv), dim3(keyw::THREADS), 0, stream, a);
-    }
+        launch_pdl(keyw::key_weights_lse_kernel, dim3((unsigned)t.rows), dim3(keyw::TM), 0, stream, a);
+        // four tiles of rows a block or more
+        int tiles = 0;
+        for (int r = 0; r < a.requests; ++r) tiles = a.p[r].row_tiles > tiles ? a.p[r].row_tiles : tiles;
+        int parts = tiles / 4;
+        parts = parts < 1 ? 1 : parts > keyw::COL_PARTS ? keyw::COL_PARTS : parts;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)t.keys, parts);
+        cfg.blockDim = dim3(keyw::COL_THREADS);
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = 1;
+        attr[1].val.clusterDim.y = parts;
+        attr[1].val.clusterDim.z = 1;
+        cfg.attrs = pdl_enabled() ? attr : attr + 1;
+        cfg.numAttrs = pdl_enabled() ? 2 : 1;
+        cudaLaunchKernelEx(&cfg, keyw::key_weights_columns_kernel, a);
+        return 0;
+    });
+    if (rc) return rc;
     LILY_CHECK_LAUNCH("attention_key_weights");
     return 0;
 }

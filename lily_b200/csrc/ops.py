@@ -101,7 +101,7 @@ _SIGNATURES = {
     "lily_axes_rope_write": [_vp, _i, _i, _sz, _i, _vp, _vp, _i, _f, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _vp,
                              _i, _i, _i, _i, _i, _i, _vp],
     "lily_attention_decode_weighed": [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp],
-    "lily_key_weights": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _f, _i, _vp],
+    "lily_key_weights": [_vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _vp],
     "lily_key_weights_tc": [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp],
     "lily_select_keys": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
     "lily_move_keys": [_vp, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
@@ -144,7 +144,7 @@ def library():
         lib.lily_attention_decode_scratch_floats.restype = _sz
         lib.lily_attention_decode_weighed_floats.argtypes = [_i, _i, _i, _i, _i, _i, _i]
         lib.lily_attention_decode_weighed_floats.restype = _sz
-        lib.lily_key_weights_floats.argtypes = [_i, _i, _i, _i, _i]
+        lib.lily_key_weights_floats.argtypes = [_i, _vp, _vp, _i, _i, _i]
         lib.lily_key_weights_floats.restype = _sz
         lib.lily_key_weights_tc_floats.argtypes = [_i, _vp, _vp, _i, _i, _i]
         lib.lily_key_weights_tc_floats.restype = _sz
@@ -1316,8 +1316,7 @@ def _portions(h_prefix_lens: Tuple[int, ...], h_new_lens: Tuple[int, ...], nq: i
     prefix, new = (ctypes.c_int * n)(*h_prefix_lens), (ctypes.c_int * n)(*h_new_lens)
     if dtype == torch.bfloat16 and lib.lily_key_weights_tc_takes(nq, nkv, d, page_size, scale):
         return True, int(lib.lily_key_weights_tc_floats(n, prefix, new, observe, nq, nkv)), prefix, new
-    longest = max((p + m for p, m in zip(h_prefix_lens, h_new_lens)), default=0)
-    return False, int(lib.lily_key_weights_floats(n, nq, nkv, _heard(h_new_lens, observe), longest)), prefix, new
+    return False, int(lib.lily_key_weights_floats(n, prefix, new, observe, nq, nkv)), prefix, new
 
 
 def key_weights_scratch_floats(h_prefix_lens: Sequence[int], h_new_lens: Sequence[int], nq: int, nkv: int, d: int, page_size: int, scale: float,
@@ -1367,8 +1366,8 @@ def attention_key_weights(q: torch.Tensor, kv_layer: torch.Tensor, weights: torc
               requests, prefix, new, int(observe or 0), nq, nkv, d, page_size, float(scale), _stream())
         launches["count"] += 2                                   # rows, their joining, columns
         return
-    _call("lily_key_weights", _p(q), _p(kv_layer), _p(weights), _i32(block_table, "block_table"), width, _p(cu_seqlens),
-          _p(prefix_lens), _p(scratch), requests, int(observe or 0), heard, longest, nq, nkv, d, page_size, float(scale), _dt(q), _stream())
+    _call("lily_key_weights", _p(q), _p(kv_layer), _p(weights), _i32(block_table, "block_table"), width, _p(scratch), requests, prefix, new,
+          int(observe or 0), nq, nkv, d, page_size, float(scale), _dt(q), _stream())
     launches["count"] += 2                                       # scores, the rows' lse, columns
 
 
