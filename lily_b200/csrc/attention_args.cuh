@@ -53,6 +53,8 @@ struct AttnArgs {
     int v_all;                // CUDA-core kernels: a query head is weighted over the values of every kv head, not only its own:
                               // its output row is [nkv][dv] (the caller mixes heads afterwards); `dv` stays one head's size
     int out_f32;              // CUDA-core kernels: outputs are written in float32 whatever the cache's dtype
+    float* scores;            // float32 decode kernel that weighs its keys: [requests, nq, score_stride], in units of log2 e
+    int score_stride, max_len;      // ... and the places a row has at most
     int stages;               // decode, tensor-core kernel: key/value tiles a block keeps in shared memory (0: the default, 2;
                               // 3: two blocks a SM instead of three, each with two tiles in flight; head sizes up to 128)
 };

@@ -23,7 +23,9 @@ constexpr int MAX_G = 8;
 // Query heads a block takes (G, at least the heads of a kv head) x pieces of 128 columns (C): as many warps as the registers allow.
 __host__ __device__ constexpr int warps_of(int g, int c) { return c == 1 && g <= 4 ? 16 : 8; }
 
-template <int G, int C>
+// WEIGHED: the scores go to `a.scores` as they are formed, and a row's results to scratch in units of log2 e whatever the ranges, for the
+// kernel that turns them into outputs and the weights of the keys (attention_weighed.cu).
+template <int G, int C, bool WEIGHED = false>
 __global__ void __launch_bounds__(warps_of(G, C) * 32)
 attention_decode_f32_kernel(const AttnArgs a) {
     constexpr int WARPS = warps_of(G, C), N = KB * G, STEP = WARPS * KB;
@@ -35,7 +37,7 @@ attention_decode_f32_kernel(const AttnArgs a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int d = a.d, dv = a.dv, group = a.nq / a.nkv;
     const int req = blockIdx.x, kvh = blockIdx.y;
-    const int seq = a.seq_lens[req];
+    const int seq = WEIGHED ? min(max(a.seq_lens[req], 0), a.max_len) : a.seq_lens[req];
     const int klo = (a.window > 0 && seq > a.window) ? seq - a.window : 0;
     const int nkeep = min(a.keep_first, klo);
     const int total = nkeep + seq - klo;
@@ -110,6 +112,8 @@ attention_decode_f32_kernel(const AttnArgs a) {
         constexpr int REST = 32 / N;                          // lanes that hold the same sum
         const int key = lane / REST % KB;
         const float sv = u0 + key < uend ? (cap > 0.f ? cap * tanhf(s[0] * cap_in) : s[0] * a.scale) : -INFINITY;
+        if (WEIGHED && lane % REST == 0 && head < group && u0 + key < uend)
+            a.scores[((size_t)req * a.nq + kvh * group + head) * a.score_stride + u0 + key] = sv * 1.4426950408889634f;
         float mx = sv;
 #pragma unroll
         for (int off = REST; off < PER_HEAD; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
@@ -182,11 +186,11 @@ attention_decode_f32_kernel(const AttnArgs a) {
             den = fmaf(lw, f, den);
         }
         const size_t row = (size_t)req * a.nq + kvh * group + h;
-        if (a.splits > 1) {
+        if (WEIGHED || a.splits > 1) {
             const size_t at = row * a.splits + blockIdx.z;
             *reinterpret_cast<float4*>(a.part_o + at * dv + col) = sum;
             if (col == 0) {
-                a.part_ml[at * 2] = mx;
+                a.part_ml[at * 2] = WEIGHED ? mx * 1.4426950408889634f : mx;
                 a.part_ml[at * 2 + 1] = den;
             }
         } else {
@@ -196,11 +200,11 @@ attention_decode_f32_kernel(const AttnArgs a) {
     }
 }
 
-template <int G, int C>
+template <int G, int C, bool WEIGHED = false>
 static int launch(const AttnArgs& a, int requests, cudaStream_t stream) {
     constexpr int WARPS = warps_of(G, C);
     const size_t smem = sizeof(float) * WARPS * G * ((size_t)a.dv + 2);
-    auto kern = attention_decode_f32_kernel<G, C>;
+    auto kern = attention_decode_f32_kernel<G, C, WEIGHED>;
     static bool configured = false;                            // set once for the widest head, never while a graph is captured
     if (!configured) {
         const size_t most = sizeof(float) * WARPS * G * (128 * C + 2);
@@ -223,6 +227,16 @@ int attention_decode_f32(const AttnArgs& a, int requests, cudaStream_t stream) {
     const int g = a.nq / a.nkv;
     const bool wide = a.d > 128 || a.dv > 128;
 #define GO(G) return wide ? f32d::launch<G, 2>(a, requests, stream) : f32d::launch<G, 1>(a, requests, stream)
+    if (g == 1) GO(1);
+    if (g == 2) GO(2);
+    if (g <= 4) GO(4);
+    GO(8);
+#undef GO
+}
+
+int attention_decode_f32_weighed(const AttnArgs& a, int requests, cudaStream_t stream) {
+    const int g = a.nq / a.nkv;
+#define GO(G) return a.d > 128 ? f32d::launch<G, 2, true>(a, requests, stream) : f32d::launch<G, 1, true>(a, requests, stream)
     if (g == 1) GO(1);
     if (g == 2) GO(2);
     if (g <= 4) GO(4);

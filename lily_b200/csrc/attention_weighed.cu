@@ -5,12 +5,17 @@
 // with w float32 [pages, kv_heads, page_size] beside the keys: the newest place's weight is set, whatever an earlier owner left there.
 // The keys of a request are cut into ranges; a block leaves its scores (in units of log2 e) and its (max, sum, output) in scratch, and a
 // second kernel, which knows every range's, writes outputs and weights.
+#include "attention_args.cuh"
 #include "common.cuh"
 #include "tcgen05.cuh"
 
 #include <cooperative_groups.h>
 
 namespace lily {
+bool attention_decode_f32_takes(const AttnArgs& a);
+int attention_decode_f32_weighed(const AttnArgs& a, int requests, cudaStream_t stream);
+int* decode_lost_word();
+
 namespace weighed {
 
 constexpr float LOG2E = 1.4426950408889634f;
@@ -595,6 +600,13 @@ struct Plan { int splits; bool mma, cluster; };
 static Plan plan_of(int requests, int nq, int nkv, int d, int max_len, int page_size, int dtype) {
     const int group = nq / nkv, sms = sm_count();
     const bool mma = dtype == kBF16 && (d == 64 || d == 128) && (page_size & (page_size - 1)) == 0;
+    if (dtype == kF32 && group <= 8 && d % 4 == 0 && d <= 256) {
+        // the kernel that cuts a row's keys over the warps of a block: a wave of blocks, none under 64 keys
+        const long pairs = (long)requests * nkv, most = (max_len + 63) / 64;
+        long s = sms / pairs;
+        s = s < most ? s : most;
+        return {(int)(s < 1 ? 1 : s > 64 ? 64 : s), false, false};
+    }
     if (!mma) {
         const long pairs = (long)requests * nkv * ((group + RH - 1) / RH);
         long s = (3L * sms + pairs - 1) / pairs, most = (max_len + 127) / 128;
@@ -623,7 +635,6 @@ static Plan plan_of(int requests, int nq, int nkv, int d, int max_len, int page_
 }
 
 }  // namespace weighed
-int* decode_lost_word();
 }  // namespace lily
 
 using namespace lily;
@@ -679,6 +690,18 @@ LILY_API int lily_attention_decode_weighed(const void* q, const void* kv, float*
             launch_pdl(weighed::decode_weighed_join_kernel<__nv_bfloat16>, join, dim3(weighed::JOIN_THREADS), group * sizeof(float), stream, a);
         LILY_CHECK_LAUNCH("attention_decode_weighed");
         return 0;
+    }
+    if (dtype == kF32) {
+        AttnArgs f{};
+        f.q = q; f.kv = kv; f.out = out; f.block_table = block_table; f.bt_stride = bt_stride; f.seq_lens = seq_lens; f.part_o = a.part_o; f.part_ml = a.part_ml;
+        f.splits = plan.splits; f.nq = nq; f.nkv = nkv; f.d = d; f.dv = d; f.page_size = page_size; f.scale = scale;
+        f.scores = a.scores; f.score_stride = score_stride; f.max_len = max_len;
+        if (attention_decode_f32_takes(f)) {
+            if (int rc = attention_decode_f32_weighed(f, requests, stream)) return rc;
+            launch_pdl(weighed::decode_weighed_join_kernel<float>, join, dim3(weighed::JOIN_THREADS), group * sizeof(float), stream, a);
+            LILY_CHECK_LAUNCH("attention_decode_weighed");
+            return 0;
+        }
     }
     const dim3 grid(requests, nkv * ((group + weighed::RH - 1) / weighed::RH), plan.splits);
     const size_t smem = weighed::simt_floats(d) * sizeof(float);
