@@ -158,10 +158,21 @@ __device__ __forceinline__ void load_piece(const Args& a, const IN* src, Two (&v
         }
     }
 }
+// N gains (16-byte aligned).
 template <typename W, int N>
 __device__ __forceinline__ void load_gain(const W* g, Two (&v)[N / 2]) {
+    if constexpr (sizeof(W) == 2 && N == 8) unpack<W, N>(*reinterpret_cast<const uint4*>(g), v);
+    else if constexpr (sizeof(W) == 4) {
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) v[i] = two(to_float(g[2 * i]), to_float(g[2 * i + 1]));
+        for (int i = 0; i < N / 4; ++i) {
+            const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(g + 4 * i);
+            v[2 * i] = t.x;
+            v[2 * i + 1] = t.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) v[i] = two(to_float(g[2 * i]), to_float(g[2 * i + 1]));
+    }
 }
 template <typename T, int N>
 __device__ __forceinline__ void store_piece(T* dst, const Two (&v)[N / 2]) {
@@ -218,8 +229,11 @@ __global__ void __launch_bounds__(WIDE_THREADS, 4) axes_rope_write_wide_kernel(c
         }
         row_s[tid] = row;
     }
-    for (int e = tid; e < TOK * half; e += blockDim.x) {
-        const int k = TOK == 1 ? 0 : e / half, j = e - k * half;
+    // (a pair's threads go over the tokens: pairs first, as many tokens at a time as the block has threads for)
+    const int pairs = min((int)blockDim.x, max(half, 1)), at_once = (int)blockDim.x / pairs;
+    for (int e = tid; e < at_once * pairs; e += blockDim.x)
+    for (int j = e % pairs; j < half; j += pairs)
+    for (int k = e / pairs; k < TOK; k += at_once) {
         const int axis = a.pair_axis[j];
         const int pos = axis >= 0 && axis < a.axes && n0 + k < a.tokens ? a.positions[(size_t)axis * a.tokens + n0 + k] : -1;
         const bool known = pos >= 0 && pos < a.table_rows;
@@ -302,7 +316,7 @@ LILY_API int lily_axes_rope_write(const void* qkv, int in_dtype, int splits, siz
     const int bytes = act_dtype == kBF16 ? 2 : 4, piece = 16 / bytes, group = d / (2 * piece);
     int shift = 0;
     while (1 << shift < group) ++shift;
-    const uintptr_t where = (uintptr_t)qkv | (uintptr_t)kv | (uintptr_t)q_out;
+    const uintptr_t where = (uintptr_t)qkv | (uintptr_t)kv | (uintptr_t)q_out | (uintptr_t)q_gain | (uintptr_t)k_gain;
     // whole pieces of 16 bytes on every side; else, and for heads that are no power of two of pieces, a warp a head 
     const bool wide = d % (2 * piece) == 0 && 1 << shift == group && group <= 32 && rd % (2 * piece) == 0 && ld % piece == 0 &&
                       (in_dtype == act_dtype || ld % 4 == 0) && (size_t)stride % 4 == 0 && where % 16 == 0 && tokens <= 65535;
