@@ -94,15 +94,12 @@ __global__ void __launch_bounds__(128) axes_rope_write_kernel(const Args a) {
 
 // Sixteen bytes of activations an access (N = 8 bfloat16 or 4 float32 numbers) and G = d / (2 N) threads a head (a power of two, at most a
 // warp), each with two pieces: of the rotated features N neighbouring ones and their partners rd / 2 further, of the rest two neighbouring pieces.  So the
-// rotation needs no exchange and the norm log2(G) shuffles.  A block has heads of one token or of four.  Its cosines and sines, each pair's from its own
-// axis's row, and the tokens' rows in the cache are looked up once a block, while the heads are on their way.
-//   One token (few of them, or partial sums, of which AHEAD planes are asked for before the first is added): the chain of reads bounds it.
-//   Four: a thread's pieces come with cp.async into shared memory that it alone reads, so that 128 bytes a thread are on their way and few registers held;
-//   the bytes bound it (held in registers instead, 102 of them, two blocks a SM had 64 KB on their way where 6.5 TB/s want 150: 21.5 us).
-constexpr int WIDE_THREADS = 256, AHEAD = 4, TOKENS = 4;
+// rotation needs no exchange, the norm log2(G) shuffles, and no thread waits for another.  The positions of up to four axes are read
+// beside the axes of a thread's pairs, not behind them; where its pairs share an axis their cosines and sines are 16-byte reads.  What bounds it is the chain
+// of reads (axis and positions, tables, result), for few tokens and for many, which small blocks of short-lived threads hide best.
+constexpr int WIDE_THREADS = 128, AHEAD = 4;
 
-// Numbers in pairs (mul and fma.rn.f32x2: two IEEE operations an instruction).  For many tokens it is instructions that are short, 250 a token and
-// thread number by number.
+// Numbers in pairs (mul and fma.rn.f32x2: two IEEE operations an instruction).
 typedef unsigned long long Two;
 __device__ __forceinline__ Two two(float a, float b) {
     Two r;
@@ -188,109 +185,114 @@ __device__ __forceinline__ void store_piece(T* dst, const Two (&v)[N / 2]) {
     } else *reinterpret_cast<ulonglong2*>(dst) = make_ulonglong2(v[0], v[1]);
 }
 
-// grid (blocks of a token's heads, tokens or runs of four); dynamic shared memory: [TOK][2][rd / 2] cosines and sines, then (four tokens) the pieces
-template <typename T, typename IN, typename W, int TOK>
-__global__ void __launch_bounds__(WIDE_THREADS, 4) axes_rope_write_wide_kernel(const Args a, const int group_shift) {
+// The tables' numbers of N pairs from `j` on.
+template <int N>
+__device__ __forceinline__ void load_turn(const Args& a, int n, int j, Two (&c)[N / 2], Two (&s)[N / 2]) {
+    const int half = a.rd / 2;
+    int pos[4], axis[N];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) pos[k] = k < a.axes ? a.positions[(size_t)k * a.tokens + n] : -1;
+    bool alike = true;
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const int4 t = *reinterpret_cast<const int4*>(a.pair_axis + j + i);
+        axis[i] = t.x, axis[i + 1] = t.y, axis[i + 2] = t.z, axis[i + 3] = t.w;
+        alike = alike && t.x == axis[0] && t.y == t.x && t.z == t.x && t.w == t.x;
+    }
+    auto position = [&](int ax) {
+        int at = ax == 0 ? pos[0] : ax == 1 ? pos[1] : ax == 2 ? pos[2] : ax == 3 ? pos[3] : -1;
+        if (ax >= 4 && ax < a.axes) at = a.positions[(size_t)ax * a.tokens + n];
+        return at < a.table_rows ? at : -1;
+    };
+    const float nan = __int_as_float(0x7fffffff);
+    if (alike) {
+        const int at = position(axis[0]);
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            ulonglong2 x = make_ulonglong2(two(nan, nan), two(nan, nan)), y = x;
+            if (at >= 0) {
+                x = *reinterpret_cast<const ulonglong2*>(a.cos_t + (size_t)at * half + j + 4 * i);
+                y = *reinterpret_cast<const ulonglong2*>(a.sin_t + (size_t)at * half + j + 4 * i);
+            }
+            c[2 * i] = x.x, c[2 * i + 1] = x.y, s[2 * i] = y.x, s[2 * i + 1] = y.y;
+        }
+    } else {
+        float x[N], y[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int at = position(axis[i]);
+            x[i] = at >= 0 ? a.cos_t[(size_t)at * half + j + i] : nan;
+            y[i] = at >= 0 ? a.sin_t[(size_t)at * half + j + i] : nan;
+        }
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) c[i] = two(x[2 * i], x[2 * i + 1]), s[i] = two(y[2 * i], y[2 * i + 1]);
+    }
+}
+
+// grid (tokens, blocks of a token's heads)
+template <typename T, typename IN, typename W>
+__global__ void __launch_bounds__(WIDE_THREADS, 8) axes_rope_write_wide_kernel(const Args a, const int group_shift) {
     constexpr int N = 16 / sizeof(T);
-    static_assert(TOK == 1 || sizeof(T) == sizeof(IN), "several tokens at a time come in the cache's dtype");
-    extern __shared__ __align__(16) float turn_s[];
-    __shared__ long long row_s[TOK];                                 // the first kv head's key of the tokens' places, in rows of the cache (-1: nowhere)
     pdl_enter_small();
-    const int n0 = blockIdx.y * TOK, tid = threadIdx.x, half = a.rd / 2, group = 1 << group_shift;
-    uint4* piece_s = reinterpret_cast<uint4*>(turn_s + TOK * 2 * half);          // [TOK][2][threads]
-    const int head = (blockIdx.x * blockDim.x + tid) >> group_shift, t = tid & (group - 1);
-    const bool live = head < a.nq + 2 * a.nkv, value = head >= a.nq + a.nkv;
+    const int n = blockIdx.x, tid = threadIdx.x, half = a.rd / 2, group = 1 << group_shift;
+    const int head = (blockIdx.y * WIDE_THREADS + tid) >> group_shift, t = tid & (group - 1);
+    if (head >= a.nq + 2 * a.nkv) return;
+    const bool value = head >= a.nq + a.nkv;
     // this thread's two pieces
     const bool turned = t * N < half;
     const int i0 = turned ? t * N : a.rd + 2 * (t * N - half), i1 = turned ? i0 + half : i0 + N;
-    Two x[N / 2], y[N / 2];
-    if (live) {
-        const IN* src = (const IN*)a.qkv + (size_t)n0 * a.ld + (size_t)head * a.d;
-        if constexpr (TOK == 1) {
-            load_piece<IN, N>(a, src + i0, x);
-            load_piece<IN, N>(a, src + i1, y);
-        } else {
-#pragma unroll
-            for (int k = 0; k < TOK; ++k)
-                if (n0 + k < a.tokens)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"((uint32_t)__cvta_generic_to_shared(piece_s + (2 * k + h) * blockDim.x + tid)),
-                                     "l"(src + (size_t)k * a.ld + (h ? i1 : i0)));
-            asm volatile("cp.async.commit_group;\n" ::);
-        }
+    Two x[N / 2], y[N / 2], c[N / 2], s[N / 2];
+    const IN* src = (const IN*)a.qkv + (size_t)n * a.ld + (size_t)head * a.d;
+    uint4 raw_x, raw_y;                                              // (unpacked when they are used: fewer registers, more blocks)
+    if constexpr (sizeof(IN) == 2) raw_x = *reinterpret_cast<const uint4*>(src + i0), raw_y = *reinterpret_cast<const uint4*>(src + i1);
+    else {
+        load_piece<IN, N>(a, src + i0, x);
+        load_piece<IN, N>(a, src + i1, y);
     }
-    if (tid < TOK && n0 + tid < a.tokens) {
-        const int place = a.places[n0 + tid], at = place / a.page_size;
-        long long row = -1;
-        if (place >= 0 && at < a.bt_stride) {
-            const int page = a.block_table[(size_t)a.token_req[n0 + tid] * a.bt_stride + at];
-            if (page >= 0 && page < a.pages) row = (long long)page * 2 * a.nkv * a.page_size + place % a.page_size;
-        }
-        row_s[tid] = row;
+    const W* gain = value ? nullptr : (const W*)(head < a.nq ? a.q_gain : a.k_gain);
+    uint4 raw_gx, raw_gy;
+    if constexpr (sizeof(W) == 2 && N == 8)
+        if (gain) raw_gx = *reinterpret_cast<const uint4*>(gain + i0), raw_gy = *reinterpret_cast<const uint4*>(gain + i1);
+    if (!value && turned) load_turn<N>(a, n, i0, c, s);
+    T* dst = target<T>(a, n, head);
+    if constexpr (sizeof(IN) == 2) {
+        unpack<IN, N>(raw_x, x);
+        unpack<IN, N>(raw_y, y);
     }
-    // (a pair's threads go over the tokens: pairs first, as many tokens at a time as the block has threads for)
-    const int pairs = min((int)blockDim.x, max(half, 1)), at_once = (int)blockDim.x / pairs;
-    for (int e = tid; e < at_once * pairs; e += blockDim.x)
-    for (int j = e % pairs; j < half; j += pairs)
-    for (int k = e / pairs; k < TOK; k += at_once) {
-        const int axis = a.pair_axis[j];
-        const int pos = axis >= 0 && axis < a.axes && n0 + k < a.tokens ? a.positions[(size_t)axis * a.tokens + n0 + k] : -1;
-        const bool known = pos >= 0 && pos < a.table_rows;
-        turn_s[(2 * k) * half + j] = known ? a.cos_t[(size_t)pos * half + j] : __int_as_float(0x7fffffff);
-        turn_s[(2 * k + 1) * half + j] = known ? a.sin_t[(size_t)pos * half + j] : __int_as_float(0x7fffffff);
-    }
-    const W* gain = (const W*)(head < a.nq ? a.q_gain : a.k_gain);
-    const bool normed = live && !value && gain != nullptr;
-    Two gx[N / 2], gy[N / 2];
-    if (normed) {
-        load_gain<W, N>(gain + i0, gx);
-        load_gain<W, N>(gain + i1, gy);
-    }
-    if constexpr (TOK > 1) asm volatile("cp.async.wait_group 0;\n" ::);
-    __syncthreads();
-    const uint32_t mine = group == 32 ? 0xffffffffu : ((1u << group) - 1u) << (tid & 31 & ~(group - 1));
-#pragma unroll 1
-    for (int k = 0; k < TOK; ++k) {
-        if (!live || n0 + k >= a.tokens) break;
-        if constexpr (TOK > 1) {
-            unpack<T, N>(piece_s[(2 * k) * blockDim.x + tid], x);
-            unpack<T, N>(piece_s[(2 * k + 1) * blockDim.x + tid], y);
-        }
-        if (normed) {
-            Two squares = 0;
+    if (!value) {
+        if (gain) {
+            Two gx[N / 2], gy[N / 2], squares = 0;
+            if constexpr (sizeof(W) == 2 && N == 8) {
+                unpack<W, N>(raw_gx, gx);
+                unpack<W, N>(raw_gy, gy);
+            } else {
+                load_gain<W, N>(gain + i0, gx);
+                load_gain<W, N>(gain + i1, gy);
+            }
 #pragma unroll
             for (int i = 0; i < N / 2; ++i) squares = fma2(x[i], x[i], fma2(y[i], y[i], squares));
             const float2 both = apart(squares);
             float ssq = both.x + both.y;
+            const uint32_t mine = group == 32 ? 0xffffffffu : ((1u << group) - 1u) << (tid & 31 & ~(group - 1));
             for (int o = group >> 1; o > 0; o >>= 1) ssq += __shfl_xor_sync(mine, ssq, o);
             const float inv = rsqrtf(ssq / (float)a.d + a.eps);
             const Two inv2 = two(inv, inv);
 #pragma unroll
             for (int i = 0; i < N / 2; ++i) x[i] = mul2(mul2(x[i], inv2), gx[i]), y[i] = mul2(mul2(y[i], inv2), gy[i]);
         }
-        if (!value && turned) {
-            const ulonglong2 *cos_k = reinterpret_cast<const ulonglong2*>(turn_s + (2 * k) * half + i0), *sin_k = reinterpret_cast<const ulonglong2*>(turn_s + (2 * k + 1) * half + i0);
+        if (turned) {
             const Two minus = two(-1.f, -1.f);
 #pragma unroll
-            for (int i = 0; i < N / 4; ++i) {
-                const ulonglong2 c = cos_k[i], s = sin_k[i];
-                const Two p = x[2 * i], q = x[2 * i + 1];
-                x[2 * i] = fma2(mul2(y[2 * i], s.x), minus, mul2(p, c.x));
-                x[2 * i + 1] = fma2(mul2(y[2 * i + 1], s.y), minus, mul2(q, c.y));
-                y[2 * i] = fma2(p, s.x, mul2(y[2 * i], c.x));
-                y[2 * i + 1] = fma2(q, s.y, mul2(y[2 * i + 1], c.y));
+            for (int i = 0; i < N / 2; ++i) {
+                const Two was = x[i];
+                x[i] = fma2(mul2(y[i], s[i]), minus, mul2(was, c[i]));
+                y[i] = fma2(was, s[i], mul2(y[i], c[i]));
             }
         }
-        T* dst;
-        if (head < a.nq) dst = (T*)a.q_out + ((size_t)(n0 + k) * a.nq + head) * a.d;
-        else {
-            if (row_s[k] < 0) continue;
-            dst = (T*)a.kv + ((size_t)row_s[k] + (size_t)(head - a.nq) * a.page_size) * a.d;
-        }
-        store_piece<T, N>(dst + i0, x);
-        store_piece<T, N>(dst + i1, y);
     }
+    if (!dst) return;
+    store_piece<T, N>(dst + i0, x);
+    store_piece<T, N>(dst + i1, y);
 }
 
 }  // namespace axes
@@ -316,30 +318,16 @@ LILY_API int lily_axes_rope_write(const void* qkv, int in_dtype, int splits, siz
     const int bytes = act_dtype == kBF16 ? 2 : 4, piece = 16 / bytes, group = d / (2 * piece);
     int shift = 0;
     while (1 << shift < group) ++shift;
-    const uintptr_t where = (uintptr_t)qkv | (uintptr_t)kv | (uintptr_t)q_out | (uintptr_t)q_gain | (uintptr_t)k_gain;
-    // whole pieces of 16 bytes on every side; else, and for heads that are no power of two of pieces, a warp a head 
+    const uintptr_t where = (uintptr_t)qkv | (uintptr_t)kv | (uintptr_t)q_out | (uintptr_t)q_gain | (uintptr_t)k_gain |
+                            (uintptr_t)cos_t | (uintptr_t)sin_t | (uintptr_t)pair_axis;
+    // whole pieces of 16 bytes on every side; else, and for heads that are no power of two of pieces, a warp a head
     const bool wide = d % (2 * piece) == 0 && 1 << shift == group && group <= 32 && rd % (2 * piece) == 0 && ld % piece == 0 &&
-                      (in_dtype == act_dtype || ld % 4 == 0) && (size_t)stride % 4 == 0 && where % 16 == 0 && tokens <= 65535;
-    // the threads of a token's heads in as few equal blocks as take them
-    const int all = (nq + 2 * nkv) << shift, blocks = (all + axes::WIDE_THREADS - 1) / axes::WIDE_THREADS, threads = ((all + blocks - 1) / blocks + 31) / 32 * 32;
-    // four tokens a block once those blocks fill the device
-    const bool many = wide && splits == 1 && in_dtype == act_dtype && (long)blocks * ((tokens + axes::TOKENS - 1) / axes::TOKENS) >= sm_count();
-    const size_t turn = (size_t)(many ? axes::TOKENS : 1) * rd * sizeof(float) + (many ? (size_t)threads * axes::TOKENS * 32 : 0);
-    const dim3 grid = many ? dim3(blocks, (tokens + axes::TOKENS - 1) / axes::TOKENS) : wide ? dim3(blocks, tokens) : dim3(tokens, (nq + 2 * nkv + 3) / 4);
-#define LAUNCH(T, IN, W)                                                                                                                                              \
-    do {                                                                                                                                                              \
-        constexpr int TOK = sizeof(T) == sizeof(IN) ? axes::TOKENS : 1;                                                                                               \
-        if (many) {                                                                                                                                                   \
-            auto kern = axes::axes_rope_write_wide_kernel<T, IN, W, TOK>;                                                                                             \
-            static bool configured = false;                                                                                                                           \
-            if (!configured) {                                                                                                                                        \
-                const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024);                                             \
-                LILY_REQUIRE(e == cudaSuccess, "axes_rope_write: cannot get %d bytes of shared memory: %s", 96 * 1024, cudaGetErrorString(e));                        \
-                configured = true;                                                                                                                                    \
-            }                                                                                                                                                         \
-            launch_pdl(kern, grid, dim3(threads), turn, stream, a, shift);                                                                                            \
-        } else if (wide) launch_pdl(axes::axes_rope_write_wide_kernel<T, IN, W, 1>, grid, dim3(threads), turn, stream, a, shift);                                     \
-        else launch_pdl(axes::axes_rope_write_kernel<T, IN, W>, grid, dim3(128), 0, stream, a);                                                                       \
+                      (in_dtype == act_dtype || ld % 4 == 0) && (size_t)stride % 4 == 0 && where % 16 == 0;
+    const dim3 grid = wide ? dim3(tokens, (unsigned)((((nq + 2 * nkv) << shift) + axes::WIDE_THREADS - 1) / axes::WIDE_THREADS)) : dim3(tokens, (nq + 2 * nkv + 3) / 4);
+#define LAUNCH(T, IN, W)                                                                                                        \
+    do {                                                                                                                        \
+        if (wide) launch_pdl(axes::axes_rope_write_wide_kernel<T, IN, W>, grid, dim3(axes::WIDE_THREADS), 0, stream, a, shift); \
+        else launch_pdl(axes::axes_rope_write_kernel<T, IN, W>, grid, dim3(128), 0, stream, a);                                 \
     } while (0)
     const bool ib = in_dtype == kBF16, gb = gain_dtype == kBF16;
     if (act_dtype == kF32) LAUNCH(float, float, float);

@@ -208,12 +208,16 @@ def library():
 launches = {"count": 0}          # kernels of this package launched so far (bench.py reports the difference)
 
 
+_entries = {}                    # entry points by name, as they are first called
+
+
 def _call(name: str, *args) -> None:
-    lib = library()
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(library(), name)
     launches["count"] += 1
-    rc = getattr(lib, name)(*args)
-    if rc != 0:
-        raise KernelError(f"{name}: {lib.lily_last_error().decode(errors='replace')}")
+    if fn(*args) != 0:
+        raise KernelError(f"{name}: {library().lily_last_error().decode(errors='replace')}")
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -1218,16 +1222,22 @@ def pair_axes(sections: Sequence[int], device, in_turn: bool = False) -> torch.T
     return torch.tensor(axes, dtype=torch.int32, device=device)
 
 
-def _layer_and_weights(what: str, kv_layer: torch.Tensor, weights: torch.Tensor, nkv: int, page_size: int, d: int) -> None:
-    cache_layer_fits(kv_layer, nkv, page_size, d, d)
-    if weights.dtype != torch.float32 or tuple(weights.shape) != (kv_layer.shape[0], nkv, page_size):
-        raise KernelError(f"{what}: weights are float32 [{kv_layer.shape[0]}, {nkv}, {page_size}], got {weights.dtype} {tuple(weights.shape)}")
+def _layer_and_weights(what: str, kv_layer: torch.Tensor, weights: torch.Tensor, nkv: int, page_size: int, d: int) -> int:
+    """The pages of a cache layer that fits, with weights beside it."""
+    shape = kv_layer.shape
+    if shape[1:] != (2, nkv, page_size, d):
+        cache_layer_fits(kv_layer, nkv, page_size, d, d)
+    if weights.dtype is not torch.float32 or weights.shape != (shape[0], nkv, page_size):
+        raise KernelError(f"{what}: weights are float32 [{shape[0]}, {nkv}, {page_size}], got {weights.dtype} {tuple(weights.shape)}")
+    return shape[0]
 
 
 def _table(what: str, table: torch.Tensor, requests: int, name: str = "block_table") -> int:
-    if table.dim() != 2 or table.shape[0] != requests or table.shape[1] < 1:
-        raise KernelError(f"{what}: {name} is int32 [{requests}, pages], got {tuple(table.shape)}")
-    return table.shape[1]
+    """The width of a block table of so many requests."""
+    shape = table.shape
+    if len(shape) != 2 or shape[0] != requests or shape[1] < 1 or table.dtype is not torch.int32:
+        raise KernelError(f"{what}: {name} is int32 [{requests}, pages], got {table.dtype} {tuple(shape)}")
+    return shape[1]
 
 
 def axes_rope_write(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_gain: Optional[torch.Tensor], eps: float, cos: torch.Tensor,
@@ -1241,29 +1251,37 @@ def axes_rope_write(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_gain: O
     (nq + 2 nkv) d] in the cache's dtype or float32 partial sums [splits, tokens, ...], its rows ``row`` numbers apart.  A position outside the
     tables gives NaN; a place outside the block table is not written."""
     _dev(qkv, q_gain, k_gain, cos, sin, positions, pair_axis, places, token_req, block_table, kv_layer, q_out)
-    n = qkv.shape[-2]
     ld = int(row or (nq + 2 * nkv) * d)
-    splits, stride = _summed(qkv, n, ld, "axes_rope_write qkv")
-    if qkv.dtype not in (kv_layer.dtype, torch.float32):
-        raise KernelError(f"axes_rope_write: cache dtype {kv_layer.dtype} differs from activations {qkv.dtype}")
-    cache_layer_fits(kv_layer, nkv, page_size, d, d)
-    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.dim() != 2 or cos.shape[1] != rotary_dim // 2 or sin.shape != cos.shape:
+    shape, pages, dtype, half = qkv.shape, kv_layer.shape, kv_layer.dtype, rotary_dim // 2
+    n = shape[-2]
+    splits, stride = (1, 0) if len(shape) == 2 and shape[1] == ld else _summed(qkv, n, ld, "axes_rope_write qkv")
+    if qkv.dtype is not dtype and qkv.dtype is not torch.float32:
+        raise KernelError(f"axes_rope_write: cache dtype {dtype} differs from activations {qkv.dtype}")
+    if pages[1:] != (2, nkv, page_size, d):
+        cache_layer_fits(kv_layer, nkv, page_size, d, d)
+    rows = cos.shape
+    if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or len(rows) != 2 or rows[1] != half or sin.shape != rows:
         raise KernelError("axes_rope_write: rotation tables are float32 [positions, rotary_dim / 2]")
-    if positions.dim() != 2 or positions.shape[1] != n or pair_axis.numel() != rotary_dim // 2:
-        raise KernelError(f"axes_rope_write: positions are [axes, {n}] and there is an axis for each of the {rotary_dim // 2} pairs; got {tuple(positions.shape)} "
-                          f"and {pair_axis.numel()}")
-    if places.numel() != n or token_req.numel() != n or block_table.dim() != 2 or block_table.shape[1] < 1:
+    axes, width = positions.shape, block_table.shape
+    if len(axes) != 2 or axes[1] != n or pair_axis.numel() != half:
+        raise KernelError(f"axes_rope_write: positions are [axes, {n}] and there is an axis for each of the {half} pairs; got {tuple(axes)} and {pair_axis.numel()}")
+    if places.numel() != n or token_req.numel() != n or len(width) != 2 or width[1] < 1:
         raise KernelError(f"axes_rope_write: {n} tokens have a place and a request each")
-    if (q_gain is None) != (k_gain is None) or (q_gain is not None and (q_gain.dtype != k_gain.dtype or q_gain.numel() != d or k_gain.numel() != d)):
-        raise KernelError("axes_rope_write: q and k gains come together, with one dtype and head_dim numbers each")
+    for t, name in ((positions, "positions"), (pair_axis, "pair_axis"), (places, "places"), (token_req, "token_req"), (block_table, "block_table")):
+        if t.dtype is not torch.int32:
+            raise KernelError(f"{name} must be int32, got {t.dtype}")
+    gains = (None, None, _F32)
+    if q_gain is not None or k_gain is not None:
+        if q_gain is None or k_gain is None or q_gain.dtype is not k_gain.dtype or q_gain.numel() != d or k_gain.numel() != d:
+            raise KernelError("axes_rope_write: q and k gains come together, with one dtype and head_dim numbers each")
+        gains = (q_gain.data_ptr(), k_gain.data_ptr(), _dt(q_gain))
     if q_out is None:
-        q_out = torch.empty((n, nq * d), dtype=kv_layer.dtype, device=qkv.device)
-    elif q_out.dtype != kv_layer.dtype or q_out.numel() != n * nq * d:
+        q_out = kv_layer.new_empty((n, nq * d))
+    elif q_out.dtype is not dtype or q_out.numel() != n * nq * d:
         raise KernelError("axes_rope_write: q_out is [tokens, nq * d] in the cache's dtype")
-    _call("lily_axes_rope_write", _p(qkv), _dt(qkv), splits, stride, ld, _p(q_gain), _p(k_gain), _dt(q_gain) if q_gain is not None else _F32,
-          float(eps), _p(cos), _p(sin), cos.shape[0], _i32(positions, "positions"), _i32(pair_axis, "pair_axis"), positions.shape[0], n,
-          _i32(places, "places"), _i32(token_req, "token_req"), _i32(block_table, "block_table"), block_table.shape[1], _p(kv_layer),
-          kv_layer.shape[0], _p(q_out), _dt(kv_layer), nq, nkv, d, rotary_dim, page_size, _stream())
+    _call("lily_axes_rope_write", qkv.data_ptr(), _dt(qkv), splits, stride, ld, *gains, eps, cos.data_ptr(), sin.data_ptr(), rows[0], positions.data_ptr(),
+          pair_axis.data_ptr(), axes[0], n, places.data_ptr(), token_req.data_ptr(), block_table.data_ptr(), width[1], kv_layer.data_ptr(), pages[0],
+          q_out.data_ptr(), _dt(kv_layer), nq, nkv, d, rotary_dim, page_size, _stream())
     return q_out
 
 
@@ -1282,47 +1300,57 @@ def attention_decode_weighed(q: torch.Tensor, kv_layer: torch.Tensor, weights: t
     step's own, ``seq_lens - 1``) is set to them.  A request without places has a row of zeros.  A page belongs to one request.
     ``scratch``: float32, ``decode_weighed_scratch_floats`` of them (allocated where not given)."""
     _dev(q, kv_layer, weights, block_table, seq_lens, out, scratch)
-    requests = q.shape[0] if q.dim() else 0
-    if q.dtype != kv_layer.dtype or q.numel() != requests * nq * d:
-        raise KernelError(f"attention_decode_weighed: queries are [requests, {nq * d}] in the cache's dtype, got {q.dtype} {tuple(q.shape)}")
-    _layer_and_weights("attention_decode_weighed", kv_layer, weights, nkv, page_size, d)
+    shape, dtype = q.shape, q.dtype
+    requests = shape[0] if shape else 0
+    if dtype is not kv_layer.dtype or q.numel() != requests * nq * d:
+        raise KernelError(f"attention_decode_weighed: queries are [requests, {nq * d}] in the cache's dtype, got {dtype} {tuple(shape)}")
+    pages = _layer_and_weights("attention_decode_weighed", kv_layer, weights, nkv, page_size, d)
     width = _table("attention_decode_weighed", block_table, requests)
-    if seq_lens.numel() != requests or not 0 <= max_seq_len <= width * page_size:
-        raise KernelError(f"attention_decode_weighed: {requests} lengths of up to {max_seq_len} places; the block table holds {width * page_size}")
+    if seq_lens.numel() != requests or seq_lens.dtype is not torch.int32 or not 0 <= max_seq_len <= width * page_size:
+        raise KernelError(f"attention_decode_weighed: {requests} int32 lengths of up to {max_seq_len} places; the block table holds {width * page_size}")
     if out is None:
         out = torch.empty_like(q)
-    elif out.dtype != q.dtype or out.numel() != q.numel():
+    elif out.dtype is not dtype or out.numel() != q.numel():
         raise KernelError("attention_decode_weighed: out has the shape and dtype of q")
-    need = decode_weighed_scratch_floats(requests, nq, nkv, d, max_seq_len, page_size, q.dtype)
+    need = decode_weighed_scratch_floats(requests, nq, nkv, d, max_seq_len, page_size, dtype)
     if scratch is None:
-        scratch = torch.empty((need,), dtype=torch.float32, device=q.device)
-    elif scratch.dtype != torch.float32 or scratch.numel() < need:
+        scratch = weights.new_empty((need,))
+    elif scratch.dtype is not torch.float32 or scratch.numel() < need:
         raise KernelError(f"attention_decode_weighed: scratch of {need} float32 needed")
-    _call("lily_attention_decode_weighed", _p(q), _p(kv_layer), _p(weights), _p(out), _i32(block_table, "block_table"), width,
-          _i32(seq_lens, "seq_lens"), _p(scratch), requests, int(max_seq_len), nq, nkv, d, page_size, kv_layer.shape[0], float(scale), _dt(q), DECODE_POLLS,
-          _stream())
+    _call("lily_attention_decode_weighed", q.data_ptr(), kv_layer.data_ptr(), weights.data_ptr(), out.data_ptr(), block_table.data_ptr(), width,
+          seq_lens.data_ptr(), scratch.data_ptr(), requests, max_seq_len, nq, nkv, d, page_size, pages, scale, _dt(q), DECODE_POLLS, _stream())
     return out
 
 
-def _heard(new_lens: Sequence[int], observe: Optional[int]) -> int:
-    return max((min(int(n), int(observe)) if observe else int(n) for n in new_lens), default=0)
+@dataclass(frozen=True)
+class _Portions:
+    """What ``attention_key_weights`` works out from the lengths of its portions."""
+
+    tensor_cores: bool          # the tcgen05 kernels take them
+    floats: int                 # float32 scratch
+    tokens: int
+    longest: int                # places of the longest request
+    heard: bool                 # somebody is
+    prefix: object              # the lengths as C arrays
+    new: object
 
 
 @functools.lru_cache(maxsize=64)
 def _portions(h_prefix_lens: Tuple[int, ...], h_new_lens: Tuple[int, ...], nq: int, nkv: int, d: int, page_size: int, scale: float, dtype: torch.dtype,
-              observe: int):
-    """Of portions of these lengths: (whether the tcgen05 kernels take them, float32 scratch, the lengths as C arrays)."""
+              observe: int) -> _Portions:
+    if nkv < 1 or nq % nkv or any(n < 0 for n in h_prefix_lens + h_new_lens):
+        raise KernelError(f"attention_key_weights: portions of {h_new_lens} behind {h_prefix_lens}, {nq} query heads over {nkv} kv heads")
     lib, n = library(), len(h_new_lens)
     prefix, new = (ctypes.c_int * n)(*h_prefix_lens), (ctypes.c_int * n)(*h_new_lens)
-    if dtype == torch.bfloat16 and lib.lily_key_weights_tc_takes(nq, nkv, d, page_size, scale):
-        return True, int(lib.lily_key_weights_tc_floats(n, prefix, new, observe, nq, nkv)), prefix, new
-    return False, int(lib.lily_key_weights_floats(n, prefix, new, observe, nq, nkv)), prefix, new
+    tensor_cores = dtype == torch.bfloat16 and bool(lib.lily_key_weights_tc_takes(nq, nkv, d, page_size, scale))
+    floats = (lib.lily_key_weights_tc_floats if tensor_cores else lib.lily_key_weights_floats)(n, prefix, new, observe, nq, nkv)
+    return _Portions(tensor_cores, int(floats), sum(h_new_lens), max((a + b for a, b in zip(h_prefix_lens, h_new_lens)), default=0), any(h_new_lens), prefix, new)
 
 
 def key_weights_scratch_floats(h_prefix_lens: Sequence[int], h_new_lens: Sequence[int], nq: int, nkv: int, d: int, page_size: int, scale: float,
                                dtype: torch.dtype, observe: Optional[int] = None) -> int:
     """Float32 scratch that ``attention_key_weights`` needs for portions of these lengths."""
-    return _portions(tuple(h_prefix_lens), tuple(h_new_lens), nq, nkv, d, page_size, float(scale), dtype, int(observe or 0))[1]
+    return _portions(tuple(h_prefix_lens), tuple(h_new_lens), nq, nkv, d, page_size, scale, dtype, observe or 0).floats
 
 
 def key_weights_status() -> int:
@@ -1340,35 +1368,32 @@ def attention_key_weights(q: torch.Tensor, kv_layer: torch.Tensor, weights: torc
     given).  The portion's own places are set, also where nobody who is heard sees them.  ``h_prefix_lens``, ``h_new_lens``:
     the lengths on the host.  ``scratch``: float32, ``key_weights_scratch_floats`` of them (allocated where not given)."""
     _dev(q, kv_layer, weights, block_table, cu_seqlens, prefix_lens, scratch)
-    requests = len(h_new_lens)
-    if q.dtype != kv_layer.dtype or q.dim() != 2 or q.shape[1] != nq * d or q.shape[0] < sum(h_new_lens):
-        raise KernelError(f"attention_key_weights: queries are [tokens, {nq * d}] in the cache's dtype, got {q.dtype} {tuple(q.shape)}")
-    _layer_and_weights("attention_key_weights", kv_layer, weights, nkv, page_size, d)
-    width = _table("attention_key_weights", block_table, requests)
-    if len(h_prefix_lens) != requests or cu_seqlens.numel() != requests + 1 or prefix_lens.numel() != requests:
-        raise KernelError(f"attention_key_weights: {requests} portions have a prefix each and {requests + 1} offsets")
+    requests, shape, dtype = len(h_new_lens), q.shape, q.dtype
     if observe is not None and observe < 1:
         raise KernelError(f"attention_key_weights: the last {observe} tokens cannot be heard")
-    longest = max((int(p) + int(n) for p, n in zip(h_prefix_lens, h_new_lens)), default=0)
-    if longest > width * page_size or any(n < 0 or p < 0 for p, n in zip(h_prefix_lens, h_new_lens)):
-        raise KernelError(f"attention_key_weights: {longest} places; the block table holds {width * page_size}")
-    heard = _heard(h_new_lens, observe)
-    if heard == 0:
+    if (len(h_prefix_lens) != requests or cu_seqlens.numel() != requests + 1 or prefix_lens.numel() != requests or cu_seqlens.dtype is not torch.int32
+            or prefix_lens.dtype is not torch.int32):
+        raise KernelError(f"attention_key_weights: {requests} portions have a prefix each and {requests + 1} offsets, int32")
+    plan = _portions(tuple(h_prefix_lens), tuple(h_new_lens), nq, nkv, d, page_size, scale, dtype, observe or 0)
+    if dtype is not kv_layer.dtype or len(shape) != 2 or shape[1] != nq * d or shape[0] < plan.tokens:
+        raise KernelError(f"attention_key_weights: queries are [tokens, {nq * d}] in the cache's dtype, got {dtype} {tuple(shape)} for {plan.tokens} tokens")
+    pages = _layer_and_weights("attention_key_weights", kv_layer, weights, nkv, page_size, d)
+    width = _table("attention_key_weights", block_table, requests)
+    if plan.longest > width * page_size:
+        raise KernelError(f"attention_key_weights: {plan.longest} places; the block table holds {width * page_size}")
+    if not plan.heard:
         return
-    tensor_cores, need, prefix, new = _portions(tuple(h_prefix_lens), tuple(h_new_lens), nq, nkv, d, page_size, float(scale), q.dtype, int(observe or 0))
     if scratch is None:
-        scratch = torch.empty((need,), dtype=torch.float32, device=q.device)
-    elif scratch.dtype != torch.float32 or scratch.numel() < need:
-        raise KernelError(f"attention_key_weights: scratch of {need} float32 needed")
-    _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens")
-    if tensor_cores:
-        _call("lily_key_weights_tc", _p(q), q.shape[0], _p(kv_layer), kv_layer.shape[0], _p(weights), _i32(block_table, "block_table"), width, _p(scratch),
-              requests, prefix, new, int(observe or 0), nq, nkv, d, page_size, float(scale), _stream())
-        launches["count"] += 2                                   # rows, their joining, columns
-        return
-    _call("lily_key_weights", _p(q), _p(kv_layer), _p(weights), _i32(block_table, "block_table"), width, _p(scratch), requests, prefix, new,
-          int(observe or 0), nq, nkv, d, page_size, float(scale), _dt(q), _stream())
-    launches["count"] += 2                                       # scores, the rows' lse, columns
+        scratch = weights.new_empty((plan.floats,))
+    elif scratch.dtype is not torch.float32 or scratch.numel() < plan.floats:
+        raise KernelError(f"attention_key_weights: scratch of {plan.floats} float32 needed")
+    if plan.tensor_cores:
+        _call("lily_key_weights_tc", q.data_ptr(), shape[0], kv_layer.data_ptr(), pages, weights.data_ptr(), block_table.data_ptr(), width, scratch.data_ptr(),
+              requests, plan.prefix, plan.new, observe or 0, nq, nkv, d, page_size, scale, _stream())
+    else:
+        _call("lily_key_weights", q.data_ptr(), kv_layer.data_ptr(), weights.data_ptr(), block_table.data_ptr(), width, scratch.data_ptr(), requests, plan.prefix,
+              plan.new, observe or 0, nq, nkv, d, page_size, scale, _dt(q), _stream())
+    launches["count"] += 2                                       # rows or scores, what joins them, columns
 
 
 def select_keys(weights: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, max_length: int, keep: int, first: int = 0,
@@ -1378,20 +1403,21 @@ def select_keys(weights: torch.Tensor, block_table: torch.Tensor, lengths: torch
     lower place; of a shorter one all.  ``weights`` float32 [layers, pages, kv_heads, page_size], or of one layer without the first axis; a
     NaN counts as the heaviest.  ``max_length``: no request has more places."""
     _dev(weights, block_table, lengths)
-    if weights.dim() == 3:
-        return select_keys(weights[None], block_table, lengths, max_length, keep, first, recent)
-    if weights.dtype != torch.float32 or weights.dim() != 4:
-        raise KernelError(f"select_keys: weights are float32 [layers, pages, kv_heads, page_size], got {weights.dtype} {tuple(weights.shape)}")
-    layers, pages, nkv, page_size = weights.shape
+    shape = weights.shape
+    if len(shape) == 3:
+        shape = (1, *shape)
+    if weights.dtype is not torch.float32 or len(shape) != 4:
+        raise KernelError(f"select_keys: weights are float32 [layers, pages, kv_heads, page_size], got {weights.dtype} {tuple(shape)}")
+    layers, pages, nkv, page_size = shape
     requests = lengths.numel()
     width = _table("select_keys", block_table, requests)
     if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
         raise KernelError(f"select_keys: the first {first} and the last {recent} places do not fit into {keep}")
-    if not 0 <= max_length <= width * page_size:
-        raise KernelError(f"select_keys: {max_length} places; the block table holds {width * page_size}")
-    kept = torch.empty((layers, requests, nkv, keep), dtype=torch.int32, device=weights.device)
-    _call("lily_select_keys", _p(weights), _i32(block_table, "block_table"), width, _i32(lengths, "lengths"), _p(kept), layers, pages, requests, nkv,
-          page_size, int(max_length), int(keep), int(first), int(recent), _stream())
+    if lengths.dtype is not torch.int32 or not 0 <= max_length <= width * page_size:
+        raise KernelError(f"select_keys: int32 lengths of up to {max_length} places; the block table holds {width * page_size}")
+    kept = lengths.new_empty((layers, requests, nkv, keep))
+    _call("lily_select_keys", weights.data_ptr(), block_table.data_ptr(), width, lengths.data_ptr(), kept.data_ptr(), layers, pages, requests, nkv, page_size,
+          max_length, keep, first, recent, _stream())
     return kept
 
 
@@ -1402,23 +1428,25 @@ def move_keys(kv: torch.Tensor, weights: Optional[torch.Tensor], block_table: to
     (or None), or those of one layer without the first axis.  In place, or, with ``to_table`` int32 [requests, pages], into those pages (a fork of the request; none of them
     may be a page of ``block_table``).  Places outside their tables, and what lies behind the last kept place, stay as they are."""
     _dev(kv, weights, block_table, kept, to_table)
-    if kv.dim() == 5:
-        return move_keys(kv[None], None if weights is None else weights[None], block_table, kept, to_table)
-    if kv.dim() != 6 or kv.shape[2] != 2 or kept.dim() != 4 or kept.dtype != torch.int32:
-        raise KernelError(f"move_keys: a cache [layers, pages, 2, kv_heads, page_size, d] and int32 places [layers, requests, kv_heads, keep], got {tuple(kv.shape)}, "
-                          f"{kept.dtype} {tuple(kept.shape)}")
-    layers, pages, _, nkv, page_size, d = kv.shape
-    requests, keep = kept.shape[1], kept.shape[3]
-    if kept.shape[0] != layers or kept.shape[2] != nkv:
-        raise KernelError(f"move_keys: places of {kept.shape[0]} layers and {kept.shape[2]} kv heads for a cache of {layers} and {nkv}")
-    if weights is not None and (weights.dtype != torch.float32 or tuple(weights.shape) != (layers, pages, nkv, page_size)):
-        raise KernelError(f"move_keys: weights are float32 [{layers}, {pages}, {nkv}, {page_size}], got {weights.dtype} {tuple(weights.shape)}")
-    _dt(kv)
+    shape, places = kv.shape, kept.shape
+    beside = None if weights is None else weights.shape
+    if len(shape) == 5:
+        shape, beside = (1, *shape), None if beside is None else (1, *beside)
+    if len(shape) != 6 or shape[2] != 2 or len(places) != 4 or kept.dtype is not torch.int32:
+        raise KernelError(f"move_keys: a cache [layers, pages, 2, kv_heads, page_size, d] and int32 places [layers, requests, kv_heads, keep], got {tuple(shape)}, "
+                          f"{kept.dtype} {tuple(places)}")
+    layers, pages, _, nkv, page_size, d = shape
+    requests, keep = places[1], places[3]
+    if places[0] != layers or places[2] != nkv:
+        raise KernelError(f"move_keys: places of {places[0]} layers and {places[2]} kv heads for a cache of {layers} and {nkv}")
+    if weights is not None and (weights.dtype is not torch.float32 or beside != (layers, pages, nkv, page_size)):
+        raise KernelError(f"move_keys: weights are float32 [{layers}, {pages}, {nkv}, {page_size}], got {weights.dtype} {tuple(beside)}")
+    item = 4 if _dt(kv) == _F32 else 2
     width = _table("move_keys", block_table, requests)
-    to = block_table if to_table is None else to_table
-    _call("lily_move_keys", _p(kv), _p(weights), _i32(block_table, "block_table"), width, _i32(to, "to_table"), _table("move_keys", to, requests, "to_table"),
-          _p(kept), layers, pages, requests, nkv, page_size, d * kv.element_size(), keep,
-          int(to_table is None or to_table.data_ptr() == block_table.data_ptr()), _stream())
+    table = block_table.data_ptr()
+    to, to_width = (table, width) if to_table is None else (to_table.data_ptr(), _table("move_keys", to_table, requests, "to_table"))
+    _call("lily_move_keys", kv.data_ptr(), None if weights is None else weights.data_ptr(), table, width, to, to_width, kept.data_ptr(), layers, pages, requests,
+          nkv, page_size, d * item, keep, int(to == table), _stream())
 
 
 # ------------------------------------------------------------------------------ joining sublayers
