@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(SIMT_THREADS) decode_weighed_simt_kernel(const
 
 // ---- the ranges joined: outputs, then the places' weights ------------------------------------------
 constexpr int JOIN_THREADS = 256;
-constexpr int JOIN_KEYS = 1024;            // places a block adds up
+constexpr int JOIN_KEYS = 4 * JOIN_THREADS;      // places a block adds up
 
 template <typename T>
 __global__ void __launch_bounds__(JOIN_THREADS) decode_weighed_join_kernel(const DecodeArgs a) {
@@ -142,24 +142,60 @@ __global__ void __launch_bounds__(JOIN_THREADS) decode_weighed_join_kernel(const
     }
     __syncthreads();
     if (blockIdx.z == 0) {
-        for (int i = tid; i < group * d; i += JOIN_THREADS) {
+        const bool vec = (d & 3) == 0;
+        const int step = vec ? 4 : 1;
+        for (int i = tid * step; i < group * d; i += JOIN_THREADS * step) {
             const int h = i / d, col = i % d;
-            const size_t at = ((size_t)req * a.nq + kvh * group + h) * a.splits;
-            float o = 0.f;
-            if (n > 0)
+            const size_t row = (size_t)req * a.nq + kvh * group + h, at = row * a.splits;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (n > 0) {
+#pragma unroll 4
                 for (int s = 0; s < a.splits; ++s) {
-                    const float m = a.part_ml[(at + s) * 2];
-                    if (m == -INFINITY && a.part_ml[(at + s) * 2 + 1] == 0.f) continue;          // a range without keys
-                    o = fmaf(a.part_o[(at + s) * d + col], exp2f(m - sm[h]), o);
+                    const float m = a.part_ml[(at + s) * 2], l = a.part_ml[(at + s) * 2 + 1];
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                    const float* part = a.part_o + (at + s) * d + col;
+                    if (vec) v = *reinterpret_cast<const float4*>(part);
+                    else v.x = *part;
+                    if (m == -INFINITY && l == 0.f) continue;          // a range without keys
+                    const float f = exp2f(m - sm[h]);
+                    o.x = fmaf(v.x, f, o.x), o.y = fmaf(v.y, f, o.y), o.z = fmaf(v.z, f, o.z), o.w = fmaf(v.w, f, o.w);
                 }
-            ((T*)a.out)[((size_t)req * a.nq + kvh * group + h) * d + col] = from_float<T>(o);
+            }
+            T* to = (T*)a.out + row * d + col;
+            to[0] = from_float<T>(o.x);
+            if (vec) to[1] = from_float<T>(o.y), to[2] = from_float<T>(o.z), to[3] = from_float<T>(o.w);
         }
         return;
     }
+    // four neighbouring places a thread where they lie in one page
     const int* table = a.block_table + (size_t)req * a.bt_stride;
     const float* scores = a.scores + ((size_t)req * a.nq + kvh * group) * a.score_stride;
-    for (int j = beg + tid; j < min(n, beg + JOIN_KEYS); j += JOIN_THREADS) {
-        float* w = a.weights + ((size_t)table[j / a.page_size] * a.nkv + kvh) * a.page_size + j % a.page_size;
+    const int end = min(n, beg + JOIN_KEYS);
+    auto weights_at = [&](int j) { return a.weights + ((size_t)table[j / a.page_size] * a.nkv + kvh) * a.page_size + j % a.page_size; };
+    if ((a.page_size & 3) == 0 && ((uintptr_t)a.weights & 15) == 0) {
+        const int j = beg + 4 * tid;
+        if (j >= end) return;
+        float* at = weights_at(j);
+        float4 w = *reinterpret_cast<const float4*>(at);
+        w = make_float4(j == n - 1 ? 0.f : w.x, j + 1 == n - 1 ? 0.f : w.y, j + 2 == n - 1 ? 0.f : w.z, j + 3 == n - 1 ? 0.f : w.w);
+#pragma unroll 4
+        for (int h = 0; h < group; ++h) {
+            const float4 t = *reinterpret_cast<const float4*>(scores + (size_t)h * a.score_stride + j);
+            w.x += exp2f(t.x - sm[h]);
+            w.y += exp2f(t.y - sm[h]);
+            w.z += exp2f(t.z - sm[h]);
+            w.w += exp2f(t.w - sm[h]);
+        }
+        if (j + 4 <= n) *reinterpret_cast<float4*>(at) = w;
+        else {
+            at[0] = w.x;
+            if (j + 1 < n) at[1] = w.y;
+            if (j + 2 < n) at[2] = w.z;
+        }
+        return;
+    }
+    for (int j = beg + tid; j < end; j += JOIN_THREADS) {
+        float* w = weights_at(j);
         float sum = j < n - 1 ? *w : 0.f;
         for (int h = 0; h < group; ++h) sum += exp2f(scores[(size_t)h * a.score_stride + j] - sm[h]);
         *w = sum;
@@ -412,6 +448,20 @@ __global__ void __launch_bounds__(THREADS, 3) decode_weighed_mma_kernel(const De
         __syncthreads();
     }
 
+    // The weights of this thread's first four places and their scores are asked for here, ahead of the joining.
+    const float* scores = a.scores + ((size_t)req * a.nq + head0) * a.score_stride;
+    const int newest = places_of(a, req) - 1;
+    auto weights_at = [&](int j) { return a.weights + (((size_t)table[j >> page_shift] * a.nkv + kvh) << page_shift) + (j & page_mask); };
+    float* first_at = nullptr;
+    float4 first_w = make_float4(0.f, 0.f, 0.f, 0.f), first_s[4] = {first_w, first_w, first_w, first_w};
+    if ((CLUSTER || a.splits == 1) && kbeg + 4 * tid < kend) {
+        first_at = weights_at(kbeg + 4 * tid);
+        first_w = *reinterpret_cast<const float4*>(first_at);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (r < nrows) first_s[r] = *reinterpret_cast<const float4*>(scores + (size_t)r * a.score_stride + kbeg + 4 * tid);
+    }
+
     // ---- the four warps' results joined --------------------------------------------------------------
     float* mo = reinterpret_cast<float*>(k_s);                      // [4 warps][16 rows][D]
     float* mml = mo + 4 * 16 * D;                                   // [4 warps][16 rows][2]
@@ -492,26 +542,31 @@ __global__ void __launch_bounds__(THREADS, 3) decode_weighed_mma_kernel(const De
             *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)req * a.nq + head0 + r) * D + col) =
                 make_uint2(tc5::pack2(acc.x, acc.y), tc5::pack2(acc.z, acc.w));
         }
-    // ---- what the places of this range were given ----------------------------------------------------
-    const float* scores = a.scores + ((size_t)req * a.nq + head0) * a.score_stride;
-    const int newest = places_of(a, req) - 1;
-    for (int j0 = kbeg + tid; j0 < kend; j0 += 4 * THREADS) {
-        float w[4];
-        float* at[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int j = j0 + u * THREADS;
-            at[u] = j < kend ? a.weights + (((size_t)table[j >> page_shift] * a.nkv + kvh) << page_shift) + (j & page_mask) : nullptr;
-            w[u] = j < kend && j != newest ? *at[u] : 0.f;
+    // ---- what the places of this range were given: four neighbouring places a thread, which lie in one page ------------
+    for (int j = kbeg + 4 * tid, turn = 0; j < kend; j += 4 * THREADS, ++turn) {
+        float* at = first_at;
+        float4 w = first_w;
+        if (turn > 0) {
+            at = weights_at(j);
+            w = *reinterpret_cast<const float4*>(at);
         }
+        // the newest place is set
+        w = make_float4(j == newest ? 0.f : w.x, j + 1 == newest ? 0.f : w.y, j + 2 == newest ? 0.f : w.z, j + 3 == newest ? 0.f : w.w);
         for (int r = 0; r < nrows; ++r) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (j0 + u * THREADS < kend) w[u] += exp2f(scores[(size_t)r * a.score_stride + j0 + u * THREADS] - lse_s[r]);
+            const float4 t = turn == 0 && r < 4 ? (r == 0 ? first_s[0] : r == 1 ? first_s[1] : r == 2 ? first_s[2] : first_s[3])
+                                                : *reinterpret_cast<const float4*>(scores + (size_t)r * a.score_stride + j);
+            const float lse = lse_s[r];
+            w.x += exp2f(t.x - lse);
+            w.y += exp2f(t.y - lse);
+            w.z += exp2f(t.z - lse);
+            w.w += exp2f(t.w - lse);
         }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (at[u]) *at[u] = w[u];
+        if (j + 4 <= kend) *reinterpret_cast<float4*>(at) = w;
+        else {
+            at[0] = w.x;
+            if (j + 1 < kend) at[1] = w.y;
+            if (j + 2 < kend) at[2] = w.z;
+        }
     }
 }
 
@@ -599,7 +654,7 @@ struct Plan { int splits; bool mma, cluster; };
 // How the keys are cut; a function of the sizes alone.
 static Plan plan_of(int requests, int nq, int nkv, int d, int max_len, int page_size, int dtype) {
     const int group = nq / nkv, sms = sm_count();
-    const bool mma = dtype == kBF16 && (d == 64 || d == 128) && (page_size & (page_size - 1)) == 0;
+    const bool mma = dtype == kBF16 && (d == 64 || d == 128) && page_size >= 4 && (page_size & (page_size - 1)) == 0;
     if (dtype == kF32 && group <= 8 && d % 4 == 0 && d <= 256) {
         // the kernel that cuts a row's keys over the warps of a block: a wave of blocks, none under 64 keys
         const long pairs = (long)requests * nkv, most = (max_len + 63) / 64;
@@ -654,6 +709,7 @@ LILY_API int lily_attention_decode_weighed(const void* q, const void* kv, float*
     LILY_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "attention_decode_weighed: %d query heads over %d kv heads", nq, nkv);
     LILY_REQUIRE(d >= 1 && d <= 256 && page_size > 0 && max_len >= 0, "attention_decode_weighed: head size %d (takes up to 256), pages of %d", d, page_size);
     LILY_REQUIRE(dtype == kF32 || dtype == kBF16, "attention_decode_weighed: dtype %d", dtype);
+    LILY_REQUIRE(((uintptr_t)scratch & 15) == 0, "attention_decode_weighed: scratch must be 16-byte aligned");
     const int score_stride = (max_len + 3) / 4 * 4, group = nq / nkv;
     const weighed::Plan plan = weighed::plan_of(requests, nq, nkv, d, max_len, page_size, dtype);
     weighed::DecodeArgs a{};
@@ -664,7 +720,7 @@ LILY_API int lily_attention_decode_weighed(const void* q, const void* kv, float*
     a.part_ml = a.part_o + (size_t)requests * nq * plan.splits * d;
     const dim3 join(requests, nkv, 1 + (max_len + weighed::JOIN_KEYS - 1) / weighed::JOIN_KEYS);
     if (plan.mma) {
-        LILY_REQUIRE((((uintptr_t)q | (uintptr_t)kv | (uintptr_t)out | (uintptr_t)scratch) & 15) == 0, "attention_decode_weighed: operands must be 16-byte aligned");
+        LILY_REQUIRE((((uintptr_t)q | (uintptr_t)kv | (uintptr_t)out | (uintptr_t)scratch | (uintptr_t)weights) & 15) == 0, "attention_decode_weighed: operands must be 16-byte aligned");
         LILY_REQUIRE(nkv * ((group + 15) / 16) <= 65535, "attention_decode_weighed: %d kv heads", nkv);
         int shift = 0;
         while ((1 << shift) < page_size) ++shift;
