@@ -18,7 +18,7 @@
 // comes last), so the results do not depend on who is first.
 //
 // Every wait is bounded: one that runs out sets a status word (lily_key_weights_status), the roles leave their loops and the block frees its
-// tensor memory; the weights are then NaN.
+// tensor memory; the weights are then void (NaN, or some of them as they were).
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -52,8 +52,7 @@ struct Params {
     float* weights;                       // [pages, nkv, page_size]
     float2* parts;                        // rows: [unit + block][group][128] (max, sum)
     float* lse;                           // [units][128], negative
-    int2* info;                           // [units] first block, blocks
-    int* done;                            // [tiles] parts that have arrived
+    int* done;                            // [tiles][4] parts that have arrived, for each 32 keys
     float* sums;                          // columns: [tile + block][group][128]
     int bt_stride, requests, nkv, group, tq, page_size, pages, units, tiles;
     int steps1, quota1, steps2, quota2;   // steps in all and of a block
@@ -77,13 +76,14 @@ __host__ __device__ inline int steps2_of(const Portion& p, int tq, int i) { retu
 
 constexpr int a_bytes(int d) { return AR * d * 2; }
 constexpr int b_bytes(int d) { return BR * d * 2; }
-constexpr int LSE = 4;                    // steps whose lse are held
+constexpr int LSE = 4;                    // steps whose description (and lse) is held
 constexpr int SUMS = 8;                   // tiles whose groups' sums are
-// shared memory: two standing tiles | stages | lse of the columns | the groups' sums | token of each row of a tile | barriers
+// shared memory: two standing tiles | stages | lse of the columns | the groups' sums | descriptions | token of each row of a tile | barriers
 constexpr int off_b(int d) { return 2 * a_bytes(d); }
 constexpr int off_lse(int d) { return off_b(d) + STAGES * b_bytes(d); }
 constexpr int off_sums(int d) { return off_lse(d) + LSE * BR * 4; }
-constexpr int off_tok(int d) { return off_sums(d) + SUMS * GROUPS * AR * 4; }
+constexpr int off_desc(int d) { return off_sums(d) + SUMS * GROUPS * AR * 4; }
+constexpr int off_tok(int d) { return off_desc(d) + LSE * 32; }
 constexpr int off_bars(int d) { return off_tok(d) + AR * 4; }
 constexpr int NUM_BARS = 4 + 2 * STAGES + 4 + 2 * LSE + SUMS;
 constexpr int off_misc(int d) { return off_bars(d) + 8 * NUM_BARS; }
@@ -102,6 +102,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code));
 }
+__device__ __forceinline__ void mbar_arrive_many(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
+}
 __device__ __forceinline__ void warp_arrive(uint32_t bar) {
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
@@ -109,7 +112,18 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void group_sync(int group) { asm volatile("bar.sync %0, 128;\n" ::"r"(group + 1) : "memory"); }
+// One step as the loader describes it to the groups.
+//   at        rows: the place of the tile's first token less the step's first key; columns: the tile's first place less that of the step's first token
+//   live      columns: heard tokens from the step's first on
+//   flags     FIRST, LAST: the first and last step of the tile that this pair of groups takes in this block; EVEN: the pair takes the tile's first step in this
+//             block; ALONE: all of the tile's steps are this block's; SINGLE: the tile has one step here; above them the number of such tiles in the block up to this one
+//   unit, begin, steps, where (kv head, request), i: the tile
+struct Step { int at, live, flags, unit, begin, steps, where, i; };
+enum : int { FIRST = 1, LAST = 2, EVEN = 4, ALONE = 8, SINGLE = 16, TILE_SHIFT = 8 };
+// Parts that block `b` leaves of a tile: a pair's two groups, or all four where it has two steps or more of it.
+__device__ __forceinline__ int parts_of(int begin, int steps, int quota, int b) {
+    return min(begin + steps, (b + 1) * quota) - max(begin, b * quota) == 1 ? 2 : 4;
+}
 
 // ---- pairs of floats in one register pair (fma.rn.f32x2: two IEEE operations an instruction) ----
 typedef unsigned long long Two;
@@ -255,8 +269,8 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + off_bars(D));
     uint32_t& tmem_base_s = *reinterpret_cast<uint32_t*>(smem + off_misc(D));
     int& abort_s = *reinterpret_cast<int*>(smem + off_misc(D) + 4);
-    int* last_s = reinterpret_cast<int*>(smem + off_misc(D) + 8);     // [GROUPS]
-    Cursor& start_s = *reinterpret_cast<Cursor*>(smem + off_misc(D) + 8 + 4 * GROUPS);
+    int4* desc_s = reinterpret_cast<int4*>(smem + off_desc(D));       // [LSE][2]
+    Cursor& start_s = *reinterpret_cast<Cursor*>(smem + off_misc(D) + 8);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = smem_u32(smem);
     const uint32_t a_smem = base, b_smem = base + off_b(D);
@@ -342,7 +356,10 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
         };
         const int q_bytes = group_rows * D * 2;
         bool ok = true;
-        int tile = 0, sent_a = 0, sent_b = 0, sent_l = 0;
+        int tile = 0, sent_a = 0, sent_b = 0, sent_l = 0, share_k = 0, share_n = 0, alone = 0;      // the tile's first step here, its steps here; tiles that were all this block's
+        int rows_in[STAGES], lse_in[LSE];                             // columns: the row tile that a stage, an lse buffer holds (few rows: the same for tile after tile)
+        for (int i = 0; i < STAGES; ++i) rows_in[i] = -1;
+        for (int i = 0; i < LSE; ++i) lse_in[i] = -1;
         auto look_ahead = [&](bool fresh) {
             if (PASS == 1) page = look_up(cur, cur.s * BR, BR);
             else if (fresh) page_a = look_up(cur, cur.i * AR, AR);
@@ -359,31 +376,55 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
                 else load_keys(dst, AR, AR * 128, cur.kvh, cur.i * AR, page_a, bar);
                 ++tile;
                 ++sent_a;
+                share_k = k;
+                share_n = min(cur.n - cur.s, mine - k);
+                alone += share_n == cur.n;
             }
             const int st = k % STAGES;
             ok = warp_wait(b_empty + 8 * st, ((k / STAGES) & 1) ^ 1, abort_flag, 2);
             if (!ok) break;
             const uint32_t bar = b_full + 8 * st, dst = b_smem + st * b_bytes(D);
-            if (lane == 0) mbar_expect_tx(bar, PASS == 1 ? b_bytes(D) : 2 * q_bytes);
+            const int t0 = PASS == 2 ? 2 * (cur.f + cur.s) : 0, unit = cur.unit0 + cur.kvh * 2 * p.p[cur.r].row_steps + t0;      // columns: the step's row tiles
+            bool held = false;
+            if (PASS == 2) {
+#pragma unroll
+                for (int i = 0; i < STAGES; ++i)
+                    if (i == st) held = rows_in[i] == unit, rows_in[i] = unit;
+            }
+            if (lane == 0) {
+                if (held) mbar_arrive(bar);
+                else mbar_expect_tx(bar, PASS == 1 ? b_bytes(D) : 2 * q_bytes);
+            }
             __syncwarp();
-            if (PASS == 1) {
-                load_keys(dst, BR, BR * 128, cur.kvh, cur.s * BR, page, bar);
-                ++sent_b;
-            } else {
-                const int t0 = 2 * (cur.f + cur.s);
+            if (PASS == 1) load_keys(dst, BR, BR * 128, cur.kvh, cur.s * BR, page, bar);
+            else if (!held) {
                 load_rows(dst, BR * 128, cur.kvh, cur.first + t0 * p.tq, bar);
                 load_rows(dst + AR * 128, BR * 128, cur.kvh, cur.first + (t0 + 1) * p.tq, bar);
-                ++sent_b;
-                if (k == 0) pdl_wait();
-                const int ls = k % LSE;
-                ok = warp_wait(l_empty + 8 * ls, ((k / LSE) & 1) ^ 1, abort_flag, 3);       // the lse of step k - LSE have been read
-                if (!ok) break;
-                if (lane == 0) {
-                    mbar_expect_tx(l_full + 8 * ls, BR * 4);
-                    bulk_load(smem_u32(lse_s + ls * BR), p.lse + (size_t)(cur.unit0 + cur.kvh * 2 * p.p[cur.r].row_steps + t0) * AR, BR * 4, l_full + 8 * ls);
-                }
-                ++sent_l;
             }
+            ++sent_b;
+            if (PASS == 2 && k == 0) pdl_wait();
+            const int ls = k % LSE, begin = g0 + k - cur.s, j = k - share_k;
+            ok = warp_wait(l_empty + 8 * ls, ((k / LSE) & 1) ^ 1, abort_flag, 3);           // step k - LSE has been read
+            if (!ok) break;
+            held = false;
+            if (PASS == 2) {
+#pragma unroll
+                for (int i = 0; i < LSE; ++i)
+                    if (i == ls) held = lse_in[i] == unit, lse_in[i] = unit;
+            }
+            if (lane == 0) {
+                const int at = PASS == 1 ? cur.place0 + cur.i * p.tq - cur.s * BR : cur.i * AR - cur.place0 - t0 * p.tq;
+                const int flags = (j < 2 ? FIRST : 0) | (j + 2 >= share_n ? LAST : 0) | (j & 1 ? 0 : EVEN) | (share_n == cur.n ? ALONE : 0) | (share_n == 1 ? SINGLE : 0) |
+                                  alone << TILE_SHIFT;
+                desc_s[2 * ls] = make_int4(at, cur.heard - t0 * p.tq, flags, cur.unit);
+                desc_s[2 * ls + 1] = make_int4(begin, cur.n, cur.kvh | cur.r << 16, cur.i);
+                if (PASS == 1 || held) mbar_arrive(l_full + 8 * ls);
+                else {
+                    mbar_expect_tx(l_full + 8 * ls, BR * 4);
+                    bulk_load(smem_u32(lse_s + ls * BR), p.lse + (size_t)unit * AR, BR * 4, l_full + 8 * ls);
+                }
+            }
+            ++sent_l;
             const bool fresh = ++cur.s == cur.n;
             if (fresh) next_tile<PASS>(p, cur);
             if (k + 1 < mine) look_ahead(fresh);
@@ -428,155 +469,159 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
         }
     } else {
         // ---- groups of 128 threads, a lane of tensor memory each: pair k & 1 takes step k, each of its groups 128 columns ----
-        // The pairs drift half a period apart, so that one's exponentials run under what the other does around its own.
-        // (Where a wait runs out the threads go on without it to the ends of the tiles, where they meet, and what they leave is NaN.)
-        const int which = (warp - 2) >> 2, pair = which >> 1, quarter = warp & 3, row = quarter * 32 + lane;
-        const int col0 = (which & 1) * COLS;
-        const uint32_t my = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(pair * BR + col0);
-        const int tok = tok_s[row];
+        const int which = (warp - 2) >> 2, pair = which >> 1, half = which & 1, quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t my = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(pair * BR + half * COLS);
+        const int tok = tok_s[row], tok_first = tok_s[quarter * 32], tok_last = tok_s[quarter * 32 + 31];
         const float c = p.c;
         float m = -INFINITY, l = 0.f;                                 // rows: running maximum (log2 units) and sum; columns: l is the sum
-        bool ok = true;
-        int tile = 0;
-        float* at = nullptr;
+        float* to = nullptr;
         float old = 0.f;
-        for (int k = 0; k < mine; ++k) {
-            const int buf = k & 1, ls = k % LSE;
-            if (PASS == 2 && which == 0 && (k == 0 || cur.s == 0)) {
-                // where this thread's place has its weight, and what it is: asked for ahead of the tile's steps
-                const int place = cur.i * AR + row;
-                at = nullptr;
-                if (place < cur.total) {
-                    at = p.weights + (((size_t)p.block_table[(size_t)cur.r * p.bt_stride + (place >> p.page_shift)] * p.nkv + cur.kvh) << p.page_shift) +
-                         (place & (p.page_size - 1));
-                    old = place < cur.prefix ? *at : 0.f;
+        for (int k = pair; k < mine; k += 2) {
+            const int ls = k % LSE;
+            if (!warp_wait(l_full + 8 * ls, (k / LSE) & 1, abort_flag, 8)) break;
+            const int4 d0 = desc_s[2 * ls], d1 = desc_s[2 * ls + 1];
+            const Step st{d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+            const bool collects = PASS == 2 && (st.flags & (EVEN | ALONE)) == (EVEN | ALONE) && half == 0;
+            if (st.flags & FIRST) {
+                m = -INFINITY;
+                l = 0.f;
+                if (collects) {
+                    // where this thread's place has its weight, and what it is: asked for ahead of the tile's steps
+                    const int r = st.where >> 16, place = st.i * AR + row;
+                    to = nullptr;
+                    if (place < p.p[r].total) {
+                        to = p.weights + (((size_t)p.block_table[(size_t)r * p.bt_stride + (place >> p.page_shift)] * p.nkv + (st.where & 0xffff)) << p.page_shift) +
+                             (place & (p.page_size - 1));
+                        old = place < p.p[r].prefix ? *to : 0.f;
+                    }
                 }
             }
-            if (buf == pair && ok) ok = warp_wait(s_full + 8 * buf, (k >> 1) & 1, abort_flag, 7);
-            if (PASS == 2 && buf == pair && ok) ok = warp_wait(l_full + 8 * ls, (k / LSE) & 1, abort_flag, 8);
-            if (!ok) l = __int_as_float(0x7fffffff);
-            else if (buf == pair) {
-                tc_fence_after();
-                const int key0 = cur.s * BR + col0, own = cur.place0 + cur.i * p.tq + tok;              // rows: the last place this one sees
-                // columns: the first token of their row tile
-                const int t0 = PASS == 2 ? ((cur.f + cur.s) * 2 + col0 / AR) * p.tq : 0, key = cur.i * AR + row;
-                const bool masked = PASS == 1 ? key0 + COLS - 1 > own - tok : cur.i * AR + AR - 1 > cur.place0 + t0 || t0 + p.tq > cur.heard;
-                Two sum[4] = {two(l, 0.f), 0, 0, 0};
+            if (!warp_wait(s_full + 8 * pair, (k >> 1) & 1, abort_flag, 7)) break;
+            tc_fence_after();
+            // Pieces of 32 columns, which a warp leaves out where no lane sees any of them and masks where not all are seen: rows and keys ascend
+            // along lanes and columns, so the first and the last say which it is.
+            const int own = st.at + tok - half * COLS;                // rows: the last column this one sees
+            const int from = st.at + row - half * p.tq, live = st.live - half * p.tq;      // columns: the row tile's tokens [from, live) see this place
+            Two sum[4] = {two(l, 0.f), 0, 0, 0};
 #pragma unroll
-                for (int c0 = 0; c0 < COLS; c0 += 32) {
-                    float s[32];
+            for (int c0 = 0; c0 < COLS; c0 += 32) {
+                bool some, all;
+                if (PASS == 1) some = c0 <= own - tok + tok_last, all = c0 + 31 <= own - tok + tok_first;
+                else {
+                    const int first = tok_s[c0], last = tok_s[c0 + 31];
+                    some = last >= from - lane && first < live;
+                    all = first >= from - lane + 31 && last < live;
+                }
+                float s[32];
+                if (some) {
                     tmem_ld32(my + (uint32_t)c0, s);
                     wait_loaded(s);
-                    if (c0 + 32 == COLS) {                            // the last has come: the accumulator goes back to the products
-                        tc_fence_before();
-                        warp_arrive(s_empty + 8 * buf);
+                }
+                if (c0 + 32 == COLS) {                                // the last has come: the accumulator goes back to the products
+                    tc_fence_before();
+                    warp_arrive(s_empty + 8 * pair);
+                }
+                if (!some) continue;
+                if (PASS == 1) {
+                    if (!all) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) s[e] = c0 + e <= own ? s[e] : -INFINITY;
                     }
-                    if (PASS == 1) {
-                        if (masked) {
+                    float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) s[e] = key0 + c0 + e <= own ? s[e] : -INFINITY;
-                        }
-                        float mx[4] = {s[0], s[1], s[2], s[3]};
+                    for (int e = 4; e < 28; e += 8)
 #pragma unroll
-                        for (int e = 4; e < 28; e += 8)
+                        for (int j = 0; j < 4; ++j) mx[j] = max3(mx[j], s[e + 2 * j], s[e + 2 * j + 1]);
+                    mx[0] = max3(mx[0], s[28], s[29]);
+                    mx[1] = max3(mx[1], s[30], s[31]);
+                    const float now = fmaxf(m, fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * c);
+                    if (__any_sync(0xffffffffu, now > m)) {
+                        const float f = now > m ? ex2(m - now) : 1.f;                 // (0 where m is -inf)
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) mx[j] = max3(mx[j], s[e + 2 * j], s[e + 2 * j + 1]);
-                        mx[0] = max3(mx[0], s[28], s[29]);
-                        mx[1] = max3(mx[1], s[30], s[31]);
-                        const float now = fmaxf(m, fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * c);
-                        if (__any_sync(0xffffffffu, now > m)) {
-                            const float f = now > m ? ex2(m - now) : 1.f;             // (0 where m is -inf)
+                        for (int j = 0; j < 4; ++j) sum[j] = mul2(sum[j], two(f, f));
+                        m = now;
+                    }
+                    const float off = m == -INFINITY ? 0.f : -m;
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) sum[j] = mul2(sum[j], two(f, f));
-                            m = now;
-                        }
-                        const float off = m == -INFINITY ? 0.f : -m;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const Two x = fma2(two(s[2 * e], s[2 * e + 1]), two(c, c), two(off, off));
-                            sum[e & 3] = add2(sum[e & 3], exp2_of(x));
-                        }
-                    } else {
-                        const ulonglong2* minus_lse = reinterpret_cast<const ulonglong2*>(lse_s + ls * BR + col0 + c0);
-                        Two v[16];
+                    for (int e = 0; e < 16; ++e) sum[e & 3] = add2(sum[e & 3], exp2_of(fma2(two(s[2 * e], s[2 * e + 1]), two(c, c), two(off, off))));
+                } else {
+                    const ulonglong2* minus_lse = reinterpret_cast<const ulonglong2*>(lse_s + ls * BR + half * COLS + c0);
+                    if (all) {
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
                             const ulonglong2 z = minus_lse[e >> 1];
-                            const Two x = fma2(two(s[2 * e], s[2 * e + 1]), two(c, c), z.x), y = fma2(two(s[2 * e + 2], s[2 * e + 3]), two(c, c), z.y);
-                            v[e] = exp2_of(x);
-                            v[e + 1] = exp2_of(y);
+                            sum[e & 3] = add2(sum[e & 3], exp2_of(fma2(two(s[2 * e], s[2 * e + 1]), two(c, c), z.x)));
+                            sum[(e + 1) & 3] = add2(sum[(e + 1) & 3], exp2_of(fma2(two(s[2 * e + 2], s[2 * e + 3]), two(c, c), z.y)));
                         }
-                        if (masked) {
-                            // the columns' tokens that are heard and see this place: [from, heard), in tokens of the row tile
-                            const int from = max(key - cur.place0 - t0, 0);
-                            const uint32_t some = max(cur.heard - t0 - from, 0);
-                            const int4* tok4 = reinterpret_cast<const int4*>(tok_s + c0);
+                    } else {
+                        const int low = max(from, 0);
+                        const uint32_t seen = max(live - low, 0);
+                        const int4* tok4 = reinterpret_cast<const int4*>(tok_s + c0);
 #pragma unroll
-                            for (int e = 0; e < 16; e += 2) {
-                                const int4 t = tok4[e >> 1];
-                                float a, b;
-                                apart(v[e], a, b);
-                                v[e] = two((uint32_t)(t.x - from) < some ? a : 0.f, (uint32_t)(t.y - from) < some ? b : 0.f);
-                                apart(v[e + 1], a, b);
-                                v[e + 1] = two((uint32_t)(t.z - from) < some ? a : 0.f, (uint32_t)(t.w - from) < some ? b : 0.f);
-                            }
+                        for (int e = 0; e < 16; e += 2) {
+                            const ulonglong2 z = minus_lse[e >> 1];
+                            const int4 t = tok4[e >> 1];
+                            float a, b;
+                            apart(exp2_of(fma2(two(s[2 * e], s[2 * e + 1]), two(c, c), z.x)), a, b);
+                            sum[e & 3] = add2(sum[e & 3], two((uint32_t)(t.x - low) < seen ? a : 0.f, (uint32_t)(t.y - low) < seen ? b : 0.f));
+                            apart(exp2_of(fma2(two(s[2 * e + 2], s[2 * e + 3]), two(c, c), z.y)), a, b);
+                            sum[(e + 1) & 3] = add2(sum[(e + 1) & 3], two((uint32_t)(t.z - low) < seen ? a : 0.f, (uint32_t)(t.w - low) < seen ? b : 0.f));
                         }
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) sum[e & 3] = add2(sum[e & 3], v[e]);
                     }
                 }
-                float a, b;
-                apart(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, b);
-                l = a + b;
-                if (PASS == 2) warp_arrive(l_empty + 8 * ls);
             }
-            if (cur.s + 1 == cur.n || k + 1 == mine) {
-                // the end of this block's share of the tile, whose first step is `begin`
-                const int begin = g0 + k - cur.s, end = begin + cur.n;
-                const bool alone = begin >= g0 && end <= g0 + quota;
-                const size_t slot = ((size_t)(cur.unit + (int)blockIdx.x) * GROUPS + which) * AR + row;
-                if (PASS == 1) {
-                    p.parts[slot] = make_float2(m, l);
-                    if (begin >= g0 && which == 0 && row == 0) p.info[cur.unit] = make_int2(blockIdx.x, alone ? 1 : (end - 1) / quota - (int)blockIdx.x + 1);
-                } else if (alone) {
-                    // The groups' sums through shared memory, joined by the first group; the others go on.  (SUMS tiles of room: a group is at most five
-                    // tiles ahead of the first, whose accumulators the products behind wait for.)
-                    float* sums = sums_s + (size_t)(tile % SUMS) * GROUPS * AR;
-                    sums[which * AR + row] = l;
-                    if (which) warp_arrive(sums_full + 8 * (tile % SUMS));
-                    else {
-                        ok = warp_wait(sums_full + 8 * (tile % SUMS), (tile / SUMS) & 1, abort_flag, 9) && ok;
-                        float w = old;
-#pragma unroll
-                        for (int j = 0; j < GROUPS; ++j) w += sums[j * AR + row];
-                        if (at) *at = ok ? w : __int_as_float(0x7fffffff);
-                    }
-                    ++tile;
+            float a, b;
+            apart(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, b);
+            l = a + b;
+            warp_arrive(l_empty + 8 * ls);
+            if (!(st.flags & LAST)) continue;
+            // the end of what this pair has of the tile here; its part's number: the pair with the tile's first step comes first
+            const int part = (st.flags & EVEN ? 0 : 2) + half;
+            const size_t slot = ((size_t)(st.unit + (int)blockIdx.x) * GROUPS + part) * AR + row;
+            if (PASS == 1) {
+                p.parts[slot] = make_float2(m, l);
+            } else if (st.flags & ALONE) {
+                // The groups' sums through shared memory, added up by the group that has the tile's first columns; the others go on.  (SUMS tiles of room: a
+                // group is at most four tiles ahead of another, whose accumulators the products behind wait for.)
+                const int at = (st.flags >> TILE_SHIFT) - 1;
+                const uint32_t full = sums_full + 8 * (at % SUMS);
+                float* sums = sums_s + (size_t)(at % SUMS) * GROUPS * AR;
+                sums[part * AR + row] = l;
+                __syncwarp();
+                if (part) {
+                    // twelve warps' worth of arrivals, of three groups or of one
+                    if (lane == 0) mbar_arrive_many(full, st.flags & SINGLE ? 3 : 1);
                 } else {
-                    // several blocks: the one that comes last joins what all have left in scratch
-                    const int blocks_first = begin / quota, parts = GROUPS * ((end - 1) / quota - blocks_first + 1);
-                    __stcg(p.sums + slot, l);
-                    __threadfence();
-                    group_sync(which);
-                    if (row == 0) last_s[which] = atomicAdd(p.done + cur.unit, 1) == parts - 1;
-                    group_sync(which);
-                    if (last_s[which]) {
-                        __threadfence();
-                        float w = 0.f;
-                        for (int b = 0; b < parts; ++b) w += __ldcg(p.sums + ((size_t)(cur.unit + blocks_first) * GROUPS + b) * AR + row);
-                        const int place = cur.i * AR + row;
-                        if (place < cur.total) {
-                            float* to = p.weights + (((size_t)p.block_table[(size_t)cur.r * p.bt_stride + (place >> p.page_shift)] * p.nkv + cur.kvh) << p.page_shift) +
-                                        (place & (p.page_size - 1));
-                            *to = (place < cur.prefix ? *to : 0.f) + w;
-                        }
-                    }
-                    group_sync(which);                                // (the word is read before the next tile's)
+                    if (!warp_wait(full, (at / SUMS) & 1, abort_flag, 9)) break;
+                    const int parts = st.flags & SINGLE ? 2 : 4;
+                    float w = old;
+                    for (int j = 0; j < parts; ++j) w += sums[j * AR + row];
+                    if (to) *to = w;
                 }
-                m = -INFINITY;
-                l = 0.f;
+            } else {
+                // several blocks: of the warps with these 32 keys the one that comes last joins what all have left in scratch, in their order
+                const int b0 = st.begin / quota, b1 = (st.begin + st.steps - 1) / quota;
+                int expected = 0;
+                for (int b = b0; b <= b1; ++b) expected += parts_of(st.begin, st.steps, quota, b);
+                __stcg(p.sums + slot, l);
+                __threadfence();
+                __syncwarp();
+                int before = 0;
+                if (lane == 0) before = atomicAdd(p.done + 4 * st.unit + quarter, 1);
+                if (__shfl_sync(0xffffffffu, before, 0) == expected - 1) {
+                    __threadfence();
+                    const int r = st.where >> 16, place = st.i * AR + row;
+                    float w = 0.f;
+                    for (int b = b0; b <= b1; ++b)
+                        for (int j = 0, parts = parts_of(st.begin, st.steps, quota, b); j < parts; ++j)
+                            w += __ldcg(p.sums + ((size_t)(st.unit + b) * GROUPS + j) * AR + row);
+                    if (place < p.p[r].total) {
+                        float* at = p.weights + (((size_t)p.block_table[(size_t)r * p.bt_stride + (place >> p.page_shift)] * p.nkv + (st.where & 0xffff)) << p.page_shift) +
+                                    (place & (p.page_size - 1));
+                        *at = (place < p.p[r].prefix ? *at : 0.f) + w;
+                    }
+                }
             }
-            if (++cur.s == cur.n) next_tile<PASS>(p, cur);
         }
     }
     if (PASS == 2 && warp < 2) pdl_wait();                            // (a block ends behind the kernels ahead)
@@ -589,27 +634,57 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
     }
 }
 
-// A row tile a block: its parts in the order of the blocks that made them, lse = max + log2(sum); +inf for rows that are none.  Also
-// clears the column kernel's counters.
-__global__ void __launch_bounds__(AR) key_weights_join_kernel(const __grid_constant__ Params p) {
+// A row tile a block: its parts joined, lse = max + log2(sum); +inf (its negative is kept) for rows that are none.  Four threads a row, or eight where a tile has
+// many blocks' parts, each with one number's part of every (second) block, four of them on their way, joined in the order of the threads.  Also clears the column kernel's counters.
+constexpr int JOIN_THREADS = 8 * AR;       // at most
+__device__ __forceinline__ void join_part(float& m, float& l, float2 v) {
+    if (v.x == -INFINITY && v.y == 0.f) return;                       // no keys (a NaN is no maximum, but makes the sum one)
+    const float now = fmaxf(m, v.x);
+    l = fmaf(v.y, exp2f(v.x - now), m == -INFINITY && l == 0.f ? 0.f : l * exp2f(m - now));
+    m = now;
+}
+__global__ void __launch_bounds__(JOIN_THREADS) key_weights_join_kernel(const __grid_constant__ Params p) {
+    __shared__ float2 part_s[8][AR];
+    __shared__ int sum_s[32];
     pdl_enter_small();
-    const int unit = blockIdx.x, row = threadIdx.x;
-    for (int i = unit * AR + row; i < p.tiles; i += gridDim.x * AR) p.done[i] = 0;
+    const int unit = blockIdx.x, tid = threadIdx.x, row = tid & (AR - 1), sub = tid / AR, subs = blockDim.x / AR;
+    for (int i = unit * blockDim.x + tid; i < 4 * p.tiles; i += gridDim.x * blockDim.x) p.done[i] = 0;
     int r = 0;
     while (r + 1 < p.requests && p.p[r + 1].unit0 <= unit) ++r;
     const Portion& q = p.p[r];
-    const int i = (unit - q.unit0) % row_tiles(q, p.tq);
-    float lse = -INFINITY;                                            // negative
-    if (row < p.group * p.tq && i * p.tq + row / p.group < q.heard) {
-        const int2 in = p.info[unit];
-        const float2* part = p.parts + (size_t)(unit + in.x) * GROUPS * AR + row;
-        float m = -INFINITY, l = 0.f;
-        for (int b = 0; b < GROUPS * in.y; ++b) m = fmaxf(m, part[b * AR].x);
-        for (int b = 0; b < GROUPS * in.y; ++b) {
-            const float2 v = part[b * AR];
-            if (v.x > -INFINITY || v.y != 0.f) l = fmaf(v.y, exp2f(v.x - m), l);      // (a NaN is no maximum, but makes the sum one)
+    const int tiles = row_tiles(q, p.tq), i = (unit - q.unit0) % tiles;
+    // the tile's steps [begin, begin + steps)
+    int ahead = 0;
+    for (int j = tid; j < i; j += blockDim.x) ahead += steps1_of(q, p.tq, j);
+    ahead = __reduce_add_sync(0xffffffffu, ahead);
+    if ((tid & 31) == 0) sum_s[tid >> 5] = ahead;
+    __syncthreads();
+    const int warps = blockDim.x >> 5, begin = q.step1 + (unit - q.unit0) / tiles * q.per1 + __reduce_add_sync(0xffffffffu, (tid & 31) < warps ? sum_s[tid & 31] : 0), steps = steps1_of(q, p.tq, i);
+    const bool live = row < p.group * p.tq && i * p.tq + row / p.group < q.heard;
+    float m = -INFINITY, l = 0.f;
+    if (live) {
+        const int b0 = begin / p.quota1, b1 = (begin + steps - 1) / p.quota1, j = sub & 3;
+        const int every = subs >> 2;
+        for (int b = b0 + (sub >> 2); b <= b1; b += 4 * every) {
+            float2 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int at = b + u * every;
+                v[u] = at <= b1 && j < parts_of(begin, steps, p.quota1, at) ? p.parts[((size_t)(unit + at) * GROUPS + j) * AR + row] : make_float2(-INFINITY, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) join_part(m, l, v[u]);
         }
+    }
+    part_s[sub][row] = make_float2(m, l);
+    __syncthreads();
+    if (sub) return;
+    float lse = -INFINITY;                                            // negative
+    if (live) {
+        m = -INFINITY, l = 0.f;
+        for (int u = 0; u < subs; ++u) join_part(m, l, part_s[u][row]);
         lse = -(m + log2f(l));
+        if (*(volatile int*)&g_status) lse = __int_as_float(0x7fffffff);                  // a wait of the row kernel gave up: its parts are void
     }
     p.lse[(size_t)unit * AR + row] = lse;
 }
@@ -627,7 +702,9 @@ static int launch(const Params& p, const CUtensorMap& map_q, const CUtensorMap& 
         configured = true;
     }
     launch_pdl(key_weights_tc_kernel<D, 1>, dim3((p.steps1 + p.quota1 - 1) / p.quota1), dim3(THREADS), (size_t)smem_bytes(D), stream, map_q, map_kv, p);
-    launch_pdl(key_weights_join_kernel, dim3(p.units), dim3(AR), 0, stream, p);
+    int most = 0;                             // steps of a row tile
+    for (int r = 0; r < p.requests; ++r) most = p.p[r].heard > 0 && (p.p[r].total + BR - 1) / BR > most ? (p.p[r].total + BR - 1) / BR : most;
+    launch_pdl(key_weights_join_kernel, dim3(p.units), dim3(most > 4 * p.quota1 ? JOIN_THREADS : JOIN_THREADS / 2), 0, stream, p);
     launch_pdl(key_weights_tc_kernel<D, 2>, dim3((p.steps2 + p.quota2 - 1) / p.quota2), dim3(THREADS), (size_t)smem_bytes(D), stream, map_q, map_kv, p);
     return 0;
 }
@@ -671,8 +748,8 @@ static size_t plan(Params& p, int requests, const int* prefix, const int* fresh,
     p.quota1 = s1 > 0 ? (int)((s1 + sms - 1) / sms) : 1;
     p.quota2 = s2 > 0 ? (int)((s2 + sms - 1) / sms) : 1;
     const int b1 = (p.steps1 + p.quota1 - 1) / p.quota1, b2 = (p.steps2 + p.quota2 - 1) / p.quota2;
-    // parts | lse | info | counters | sums, each on 16 bytes
-    return (size_t)(unit + b1) * 2 * GROUPS * AR + (size_t)unit * AR + (size_t)unit * 2 + ((size_t)tile + 3) / 4 * 4 + (size_t)(tile + b2) * GROUPS * AR + 16;
+    // parts | lse | counters | sums, each on 16 bytes
+    return (size_t)(unit + b1) * 2 * GROUPS * AR + (size_t)unit * AR + (size_t)tile * 4 + (size_t)(tile + b2) * GROUPS * AR + 16;
 }
 
 }  // namespace keyw5
@@ -752,10 +829,8 @@ LILY_API int lily_key_weights_tc(const void* q, int tokens, const void* kv, int 
             at += (size_t)(p.units + b1) * 2 * keyw5::GROUPS * keyw5::AR;
             p.lse = at;
             at += (size_t)p.units * keyw5::AR;
-            p.info = reinterpret_cast<int2*>(at);
-            at += (size_t)p.units * 2;
             p.done = reinterpret_cast<int*>(at);
-            at += ((size_t)p.tiles + 3) / 4 * 4;
+            at += (size_t)p.tiles * 4;
             p.sums = at;
             const int rc = d == 64 ? keyw5::launch<64>(p, map_q, map_kv, stream) : keyw5::launch<128>(p, map_q, map_kv, stream);
             if (rc) return rc;
