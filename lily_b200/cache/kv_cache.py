@@ -132,6 +132,16 @@ class KVCacheManager:
         no later query can see.  Returns the number of pages given back."""
         return sum(g.tables.pass_window(slot, seq_len) for g in self.groups)
 
+    def shrink(self, slot: int, new_len: int) -> int:
+        """Gives back the pages behind the first ``new_len`` positions of a request (whose keys were moved there, or are let go
+        of).  Returns the number of pages given back."""
+        if not 0 <= new_len <= self.lengths[slot]:
+            raise ValueError(f"request of {self.lengths[slot]} positions cannot shrink to {new_len}")
+        if any(g.tables.window is not None for g in self.groups):
+            raise ValueError("a group with a window gives its pages back as the window passes them")
+        self.lengths[slot] = new_len
+        return sum(g.tables.shrink(slot, new_len) for g in self.groups)
+
     def close_request(self, slot: int) -> None:
         for g in self.groups:
             g.tables.close(slot)

@@ -152,6 +152,18 @@ class GroupTables:
         self.pool.free(gone)
         return len(gone)
 
+    def shrink(self, slot: int, new_len: int) -> int:
+        """Gives back the pages behind the first ``new_len`` positions."""
+        t = self.tables[slot]
+        count = pages_for(new_len, self.page_size)
+        gone = [p for p in t.pages[count:] if p]
+        if len(t.pages) > count:
+            del t.pages[count:]
+            t.first_live = min(t.first_live, count)
+            t.touch()
+        self.pool.free(gone)
+        return len(gone)
+
     def close(self, slot: int) -> None:
         t = self.tables.pop(slot)
         self.pool.free([p for p in t.pages if p])

@@ -870,3 +870,113 @@ def mlstm_out(y, nq, m, gate, gate_col, gain, floor, eps, state, m_off, cu_seqle
         last = int(cu_seqlens[r + 1]) - 1
         state[int(slots[r]), m_off:m_off + heads] = m[last]
     return (o * gain * torch.sigmoid(_sum(gate).float()[:, gate_col:gate_col + y.shape[1]])).to(out_dtype)
+
+
+# ---------------------------------------------------------------------------- a cache held to a budget of places
+
+def pair_axes(sections, device, in_turn=False):
+    if in_turn:
+        axes = [a for i in range(max(sections)) for a, n in enumerate(sections) if i < n]
+    else:
+        axes = [a for a, n in enumerate(sections) for _ in range(n)]
+    return torch.tensor(axes, dtype=torch.int32, device=device)
+
+
+def _places(table_row, n, page_size):
+    """(page, offset) of the first n places of a request."""
+    at = torch.arange(n, device=table_row.device)
+    return table_row[at // page_size].long(), at % page_size
+
+
+def axes_rope_write(qkv, q_gain, k_gain, eps, cos, sin, positions, pair_axis, places, token_req, block_table, kv_layer, nq, nkv, d,
+                    rotary_dim, page_size, q_out=None, row=None):
+    x = _sum(qkv).float()
+    n, half = x.shape[0], rotary_dim // 2
+    q, k, v = (t.reshape(n, -1, d) for t in x[:, :(nq + 2 * nkv) * d].split([nq * d, nkv * d, nkv * d], 1))
+    at = positions.long()[pair_axis.long()].t()                                  # [tokens, pairs]
+    pair = torch.arange(half, device=x.device)
+    c, s = cos[at, pair][:, None], sin[at, pair][:, None]
+
+    def turned(t, gain):
+        if gain is not None:
+            t = t * torch.rsqrt(t.pow(2).mean(-1, keepdim=True) + eps) * gain.float()
+        a, b = t[..., :half], t[..., half:rotary_dim]
+        return torch.cat([a * c - b * s, b * c + a * s, t[..., rotary_dim:]], -1)
+    q, k = turned(q, q_gain), turned(k, k_gain)
+    for t in range(n):
+        p = int(places[t])
+        page = int(block_table[int(token_req[t]), p // page_size])
+        kv_layer[page, 0, :, p % page_size] = k[t].to(kv_layer.dtype)
+        kv_layer[page, 1, :, p % page_size] = v[t].to(kv_layer.dtype)
+    q = q.reshape(n, nq * d).to(kv_layer.dtype)
+    return q if q_out is None else q_out.copy_(q)
+
+
+def _given(q, k, q_pos, scale):
+    """What rows q [rows, nq, d] at places ``q_pos`` give to keys k [keys, nkv, d]: [keys, nkv] over the rows and each kv head's query heads."""
+    nkv = k.shape[1]
+    s = torch.einsum("qghd,kgd->ghqk", q.reshape(q.shape[0], nkv, -1, q.shape[-1]), k) * scale
+    s = s.masked_fill(torch.arange(k.shape[0], device=q.device)[None] > q_pos[:, None], float("-inf"))
+    return torch.softmax(s, -1).sum((1, 2)).t()
+
+
+def attention_decode_weighed(q, kv_layer, weights, block_table, seq_lens, max_seq_len, nq, nkv, d, page_size, scale, out=None, scratch=None):
+    out = torch.empty_like(q) if out is None else out
+    for r in range(q.shape[0]):
+        n = int(seq_lens[r])
+        if not n:
+            out[r] = 0
+            continue
+        k, v = _gather_kv(kv_layer, block_table[r], n, page_size)
+        rows, at = q[r:r + 1].float().view(1, nq, d), torch.tensor([n - 1], device=q.device)
+        out[r] = _attend(rows, k, v, at, scale, None).reshape(-1).to(out.dtype)
+        page, off = _places(block_table[r], n, page_size)
+        weights[page[-1], :, off[-1]] = 0
+        weights[page, :, off] += _given(rows, k, at, scale)
+    return out
+
+
+def attention_key_weights(q, kv_layer, weights, block_table, cu_seqlens, prefix_lens, h_prefix_lens, h_new_lens, nq, nkv, d, page_size, scale,
+                          observe=None, scratch=None):
+    for r, (cached, new) in enumerate(zip(h_prefix_lens, h_new_lens)):
+        if not new:
+            continue
+        start, heard = int(cu_seqlens[r]), min(new, observe or new)
+        k, _ = _gather_kv(kv_layer, block_table[r], cached + new, page_size)
+        rows = q[start + new - heard:start + new].float().view(heard, nq, d)
+        page, off = _places(block_table[r], cached + new, page_size)
+        weights[page[cached:], :, off[cached:]] = 0
+        weights[page, :, off] += _given(rows, k, torch.arange(cached + new - heard, cached + new, device=q.device), scale)
+
+
+def select_keys(weights, block_table, lengths, max_length, keep, first=0, recent=0):
+    w = weights if weights.dim() == 4 else weights[None]
+    layers, _, nkv, page_size = w.shape
+    kept = torch.full((layers, lengths.numel(), nkv, keep), -1, dtype=torch.int32, device=w.device)
+    for r in range(lengths.numel()):
+        n = int(lengths[r])
+        if n <= keep:
+            kept[:, r, :, :n] = torch.arange(n, dtype=torch.int32, device=w.device)
+            continue
+        page, off = _places(block_table[r], n, page_size)
+        value = torch.nan_to_num(w[:, page, :, off], nan=float("inf"), posinf=3e38).permute(1, 2, 0).clone()      # [layers, kv heads, places]
+        value[..., :first] = float("inf")
+        value[..., n - recent:] = float("inf")
+        order = torch.sort(value, dim=-1, descending=True, stable=True).indices[..., :keep]
+        kept[:, r] = order.sort(-1).values.int()
+    return kept
+
+
+def move_keys(kv, weights, block_table, kept, to_table=None):
+    kv = kv if kv.dim() == 6 else kv[None]
+    weights = weights[None] if weights is not None and weights.dim() == 3 else weights
+    to_table = block_table if to_table is None else to_table
+    page_size = kv.shape[4]
+    for layer, r, g in [(a, b, c) for a in range(kept.shape[0]) for b in range(kept.shape[1]) for c in range(kept.shape[2])]:
+        at = kept[layer, r, g]
+        at = at[at >= 0].long()
+        page, off = block_table[r][at // page_size].long(), at % page_size
+        to, to_off = _places(to_table[r], at.numel(), page_size)
+        kv[layer, to, :, g, to_off] = kv[layer, page, :, g, off].clone()
+        if weights is not None:
+            weights[layer, to, g, to_off] = weights[layer, page, g, off].clone()
