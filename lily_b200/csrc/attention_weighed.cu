@@ -498,9 +498,9 @@ __global__ void __launch_bounds__(THREADS, 3) decode_weighed_mma_kernel(const De
         }
         if (CLUSTER) {
             const int owner = i / share;
-            *reinterpret_cast<float4*>(cluster.map_shared_rank(recv_o, owner) + bz * share + (i - owner * share)) = acc;
+            write_to_block(reinterpret_cast<float4*>(recv_o + bz * share + (i - owner * share)), owner, acc);
             if (col / 4 < splits)                                   // group p of four columns tells block p the row's (max, sum)
-                *reinterpret_cast<float2*>(cluster.map_shared_rank(recv_ml, col / 4) + (bz * 16 + r) * 2) = make_float2(mx, den);
+                write_to_block(reinterpret_cast<float2*>(recv_ml + (bz * 16 + r) * 2), col / 4, make_float2(mx, den));
         } else if (splits > 1) {
             const size_t at = ((size_t)req * a.nq + head0 + r) * splits + bz;
             *reinterpret_cast<float4*>(a.part_o + at * D + col) = acc;

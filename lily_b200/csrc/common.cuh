@@ -5,6 +5,7 @@
 // `lily_last_error()` gives the message of the last failure on the calling thread.
 #pragma once
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
@@ -114,6 +115,9 @@ __device__ __forceinline__ float xielu_fast(float z, float a, float b) {
 // access.  The two lie around the wait for the kernel ahead and the loads, where the barrier costs nothing that shows.
 __device__ __forceinline__ void cluster_arrive_started() { asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait_started() { asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory"); }
+// Writes ``value`` where ``at`` lies in the shared memory of the cluster's block ``rank`` (after the wait above).
+template <typename T>
+__device__ __forceinline__ void write_to_block(T* at, unsigned rank, T value) { *cooperative_groups::this_cluster().map_shared_rank(at, rank) = value; }
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

@@ -237,18 +237,15 @@ __global__ void __launch_bounds__(COL_THREADS) key_weights_columns_kernel(const 
     }
     *reinterpret_cast<float4*>(&sum_s[ty][4 * tx]) = w;
     __syncthreads();
+    if (parts > 1) cluster_wait_started();
     if (tid < TN) {
         float mine = 0.f;
 #pragma unroll
         for (int i = 0; i < 32; ++i) mine += sum_s[i][tid];
         if (parts == 1) sum += mine;
-        else {
-            cluster_wait_started();                                  // (the warps of these threads; the others below)
-            *cg::this_cluster().map_shared_rank(&parts_s[part][tid], 0) = mine;
-        }
+        else write_to_block(&parts_s[part][tid], 0, mine);
     }
     if (parts > 1) {
-        if (tid >= TN) cluster_wait_started();
         cg::this_cluster().sync();
         if (tid < TN)
             for (int i = 0; i < parts; ++i) sum += parts_s[i][tid];

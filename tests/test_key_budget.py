@@ -280,3 +280,25 @@ def test_stack_of_kernels_in_bfloat16_keeps_its_books(nq, nkv, d, page):
                 torch.testing.assert_close(total, torch.full_like(total, h * nq / nkv), atol=0, rtol=1e-2)
             else:
                 assert bool((total > 0).all()) and bool((total < h * nq / nkv).all())
+
+
+def test_no_block_writes_to_a_block_that_may_not_have_started():
+    """Every kernel that writes to other blocks of its cluster waits until they run, once and ahead of its first write."""
+    import os
+    import re
+
+    from lily_b200.csrc import build
+    found = []
+    for name in ("attention_weighed.cu", "key_weights.cu", "key_weights_tcgen05.cu", "key_budget.cu", "axes_rope.cu"):
+        with open(os.path.join(build.HERE, name)) as f:
+            text = re.sub(r"//[^\n]*", "", f.read())
+        heads = [m.start() for m in re.finditer(r"__global__", text)] + [len(text)]
+        for body in (text[a:b] for a, b in zip(heads, heads[1:])):
+            write = body.find("write_to_block(")
+            if write < 0:
+                assert "map_shared_rank" not in body, name
+                continue
+            found.append(name)
+            assert 0 < body.find("cluster_arrive_started();") < body.find("cluster_wait_started();") < write, name
+            assert body.count("cluster_arrive_started();") == body.count("cluster_wait_started();") == 1, name
+    assert found == ["attention_weighed.cu", "key_weights.cu"]
