@@ -50,7 +50,24 @@ attention_decode_f32_kernel(const AttnArgs a) {
     const size_t kbase = (size_t)kvh * khead, vbase = (size_t)a.nkv * khead + (size_t)((kvh + a.v_shift) % a.nkv) * vhead;
 
     float4 k[KB][C], v[KB][C], kn[AHEAD ? KB : 1][C], vn[AHEAD ? KB : 1][C];
+    // WEIGHED, pages of whole keys of a step: lane i looks up the page of the warp's step i ahead, so that a step's reads do not wait for the table's
+    int pages = 0, looked = 0;
     auto fetch = [&](int u0, float4 (*kd)[C], float4 (*vd)[C]) {
+        if (WEIGHED && a.page_size % KB == 0) {
+            if (looked % 32 == 0) pages = u0 + lane * STEP < uend ? table[(u0 + lane * STEP) / a.page_size] : 0;
+            const float* page = kv + (size_t)__shfl_sync(0xffffffffu, pages, looked++ % 32) * page_stride;
+            const size_t row0 = u0 % a.page_size;
+#pragma unroll
+            for (int j = 0; j < KB; ++j)
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    const int col = c * 128 + lane * 4;
+                    const bool in = u0 + j < uend && col < d;
+                    kd[j][c] = in ? *reinterpret_cast<const float4*>(page + kbase + (row0 + j) * d + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    vd[j][c] = in ? *reinterpret_cast<const float4*>(page + vbase + (row0 + j) * d + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < KB; ++j) {
             const int u = u0 + j, kpos = u < nkeep ? u : klo + (u - nkeep);

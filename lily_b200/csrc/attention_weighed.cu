@@ -134,11 +134,14 @@ __global__ void __launch_bounds__(JOIN_THREADS) decode_weighed_join_kernel(const
     for (int h = warp; h < group; h += JOIN_THREADS / 32) {
         const float* ml = a.part_ml + ((size_t)req * a.nq + kvh * group + h) * a.splits * 2;
         float m = -INFINITY, l = 0.f;
-        for (int s = lane; s < a.splits; s += 32) m = fmaxf(m, ml[2 * s]);
-        m = warp_max(m);
-        for (int s = lane; s < a.splits; s += 32) l += ml[2 * s + 1] * exp2f(ml[2 * s] - (m == -INFINITY ? 0.f : m));
-        l = warp_sum(l);
-        if (lane == 0) sm[h] = m + log2f(l);
+        for (int s = lane; s < a.splits; s += 32) {
+            const float ms = ml[2 * s], ls = ml[2 * s + 1], mn = fmaxf(m, ms), base = mn == -INFINITY ? 0.f : mn;
+            l = fmaf(ls, exp2f(ms - base), l * exp2f(m - base));
+            m = mn;
+        }
+        const float most = warp_max(m);
+        l = warp_sum(l * exp2f(m - (most == -INFINITY ? 0.f : most)));
+        if (lane == 0) sm[h] = most + log2f(l);
     }
     __syncthreads();
     if (blockIdx.z == 0) {
@@ -149,7 +152,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) decode_weighed_join_kernel(const
             const size_t row = (size_t)req * a.nq + kvh * group + h, at = row * a.splits;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
             if (n > 0) {
-#pragma unroll 4
+#pragma unroll 8
                 for (int s = 0; s < a.splits; ++s) {
                     const float m = a.part_ml[(at + s) * 2], l = a.part_ml[(at + s) * 2 + 1];
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -262,11 +265,11 @@ __global__ void __launch_bounds__(THREADS, 3) decode_weighed_mma_kernel(const De
     }
     pdl_enter_small();
     int bx = blockIdx.x, by = blockIdx.y, bz = blockIdx.z;
-    if (!CLUSTER && a.longest_first) {
+    if (a.longest_first) {
         // the blocks of the row that is next by length: its kv heads and ranges side by side
         int* len_s = reinterpret_cast<int*>(q_s);                   // the queries come there later
-        const int rows = gridDim.x, part = gridDim.y * gridDim.z;
-        const int at = blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z), want = at / part;
+        const int rows = gridDim.x, part = CLUSTER ? gridDim.y : gridDim.y * gridDim.z;
+        const int at = blockIdx.x + gridDim.x * (blockIdx.y + (CLUSTER ? 0 : gridDim.y * blockIdx.z)), want = at / part;
         const int mine = tid < rows ? a.seq_lens[tid] : 0;
         len_s[tid] = mine;
         __syncthreads();
@@ -279,8 +282,8 @@ __global__ void __launch_bounds__(THREADS, 3) decode_weighed_mma_kernel(const De
         if (tid < rows && rank == want) row_s = tid;
         __syncthreads();
         bx = row_s;
-        by = at % part / gridDim.z;
-        bz = at % part % gridDim.z;
+        by = CLUSTER ? at % part : at % part / gridDim.z;
+        bz = CLUSTER ? blockIdx.z : at % part % gridDim.z;
     }
     const int group = a.nq / a.nkv, chunks = (group + 15) / 16, req = bx, kvh = by / chunks, r0 = by % chunks * 16;
     const int nrows = min(16, group - r0), head0 = kvh * group + r0;
@@ -589,6 +592,8 @@ template <int D, bool TMA>
 static int launch_mma(DecodeArgs a, int requests, bool cluster, int page_shift, const CUtensorMap& map, cudaStream_t stream) {
     const int group = a.nq / a.nkv, rows = group < 16 ? group : 16;
     const dim3 grid(requests, a.nkv * ((group + 15) / 16), a.splits);
+    const long blocks = (long)grid.x * grid.y * grid.z, places = 3L * sm_count();
+    a.longest_first = grid.x > 1 && grid.x <= THREADS && blocks > places && blocks <= (cluster ? 3 : 2) * places;
     if (cluster) {
         const size_t smem = tiles_bytes(D) + recv_bytes(rows, D, a.splits);
         if (!allow_smem<D, true, TMA>(smem)) {
@@ -617,8 +622,6 @@ static int launch_mma(DecodeArgs a, int requests, bool cluster, int page_shift, 
         set_error("attention_decode_weighed: cannot get %zu bytes of shared memory", smem);
         return 2;
     }
-    const long blocks = (long)grid.x * grid.y * grid.z, places = 3L * sm_count();
-    a.longest_first = grid.x > 1 && grid.x <= THREADS && blocks > places && blocks <= 2 * places;
     launch_pdl(decode_weighed_mma_kernel<D, false, TMA>, grid, dim3(THREADS), smem, stream, a, page_shift, map);
     return 0;
 }
@@ -682,6 +685,11 @@ static Plan plan_of(int requests, int nq, int nkv, int d, int max_len, int page_
             if (wave * 4 >= s * 5 && max_len >= 16384) return {wave, true, false};
             return {s, true, true};
         }
+    // A little more pairs than places, long rows: the second wave would run nearly empty, so two blocks share a pair, longest first.  Measured, us,
+    // one / two, 512 pairs of 128 on 444 places: 4,096 keys each 223 / 191, 100 to 8,000 199 / 166, 1,000 60 / 60, 250 to 1,750 54 / 58, 250 to 500 23 / 30;
+    // 800 pairs of 4,096 279 / 280.
+    if (chunks == 1 && max_len >= 4096 && pairs > places && 4 * pairs <= 5 * places && (d == 64 ? cluster_room<64>(rows, 2) : cluster_room<128>(rows, 2)) > 0)
+        return {2, true, true};
     // more pairs than clusters: just enough ranges to take every place, none under 768 keys
     long s = (places + pairs - 1) / pairs, most = max_len / 768;
     s = s < most ? s : most;

@@ -27,62 +27,87 @@ struct SelectArgs {
 constexpr int SELECT_MOST = 1024;          // threads of a block at most
 constexpr int SELECT_HELD = 48 * 1024;     // places whose ranks a block holds in shared memory; of longer rows they are worked out again a pass
 
-// One block a (layer, request, kv head).  The weights are read once, as ranks; the rank that the last kept weight has comes out eight bits a
-// pass (a histogram of the competing ranks that share the bits found so far, in shared memory; lanes that meet in a counter are added up by the
-// hardware, gathering them ahead with match costs more: 8.2 against 13.6 us for 64 rows of 4,096); then every warp counts what it keeps of its stretch
-// of the row, and writes it behind what the warps ahead keep.  What bounds it is the chain of passes, not the bytes.
+// One block a (layer, request, kv head); a warp has a stretch of the row.  The weights are read once, as ranks that a thread keeps in REGS registers
+// (0: rows of more than eight places a thread, in shared memory), and are asked for before the row's length has arrived.  The rank that the last kept weight has comes
+// out eight bits a pass (a histogram of the competing ranks that share the bits found so far, in shared memory; lanes that meet in a counter are added
+// up by the hardware), until a bin has no more than 32, which every warp then ranks by itself.  Then every warp counts what it
+// keeps of its stretch and writes it behind what the warps ahead keep.  What bounds it is the chain of reads and passes, not the bytes.
+template <int REGS>
 __global__ void __launch_bounds__(SELECT_MOST) select_keys_kernel(const SelectArgs a) {
-    extern __shared__ uint32_t rank_s[];                             // [min(max_length, SELECT_HELD)]
+    constexpr int P = REGS ? REGS : 4;
+    extern __shared__ uint32_t rank_s[];                             // [min(max_length, SELECT_HELD)] without registers
     __shared__ __align__(16) int hists[4][256];
     __shared__ int2 warp_s[32];
-    __shared__ uint32_t prefix_s;
-    __shared__ int need_s;
+    __shared__ uint32_t prefix_s, few_s[32];
+    __shared__ int need_s, bin_s, few;
     pdl_enter_small();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x, warps = threads >> 5;
     const int kvh = blockIdx.x % a.nkv, req = blockIdx.x / a.nkv % a.requests, layer = blockIdx.x / a.nkv / a.requests;
-    const int n = min(max(a.lengths[req], 0), a.max_length);
+    const int* table = a.block_table + (size_t)req * a.bt_stride;
+    const float* base = a.weights + ((size_t)layer * a.pages * a.nkv + kvh) * a.page_size;
+    const size_t page_stride = (size_t)a.nkv * a.page_size;
+    const int length = a.lengths[req];
+    float w[P];
+    uint32_t mine[P];
+    auto ask = [&](int j0, int step) {                               // the weights of P places; one without a page counts as the lightest
+        int page[P];
+#pragma unroll
+        for (int u = 0; u < P; ++u) page[u] = j0 + u * step < a.max_length ? table[(j0 + u * step) >> a.page_shift] : -1;
+#pragma unroll
+        for (int u = 0; u < P; ++u)
+            w[u] = page[u] >= 0 && page[u] < a.pages ? base[page[u] * page_stride + ((j0 + u * step) & (a.page_size - 1))] : -INFINITY;
+    };
+    if (REGS) ask(warp * (32 * P) + lane, 32);
+    for (int i = tid; i < 1024; i += threads) hists[0][i] = 0;
+    if (tid == 0) few = 0;
+    const int n = min(max(length, 0), a.max_length);
     int* out = a.kept + (size_t)blockIdx.x * a.keep;
     if (n <= a.keep) {
         for (int i = tid; i < a.keep; i += threads) out[i] = i < n ? i : -1;
         return;
     }
-    const int* table = a.block_table + (size_t)req * a.bt_stride;
-    const float* base = a.weights + ((size_t)layer * a.pages * a.nkv + kvh) * a.page_size;
-    const size_t page_stride = (size_t)a.nkv * a.page_size;
-    auto look = [&](int j) {
-        const int page = table[j >> a.page_shift];
-        return page >= 0 && page < a.pages ? rank_of(base[page * page_stride + (j & (a.page_size - 1))]) : 0u;
-    };
     const int wanted = a.keep - a.first - a.recent, lo = a.first, hi = n - a.recent;      // more than `wanted` places compete, [lo, hi)
-    const bool held = n <= SELECT_HELD;
-    for (int i = tid; i < 1024; i += threads) hists[0][i] = 0;
-    if (held && wanted > 0) {
-        for (int j0 = lo + tid; j0 < hi; j0 += 4 * threads) {
-            int page[4];
-            float w[4];
+    const bool held = REGS || n <= SELECT_HELD;
+    const int per = REGS ? 32 * P : (n + threads - 1) / threads * 32, beg = warp * per, end = min(n, beg + per);      // this warp's stretch
+    if (REGS) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) page[u] = j0 + u * threads < hi ? table[(j0 + u * threads) >> a.page_shift] : -1;
+        for (int u = 0; u < P; ++u) mine[u] = rank_of(w[u]);
+    } else if (held) {
+        for (int j0 = beg + lane; j0 < end; j0 += 32 * P) {
+            ask(j0, 32);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                w[u] = page[u] >= 0 && page[u] < a.pages ? base[page[u] * page_stride + ((j0 + u * threads) & (a.page_size - 1))] : -INFINITY;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (j0 + u * threads < hi) rank_s[j0 + u * threads] = rank_of(w[u]);
+            for (int u = 0; u < P; ++u)
+                if (j0 + 32 * u < end) rank_s[j0 + 32 * u] = rank_of(w[u]);
         }
+        __syncwarp();
     }
-    auto rank = [&](int j) { return held ? rank_s[j] : look(j); };
+    // f(place, rank) for this thread's places that compete
+    auto each = [&](auto f) {
+        if (REGS) {
+#pragma unroll
+            for (int u = 0; u < P; ++u) {
+                const int j = beg + 32 * u + lane;
+                if (j >= lo && j < hi) f(mine[u]);
+            }
+        } else
+            for (int j = beg + lane; j < end; j += 32) {
+                if (j < lo || j >= hi) continue;
+                if (held) f(rank_s[j]);
+                else {
+                    const int page = table[j >> a.page_shift];
+                    f(page >= 0 && page < a.pages ? rank_of(base[page * page_stride + (j & (a.page_size - 1))]) : rank_of(-INFINITY));
+                }
+            }
+    };
     uint32_t prefix = 0;
     int need = wanted;
+    __syncthreads();
     if (wanted > 0) {
         for (int shift = 24; shift >= 0; shift -= 8) {
             int* hist = hists[shift >> 3];
-            if (shift == 24) __syncthreads();
-            for (int j0 = lo + warp * 32; j0 < hi; j0 += threads) {
-                const int j = j0 + lane;
-                const uint32_t r = j < hi ? rank(j) : 0u;
-                const bool in = j < hi && (shift == 24 || r >> ((shift + 8) & 31) == prefix >> ((shift + 8) & 31));
-                if (in) atomicAdd(&hist[r >> shift & 255u], 1);
-            }
+            each([&](uint32_t r) {
+                if (shift == 24 || r >> ((shift + 8) & 31) == prefix >> ((shift + 8) & 31)) atomicAdd(&hist[r >> shift & 255u], 1);
+            });
             __syncthreads();
             if (warp == 0) {
                 // eight bins a lane, the highest with the first: the bin in which the count from above reaches what is needed
@@ -107,6 +132,7 @@ __global__ void __launch_bounds__(SELECT_MOST) select_keys_kernel(const SelectAr
                             const bool whole = need == above + c[i];
                             prefix_s = (prefix | (uint32_t)(top + 7 - i) << shift) - (whole ? 1u : 0u);
                             need_s = whole ? 0 : need - above;
+                            bin_s = c[i];
                             break;
                         }
                         above += c[i];
@@ -116,47 +142,77 @@ __global__ void __launch_bounds__(SELECT_MOST) select_keys_kernel(const SelectAr
             __syncthreads();
             prefix = prefix_s;
             need = need_s;
+            const int rest = bin_s;
             if (need == 0) break;
+            if (shift > 0 && rest <= 32) {
+                each([&](uint32_t r) {
+                    if (r >> shift == prefix >> shift) few_s[atomicAdd(&few, 1)] = r;
+                });
+                __syncthreads();
+                // the one of these with fewer than `need` above it and `need` or more up to it
+                const uint32_t r = few_s[lane];
+                int above = 0, upto = 0;
+                for (int i = 0; i < rest; ++i) {
+                    const uint32_t other = few_s[i];
+                    above += other > r;
+                    upto += other >= r;
+                }
+                const uint32_t last = __ballot_sync(0xffffffffu, lane < rest && above < need && need <= upto);
+                prefix = __shfl_sync(0xffffffffu, r, __ffs(last) - 1);
+                need -= __shfl_sync(0xffffffffu, above, __ffs(last) - 1);
+                break;
+            }
         }
     }
     // now `prefix` is the rank of the last kept weight and `need` how many of that rank are kept, the lowest places first (none: what is above it is kept)
-    const int per = (n + threads - 1) / threads * 32, beg = warp * per, end = min(n, beg + per);
-    auto kinds = [&](int j0, uint32_t& sure, uint32_t& tie) {
+    auto kinds = [&](int j0, uint32_t r, uint32_t& sure, uint32_t& tie) {
         const int j = j0 + lane;
-        bool s = false, t = false;
-        if (j < end) {
-            if (j < lo || j >= hi) s = true;
-            else if (wanted > 0) {
-                const uint32_t r = rank(j);
-                s = r > prefix;
-                t = r == prefix;
-            }
-        }
-        sure = __ballot_sync(0xffffffffu, s);
-        tie = __ballot_sync(0xffffffffu, t);
+        const bool in = j < end, fixed = j < lo || j >= hi;
+        sure = __ballot_sync(0xffffffffu, in && (fixed || (wanted > 0 && r > prefix)));
+        tie = __ballot_sync(0xffffffffu, in && !fixed && wanted > 0 && r == prefix);
+    };
+    auto rank = [&](int j) {
+        if (j >= end) return 0u;
+        if (held) return rank_s[j];
+        const int page = table[j >> a.page_shift];
+        return page >= 0 && page < a.pages ? rank_of(base[page * page_stride + (j & (a.page_size - 1))]) : rank_of(-INFINITY);
     };
     int sures = 0, ties = 0;
-    for (int j0 = beg; j0 < end; j0 += 32) {
-        uint32_t s, t;
-        kinds(j0, s, t);
-        sures += __popc(s);
-        ties += __popc(t);
-    }
+    uint32_t sure[P], tie[P];
+    if (REGS) {
+#pragma unroll
+        for (int u = 0; u < P; ++u) {
+            kinds(beg + 32 * u, mine[u], sure[u], tie[u]);
+            sures += __popc(sure[u]);
+            ties += __popc(tie[u]);
+        }
+    } else
+        for (int j0 = beg; j0 < end; j0 += 32) {
+            kinds(j0, rank(j0 + lane), sure[0], tie[0]);
+            sures += __popc(sure[0]);
+            ties += __popc(tie[0]);
+        }
     if (lane == 0) warp_s[warp] = make_int2(sures, ties);
     __syncthreads();
-    int2 before = lane < warps && lane < warp ? warp_s[lane] : make_int2(0, 0);
+    const int2 before = lane < warps && lane < warp ? warp_s[lane] : make_int2(0, 0);
     int at_sure = __reduce_add_sync(0xffffffffu, before.x), at_tie = __reduce_add_sync(0xffffffffu, before.y);
     const uint32_t ahead = (1u << lane) - 1u;
-    for (int j0 = beg; j0 < end; j0 += 32) {
-        uint32_t s, t;
-        kinds(j0, s, t);
+    auto put = [&](int j0, uint32_t s, uint32_t t) {
         const int tb = at_tie + __popc(t & ahead);
-        const bool mine = (s >> lane & 1u) || ((t >> lane & 1u) && tb < need);
+        const bool kept = (s >> lane & 1u) || ((t >> lane & 1u) && tb < need);
         const int at = at_sure + __popc(s & ahead) + min(tb, need);
-        if (mine && at < a.keep) out[at] = j0 + lane;
+        if (kept && at < a.keep) out[at] = j0 + lane;
         at_sure += __popc(s);
         at_tie += __popc(t);
-    }
+    };
+    if (REGS) {
+#pragma unroll
+        for (int u = 0; u < P; ++u) put(beg + 32 * u, sure[u], tie[u]);
+    } else
+        for (int j0 = beg; j0 < end; j0 += 32) {
+            kinds(j0, rank(j0 + lane), sure[0], tie[0]);
+            put(j0, sure[0], tie[0]);
+        }
 }
 
 struct MoveArgs {
@@ -280,7 +336,7 @@ LILY_API int lily_select_keys(const float* weights, const int* block_table, int 
     while (1 << a.page_shift < page_size) ++a.page_shift;
     static bool configured = false;
     if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(budget::select_keys_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, budget::SELECT_HELD * 4);
+        const cudaError_t e = cudaFuncSetAttribute(budget::select_keys_kernel<0>, cudaFuncAttributeMaxDynamicSharedMemorySize, budget::SELECT_HELD * 4);
         LILY_REQUIRE(e == cudaSuccess, "select_keys: cannot get %d bytes of shared memory: %s", budget::SELECT_HELD * 4, cudaGetErrorString(e));
         configured = true;
     }
@@ -288,7 +344,9 @@ LILY_API int lily_select_keys(const float* weights, const int* block_table, int 
     int threads = 128;
     while (threads < budget::SELECT_MOST && threads * 4 < max_length && rows * threads * 2 <= 2048LL * sm_count()) threads *= 2;
     const size_t smem = (size_t)(max_length < budget::SELECT_HELD ? max_length : budget::SELECT_HELD) * 4;
-    launch_pdl(budget::select_keys_kernel, dim3((unsigned)rows), dim3(threads), smem, stream, a);
+    if (max_length <= 4 * threads) launch_pdl(budget::select_keys_kernel<4>, dim3((unsigned)rows), dim3(threads), 0, stream, a);
+    else if (max_length <= 8 * threads) launch_pdl(budget::select_keys_kernel<8>, dim3((unsigned)rows), dim3(threads), 0, stream, a);
+    else launch_pdl(budget::select_keys_kernel<0>, dim3((unsigned)rows), dim3(threads), smem, stream, a);
     LILY_CHECK_LAUNCH("select_keys");
     return 0;
 }

@@ -1210,6 +1210,10 @@ def attention_decode_fused(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_
 
 # ------------------------------------------------------------------------------ a cache held to a budget of places
 
+_f32, _i32_dtype = torch.float32, torch.int32
+_codes = {torch.float32: _F32, torch.bfloat16: _BF16}
+
+
 def pair_axes(sections: Sequence[int], device, in_turn: bool = False) -> torch.Tensor:
     """The axis of each rotated pair, int32 [sum(sections)]: ``sections[a]`` pairs belong to axis a, in runs (16, 24, 24: sixteen
     pairs by time, 24 by height, 24 by width) or, ``in_turn``, one after the other (0, 1, 2, 0, 1, 2, ...) while an axis has pairs left."""
@@ -1251,37 +1255,41 @@ def axes_rope_write(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_gain: O
     (nq + 2 nkv) d] in the cache's dtype or float32 partial sums [splits, tokens, ...], its rows ``row`` numbers apart.  A position outside the
     tables gives NaN; a place outside the block table is not written."""
     _dev(qkv, q_gain, k_gain, cos, sin, positions, pair_axis, places, token_req, block_table, kv_layer, q_out)
-    ld = int(row or (nq + 2 * nkv) * d)
-    shape, pages, dtype, half = qkv.shape, kv_layer.shape, kv_layer.dtype, rotary_dim // 2
-    n = shape[-2]
-    splits, stride = (1, 0) if len(shape) == 2 and shape[1] == ld else _summed(qkv, n, ld, "axes_rope_write qkv")
-    if qkv.dtype is not dtype and qkv.dtype is not torch.float32:
-        raise KernelError(f"axes_rope_write: cache dtype {dtype} differs from activations {qkv.dtype}")
+    ld = row or (nq + 2 * nkv) * d
+    shape, pages, rows, axes, width = qkv.shape, kv_layer.shape, cos.shape, positions.shape, block_table.shape
+    dtype, of, half = kv_layer.dtype, qkv.dtype, rotary_dim // 2
+    code, n = _codes.get(dtype), shape[-2]
+    if len(shape) == 2 and shape[1] == ld:
+        splits, stride = 1, 0
+        if of is not dtype and of is not _f32:
+            raise KernelError(f"axes_rope_write: cache dtype {dtype} differs from activations {of}")
+    else:
+        splits, stride = _summed(qkv, n, ld, "axes_rope_write qkv")
+    if code is None:
+        raise KernelError(f"kernels take float32 or bfloat16 tensors, got {dtype}")
     if pages[1:] != (2, nkv, page_size, d):
         cache_layer_fits(kv_layer, nkv, page_size, d, d)
-    rows = cos.shape
-    if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or len(rows) != 2 or rows[1] != half or sin.shape != rows:
+    if cos.dtype is not _f32 or sin.dtype is not _f32 or len(rows) != 2 or rows[1] != half or sin.shape != rows:
         raise KernelError("axes_rope_write: rotation tables are float32 [positions, rotary_dim / 2]")
-    axes, width = positions.shape, block_table.shape
     if len(axes) != 2 or axes[1] != n or pair_axis.numel() != half:
         raise KernelError(f"axes_rope_write: positions are [axes, {n}] and there is an axis for each of the {half} pairs; got {tuple(axes)} and {pair_axis.numel()}")
     if places.numel() != n or token_req.numel() != n or len(width) != 2 or width[1] < 1:
         raise KernelError(f"axes_rope_write: {n} tokens have a place and a request each")
-    for t, name in ((positions, "positions"), (pair_axis, "pair_axis"), (places, "places"), (token_req, "token_req"), (block_table, "block_table")):
-        if t.dtype is not torch.int32:
-            raise KernelError(f"{name} must be int32, got {t.dtype}")
-    gains = (None, None, _F32)
+    if not (positions.dtype is pair_axis.dtype is places.dtype is token_req.dtype is block_table.dtype is _i32_dtype):
+        for t, name in ((positions, "positions"), (pair_axis, "pair_axis"), (places, "places"), (token_req, "token_req"), (block_table, "block_table")):
+            _i32(t, name)
+    q_at, k_at, gain = None, None, _F32
     if q_gain is not None or k_gain is not None:
         if q_gain is None or k_gain is None or q_gain.dtype is not k_gain.dtype or q_gain.numel() != d or k_gain.numel() != d:
             raise KernelError("axes_rope_write: q and k gains come together, with one dtype and head_dim numbers each")
-        gains = (q_gain.data_ptr(), k_gain.data_ptr(), _dt(q_gain))
+        q_at, k_at, gain = q_gain.data_ptr(), k_gain.data_ptr(), _dt(q_gain)
     if q_out is None:
         q_out = kv_layer.new_empty((n, nq * d))
     elif q_out.dtype is not dtype or q_out.numel() != n * nq * d:
         raise KernelError("axes_rope_write: q_out is [tokens, nq * d] in the cache's dtype")
-    _call("lily_axes_rope_write", qkv.data_ptr(), _dt(qkv), splits, stride, ld, *gains, eps, cos.data_ptr(), sin.data_ptr(), rows[0], positions.data_ptr(),
+    _call("lily_axes_rope_write", qkv.data_ptr(), _codes[of], splits, stride, ld, q_at, k_at, gain, eps, cos.data_ptr(), sin.data_ptr(), rows[0], positions.data_ptr(),
           pair_axis.data_ptr(), axes[0], n, places.data_ptr(), token_req.data_ptr(), block_table.data_ptr(), width[1], kv_layer.data_ptr(), pages[0],
-          q_out.data_ptr(), _dt(kv_layer), nq, nkv, d, rotary_dim, page_size, _stream())
+          q_out.data_ptr(), code, nq, nkv, d, rotary_dim, page_size, _stream())
     return q_out
 
 
