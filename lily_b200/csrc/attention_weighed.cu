@@ -3,8 +3,8 @@
 // For a request of n cached places (the newest token's own among them) and the query heads h of a kv head g:
 //   p_hj = exp(c q_h . k_j - lse_h),  o_h = sum_j p_hj v_j,  w_gj <- (j < n - 1 ? w_gj : 0) + sum_h p_hj,
 // with w float32 [pages, kv_heads, page_size] beside the keys: the newest place's weight is set, whatever an earlier owner left there.
-// The keys of a request are cut into ranges; a block leaves its scores (in units of log2 e) and its (max, sum, output) in scratch, and a
-// second kernel, which knows every range's, writes outputs and weights.
+// The keys of a request are cut into ranges of a block each.  A key's weight needs the row's (max, sum) over all ranges, so scores are kept in scratch (in
+// units of log2 e) and read again when that is known: from the blocks of a cluster, or by a second kernel that joins what the ranges left.
 #include "attention_args.cuh"
 #include "common.cuh"
 #include "tcgen05.cuh"
@@ -655,11 +655,19 @@ static int cluster_room(int rows, int splits) {
 struct Plan { int splits; bool mma, cluster; };
 
 // How the keys are cut; a function of the sizes alone.
+// Which kernel takes a call, and how many ranges.  Measured, us, bfloat16 heads of 128, 32 over 8 where not said:
+//   tensor cores / CUDA cores: eight rows of 4,096 keys 29 / 428 (heads of 64: 16 / 232), one of 900, 16 over 4, 6.3 / 57; float32, the kernel that cuts a row over
+//   warps / the tiles: three rows 15 / 69 at best, 32 of 2,000 114 / 1,656.  Tiles by TMA / piece by piece: 29.4 / 30.9, heads of 64 15.5 / 17.7.
+//   clusters as long as they fit at once, the longest first: one row of 4,096 in 16 blocks 10.4, 8 11.3, 4 18, in 16 ranges with the second kernel 11.9; eight rows in 4 or 6
+//   29.2, 8 34.6, 16 43.7, 16 ranges 31.9; four of 2,000 in 8 10.6, 4 13.7;
+//   a wave of ranges from 16,384 keys on where it has a quarter more blocks: one row of 16,384 48 ranges 20, a cluster of 16 24; of 65,536 57 and 83.
+//   rows that would not all run at once go by length where they differ: 64 of 250 to 1,750 keys 54.6 / 58.9 as they come.
 static Plan plan_of(int requests, int nq, int nkv, int d, int max_len, int page_size, int dtype) {
     const int group = nq / nkv, sms = sm_count();
     const bool mma = dtype == kBF16 && (d == 64 || d == 128) && page_size >= 4 && (page_size & (page_size - 1)) == 0;
     if (dtype == kF32 && group <= 8 && d % 4 == 0 && d <= 256) {
-        // the kernel that cuts a row's keys over the warps of a block: a wave of blocks, none under 64 keys
+        // the kernel that cuts a row's keys over the warps of a block: a wave of blocks, none under 64 keys (three rows of up to 2,900 keys, 16 heads
+        // over 4: 6 ranges 20.2 us, 12, a wave, 15.1, 24 17.3; 32 rows of 2,000 over 8: 1 range 114, 2 and 4 121)
         const long pairs = (long)requests * nkv, most = (max_len + 63) / 64;
         long s = sms / pairs;
         s = s < most ? s : most;

@@ -94,9 +94,10 @@ __global__ void __launch_bounds__(128) axes_rope_write_kernel(const Args a) {
 
 // Sixteen bytes of activations an access (N = 8 bfloat16 or 4 float32 numbers) and G = d / (2 N) threads a head (a power of two, at most a
 // warp), each with two pieces: of the rotated features N neighbouring ones and their partners rd / 2 further, of the rest two neighbouring pieces.  So the
-// rotation needs no exchange, the norm log2(G) shuffles, and no thread waits for another.  The positions of up to four axes are read
-// beside the axes of a thread's pairs, not behind them; where its pairs share an axis their cosines and sines are 16-byte reads.  What bounds it is the chain
-// of reads (axis and positions, tables, result), for few tokens and for many, which small blocks of short-lived threads hide best.
+// rotation needs no exchange and the norm log2(G) shuffles.  The positions of up to four axes are read
+// beside the axes of a thread's pairs, not behind them.  What bounds it is the chain of reads (axis and positions, tables, result), for few tokens
+// and for many, which small blocks of short-lived threads hide best: 2,048 tokens of 32 + 2 x 8 heads of 128 in bfloat16 take 15.1 us (51 MB: 3.4 TB/s; a
+// plain copy of as many bytes 9.3), eight tokens out of four planes of partial sums 3.1.
 constexpr int WIDE_THREADS = 128, AHEAD = 4;
 
 // Numbers in pairs (mul and fma.rn.f32x2: two IEEE operations an instruction).
@@ -185,19 +186,23 @@ __device__ __forceinline__ void store_piece(T* dst, const Two (&v)[N / 2]) {
     } else *reinterpret_cast<ulonglong2*>(dst) = make_ulonglong2(v[0], v[1]);
 }
 
-// The tables' numbers of N pairs from `j` on.
+// The tables' numbers of N pairs from `j` on, for the lanes of a warp that `need` them (of one token, `mine`: shared memory of the warp's, room for
+// two rows of the tables).  Where each lane's pairs share an axis they are 16-byte reads; else the warp brings each pair of the token once, side by side, and
+// hands them round through shared memory (axes in turn, 2,048 tokens: 15.3 us; a read a pair and thread took 20.7).
 template <int N>
-__device__ __forceinline__ void load_turn(const Args& a, int n, int j, Two (&c)[N / 2], Two (&s)[N / 2]) {
+__device__ __forceinline__ void load_turn(const Args& a, int n, int j, bool need, float* mine, Two (&c)[N / 2], Two (&s)[N / 2]) {
     const int half = a.rd / 2;
-    int pos[4], axis[N];
+    int pos[4], axis = -1;
 #pragma unroll
     for (int k = 0; k < 4; ++k) pos[k] = k < a.axes ? a.positions[(size_t)k * a.tokens + n] : -1;
     bool alike = true;
+    if (need) {
 #pragma unroll
-    for (int i = 0; i < N; i += 4) {
-        const int4 t = *reinterpret_cast<const int4*>(a.pair_axis + j + i);
-        axis[i] = t.x, axis[i + 1] = t.y, axis[i + 2] = t.z, axis[i + 3] = t.w;
-        alike = alike && t.x == axis[0] && t.y == t.x && t.z == t.x && t.w == t.x;
+        for (int i = 0; i < N; i += 4) {
+            const int4 t = *reinterpret_cast<const int4*>(a.pair_axis + j + i);
+            if (i == 0) axis = t.x;
+            alike = alike && t.x == axis && t.y == axis && t.z == axis && t.w == axis;
+        }
     }
     auto position = [&](int ax) {
         int at = ax == 0 ? pos[0] : ax == 1 ? pos[1] : ax == 2 ? pos[2] : ax == 3 ? pos[3] : -1;
@@ -205,8 +210,9 @@ __device__ __forceinline__ void load_turn(const Args& a, int n, int j, Two (&c)[
         return at < a.table_rows ? at : -1;
     };
     const float nan = __int_as_float(0x7fffffff);
-    if (alike) {
-        const int at = position(axis[0]);
+    if (__all_sync(0xffffffffu, alike)) {
+        if (!need) return;
+        const int at = position(axis);
 #pragma unroll
         for (int i = 0; i < N / 4; ++i) {
             ulonglong2 x = make_ulonglong2(two(nan, nan), two(nan, nan)), y = x;
@@ -216,16 +222,19 @@ __device__ __forceinline__ void load_turn(const Args& a, int n, int j, Two (&c)[
             }
             c[2 * i] = x.x, c[2 * i + 1] = x.y, s[2 * i] = y.x, s[2 * i + 1] = y.y;
         }
-    } else {
-        float x[N], y[N];
+        return;
+    }
+    for (int p = threadIdx.x & 31; p < half; p += 32) {
+        const int at = position(a.pair_axis[p]);
+        mine[p] = at >= 0 ? a.cos_t[(size_t)at * half + p] : nan;
+        mine[half + p] = at >= 0 ? a.sin_t[(size_t)at * half + p] : nan;
+    }
+    __syncwarp();
+    if (!need) return;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int at = position(axis[i]);
-            x[i] = at >= 0 ? a.cos_t[(size_t)at * half + j + i] : nan;
-            y[i] = at >= 0 ? a.sin_t[(size_t)at * half + j + i] : nan;
-        }
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i) c[i] = two(x[2 * i], x[2 * i + 1]), s[i] = two(y[2 * i], y[2 * i + 1]);
+    for (int i = 0; i < N / 4; ++i) {
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(mine + j + 4 * i), y = *reinterpret_cast<const ulonglong2*>(mine + half + j + 4 * i);
+        c[2 * i] = x.x, c[2 * i + 1] = x.y, s[2 * i] = y.x, s[2 * i + 1] = y.y;
     }
 }
 
@@ -233,10 +242,12 @@ __device__ __forceinline__ void load_turn(const Args& a, int n, int j, Two (&c)[
 template <typename T, typename IN, typename W>
 __global__ void __launch_bounds__(WIDE_THREADS, 8) axes_rope_write_wide_kernel(const Args a, const int group_shift) {
     constexpr int N = 16 / sizeof(T);
+    extern __shared__ __align__(16) float turns_s[];                 // [warps][rd]
     pdl_enter_small();
     const int n = blockIdx.x, tid = threadIdx.x, half = a.rd / 2, group = 1 << group_shift;
-    const int head = (blockIdx.y * WIDE_THREADS + tid) >> group_shift, t = tid & (group - 1);
-    if (head >= a.nq + 2 * a.nkv) return;
+    const int most = a.nq + 2 * a.nkv - 1, asked = (blockIdx.y * WIDE_THREADS + tid) >> group_shift, t = tid & (group - 1);
+    if ((blockIdx.y * WIDE_THREADS + (tid & ~31)) >> group_shift > most) return;
+    const int head = min(asked, most);                               // (a warp's threads behind the last head follow it and write nothing)
     const bool value = head >= a.nq + a.nkv;
     // this thread's two pieces
     const bool turned = t * N < half;
@@ -253,8 +264,8 @@ __global__ void __launch_bounds__(WIDE_THREADS, 8) axes_rope_write_wide_kernel(c
     uint4 raw_gx, raw_gy;
     if constexpr (sizeof(W) == 2 && N == 8)
         if (gain) raw_gx = *reinterpret_cast<const uint4*>(gain + i0), raw_gy = *reinterpret_cast<const uint4*>(gain + i1);
-    if (!value && turned) load_turn<N>(a, n, i0, c, s);
-    T* dst = target<T>(a, n, head);
+    load_turn<N>(a, n, i0, !value && turned, turns_s + (tid >> 5) * a.rd, c, s);
+    T* dst = asked > most ? nullptr : target<T>(a, n, head);
     if constexpr (sizeof(IN) == 2) {
         unpack<IN, N>(raw_x, x);
         unpack<IN, N>(raw_y, y);
@@ -320,13 +331,15 @@ LILY_API int lily_axes_rope_write(const void* qkv, int in_dtype, int splits, siz
     while (1 << shift < group) ++shift;
     const uintptr_t where = (uintptr_t)qkv | (uintptr_t)kv | (uintptr_t)q_out | (uintptr_t)q_gain | (uintptr_t)k_gain |
                             (uintptr_t)cos_t | (uintptr_t)sin_t | (uintptr_t)pair_axis;
-    // whole pieces of 16 bytes on every side; else, and for heads that are no power of two of pieces, a warp a head
+    // Whole pieces of 16 bytes on every side; else, and for heads that are no power of two of pieces, a warp a head.  Measured, us, in pieces / a warp a
+    // head, on the same operands: 2,048 tokens of 48 heads of 128 in bfloat16 13.1 / 35.6 (axes in turn 15.3 / 35.3), eight tokens from four planes 3.1 / 5.4;
+    // float32, 1,000 tokens of 24 heads of 128 with half of each turned 7.9 / 8.4, of 64 5.1 / 7.9.
     const bool wide = d % (2 * piece) == 0 && 1 << shift == group && group <= 32 && rd % (2 * piece) == 0 && ld % piece == 0 &&
                       (in_dtype == act_dtype || ld % 4 == 0) && (size_t)stride % 4 == 0 && where % 16 == 0;
     const dim3 grid = wide ? dim3(tokens, (unsigned)((((nq + 2 * nkv) << shift) + axes::WIDE_THREADS - 1) / axes::WIDE_THREADS)) : dim3(tokens, (nq + 2 * nkv + 3) / 4);
 #define LAUNCH(T, IN, W)                                                                                                        \
     do {                                                                                                                        \
-        if (wide) launch_pdl(axes::axes_rope_write_wide_kernel<T, IN, W>, grid, dim3(axes::WIDE_THREADS), 0, stream, a, shift); \
+        if (wide) launch_pdl(axes::axes_rope_write_wide_kernel<T, IN, W>, grid, dim3(axes::WIDE_THREADS), axes::WIDE_THREADS / 32 * rd * sizeof(float), stream, a, shift); \
         else launch_pdl(axes::axes_rope_write_kernel<T, IN, W>, grid, dim3(128), 0, stream, a);                                 \
     } while (0)
     const bool ib = in_dtype == kBF16, gb = gain_dtype == kBF16;

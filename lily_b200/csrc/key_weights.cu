@@ -89,7 +89,8 @@ __device__ __forceinline__ float4 four(const T* row, int c, int d) {
 // A tile of scores a block (kv heads, row tiles, key tiles of each request, numbered through).  A thread has the 4 x 4 of rows ty + 16 i and keys tx + 16 j, so that the
 // rows of both tiles lie in shared memory as they come (36 numbers a row of 32: no two lanes meet in a bank) and products are packed pairs along the
 // head; the 32 products of a chunk are added up by themselves, which quarters the error of a long sum of like terms.  The next chunk is on its way
-// while one is multiplied.  What bounds it are the multiply-adds.
+// while one is multiplied.  What bounds it are the reads of shared memory (a warp waits for them 2.6 cycles of 6.7; the multiply-adds' unit is busy 46 % of the
+// time): 2,048 tokens of 32 heads of 128 take 666 us, 27 TFLOP/s; 8 x 4 a thread gave 608, and more for few tokens (13.3 us became 14.2).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) key_weights_scores_kernel(const __grid_constant__ Args a) {
     __shared__ __align__(16) float q_s[TM][LD], k_s[TN][LD];
@@ -191,9 +192,9 @@ __global__ void __launch_bounds__(TM) key_weights_lse_kernel(const __grid_consta
 }
 
 // grid (tiles of keys, parts): the sums of a tile's columns, four a thread over every 32nd row.  What bounds it is the chain of
-// reads: the parts, a cluster of up to eight blocks, take turns at the tiles of rows, eight rows a thread on their way, and the first adds up what all have
+// reads: the parts, a cluster of up to four blocks, take turns at the tiles of rows, eight rows a thread on their way, and the first adds up what all have
 // found, in their order.
-constexpr int COL_THREADS = 512, COL_PARTS = 8;
+constexpr int COL_THREADS = 512, COL_PARTS = 4;
 __global__ void __launch_bounds__(COL_THREADS) key_weights_columns_kernel(const __grid_constant__ Args a) {
     __shared__ __align__(16) float sum_s[32][TN];
     __shared__ float parts_s[COL_PARTS][TN];
@@ -344,6 +345,7 @@ LILY_API int lily_key_weights(const void* q, const void* kv, float* weights, con
     a.q = q; a.kv = kv; a.weights = weights; a.scores = scratch; a.block_table = block_table; a.bt_stride = bt_stride; a.nq = nq; a.nkv = nkv; a.d = d;
     a.page_size = page_size; a.scale = scale;
     while (1 << a.page_shift < page_size) ++a.page_shift;
+    // (reads of four numbers, or of one where rows are not aligned for it: 106 and 115 us for 1,000 tokens of 16 heads of 128)
     const bool vec = d % 4 == 0 && (((uintptr_t)q | (uintptr_t)kv) & 15) == 0;
     const int rc = keyw::each_run(a, requests, prefix, fresh, observe, [&](const keyw::Tiles& t) {
         LILY_REQUIRE(t.scores <= 0x7fffffff, "attention_key_weights: %lld tiles", t.scores);
@@ -355,7 +357,8 @@ LILY_API int lily_key_weights(const void* q, const void* kv, float* weights, con
         else { if (vec) LAUNCH(__nv_bfloat16, true); else LAUNCH(__nv_bfloat16, false); }
 #undef LAUNCH
         launch_pdl(keyw::key_weights_lse_kernel, dim3((unsigned)t.rows), dim3(keyw::TM), 0, stream, a);
-        // four tiles of rows a block or more
+        // four tiles of rows a block or more (us, float32, 16 heads of 128 over 4, in 1 / 2 / 4 / 8 parts: 1,000 tokens 113 / 102 / 102 / 106, 200 tokens 22 / 19 / 18 / 20,
+        // 64 behind 4,000 places 51 / 57 / 66 / 89)
         int tiles = 0;
         for (int r = 0; r < a.requests; ++r) tiles = a.p[r].row_tiles > tiles ? a.p[r].row_tiles : tiles;
         int parts = tiles / 4;
