@@ -195,7 +195,7 @@ def main() -> None:
     ap.add_argument("--image", action="store_true")
     args = ap.parse_args()
     for keep in (None, args.keep):
-        measure(argparse.Namespace(**{**vars(args), "prompt": 2 * args.page, "steps": 4}), keep)        # libraries and kernels set themselves up
+        measure(argparse.Namespace(**{**vars(args), "prompt": min(args.prompt, args.portion), "steps": 4}), keep)        # libraries and kernels set themselves up
         print(json.dumps(measure(args, keep)))
 
 

@@ -9,6 +9,11 @@ be written (a read-only checkout) a per-user folder under the temporary director
 The first call in a fresh checkout compiles (a line is printed as each file starts and ends);
 there is no fallback: without ``nvcc`` or without the library every kernel call raises.
 
+One part is not plain C: ``faces.cpp``, a Python extension that looks at tensors, checks and launches for
+operators whose small calls are shorter than a face in Python.  It is compiled (by nvcc's host compiler) against
+torch's headers, lies beside the library (its name also says for which torch and Python), and is given the
+library's addresses when it is loaded.
+
 Plays the role of lily/layers/quantization/cuda_ops.py:27-65 (JIT build of lily/csrc), except
 that a failed build there makes callers fall back to PyTorch and here it is an error.
 """
@@ -137,6 +142,39 @@ def build(verbose: bool = True) -> str:
     _run([nvcc, "-shared", "-o", tmp, *objects], "linking")
     os.replace(tmp, lib)
     return lib
+
+
+FACES = "faces.cpp"
+FACES_FLAGS = ["-O2", "-std=c++17", "-shared", "-cudart", "none", "-Xcompiler", "-fPIC,-fvisibility=hidden"]
+
+
+def build_faces() -> str:
+    """Compiles ``faces.cpp`` where it is missing and returns the path of the extension.  By nvcc, so by the host compiler that
+    the kernels' launchers have: one that brought a C++ runtime of its own into the process could not throw through torch's."""
+    import sysconfig
+    import torch
+    src, abi = os.path.join(HERE, FACES), f"-D_GLIBCXX_USE_CXX11_ABI={torch._C._GLIBCXX_USE_CXX11_ABI:d}"
+    lib = os.path.join(_build_dir(), f"lily_faces_{_digest([src], ' '.join([*FACES_FLAGS, abi, torch.__version__, sys.version]))}.so")
+    if os.path.isfile(lib):
+        return lib
+    folder = os.path.dirname(torch.__file__)
+    headers = [os.path.join(folder, "include"), os.path.join(folder, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"]]
+    tmp = f"{lib}.{os.getpid()}.tmp"
+    _run([find_nvcc(), *FACES_FLAGS, abi, *[f"-I{h}" for h in headers], src, "-o", tmp, "-L" + os.path.join(folder, "lib"),
+          "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"], f"compiling {FACES}")
+    os.replace(tmp, lib)
+    return lib
+
+
+def load_faces():
+    """The extension module of ``faces.cpp``; built first when needed.  Its caller binds it to the library."""
+    import importlib.machinery
+    import importlib.util
+    with _LOCK:
+        loader = importlib.machinery.ExtensionFileLoader("lily_faces", build_faces())
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("lily_faces", loader))
+        loader.exec_module(module)
+        return module
 
 
 _LIB: Optional[ctypes.CDLL] = None

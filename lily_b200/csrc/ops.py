@@ -98,13 +98,6 @@ _SIGNATURES = {
     "lily_moe_gather": [_vp, _i, _vp, _i, _vp, _i, _i, _vp, _vp],
     "lily_moe_activation": [_vp, _i, _i, _vp, _i, _f, _f, _vp, _vp, _i, _vp, _vp],
     "lily_moe_relu2": [_vp, _i, _i, _vp, _vp, _vp, _i, _vp, _vp],
-    "lily_axes_rope_write": [_vp, _i, _i, _sz, _i, _vp, _vp, _i, _f, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _vp,
-                             _i, _i, _i, _i, _i, _i, _vp],
-    "lily_attention_decode_weighed": [_vp, _vp, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp],
-    "lily_key_weights": [_vp, _vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _vp],
-    "lily_key_weights_tc": [_vp, _i, _vp, _i, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp],
-    "lily_select_keys": [_vp, _vp, _i, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
-    "lily_move_keys": [_vp, _vp, _vp, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp],
     "lily_argmax": [_vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_apply_penalties": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_top_logprobs": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
@@ -144,12 +137,6 @@ def library():
         lib.lily_attention_decode_scratch_floats.restype = _sz
         lib.lily_attention_decode_weighed_floats.argtypes = [_i, _i, _i, _i, _i, _i, _i]
         lib.lily_attention_decode_weighed_floats.restype = _sz
-        lib.lily_key_weights_floats.argtypes = [_i, _vp, _vp, _i, _i, _i]
-        lib.lily_key_weights_floats.restype = _sz
-        lib.lily_key_weights_tc_floats.argtypes = [_i, _vp, _vp, _i, _i, _i]
-        lib.lily_key_weights_tc_floats.restype = _sz
-        lib.lily_key_weights_tc_takes.argtypes = [_i, _i, _i, _i, _f]
-        lib.lily_key_weights_tc_takes.restype = _i
         lib.lily_key_weights_status.restype = _i
         lib.lily_normed_mean_max.restype = _i
         lib.lily_row_cluster_threads.argtypes = [_i]
@@ -1210,8 +1197,19 @@ def attention_decode_fused(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_
 
 # ------------------------------------------------------------------------------ a cache held to a budget of places
 
-_f32, _i32_dtype = torch.float32, torch.int32
-_codes = {torch.float32: _F32, torch.bfloat16: _BF16}
+_module = None
+
+
+def _faces():
+    """The extension that checks the arguments of these operators and launches them, bound to the kernels (csrc/faces.cpp)."""
+    global _module
+    if _module is None:
+        module, lib = _build.load_faces(), library()
+        names = ("lily_last_error", "lily_axes_rope_write", "lily_attention_decode_weighed_floats", "lily_attention_decode_weighed", "lily_select_keys", "lily_move_keys",
+                 "lily_key_weights", "lily_key_weights_floats", "lily_key_weights_tc", "lily_key_weights_tc_floats", "lily_key_weights_tc_takes")
+        module.bind(KernelError, *[ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names])
+        _module = module
+    return _module
 
 
 def pair_axes(sections: Sequence[int], device, in_turn: bool = False) -> torch.Tensor:
@@ -1254,43 +1252,10 @@ def axes_rope_write(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_gain: O
     ``q_out`` [tokens, nq * d], k and v to ``places[token]`` of the pages of request ``token_req[token]``.  ``qkv`` is [tokens,
     (nq + 2 nkv) d] in the cache's dtype or float32 partial sums [splits, tokens, ...], its rows ``row`` numbers apart.  A position outside the
     tables gives NaN; a place outside the block table is not written."""
-    _dev(qkv, q_gain, k_gain, cos, sin, positions, pair_axis, places, token_req, block_table, kv_layer, q_out)
-    ld = row or (nq + 2 * nkv) * d
-    shape, pages, rows, axes, width = qkv.shape, kv_layer.shape, cos.shape, positions.shape, block_table.shape
-    dtype, of, half = kv_layer.dtype, qkv.dtype, rotary_dim // 2
-    code, n = _codes.get(dtype), shape[-2]
-    if len(shape) == 2 and shape[1] == ld:
-        splits, stride = 1, 0
-        if of is not dtype and of is not _f32:
-            raise KernelError(f"axes_rope_write: cache dtype {dtype} differs from activations {of}")
-    else:
-        splits, stride = _summed(qkv, n, ld, "axes_rope_write qkv")
-    if code is None:
-        raise KernelError(f"kernels take float32 or bfloat16 tensors, got {dtype}")
-    if pages[1:] != (2, nkv, page_size, d):
-        cache_layer_fits(kv_layer, nkv, page_size, d, d)
-    if cos.dtype is not _f32 or sin.dtype is not _f32 or len(rows) != 2 or rows[1] != half or sin.shape != rows:
-        raise KernelError("axes_rope_write: rotation tables are float32 [positions, rotary_dim / 2]")
-    if len(axes) != 2 or axes[1] != n or pair_axis.numel() != half:
-        raise KernelError(f"axes_rope_write: positions are [axes, {n}] and there is an axis for each of the {half} pairs; got {tuple(axes)} and {pair_axis.numel()}")
-    if places.numel() != n or token_req.numel() != n or len(width) != 2 or width[1] < 1:
-        raise KernelError(f"axes_rope_write: {n} tokens have a place and a request each")
-    if not (positions.dtype is pair_axis.dtype is places.dtype is token_req.dtype is block_table.dtype is _i32_dtype):
-        for t, name in ((positions, "positions"), (pair_axis, "pair_axis"), (places, "places"), (token_req, "token_req"), (block_table, "block_table")):
-            _i32(t, name)
-    q_at, k_at, gain = None, None, _F32
-    if q_gain is not None or k_gain is not None:
-        if q_gain is None or k_gain is None or q_gain.dtype is not k_gain.dtype or q_gain.numel() != d or k_gain.numel() != d:
-            raise KernelError("axes_rope_write: q and k gains come together, with one dtype and head_dim numbers each")
-        q_at, k_at, gain = q_gain.data_ptr(), k_gain.data_ptr(), _dt(q_gain)
-    if q_out is None:
-        q_out = kv_layer.new_empty((n, nq * d))
-    elif q_out.dtype is not dtype or q_out.numel() != n * nq * d:
-        raise KernelError("axes_rope_write: q_out is [tokens, nq * d] in the cache's dtype")
-    _call("lily_axes_rope_write", qkv.data_ptr(), _codes[of], splits, stride, ld, q_at, k_at, gain, eps, cos.data_ptr(), sin.data_ptr(), rows[0], positions.data_ptr(),
-          pair_axis.data_ptr(), axes[0], n, places.data_ptr(), token_req.data_ptr(), block_table.data_ptr(), width[1], kv_layer.data_ptr(), pages[0],
-          q_out.data_ptr(), code, nq, nkv, d, rotary_dim, page_size, _stream())
-    return q_out
+    q = (_module or _faces()).axes_rope_write(qkv, q_gain, k_gain, eps, cos, sin, positions, pair_axis, places, token_req, block_table, kv_layer, nq, nkv, d,
+                                              rotary_dim, page_size, q_out, row)
+    launches["count"] += 1
+    return q
 
 
 @functools.lru_cache(maxsize=1024)
@@ -1307,58 +1272,16 @@ def attention_decode_weighed(q: torch.Tensor, kv_layer: torch.Tensor, weights: t
     layer's pages, a place's entry grows by the softmax weights that the query heads of its kv head gave it, and the newest place's (this
     step's own, ``seq_lens - 1``) is set to them.  A request without places has a row of zeros.  A page belongs to one request.
     ``scratch``: float32, ``decode_weighed_scratch_floats`` of them (allocated where not given)."""
-    _dev(q, kv_layer, weights, block_table, seq_lens, out, scratch)
-    shape, dtype = q.shape, q.dtype
-    requests = shape[0] if shape else 0
-    if dtype is not kv_layer.dtype or q.numel() != requests * nq * d:
-        raise KernelError(f"attention_decode_weighed: queries are [requests, {nq * d}] in the cache's dtype, got {dtype} {tuple(shape)}")
-    pages = _layer_and_weights("attention_decode_weighed", kv_layer, weights, nkv, page_size, d)
-    width = _table("attention_decode_weighed", block_table, requests)
-    if seq_lens.numel() != requests or seq_lens.dtype is not torch.int32 or not 0 <= max_seq_len <= width * page_size:
-        raise KernelError(f"attention_decode_weighed: {requests} int32 lengths of up to {max_seq_len} places; the block table holds {width * page_size}")
-    if out is None:
-        out = torch.empty_like(q)
-    elif out.dtype is not dtype or out.numel() != q.numel():
-        raise KernelError("attention_decode_weighed: out has the shape and dtype of q")
-    need = decode_weighed_scratch_floats(requests, nq, nkv, d, max_seq_len, page_size, dtype)
-    if scratch is None:
-        scratch = weights.new_empty((need,))
-    elif scratch.dtype is not torch.float32 or scratch.numel() < need:
-        raise KernelError(f"attention_decode_weighed: scratch of {need} float32 needed")
-    _call("lily_attention_decode_weighed", q.data_ptr(), kv_layer.data_ptr(), weights.data_ptr(), out.data_ptr(), block_table.data_ptr(), width,
-          seq_lens.data_ptr(), scratch.data_ptr(), requests, max_seq_len, nq, nkv, d, page_size, pages, scale, _dt(q), DECODE_POLLS, _stream())
+    out = (_module or _faces()).attention_decode_weighed(q, kv_layer, weights, block_table, seq_lens, max_seq_len, nq, nkv, d, page_size, scale, out, scratch,
+                                                         DECODE_POLLS)
+    launches["count"] += 1
     return out
-
-
-@dataclass(frozen=True)
-class _Portions:
-    """What ``attention_key_weights`` works out from the lengths of its portions."""
-
-    tensor_cores: bool          # the tcgen05 kernels take them
-    floats: int                 # float32 scratch
-    tokens: int
-    longest: int                # places of the longest request
-    heard: bool                 # somebody is
-    prefix: object              # the lengths as C arrays
-    new: object
-
-
-@functools.lru_cache(maxsize=64)
-def _portions(h_prefix_lens: Tuple[int, ...], h_new_lens: Tuple[int, ...], nq: int, nkv: int, d: int, page_size: int, scale: float, dtype: torch.dtype,
-              observe: int) -> _Portions:
-    if nkv < 1 or nq % nkv or any(n < 0 for n in h_prefix_lens + h_new_lens):
-        raise KernelError(f"attention_key_weights: portions of {h_new_lens} behind {h_prefix_lens}, {nq} query heads over {nkv} kv heads")
-    lib, n = library(), len(h_new_lens)
-    prefix, new = (ctypes.c_int * n)(*h_prefix_lens), (ctypes.c_int * n)(*h_new_lens)
-    tensor_cores = dtype == torch.bfloat16 and bool(lib.lily_key_weights_tc_takes(nq, nkv, d, page_size, scale))
-    floats = (lib.lily_key_weights_tc_floats if tensor_cores else lib.lily_key_weights_floats)(n, prefix, new, observe, nq, nkv)
-    return _Portions(tensor_cores, int(floats), sum(h_new_lens), max((a + b for a, b in zip(h_prefix_lens, h_new_lens)), default=0), any(h_new_lens), prefix, new)
 
 
 def key_weights_scratch_floats(h_prefix_lens: Sequence[int], h_new_lens: Sequence[int], nq: int, nkv: int, d: int, page_size: int, scale: float,
                                dtype: torch.dtype, observe: Optional[int] = None) -> int:
     """Float32 scratch that ``attention_key_weights`` needs for portions of these lengths."""
-    return _portions(tuple(h_prefix_lens), tuple(h_new_lens), nq, nkv, d, page_size, scale, dtype, observe or 0).floats
+    return (_module or _faces()).key_weights_scratch_floats(h_prefix_lens, h_new_lens, nq, nkv, d, page_size, scale, dtype == torch.bfloat16, observe)
 
 
 def key_weights_status() -> int:
@@ -1375,33 +1298,9 @@ def attention_key_weights(q: torch.Tensor, kv_layer: torch.Tensor, weights: torc
     prefix and themselves, whose keys are in the cache already.  ``observe``: only the last that many tokens of each portion are heard (all where not
     given).  The portion's own places are set, also where nobody who is heard sees them.  ``h_prefix_lens``, ``h_new_lens``:
     the lengths on the host.  ``scratch``: float32, ``key_weights_scratch_floats`` of them (allocated where not given)."""
-    _dev(q, kv_layer, weights, block_table, cu_seqlens, prefix_lens, scratch)
-    requests, shape, dtype = len(h_new_lens), q.shape, q.dtype
-    if observe is not None and observe < 1:
-        raise KernelError(f"attention_key_weights: the last {observe} tokens cannot be heard")
-    if (len(h_prefix_lens) != requests or cu_seqlens.numel() != requests + 1 or prefix_lens.numel() != requests or cu_seqlens.dtype is not torch.int32
-            or prefix_lens.dtype is not torch.int32):
-        raise KernelError(f"attention_key_weights: {requests} portions have a prefix each and {requests + 1} offsets, int32")
-    plan = _portions(tuple(h_prefix_lens), tuple(h_new_lens), nq, nkv, d, page_size, scale, dtype, observe or 0)
-    if dtype is not kv_layer.dtype or len(shape) != 2 or shape[1] != nq * d or shape[0] < plan.tokens:
-        raise KernelError(f"attention_key_weights: queries are [tokens, {nq * d}] in the cache's dtype, got {dtype} {tuple(shape)} for {plan.tokens} tokens")
-    pages = _layer_and_weights("attention_key_weights", kv_layer, weights, nkv, page_size, d)
-    width = _table("attention_key_weights", block_table, requests)
-    if plan.longest > width * page_size:
-        raise KernelError(f"attention_key_weights: {plan.longest} places; the block table holds {width * page_size}")
-    if not plan.heard:
-        return
-    if scratch is None:
-        scratch = weights.new_empty((plan.floats,))
-    elif scratch.dtype is not torch.float32 or scratch.numel() < plan.floats:
-        raise KernelError(f"attention_key_weights: scratch of {plan.floats} float32 needed")
-    if plan.tensor_cores:
-        _call("lily_key_weights_tc", q.data_ptr(), shape[0], kv_layer.data_ptr(), pages, weights.data_ptr(), block_table.data_ptr(), width, scratch.data_ptr(),
-              requests, plan.prefix, plan.new, observe or 0, nq, nkv, d, page_size, scale, _stream())
-    else:
-        _call("lily_key_weights", q.data_ptr(), kv_layer.data_ptr(), weights.data_ptr(), block_table.data_ptr(), width, scratch.data_ptr(), requests, plan.prefix,
-              plan.new, observe or 0, nq, nkv, d, page_size, scale, _dt(q), _stream())
-    launches["count"] += 2                                       # rows or scores, what joins them, columns
+    if (_module or _faces()).attention_key_weights(q, kv_layer, weights, block_table, cu_seqlens, prefix_lens, h_prefix_lens, h_new_lens, nq, nkv, d, page_size,
+                                                   scale, observe, scratch):
+        launches["count"] += 3                                   # rows or scores, what joins them, columns
 
 
 def select_keys(weights: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor, max_length: int, keep: int, first: int = 0,
@@ -1410,22 +1309,8 @@ def select_keys(weights: torch.Tensor, block_table: torch.Tensor, lengths: torch
     request of ``lengths`` places with more than ``keep``: the first ``first``, the last ``recent`` and the heaviest of the rest, ties to the
     lower place; of a shorter one all.  ``weights`` float32 [layers, pages, kv_heads, page_size], or of one layer without the first axis; a
     NaN counts as the heaviest.  ``max_length``: no request has more places."""
-    _dev(weights, block_table, lengths)
-    shape = weights.shape
-    if len(shape) == 3:
-        shape = (1, *shape)
-    if weights.dtype is not torch.float32 or len(shape) != 4:
-        raise KernelError(f"select_keys: weights are float32 [layers, pages, kv_heads, page_size], got {weights.dtype} {tuple(shape)}")
-    layers, pages, nkv, page_size = shape
-    requests = lengths.numel()
-    width = _table("select_keys", block_table, requests)
-    if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
-        raise KernelError(f"select_keys: the first {first} and the last {recent} places do not fit into {keep}")
-    if lengths.dtype is not torch.int32 or not 0 <= max_length <= width * page_size:
-        raise KernelError(f"select_keys: int32 lengths of up to {max_length} places; the block table holds {width * page_size}")
-    kept = lengths.new_empty((layers, requests, nkv, keep))
-    _call("lily_select_keys", weights.data_ptr(), block_table.data_ptr(), width, lengths.data_ptr(), kept.data_ptr(), layers, pages, requests, nkv, page_size,
-          max_length, keep, first, recent, _stream())
+    kept = (_module or _faces()).select_keys(weights, block_table, lengths, max_length, keep, first, recent)
+    launches["count"] += 1
     return kept
 
 
@@ -1435,26 +1320,8 @@ def move_keys(kv: torch.Tensor, weights: Optional[torch.Tensor], block_table: to
     head) becomes what was at ``kept[..., i]``.  ``kv`` [layers, pages, 2, kv_heads, page_size, d] and ``weights`` [layers, pages, kv_heads, page_size]
     (or None), or those of one layer without the first axis.  In place, or, with ``to_table`` int32 [requests, pages], into those pages (a fork of the request; none of them
     may be a page of ``block_table``).  Places outside their tables, and what lies behind the last kept place, stay as they are."""
-    _dev(kv, weights, block_table, kept, to_table)
-    shape, places = kv.shape, kept.shape
-    beside = None if weights is None else weights.shape
-    if len(shape) == 5:
-        shape, beside = (1, *shape), None if beside is None else (1, *beside)
-    if len(shape) != 6 or shape[2] != 2 or len(places) != 4 or kept.dtype is not torch.int32:
-        raise KernelError(f"move_keys: a cache [layers, pages, 2, kv_heads, page_size, d] and int32 places [layers, requests, kv_heads, keep], got {tuple(shape)}, "
-                          f"{kept.dtype} {tuple(places)}")
-    layers, pages, _, nkv, page_size, d = shape
-    requests, keep = places[1], places[3]
-    if places[0] != layers or places[2] != nkv:
-        raise KernelError(f"move_keys: places of {places[0]} layers and {places[2]} kv heads for a cache of {layers} and {nkv}")
-    if weights is not None and (weights.dtype is not torch.float32 or beside != (layers, pages, nkv, page_size)):
-        raise KernelError(f"move_keys: weights are float32 [{layers}, {pages}, {nkv}, {page_size}], got {weights.dtype} {tuple(beside)}")
-    item = 4 if _dt(kv) == _F32 else 2
-    width = _table("move_keys", block_table, requests)
-    table = block_table.data_ptr()
-    to, to_width = (table, width) if to_table is None else (to_table.data_ptr(), _table("move_keys", to_table, requests, "to_table"))
-    _call("lily_move_keys", kv.data_ptr(), None if weights is None else weights.data_ptr(), table, width, to, to_width, kept.data_ptr(), layers, pages, requests,
-          nkv, page_size, d * item, keep, int(to == table), _stream())
+    (_module or _faces()).move_keys(kv, weights, block_table, kept, to_table)
+    launches["count"] += 1
 
 
 # ------------------------------------------------------------------------------ joining sublayers
