@@ -18,8 +18,8 @@
 // several blocks share leaves a part in scratch for each, joined in their order (rows: by the join kernel; columns: by the warps that
 // come last), so the results do not depend on who is first.
 //
-// Measured: 2,048 tokens of 32 heads of 128 over 8, 63.5 us (the rows 28, the columns 28, some 7 between the kernels; the exponentials alone 34, the products
-// 10); the last 64 of 1,024 tokens behind 15,360 places 38.  The CUDA cores of key_weights.cu take 768 for the first, and on the same pages 12.6 for 16 tokens (here 9.5),
+// Measured: 2,048 tokens of 32 heads of 128 over 8, 61.4 us (some 7 of them between the kernels; all exponentials on their unit would take 34, the products
+// 10); the last 64 of 1,024 tokens behind 15,360 places 36.7.  The CUDA cores of key_weights.cu take 768 for the first, and on the same pages 12.6 for 16 tokens (here 9.5),
 // 17.8 for 128 (13.0); they are ahead for 300 tokens of seven heads of 64 over one (14.6, here 17.4), where a dozen tiles leave most SMs idle either way.
 //
 // Every wait is bounded: one that runs out sets a status word (lily_key_weights_status), the roles leave their loops and the block frees its
@@ -164,6 +164,29 @@ __device__ __forceinline__ Two exp2_of(Two x) {
     apart(x, a, b);
     return two(ex2(a), ex2(b));
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// The same on the multiply-add unit, for weights (x at most a little above 0, or NaN): x = i + f with |f| <= 1/2, 2^f by the polynomial of degree five whose largest
+// relative error is least (7.5e-8 by its coefficients, 2.3e-7 as computed; fitted by Lawson's iteration), 2^i by its exponent; below 2^-126.5 it is 0.
+__device__ __forceinline__ Two exp2_by_terms(Two x) {
+    constexpr float SHIFT = 12582912.f + 127.f;                       // 1.5 * 2^23: the sum's last bits are i + 127
+    float a, b;
+    apart(x, a, b);
+    x = two(max_nan(a, -127.f), max_nan(b, -127.f));
+    const Two r = add2(x, two(SHIFT, SHIFT)), f = fma2(add2(r, two(-SHIFT, -SHIFT)), two(-1.f, -1.f), x);
+    Two p = fma2(f, two(1.3276472454890609e-3f, 1.3276472454890609e-3f), two(9.675540961325169e-3f, 9.675540961325169e-3f));
+    p = fma2(p, f, two(5.550713092088699e-2f, 5.550713092088699e-2f));
+    p = fma2(p, f, two(0.24022120237350464f, 0.24022120237350464f));
+    p = fma2(p, f, two(0.6931469440460205f, 0.6931469440460205f));
+    p = fma2(p, f, two(1.0000001192092896f, 1.0000001192092896f));
+    apart(r, a, b);
+    return mul2(p, two(__uint_as_float(__float_as_uint(a) << 23), __uint_as_float(__float_as_uint(b) << 23)));
+}
+// Pair e of sixteen: three of them by terms, the others by the exponentials' unit (2,048 tokens 61.4 us, 8,192 614; none by terms 63.8 and 654, two 61.9 and 621, four 62.2 and 628).
+__device__ __forceinline__ Two exp2_of(Two x, int e) { return e % 5 == 2 ? exp2_by_terms(x) : exp2_of(x); }
 
 // Waits for the loads from tensor memory; what they bring is not used ahead of this.
 __device__ __forceinline__ void wait_loaded(float (&r)[32]) {
@@ -548,15 +571,15 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
                     }
                     const float off = m == -INFINITY ? 0.f : -m;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) sum[e & 3] = add2(sum[e & 3], exp2_of(fma2(two(s[2 * e], s[2 * e + 1]), two(c, c), two(off, off))));
+                    for (int e = 0; e < 16; ++e) sum[e & 3] = add2(sum[e & 3], exp2_of(fma2(two(s[2 * e], s[2 * e + 1]), two(c, c), two(off, off)), e));
                 } else {
                     const ulonglong2* minus_lse = reinterpret_cast<const ulonglong2*>(lse_s + ls * BR + half * COLS + c0);
                     if (all) {
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
                             const ulonglong2 z = minus_lse[e >> 1];
-                            sum[e & 3] = add2(sum[e & 3], exp2_of(fma2(two(s[2 * e], s[2 * e + 1]), two(c, c), z.x)));
-                            sum[(e + 1) & 3] = add2(sum[(e + 1) & 3], exp2_of(fma2(two(s[2 * e + 2], s[2 * e + 3]), two(c, c), z.y)));
+                            sum[e & 3] = add2(sum[e & 3], exp2_of(fma2(two(s[2 * e], s[2 * e + 1]), two(c, c), z.x), e));
+                            sum[(e + 1) & 3] = add2(sum[(e + 1) & 3], exp2_of(fma2(two(s[2 * e + 2], s[2 * e + 3]), two(c, c), z.y), e + 1));
                         }
                     } else {
                         const int low = max(from, 0);
