@@ -31,8 +31,8 @@ constexpr int SELECT_HELD = 48 * 1024;     // places whose ranks a block holds i
 // (0: rows of more than eight places a thread, in shared memory), and are asked for before the row's length has arrived.  The rank that the last kept weight has comes
 // out eight bits a pass (a histogram of the competing ranks that share the bits found so far, in shared memory; lanes that meet in a counter are added
 // up by the hardware), until a bin has no more than 32, which every warp then ranks by itself.  Then every warp counts what it
-// keeps of its stretch and writes it behind what the warps ahead keep.  What bounds it is the chain of reads and passes, not the bytes: 6.0 us for 64 rows of 4,096,
-// 11.3 for 384 of up to 3,500 (12.9 with 48 registers, where an SM holds two of these blocks).
+// keeps of its stretch and writes it behind what the warps ahead keep.  What bounds it is the chain of reads and passes, not the bytes: 6.2 us for 64 rows of 4,096,
+// 10.4 for 384 of up to 3,500 (12.9 with 48 registers, where an SM holds two of these blocks).
 template <int REGS>
 __global__ void __maxnreg__(40) select_keys_kernel(const SelectArgs a) {
     constexpr int P = REGS ? REGS : 4;
@@ -72,7 +72,8 @@ __global__ void __maxnreg__(40) select_keys_kernel(const SelectArgs a) {
     const int per = REGS ? 32 * P : (n + threads - 1) / threads * 32, beg = warp * per, end = min(n, beg + per);      // this warp's stretch
     if (REGS) {
 #pragma unroll
-        for (int u = 0; u < P; ++u) mine[u] = rank_of(w[u]);
+        for (int u = 0; u < P; ++u)
+            if (beg + 32 * u < end) mine[u] = rank_of(w[u]);
     } else if (held) {
         for (int j0 = beg + lane; j0 < end; j0 += 32 * P) {
             ask(j0, 32);
@@ -88,7 +89,7 @@ __global__ void __maxnreg__(40) select_keys_kernel(const SelectArgs a) {
 #pragma unroll
             for (int u = 0; u < P; ++u) {
                 const int j = beg + 32 * u + lane;
-                if (j >= lo && j < hi) f(mine[u]);
+                if (beg + 32 * u < end && j >= lo && j < hi) f(mine[u]);
             }
         } else
             for (int j = beg + lane; j < end; j += 32) {
@@ -183,6 +184,7 @@ __global__ void __maxnreg__(40) select_keys_kernel(const SelectArgs a) {
     if (REGS) {
 #pragma unroll
         for (int u = 0; u < P; ++u) {
+            if (beg + 32 * u >= end) break;
             kinds(beg + 32 * u, mine[u], sure[u], tie[u]);
             sures += __popc(sure[u]);
             ties += __popc(tie[u]);
@@ -208,7 +210,10 @@ __global__ void __maxnreg__(40) select_keys_kernel(const SelectArgs a) {
     };
     if (REGS) {
 #pragma unroll
-        for (int u = 0; u < P; ++u) put(beg + 32 * u, sure[u], tie[u]);
+        for (int u = 0; u < P; ++u) {
+            if (beg + 32 * u >= end) break;
+            put(beg + 32 * u, sure[u], tie[u]);
+        }
     } else
         for (int j0 = beg; j0 < end; j0 += 32) {
             kinds(j0, rank(j0 + lane), sure[0], tie[0]);

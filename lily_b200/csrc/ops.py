@@ -1224,24 +1224,6 @@ def pair_axes(sections: Sequence[int], device, in_turn: bool = False) -> torch.T
     return torch.tensor(axes, dtype=torch.int32, device=device)
 
 
-def _layer_and_weights(what: str, kv_layer: torch.Tensor, weights: torch.Tensor, nkv: int, page_size: int, d: int) -> int:
-    """The pages of a cache layer that fits, with weights beside it."""
-    shape = kv_layer.shape
-    if shape[1:] != (2, nkv, page_size, d):
-        cache_layer_fits(kv_layer, nkv, page_size, d, d)
-    if weights.dtype is not torch.float32 or weights.shape != (shape[0], nkv, page_size):
-        raise KernelError(f"{what}: weights are float32 [{shape[0]}, {nkv}, {page_size}], got {weights.dtype} {tuple(weights.shape)}")
-    return shape[0]
-
-
-def _table(what: str, table: torch.Tensor, requests: int, name: str = "block_table") -> int:
-    """The width of a block table of so many requests."""
-    shape = table.shape
-    if len(shape) != 2 or shape[0] != requests or shape[1] < 1 or table.dtype is not torch.int32:
-        raise KernelError(f"{what}: {name} is int32 [{requests}, pages], got {table.dtype} {tuple(shape)}")
-    return shape[1]
-
-
 def axes_rope_write(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_gain: Optional[torch.Tensor], eps: float, cos: torch.Tensor,
                     sin: torch.Tensor, positions: torch.Tensor, pair_axis: torch.Tensor, places: torch.Tensor, token_req: torch.Tensor,
                     block_table: torch.Tensor, kv_layer: torch.Tensor, nq: int, nkv: int, d: int, rotary_dim: int, page_size: int,

@@ -4,6 +4,7 @@ steps captured in a graph."""
 import pytest
 import torch
 
+import test_key_budget_gpu as base
 from test_key_budget_gpu import BF16, DEV, F32, close, decode_want, pool, portion_want, same
 
 pytestmark = pytest.mark.gpu
@@ -107,3 +108,34 @@ def test_a_captured_step_runs_again_on_what_has_changed():
         other, other_w = kv.clone(), w.clone()
         want = step(other, other_w)
         assert torch.equal(out, want) and same(mine, other) and same(given, other_w)
+
+
+@pytest.mark.parametrize("dtype,d,page", [(F32, 128, 16), (F32, 40, 2), (BF16, 128, 64), (BF16, 64, 16), (BF16, 24, 8)])
+@pytest.mark.parametrize("rows,longest", [(1, 0), (3, 0), (3, 5), (1, 1)])
+def test_rows_without_places(dtype, d, page, rows, longest):
+    """All rows empty (a plan for none, or for some), and a single place."""
+    lengths = [longest if longest == 1 else 0] * rows
+    kv, w, table = pool([max(1, longest)] * rows, 2, page, d, dtype, 3)
+    q = torch.randn(rows, 4 * d, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).to(dtype)
+    want, want_w = decode_want(q, kv, w, table, lengths, 4, 2, d, page, 0.2)
+    got = ops().attention_decode_weighed(q, kv, w, table, torch.tensor(lengths, dtype=torch.int32, device=DEV), longest, 4, 2, d, page, 0.2)
+    close(got, want, dtype)
+    close(w, want_w, F32)
+    kept = ops().select_keys(w, table, torch.tensor(lengths, dtype=torch.int32, device=DEV), longest, 4, 1, 1)
+    assert kept.shape == (1, rows, 2, 4) and kept[..., 0].tolist() == [[[lengths[0] - 1] * 2] * rows] and bool((kept[..., 1:] == -1).all())
+
+
+@pytest.mark.parametrize("n,keep,first,recent", [(3000, 512, 4, 64), (8192, 100, 0, 0), (8193, 8192, 1, 8191), (60000, 1024, 4, 128), (4097, 4096, 0, 1), (33, 32, 0, 0)])
+@pytest.mark.parametrize("kind", ["few values", "all alike", "negative and infinite", "neighbours"])
+def test_selection_of_equal_and_close_weights(n, keep, first, recent, kind):
+    """Ties go to the lower place, however many share a weight; weights that differ in their last bits alone."""
+    nkv, page = 2, 64
+    g = torch.Generator().manual_seed(n)
+    _, w, table = pool([n], nkv, page, 4, F32, 6)
+    rows = {"few values": torch.randint(0, 5, (nkv, n), generator=g).float(), "all alike": torch.full((nkv, n), 0.25), "neighbours": (1.0 + torch.randint(0, 40, (nkv, n), generator=g) * 2.0 ** -23),
+            "negative and infinite": torch.where(torch.rand(nkv, n, generator=g) < 0.01, torch.tensor(float("inf")), torch.randn(nkv, n, generator=g))}[kind]
+    base.put_rows(w, table, 0, rows.to(DEV), page)
+    kept = ops().select_keys(w, table, torch.tensor([n], dtype=torch.int32, device=DEV), n, keep, first, recent)[0, 0].cpu()
+    for h in range(nkv):
+        order = sorted(range(first, n - recent), key=lambda j: (-float(rows[h, j]), j))[:keep - first - recent]
+        assert kept[h].tolist() == sorted([*range(first), *order, *range(n - recent, n)])
