@@ -38,11 +38,11 @@ struct Args {
 
 // Where a head of a token goes: its row of `q_out` or of a page (null: nowhere).
 template <typename T>
-__device__ __forceinline__ T* target(const Args& a, int n, int head) {
+__device__ __forceinline__ T* target(const Args& a, int n, int head, int place, int req) {
     if (head < a.nq) return (T*)a.q_out + ((size_t)n * a.nq + head) * a.d;
-    const int place = a.places[n], at = place / a.page_size;
+    const int at = place / a.page_size;
     if (place < 0 || at >= a.bt_stride) return nullptr;
-    const int page = a.block_table[(size_t)a.token_req[n] * a.bt_stride + at];
+    const int page = a.block_table[(size_t)req * a.bt_stride + at];
     if (page < 0 || page >= a.pages) return nullptr;
     return (T*)a.kv + (((size_t)page * 2 * a.nkv + (head - a.nq)) * a.page_size + place % a.page_size) * a.d;
 }
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(128) axes_rope_write_kernel(const Args a) {
     pdl_enter_small();
     const int n = blockIdx.x, head = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (head >= a.nq + 2 * a.nkv) return;
-    T* dst = target<T>(a, n, head);
+    T* dst = target<T>(a, n, head, head < a.nq ? 0 : a.places[n], head < a.nq ? 0 : a.token_req[n]);
     if (!dst) return;
     const IN* src = (const IN*)a.qkv + (size_t)n * a.ld + (size_t)head * a.d;
     auto in = [&](int i) {
@@ -96,8 +96,8 @@ __global__ void __launch_bounds__(128) axes_rope_write_kernel(const Args a) {
 // warp), each with two pieces: of the rotated features N neighbouring ones and their partners rd / 2 further, of the rest two neighbouring pieces.  So the
 // rotation needs no exchange and the norm log2(G) shuffles.  The positions of up to four axes are read
 // beside the axes of a thread's pairs, not behind them.  What bounds it is the chain of reads (axis and positions, tables, result), for few tokens
-// and for many, which small blocks of short-lived threads hide best: 2,048 tokens of 32 + 2 x 8 heads of 128 in bfloat16 take 15.1 us (51 MB: 3.4 TB/s; a
-// plain copy of as many bytes 9.3), eight tokens out of four planes of partial sums 3.1.
+// and for many, which small blocks of short-lived threads hide best: 2,048 tokens of 32 + 2 x 8 heads of 128 in bfloat16 take 13.8 us (51 MB: 3.7 TB/s; a
+// plain copy of as many bytes 9.3; with the places read behind the tables 15.1), eight tokens out of four planes of partial sums 3.0.
 constexpr int WIDE_THREADS = 128, AHEAD = 4;
 
 // Numbers in pairs (mul and fma.rn.f32x2: two IEEE operations an instruction).
@@ -188,7 +188,7 @@ __device__ __forceinline__ void store_piece(T* dst, const Two (&v)[N / 2]) {
 
 // The tables' numbers of N pairs from `j` on, for the lanes of a warp that `need` them (of one token, `mine`: shared memory of the warp's, room for
 // two rows of the tables).  Where each lane's pairs share an axis they are 16-byte reads; else the warp brings each pair of the token once, side by side, and
-// hands them round through shared memory (axes in turn, 2,048 tokens: 15.3 us; a read a pair and thread took 20.7).
+// hands them round through shared memory (axes in turn, 2,048 tokens: 15.2 us; a read a pair and thread took 20.7).
 template <int N>
 __device__ __forceinline__ void load_turn(const Args& a, int n, int j, bool need, float* mine, Two (&c)[N / 2], Two (&s)[N / 2]) {
     const int half = a.rd / 2;
@@ -264,8 +264,10 @@ __global__ void __launch_bounds__(WIDE_THREADS, 8) axes_rope_write_wide_kernel(c
     uint4 raw_gx, raw_gy;
     if constexpr (sizeof(W) == 2 && N == 8)
         if (gain) raw_gx = *reinterpret_cast<const uint4*>(gain + i0), raw_gy = *reinterpret_cast<const uint4*>(gain + i1);
+    const bool cached = head >= a.nq;
+    const int place = cached ? a.places[n] : 0, req = cached ? a.token_req[n] : 0;      // asked for beside the positions, not behind the tables
     load_turn<N>(a, n, i0, !value && turned, turns_s + (tid >> 5) * a.rd, c, s);
-    T* dst = asked > most ? nullptr : target<T>(a, n, head);
+    T* dst = asked > most ? nullptr : target<T>(a, n, head, place, req);
     if constexpr (sizeof(IN) == 2) {
         unpack<IN, N>(raw_x, x);
         unpack<IN, N>(raw_y, y);
@@ -332,8 +334,8 @@ LILY_API int lily_axes_rope_write(const void* qkv, int in_dtype, int splits, siz
     const uintptr_t where = (uintptr_t)qkv | (uintptr_t)kv | (uintptr_t)q_out | (uintptr_t)q_gain | (uintptr_t)k_gain |
                             (uintptr_t)cos_t | (uintptr_t)sin_t | (uintptr_t)pair_axis;
     // Whole pieces of 16 bytes on every side; else, and for heads that are no power of two of pieces, a warp a head.  Measured, us, in pieces / a warp a
-    // head, on the same operands: 2,048 tokens of 48 heads of 128 in bfloat16 13.1 / 35.6 (axes in turn 15.3 / 35.3), eight tokens from four planes 3.1 / 5.4;
-    // float32, 1,000 tokens of 24 heads of 128 with half of each turned 7.9 / 8.4, of 64 5.1 / 7.9.
+    // head, on the same operands: 2,048 tokens of 48 heads of 128 in bfloat16 12.3 / 35.6 (axes in turn 15.2 / 35.3), eight tokens from four planes 3.1 / 5.4;
+    // float32, 1,000 tokens of 24 heads of 128 with half of each turned 8.0 / 8.4, of 64 5.1 / 7.9.
     const bool wide = d % (2 * piece) == 0 && 1 << shift == group && group <= 32 && rd % (2 * piece) == 0 && ld % piece == 0 &&
                       (in_dtype == act_dtype || ld % 4 == 0) && (size_t)stride % 4 == 0 && where % 16 == 0;
     const dim3 grid = wide ? dim3(tokens, (unsigned)((((nq + 2 * nkv) << shift) + axes::WIDE_THREADS - 1) / axes::WIDE_THREADS)) : dim3(tokens, (nq + 2 * nkv + 3) / 4);
