@@ -51,6 +51,7 @@ attention_decode_f32_kernel(const AttnArgs a) {
 
     float4 k[KB][C], v[KB][C], kn[AHEAD ? KB : 1][C], vn[AHEAD ? KB : 1][C];
     // WEIGHED, pages of whole keys of a step: lane i looks up the page of the warp's step i ahead, so that a step's reads do not wait for the table's
+    // (three rows of up to 2,900 keys, 16 heads of 128 over 4, with the kernel behind: 14.7 us; looked up at each step 17.1)
     int pages = 0, looked = 0;
     auto fetch = [&](int u0, float4 (*kd)[C], float4 (*vd)[C]) {
         if (WEIGHED && a.page_size % KB == 0) {

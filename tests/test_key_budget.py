@@ -302,3 +302,32 @@ def test_no_block_writes_to_a_block_that_may_not_have_started():
             assert 0 < body.find("cluster_arrive_started();") < body.find("cluster_wait_started();") < write, name
             assert body.count("cluster_arrive_started();") == body.count("cluster_wait_started();") == 1, name
     assert found == ["attention_weighed.cu", "key_weights.cu"]
+
+
+def test_faces_refuse_on_the_host():
+    """What is no tensor, lies on the host, or is no number is refused with the package's error (or Python's own), not with a crash."""
+    from lily_b200.csrc import build, ops
+    try:
+        ops.library(), ops._faces()
+    except build.BuildError as exc:
+        pytest.skip(f"no kernel library here: {exc}")
+    t = torch.zeros(4)
+    calls = [lambda x: ops.axes_rope_write(x, None, None, 1e-6, x, x, x, x, x, x, x, x, 1, 1, 4, 4, 4), lambda x: ops.attention_decode_weighed(x, x, x, x, x, 1, 1, 1, 4, 4, 0.5),
+             lambda x: ops.attention_key_weights(x, x, x, x, x, x, [0], [1], 1, 1, 4, 4, 0.5), lambda x: ops.select_keys(x, x, x, 1, 1), lambda x: ops.move_keys(x, x, x, x)]
+    for call in calls:
+        with pytest.raises(ops.KernelError, match="CUDA device"):
+            call(t)
+        with pytest.raises(ops.KernelError, match="take tensors, got int"):
+            call(3)
+    floats = lambda *a, **k: ops.key_weights_scratch_floats(*a, 16, 4, 128, 16, 0.1, torch.float32, **k)
+    assert floats([0, 300], [333, 70]) > floats([0], [333]) > floats([0], [0]) == 0
+    for bad in (([0], [-1]), ([-1], [1]), ([0], [1, 2])):
+        with pytest.raises(ops.KernelError):
+            floats(*bad)
+    for bad in (([0], 3), ([0], ["a"])):
+        with pytest.raises(TypeError):
+            floats(*bad)
+    with pytest.raises(ops.KernelError, match="heard"):
+        floats([0], [1], observe=0)
+    with pytest.raises(ops.KernelError, match="32-bit"):
+        floats([0], [1 << 40])
