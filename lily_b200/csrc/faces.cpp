@@ -40,8 +40,8 @@ struct Entries {
     int (*decode_weighed)(const void*, const void*, float*, void*, const int*, int, const int*, float*, int, int, int, int, int, int, int, float, int, int, void*);
     int (*select_keys)(const float*, const int*, int, const int*, int*, int, int, int, int, int, int, int, int, int, void*);
     int (*move_keys)(void*, float*, const int*, int, const int*, int, const int*, int, int, int, int, int, int, int, int, void*);
-    int (*key_weights)(const void*, const void*, float*, const int*, int, float*, int, const int*, const int*, int, int, int, int, int, float, int, void*);
-    size_t (*key_weights_floats)(int, const int*, const int*, int, int, int);
+    int (*key_weights)(const void*, const void*, float*, const int*, int, float*, int, const int*, const int*, int, int, int, int, int, float, int, int, void*);
+    size_t (*key_weights_floats)(int, const int*, const int*, int, int, int, int);
     int (*key_weights_tc)(const void*, int, const void*, int, float*, const int*, int, float*, int, const int*, const int*, int, int, int, int, int, float, void*);
     size_t (*key_weights_tc_floats)(int, const int*, const int*, int, int, int);
     int (*key_weights_tc_takes)(int, int, int, int, float);
@@ -283,7 +283,7 @@ std::vector<int> lengths(PyObject* o) {
 }
 // What portions need: whether the tcgen05 kernels take them, and the scratch.
 struct Plan { bool tensor_cores; int64_t floats, tokens, longest; };
-Plan plan(const std::vector<int>& prefix, const std::vector<int>& fresh, int nq, int nkv, int d, int page, float scale, int code, int observe) {
+Plan plan(const std::vector<int>& prefix, const std::vector<int>& fresh, int nq, int nkv, int d, int page, float scale, int code, int observe, int most_scores) {
     if (entry.key_weights_tc_takes == nullptr) refuse("the kernels are not bound");
     bool fits = nkv >= 1 && nq >= 0 && nq % nkv == 0 && prefix.size() == fresh.size();
     Plan p{};
@@ -294,7 +294,9 @@ Plan plan(const std::vector<int>& prefix, const std::vector<int>& fresh, int nq,
     }
     if (!fits) refuse("attention_key_weights: portions of ", words(std::vector<int64_t>(fresh.begin(), fresh.end())), " behind ", words(std::vector<int64_t>(prefix.begin(), prefix.end())), ", ", nq, " query heads over ", nkv, " kv heads");
     p.tensor_cores = code == BF16 && entry.key_weights_tc_takes(nq, nkv, d, page, scale);
-    p.floats = (int64_t)(p.tensor_cores ? entry.key_weights_tc_floats : entry.key_weights_floats)((int)fresh.size(), prefix.data(), fresh.data(), observe, nq, nkv);
+    const int requests = (int)fresh.size();
+    p.floats = (int64_t)(p.tensor_cores ? entry.key_weights_tc_floats(requests, prefix.data(), fresh.data(), observe, nq, nkv)
+                                        : entry.key_weights_floats(requests, prefix.data(), fresh.data(), observe, nq, nkv, most_scores));
     return p;
 }
 int observed(PyObject* o) {
@@ -304,27 +306,27 @@ int observed(PyObject* o) {
     return n;
 }
 
-// prefix lengths, new lengths, nq, nkv, d, page_size, scale, bfloat16 or not, observe
+// prefix lengths, new lengths, nq, nkv, d, page_size, scale, bfloat16 or not, observe, scores kept at a time
 PyObject* key_weights_scratch_floats(PyObject*, PyObject* const* p, Py_ssize_t count) {
-    return guarded(count, 9, [&]() -> PyObject* {
-        return PyLong_FromLongLong(plan(lengths(p[0]), lengths(p[1]), number(p[2]), number(p[3]), number(p[4]), number(p[5]), real(p[6]), number(p[7]) ? BF16 : F32, observed(p[8])).floats);
+    return guarded(count, 10, [&]() -> PyObject* {
+        return PyLong_FromLongLong(plan(lengths(p[0]), lengths(p[1]), number(p[2]), number(p[3]), number(p[4]), number(p[5]), real(p[6]), number(p[7]) ? BF16 : F32, observed(p[8]), number(p[9])).floats);
     });
 }
 
-// q, kv_layer, weights, block_table, cu_seqlens, prefix_lens, prefix lengths, new lengths, nq, nkv, d, page_size, scale, observe, scratch
+// q, kv_layer, weights, block_table, cu_seqlens, prefix_lens, prefix lengths, new lengths, nq, nkv, d, page_size, scale, observe, scratch, scores kept at a time
 PyObject* attention_key_weights(PyObject*, PyObject* const* p, Py_ssize_t count) {
-    return guarded(count, 15, [&]() -> PyObject* {
+    return guarded(count, 16, [&]() -> PyObject* {
         const char* what = "attention_key_weights";
         const Tensor &q = tensor(p[0]), &kv = tensor(p[1]), &weights = tensor(p[2]), &table = tensor(p[3]), &cu = tensor(p[4]), &cached = tensor(p[5]);
         const Tensor* room = maybe(p[14]);
         const std::vector<int> prefix = lengths(p[6]), fresh = lengths(p[7]);
-        const int nq = number(p[8]), nkv = number(p[9]), d = number(p[10]), page = number(p[11]), observe = observed(p[13]);
+        const int nq = number(p[8]), nkv = number(p[9]), d = number(p[10]), page = number(p[11]), observe = observed(p[13]), most_scores = number(p[15]);
         const float scale = real(p[12]);
         const int64_t requests = (int64_t)fresh.size();
         if ((int64_t)prefix.size() != requests || cu.numel() != requests + 1 || cached.numel() != requests || !is(cu, at::kInt) || !is(cached, at::kInt))
             refuse(what, ": ", requests, " portions have a prefix each and ", requests + 1, " offsets, int32");
         const int code = code_of(q);
-        const Plan plan_ = plan(prefix, fresh, nq, nkv, d, page, scale, code, observe);
+        const Plan plan_ = plan(prefix, fresh, nq, nkv, d, page, scale, code, observe, most_scores);
         if (q.scalar_type() != kv.scalar_type() || q.dim() != 2 || q.size(1) != (int64_t)nq * d || q.size(0) < plan_.tokens)
             refuse(what, ": queries are [tokens, ", (int64_t)nq * d, "] in the cache's dtype, got ", words(q), " for ", plan_.tokens, " tokens");
         layer_fits(kv, nkv, page, d);
@@ -340,7 +342,7 @@ PyObject* attention_key_weights(PyObject*, PyObject* const* p, Py_ssize_t count)
                                              width, scratch.data_ptr<float>(), (int)requests, prefix.data(), fresh.data(), observe, nq, nkv, d, page, scale, stream()));
         else
             done("lily_key_weights", call(entry.key_weights, q.const_data_ptr(), kv.const_data_ptr(), weights.data_ptr<float>(), table.const_data_ptr<int>(), width, scratch.data_ptr<float>(),
-                                          (int)requests, prefix.data(), fresh.data(), observe, nq, nkv, d, page, scale, code, stream()));
+                                          (int)requests, prefix.data(), fresh.data(), observe, nq, nkv, d, page, scale, code, most_scores, stream()));
         Py_RETURN_TRUE;
     });
 }

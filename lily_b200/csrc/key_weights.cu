@@ -54,6 +54,10 @@ __device__ __forceinline__ const Portion& request_of(const Args& a, int& at) {
     return a.p[r];
 }
 
+// Whether a row of the run ahead of row `end` sees a place from `k0` on.  Both the kernel that makes tiles of scores and the one that reads them go by it: a tile
+// that it does not name is neither written nor read, whatever the run's last tile of rows is filled to.
+__device__ __forceinline__ bool seen(const Portion& p, int end, int k0, int group) { return k0 <= p.place0 + (min(end, p.rows) - 1) / group; }
+
 __device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
     unsigned long long r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
@@ -99,7 +103,7 @@ __global__ void __launch_bounds__(THREADS, 2) key_weights_scores_kernel(const __
     const Portion& sp = request_of<&Portion::tile0>(a, at);
     const int kt = at % sp.key_tiles, rt = at / sp.key_tiles % sp.row_tiles, kvh = at / sp.key_tiles / sp.row_tiles;
     const int group = a.nq / a.nkv, row0 = rt * TM, k0 = kt * TN;
-    if (k0 > sp.place0 + (min(row0 + TM, sp.rows) - 1) / group) return;
+    if (!seen(sp, row0 + TM, k0, group)) return;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int* table = a.block_table + (size_t)sp.request * a.bt_stride;
     // a thread brings columns 4 (tid % 8) of rows tid / 8 and tid / 8 + 32 of either tile
@@ -213,7 +217,8 @@ __global__ void __launch_bounds__(COL_THREADS) key_weights_columns_kernel(const 
         sum = place < sp.prefix || a.again ? *at : 0.f;
     }
     float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int first = max(0, k0 - sp.place0) * group / TM, tiles = sp.row_tiles;      // the tiles of rows that see any of these places
+    // the tiles of rows that see any of these places (none where the run ends ahead of them)
+    const int tiles = seen(sp, sp.rows, k0, group) ? sp.row_tiles : 0, first = tiles ? max(0, k0 - sp.place0) * group / TM : 0;
     for (int t0 = first + part; t0 < tiles; t0 += 4 * parts) {
         float4 s[8];
         float e[8];
@@ -285,20 +290,20 @@ static Tiles plan(Args& a, int requests, int request0, int token0, const int* pr
 }
 static size_t floats_of(const Tiles& t) { return (size_t)t.scores * (TM * TN + 2 * TM) + (size_t)t.rows * TM; }
 
-// Heard tokens of a run: as many as keep the scores of MAX_R requests within about a gigabyte, a tile of rows at least.
-static int run_of(const Args& a, int requests, const int* prefix, const int* fresh) {
+// Heard tokens of a run: as many as keep its scores within about `scores`, a tile of rows at least.
+static int run_of(const Args& a, int requests, const int* prefix, const int* fresh, int scores) {
     long long places = 0;
     for (int r = 0; r < requests; ++r) places += prefix[r] + fresh[r] + TN;
     const int group = a.nq / a.nkv, least = (TM + group - 1) / group;
-    const long long most = ((long long)1 << 28) / (places * a.nq > 0 ? places * a.nq : 1);
+    const long long most = scores / (places * a.nq > 0 ? places * a.nq : 1);
     return most < least ? least : most > 0x7fffff ? 0x7fffff : (int)most;
 }
 
 template <typename F>
-static int each_run(Args& a, int requests, const int* prefix, const int* fresh, int observe, F&& use) {
+static int each_run(Args& a, int requests, const int* prefix, const int* fresh, int observe, int scores, F&& use) {
     int token0 = 0;
     for (int r = 0; r < requests; r += MAX_R) {
-        const int now = requests - r < MAX_R ? requests - r : MAX_R, some = run_of(a, now, prefix + r, fresh + r);
+        const int now = requests - r < MAX_R ? requests - r : MAX_R, some = run_of(a, now, prefix + r, fresh + r, scores);
         int heard = 0, tokens = 0;
         for (int i = r; i < r + now; ++i) {
             const int h = observe > 0 && observe < fresh[i] ? observe : fresh[i];
@@ -320,13 +325,13 @@ static int each_run(Args& a, int requests, const int* prefix, const int* fresh, 
 
 using namespace lily;
 
-// Floats of scratch for portions of `fresh` tokens behind `prefix` places (host arrays): scores, the rows' parts, their lse.
-LILY_API size_t lily_key_weights_floats(int requests, const int* prefix, const int* fresh, int observe, int nq, int nkv) {
+// Floats of scratch for portions of `fresh` tokens behind `prefix` places (host arrays): the scores of a run (about `most_scores` of them), the rows' parts, their lse.
+LILY_API size_t lily_key_weights_floats(int requests, const int* prefix, const int* fresh, int observe, int nq, int nkv, int most_scores) {
     static thread_local keyw::Args a;
     a.nq = nq;
     a.nkv = nkv;
     size_t most = 0;
-    keyw::each_run(a, requests, prefix, fresh, observe, [&](const keyw::Tiles& t) {
+    keyw::each_run(a, requests, prefix, fresh, observe, most_scores, [&](const keyw::Tiles& t) {
         const size_t n = keyw::floats_of(t);
         most = n > most ? n : most;
         return 0;
@@ -336,7 +341,7 @@ LILY_API size_t lily_key_weights_floats(int requests, const int* prefix, const i
 
 LILY_API int lily_key_weights(const void* q, const void* kv, float* weights, const int* block_table, int bt_stride, float* scratch, int requests,
                               const int* prefix, const int* fresh, int observe, int nq, int nkv, int d, int page_size, float scale, int dtype,
-                              cudaStream_t stream) {
+                              int most_scores, cudaStream_t stream) {
     LILY_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "attention_key_weights: %d query heads over %d kv heads", nq, nkv);
     LILY_REQUIRE(d >= 1 && page_size > 0 && (page_size & (page_size - 1)) == 0 && observe >= 0, "attention_key_weights: head size %d, pages of %d, the last %d heard", d, page_size,
                  observe);
@@ -347,7 +352,7 @@ LILY_API int lily_key_weights(const void* q, const void* kv, float* weights, con
     while (1 << a.page_shift < page_size) ++a.page_shift;
     // (reads of four numbers, or of one where rows are not aligned for it: 106 and 115 us for 1,000 tokens of 16 heads of 128)
     const bool vec = d % 4 == 0 && (((uintptr_t)q | (uintptr_t)kv) & 15) == 0;
-    const int rc = keyw::each_run(a, requests, prefix, fresh, observe, [&](const keyw::Tiles& t) {
+    const int rc = keyw::each_run(a, requests, prefix, fresh, observe, most_scores, [&](const keyw::Tiles& t) {
         LILY_REQUIRE(t.scores <= 0x7fffffff, "attention_key_weights: %lld tiles", t.scores);
         a.parts = (float2*)(a.scores + (size_t)t.scores * (keyw::TM * keyw::TN));
         a.lse = (float*)(a.parts + (size_t)t.scores * keyw::TM);

@@ -1260,10 +1260,14 @@ def attention_decode_weighed(q: torch.Tensor, kv_layer: torch.Tensor, weights: t
     return out
 
 
+KEY_WEIGHTS_SCORES = 1 << 28      # scores that the CUDA-core kernels of `attention_key_weights` keep at a time (a gigabyte); longer portions come in runs of tokens
+
+
 def key_weights_scratch_floats(h_prefix_lens: Sequence[int], h_new_lens: Sequence[int], nq: int, nkv: int, d: int, page_size: int, scale: float,
                                dtype: torch.dtype, observe: Optional[int] = None) -> int:
     """Float32 scratch that ``attention_key_weights`` needs for portions of these lengths."""
-    return (_module or _faces()).key_weights_scratch_floats(h_prefix_lens, h_new_lens, nq, nkv, d, page_size, scale, dtype == torch.bfloat16, observe)
+    return (_module or _faces()).key_weights_scratch_floats(h_prefix_lens, h_new_lens, nq, nkv, d, page_size, scale, dtype == torch.bfloat16, observe,
+                                                           KEY_WEIGHTS_SCORES)
 
 
 def key_weights_status() -> int:
@@ -1281,7 +1285,7 @@ def attention_key_weights(q: torch.Tensor, kv_layer: torch.Tensor, weights: torc
     given).  The portion's own places are set, also where nobody who is heard sees them.  ``h_prefix_lens``, ``h_new_lens``:
     the lengths on the host.  ``scratch``: float32, ``key_weights_scratch_floats`` of them (allocated where not given)."""
     if (_module or _faces()).attention_key_weights(q, kv_layer, weights, block_table, cu_seqlens, prefix_lens, h_prefix_lens, h_new_lens, nq, nkv, d, page_size,
-                                                   scale, observe, scratch):
+                                                   scale, observe, scratch, KEY_WEIGHTS_SCORES):
         launches["count"] += 3                                   # rows or scores, what joins them, columns
 
 
