@@ -285,7 +285,7 @@ std::vector<int> lengths(PyObject* o) {
 struct Plan { bool tensor_cores; int64_t floats, tokens, longest; };
 Plan plan(const std::vector<int>& prefix, const std::vector<int>& fresh, int nq, int nkv, int d, int page, float scale, int code, int observe, int most_scores) {
     if (entry.key_weights_tc_takes == nullptr) refuse("the kernels are not bound");
-    bool fits = nkv >= 1 && nq >= 0 && nq % nkv == 0 && prefix.size() == fresh.size();
+    bool fits = nkv >= 1 && nq >= 1 && nq % nkv == 0 && prefix.size() == fresh.size();
     Plan p{};
     for (size_t r = 0; fits && r < fresh.size(); ++r) {
         fits = prefix[r] >= 0 && fresh[r] >= 0;

@@ -326,7 +326,9 @@ static int each_run(Args& a, int requests, const int* prefix, const int* fresh, 
 using namespace lily;
 
 // Floats of scratch for portions of `fresh` tokens behind `prefix` places (host arrays): the scores of a run (about `most_scores` of them), the rows' parts, their lse.
+// (0 for heads that do not fit, which the launch refuses)
 LILY_API size_t lily_key_weights_floats(int requests, const int* prefix, const int* fresh, int observe, int nq, int nkv, int most_scores) {
+    if (nq <= 0 || nkv <= 0 || nq % nkv != 0) return 0;
     static thread_local keyw::Args a;
     a.nq = nq;
     a.nkv = nkv;

@@ -791,8 +791,9 @@ LILY_API int lily_key_weights_tc_takes(int nq, int nkv, int d, int page_size, fl
            scale < INFINITY;
 }
 
-// Floats of scratch for portions of `fresh` tokens behind `prefix` places (host arrays); 0: nothing to do or too much to number.
+// Floats of scratch for portions of `fresh` tokens behind `prefix` places (host arrays); 0: nothing to do, too much to number, or heads that these kernels do not take.
 LILY_API size_t lily_key_weights_tc_floats(int requests, const int* prefix, const int* fresh, int observe, int nq, int nkv) {
+    if (nq <= 0 || nkv <= 0 || nq % nkv != 0 || nq / nkv > keyw5::AR) return 0;
     static thread_local keyw5::Params p;
     size_t most = 0;
     for (int r = 0; r < requests; r += keyw5::MAX_R) {

@@ -1,0 +1,57 @@
+"""What the operators of a budgeted cache refuse on the host, looked at without a GPU: each call in a process of its own where a mistake would
+end it."""
+
+import subprocess
+import sys
+
+import pytest
+import torch
+
+
+def kernels():
+    """The package's operators with their library, where one can be built."""
+    from lily_b200.csrc import build, ops
+    try:
+        ops.library(), ops._faces()
+    except build.BuildError as exc:
+        pytest.skip(f"no kernel library here: {exc}")
+    return ops
+
+
+def outcome(lines):
+    """How a process that runs these lines ends: what it printed, or the signal that ended it."""
+    done = subprocess.run([sys.executable, "-c", lines], capture_output=True, text=True, timeout=300)
+    assert done.returncode >= 0, f"ended by signal {-done.returncode}"
+    assert done.returncode == 0, done.stderr[-2000:]
+    return done.stdout.strip()
+
+
+@pytest.mark.parametrize("nq,nkv", [(0, 4), (0, 1), (3, 4), (-4, 4), (4, 0), (4, -4)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_heads_that_do_not_fit_have_no_plan(nq, nkv, dtype):
+    kernels()
+    assert outcome(f"""
+import torch
+from lily_b200.csrc import ops
+try:
+    ops.key_weights_scratch_floats([0], [10], {nq}, {nkv}, 128, 16, 0.1, {dtype})
+except ops.KernelError as exc:
+    print("refused" if "query heads over" in str(exc) else exc)
+""") == "refused"
+
+
+@pytest.mark.parametrize("nq,nkv", [(0, 4), (3, 4), (4, 0), (129, 1)])
+def test_the_kernels_own_entries_size_nothing_for_heads_that_do_not_fit(nq, nkv):
+    kernels()
+    assert outcome(f"""
+import ctypes
+from lily_b200.csrc import ops
+one = (ctypes.c_int * 1)(10)
+lib = ops.library()
+for name, more in (("lily_key_weights_tc_floats", ()), ("lily_key_weights_floats", (1 << 28,))):
+    size = getattr(lib, name)
+    size.restype = ctypes.c_size_t
+    print(size(1, one, one, 0, {nq}, {nkv}, *more) > 0, end=" ")
+""") == ("False True" if (nq, nkv) == (129, 1) else "False False")
+
+
