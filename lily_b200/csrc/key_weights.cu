@@ -348,6 +348,7 @@ LILY_API int lily_key_weights(const void* q, const void* kv, float* weights, con
     LILY_REQUIRE(d >= 1 && page_size > 0 && (page_size & (page_size - 1)) == 0 && observe >= 0, "attention_key_weights: head size %d, pages of %d, the last %d heard", d, page_size,
                  observe);
     LILY_REQUIRE(dtype == kF32 || dtype == kBF16, "attention_key_weights: dtype %d", dtype);
+    LILY_REQUIRE(((uintptr_t)scratch & 15) == 0, "attention_key_weights: scratch must be 16-byte aligned");
     keyw::Args a{};
     a.q = q; a.kv = kv; a.weights = weights; a.scores = scratch; a.block_table = block_table; a.bt_stride = bt_stride; a.nq = nq; a.nkv = nkv; a.d = d;
     a.page_size = page_size; a.scale = scale;

@@ -55,3 +55,21 @@ for name, more in (("lily_key_weights_tc_floats", ()), ("lily_key_weights_floats
 """) == ("False True" if (nq, nkv) == (129, 1) else "False False")
 
 
+def answer(name, *args):
+    """What a kernels' own entry says to arguments that it refuses ahead of any launch (addresses that nothing is read from)."""
+    lib = kernels().library()
+    assert getattr(lib, name)(*args) != 0
+    return lib.lily_last_error().decode()
+
+
+@pytest.mark.parametrize("off", [4, 8, 12])
+def test_scratch_that_is_not_aligned_is_refused(off):
+    import ctypes
+    none, ten = (ctypes.c_int * 1)(0), (ctypes.c_int * 1)(10)
+    at = lambda x: ctypes.c_void_p(4096 + x)
+    said = answer("lily_key_weights", at(0), at(0), at(0), at(0), 1, at(off), 1, none, ten, 0, 4, 2, 48, 16, ctypes.c_float(0.1), 0, 1 << 28, None)
+    assert "16-byte aligned" in said
+    said = answer("lily_key_weights_tc", at(0), 10, at(0), 1, at(0), at(0), 1, at(off), 1, none, ten, 0, 4, 2, 64, 16, ctypes.c_float(0.1), None)
+    assert "16-byte aligned" in said
+    said = answer("lily_attention_decode_weighed", at(0), at(0), at(0), at(0), at(0), 1, at(0), at(off), 1, 16, 4, 2, 48, 16, 1, ctypes.c_float(0.1), 0, 1, None)
+    assert "16-byte aligned" in said
