@@ -6,8 +6,8 @@
 // the rest as it is; queries go to `q_out`, keys and values to the token's place in its request's pages.  (`qk_norm_rope_write` is the
 // case of one axis whose position is also the place.)  The reference's rotation is lily/layers/rotary.py:18-20, 70-87.
 //
-// A position outside the tables gives NaN (keys and queries that nobody can take for others); a place outside the block table, or in a
-// page outside the cache, is not written.
+// A position outside the tables gives NaN (keys and queries that nobody can take for others); a place or a request outside the block table, or
+// a page outside the cache, is not written.
 #include "common.cuh"
 
 namespace lily {
@@ -28,8 +28,8 @@ struct Args {
     int axes, tokens;
     const int* places;               // [tokens]
     const int* token_req;
-    const int* block_table;
-    int bt_stride;
+    const int* block_table;          // [requests, bt_stride]
+    int requests, bt_stride;
     void* kv;                        // [pages, 2, nkv, page_size, d]
     int pages;
     void* q_out;                     // [tokens, nq * d]
@@ -41,7 +41,7 @@ template <typename T>
 __device__ __forceinline__ T* target(const Args& a, int n, int head, int place, int req) {
     if (head < a.nq) return (T*)a.q_out + ((size_t)n * a.nq + head) * a.d;
     const int at = place / a.page_size;
-    if (place < 0 || at >= a.bt_stride) return nullptr;
+    if (place < 0 || at >= a.bt_stride || req < 0 || req >= a.requests) return nullptr;
     const int page = a.block_table[(size_t)req * a.bt_stride + at];
     if (page < 0 || page >= a.pages) return nullptr;
     return (T*)a.kv + (((size_t)page * 2 * a.nkv + (head - a.nq)) * a.page_size + place % a.page_size) * a.d;
@@ -316,7 +316,7 @@ using namespace lily;
 LILY_API int lily_axes_rope_write(const void* qkv, int in_dtype, int splits, size_t stride, int ld, const void* q_gain, const void* k_gain,
                                   int gain_dtype, float eps, const float* cos_t, const float* sin_t, int table_rows,
                                   const int* positions, const int* pair_axis, int axes, int tokens, const int* places,
-                                  const int* token_req, const int* block_table, int bt_stride, void* kv, int pages, void* q_out,
+                                  const int* token_req, const int* block_table, int requests, int bt_stride, void* kv, int pages, void* q_out,
                                   int act_dtype, int nq, int nkv, int d, int rd, int page_size, cudaStream_t stream) {
     if (tokens == 0) return 0;
     LILY_REQUIRE(d > 0 && rd >= 0 && rd <= d && rd % 2 == 0, "axes_rope_write: rotary_dim %d does not fit head_dim %d", rd, d);
@@ -327,7 +327,7 @@ LILY_API int lily_axes_rope_write(const void* qkv, int in_dtype, int splits, siz
     LILY_REQUIRE(act_dtype == kBF16 || gain_dtype == kF32 || q_gain == nullptr, "axes_rope_write: float32 heads keep float32 gains");
     LILY_REQUIRE(splits >= 1 && (splits == 1 || in_dtype == kF32), "axes_rope_write: partial sums are float32");
     const axes::Args a{qkv, stride, splits, ld, q_gain, k_gain, eps, cos_t, sin_t, table_rows, positions, pair_axis, axes, tokens, places, token_req,
-                       block_table, bt_stride, kv, pages, q_out, nq, nkv, d, rd, page_size};
+                       block_table, requests, bt_stride, kv, pages, q_out, nq, nkv, d, rd, page_size};
     const int bytes = act_dtype == kBF16 ? 2 : 4, piece = 16 / bytes, group = d / (2 * piece);
     int shift = 0;
     while (1 << shift < group) ++shift;

@@ -35,7 +35,7 @@ PyObject* kernel_error = nullptr;
 struct Entries {
     const char* (*last_error)();
     int (*axes_rope_write)(const void*, int, int, size_t, int, const void*, const void*, int, float, const float*, const float*, int, const int*, const int*, int, int,
-                           const int*, const int*, const int*, int, void*, int, void*, int, int, int, int, int, int, void*);
+                           const int*, const int*, const int*, int, int, void*, int, void*, int, int, int, int, int, int, void*);
     size_t (*decode_weighed_floats)(int, int, int, int, int, int, int);
     int (*decode_weighed)(const void*, const void*, float*, void*, const int*, int, const int*, float*, int, int, int, int, int, int, int, float, int, int, void*);
     int (*select_keys)(const float*, const int*, int, const int*, int*, int, int, int, int, int, int, int, int, int, void*);
@@ -190,7 +190,7 @@ PyObject* axes_rope_write(PyObject*, PyObject* const* p, Py_ssize_t count) {
         done("lily_axes_rope_write",
              call(entry.axes_rope_write, qkv.const_data_ptr(), in, narrow(splits), (size_t)stride, narrow(ld), q_gain ? q_gain->const_data_ptr() : nullptr,
                   k_gain ? k_gain->const_data_ptr() : nullptr, gain, eps, cos.const_data_ptr<float>(), sin.const_data_ptr<float>(), narrow(cos.size(0)), at, axis,
-                  narrow(positions.size(0)), narrow(n), to, of, bt, narrow(table.size(1)), kv.data_ptr(), narrow(kv.size(0)), q.data_ptr(), code, nq, nkv, d, rd, page, stream()));
+                  narrow(positions.size(0)), narrow(n), to, of, bt, narrow(table.size(0)), narrow(table.size(1)), kv.data_ptr(), narrow(kv.size(0)), q.data_ptr(), code, nq, nkv, d, rd, page, stream()));
         return THPVariable_Wrap(std::move(q));
     });
 }

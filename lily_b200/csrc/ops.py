@@ -1233,7 +1233,7 @@ def axes_rope_write(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_gain: O
     ``positions[pair_axis[j], token]`` (``positions`` int32 [axes, tokens], ``pair_axis`` int32 [rotary_dim / 2]: ``pair_axes``), q to
     ``q_out`` [tokens, nq * d], k and v to ``places[token]`` of the pages of request ``token_req[token]``.  ``qkv`` is [tokens,
     (nq + 2 nkv) d] in the cache's dtype or float32 partial sums [splits, tokens, ...], its rows ``row`` numbers apart.  A position outside the
-    tables gives NaN; a place outside the block table is not written."""
+    tables gives NaN; what has a place or a request outside the block table is not written."""
     q = (_module or _faces()).axes_rope_write(qkv, q_gain, k_gain, eps, cos, sin, positions, pair_axis, places, token_req, block_table, kv_layer, nq, nkv, d,
                                               rotary_dim, page_size, q_out, row)
     launches["count"] += 1
