@@ -320,6 +320,7 @@ LILY_API int lily_axes_rope_write(const void* qkv, int in_dtype, int splits, siz
                                   int act_dtype, int nq, int nkv, int d, int rd, int page_size, cudaStream_t stream) {
     if (tokens == 0) return 0;
     LILY_REQUIRE(d > 0 && rd >= 0 && rd <= d && rd % 2 == 0, "axes_rope_write: rotary_dim %d does not fit head_dim %d", rd, d);
+    LILY_REQUIRE(page_size > 0, "axes_rope_write: pages of %d places", page_size);
     LILY_REQUIRE(nq >= 0 && nkv >= 0 && nq + nkv > 0 && ld >= (nq + 2 * nkv) * d, "axes_rope_write: rows of %d numbers", ld);
     LILY_REQUIRE((q_gain == nullptr) == (k_gain == nullptr), "axes_rope_write: q and k gains come together");
     LILY_REQUIRE(act_dtype == kF32 || act_dtype == kBF16, "axes_rope_write: dtype %d", act_dtype);

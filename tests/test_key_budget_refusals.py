@@ -73,3 +73,20 @@ def test_scratch_that_is_not_aligned_is_refused(off):
     assert "16-byte aligned" in said
     said = answer("lily_attention_decode_weighed", at(0), at(0), at(0), at(0), at(0), 1, at(0), at(off), 1, 16, 4, 2, 48, 16, 1, ctypes.c_float(0.1), 0, 1, None)
     assert "16-byte aligned" in said
+
+
+@pytest.mark.parametrize("page", [0, -16])
+def test_pages_without_places_are_refused(page):
+    """(The kernel divides by the size of a page.)"""
+    import ctypes
+    at, f = ctypes.c_void_p(4096), ctypes.c_float
+    said = answer("lily_axes_rope_write", at, 1, 1, ctypes.c_size_t(0), 1024, None, None, 0, f(1e-6), at, at, 9, at, at, 1, 3, at, at, at, 1, 1, at, 0, at, 1, 4, 2, 128, 128, page, None)
+    assert "pages of" in said
+    said = answer("lily_attention_decode_weighed", at, at, at, at, at, 1, at, at, 1, 16, 4, 2, 64, page, 1, f(0.1), 1, 1, None)
+    assert "pages of" in said
+    said = answer("lily_key_weights", at, at, at, at, 1, at, 1, (ctypes.c_int * 1)(0), (ctypes.c_int * 1)(10), 0, 4, 2, 48, page, f(0.1), 0, 1 << 28, None)
+    assert "pages of" in said
+    said = answer("lily_select_keys", at, at, 1, at, at, 1, 2, 1, 2, page, 0, 4, 1, 1, None)
+    assert "page_size" in said
+    said = answer("lily_move_keys", at, at, at, 1, at, 1, at, 1, 2, 1, 2, page, 256, 4, 1, None)
+    assert "page_size" in said
