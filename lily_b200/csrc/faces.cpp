@@ -293,10 +293,13 @@ Plan plan(const std::vector<int>& prefix, const std::vector<int>& fresh, int nq,
         p.longest = std::max(p.longest, (int64_t)prefix[r] + fresh[r]);
     }
     if (!fits) refuse("attention_key_weights: portions of ", words(std::vector<int64_t>(fresh.begin(), fresh.end())), " behind ", words(std::vector<int64_t>(prefix.begin(), prefix.end())), ", ", nq, " query heads over ", nkv, " kv heads");
+    // (the kernels round places and tokens up to whole tiles in 32 bits)
+    if (std::max(p.longest, p.tokens) > INT32_MAX - 1024) refuse("attention_key_weights: kernels take 32-bit sizes, got ", p.longest, " places and ", p.tokens, " tokens");
     p.tensor_cores = code == BF16 && entry.key_weights_tc_takes(nq, nkv, d, page, scale);
     const int requests = (int)fresh.size();
     p.floats = (int64_t)(p.tensor_cores ? entry.key_weights_tc_floats(requests, prefix.data(), fresh.data(), observe, nq, nkv)
                                         : entry.key_weights_floats(requests, prefix.data(), fresh.data(), observe, nq, nkv, most_scores));
+    if (p.tokens > 0 && p.floats == 0) refuse("attention_key_weights: too many tiles for one call, ", p.tokens, " tokens of up to ", p.longest, " places");
     return p;
 }
 int observed(PyObject* o) {

@@ -756,18 +756,20 @@ static size_t plan(Params& p, int requests, const int* prefix, const int* fresh,
         q.tile0 = tile;
         q.step1 = (int)s1;
         q.step2 = (int)s2;
-        q.per1 = q.per2 = 0;
+        long long per1 = 0, per2 = 0;
         const int rows = row_tiles(q, p.tq), keys = key_tiles(q);
         q.row_steps = rows / 2;
-        for (int i = 0; i < rows; ++i) q.per1 += steps1_of(q, p.tq, i);
-        for (int i = 0; i < keys; ++i) q.per2 += steps2_of(q, p.tq, i);
-        s1 += (long long)q.per1 * nkv;
-        s2 += (long long)q.per2 * nkv;
+        for (int i = 0; i < rows; ++i) per1 += steps1_of(q, p.tq, i);
+        for (int i = 0; i < keys; ++i) per2 += steps2_of(q, p.tq, i);
+        s1 += per1 * nkv;
+        s2 += per2 * nkv;
+        if (s1 > 0x3fffffff || s2 > 0x3fffffff) return 0;
+        q.per1 = (int)per1;
+        q.per2 = (int)per2;
         unit += rows * nkv;
         tile += keys * nkv;
         first += fresh[r];
     }
-    if (s1 > 0x3fffffff || s2 > 0x3fffffff) return 0;
     const int sms = sm_count();
     p.units = unit;
     p.tiles = tile;
@@ -798,6 +800,7 @@ LILY_API size_t lily_key_weights_tc_floats(int requests, const int* prefix, cons
     size_t most = 0;
     for (int r = 0; r < requests; r += keyw5::MAX_R) {
         const size_t n = keyw5::plan(p, requests - r < keyw5::MAX_R ? requests - r : keyw5::MAX_R, prefix + r, fresh + r, observe, nq / nkv, nkv);
+        if (n == 0) return 0;
         most = n > most ? n : most;
     }
     return most;

@@ -90,3 +90,21 @@ def test_pages_without_places_are_refused(page):
     assert "page_size" in said
     said = answer("lily_move_keys", at, at, at, 1, at, 1, at, 1, 2, 1, 2, page, 256, 4, 1, None)
     assert "page_size" in said
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cached,new", [([2 ** 31 - 5], [100]), ([0], [2 ** 31 - 1]), ([2 ** 31 - 1], [2 ** 31 - 1]), ([0] * 3, [2 ** 30] * 3)])
+def test_places_and_tokens_that_pass_32_bits_have_no_plan(cached, new, dtype):
+    ops = kernels()
+    with pytest.raises(ops.KernelError, match="32-bit"):
+        ops.key_weights_scratch_floats(cached, new, 4, 4, 128, 16, 0.1, dtype)
+
+
+def test_portions_of_more_tiles_than_can_be_numbered_have_no_plan():
+    """A million tokens of 128 heads over one kv head: a tile of rows a token, each of up to 4,096 pieces of keys."""
+    ops = kernels()
+    floats = lambda n: ops.key_weights_scratch_floats([0], [n], 128, 1, 64, 64, 0.1, torch.bfloat16)
+    assert floats(1 << 18) > 0
+    for n in (1 << 20, 3 << 20):
+        with pytest.raises(ops.KernelError, match="too many tiles"):
+            floats(n)
