@@ -27,7 +27,8 @@ constexpr int MAX_R = 48;                 // requests a launch
 struct Portion {
     int request;                  // row of the block table
     int first, rows;              // row of q of the run's first token; rows
-    int place0, prefix, total;    // that token's place, cached places before and after the portion
+    int place0, last;             // the places of that token and of the run's last
+    int prefix, total;            // cached places before and after the portion
     int row_tiles, key_tiles;
     int tile0, rows0, cols0;      // its first tile of scores, tile of rows, tile of keys (of its first kv head)
 };
@@ -56,7 +57,7 @@ __device__ __forceinline__ const Portion& request_of(const Args& a, int& at) {
 
 // Whether a row of the run ahead of row `end` sees a place from `k0` on.  Both the kernel that makes tiles of scores and the one that reads them go by it: a tile
 // that it does not name is neither written nor read, whatever the run's last tile of rows is filled to.
-__device__ __forceinline__ bool seen(const Portion& p, int end, int k0, int group) { return k0 <= p.place0 + (min(end, p.rows) - 1) / group; }
+__device__ __forceinline__ bool seen(const Portion& p, int end, int k0, int group) { return k0 <= min(p.last, p.place0 + (end - 1) / group); }
 
 __device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
     unsigned long long r;
@@ -225,7 +226,7 @@ __global__ void __launch_bounds__(COL_THREADS) key_weights_columns_kernel(const 
     }
     float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
     // the tiles of rows that see any of these places (none where the run ends ahead of them)
-    const int tiles = seen(sp, sp.rows, k0, group) ? sp.row_tiles : 0, first = tiles ? max(0, k0 - sp.place0) * group / TM : 0;
+    const int tiles = k0 <= sp.last ? sp.row_tiles : 0, first = max(0, k0 - sp.place0) * group / TM;
     for (int t0 = first + part; t0 < tiles; t0 += 4 * parts) {
         float4 s[8];
         float e[8];
@@ -280,6 +281,7 @@ static Tiles plan(Args& a, int requests, int request0, int token0, const int* pr
             p.first = token0 + fresh[r] - heard + from;
             p.rows = mine * group;
             p.place0 = prefix[r] + fresh[r] - heard + from;
+            p.last = p.place0 + mine - 1;
             p.prefix = prefix[r];
             p.total = prefix[r] + fresh[r];
             p.row_tiles = (p.rows + TM - 1) / TM;
