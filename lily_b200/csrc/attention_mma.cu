@@ -1056,20 +1056,27 @@ LILY_API int lily_attention_decode_mma_clusters(int d, int splits, int group) {
     return 0;
 }
 
-// The host's word in which the decode kernel says that a wait for a tile ran out; made once, with the first launch that may, also while a
-// graph is captured.
+// A word of the host's memory (0) that kernels write, for good; also while a graph is captured.  Null: there is none.
+namespace lily {
+int* new_host_word() {
+    int* p = nullptr;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (cudaHostAlloc(reinterpret_cast<void**>(&p), sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
+        cudaGetLastError();
+        p = nullptr;
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (p) *p = 0;
+    return p;
+}
+}
+
+// The host's word in which the decode kernel says that a wait for a tile ran out; made once, with the first launch that may.
 static std::atomic<int*> g_lost_word{nullptr};
 static int* lost_word() {
     static int* word = [] {
-        int* p = nullptr;
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        if (cudaHostAlloc(reinterpret_cast<void**>(&p), sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
-            cudaGetLastError();
-            p = nullptr;
-        }
-        cudaThreadExchangeStreamCaptureMode(&mode);
-        if (p) *p = 0;
+        int* p = new_host_word();
         g_lost_word = p;
         return p;
     }();

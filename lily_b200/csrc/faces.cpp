@@ -42,7 +42,7 @@ struct Entries {
     int (*move_keys)(void*, float*, const int*, int, const int*, int, const int*, int, int, int, int, int, int, int, int, void*);
     int (*key_weights)(const void*, const void*, float*, const int*, int, float*, int, const int*, const int*, int, int, int, int, int, float, int, int, void*);
     size_t (*key_weights_floats)(int, const int*, const int*, int, int, int, int);
-    int (*key_weights_tc)(const void*, int, const void*, int, float*, const int*, int, float*, int, const int*, const int*, int, int, int, int, int, float, void*);
+    int (*key_weights_tc)(const void*, int, const void*, int, float*, const int*, int, float*, int, const int*, const int*, int, int, int, int, int, float, int, int, void*);
     size_t (*key_weights_tc_floats)(int, const int*, const int*, int, int, int);
     int (*key_weights_tc_takes)(int, int, int, int, float);
 } entry;
@@ -316,14 +316,15 @@ PyObject* key_weights_scratch_floats(PyObject*, PyObject* const* p, Py_ssize_t c
     });
 }
 
-// q, kv_layer, weights, block_table, cu_seqlens, prefix_lens, prefix lengths, new lengths, nq, nkv, d, page_size, scale, observe, scratch, scores kept at a time
+// q, kv_layer, weights, block_table, cu_seqlens, prefix_lens, prefix lengths, new lengths, nq, nkv, d, page_size, scale, observe, scratch, scores kept at a time, polls of the row
+// and of the column kernel
 PyObject* attention_key_weights(PyObject*, PyObject* const* p, Py_ssize_t count) {
-    return guarded(count, 16, [&]() -> PyObject* {
+    return guarded(count, 18, [&]() -> PyObject* {
         const char* what = "attention_key_weights";
         const Tensor &q = tensor(p[0]), &kv = tensor(p[1]), &weights = tensor(p[2]), &table = tensor(p[3]), &cu = tensor(p[4]), &cached = tensor(p[5]);
         const Tensor* room = maybe(p[14]);
         const std::vector<int> prefix = lengths(p[6]), fresh = lengths(p[7]);
-        const int nq = number(p[8]), nkv = number(p[9]), d = number(p[10]), page = number(p[11]), observe = observed(p[13]), most_scores = number(p[15]);
+        const int nq = number(p[8]), nkv = number(p[9]), d = number(p[10]), page = number(p[11]), observe = observed(p[13]), most_scores = number(p[15]), row_polls = number(p[16]), column_polls = number(p[17]);
         const float scale = real(p[12]);
         const int64_t requests = (int64_t)fresh.size();
         if ((int64_t)prefix.size() != requests || cu.numel() != requests + 1 || cached.numel() != requests || !is(cu, at::kInt) || !is(cached, at::kInt))
@@ -342,7 +343,8 @@ PyObject* attention_key_weights(PyObject*, PyObject* const* p, Py_ssize_t count)
         Tensor scratch = room ? *room : at::empty({plan_.floats}, weights.options());
         if (plan_.tensor_cores)
             done("lily_key_weights_tc", call(entry.key_weights_tc, q.const_data_ptr(), narrow(q.size(0)), kv.const_data_ptr(), narrow(kv.size(0)), weights.data_ptr<float>(), table.const_data_ptr<int>(),
-                                             width, scratch.data_ptr<float>(), (int)requests, prefix.data(), fresh.data(), observe, nq, nkv, d, page, scale, stream()));
+                                             width, scratch.data_ptr<float>(), (int)requests, prefix.data(), fresh.data(), observe, nq, nkv, d, page, scale, row_polls, column_polls,
+                                             stream()));
         else
             done("lily_key_weights", call(entry.key_weights, q.const_data_ptr(), kv.const_data_ptr(), weights.data_ptr<float>(), table.const_data_ptr<int>(), width, scratch.data_ptr<float>(),
                                           (int)requests, prefix.data(), fresh.data(), observe, nq, nkv, d, page, scale, code, most_scores, stream()));

@@ -22,12 +22,17 @@
 // 10); the last 64 of 1,024 tokens behind 15,360 places 36.7.  The CUDA cores of key_weights.cu take 768 for the first, and on the same pages 12.6 for 16 tokens (here 9.5),
 // 17.8 for 128 (13.0); they are ahead for 300 tokens of seven heads of 64 over one (14.6, here 17.4), where a dozen tiles leave most SMs idle either way.
 //
-// Every wait is bounded: one that runs out sets a status word (lily_key_weights_status), the roles leave their loops and the block frees its
-// tensor memory; the weights are then void (NaN, or some of them as they were).
+// Every wait is bounded: one that runs out says so in a word of the host's memory (lily_key_weights_status), the roles leave their loops, what the block
+// has on its way is waited for (bounded too), its tensor memory is freed, and what it was to write becomes NaN: the parts of its row tiles, from which all
+// that these rows give is NaN, or the weights of its key tiles.  Nothing of it is left to the next call.
 #include "common.cuh"
 #include "tcgen05.cuh"
 
+#include <atomic>
+
 namespace lily {
+int* new_host_word();
+
 namespace keyw5 {
 
 using namespace tc5;
@@ -38,10 +43,7 @@ constexpr int STAGES = 2;
 constexpr int GROUPS = 4;                 // groups of four warps: two pairs that take steps in turn, each group half of a step's columns
 constexpr int COLS = BR / 2;
 constexpr int THREADS = 64 + GROUPS * 128;
-constexpr uint32_t SPIN_LIMIT = 1u << 24;
 constexpr float LOG2E = 1.4426950408889634f;
-
-__device__ int g_status = 0;              // 0 ok; else (code << 24 | block) of the first wait that gave up
 
 // One request of a launch.
 struct Portion {
@@ -64,6 +66,8 @@ struct Params {
     float c;                              // scale * log2 e
     float per_step;                       // 1 / (2 tq)
     int page_shift;
+    int polls[2];                         // polls before a wait of the row, the column kernel gives up
+    int* lost;                            // a word of the host's where it says so
     Portion p[MAX_R];
 };
 
@@ -94,18 +98,24 @@ constexpr int NUM_BARS = 4 + 2 * STAGES + 4 + 2 * LSE + SUMS;
 constexpr int off_misc(int d) { return off_bars(d) + 8 * NUM_BARS; }
 constexpr int smem_bytes(int d) { return off_misc(d) + 128; }
 
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
-    for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
+// How the waits of a block end when what they wait for does not come.
+struct Waits { volatile int* abort; int* lost; int polls; };
+__device__ __forceinline__ void give_up(const Waits& w, int code) {
+    *w.abort = 1;
+    *(volatile int*)w.lost = (code << 24) | (int)(blockIdx.x & 0xFFFFFF);
+    __threadfence_system();
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Waits& w, int code) {
+    for (int i = 0; i < w.polls; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 1023u) == 1023u && *abort_flag) return false;
+        if ((i & 1023) == 1023 && *w.abort) return false;
     }
-    *abort_flag = 1;
-    atomicCAS(&g_status, 0, (code << 24) | (int)(blockIdx.x & 0xFFFFFF));
+    give_up(w, code);
     return false;
 }
 // The same for a whole warp, whose lanes then agree.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, code));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const Waits& w, int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, w, code));
 }
 __device__ __forceinline__ void mbar_arrive_many(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0], %1;\n" ::"r"(bar), "r"(count) : "memory");
@@ -286,6 +296,19 @@ __device__ Cursor find(const Params& p, int g) {
     return c;
 }
 
+// What a block was to write of its `mine` steps from `g0` on, made NaN by all its threads.
+template <int PASS>
+__device__ __forceinline__ void make_void(const Params& p, int g0, int mine) {
+    const float nan = __int_as_float(0x7fffffff);
+    Cursor c = find<PASS>(p, g0);
+    for (int k = 0; k < mine; k += c.n - c.s, next_tile<PASS>(p, c)) {
+        if (PASS == 1)
+            for (int i = threadIdx.x; i < GROUPS * AR; i += THREADS) p.parts[(size_t)(c.unit + (int)blockIdx.x) * GROUPS * AR + i] = make_float2(-INFINITY, nan);
+        else if (const int place = c.i * AR + (int)threadIdx.x; threadIdx.x < AR && place < c.total)
+            p.weights[(((size_t)p.block_table[(size_t)c.r * p.bt_stride + (place >> p.page_shift)] * p.nkv + c.kvh) << p.page_shift) + (place & (p.page_size - 1))] = nan;
+    }
+}
+
 template <int D, int PASS>
 __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv,
                                                                     const __grid_constant__ Params p) {
@@ -299,13 +322,20 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
     int& abort_s = *reinterpret_cast<int*>(smem + off_misc(D) + 4);
     int4* desc_s = reinterpret_cast<int4*>(smem + off_desc(D));       // [LSE][2]
     Cursor& start_s = *reinterpret_cast<Cursor*>(smem + off_misc(D) + 8);
+    static_assert(sizeof(Cursor) <= 56, "");
+    int* issued_s = reinterpret_cast<int*>(smem + off_misc(D) + 64);  // what was put on its way: standing tiles, stages, lse, products
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t base = smem_u32(smem);
     const uint32_t a_smem = base, b_smem = base + off_b(D);
     const uint32_t a_full = smem_u32(bars), a_empty = a_full + 16, b_full = a_empty + 16, b_empty = b_full + 8 * STAGES, s_full = b_empty + 8 * STAGES,
                    s_empty = s_full + 16, l_full = s_empty + 16, l_empty = l_full + 8 * LSE, sums_full = l_empty + 8 * LSE;
+    const int steps = PASS == 1 ? p.steps1 : p.steps2, quota = PASS == 1 ? p.quota1 : p.quota2;
+    const int g0 = blockIdx.x * quota, mine = min(quota, steps - g0);
+    const Waits waits{&abort_s, p.lost, p.polls[PASS - 1]};
     if (base & 1023u) {                                               // the swizzled tiles need it; never seen, but checked
-        if (threadIdx.x == 0) atomicCAS(&g_status, 0, (11 << 24) | (int)(blockIdx.x & 0xFFFFFF));
+        if (threadIdx.x == 0) give_up(waits, 11);
+        pdl_wait();
+        make_void<PASS>(p, g0, mine);
         return;
     }
     if (threadIdx.x == 0) {
@@ -344,8 +374,6 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
     }
     const int group_rows = p.group * p.tq;
-    const int steps = PASS == 1 ? p.steps1 : p.steps2, quota = PASS == 1 ? p.quota1 : p.quota2;
-    const int g0 = blockIdx.x * quota, mine = min(quota, steps - g0);
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_base_s)), "r"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
@@ -358,7 +386,6 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base_s;
-    volatile int* abort_flag = &abort_s;
     Cursor cur = start_s;
     // The column kernel's loader, products and waits begin ahead of the wait for the join kernel: queries and keys were there before the row
     // kernel began.  What reads the lse (the loader, further down) or writes waits.
@@ -395,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
         look_ahead(true);
         for (int k = 0; k < mine && ok; ++k) {
             if (k == 0 || cur.s == 0) {                               // a new standing tile
-                ok = warp_wait(a_empty + 8 * (tile & 1), ((tile >> 1) & 1) ^ 1, abort_flag, 1);
+                ok = warp_wait(a_empty + 8 * (tile & 1), ((tile >> 1) & 1) ^ 1, waits, 1);
                 if (!ok) break;
                 const uint32_t bar = a_full + 8 * (tile & 1), dst = a_smem + (tile & 1) * a_bytes(D);
                 if (lane == 0) mbar_expect_tx(bar, PASS == 1 ? q_bytes : a_bytes(D));
@@ -409,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
                 alone += share_n == cur.n;
             }
             const int st = k % STAGES;
-            ok = warp_wait(b_empty + 8 * st, ((k / STAGES) & 1) ^ 1, abort_flag, 2);
+            ok = warp_wait(b_empty + 8 * st, ((k / STAGES) & 1) ^ 1, waits, 2);
             if (!ok) break;
             const uint32_t bar = b_full + 8 * st, dst = b_smem + st * b_bytes(D);
             const int t0 = PASS == 2 ? 2 * (cur.f + cur.s) : 0, unit = cur.unit0 + cur.kvh * 2 * p.p[cur.r].row_steps + t0;      // columns: the step's row tiles
@@ -432,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
             ++sent_b;
             if (PASS == 2 && k == 0) pdl_wait();
             const int ls = k % LSE, begin = g0 + k - cur.s, j = k - share_k;
-            ok = warp_wait(l_empty + 8 * ls, ((k / LSE) & 1) ^ 1, abort_flag, 3);           // step k - LSE has been read
+            ok = warp_wait(l_empty + 8 * ls, ((k / LSE) & 1) ^ 1, waits, 3);           // step k - LSE has been read
             if (!ok) break;
             held = false;
             if (PASS == 2) {
@@ -457,28 +484,20 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
             if (fresh) next_tile<PASS>(p, cur);
             if (k + 1 < mine) look_ahead(fresh);
         }
-        if (*abort_flag && lane == 0) {
-            // copies already issued still land in this block's shared memory: give each a bounded wait
-            for (int j = max(0, sent_a - 2); j < sent_a; ++j)
-                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(a_full + 8 * (j & 1), (j >> 1) & 1); ++i) {}
-            for (int j = max(0, sent_b - STAGES); j < sent_b; ++j)
-                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(b_full + 8 * (j % STAGES), (j / STAGES) & 1); ++i) {}
-            for (int j = max(0, sent_l - LSE); j < sent_l; ++j)
-                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(l_full + 8 * (j % LSE), (j / LSE) & 1); ++i) {}
-        }
+        if (lane == 0) issued_s[0] = sent_a, issued_s[1] = sent_b, issued_s[2] = sent_l;
     } else if (warp == 1) {
         // ---- products: accumulator k & 1 = standing tile x streamed tile of step k ----
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BR >> 3) << 17) | ((uint32_t)(AR >> 4) << 24);
         bool ok = true;
-        int tile = -1;
-        for (int k = 0; k < mine && ok; ++k) {
+        int tile = -1, k = 0;
+        for (; k < mine; ++k) {
             const int st = k % STAGES;
             if (k == 0 || cur.s == 0) {
                 ++tile;
-                ok = warp_wait(a_full + 8 * (tile & 1), (tile >> 1) & 1, abort_flag, 4);
+                ok = warp_wait(a_full + 8 * (tile & 1), (tile >> 1) & 1, waits, 4);
                 if (!ok) break;
             }
-            ok = warp_wait(b_full + 8 * st, (k / STAGES) & 1, abort_flag, 5) && warp_wait(s_empty + 8 * (k & 1), ((k >> 1) & 1) ^ 1, abort_flag, 6);
+            ok = warp_wait(b_full + 8 * st, (k / STAGES) & 1, waits, 5) && warp_wait(s_empty + 8 * (k & 1), ((k >> 1) & 1) ^ 1, waits, 6);
             if (!ok) break;
             tc_fence_after();
             const bool last = cur.s + 1 == cur.n || k + 1 == mine;
@@ -495,6 +514,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
             __syncwarp();
             if (++cur.s == cur.n) next_tile<PASS>(p, cur);
         }
+        if (lane == 0) issued_s[3] = k;
     } else {
         // ---- groups of 128 threads, a lane of tensor memory each: pair k & 1 takes step k, each of its groups 128 columns ----
         const int which = (warp - 2) >> 2, pair = which >> 1, half = which & 1, quarter = warp & 3, row = quarter * 32 + lane;
@@ -506,7 +526,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
         float old = 0.f;
         for (int k = pair; k < mine; k += 2) {
             const int ls = k % LSE;
-            if (!warp_wait(l_full + 8 * ls, (k / LSE) & 1, abort_flag, 8)) break;
+            if (!warp_wait(l_full + 8 * ls, (k / LSE) & 1, waits, 8)) break;
             const int4 d0 = desc_s[2 * ls], d1 = desc_s[2 * ls + 1];
             const Step st{d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
             const bool collects = PASS == 2 && (st.flags & (EVEN | ALONE)) == (EVEN | ALONE) && half == 0;
@@ -524,7 +544,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
                     }
                 }
             }
-            if (!warp_wait(s_full + 8 * pair, (k >> 1) & 1, abort_flag, 7)) break;
+            if (!warp_wait(s_full + 8 * pair, (k >> 1) & 1, waits, 7)) break;
             tc_fence_after();
             // Pieces of 32 columns, which a warp leaves out where no lane sees any of them and masks where not all are seen: rows and keys ascend
             // along lanes and columns, so the first and the last say which it is.
@@ -620,7 +640,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
                     // twelve warps' worth of arrivals, of three groups or of one
                     if (lane == 0) mbar_arrive_many(full, st.flags & SINGLE ? 3 : 1);
                 } else {
-                    if (!warp_wait(full, (at / SUMS) & 1, abort_flag, 9)) break;
+                    if (!warp_wait(full, (at / SUMS) & 1, waits, 9)) break;
                     const int parts = st.flags & SINGLE ? 2 : 4;
                     float w = old;
                     for (int j = 0; j < parts; ++j) w += sums[j * AR + row];
@@ -656,6 +676,23 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_tc_kernel(const __grid
     if (PASS == 2) pdl_launch_dependents();
     tc_fence_before();
     __syncthreads();
+    if (*waits.abort) {
+        // Every role has left.  Copies on their way still land in this block's shared memory and products in its tensor memory: each gets a bounded wait.
+        if (threadIdx.x == 0) {
+            for (int j = max(0, issued_s[0] - 2); j < issued_s[0]; ++j)
+                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(a_full + 8 * (j & 1), (j >> 1) & 1); ++i) {}
+            for (int j = max(0, issued_s[1] - STAGES); j < issued_s[1]; ++j)
+                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(b_full + 8 * (j % STAGES), (j / STAGES) & 1); ++i) {}
+            for (int j = max(0, issued_s[2] - LSE); j < issued_s[2]; ++j)
+                for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(l_full + 8 * (j % LSE), (j / LSE) & 1); ++i) {}
+        }
+        if (warp == 1 && issued_s[3] > 0) {
+            const int k = issued_s[3] - 1;
+            for (uint32_t i = 0; i < (1u << 20) && !mbar_try_wait(s_full + 8 * (k & 1), (k >> 1) & 1); ++i) {}
+            __syncwarp();
+        }
+        make_void<PASS>(p, g0, mine);
+    }
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512) : "memory");
@@ -712,7 +749,6 @@ __global__ void __launch_bounds__(JOIN_THREADS) key_weights_join_kernel(const __
         m = -INFINITY, l = 0.f;
         for (int u = 0; u < subs; ++u) join_part(m, l, part_s[u][row]);
         lse = -(m + log2f(l));
-        if (*(volatile int*)&g_status) lse = __int_as_float(0x7fffffff);                  // a wait of the row kernel gave up: its parts are void
     }
     p.lse[(size_t)unit * AR + row] = lse;
 }
@@ -806,17 +842,30 @@ LILY_API size_t lily_key_weights_tc_floats(int requests, const int* prefix, cons
     return most;
 }
 
-// 0, or (code << 24 | block) of the first bounded wait that gave up (synchronises; the word is cleared when read).
-LILY_API int lily_key_weights_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, keyw5::g_status, sizeof(int)) != cudaSuccess) return -1;
-    if (v != 0) cudaMemcpyToSymbol(keyw5::g_status, &zero, sizeof(int));
+// The host's word in which these kernels say that a wait ran out; made with the first launch that may.
+static std::atomic<int*> g_lost_word{nullptr};
+static int* lost_word() {
+    static int* word = [] {
+        int* p = new_host_word();
+        g_lost_word = p;
+        return p;
+    }();
+    return word;
+}
+
+// 0, or (code << 24 | block) of a bounded wait that gave up since the last call; clears it.  `wait`: behind all work of the device; else as far as the host
+// knows (the kernels it has waited for).
+LILY_API int lily_key_weights_status(int wait) {
+    if (wait && cudaDeviceSynchronize() != cudaSuccess) return -1;
+    volatile int* word = g_lost_word;
+    const int v = word ? *word : 0;
+    if (v != 0) *word = 0;
     return v;
 }
 
 LILY_API int lily_key_weights_tc(const void* q, int tokens, const void* kv, int pages, float* weights, const int* block_table, int bt_stride, float* scratch,
                                  int requests, const int* prefix, const int* fresh, int observe, int nq, int nkv, int d, int page_size, float scale,
-                                 cudaStream_t stream) {
+                                 int row_polls, int column_polls, cudaStream_t stream) {
     LILY_REQUIRE(lily_key_weights_tc_takes(nq, nkv, d, page_size, scale), "attention_key_weights: the tcgen05 kernels do not take %d heads over %d of %d, pages of %d", nq, nkv, d, page_size);
     LILY_REQUIRE((((uintptr_t)q | (uintptr_t)kv | (uintptr_t)scratch) & 15) == 0, "attention_key_weights: operands must be 16-byte aligned");
     tc5::EncodeTiled enc = tc5::encoder();
@@ -840,6 +889,10 @@ LILY_API int lily_key_weights_tc(const void* q, int tokens, const void* kv, int 
         LILY_REQUIRE(rc == CUDA_SUCCESS, "attention_key_weights: cuTensorMapEncodeTiled (cache) failed with %d", (int)rc);
     }
     keyw5::Params p{};
+    p.polls[0] = row_polls;
+    p.polls[1] = column_polls;
+    p.lost = lost_word();
+    LILY_REQUIRE(p.lost != nullptr, "attention_key_weights: no word of the host's memory");
     int row0 = 0;
     for (int r = 0; r < requests; r += keyw5::MAX_R) {
         const int some = requests - r < keyw5::MAX_R ? requests - r : keyw5::MAX_R;

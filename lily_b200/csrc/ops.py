@@ -137,7 +137,6 @@ def library():
         lib.lily_attention_decode_scratch_floats.restype = _sz
         lib.lily_attention_decode_weighed_floats.argtypes = [_i, _i, _i, _i, _i, _i, _i]
         lib.lily_attention_decode_weighed_floats.restype = _sz
-        lib.lily_key_weights_status.restype = _i
         lib.lily_normed_mean_max.restype = _i
         lib.lily_row_cluster_threads.argtypes = [_i]
         lib.lily_row_cluster_threads.restype = _i
@@ -1270,10 +1269,19 @@ def key_weights_scratch_floats(h_prefix_lens: Sequence[int], h_new_lens: Sequenc
                                                            KEY_WEIGHTS_SCORES)
 
 
+KEY_WEIGHTS_POLLS = (1 << 24, 1 << 24)      # how often a wait of the row, the column kernel of `attention_key_weights` (tcgen05) asks before it gives up
+
+
 def key_weights_status() -> int:
-    """0, or a code of the first bounded wait that gave up in the tcgen05 kernels of ``attention_key_weights`` (its weights are NaN;
-    synchronises, and clears the code)."""
-    return int(library().lily_key_weights_status())
+    """0, or a code of a bounded wait that gave up in the tcgen05 kernels of ``attention_key_weights`` since the code was last read
+    (synchronises, and clears it).  What the block with that wait was to give is NaN: all weights of its key tiles, or all that its rows
+    give to the places they see; other calls are not touched."""
+    return int(library().lily_key_weights_status(1))
+
+
+def key_weights_lost() -> int:
+    """``key_weights_status`` for the kernels that the host has waited for; waits for nothing."""
+    return int(library().lily_key_weights_status(0))
 
 
 def attention_key_weights(q: torch.Tensor, kv_layer: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor,
@@ -1285,7 +1293,7 @@ def attention_key_weights(q: torch.Tensor, kv_layer: torch.Tensor, weights: torc
     given).  The portion's own places are set, also where nobody who is heard sees them.  ``h_prefix_lens``, ``h_new_lens``:
     the lengths on the host.  ``scratch``: float32, ``key_weights_scratch_floats`` of them (allocated where not given)."""
     if (_module or _faces()).attention_key_weights(q, kv_layer, weights, block_table, cu_seqlens, prefix_lens, h_prefix_lens, h_new_lens, nq, nkv, d, page_size,
-                                                   scale, observe, scratch, KEY_WEIGHTS_SCORES):
+                                                   scale, observe, scratch, KEY_WEIGHTS_SCORES, *KEY_WEIGHTS_POLLS):
         launches["count"] += 3                                   # rows or scores, what joins them, columns
 
 
