@@ -24,6 +24,7 @@ import torch
 
 from lily_b200.cache.key_budget import KeyBudget
 from lily_b200.cache.kv_cache import KVCacheManager
+from lily_b200.csrc.waits import Listener
 from lily_b200.parts.base import CacheNeed
 
 
@@ -62,6 +63,7 @@ class AttentionStack:
         self.pair_axis = ops.pair_axes(sections, self.device)
         angle = torch.outer(torch.arange(max_position, dtype=torch.float32), 1.0 / 10000.0 ** (torch.arange(0, d, 2, dtype=torch.float32) / d))
         self.cos, self.sin = angle.cos().to(self.device), angle.sin().to(self.device)
+        self.check_waits = self.budget.check_waits if keep else Listener(ops).check        # raises when an attention kernel of a step that the host has waited for gave up a wait
         self.next_position = {}                       # by slot: the caller of a budgeted cache counts positions
 
     # ---- requests --------------------------------------------------------------------
@@ -182,6 +184,7 @@ def measure(args, keep: Optional[int]) -> dict:
         stack.budget.evict(slots, force=True)
     row = torch.randn(args.rows, args.width, device="cuda", generator=g)
     times = sorted(timed(lambda: stack.decode(slots, row)) for _ in range(args.steps))
+    stack.check_waits()
     data = stack.cache.groups[0].data
     return {"keep": keep, "prompt_ms": round(fill, 2), "decode_ms_median": round(times[len(times) // 2], 3), "decode_ms_worst": round(times[-1], 3),
             "places": stack.cache.lengths[slots[0]], "cache_mb": round(data.numel() * data.element_size() / 2 ** 20, 1)}

@@ -11,6 +11,9 @@ From then on a token's place in the cache is not its position: keys were rotated
 written and stay so, the next token is written behind the kept places (``ops.axes_rope_write`` takes place and position apart), and the
 caller counts positions.  ``slack`` spreads the cost: with 128 a request is evicted once in 128 decoded tokens.
 
+A key that was let go of does not come back, so an eviction first waits for the work that the weights come from and looks whether a kernel of
+it gave up a wait (``check_waits``): it raises then, and nothing has been let go of.
+
 The reference keeps every key of a request until it ends (lily/mem_cache/memory_pool.py:78-143) or slides a window.
 """
 
@@ -22,6 +25,7 @@ import numpy as np
 import torch
 
 from lily_b200.cache.kv_cache import KVCacheManager
+from lily_b200.csrc.waits import Listener
 
 
 class KeyBudget:
@@ -38,7 +42,7 @@ class KeyBudget:
             raise ValueError("a mixer with a state of its own does not live on cached keys alone")
         if ops is None:
             from lily_b200.csrc import ops
-        self.cache, self.ops = cache, ops
+        self.cache, self.ops, self._waits = cache, ops, Listener(ops)
         self.keep, self.first, self.recent, self.slack = keep, first, recent, slack
         self.weights: List[torch.Tensor] = [
             torch.zeros((g.num_layers, cache.num_pages + 1, g.need.kv_heads, cache.page_size), dtype=torch.float32, device=cache.device) for g in cache.groups]
@@ -60,16 +64,25 @@ class KeyBudget:
             host[i, :len(r)] = r
         return torch.from_numpy(host).to(self.cache.device, non_blocking=True)
 
+    def check_waits(self, wait: bool = False) -> None:
+        """Raises when a kernel that weighs keys gave up a wait of its own, so that what came of its step is void: in the work that the host has waited
+        for, or (``wait``) in all that is enqueued on the current stream."""
+        if wait and torch.device(self.cache.device).type == "cuda":
+            torch.cuda.current_stream(self.cache.device).synchronize()
+        self._waits.check()
+
     def evict(self, slots: Sequence[int], force: bool = False) -> List[int]:
         """Brings those of these requests that hold ``slack`` places or more past the budget (with ``force``: any past it) back to it and
-        gives their slots.  Enqueued on the current stream; the pages behind are free for what is enqueued after."""
+        gives their slots.  Where there are some, the host first waits for the current stream and looks for waits that ran out
+        (``check_waits``); the rest is enqueued, and the pages behind are free for what is enqueued after."""
         over = [s for s in slots if self.cache.lengths[s] >= self.keep + (1 if force else self.slack)]
         if not over:
             return []
         held = [self.cache.lengths[s] for s in over]
         lengths = torch.tensor(held, dtype=torch.int32).to(self.cache.device, non_blocking=True)
-        for g, group in enumerate(self.cache.groups):
-            table = self.table(g, over)
+        tables = [self.table(g, over) for g in range(len(self.cache.groups))]
+        self.check_waits(wait=True)
+        for g, (group, table) in enumerate(zip(self.cache.groups, tables)):
             kept = self.ops.select_keys(self.weights[g], table, lengths, max(held), self.keep, self.first, self.recent)
             self.ops.move_keys(group.data, self.weights[g], table, kept)
         for s in over:

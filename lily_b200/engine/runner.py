@@ -25,6 +25,7 @@ from lily_b200.cache.kv_cache import KVCacheManager, OutOfPages, bytes_per_token
 from lily_b200.config.model_config import read_model_dir
 from lily_b200.config.registry import architecture_names, resolve_architecture
 from lily_b200.config.server_args import ServerArgs
+from lily_b200.csrc.waits import DECODE as _LOST
 from lily_b200.engine import check
 from lily_b200.engine.batch import FUTURE, Lane, StepBatch, StepEntry, Workspace, build_step_batch, order_entries, rows_are_even, wire_array
 from lily_b200.engine.profiler import DecodeProfiler
@@ -74,26 +75,6 @@ def _load_library_products(device) -> None:
 
 
 _CAPTURING = threading.local()
-
-
-class _Lost:
-    """The waits that kernels of this process gave up, as the host has heard of them.  The kernels share one word, which its reader clears,
-    and it does not say whose step it was: so every runner hears of each, whichever of them read the word."""
-
-    def __init__(self):
-        self.lock = threading.Lock()
-        self.count = self.row = 0
-
-    def heard(self, read) -> int:
-        with self.lock:
-            found = read()
-            if found:
-                self.count += 1
-                self.row = found
-            return self.count
-
-
-_LOST = _Lost()
 
 
 def _lane_streams(device, count: int, library: bool) -> List["torch.cuda.Stream"]:
