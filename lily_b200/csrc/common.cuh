@@ -91,6 +91,14 @@ inline int sm_count() {
     return sms;
 }
 
+// Makes the device's context the calling thread's, once a thread.  The runtime does so with a thread's first call that needs it, but calls of the driver (the
+// encoder of tensor maps) do not, and a thread whose first call is one of these has none.
+inline void bind_thread() {
+    static thread_local bool bound = false;
+    int dev = 0;
+    if (!bound) bound = cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+}
+
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 

@@ -483,6 +483,7 @@ static EncodeTiled encoder() {
             q == cudaDriverEntryPointSuccess)
             fn = (EncodeTiled)p;
     });
+    lily::bind_thread();
     return fn;
 }
 

@@ -142,6 +142,7 @@ inline EncodeTiled encoder() {
             q == cudaDriverEntryPointSuccess)
             fn = (EncodeTiled)ptr;
     });
+    bind_thread();
     return fn;
 }
 
