@@ -11,6 +11,8 @@
 
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 namespace lily {
 bool attention_decode_f32_takes(const AttnArgs& a);
 int attention_decode_f32_weighed(const AttnArgs& a, int requests, cudaStream_t stream);
@@ -240,8 +242,8 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
 // Shared memory: [1024-byte aligned] key tiles, value tiles, queries; behind them, in a cluster, what the other blocks send.
 __host__ __device__ constexpr size_t tiles_bytes(int d) { return 1024 + 2 * (size_t)stages_of(d) * BN * d * 2 + 16 * (size_t)d * 2; }
 // Output sums a block of a cluster of `splits` blocks finishes: its share of rows x d.
-__host__ __device__ inline int cluster_share(int rows, int d, int splits) { return ((rows * d + splits - 1) / splits + 3) / 4 * 4; }
-inline size_t recv_bytes(int rows, int d, int splits) { return ((size_t)splits * cluster_share(rows, d, splits) + (size_t)splits * 32) * sizeof(float); }
+__host__ __device__ constexpr int cluster_share(int rows, int d, int splits) { return ((rows * d + splits - 1) / splits + 3) / 4 * 4; }
+constexpr size_t recv_bytes(int rows, int d, int splits) { return ((size_t)splits * cluster_share(rows, d, splits) + (size_t)splits * 32) * sizeof(float); }
 
 template <int D, bool CLUSTER, bool TMA>
 __global__ void __launch_bounds__(THREADS, 3) decode_weighed_mma_kernel(const DecodeArgs a, const int page_shift, const __grid_constant__ CUtensorMap map_kv) {
@@ -575,17 +577,24 @@ __global__ void __launch_bounds__(THREADS, 3) decode_weighed_mma_kernel(const De
     }
 }
 
-// Raises the kernel's limit of dynamic shared memory (once a size class, never lowered).
+// What any of the kernel's blocks may ask for.
+template <int D, bool CLUSTER>
+constexpr size_t most_smem() {
+    size_t most = 0;
+    for (int splits = 2; CLUSTER && splits <= MAX_CLUSTER; ++splits) most = recv_bytes(16, D, splits) > most ? recv_bytes(16, D, splits) : most;
+    return tiles_bytes(D) + most;
+}
+// Raises the kernel's limit of dynamic shared memory, once and to that: threads that launch other sizes at the same time set the same limit.
 template <int D, bool CLUSTER, bool TMA>
-static bool allow_smem(size_t bytes) {
-    static size_t granted = 0;
-    if (bytes > granted) {
-        if (cudaFuncSetAttribute(decode_weighed_mma_kernel<D, CLUSTER, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess ||
+static bool allow_smem() {
+    static std::atomic<bool> allowed{false};
+    if (!allowed) {
+        if (cudaFuncSetAttribute(decode_weighed_mma_kernel<D, CLUSTER, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most_smem<D, CLUSTER>()) != cudaSuccess ||
             (CLUSTER && cudaFuncSetAttribute(decode_weighed_mma_kernel<D, CLUSTER, TMA>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)) {
             cudaGetLastError();
             return false;
         }
-        granted = bytes;
+        allowed = true;
     }
     return true;
 }
@@ -598,7 +607,7 @@ static int launch_mma(DecodeArgs a, int requests, bool cluster, int page_shift, 
     a.longest_first = grid.x > 1 && grid.x <= THREADS && blocks > places && blocks <= (cluster ? 3 : 2) * places;
     if (cluster) {
         const size_t smem = tiles_bytes(D) + recv_bytes(rows, D, a.splits);
-        if (!allow_smem<D, true, TMA>(smem)) {
+        if (!allow_smem<D, true, TMA>()) {
             set_error("attention_decode_weighed: cannot get %zu bytes of shared memory in clusters", smem);
             return 2;
         }
@@ -620,7 +629,7 @@ static int launch_mma(DecodeArgs a, int requests, bool cluster, int page_shift, 
         return 0;
     }
     const size_t smem = tiles_bytes(D);
-    if (!allow_smem<D, false, TMA>(smem)) {
+    if (!allow_smem<D, false, TMA>()) {
         set_error("attention_decode_weighed: cannot get %zu bytes of shared memory", smem);
         return 2;
     }
@@ -647,7 +656,7 @@ static int cluster_room(int rows, int splits) {
         attr[0].val.clusterDim.z = splits;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        const bool ok = allow_smem<D, true, true>(smem) && cudaOccupancyMaxActiveClusters(&clusters, decode_weighed_mma_kernel<D, true, true>, &cfg) == cudaSuccess && clusters > 0;
+        const bool ok = allow_smem<D, true, true>() && cudaOccupancyMaxActiveClusters(&clusters, decode_weighed_mma_kernel<D, true, true>, &cfg) == cudaSuccess && clusters > 0;
         if (!ok) cudaGetLastError();
         k = ok ? clusters : -1;
     }

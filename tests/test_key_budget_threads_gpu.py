@@ -1,5 +1,8 @@
 """Threads of one process whose first call of all is one of the kernels'."""
 
+import os
+import subprocess
+import sys
 import threading
 
 import pytest
@@ -59,3 +62,39 @@ def test_a_thread_may_begin_with_a_kernel_whose_tiles_come_by_tma(kind):
     assert not isinstance(failed, Exception), failed
     torch.cuda.synchronize()
     assert same(out, want) and same(w, given)
+
+
+FIRST_CALLS = """
+import threading, torch
+from lily_b200.csrc import ops
+page, d, nq, nkv = {page}, {d}, 16, 4
+ops.library(), ops._faces()
+start, wrong, calls = threading.Barrier(12), [], []
+for i in range(12):
+    n = 256 << i % 4
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda")[None]
+    calls.append((torch.randn(1, nq * d, device="cuda", dtype=torch.bfloat16), torch.randn(n // page, 2, nkv, page, d, device="cuda", dtype=torch.bfloat16),
+                  torch.zeros(n // page, nkv, page, device="cuda"), table, torch.tensor([n], dtype=torch.int32, device="cuda"), n))
+torch.cuda.synchronize()
+def one(q, kv, w, table, lens, n):
+    start.wait()
+    try:
+        ops.attention_decode_weighed(q, kv, w, table, lens, n, nq, nkv, d, page, d ** -0.5)
+    except Exception as exc:
+        wrong.append(str(exc))
+threads = [threading.Thread(target=one, args=c) for c in calls]
+[t.start() for t in threads], [t.join() for t in threads]
+torch.cuda.synchronize()
+sums = [float(c[2].sum()) for c in calls]
+print(wrong or [s for s in sums if abs(s - nq) > 0.01] or "as asked")
+"""
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("page", [16, 64])
+def test_first_calls_of_several_threads_are_all_served(page, d):
+    """Clusters of 2 to 16 blocks, whose launches raise the kernel's limit of shared memory, in a process that has launched none."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(page=page, d=d)], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+    assert done.stdout.strip().endswith("as asked"), done.stdout[-2000:]
