@@ -75,8 +75,8 @@ class KeyBudget:
         """Brings those of these requests that hold ``slack`` places or more past the budget (with ``force``: any past it) back to it and
         gives their slots.  Where there are some, the host first waits for the current stream and looks for waits that ran out
         (``check_waits``); the rest is enqueued, and the pages behind are free for what is enqueued after."""
-        over = [s for s in slots if self.cache.lengths[s] >= self.keep + (1 if force else self.slack)]
-        if not over:
+        over = [s for s in dict.fromkeys(slots) if self.cache.lengths[s] >= self.keep + (1 if force else self.slack)]
+        if not over:                       # (a request that is named twice is moved once: two moves in place would meet)
             return []
         held = [self.cache.lengths[s] for s in over]
         lengths = torch.tensor(held, dtype=torch.int32).to(self.cache.device, non_blocking=True)

@@ -1,4 +1,4 @@
-"""A budget of cached keys hears of waits that kernels gave up before it lets go of anything."""
+"""What a budget of cached keys looks at before it lets go of anything: waits that kernels gave up, requests that are named twice."""
 
 import types
 
@@ -39,6 +39,15 @@ def test_nothing_is_let_go_of_where_a_wait_was_given_up(words, said):
         budget.evict([slot])
     assert torch.equal(cache.groups[0].data, data) and torch.equal(budget.weights[0], w) and cache.block_table(0, slot) == pages and cache.lengths[slot] == 13
     assert budget.evict([slot]) == [slot] and cache.lengths[slot] == 8          # heard once
+
+
+def test_a_request_that_is_named_twice_is_evicted_once(monkeypatch):
+    """Two lists of one request would be moved in place at the same time."""
+    ops = reporting()
+    cache, budget, slot = full(ops)
+    asked = []
+    monkeypatch.setattr(ops, "move_keys", lambda kv, w, table, kept: asked.append(table.shape[0]))
+    assert budget.evict([slot, slot]) == [slot] and asked == [1] and cache.lengths[slot] == 8
 
 
 def test_a_request_within_its_budget_asks_for_nothing():
