@@ -96,8 +96,9 @@ __global__ void __launch_bounds__(128) axes_rope_write_kernel(const Args a) {
 // warp), each with two pieces: of the rotated features N neighbouring ones and their partners rd / 2 further, of the rest two neighbouring pieces.  So the
 // rotation needs no exchange and the norm log2(G) shuffles.  The positions of up to four axes are read
 // beside the axes of a thread's pairs, not behind them.  What bounds it is the chain of reads (axis and positions, tables, result), for few tokens
-// and for many, which small blocks of short-lived threads hide best: 2,048 tokens of 32 + 2 x 8 heads of 128 in bfloat16 take 13.8 us (51 MB: 3.7 TB/s; a
-// plain copy of as many bytes 9.3; with the places read behind the tables 15.1), eight tokens out of four planes of partial sums 3.0.
+// and for many, which small blocks of short-lived threads hide best: 2,048 tokens of 32 + 2 x 8 heads of 128 in bfloat16, with gains, take 13.8 us (51 MB: 3.7 TB/s; a
+// plain copy of as many bytes 9.3; with the places read behind the tables 15.1), eight tokens out of four planes of partial sums 3.0.  (For many tokens the
+// chain does not explain it all: 8,192 take 4.1 times as long as 2,048, and each warp looks up what its token's other warps have looked up.)
 constexpr int WIDE_THREADS = 128, AHEAD = 4;
 
 // Numbers in pairs (mul and fma.rn.f32x2: two IEEE operations an instruction).
@@ -335,8 +336,9 @@ LILY_API int lily_axes_rope_write(const void* qkv, int in_dtype, int splits, siz
     const uintptr_t where = (uintptr_t)qkv | (uintptr_t)kv | (uintptr_t)q_out | (uintptr_t)q_gain | (uintptr_t)k_gain |
                             (uintptr_t)cos_t | (uintptr_t)sin_t | (uintptr_t)pair_axis;
     // Whole pieces of 16 bytes on every side; else, and for heads that are no power of two of pieces, a warp a head.  Measured, us, in pieces / a warp a
-    // head, on the same operands: 2,048 tokens of 48 heads of 128 in bfloat16 12.3 / 35.6 (axes in turn 15.2 / 35.3), eight tokens from four planes 3.1 / 5.4;
-    // float32, 1,000 tokens of 24 heads of 128 with half of each turned 8.0 / 8.4, of 64 5.1 / 7.9.
+    // head, on the same operands, other ones each call: 2,048 tokens of 48 heads of 128 in bfloat16 with gains 14.0 / 39.6 (axes in turn 16.2 / 39.1), without 11.6 / 39.7 (13.9 / 38.9),
+    // 8,192 tokens with gains 55.9 / 157, eight tokens 2.5 / 3.4, from four planes 3.3 / 5.4; float32 without gains, 1,000 tokens of 24 heads of 128 with half of each turned
+    // 8.1 / 10.2, of 64 5.1 / 7.9.
     const bool wide = d % (2 * piece) == 0 && 1 << shift == group && group <= 32 && rd % (2 * piece) == 0 && ld % piece == 0 &&
                       (in_dtype == act_dtype || ld % 4 == 0) && (size_t)stride % 4 == 0 && where % 16 == 0;
     const dim3 grid = wide ? dim3(tokens, (unsigned)((((nq + 2 * nkv) << shift) + axes::WIDE_THREADS - 1) / axes::WIDE_THREADS)) : dim3(tokens, (nq + 2 * nkv + 3) / 4);

@@ -1291,7 +1291,8 @@ def attention_key_weights(q: torch.Tensor, kv_layer: torch.Tensor, weights: torc
     column sums of the causal softmax of each request's new tokens (rows ``cu_seqlens`` of ``q`` [tokens, nq * d]) over its cached
     prefix and themselves, whose keys are in the cache already.  ``observe``: only the last that many tokens of each portion are heard (all where not
     given).  The portion's own places are set, also where nobody who is heard sees them.  ``h_prefix_lens``, ``h_new_lens``:
-    the lengths on the host.  ``scratch``: float32, ``key_weights_scratch_floats`` of them (allocated where not given)."""
+    the lengths on the host, by which the work is cut and which alone count; ``cu_seqlens`` and ``prefix_lens`` are the tensors that
+    ``attention_prefill`` takes for the same portions, looked at for their type and size and not read.  ``scratch``: float32, ``key_weights_scratch_floats`` of them (allocated where not given)."""
     if (_module or _faces()).attention_key_weights(q, kv_layer, weights, block_table, cu_seqlens, prefix_lens, h_prefix_lens, h_new_lens, nq, nkv, d, page_size,
                                                    scale, observe, scratch, KEY_WEIGHTS_SCORES, *KEY_WEIGHTS_POLLS):
         launches["count"] += 3                                   # rows or scores, what joins them, columns
