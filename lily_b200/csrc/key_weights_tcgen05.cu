@@ -181,7 +181,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 // The same on the multiply-add unit, for weights (x at most a little above 0, or NaN): x = i + f with |f| <= 1/2, 2^f by the polynomial of degree five whose largest
 // relative error is least (fitted by Lawson's iteration: 7.5e-8; 1.6e-7 with its coefficients rounded to float32, the constant term 1 + 2^-23 among them, and
-// 2.3e-7 as computed, where ex2.approx has 1.2e-7: of a weight, beside scores whose own rounding is worth some 1e-6 of it), 2^i by its exponent; below 2^-126.5 it is 0.
+// 2.3e-7 as computed), 2^i by its exponent; below 2^-126.5 it is 0.
 __device__ __forceinline__ Two exp2_by_terms(Two x) {
     constexpr float SHIFT = 12582912.f + 127.f;                       // 1.5 * 2^23: the sum's last bits are i + 127
     float a, b;
