@@ -34,17 +34,19 @@ struct Args {
     int pages;
     void* q_out;                     // [tokens, nq * d]
     int nq, nkv, d, rd, page_size;
+    int page_shift;                  // log2 of page_size, or -1
 };
 
 // Where a head of a token goes: its row of `q_out` or of a page (null: nowhere).
 template <typename T>
 __device__ __forceinline__ T* target(const Args& a, int n, int head, int place, int req) {
     if (head < a.nq) return (T*)a.q_out + ((size_t)n * a.nq + head) * a.d;
-    const int at = place / a.page_size;
-    if (place < 0 || at >= a.bt_stride || req < 0 || req >= a.requests) return nullptr;
-    const int page = a.block_table[(size_t)req * a.bt_stride + at];
-    if (page < 0 || page >= a.pages) return nullptr;
-    return (T*)a.kv + (((size_t)page * 2 * a.nkv + (head - a.nq)) * a.page_size + place % a.page_size) * a.d;
+    // (the quotient, a page that is not a power of two, is some thirty instructions in the chain)
+    const int at = a.page_shift >= 0 ? place >> a.page_shift : place / a.page_size;
+    const bool in = place >= 0 && at < a.bt_stride && (unsigned)req < (unsigned)a.requests;
+    const int page = in ? a.block_table[(size_t)req * a.bt_stride + at] : -1;
+    if ((unsigned)page >= (unsigned)a.pages) return nullptr;
+    return (T*)a.kv + (((size_t)page * 2 * a.nkv + (head - a.nq)) * a.page_size + (place - at * a.page_size)) * a.d;
 }
 
 // A warp a head, a feature pair a lane and step: any even rotary width, any head size, any alignment.
@@ -96,8 +98,8 @@ __global__ void __launch_bounds__(128) axes_rope_write_kernel(const Args a) {
 // warp), each with two pieces: of the rotated features N neighbouring ones and their partners rd / 2 further, of the rest two neighbouring pieces.  So the
 // rotation needs no exchange and the norm log2(G) shuffles.  The positions of up to four axes are read
 // beside the axes of a thread's pairs, not behind them.  What bounds it is the chain of reads (axis and positions, tables, result), for few tokens
-// and for many, which small blocks of short-lived threads hide best: 2,048 tokens of 32 + 2 x 8 heads of 128 in bfloat16, with gains, take 13.8 us (51 MB: 3.7 TB/s; a
-// plain copy of as many bytes 9.3; with the places read behind the tables 15.1), eight tokens out of four planes of partial sums 3.0.  (For many tokens the
+// and for many, which small blocks of short-lived threads hide best: 2,048 tokens of 32 + 2 x 8 heads of 128 in bfloat16, with gains, take 13.7 us (51 MB: 3.7 TB/s; a
+// plain copy of as many bytes 9.3; with the places read behind the tables 15.1), eight tokens out of four planes of partial sums 3.2.  (For many tokens the
 // chain does not explain it all: 8,192 take 4.1 times as long as 2,048, and each warp looks up what its token's other warps have looked up.)
 constexpr int WIDE_THREADS = 128, AHEAD = 4;
 
@@ -328,17 +330,20 @@ LILY_API int lily_axes_rope_write(const void* qkv, int in_dtype, int splits, siz
     LILY_REQUIRE(in_dtype == act_dtype || in_dtype == kF32, "axes_rope_write: products are of the cache's dtype or float32");
     LILY_REQUIRE(act_dtype == kBF16 || gain_dtype == kF32 || q_gain == nullptr, "axes_rope_write: float32 heads keep float32 gains");
     LILY_REQUIRE(splits >= 1 && (splits == 1 || in_dtype == kF32), "axes_rope_write: partial sums are float32");
+    int page_shift = -1;
+    if ((page_size & (page_size - 1)) == 0)
+        for (page_shift = 0; 1 << page_shift < page_size;) ++page_shift;
     const axes::Args a{qkv, stride, splits, ld, q_gain, k_gain, eps, cos_t, sin_t, table_rows, positions, pair_axis, axes, tokens, places, token_req,
-                       block_table, requests, bt_stride, kv, pages, q_out, nq, nkv, d, rd, page_size};
+                       block_table, requests, bt_stride, kv, pages, q_out, nq, nkv, d, rd, page_size, page_shift};
     const int bytes = act_dtype == kBF16 ? 2 : 4, piece = 16 / bytes, group = d / (2 * piece);
     int shift = 0;
     while (1 << shift < group) ++shift;
     const uintptr_t where = (uintptr_t)qkv | (uintptr_t)kv | (uintptr_t)q_out | (uintptr_t)q_gain | (uintptr_t)k_gain |
                             (uintptr_t)cos_t | (uintptr_t)sin_t | (uintptr_t)pair_axis;
     // Whole pieces of 16 bytes on every side; else, and for heads that are no power of two of pieces, a warp a head.  Measured, us, in pieces / a warp a
-    // head, on the same operands, other ones each call: 2,048 tokens of 48 heads of 128 in bfloat16 with gains 14.0 / 39.6 (axes in turn 16.2 / 39.1), without 11.6 / 39.7 (13.9 / 38.9),
-    // 8,192 tokens with gains 55.9 / 157, eight tokens 2.5 / 3.4, from four planes 3.3 / 5.4; float32 without gains, 1,000 tokens of 24 heads of 128 with half of each turned
-    // 8.1 / 10.2, of 64 5.1 / 7.9.
+    // head, on the same operands, other ones each call: 2,048 tokens of 48 heads of 128 in bfloat16 with gains 13.7 / 38.7 (axes in turn 15.9 / 38.1), without 11.4 / 38.7 (13.6 / 37.9),
+    // 8,192 tokens with gains 54.8 / 153, eight tokens 2.4 / 3.4, from four planes 3.2 / 5.4; float32 without gains, 1,000 tokens of 24 heads of 128 with half of each turned
+    // 8.1 / 10.0, of 64 5.1 / 7.2.
     const bool wide = d % (2 * piece) == 0 && 1 << shift == group && group <= 32 && rd % (2 * piece) == 0 && ld % piece == 0 &&
                       (in_dtype == act_dtype || ld % 4 == 0) && (size_t)stride % 4 == 0 && where % 16 == 0;
     const dim3 grid = wide ? dim3(tokens, (unsigned)((((nq + 2 * nkv) << shift) + axes::WIDE_THREADS - 1) / axes::WIDE_THREADS)) : dim3(tokens, (nq + 2 * nkv + 3) / 4);
