@@ -18,8 +18,8 @@
 // several blocks share leaves a part in scratch for each, joined in their order (rows: by the join kernel; columns: by the warps that
 // come last), so the results do not depend on who is first.
 //
-// Measured: 2,048 tokens of 32 heads of 128 over 8, 61.4 us (some 7 of them between the kernels; all exponentials on their unit would take 34, the products
-// 10); the last 64 of 1,024 tokens behind 15,360 places 36.7.  The CUDA cores of key_weights.cu take 768 for the first, and on the same pages 12.6 for 16 tokens (here 9.5),
+// Measured: 2,048 tokens of 32 heads of 128 over 8, 60.4 us (some 7 of them between the kernels; all exponentials on their unit would take 34, the products
+// 10); the last 64 of 1,024 tokens behind 15,360 places 36.6.  The CUDA cores of key_weights.cu take 768 for the first, and on the same pages 12.6 for 16 tokens (here 9.5),
 // 17.8 for 128 (13.0); they are ahead for 300 tokens of seven heads of 64 over one (14.6, here 17.4), where a dozen tiles leave most SMs idle either way.
 //
 // Every wait is bounded: one that runs out says so in a word of the host's memory (lily_key_weights_status), the roles leave their loops, what the block
