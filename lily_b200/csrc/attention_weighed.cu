@@ -425,8 +425,8 @@ __global__ void __launch_bounds__(THREADS, 3) decode_weighed_mma_kernel(const De
             o[j][2] *= al_hi;
             o[j][3] *= al_hi;
         }
-        // the weights are rounded to bfloat16 for the product with the values, as in the other attention kernels of this precision (in two halves 1 to 4 % slower, and what the
-        // outputs are from 64 bits, 1.5e-3 of them, is their own rounding either way)
+        // the weights are rounded to bfloat16 for the product with the values, as in the other attention kernels of this precision (in two halves 1 to 4 % slower; what the
+        // outputs are from 64 bits, 1.5e-3 of them at some hundred places and 2.0e-3 at four, is mostly their own rounding, 1.7e-3 where the weights keep 32 bits)
         const uint32_t a0 = tc5::pack2(s[0][0], s[0][1]), a1 = tc5::pack2(s[0][2], s[0][3]), a2 = tc5::pack2(s[1][0], s[1][1]), a3 = tc5::pack2(s[1][2], s[1][3]);
 #pragma unroll
         for (int jp = 0; jp < D / 16; ++jp) {
