@@ -1,0 +1,261 @@
+// A paged cache held in four bits (four.cuh says how it lies): what writes it and what reads it as numbers again.
+//
+// Writing: a head x of a token, y = x r g with r = (mean x^2 + eps)^(-1/2) where there are gains, the first rd features turned by halves
+//   (y_j, y_(j + rd/2)) <- (y_j c - y_(j + rd/2) s, y_(j + rd/2) c + y_j s),   c, s = tables[position][j],
+// queries to their row of `q_out`; of keys and values each group of 64 features becomes
+//   step = bf16((max - min) / 15), lowest = bf16(min), code = min(15, max(0, rint((y - lowest) / step)))
+// at the place `position` of the token's request.  A group that holds what is not finite, or whose spread is not, has NaN for both and reads as NaN.
+//
+// A number next to the border of two codes is a whole step off where its last bit falls the other way, so a token's codes are made a function of its numbers
+// alone: the sum of squares is taken in 64 bits (squares of float32 numbers are exact there, and no order of adding them up shows in the root's 24 bits), and every other
+// operation is one IEEE operation, none contracted.  The same token gets the same codes in a prompt, alone, and from a statement in plain operations.
+#include "four.cuh"
+
+namespace lily {
+namespace four {
+
+struct WriteArgs {
+    const void* qkv;                 // [tokens, (nq + 2 nkv) d]
+    int ld;
+    const void* q_gain;
+    const void* k_gain;
+    double eps;
+    const float* cos_t;              // [table_rows, rd / 2]
+    const float* sin_t;
+    int table_rows;
+    const int* positions;            // [tokens]
+    const int* token_req;
+    const int* block_table;          // [requests, bt_stride]
+    int requests, bt_stride;
+    uint8_t* kv;
+    int pages;
+    void* q_out;                     // [tokens, nq * d]
+    int nq, nkv, d, rd, page_size, tokens;
+};
+
+template <typename T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]);
+template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(p);
+    v[0] = low(raw.x), v[1] = high(raw.x), v[2] = low(raw.y), v[3] = high(raw.y);
+    v[4] = low(raw.z), v[5] = high(raw.z), v[6] = low(raw.w), v[7] = high(raw.w);
+}
+template <> __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(bits(__floats2bfloat162_rn(v[0], v[1])), bits(__floats2bfloat162_rn(v[2], v[3])), bits(__floats2bfloat162_rn(v[4], v[5])),
+                                              bits(__floats2bfloat162_rn(v[6], v[7])));
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+constexpr int WRITE_WARPS = 4;
+
+// A thread eight features, d / 8 threads a head, 32 / (d / 8) heads a warp.  grid (blocks of a token's heads, tokens)
+template <typename T, typename W, bool WHOLE_PIECES>
+__global__ void __launch_bounds__(32 * WRITE_WARPS) write_kernel(const WriteArgs a) {
+    __shared__ __align__(16) float turn_s[WRITE_WARPS][256];
+    pdl_enter_small();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, words = a.d / 8, per_warp = 32 / words;
+    const int mine = min(lane / words, per_warp - 1), l = lane - mine * words;                 // (d = 192: lanes 24 to 31 have no word)
+    const int n = blockIdx.y, asked = (blockIdx.x * WRITE_WARPS + warp) * per_warp + mine, most = a.nq + 2 * a.nkv;
+    const bool in = asked < most && l < words;
+    const int head = min(asked, most - 1), f = min(l, words - 1) * 8;
+    const int kind = head < a.nq ? 0 : head < a.nq + a.nkv ? 1 : 2;
+    float y[8];
+    load8((const T*)a.qkv + (size_t)n * a.ld + (size_t)head * a.d + f, y);
+    const W* gain = kind == 2 ? nullptr : (const W*)(kind ? a.k_gain : a.q_gain);
+    const int pos = a.positions[n], req = kind ? a.token_req[n] : 0;
+    double squares = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) squares = fma((double)y[i], (double)y[i], squares);
+    if (l >= words) squares = 0.0;
+    if (words == 24)                                     // (a head over 24 of 32 lanes; the others bring nothing)
+        for (int o = 16; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+    else
+        for (int o = words >> 1; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+    if (gain) {
+        const float r = (float)(1.0 / sqrt(squares / (double)a.d + a.eps));
+        float g[8];
+        load8(gain + f, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(__fmul_rn(y[i], r), g[i]);
+    }
+    float* row = turn_s[warp] + mine * a.d;
+    if (l < words) store8(row + f, y);
+    __syncwarp();
+    const int half = a.rd / 2;
+    if (kind != 2 && f < a.rd) {
+        const bool known = pos >= 0 && pos < a.table_rows;
+        const float nan = __int_as_float(0x7fffffff);
+        const float *ct = a.cos_t + (size_t)(known ? pos : 0) * half, *st = a.sin_t + (size_t)(known ? pos : 0) * half;
+        if (WHOLE_PIECES) {                              // half a multiple of eight: a thread's features are of one half
+            const int j = f < half ? f : f - half;
+            float c[8], s[8], other[8];
+            load8(ct + j, c);
+            load8(st + j, s);
+            load8(row + (f < half ? f + half : j), other);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float first = __fmul_rn(y[i], c[i]), second = __fmul_rn(other[i], s[i]);
+                y[i] = !known ? nan : f < half ? __fsub_rn(first, second) : __fadd_rn(first, second);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int e = f + i, j = e < half ? e : e - half;
+                if (e >= a.rd) continue;
+                const float first = __fmul_rn(y[i], ct[j]), second = __fmul_rn(row[e < half ? e + half : j], st[j]);
+                y[i] = !known ? nan : e < half ? __fsub_rn(first, second) : __fadd_rn(first, second);
+            }
+        }
+    }
+    if (kind == 0 && in) store8((T*)a.q_out + ((size_t)n * a.nq + head) * a.d + f, y);
+    // eight neighbouring lanes hold a group of 64 features
+    float most_v = y[0], least = y[0];
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        most_v = fmaxf(most_v, y[i]);
+        least = fminf(least, y[i]);
+        fine = fine && isfinite(y[i]);
+    }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+        most_v = fmaxf(most_v, __shfl_xor_sync(0xffffffffu, most_v, o));
+        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+    }
+    fine = (__ballot_sync(0xffffffffu, fine) >> (lane & 24) & 0xffu) == 0xffu;
+    const __nv_bfloat16 step_b = __float2bfloat16_rn(__fmul_rn(__fsub_rn(most_v, least), (float)(1.0 / 15.0))), low_b = __float2bfloat16_rn(least);
+    const float step = __bfloat162float(step_b), lowest = __bfloat162float(low_b);
+    fine = fine && isfinite(step) && isfinite(lowest);
+    if (kind == 0 || !in) return;
+    const int at = pos >= 0 ? pos / a.page_size : -1;
+    if (at < 0 || at >= a.bt_stride || (unsigned)req >= (unsigned)a.requests) return;
+    const int page = a.block_table[(size_t)req * a.bt_stride + at];
+    if ((unsigned)page >= (unsigned)a.pages) return;
+    uint32_t word = 0;
+    if (fine && step > 0.f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(y[i], lowest), step)), 0.f), 15.f);
+            word |= (uint32_t)c << (4 * i);
+        }
+    }
+    const int groups = a.d / GROUP, slot = pos - at * a.page_size;
+    uint8_t* rows = a.kv + (((size_t)page * a.nkv + (head - a.nq - (kind == 2 ? a.nkv : 0))) * 2 + (kind == 2)) * ((size_t)a.page_size * row_bytes(a.d));
+    reinterpret_cast<uint32_t*>(rows + (size_t)slot * (a.d / 2))[kind == 1 ? key_word(l, groups) : value_word(l, groups)] = word;
+    if ((l & 7) == 0) {
+        const __nv_bfloat16 nan = __float2bfloat16_rn(__int_as_float(0x7fffffff));
+        reinterpret_cast<uint32_t*>(rows + (size_t)a.page_size * (a.d / 2))[slot * groups + (l >> 3)] =
+            bits(fine ? __halves2bfloat162(step_b, low_b) : __halves2bfloat162(nan, nan));
+    }
+}
+
+// Pages as numbers, lowest + step code in one rounding: of every page that a block table names to [requests, width, 2, nkv, page_size, d] (``compact`` false), or of the pages
+// that portions of prompts see, one request's behind the other's, [pages, 2, nkv, page_size, d], with a block table of them and zeros behind a request's last place.
+// A thread a word of eight codes, bound by the numbers it writes.  grid (pages, requests, kv heads x 2)
+template <typename T>
+__global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__ kv, int pages, const int* __restrict__ block_table, int width, T* __restrict__ out, int nkv,
+                                                     int d, int page_size, const int* __restrict__ cu, const int* __restrict__ prefix, int* __restrict__ table_out,
+                                                     int table_width, int most_pages) {
+    __shared__ int sum_s[8];
+    pdl_enter_small();
+    const int r = blockIdx.y, at = blockIdx.x, head = blockIdx.z >> 1, value = blockIdx.z & 1, words = d / 8, groups = d / GROUP;
+    size_t to = (size_t)r * width + at;
+    int places = page_size;
+    if (cu) {
+        // pages of the requests ahead of this one
+        auto places_of = [&](int i) { return cu[i + 1] > cu[i] ? prefix[i] + cu[i + 1] - cu[i] : 0; };
+        const int total = places_of(r);
+        if (at >= (total + page_size - 1) / page_size) return;
+        places = min(page_size, total - at * page_size);
+        int before = 0;
+        for (int i = threadIdx.x; i < r; i += 256) before += (places_of(i) + page_size - 1) / page_size;
+        for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+        if ((threadIdx.x & 31) == 0) sum_s[threadIdx.x >> 5] = before;
+        __syncthreads();
+        before = 0;
+        for (int w = 0; w < 8; ++w) before += sum_s[w];
+        to = (size_t)before + at;
+        if (to >= (size_t)most_pages || at >= table_width) return;
+        if (threadIdx.x == 0 && blockIdx.z == 0) table_out[(size_t)r * table_width + at] = (int)to;
+    }
+    int page = at < width ? block_table[(size_t)r * width + at] : 0;
+    if ((unsigned)page >= (unsigned)pages) page = 0;
+    const uint8_t* rows = kv + (((size_t)page * nkv + head) * 2 + value) * ((size_t)page_size * row_bytes(d));
+    const uint32_t* held = reinterpret_cast<const uint32_t*>(rows + (size_t)page_size * (d / 2));
+    T* dst = out + ((to * 2 + value) * nkv + head) * ((size_t)page_size * d);
+    for (int i = threadIdx.x; i < page_size * words; i += 256) {
+        const int slot = i / words, l = i - slot * words;
+        const uint32_t w = reinterpret_cast<const uint32_t*>(rows + (size_t)slot * (d / 2))[value ? value_word(l, groups) : key_word(l, groups)];
+        const uint32_t h = held[slot * groups + (l >> 3)];
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = slot < places ? fmaf((float)(w >> (4 * e) & 15u), low(h), high(h)) : 0.f;
+        store8(dst + (size_t)slot * d + l * 8, v);
+    }
+}
+
+inline bool head_fits(int d) { return d >= GROUP && d <= 256 && d % GROUP == 0; }
+
+}  // namespace four
+}  // namespace lily
+
+using namespace lily;
+
+LILY_API int lily_qk_norm_rope_write4(const void* qkv, int dtype, int ld, const void* q_gain, const void* k_gain, int gain_dtype, double eps, const float* cos_t, const float* sin_t,
+                                      int table_rows, const int* positions, int tokens, const int* token_req, const int* block_table, int requests, int bt_stride, void* kv, int pages,
+                                      void* q_out, int nq, int nkv, int d, int rd, int page_size, cudaStream_t stream) {
+    if (tokens == 0) return 0;
+    LILY_REQUIRE(four::head_fits(d), "qk_norm_rope_write4: heads of 64, 128, 192 or 256 features, not %d", d);
+    LILY_REQUIRE(rd >= 0 && rd <= d && rd % 2 == 0 && (rd == 0 || (cos_t && sin_t)), "qk_norm_rope_write4: rotary_dim %d does not fit head_dim %d", rd, d);
+    LILY_REQUIRE(page_size > 0 && tokens > 0 && tokens <= 65535 * 32, "qk_norm_rope_write4: %d tokens, pages of %d places", tokens, page_size);
+    LILY_REQUIRE(nq >= 0 && nkv >= 0 && nq + nkv > 0 && ld >= (nq + 2 * nkv) * d, "qk_norm_rope_write4: rows of %d numbers", ld);
+    LILY_REQUIRE((q_gain == nullptr) == (k_gain == nullptr), "qk_norm_rope_write4: q and k gains come together");
+    LILY_REQUIRE(dtype == kF32 || (dtype == kBF16), "qk_norm_rope_write4: dtype %d", dtype);
+    LILY_REQUIRE(dtype == kBF16 || gain_dtype == kF32 || !q_gain, "qk_norm_rope_write4: float32 heads keep float32 gains");
+    const uintptr_t where = (uintptr_t)qkv | (uintptr_t)kv | (uintptr_t)q_out | (uintptr_t)q_gain | (uintptr_t)k_gain | (uintptr_t)cos_t | (uintptr_t)sin_t;
+    LILY_REQUIRE(where % 16 == 0 && ld % 8 == 0, "qk_norm_rope_write4: tensors on boundaries of sixteen bytes");
+    const int per_block = four::WRITE_WARPS * (32 / (d / 8));
+    const bool pieces = rd % 16 == 0;
+    for (int t0 = 0; t0 < tokens; t0 += 65535) {
+        const int n = min(65535, tokens - t0), item = dtype == kBF16 ? 2 : 4;
+        const four::WriteArgs a{(const char*)qkv + (size_t)t0 * ld * item, ld, q_gain, k_gain, eps, cos_t, sin_t, table_rows, positions + t0, token_req + t0, block_table, requests, bt_stride,
+                                (uint8_t*)kv, pages, (char*)q_out + (size_t)t0 * nq * d * item, nq, nkv, d, rd, page_size, n};
+        const dim3 grid((nq + 2 * nkv + per_block - 1) / per_block, n);
+#define LAUNCH(T, W)                                                                                                              \
+    do {                                                                                                                          \
+        if (pieces) launch_pdl(four::write_kernel<T, W, true>, grid, dim3(32 * four::WRITE_WARPS), 0, stream, a);                  \
+        else launch_pdl(four::write_kernel<T, W, false>, grid, dim3(32 * four::WRITE_WARPS), 0, stream, a);                        \
+    } while (0)
+        if (dtype == kF32) LAUNCH(float, float);
+        else if (gain_dtype == kBF16) LAUNCH(__nv_bfloat16, __nv_bfloat16);
+        else LAUNCH(__nv_bfloat16, float);
+#undef LAUNCH
+        LILY_CHECK_LAUNCH("qk_norm_rope_write4");
+    }
+    return 0;
+}
+
+// cu, prefix, table_out: null, or of a step's portions (offsets of their tokens, tokens cached ahead of them, a block table [requests, table_width] of the pages
+// written, of which there is room for `most_pages`).
+LILY_API int lily_cache4_values(const void* kv, int pages, const int* block_table, int requests, int width, void* out, int dtype, int nkv, int d, int page_size, const int* cu,
+                                const int* prefix, int* table_out, int table_width, int most_pages, cudaStream_t stream) {
+    if (requests == 0 || width == 0) return 0;
+    LILY_REQUIRE(four::head_fits(d), "cache4_values: heads of 64, 128, 192 or 256 features, not %d", d);
+    LILY_REQUIRE(page_size > 0 && nkv > 0 && nkv <= 32767 && requests > 0 && requests <= 65535 && width > 0, "cache4_values: %d requests, %d kv heads, pages of %d places", requests, nkv, page_size);
+    LILY_REQUIRE(((uintptr_t)kv | (uintptr_t)out) % 16 == 0, "cache4_values: tensors on boundaries of sixteen bytes");
+    const dim3 grid(cu ? table_width : width, requests, 2 * nkv);
+    if (grid.x == 0) return 0;
+    if (dtype == kF32)
+        launch_pdl(four::values_kernel<float>, grid, dim3(256), 0, stream, (const uint8_t*)kv, pages, block_table, width, (float*)out, nkv, d, page_size, cu, prefix, table_out, table_width, most_pages);
+    else
+        launch_pdl(four::values_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, (const uint8_t*)kv, pages, block_table, width, (__nv_bfloat16*)out, nkv, d, page_size, cu, prefix, table_out,
+                   table_width, most_pages);
+    LILY_CHECK_LAUNCH("cache4_values");
+    return 0;
+}

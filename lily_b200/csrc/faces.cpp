@@ -11,6 +11,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -45,6 +46,14 @@ struct Entries {
     int (*key_weights_tc)(const void*, int, const void*, int, float*, const int*, int, float*, int, const int*, const int*, int, int, int, int, int, float, int, int, void*);
     size_t (*key_weights_tc_floats)(int, const int*, const int*, int, int, int);
     int (*key_weights_tc_takes)(int, int, int, int, float);
+    // numbers held in four bits
+    int (*linear4)(const void*, int, const void*, const void*, const void*, const void*, int, void*, int, int, int, int, int, void*);
+    int (*weights4)(const void*, const void*, const void*, void*, int, int, int, int, void*);
+    int (*write4)(const void*, int, int, const void*, const void*, int, double, const float*, const float*, int, const int*, int, const int*, const int*, int, int, void*, int, void*, int, int,
+                  int, int, int, void*);
+    int (*values4)(const void*, int, const int*, int, int, void*, int, int, int, int, const int*, const int*, int*, int, int, void*);
+    size_t (*decode4_floats)(int, int, int, int, int, int, int);
+    int (*decode4)(const void*, const void*, void*, const int*, int, const int*, float*, int, int, int, int, int, int, int, float, int, void*);
 } entry;
 
 // ---- words ----
@@ -375,9 +384,168 @@ PyObject* bind(PyObject*, PyObject* const* p, Py_ssize_t count) {
     });
 }
 
+// ---- numbers held in four bits ----
+
+// All of a call's tensors lie on the current device, where its kernels run.
+void here(std::initializer_list<const Tensor*> all) {
+    const int device = c10::cuda::current_device();
+    for (const Tensor* t : all)
+        if (t && t->get_device() != device) refuse("kernels run on the current device, ", device, "; got a tensor on ", t->device().str());
+}
+// A layer of a cache held in four bits: uint8 [pages, kv_heads, 2, page_size (d / 2 + d / 16)].
+void layer4_fits(const char* what, const Tensor& kv, int64_t nkv, int64_t page, int64_t d) {
+    if (d < 64 || d > 256 || d % 64) refuse(what, ": heads of 64, 128, 192 or 256 features, not ", d);
+    if (!is(kv, at::kByte) || kv.dim() != 4 || !shaped(kv, {kv.size(0), nkv, 2, page * (d / 2 + d / 16)}) || kv.size(0) < 1)
+        refuse(what, ": a cache layer is uint8 [pages, ", nkv, ", 2, ", page * (d / 2 + d / 16), "], got ", words(kv));
+}
+struct Matrix4 { const Tensor &codes, &scales; const Tensor* zeros; int n, k, group; };
+// codes, scales, zeros, n, k, group from p[0] on
+Matrix4 matrix4(const char* what, PyObject* const* p) {
+    const Matrix4 w{tensor(p[0]), tensor(p[1]), maybe(p[2]), number(p[3]), number(p[4]), number(p[5])};
+    if (w.n < 1 || w.k < 1 || w.n > INT32_MAX - 256 || w.k > INT32_MAX - 256 || (w.group != 32 && w.group != 64 && w.group != 128) || w.k % w.group)
+        refuse(what, ": a matrix [", w.n, ", ", w.k, "] does not come in groups of ", w.group, " columns (32, 64 or 128)");
+    const int64_t rows = (w.n + 127) / 128, tiles = (w.k + 127) / 128, groups = tiles * 128 / w.group;
+    if (!is(w.codes, at::kByte) || !shaped(w.codes, {rows, tiles, 128, 64})) refuse(what, ": codes are uint8 [", rows, ", ", tiles, ", 128, 64], got ", words(w.codes));
+    if (!is(w.scales, at::kBFloat16) || !shaped(w.scales, {rows, groups, 128})) refuse(what, ": scales are bfloat16 [", rows, ", ", groups, ", 128], got ", words(w.scales));
+    if (w.zeros && (!is(*w.zeros, at::kByte) || w.zeros->sizes() != w.scales.sizes())) refuse(what, ": zero points are uint8 ", words(w.scales.sizes()), ", got ", words(*w.zeros));
+    return w;
+}
+
+// x, codes, scales, zeros, n, k, group, bias, whether the result is float32 whatever x is
+PyObject* linear4(PyObject*, PyObject* const* p, Py_ssize_t count) {
+    return guarded(count, 9, [&]() -> PyObject* {
+        const Tensor& x = tensor(p[0]);
+        const Matrix4 w = matrix4("linear4", p + 1);
+        const Tensor* bias = maybe(p[7]);
+        const int code = code_of(x), wide = code == F32 || PyObject_IsTrue(p[8]);
+        if (x.dim() != 2 || x.size(1) != w.k) refuse("linear4: x ", words(x), " against a matrix [", w.n, ", ", w.k, "]");
+        if (bias && (bias->dim() != 1 || bias->numel() != w.n || (code_of(*bias) == BF16 && code == F32))) refuse("linear4: a bias of ", w.n, " numbers, got ", words(*bias));
+        here({&x, &w.codes, &w.scales, w.zeros, bias});
+        Tensor out = at::empty({x.size(0), (int64_t)w.n}, x.options().dtype(wide ? at::kFloat : at::kBFloat16));
+        done("lily_linear4", call(entry.linear4, x.const_data_ptr(), code, w.codes.const_data_ptr(), w.scales.const_data_ptr(), w.zeros ? w.zeros->const_data_ptr() : nullptr,
+                                  bias ? bias->const_data_ptr() : nullptr, bias ? (int)(code_of(*bias) == F32) : 0, out.data_ptr(), wide, narrow(x.size(0)), w.n, w.k, w.group, stream()));
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// codes, scales, zeros, n, k, group, whether float32
+PyObject* weights4(PyObject*, PyObject* const* p, Py_ssize_t count) {
+    return guarded(count, 7, [&]() -> PyObject* {
+        const Matrix4 w = matrix4("weights4", p);
+        const bool wide = PyObject_IsTrue(p[6]);
+        here({&w.codes, &w.scales, w.zeros});
+        Tensor out = at::empty({(int64_t)w.n, (int64_t)w.k}, w.scales.options().dtype(wide ? at::kFloat : at::kBFloat16));
+        done("lily_weights4", call(entry.weights4, w.codes.const_data_ptr(), w.scales.const_data_ptr(), w.zeros ? w.zeros->const_data_ptr() : nullptr, out.data_ptr(), wide ? F32 : BF16, w.n, w.k,
+                                   w.group, stream()));
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// qkv, q_gain, k_gain, eps, cos, sin, positions, token_req, block_table, kv_layer, nq, nkv, d, rotary_dim, page_size, q_out
+PyObject* qk_norm_rope_write4(PyObject*, PyObject* const* p, Py_ssize_t count) {
+    return guarded(count, 16, [&]() -> PyObject* {
+        const char* what = "qk_norm_rope_write4";
+        const Tensor &qkv = tensor(p[0]), &positions = tensor(p[6]), &req = tensor(p[7]), &table = tensor(p[8]), &kv = tensor(p[9]);
+        const Tensor *q_gain = maybe(p[1]), *k_gain = maybe(p[2]), *cos = maybe(p[4]), *sin = maybe(p[5]), *given = maybe(p[15]);
+        const double eps = PyFloat_AsDouble(p[3]);
+        if (eps == -1.0 && PyErr_Occurred()) throw Raised{};
+        const int nq = number(p[10]), nkv = number(p[11]), d = number(p[12]), rd = number(p[13]), page = number(p[14]);
+        if (nq < 1 || nkv < 1 || page < 1) refuse(what, ": ", nq, " query and ", nkv, " kv heads, pages of ", page, " places");
+        layer4_fits(what, kv, nkv, page, d);
+        const int64_t ld = ((int64_t)nq + 2 * (int64_t)nkv) * d;
+        if (qkv.dim() != 2 || qkv.size(1) != ld) refuse(what, ": qkv is [tokens, ", ld, "], got ", words(qkv));
+        const int64_t n = qkv.size(0);
+        const int code = code_of(qkv);
+        if (rd < 0 || rd > d || rd % 2 || (rd && (!cos || !sin))) refuse(what, ": rotary_dim ", rd, " does not fit head_dim ", d, ", or has no tables");
+        if (rd && (!is(*cos, at::kFloat) || !is(*sin, at::kFloat) || cos->dim() != 2 || cos->size(1) != rd / 2 || sin->sizes() != cos->sizes()))
+            refuse(what, ": rotation tables are float32 [positions, rotary_dim / 2]");
+        if (positions.numel() != n || req.numel() != n || table.dim() != 2 || table.size(1) < 1) refuse(what, ": ", n, " tokens have a position and a request each, and there is a block table");
+        int gain = F32;
+        if (q_gain || k_gain) {
+            if (!q_gain || !k_gain || q_gain->scalar_type() != k_gain->scalar_type() || q_gain->numel() != d || k_gain->numel() != d)
+                refuse(what, ": q and k gains come together, with one dtype and head_dim numbers each");
+            gain = code_of(*q_gain);
+        }
+        if (given && (given->scalar_type() != qkv.scalar_type() || given->numel() != n * nq * d)) refuse(what, ": q_out is [tokens, nq * d] in the dtype of qkv");
+        const int *at = ints(positions, "positions"), *of = ints(req, "token_req"), *bt = ints(table, "block_table");
+        here({&qkv, q_gain, k_gain, cos, sin, &positions, &req, &table, &kv, given});
+        Tensor q = given ? *given : at::empty({n, (int64_t)nq * d}, qkv.options());
+        done("lily_qk_norm_rope_write4",
+             call(entry.write4, qkv.const_data_ptr(), code, narrow(ld), q_gain ? q_gain->const_data_ptr() : nullptr, k_gain ? k_gain->const_data_ptr() : nullptr, gain, eps,
+                  rd ? cos->const_data_ptr<float>() : nullptr, rd ? sin->const_data_ptr<float>() : nullptr, rd ? narrow(cos->size(0)) : 0, at, narrow(n), of, bt, narrow(table.size(0)),
+                  narrow(table.size(1)), kv.data_ptr(), narrow(kv.size(0)), q.data_ptr(), nq, nkv, d, rd, page, stream()));
+        return THPVariable_Wrap(std::move(q));
+    });
+}
+
+// kv_layer, block_table, nkv, d, page_size, whether float32
+PyObject* cache4_values(PyObject*, PyObject* const* p, Py_ssize_t count) {
+    return guarded(count, 6, [&]() -> PyObject* {
+        const Tensor &kv = tensor(p[0]), &table = tensor(p[1]);
+        const int nkv = number(p[2]), d = number(p[3]), page = number(p[4]);
+        const bool wide = PyObject_IsTrue(p[5]);
+        if (nkv < 1 || page < 1) refuse("cache4_values: ", nkv, " kv heads, pages of ", page, " places");
+        layer4_fits("cache4_values", kv, nkv, page, d);
+        if (table.dim() != 2 || !is(table, at::kInt)) refuse("cache4_values: block_table is int32 [requests, pages], got ", words(table));
+        here({&kv, &table});
+        Tensor out = at::empty({table.size(0), table.size(1), 2, (int64_t)nkv, (int64_t)page, (int64_t)d}, kv.options().dtype(wide ? at::kFloat : at::kBFloat16));
+        done("lily_cache4_values", call(entry.values4, kv.const_data_ptr(), narrow(kv.size(0)), table.const_data_ptr<int>(), narrow(table.size(0)), narrow(table.size(1)), out.data_ptr(),
+                                        wide ? F32 : BF16, nkv, d, page, (const int*)nullptr, (const int*)nullptr, (int*)nullptr, 0, 0, stream()));
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// q, kv_layer, block_table, seq_lens, max_seq_len, nq, nkv, d, page_size, scale, out, scratch
+PyObject* attention_decode4(PyObject*, PyObject* const* p, Py_ssize_t count) {
+    return guarded(count, 12, [&]() -> PyObject* {
+        const char* what = "attention_decode4";
+        const Tensor &q = tensor(p[0]), &kv = tensor(p[1]), &table = tensor(p[2]), &lens = tensor(p[3]);
+        const Tensor *given = maybe(p[10]), *room = maybe(p[11]);
+        const int longest = number(p[4]), nq = number(p[5]), nkv = number(p[6]), d = number(p[7]), page = number(p[8]);
+        const float scale = real(p[9]);
+        if (nkv < 1 || nq < 1 || nq % nkv || page < 1) refuse(what, ": ", nq, " query heads over ", nkv, " kv heads, pages of ", page, " places");
+        layer4_fits(what, kv, nkv, page, d);
+        const int64_t requests = q.dim() ? q.size(0) : 0;
+        const int code = code_of(q);
+        if (q.dim() != 2 || q.size(1) != (int64_t)nq * d) refuse(what, ": queries are [requests, ", (int64_t)nq * d, "], got ", words(q));
+        const int width = table_width(what, table, requests);
+        if (lens.numel() != requests || !is(lens, at::kInt) || longest < 0 || longest > (int64_t)width * page)
+            refuse(what, ": ", requests, " int32 lengths of up to ", longest, " places; the block table holds ", (int64_t)width * page);
+        if (given && (given->scalar_type() != q.scalar_type() || given->numel() != q.numel())) refuse(what, ": out has the shape and dtype of q");
+        here({&q, &kv, &table, &lens, given, room});
+        if (entry.decode4_floats == nullptr) refuse("the kernels are not bound");
+        const int64_t need = (int64_t)entry.decode4_floats(narrow(requests), nq, nkv, d, longest, page, code);
+        if (room && (!is(*room, at::kFloat) || room->numel() < need)) refuse(what, ": scratch of ", need, " float32 needed");
+        Tensor out = given ? *given : at::empty_like(q), scratch;
+        float* floats = nullptr;
+        if (need) {
+            scratch = room ? *room : at::empty({need}, q.options().dtype(at::kFloat));
+            floats = scratch.data_ptr<float>();
+        }
+        done("lily_attention_decode4", call(entry.decode4, q.const_data_ptr(), kv.const_data_ptr(), out.data_ptr(), table.const_data_ptr<int>(), width, lens.const_data_ptr<int>(), floats,
+                                            (int)requests, longest, nq, nkv, d, page, narrow(kv.size(0)), scale, code, stream()));
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// the addresses of the entries for numbers held in four bits, in their order
+PyObject* bind4(PyObject*, PyObject* const* p, Py_ssize_t count) {
+    return guarded(count, 6, [&]() -> PyObject* {
+        void* at[6];
+        for (int i = 0; i < 6; ++i) at[i] = (void*)(uintptr_t)whole(p[i]);
+        entry.linear4 = (decltype(entry.linear4))at[0];
+        entry.weights4 = (decltype(entry.weights4))at[1];
+        entry.write4 = (decltype(entry.write4))at[2];
+        entry.values4 = (decltype(entry.values4))at[3];
+        entry.decode4_floats = (decltype(entry.decode4_floats))at[4];
+        entry.decode4 = (decltype(entry.decode4))at[5];
+        Py_RETURN_NONE;
+    });
+}
+
 #define FACE(name) {#name, (PyCFunction)(void (*)())name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FACE(axes_rope_write), FACE(attention_decode_weighed), FACE(select_keys), FACE(move_keys), FACE(key_weights_scratch_floats), FACE(attention_key_weights),
-                         FACE(bind), {nullptr, nullptr, 0, nullptr}};
+                         FACE(bind), FACE(linear4), FACE(weights4), FACE(qk_norm_rope_write4), FACE(cache4_values), FACE(attention_decode4), FACE(bind4), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "lily_faces", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,0 +1,270 @@
+// Products with weights held in four bits: y = x W^T, W_rc = s_rg (code_rc - z_rg), g the group of 32, 64 or 128 columns that c is in (four.cuh says how they lie).
+//
+// A few tokens are bound by the weights' bytes: a quarter of a bfloat16 matrix's, and a scale a group.  Codes become bfloat16 numbers 128 + code by one logical operation a pair and
+// code - z, exactly, by one subtraction; the tensor cores add up a group's products in float32, and its scale multiplies the sum, so no weight is ever rounded.
+#include "four.cuh"
+#include "mma.cuh"
+
+namespace lily {
+namespace four {
+
+struct ProductArgs {
+    const void* x;                // [m, k]
+    const uint8_t* codes;         // [n / 128, k / 128, 128, 64]
+    const __nv_bfloat16* scales;  // [n / 128, groups, 128], groups those of whole tiles of columns
+    const uint8_t* zeros;         // the same, or null: 8
+    const void* bias;             // [n] or null
+    int bias_f32;
+    void* out;                    // [m, n]
+    int out_f32;
+    int m, n, k, tiles;           // tiles of 128 columns
+};
+
+__device__ __forceinline__ uint4 weights16(const void* p) {          // weights are read once: not kept in the L1, which the tokens are to stay in
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t minus(uint32_t a, uint32_t b) { return bits(__hsub2(two(a), two(b))); }
+
+constexpr int FEW_WARPS = 8, FEW_ROWS = 32;
+
+// Up to 8 NT tokens: a block 32 rows, its warps an eighth of the columns' tiles each; weights on the rows of the products, tokens on their eight columns.  The first
+// weights are on their way before the kernel ahead has ended.  grid (rows / 32)
+template <int NT, int PER_GROUP>                                      // words of a lane (32 columns each) that share a scale: 1, 2 or 4
+__global__ void __launch_bounds__(32 * FEW_WARPS, 2) product_few_kernel(const ProductArgs a) {
+    constexpr int MT = FEW_ROWS / 16, GROUPS = 4 / PER_GROUP;
+    __shared__ float sum_s[FEW_WARPS][8 * NT][FEW_ROWS + 1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int row0 = blockIdx.x * FEW_ROWS, tile_row = row0 / 128, in_tile = row0 % 128;
+    const uint8_t* codes = a.codes + ((size_t)tile_row * a.tiles * 128 + in_tile) * 64 + lane * 16;        // (a lane's sixteen bytes: row g, piece t)
+    const size_t groups = (size_t)a.tiles * GROUPS, held0 = (size_t)tile_row * groups * 128 + in_tile + g;
+    struct Step { uint4 w[MT][2]; unsigned short s[MT][2][GROUPS]; unsigned char z[MT][2][GROUPS]; };
+    auto load = [&](int kt, Step& c) {
+        const uint8_t* p = codes + (size_t)kt * 128 * 64;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                c.w[mt][e] = weights16(p + (mt * 16 + e * 8) * 64);
+#pragma unroll
+                for (int i = 0; i < GROUPS; ++i) {
+                    const size_t at = held0 + ((size_t)kt * GROUPS + i) * 128 + mt * 16 + e * 8;
+                    const bool in = kt * 128 + i * (128 / GROUPS) < a.k;               // (what stands behind the last column may be no number)
+                    c.s[mt][e][i] = in ? __ldg(reinterpret_cast<const unsigned short*>(a.scales) + at) : 0;
+                    c.z[mt][e][i] = a.zeros ? __ldg(a.zeros + at) : 8;
+                }
+            }
+    };
+    Step cur, next;
+    if (warp < a.tiles) load(warp, cur);
+    pdl_launch_dependents();
+    pdl_wait();
+    float total[MT][NT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) total[mt][nt][e] = 0.f;
+    for (int kt = warp; kt < a.tiles; kt += FEW_WARPS) {
+        if (kt + FEW_WARPS < a.tiles) load(kt + FEW_WARPS, next);
+        uint4 xv[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int token = nt * 8 + g, col = kt * 128 + 32 * w + 8 * t;
+                xv[nt][w] = make_uint4(0, 0, 0, 0);
+                if (token < a.m && col < a.k) xv[nt][w] = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.x + (size_t)token * a.k + col);
+            }
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) {
+            float sum[MT][NT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[mt][nt][e] = 0.f;
+            uint32_t zero[MT][2];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) zero[mt][e] = (0x4300u | cur.z[mt][e][i]) * 0x10001u;
+#pragma unroll
+            for (int v = 0; v < PER_GROUP; ++v) {
+                const int w = i * PER_GROUP + v;
+                uint32_t b[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    b[nt][0] = __byte_perm(xv[nt][w].x, xv[nt][w].z, 0x5410);
+                    b[nt][1] = __byte_perm(xv[nt][w].x, xv[nt][w].z, 0x7632);
+                    b[nt][2] = __byte_perm(xv[nt][w].y, xv[nt][w].w, 0x5410);
+                    b[nt][3] = __byte_perm(xv[nt][w].y, xv[nt][w].w, 0x7632);
+                }
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const uint32_t p = (&cur.w[mt][0].x)[w], q = (&cur.w[mt][1].x)[w], zp = zero[mt][0], zq = zero[mt][1];
+                    const uint32_t a0[4] = {minus(pair(p, 0), zp), minus(pair(q, 0), zq), minus(pair(p, 1), zp), minus(pair(q, 1), zq)};
+                    const uint32_t a1[4] = {minus(pair(p, 2), zp), minus(pair(q, 2), zq), minus(pair(p, 3), zp), minus(pair(q, 3), zq)};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16::mma_bf16(sum[mt][nt], a0, b[nt][0], b[nt][1]);
+                        mma16::mma_bf16(sum[mt][nt], a1, b[nt][2], b[nt][3]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const float s0 = __uint_as_float((uint32_t)cur.s[mt][0][i] << 16), s1 = __uint_as_float((uint32_t)cur.s[mt][1][i] << 16);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    total[mt][nt][0] = fmaf(s0, sum[mt][nt][0], total[mt][nt][0]);
+                    total[mt][nt][1] = fmaf(s0, sum[mt][nt][1], total[mt][nt][1]);
+                    total[mt][nt][2] = fmaf(s1, sum[mt][nt][2], total[mt][nt][2]);
+                    total[mt][nt][3] = fmaf(s1, sum[mt][nt][3], total[mt][nt][3]);
+                }
+            }
+        }
+        cur = next;
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum_s[warp][nt * 8 + 2 * t + (e & 1)][mt * 16 + g + (e >> 1) * 8] = total[mt][nt][e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 8 * NT * FEW_ROWS; i += 32 * FEW_WARPS) {
+        const int token = i / FEW_ROWS, r = i % FEW_ROWS, row = row0 + r;
+        if (token >= a.m || row >= a.n) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < FEW_WARPS; ++w) v += sum_s[w][token][r];
+        if (a.bias) v += a.bias_f32 ? ((const float*)a.bias)[row] : __bfloat162float(((const __nv_bfloat16*)a.bias)[row]);
+        const size_t at = (size_t)token * a.n + row;
+        if (a.out_f32) ((float*)a.out)[at] = v;
+        else ((__nv_bfloat16*)a.out)[at] = __float2bfloat16_rn(v);
+    }
+}
+
+// Up to eight tokens in float32: a warp eight rows, a lane 32 columns of one of them at a time, all products and sums in float32.  grid (rows / 64)
+constexpr int F32_TOKENS = 8;
+template <int TOKENS>
+__global__ void __launch_bounds__(256) product_f32_kernel(const ProductArgs a, int group) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int row0 = blockIdx.x * 64 + warp * 8, row = row0 + g, tile_row = row0 / 128;
+    pdl_enter_small();
+    if (row0 >= a.n) return;
+    const uint8_t* codes = a.codes + ((size_t)tile_row * a.tiles * 128 + row0 % 128) * 64 + lane * 16;
+    const int per_tile = 128 / group;
+    const size_t held0 = (size_t)tile_row * a.tiles * per_tile * 128 + row0 % 128 + g;
+    float total[TOKENS];
+#pragma unroll
+    for (int i = 0; i < TOKENS; ++i) total[i] = 0.f;
+    for (int kt = 0; kt < a.tiles; ++kt) {
+        const uint4 v = weights16(codes + (size_t)kt * 128 * 64);
+        const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int col = kt * 128 + 32 * w + 8 * t;
+            if (col >= a.k) continue;
+            const size_t at = held0 + (size_t)((kt * 128 + 32 * w) / group) * 128;
+            const float s = __bfloat162float(a.scales[at]), z = a.zeros ? (float)a.zeros[at] : 8.f;
+            float c[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) c[e] = ((float)(words[w] >> (4 * e) & 15u) - z) * s;
+#pragma unroll
+            for (int i = 0; i < TOKENS; ++i) {
+                if (i >= a.m) break;
+                const float4 *p = reinterpret_cast<const float4*>((const float*)a.x + (size_t)i * a.k + col), x0 = p[0], x1 = p[1];
+                total[i] = fmaf(c[0], x0.x, fmaf(c[1], x0.y, fmaf(c[2], x0.z, fmaf(c[3], x0.w, total[i]))));
+                total[i] = fmaf(c[4], x1.x, fmaf(c[5], x1.y, fmaf(c[6], x1.z, fmaf(c[7], x1.w, total[i]))));
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TOKENS; ++i) {
+        total[i] += __shfl_xor_sync(0xffffffffu, total[i], 1);
+        total[i] += __shfl_xor_sync(0xffffffffu, total[i], 2);
+        if (i < a.m && t == 0 && row < a.n) ((float*)a.out)[(size_t)i * a.n + row] = total[i] + (a.bias ? ((const float*)a.bias)[row] : 0.f);
+    }
+}
+
+// The weights as numbers [n, k] (float32: exact; bfloat16: rounded once).  A thread a word of eight codes.
+template <typename T>
+__global__ void __launch_bounds__(256) weights_kernel(const ProductArgs a, int group) {
+    pdl_enter_small();
+    const int words = a.k / 8, row = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int per_tile = 128 / group;
+    if (row >= a.n) return;
+    for (int l = blockIdx.x * 32 + (threadIdx.x & 31); l < words; l += gridDim.x * 32) {
+        const int kt = l >> 4, in = l & 15;                           // word `in` of the tile: columns 8 in + (0..7)
+        const uint32_t w = reinterpret_cast<const uint32_t*>(a.codes + (((size_t)(row / 128) * a.tiles + kt) * 128 + row % 128) * 64)[(in & 3) * 4 + (in >> 2)];
+        const size_t at = ((size_t)(row / 128) * a.tiles * per_tile + (size_t)l * 8 / group) * 128 + row % 128;
+        const float s = __bfloat162float(a.scales[at]), z = a.zeros ? (float)a.zeros[at] : 8.f;
+        T* dst = (T*)a.out + (size_t)row * a.k + (size_t)l * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = ((float)(w >> (4 * e) & 15u) - z) * s;
+        if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint4*>(dst) = make_uint4(bits(__floats2bfloat162_rn(v[0], v[1])), bits(__floats2bfloat162_rn(v[2], v[3])), bits(__floats2bfloat162_rn(v[4], v[5])),
+                                                        bits(__floats2bfloat162_rn(v[6], v[7])));
+        else {
+            reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        }
+    }
+}
+
+}  // namespace four
+}  // namespace lily
+
+using namespace lily;
+
+static bool weights_fit(int n, int k, int group) { return n > 0 && k > 0 && (group == 32 || group == 64 || group == 128) && k % group == 0 && n <= INT32_MAX - 256 && k <= INT32_MAX - 256; }
+
+// Tokens that the kernels for few of them take.
+LILY_API int lily_linear4_few(int dtype) { return dtype == kBF16 ? 16 : four::F32_TOKENS; }
+
+LILY_API int lily_linear4(const void* x, int dtype, const void* codes, const void* scales, const void* zeros, const void* bias, int bias_f32, void* out, int out_f32, int m, int n, int k,
+                          int group, cudaStream_t stream) {
+    if (m == 0 || n == 0) return 0;
+    LILY_REQUIRE(weights_fit(n, k, group), "linear4: a matrix [%d, %d] in groups of %d", n, k, group);
+    LILY_REQUIRE(m > 0 && m <= lily_linear4_few(dtype), "linear4: %d tokens", m);
+    LILY_REQUIRE(dtype == kBF16 || (out_f32 && (!bias || bias_f32)), "linear4: float32 tokens keep float32");
+    LILY_REQUIRE(((uintptr_t)x | (uintptr_t)codes) % 16 == 0, "linear4: tensors on boundaries of sixteen bytes");
+    const four::ProductArgs a{x, (const uint8_t*)codes, (const __nv_bfloat16*)scales, (const uint8_t*)zeros, bias, bias_f32, out, out_f32, m, n, k, (k + 127) / 128};
+    if (dtype == kF32) {
+        const dim3 grid((n + 63) / 64);
+        if (m == 1) launch_pdl(four::product_f32_kernel<1>, grid, dim3(256), 0, stream, a, group);
+        else launch_pdl(four::product_f32_kernel<four::F32_TOKENS>, grid, dim3(256), 0, stream, a, group);
+    } else {
+        const dim3 grid((n + four::FEW_ROWS - 1) / four::FEW_ROWS), block(32 * four::FEW_WARPS);
+#define FEW(NT)                                                                                          \
+    do {                                                                                                 \
+        if (group == 128) launch_pdl(four::product_few_kernel<NT, 4>, grid, block, 0, stream, a);        \
+        else if (group == 64) launch_pdl(four::product_few_kernel<NT, 2>, grid, block, 0, stream, a);    \
+        else launch_pdl(four::product_few_kernel<NT, 1>, grid, block, 0, stream, a);                     \
+    } while (0)
+        if (m <= 8) FEW(1);
+        else FEW(2);
+#undef FEW
+    }
+    LILY_CHECK_LAUNCH("linear4");
+    return 0;
+}
+
+LILY_API int lily_weights4(const void* codes, const void* scales, const void* zeros, void* out, int dtype, int n, int k, int group, cudaStream_t stream) {
+    LILY_REQUIRE(weights_fit(n, k, group), "weights4: a matrix [%d, %d] in groups of %d", n, k, group);
+    LILY_REQUIRE(((uintptr_t)out | (uintptr_t)codes) % 16 == 0, "weights4: tensors on boundaries of sixteen bytes");
+    const four::ProductArgs a{nullptr, (const uint8_t*)codes, (const __nv_bfloat16*)scales, (const uint8_t*)zeros, nullptr, 0, out, 0, 0, n, k, (k + 127) / 128};
+    const int rows = (n + 7) / 8;
+    LILY_REQUIRE(rows <= 65535, "weights4: %d rows", n);
+    const dim3 grid((k / 8 + 127) / 128, rows);
+    if (dtype == kF32) launch_pdl(four::weights_kernel<float>, grid, dim3(256), 0, stream, a, group);
+    else launch_pdl(four::weights_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, a, group);
+    LILY_CHECK_LAUNCH("weights4");
+    return 0;
+}

@@ -14,7 +14,7 @@ import ctypes
 import functools
 import os
 from dataclasses import dataclass
-from typing import Callable, Optional, Sequence, Tuple
+from typing import Callable, NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -101,6 +101,7 @@ _SIGNATURES = {
     "lily_argmax": [_vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_apply_penalties": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_top_logprobs": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
+    "lily_cache4_values": [_vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _vp],
     "lily_sample": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
 }
 
@@ -187,6 +188,10 @@ def library():
         lib.lily_mlstm_chunk_takes.restype = _i
         lib.lily_mlstm_chunk_floats.argtypes = [_i, _i, _i, _i, _i]
         lib.lily_mlstm_chunk_floats.restype = _sz
+        lib.lily_attention_decode4_floats.argtypes = [_i, _i, _i, _i, _i, _i, _i]
+        lib.lily_attention_decode4_floats.restype = _sz
+        lib.lily_linear4_few.argtypes = [_i]
+        lib.lily_linear4_few.restype = _i
         _lib = lib
     return _lib
 
@@ -1206,7 +1211,9 @@ def _faces():
         module, lib = _build.load_faces(), library()
         names = ("lily_last_error", "lily_axes_rope_write", "lily_attention_decode_weighed_floats", "lily_attention_decode_weighed", "lily_select_keys", "lily_move_keys",
                  "lily_key_weights", "lily_key_weights_floats", "lily_key_weights_tc", "lily_key_weights_tc_floats", "lily_key_weights_tc_takes")
-        module.bind(KernelError, *[ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names])
+        address = lambda n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value
+        module.bind(KernelError, *[address(n) for n in names])
+        module.bind4(*[address(n) for n in ("lily_linear4", "lily_weights4", "lily_qk_norm_rope_write4", "lily_cache4_values", "lily_attention_decode4_floats", "lily_attention_decode4")])
         _module = module
     return _module
 
@@ -1317,6 +1324,176 @@ def move_keys(kv: torch.Tensor, weights: Optional[torch.Tensor], block_table: to
     may be a page of ``block_table``).  Places outside their tables, and what lies behind the last kept place, stay as they are."""
     (_module or _faces()).move_keys(kv, weights, block_table, kept, to_table)
     launches["count"] += 1
+
+
+# ------------------------------------------------------------------------------ serving in four bits
+
+class Weight4(NamedTuple):
+    """A matrix [n, k] held in 4-bit codes: W[r, c] = scale (code - zero) with a scale, and perhaps a zero point, for each row and ``group`` of 32, 64 or 128
+    columns.  ``codes`` uint8 [ceil(n / 128), ceil(k / 128), 128, 64]: tiles of 128 rows and columns, two codes a byte (the lower bits first), a row of a tile 16 words of
+    eight codes of which word 4 t + w holds columns 32 w + 8 t + (0..7).  ``scales`` bfloat16 [ceil(n / 128), groups of whole tiles, 128]; ``zeros`` uint8 0..15 of the same shape, or
+    None: 8.  What lies behind row n or column k is not looked at.  ``pack_weight4`` lays codes out so, ``quantize_weight4`` makes them from numbers."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    zeros: Optional[torch.Tensor]
+    n: int
+    k: int
+    group: int = 128
+
+    @property
+    def shape(self) -> Tuple[int, int]:
+        return self.n, self.k
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def bytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in self[:3] if t is not None)
+
+
+def pack_weight4(codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None) -> Weight4:
+    """Codes 0..15 [n, k] (any integer type), scales [n, k / group] and zero points 0..15 [n, k / group] (None: 8) as the products take them."""
+    n, k = codes.shape
+    groups = scales.shape[1] if scales.dim() == 2 and scales.shape[0] == n else 0
+    group = k // groups if groups else 0
+    if group not in (32, 64, 128) or group * groups != k or (zeros is not None and zeros.shape != scales.shape):
+        raise KernelError(f"pack_weight4: codes {tuple(codes.shape)} and scales {tuple(scales.shape)} do not come in groups of 32, 64 or 128 columns"
+                          + ("" if zeros is None else f", with zero points {tuple(zeros.shape)}"))
+    if codes.dtype.is_floating_point or (codes.numel() and not 0 <= int(codes.min()) <= int(codes.max()) <= 15):
+        raise KernelError("pack_weight4: codes are whole numbers 0 to 15")
+    if zeros is not None and (zeros.dtype.is_floating_point or (zeros.numel() and not 0 <= int(zeros.min()) <= int(zeros.max()) <= 15)):
+        raise KernelError("pack_weight4: zero points are whole numbers 0 to 15")
+    c = torch.nn.functional.pad(codes.to(torch.uint8), (0, -k % 128, 0, -n % 128)).unflatten(1, (-1, 4, 4, 8)).unflatten(0, (-1, 128))     # [rows / 128, 128, k / 128, w, t, 8]
+    c = c.permute(0, 2, 1, 4, 3, 5)
+    held = lambda t: torch.nn.functional.pad(t, (0, -k % 128 // group, 0, -n % 128)).unflatten(0, (-1, 128)).transpose(1, 2).contiguous()
+    return Weight4((c[..., ::2] | (c[..., 1::2] << 4)).flatten(-3).contiguous(), held(scales.to(torch.bfloat16)),
+                   None if zeros is None else held(zeros.to(torch.uint8)), n, k, group)
+
+
+def quantize_weight4(weight: torch.Tensor, group: int = 128, zeros: bool = False) -> Weight4:
+    """The nearest codes of a matrix [n, k], group by group: scale = (largest magnitude) / 7.5 around the zero point 8 (codes 0.5 to 15.5 before they are rounded and kept below 16), or, with
+    ``zeros``, scale = (max - min) / 15 over a range that holds zero, and a zero point each."""
+    n, k = weight.shape
+    if group not in (32, 64, 128) or k % group:
+        raise KernelError(f"quantize_weight4: {k} columns do not come in groups of {group} (32, 64 or 128)")
+    w = weight.float().unflatten(1, (-1, group))
+    if zeros:
+        low, high = w.amin(-1).clamp(max=0), w.amax(-1).clamp(min=0)
+        scales = ((high - low) / 15).to(torch.bfloat16)
+        s = scales.float()
+        z = torch.where(s > 0, torch.round(-low / s), 8.0).clamp(0, 15)
+    else:
+        scales = (w.abs().amax(-1) / 7.5).to(torch.bfloat16)
+        s, z = scales.float(), torch.full_like(scales, 8.0, dtype=torch.float32)
+    c = torch.where((s > 0)[..., None], torch.round(w / s[..., None]) + z[..., None], 8.0).clamp(0, 15)
+    return pack_weight4(c.to(torch.uint8).flatten(1), scales, z.to(torch.uint8) if zeros else None)
+
+
+def weights4(w: Weight4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The matrix [n, k] that ``w`` stands for: exactly in float32, rounded once in bfloat16."""
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise KernelError(f"weights4: float32 or bfloat16, not {dtype}")
+    out = (_module or _faces()).weights4(*w, dtype == torch.float32)
+    launches["count"] += 1
+    return out
+
+
+def linear4(x: torch.Tensor, w: Weight4, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``x [M, K] . W^T (+ bias)`` [M, N] for a matrix held in four bits, in the dtype of ``x`` (or float32: ``out_dtype``)."""
+    few = 16 if x.dtype == torch.bfloat16 else 8
+    if out_dtype not in (None, x.dtype, torch.float32):
+        raise KernelError(f"linear4: the result is {x.dtype} or float32, not {out_dtype}")
+    if x.dim() == 2 and x.shape[0] > few:
+        return linear(x, weights4(w, x.dtype), bias, out_dtype)
+    out = (_module or _faces()).linear4(x, *w, bias, out_dtype == torch.float32)
+    launches["count"] += 1
+    return out
+
+
+CACHE4_GROUP = 64             # features of a head that share a step and a lowest value in a cache held in four bits
+
+
+def cache4_shape(kv_heads: int, page_size: int, d: int) -> Tuple[int, int, int]:
+    """The shape of a page of a cache held in four bits, uint8: for keys and values of each head ``page_size`` rows of codes (two a byte), then a step and a lowest value, bfloat16, for each
+    place and 64 features."""
+    if d % CACHE4_GROUP or not 64 <= d <= 256:
+        raise KernelError(f"a cache held in four bits has heads of 64, 128, 192 or 256 features, not {d}")
+    return kv_heads, 2, page_size * (d // 2 + d // 16)
+
+
+def qk_norm_rope_write4(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_gain: Optional[torch.Tensor], eps: float, cos: Optional[torch.Tensor], sin: Optional[torch.Tensor],
+                        positions: torch.Tensor, token_req: torch.Tensor, block_table: torch.Tensor, kv_layer: torch.Tensor, nq: int, nkv: int, d: int, rotary_dim: int,
+                        page_size: int, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``qk_norm_rope_write`` into a cache held in four bits (``kv_layer`` uint8 [pages, *cache4_shape]): per-head RMSNorm of q and k (when gains are given), rotation by the tables, q to ``q_out``
+    [tokens, nq * d], k and v, 64 features at a time, as codes round((x - lowest) / step) with step = (max - min) / 15.  A token's codes depend on its own numbers alone, to the bit.
+    A group that holds what is not finite reads as NaN.  ``qkv`` [tokens, (nq + 2 nkv) d] float32 or bfloat16.  A position outside the tables gives NaN; what has a position or a request outside
+    the block table is not written."""
+    q = (_module or _faces()).qk_norm_rope_write4(qkv, q_gain, k_gain, eps, cos, sin, positions, token_req, block_table, kv_layer, nq, nkv, d, rotary_dim, page_size, q_out)
+    launches["count"] += 1
+    return q
+
+
+def cache4_values(kv_layer: torch.Tensor, block_table: torch.Tensor, nkv: int, d: int, page_size: int, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The numbers that pages of a cache held in four bits stand for, lowest + step code: [requests, pages, 2 (keys, values), nkv, page_size, d] of the pages that ``block_table`` names (page 0 where it
+    names none of the cache)."""
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise KernelError(f"cache4_values: float32 or bfloat16, not {dtype}")
+    out = (_module or _faces()).cache4_values(kv_layer, block_table, nkv, d, page_size, dtype == torch.float32)
+    launches["count"] += 1
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def decode4_scratch_floats(requests: int, nq: int, nkv: int, d: int, max_seq_len: int, page_size: int, dtype: torch.dtype) -> int:
+    """Float32 scratch that ``attention_decode4`` needs for rows of up to ``max_seq_len`` places."""
+    return int(library().lily_attention_decode4_floats(requests, nq, nkv, d, max_seq_len, page_size, _BF16 if dtype == torch.bfloat16 else _F32))
+
+
+def attention_decode4(q: torch.Tensor, kv_layer: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, max_seq_len: int, nq: int, nkv: int, d: int, page_size: int, scale: float,
+                      out: Optional[torch.Tensor] = None, scratch: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token a request (rows of ``q`` [requests, nq * d], float32 or bfloat16) over its ``seq_lens`` places, none more than ``max_seq_len``, of a cache held in four bits
+    (``kv_layer`` uint8 [pages, *cache4_shape]).  A request without places has a row of zeros.  ``scratch``: float32, ``decode4_scratch_floats`` of them (allocated where not given)."""
+    out = (_module or _faces()).attention_decode4(q, kv_layer, block_table, seq_lens, max_seq_len, nq, nkv, d, page_size, scale, out, scratch)
+    launches["count"] += 1
+    return out
+
+
+def attention_prefill4(q: torch.Tensor, kv_layer: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor, prefix_lens: torch.Tensor, h_prefix_lens: Sequence[int],
+                       h_new_lens: Sequence[int], nq: int, nkv: int, d: int, page_size: int, scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of prompt portions over a cache held in four bits: each request's new tokens (rows ``cu_seqlens`` of ``q`` [tokens, nq * d]) over its cached prefix and themselves, whose keys are in
+    the cache already.  ``h_prefix_lens``, ``h_new_lens``: the lengths on the host, by which the work is cut.  The pages that the portions see are brought to numbers of ``q``'s dtype first, and
+    ``attention_prefill`` reads those."""
+    _dev(q, kv_layer, block_table, cu_seqlens, prefix_lens, out)
+    requests = len(h_new_lens)
+    if nkv < 1 or nq < 1 or nq % nkv or page_size < 1 or len(h_prefix_lens) != requests or any(int(n) < 0 or int(p) < 0 for n, p in zip(h_new_lens, h_prefix_lens)):
+        raise KernelError(f"attention_prefill4: portions of {tuple(h_new_lens)} behind {tuple(h_prefix_lens)}, {nq} query heads over {nkv} kv heads")
+    if kv_layer.dtype != torch.uint8 or tuple(kv_layer.shape[1:]) != cache4_shape(nkv, page_size, d):
+        raise KernelError(f"attention_prefill4: a cache layer is uint8 [pages, {', '.join(map(str, cache4_shape(nkv, page_size, d)))}], got {kv_layer.dtype} {tuple(kv_layer.shape)}")
+    tokens = sum(h_new_lens)
+    if q.dim() != 2 or q.shape[1] != nq * d or q.shape[0] < tokens:
+        raise KernelError(f"attention_prefill4: queries are [tokens, {nq * d}], got {tuple(q.shape)} for {tokens} tokens")
+    if cu_seqlens.numel() != requests + 1 or prefix_lens.numel() != requests or block_table.dim() != 2 or block_table.shape[0] != requests:
+        raise KernelError(f"attention_prefill4: {requests} portions have a prefix and a row of the block table each and {requests + 1} offsets")
+    pages = [-(-(p + n) // page_size) if n else 0 for p, n in zip(h_prefix_lens, h_new_lens)]
+    if max(pages, default=0) > block_table.shape[1]:
+        raise KernelError(f"attention_prefill4: {max(pages)} pages of a request; the block table holds {block_table.shape[1]}")
+    if out is None:
+        out = torch.empty_like(q)
+    elif out.shape != q.shape or out.dtype != q.dtype:
+        raise KernelError("attention_prefill4: out has the shape and dtype of q")
+    if tokens == 0:
+        return out
+    width = max(pages)
+    values = torch.empty((sum(pages), 2, nkv, page_size, d), dtype=q.dtype, device=q.device)
+    table = torch.zeros((requests, width), dtype=torch.int32, device=q.device)
+    _call("lily_cache4_values", _p(kv_layer), kv_layer.shape[0], _i32(block_table, "block_table"), requests, block_table.shape[1], _p(values), _dt(q), nkv, d, page_size,
+          _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens"), _p(table), width, values.shape[0], _stream())
+    rows = prefill_tile_rows(q.dtype, d, page_size, tokens)
+    tile_req, tile_start = prefill_tiles(h_prefix_lens, h_new_lens, 0, rows, q.device)
+    attention_prefill(q, values, table, cu_seqlens, prefix_lens, tile_req, tile_start, out, nq, nkv, d, page_size, scale, tile_rows=rows)
+    return out
 
 
 # ------------------------------------------------------------------------------ joining sublayers
