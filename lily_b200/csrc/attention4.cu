@@ -23,11 +23,13 @@ struct DecodeArgs {
     float* part_o;                // [requests, nq, splits, d]
     float* part_ml;               // [requests, nq, splits, 2]
     int splits, nq, nkv, d, page_size, pages, longest;
+    int page_shift;               // tensor-core kernel: log2 of page_size
+    int requests;
     float scale;
 };
 
 // A request's places (no more than the caller said there would be).
-__device__ __forceinline__ int places_of(const DecodeArgs& a, int req) { return min(max(a.seq_lens[req], 0), a.longest); }
+__device__ __forceinline__ int places_of(const DecodeArgs& a, int req) { return min(max(__ldcg(a.seq_lens + req), 0), a.longest); }
 // The page that place `j` of a request lies in (page 0, which is nobody's, where the table names none of the cache).
 __device__ __forceinline__ int page_of(const DecodeArgs& a, int req, int j) {
     const int page = a.block_table[(size_t)req * a.width + j / a.page_size];
@@ -58,8 +60,8 @@ __device__ __forceinline__ void leave(const DecodeArgs& a, int req, int head0, i
 }
 
 // ---- bfloat16 on the tensor cores -------------------------------------------------------------------
-constexpr int KT = 64;                        // places a tile
-constexpr int WARPS = 4, STAGES = 2;
+constexpr int KT = 32;                        // places a tile
+constexpr int WARPS = 4, STAGES = 2, BLOCKS = 2;      // warps a block, tiles in a warp's ring, blocks a SM
 constexpr int HEADS = 8;                      // query heads a block: the columns of a product
 
 template <int D> struct Tile {
@@ -68,43 +70,69 @@ template <int D> struct Tile {
     static constexpr int KEYS = 0, VALUES = KT * KEY_ROW, KEY_HELD = VALUES + KT * VALUE_ROW, VALUE_HELD = KEY_HELD + KT * G * 4, BYTES = VALUE_HELD + KT * G * 4;
 };
 
-// One tile of places from `key0` on into shared memory; what lies behind `end` is zeros, or numbers of the page that nobody looks at.
+// Where a warp stands in the row of all tiles: a request, a kv head and a chunk of its query heads (a pair), a tile of the request's places.
+struct Place {
+    int req, kvh, chunk, tile, tiles, places;
+    __device__ __forceinline__ void next_pair(const DecodeArgs& a, int chunks) {
+        tile = 0;
+        if (++chunk < chunks) return;
+        chunk = 0;
+        if (++kvh < a.nkv) return;
+        kvh = 0;
+        for (tiles = 0; tiles == 0 && ++req < a.requests;) {          // (the next request that has places)
+            places = places_of(a, req);
+            tiles = (places + KT - 1) / KT;
+        }
+    }
+};
+
+// One tile of places into shared memory; what lies behind the request's last place is zeros, or numbers of the page that nobody looks at.
 template <int D>
-__device__ __forceinline__ void fetch(const DecodeArgs& a, int req, int kvh, int key0, int end, uint32_t dst) {
+__device__ __forceinline__ void fetch(const DecodeArgs& a, const Place& at, uint32_t dst) {
     using S = Tile<D>;
     constexpr int PIECES = S::CODES / 16, HELD_ROWS = S::G == 3 ? 4 : 4 / S::G, HELD_PIECES = S::G == 3 ? 3 : 1;      // places and pieces of a run of steps
-    const int lane = threadIdx.x & 31;
-    const size_t rows = (size_t)a.page_size * row_bytes(D), page_bytes = 2 * rows * a.nkv, head_at = 2 * rows * kvh;
-    const bool whole = a.page_size >= KT;
-    const int first_page = whole ? page_of(a, req, key0) : 0;
-    auto at = [&](int row, int& slot) {           // the page of a row of the tile
-        const int j = key0 + row, in = j < end;
-        slot = j % a.page_size;
-        const int page = whole ? first_page : in ? page_of(a, req, j) : 0;
-        return a.kv + page * page_bytes + head_at;
+    constexpr int RUNS = KT / HELD_ROWS * HELD_PIECES, STEPS = KT * PIECES / 32;
+    const int lane = threadIdx.x & 31, key0 = at.tile * KT, left = at.places - key0, inside = a.page_size - 1;
+    const uint32_t rows = (uint32_t)a.page_size * (uint32_t)row_bytes(D);
+    auto of_place = [&](int j) {
+        const int page = a.block_table[(size_t)at.req * a.width + (j >> a.page_shift)];
+        return a.kv + ((size_t)((unsigned)page < (unsigned)a.pages ? page : 0) * a.nkv + at.kvh) * (2 * (size_t)rows);
     };
+    if (a.page_size >= KT && left >= KT && 32 % PIECES == 0) {        // the tile lies in one page, its rows one behind the other
+        const int slot = key0 & inside;
+        const uint8_t *page = of_place(key0), *keys = page + slot * S::CODES + lane * 16, *values = keys + rows;
+        const uint32_t to = dst + lane / PIECES * S::KEY_ROW + lane % PIECES * 16, to_v = dst + S::VALUES + lane / PIECES * S::VALUE_ROW + lane % PIECES * 16;
 #pragma unroll
-    for (int i = 0; i < KT * PIECES / 32; ++i) {
-        const int c = i * 32 + lane, row = c / PIECES, piece = c - row * PIECES;
-        int slot;
-        const uint8_t* page = at(row, slot);
-        const uint8_t* p = page + (size_t)slot * S::CODES + piece * 16;
-        const bool in = key0 + row < end;
-        mma16::cp_async16(dst + S::KEYS + row * S::KEY_ROW + piece * 16, p, in);
-        mma16::cp_async16(dst + S::VALUES + row * S::VALUE_ROW + piece * 16, p + rows, in);
+        for (int i = 0; i < STEPS; ++i) {
+            mma16::cp_async16(to + i * (32 / PIECES) * S::KEY_ROW, keys + i * 512, true);
+            mma16::cp_async16(to_v + i * (32 / PIECES) * S::VALUE_ROW, values + i * 512, true);
+        }
+        if (RUNS == 32 || lane < RUNS) {                              // (RUNS is 8, 16, 24 or 32)
+            const uint8_t* held = page + a.page_size * S::CODES + slot * S::G * 4 + lane * 16;
+            mma16::cp_async16(dst + S::KEY_HELD + lane * 16, held, true);
+            mma16::cp_async16(dst + S::VALUE_HELD + lane * 16, held + rows, true);
+        }
+        return;
     }
-    constexpr int RUNS = KT / HELD_ROWS * HELD_PIECES;
-    for (int c = lane; c < RUNS; c += 32) {
-        const int row = c / HELD_PIECES * HELD_ROWS, piece = c % HELD_PIECES;
-        int slot;
-        const uint8_t* page = at(row, slot);
-        const uint8_t* p = page + (size_t)a.page_size * S::CODES + (size_t)slot * S::G * 4 + piece * 16;
-        const bool in = key0 + row < end;
-        mma16::cp_async16(dst + S::KEY_HELD + c * 16, p, in);
-        mma16::cp_async16(dst + S::VALUE_HELD + c * 16, p + rows, in);
+    for (int i = 0; i < STEPS; ++i) {
+        const int c = i * 32 + lane, row = c / PIECES, piece = c - row * PIECES, j = min(key0 + row, at.places - 1);
+        const uint8_t* p = of_place(j) + (size_t)(j & inside) * S::CODES + piece * 16;
+        mma16::cp_async16(dst + S::KEYS + row * S::KEY_ROW + piece * 16, p, row < left);
+        mma16::cp_async16(dst + S::VALUES + row * S::VALUE_ROW + piece * 16, p + rows, row < left);
+    }
+    if (lane < RUNS) {
+        const int row = lane / HELD_PIECES * HELD_ROWS, piece = lane % HELD_PIECES, j = min(key0 + row, at.places - 1);
+        const uint8_t* p = of_place(j) + (size_t)a.page_size * S::CODES + (size_t)((j & inside) / HELD_ROWS * HELD_ROWS) * S::G * 4 + piece * 16;
+        mma16::cp_async16(dst + S::KEY_HELD + lane * 16, p, row < left);
+        mma16::cp_async16(dst + S::VALUE_HELD + lane * 16, p + rows, row < left);
     }
 }
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -129,52 +157,116 @@ template <int N> __device__ __forceinline__ void words_of(const unsigned char* p
     }
 }
 
-// Keys on the rows of the products (16 of them), query heads on their eight columns: S^T = K q^T, O^T = V^T P^T.  Each warp walks tiles of its own (every fourth of the block's
-// range) through a ring of its own, so that nobody waits for anybody until the range ends.  grid (ranges, kv heads x chunks of eight heads, requests)
-template <int D>
-__global__ void __launch_bounds__(32 * WARPS, D <= 128 ? 2 : 1) decode_mma_kernel(const DecodeArgs a) {
-    using S = Tile<D>;
-    constexpr int G = S::G;
-    extern __shared__ __align__(16) unsigned char ring_s[];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int group = a.nq / a.nkv, chunks = (group + HEADS - 1) / HEADS, kvh = blockIdx.y / chunks, chunk = blockIdx.y - kvh * chunks, req = blockIdx.z;
-    const int head0 = kvh * group + chunk * HEADS, heads = min(HEADS, group - chunk * HEADS);
-    pdl_enter_small();
-    int beg, end;
-    range_of(a, req, blockIdx.x, KT, beg, end);
-    const int tiles = (end - beg + KT - 1) / KT;
-    unsigned char* mine = ring_s + warp * STAGES * S::BYTES;
-    const uint32_t ring = mma16::smem_u32(mine);
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-        const int i = warp + s * WARPS;
-        if (i < tiles) fetch<D>(a, req, kvh, beg + i * KT, end, ring + s * S::BYTES);
-        mma16::cp_async_commit();
+// How the work is cut.  Every (request, kv head, chunk of eight query heads) is a pair; its places come in tiles of 32, and all tiles of all pairs, one pair's behind the other's, are
+// shared out over the blocks, whatever the lengths: T / B tiles each and one more for the first T % B.  A pair that lies in one block's share is finished there; else each block leaves
+// (max, sum, output) of its part in a slot, 2 b for the part that its share begins with and 2 b + 1 for another, and a second kernel joins them.
+__device__ __forceinline__ int tiles_of(const DecodeArgs& a, int req) { return (places_of(a, req) + KT - 1) / KT; }
+struct Cut {
+    int per, more;
+    __device__ __forceinline__ Cut(int total, int blocks) : per(total / blocks), more(total - per * blocks) {}
+    __device__ __forceinline__ int begins(int b) const { return b * per + min(b, more); }
+    __device__ __forceinline__ int owner(int tile) const {
+        const int wide = more * (per + 1);
+        return tile < wide ? tile / (per + 1) : more + (tile - wide) / per;      // (no tile lies behind the wide shares where the others are empty)
     }
+};
+
+// Keys on the rows of the products (16 of them), query heads on their eight columns: S^T = K q^T, O^T = V^T P^T.  The warps of a block take the tiles of its share in turn, each through
+// a ring of its own that runs on from one pair to the next; they meet where a pair's part ends.
+template <int D>
+__global__ void __launch_bounds__(32 * WARPS, BLOCKS) decode_mma_kernel(const DecodeArgs a) {
+    using S = Tile<D>;
+    constexpr int G = S::G, LD = D + 4;
+    extern __shared__ __align__(16) unsigned char ring_s[];
+    __shared__ float m_s[WARPS][HEADS], l_s[WARPS][HEADS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = a.nq / a.nkv, chunks = (group + HEADS - 1) / HEADS, pairs = a.nkv * chunks;
+    unsigned char* mine = ring_s + warp * STAGES * S::BYTES;
+    float* o_s = reinterpret_cast<float*>(ring_s + WARPS * STAGES * S::BYTES);      // [warps][heads][LD]
+    const uint32_t ring = mma16::smem_u32(mine);
+    pdl_wait();
+    pdl_launch_dependents();                                          // (the joining kernel may so read the lengths ahead of its own wait)
+    int total = 0;
+    for (int r = lane; r < a.requests; r += 32) total += tiles_of(a, r);
+    total = __reduce_add_sync(0xffffffffu, total);
+    const Cut cut(total * pairs, gridDim.x);
+    const int first = cut.begins(blockIdx.x), share = cut.per + ((int)blockIdx.x < cut.more);
+    // a request without places has zeros
+    for (int r = blockIdx.x; r < a.requests; r += gridDim.x)
+        if (places_of(a, r) == 0)
+            for (int i = threadIdx.x; i < a.nq * D / 8; i += 32 * WARPS) reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (size_t)r * a.nq * D)[i] = make_uint4(0, 0, 0, 0);
+    if (share == 0) return;
+    Place at{};
+    for (int r0 = 0, before = 0; r0 < a.requests; r0 += 32) {
+        const int own = r0 + lane < a.requests ? tiles_of(a, r0 + lane) * pairs : 0;
+        int run = own;                                                // of the requests up to this lane's
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, run, x);
+            if (lane >= x) run += y;
+        }
+        const unsigned beyond = __ballot_sync(0xffffffffu, before + run > first);
+        if (beyond) {
+            const int where = __ffs(beyond) - 1;
+            at.req = r0 + where;
+            at.places = places_of(a, at.req);
+            at.tiles = (at.places + KT - 1) / KT;
+            const int in = first - (before + __shfl_sync(0xffffffffu, run - own, where)), pair_no = in / at.tiles;
+            at.tile = in - pair_no * at.tiles;
+            at.kvh = chunks == 1 ? pair_no : pair_no / chunks;
+            at.chunk = pair_no - at.kvh * chunks;
+            break;
+        }
+        before += __shfl_sync(0xffffffffu, run, 31);
+    }
+    // the tile to ask for next, the `asked`-th of the share: this warp's own are `warp` and every fourth behind it
+    Place ahead = at;
+    int asked = warp, issued = 0;
+    ahead.tile += warp;
+    auto ask = [&]() {
+        if (asked < share) {
+            while (ahead.tile >= ahead.tiles) {
+                const int over = ahead.tile - ahead.tiles;
+                ahead.next_pair(a, chunks);
+                ahead.tile = over;
+            }
+            fetch<D>(a, ahead, ring + issued % STAGES * S::BYTES);
+            ++issued;
+            asked += WARPS;
+            ahead.tile += WARPS;
+        }
+        mma16::cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) ask();
+    int next = warp, used = 0;                                        // this warp's next tile of the share; tiles taken out of the ring
+    for (int began = 0; began < share;) {
+    const int req = at.req, head0 = at.kvh * group + at.chunk * HEADS, heads = min(HEADS, group - at.chunk * HEADS), ends = min(share, began + at.tiles - at.tile);
     // the queries as the products' second operand, in the order of the keys' words, and their sums
     uint32_t q[G][2][4];
     float sums[G];
 #pragma unroll
     for (int j = 0; j < G; ++j) {
-        float sum = 0.f;
+        float both = 0.f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             uint4 v = make_uint4(0, 0, 0, 0);
             if (g < heads) v = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + ((size_t)req * a.nq + head0 + g) * D + 64 * j + 32 * h + 8 * t);
-            sum += low(v.x) + high(v.x) + low(v.y) + high(v.y) + low(v.z) + high(v.z) + low(v.w) + high(v.w);
+            if (a.scale < 0.f) v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
+            both += low(v.x) + high(v.x) + low(v.y) + high(v.y) + low(v.z) + high(v.z) + low(v.w) + high(v.w);
             q[j][h][0] = __byte_perm(v.x, v.z, 0x5410);               // features 0 and 4, 1 and 5, 2 and 6, 3 and 7 of the eight
             q[j][h][1] = __byte_perm(v.x, v.z, 0x7632);
             q[j][h][2] = __byte_perm(v.y, v.w, 0x5410);
             q[j][h][3] = __byte_perm(v.y, v.w, 0x7632);
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sums[j] = sum + __shfl_xor_sync(0xffffffffu, sum, 2);
+        both += __shfl_xor_sync(0xffffffffu, both, 1);
+        sums[j] = both + __shfl_xor_sync(0xffffffffu, both, 2);
     }
     float qs[G][2];                                                   // of heads 2 t and 2 t + 1
 #pragma unroll
     for (int j = 0; j < G; ++j) qs[j][0] = __shfl_sync(0xffffffffu, sums[j], 8 * t), qs[j][1] = __shfl_sync(0xffffffffu, sums[j], 8 * t + 4);
-    const float scale = a.scale * LOG2E;
-    float o[G][4][4], most[2] = {-INFINITY, -INFINITY}, total[2] = {0.f, 0.f}, ones[G][4], lows[G][2];
+    const float scale = fabsf(a.scale) * LOG2E;
+    float o[G][4][4], most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, ones[G][4], lows[G][2];      // (scores and their maximum are kept unscaled)
 #pragma unroll
     for (int j = 0; j < G; ++j) {
         lows[j][0] = lows[j][1] = 0.f;
@@ -186,169 +278,207 @@ __global__ void __launch_bounds__(32 * WARPS, D <= 128 ? 2 : 1) decode_mma_kerne
         }
     }
     const uint32_t one[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-    int slot = 0;
-    for (int i = warp; i < tiles; i += WARPS) {
-        {
-            const int next = i + (STAGES - 1) * WARPS, to = slot == 0 ? STAGES - 1 : slot - 1;
-            if (next < tiles) fetch<D>(a, req, kvh, beg + next * KT, end, ring + to * S::BYTES);
-            mma16::cp_async_commit();
-        }
-        mma16::cp_async_wait<STAGES - 1>();
-        __syncwarp();
-        const unsigned char* tile = mine + slot * S::BYTES;
-        const int left = end - (beg + i * KT);                        // places of the tile that are the request's
-        for (int r0 = 0; r0 < KT && r0 < left; r0 += 32) {
-            float s[2][4];                                            // scores of keys g and g + 8, heads 2 t and 2 t + 1
+    const float margin = 8.f / scale;                                 // in units of scores
+    auto work = [&](const unsigned char* tile, const int left) {
+        float s[2][4];                                                // scores of keys g and g + 8, heads 2 t and 2 t + 1
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-                const int row = r0 + 16 * mt + g;
-                uint32_t w0[2 * G], w1[2 * G];
-                words_of<2 * G>(tile + S::KEYS + row * S::KEY_ROW + t * 8 * G, w0);
-                words_of<2 * G>(tile + S::KEYS + (row + 8) * S::KEY_ROW + t * 8 * G, w1);
-                const uint32_t* held0 = reinterpret_cast<const uint32_t*>(tile + S::KEY_HELD) + row * G;
+        for (int mt = 0; mt < 2; ++mt) {
+            const int row = 16 * mt + g;
+            uint32_t w0[2 * G], w1[2 * G], h0[G], h1[G];
+            words_of<2 * G>(tile + S::KEYS + row * S::KEY_ROW + t * 8 * G, w0);
+            words_of<2 * G>(tile + S::KEYS + (row + 8) * S::KEY_ROW + t * 8 * G, w1);
+            words_of<G>(tile + S::KEY_HELD + row * 4 * G, h0);
+            words_of<G>(tile + S::KEY_HELD + (row + 8) * 4 * G, h1);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[mt][e] = 0.f;
+            for (int e = 0; e < 4; ++e) s[mt][e] = 0.f;
 #pragma unroll
-                for (int j = 0; j < G; ++j) {
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < G; ++j) {
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t x = w0[2 * j + h], y = w1[2 * j + h];
-                        const uint32_t a0[4] = {pair(x, 0), pair(y, 0), pair(x, 1), pair(y, 1)}, a1[4] = {pair(x, 2), pair(y, 2), pair(x, 3), pair(y, 3)};
-                        mma16::mma_bf16(c, a0, q[j][h][0], q[j][h][1]);
-                        mma16::mma_bf16(c, a1, q[j][h][2], q[j][h][3]);
-                    }
-                    const uint32_t h0 = held0[j], h1 = held0[8 * G + j];
-                    const float s0 = low(h0) * scale, s1 = low(h1) * scale, b0 = fmaf(s0, -128.f, high(h0) * scale), b1 = fmaf(s1, -128.f, high(h1) * scale);
-                    s[mt][0] += fmaf(s0, c[0], b0 * qs[j][0]);
-                    s[mt][1] += fmaf(s0, c[1], b0 * qs[j][1]);
-                    s[mt][2] += fmaf(s1, c[2], b1 * qs[j][0]);
-                    s[mt][3] += fmaf(s1, c[3], b1 * qs[j][1]);
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t x = w0[2 * j + h], y = w1[2 * j + h];
+                    const uint32_t a0[4] = {pair(x, 0), pair(y, 0), pair(x, 1), pair(y, 1)}, a1[4] = {pair(x, 2), pair(y, 2), pair(x, 3), pair(y, 3)};
+                    mma16::mma_bf16(c, a0, q[j][h][0], q[j][h][1]);
+                    mma16::mma_bf16(c, a1, q[j][h][2], q[j][h][3]);
                 }
+                const float s0 = low(h0[j]), s1 = low(h1[j]), b0 = fmaf(s0, -128.f, high(h0[j])), b1 = fmaf(s1, -128.f, high(h1[j]));
+                s[mt][0] = fmaf(s0, c[0], fmaf(b0, qs[j][0], s[mt][0]));
+                s[mt][1] = fmaf(s0, c[1], fmaf(b0, qs[j][1], s[mt][1]));
+                s[mt][2] = fmaf(s1, c[2], fmaf(b1, qs[j][0], s[mt][2]));
+                s[mt][3] = fmaf(s1, c[3], fmaf(b1, qs[j][1], s[mt][3]));
+            }
+            if (left < KT) {
                 if (row >= left) s[mt][0] = s[mt][1] = -INFINITY;
                 if (row + 8 >= left) s[mt][2] = s[mt][3] = -INFINITY;
             }
-            float m0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])), m1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
+        }
+        float m0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])), m1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
+        // The maximum moves only where a score is 2^8 times its weight ahead (weights of up to 256 are as good as ones of up to 1), which after the first tile is rare.
+        if (__any_sync(0xffffffffu, m0 > most[0] + margin || m1 > most[1] + margin)) {
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) {
                 m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, x));
                 m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, x));
             }
-            if (__any_sync(0xffffffffu, m0 > most[0] || m1 > most[1])) {
-                m0 = fmaxf(m0, most[0]);
-                m1 = fmaxf(m1, most[1]);
-                const float f0 = m0 == most[0] ? 1.f : exp2f(most[0] - m0), f1 = m1 == most[1] ? 1.f : exp2f(most[1] - m1);
-                most[0] = m0;
-                most[1] = m1;
-                total[0] *= f0;
-                total[1] *= f1;
+            m0 = fmaxf(m0, most[0]);
+            m1 = fmaxf(m1, most[1]);
+            const float f0 = m0 == most[0] ? 1.f : ex2((most[0] - m0) * scale), f1 = m1 == most[1] ? 1.f : ex2((most[1] - m1) * scale);
+            most[0] = m0;
+            most[1] = m1;
+            sum[0] *= f0;
+            sum[1] *= f1;
 #pragma unroll
-                for (int j = 0; j < G; ++j) {
-                    lows[j][0] *= f0;
-                    lows[j][1] *= f1;
-                    ones[j][0] *= f0;
-                    ones[j][1] *= f1;
-                    ones[j][2] *= f0;
-                    ones[j][3] *= f1;
+            for (int j = 0; j < G; ++j) {
+                lows[j][0] *= f0;
+                lows[j][1] *= f1;
+                ones[j][0] *= f0;
+                ones[j][1] *= f1;
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) o[j][n][0] *= f0, o[j][n][1] *= f1, o[j][n][2] *= f0, o[j][n][3] *= f1;
-                }
+                for (int n = 0; n < 4; ++n) o[j][n][0] *= f0, o[j][n][1] *= f1, o[j][n][2] *= f0, o[j][n][3] *= f1;
             }
-            const float z0 = most[0] == -INFINITY ? 0.f : most[0], z1 = most[1] == -INFINITY ? 0.f : most[1];      // (nobody has a score yet)
+        }
+        const float z0 = most[0] == -INFINITY ? 0.f : -most[0] * scale, z1 = most[1] == -INFINITY ? 0.f : -most[1] * scale;      // (nobody has a score yet)
 #pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-                const int row = r0 + 16 * mt;
-                float p[4];
-                p[0] = exp2f(s[mt][0] - z0);
-                p[1] = exp2f(s[mt][1] - z1);
-                p[2] = exp2f(s[mt][2] - z0);
-                p[3] = exp2f(s[mt][3] - z1);
-                total[0] += p[0] + p[2];
-                total[1] += p[1] + p[3];
-                const uint32_t* held0 = reinterpret_cast<const uint32_t*>(tile + S::VALUE_HELD) + (row + g) * G;
-                uint32_t w[4][G];
+        for (int mt = 0; mt < 2; ++mt) {
+            const int row = 16 * mt;
+            float p[4];
+            p[0] = ex2(fmaf(s[mt][0], scale, z0));
+            p[1] = ex2(fmaf(s[mt][1], scale, z1));
+            p[2] = ex2(fmaf(s[mt][2], scale, z0));
+            p[3] = ex2(fmaf(s[mt][3], scale, z1));
+            sum[0] += p[0] + p[2];
+            sum[1] += p[1] + p[3];
+            uint32_t w[4][G], h0[G], h1[G];
+            words_of<G>(tile + S::VALUE_HELD + (row + g) * 4 * G, h0);
+            words_of<G>(tile + S::VALUE_HELD + (row + g + 8) * 4 * G, h1);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) words_of<G>(tile + S::VALUES + (row + 2 * t + (e & 1) + (e >> 1) * 8) * S::VALUE_ROW + g * 4 * G, w[e]);
+            for (int e = 0; e < 4; ++e) words_of<G>(tile + S::VALUES + (row + 2 * t + (e & 1) + (e >> 1) * 8) * S::VALUE_ROW + g * 4 * G, w[e]);
 #pragma unroll
-                for (int j = 0; j < G; ++j) {
-                    const uint32_t h0 = row + g < left ? held0[j] : 0u, h1 = row + g + 8 < left ? held0[8 * G + j] : 0u;      // (what stands behind the last place may be no number)
-                    lows[j][0] = fmaf(p[2], high(h1), fmaf(p[0], high(h0), lows[j][0]));
-                    lows[j][1] = fmaf(p[3], high(h1), fmaf(p[1], high(h0), lows[j][1]));
-                    // weights times steps, rounded to bfloat16 as the second operand asks
-                    const uint32_t b0 = transposed(bits(__floats2bfloat162_rn(p[0] * low(h0), p[1] * low(h0))));
-                    const uint32_t b1 = transposed(bits(__floats2bfloat162_rn(p[2] * low(h1), p[3] * low(h1))));
-                    mma16::mma_bf16(ones[j], one, b0, b1);
-                    const uint32_t x0 = __byte_perm(w[0][j], w[1][j], 0x5410), x1 = __byte_perm(w[0][j], w[1][j], 0x7632);
-                    const uint32_t y0 = __byte_perm(w[2][j], w[3][j], 0x5410), y1 = __byte_perm(w[2][j], w[3][j], 0x7632);
+            for (int j = 0; j < G; ++j) {
+                if (left < KT) {                                      // (what stands behind the last place may be no number)
+                    if (row + g >= left) h0[j] = 0;
+                    if (row + g + 8 >= left) h1[j] = 0;
+                }
+                lows[j][0] = fmaf(p[2], high(h1[j]), fmaf(p[0], high(h0[j]), lows[j][0]));
+                lows[j][1] = fmaf(p[3], high(h1[j]), fmaf(p[1], high(h0[j]), lows[j][1]));
+                // weights times steps, rounded to bfloat16 as the second operand asks
+                const float s0 = low(h0[j]), s1 = low(h1[j]);
+                const uint32_t b0 = transposed(bits(__floats2bfloat162_rn(p[0] * s0, p[1] * s0))), b1 = transposed(bits(__floats2bfloat162_rn(p[2] * s1, p[3] * s1)));
+                mma16::mma_bf16(ones[j], one, b0, b1);
+                const uint32_t x0 = __byte_perm(w[0][j], w[1][j], 0x5410), x1 = __byte_perm(w[0][j], w[1][j], 0x7632);
+                const uint32_t y0 = __byte_perm(w[2][j], w[3][j], 0x5410), y1 = __byte_perm(w[2][j], w[3][j], 0x7632);
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {                     // features 8 g + 2 n (rows g) and 8 g + 2 n + 1 (rows g + 8) of the group
-                        const uint32_t x = n < 2 ? x0 : x1, y = n < 2 ? y0 : y1;
-                        const int i0 = 2 * (n & 1);
-                        const uint32_t av[4] = {pair(x, i0), pair(x, i0 + 1), pair(y, i0), pair(y, i0 + 1)};
-                        mma16::mma_bf16(o[j][n], av, b0, b1);
-                    }
+                for (int n = 0; n < 4; ++n) {                         // features 8 g + 2 n (rows g) and 8 g + 2 n + 1 (rows g + 8) of the group
+                    const uint32_t x = n < 2 ? x0 : x1, y = n < 2 ? y0 : y1;
+                    const int i0 = 2 * (n & 1);
+                    const uint32_t av[4] = {pair(x, i0), pair(x, i0 + 1), pair(y, i0), pair(y, i0 + 1)};
+                    mma16::mma_bf16(o[j][n], av, b0, b1);
                 }
             }
         }
+    };
+    for (; next < ends; next += WARPS, ++used) {
+        ask();
+        mma16::cp_async_wait<STAGES - 1>();
         __syncwarp();
-        slot = slot == STAGES - 1 ? 0 : slot + 1;
+        work(mine + used % STAGES * S::BYTES, at.places - (at.tile + next - began) * KT);
+        __syncwarp();
     }
-    // the block's warps together: (max, sum, output) of each in shared memory
-    mma16::cp_async_wait<0>();
+    // the warps' sums together: finished, where the whole pair was here; else to the part's slot
 #pragma unroll
     for (int x = 4; x < 32; x <<= 1) {
-        total[0] += __shfl_xor_sync(0xffffffffu, total[0], x);
-        total[1] += __shfl_xor_sync(0xffffffffu, total[1], x);
+        sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], x);
+        sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], x);
 #pragma unroll
         for (int j = 0; j < G; ++j) {
             lows[j][0] += __shfl_xor_sync(0xffffffffu, lows[j][0], x);
             lows[j][1] += __shfl_xor_sync(0xffffffffu, lows[j][1], x);
         }
     }
-    __syncthreads();
-    constexpr int LD = D + 4;
-    float* o_s = reinterpret_cast<float*>(ring_s);                    // [warps][heads][LD]
-    float* m_s = o_s + WARPS * HEADS * LD;                            // [warps][heads]
-    float* l_s = m_s + WARPS * HEADS;
-    if (g == 0) {
-        m_s[warp * HEADS + 2 * t] = most[0];
-        m_s[warp * HEADS + 2 * t + 1] = most[1];
-        l_s[warp * HEADS + 2 * t] = total[0];
-        l_s[warp * HEADS + 2 * t + 1] = total[1];
-    }
 #pragma unroll
-    for (int j = 0; j < G; ++j)
+    for (int e = 0; e < 2; ++e) {
+        const int h = 2 * t + e;
+        if (h >= heads) continue;
+        if (g == 0) m_s[warp][h] = most[e] * scale, l_s[warp][h] = sum[e];
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int j = 0; j < G; ++j) {                                 // features 64 j + 8 g + (0..7)
+            float4* to = reinterpret_cast<float4*>(o_s + (warp * HEADS + h) * LD + 64 * j + 8 * g);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                o_s[(warp * HEADS + 2 * t + (e & 1)) * LD + 64 * j + 8 * g + 2 * n + (e >> 1)] = fmaf(-128.f, ones[j][e & 1], o[j][n][e] + lows[j][e & 1]);
-    __syncthreads();
-    float* f_s = l_s + WARPS * HEADS;                                 // [warps][heads]: what each warp's sums count
-    if (threadIdx.x < HEADS) {
-        const int h = threadIdx.x;
-        float m = -INFINITY;
-        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, m_s[w * HEADS + h]);
-        float l = 0.f;
-        for (int w = 0; w < WARPS; ++w) {
-            const float f = m_s[w * HEADS + h] == -INFINITY ? (l_s[w * HEADS + h] == 0.f ? 0.f : 1.f) : exp2f(m_s[w * HEADS + h] - m);
-            f_s[w * HEADS + h] = f;
-            l += f * l_s[w * HEADS + h];
+            for (int i = 0; i < 2; ++i)
+                to[i] = make_float4(fmaf(-128.f, ones[j][e], o[j][2 * i][e] + lows[j][e]), fmaf(-128.f, ones[j][e], o[j][2 * i][e + 2] + lows[j][e]),
+                                    fmaf(-128.f, ones[j][e], o[j][2 * i + 1][e] + lows[j][e]), fmaf(-128.f, ones[j][e], o[j][2 * i + 1][e + 2] + lows[j][e]));
         }
-        m_s[h] = m;
-        l_s[h] = l;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < heads * D; i += 32 * WARPS) {
-        const int h = i / D, f = i - h * D;
-        float v = 0.f;
+    const bool alone = at.tile == 0 && ends - began == at.tiles;
+    const size_t part = 2 * (size_t)blockIdx.x + (began != 0);
+    for (int i = threadIdx.x; i < heads * (D / 4); i += 32 * WARPS) {
+        const int h = i / (D / 4), f = 4 * (i - h * (D / 4));
+        float m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w)
-            if (f_s[w * HEADS + h] != 0.f) v += f_s[w * HEADS + h] * o_s[(w * HEADS + h) * LD + f];
-        o_s[h * LD + f] = v;                                          // (read and written by this thread alone)
+        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, m_s[w][h]);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float by = m_s[w][h] == -INFINITY ? (l_s[w][h] == 0.f ? 0.f : 1.f) : ex2(m_s[w][h] - m);
+            const float4 x = *reinterpret_cast<const float4*>(o_s + (w * HEADS + h) * LD + f);
+            if (by != 0.f) l = fmaf(by, l_s[w][h], l), v.x = fmaf(by, x.x, v.x), v.y = fmaf(by, x.y, v.y), v.z = fmaf(by, x.z, v.z), v.w = fmaf(by, x.w, v.w);
+        }
+        if (alone) {
+            const float by = l == 0.f ? 0.f : 1.f / l;
+            *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)req * a.nq + head0 + h) * D + f) =
+                make_uint2(bits(__floats2bfloat162_rn(v.x * by, v.y * by)), bits(__floats2bfloat162_rn(v.z * by, v.w * by)));
+        } else {
+            *reinterpret_cast<float4*>(a.part_o + (part * HEADS + h) * D + f) = v;
+            if (f == 0) *reinterpret_cast<float2*>(a.part_ml + (part * HEADS + h) * 2) = make_float2(m, l);
+        }
     }
-    __syncthreads();
-    leave<__nv_bfloat16>(a, req, head0, heads, m_s, l_s, o_s, LD);
+    __syncthreads();                                                  // (the next part's sums go where these were)
+    began = ends;
+    if (began < share) at.next_pair(a, chunks);
+    }
+}
+
+// The parts of a pair that several blocks have worked on: a block a pair.  grid (pairs of a request, requests)
+constexpr int JOIN_THREADS = 128;
+template <int D>
+__global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const DecodeArgs a, int blocks) {
+    const int req = blockIdx.y, group = a.nq / a.nkv, chunks = (group + HEADS - 1) / HEADS, pairs = a.nkv * chunks;
+    const int kvh = blockIdx.x / chunks, chunk = blockIdx.x - kvh * chunks, head0 = kvh * group + chunk * HEADS, heads = min(HEADS, group - chunk * HEADS);
+    pdl_launch_dependents();
+    const int tiles = tiles_of(a, req), lane = threadIdx.x & 31;
+    int total = 0, before = 0;
+    for (int r = lane; r < a.requests; r += 32) {
+        const int n = tiles_of(a, r);
+        total += n;
+        if (r < req) before += n;
+    }
+    const Cut cut(__reduce_add_sync(0xffffffffu, total) * pairs, blocks);
+    const int lo = __reduce_add_sync(0xffffffffu, before) * pairs + (int)blockIdx.x * tiles;
+    // the blocks whose shares hold its first and its last tile (those between them have tiles)
+    const int b0 = tiles ? cut.owner(lo) : 0, b1 = tiles ? cut.owner(lo + tiles - 1) : 0, behind = tiles && cut.begins(b0) != lo;
+    pdl_wait();
+    if (b0 == b1) return;
+    for (int i = threadIdx.x; i < heads * (D / 4); i += JOIN_THREADS) {
+        const int h = i / (D / 4), f = 4 * (i - h * (D / 4));
+        float m = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+        for (int b = b0; b <= b1; ++b) {
+            const size_t part = 2 * (size_t)b + (b == b0 ? behind : 0);
+            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (part * HEADS + h) * 2);
+            const float4 v = *reinterpret_cast<const float4*>(a.part_o + (part * HEADS + h) * D + f);
+            const float next = fmaxf(m, ml.x), was = m == next ? 1.f : ex2(m - next);
+            const float by = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - next);
+            m = next;
+            l *= was;
+            o.x *= was, o.y *= was, o.z *= was, o.w *= was;
+            if (by != 0.f) l = fmaf(by, ml.y, l), o.x = fmaf(by, v.x, o.x), o.y = fmaf(by, v.y, o.y), o.z = fmaf(by, v.z, o.z), o.w = fmaf(by, v.w, o.w);
+        }
+        const float by = l == 0.f ? 0.f : 1.f / l;
+        *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)req * a.nq + head0 + h) * D + f) =
+            make_uint2(bits(__floats2bfloat162_rn(o.x * by, o.y * by)), bits(__floats2bfloat162_rn(o.z * by, o.w * by)));
+    }
 }
 
 // ---- any page, float32 or bfloat16 queries, on the CUDA cores -----------------------------------------
@@ -451,13 +581,24 @@ __global__ void __launch_bounds__(128) join_kernel(const DecodeArgs a) {
     }
 }
 
-// Ranges a row's places are cut into.
-inline int ranges_of(int requests, int nq, int nkv, int d, int longest, int page_size, int dtype) {
-    const bool tensor_cores = dtype == kBF16 && page_size % 16 == 0;
+inline int log2_of(int page_size) {
+    int shift = 0;
+    while (1 << shift < page_size) ++shift;
+    return 1 << shift == page_size ? shift : -1;
+}
+// The tensor-core kernel takes bfloat16 and pages of a power of two from 16 places on (a run of sixteen bytes of steps lies in one page).
+inline bool on_tensor_cores(int page_size, int dtype) { return dtype == kBF16 && page_size >= 16 && log2_of(page_size) >= 0; }
+
+// Ranges a row's places are cut into on the CUDA cores: as many as fill the device, none too short.
+inline int ranges_of(int requests, int nq, int nkv, int longest) {
     const long long pairs = (long long)requests * nkv * ((nq / nkv + HEADS - 1) / HEADS);
-    const int room = (tensor_cores ? (d <= 128 ? 2 : 1) : 3) * sm_count(), step = tensor_cores ? KT * WARPS : SIMT_KT * 2;
-    const long long want = pairs > 0 ? room / pairs : 1, most = ((long long)longest + step - 1) / step;
+    const long long want = pairs > 0 ? 3 * sm_count() / pairs : 1, most = ((long long)longest + 2 * SIMT_KT - 1) / (2 * SIMT_KT);
     return (int)max(1ll, min(min(want, most), 256ll));
+}
+// Blocks of the tensor-core kernel: as many as are on the device at once, a tile a warp at least.
+inline int blocks_of(int requests, int nq, int nkv, int d, int longest) {
+    const long long pairs = (long long)requests * nkv * ((nq / nkv + HEADS - 1) / HEADS), tiles = pairs * (((long long)longest + KT - 1) / KT);
+    return (int)max(1ll, min((long long)BLOCKS * sm_count(), (tiles + WARPS - 1) / WARPS));
 }
 
 }  // namespace four
@@ -468,7 +609,8 @@ using namespace lily;
 // float32 of scratch that lily_attention_decode4 needs
 LILY_API size_t lily_attention_decode4_floats(int requests, int nq, int nkv, int d, int longest, int page_size, int dtype) {
     if (requests <= 0 || nkv <= 0 || nq <= 0 || nq % nkv || page_size <= 0) return 0;
-    const int splits = four::ranges_of(requests, nq, nkv, d, longest, page_size, dtype);
+    if (four::on_tensor_cores(page_size, dtype)) return (size_t)2 * four::blocks_of(requests, nq, nkv, d, longest) * four::HEADS * (d + 2);
+    const int splits = four::ranges_of(requests, nq, nkv, longest);
     return splits == 1 ? 0 : (size_t)requests * nq * splits * (d + 2);
 }
 
@@ -481,30 +623,43 @@ LILY_API int lily_attention_decode4(const void* q, const void* kv, void* out, co
                  requests, longest, width, page_size);
     LILY_REQUIRE(longest <= INT32_MAX - 1024, "attention_decode4: rows of %d places", longest);
     LILY_REQUIRE(((uintptr_t)q | (uintptr_t)kv | (uintptr_t)out) % 16 == 0, "attention_decode4: tensors on boundaries of sixteen bytes");
+    LILY_REQUIRE(scale != 0.f && scale - scale == 0.f, "attention_decode4: a scale of %g", (double)scale);
     const int chunks = (nq / nkv + four::HEADS - 1) / four::HEADS;
     LILY_REQUIRE((long long)nkv * chunks <= 65535, "attention_decode4: %d kv heads", nkv);
     four::DecodeArgs a{};
     a.q = q; a.kv = (const uint8_t*)kv; a.out = out; a.block_table = block_table; a.width = width; a.seq_lens = seq_lens;
-    a.splits = four::ranges_of(requests, nq, nkv, d, longest, page_size, dtype);
-    a.part_o = scratch;
-    a.part_ml = scratch + (size_t)requests * nq * a.splits * d;
+    const bool tensor_cores = four::on_tensor_cores(page_size, dtype);
+    a.requests = requests;
     a.nq = nq; a.nkv = nkv; a.d = d; a.page_size = page_size; a.pages = pages; a.longest = longest; a.scale = scale;
-    LILY_REQUIRE(a.splits == 1 || scratch != nullptr, "attention_decode4: %d ranges need scratch", a.splits);
-    const dim3 grid(a.splits, nkv * chunks, requests);
-    if (dtype == kBF16 && page_size % 16 == 0) {
+    if (tensor_cores) {
+        a.page_shift = four::log2_of(page_size);
+        LILY_REQUIRE((long long)requests * nkv * chunks * ((longest + four::KT - 1) / four::KT) <= INT32_MAX, "attention_decode4: %d requests of up to %d places are too many for one call", requests, longest);
+        const int blocks = four::blocks_of(requests, nq, nkv, d, longest);
+        LILY_REQUIRE(scratch != nullptr && (uintptr_t)scratch % 16 == 0, "attention_decode4: the parts of %d blocks need scratch on a boundary of sixteen bytes", blocks);
+        a.part_o = scratch;
+        a.part_ml = scratch + (size_t)2 * blocks * four::HEADS * d;
 #define DECODE(D)                                                                                                                     \
     {                                                                                                                                 \
-        constexpr int ring = four::WARPS * four::STAGES * four::Tile<D>::BYTES, join = four::WARPS * four::HEADS * (D + 4 + 3) * 4;   \
-        constexpr int bytes = ring > join ? ring : join;                                                                              \
+        constexpr int bytes = four::WARPS * (four::STAGES * four::Tile<D>::BYTES + four::HEADS * (D + 4) * 4);                        \
         cudaFuncSetAttribute(four::decode_mma_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);                         \
-        launch_pdl(four::decode_mma_kernel<D>, grid, dim3(32 * four::WARPS), bytes, stream, a);                                       \
+        launch_pdl(four::decode_mma_kernel<D>, dim3(blocks), dim3(32 * four::WARPS), bytes, stream, a);                               \
+        LILY_CHECK_LAUNCH("attention_decode4");                                                                                       \
+        launch_pdl(four::join_parts_kernel<D>, dim3(nkv * chunks, requests), dim3(four::JOIN_THREADS), 0, stream, a, blocks); \
     }
         if (d == 64) DECODE(64)
         else if (d == 128) DECODE(128)
         else if (d == 192) DECODE(192)
         else DECODE(256)
 #undef DECODE
-    } else {
+        LILY_CHECK_LAUNCH("attention_decode4 (join)");
+        return 0;
+    }
+    a.splits = four::ranges_of(requests, nq, nkv, longest);
+    a.part_o = scratch;
+    a.part_ml = scratch + (size_t)requests * nq * a.splits * d;
+    LILY_REQUIRE(a.splits == 1 || scratch != nullptr, "attention_decode4: %d ranges need scratch", a.splits);
+    const dim3 grid(a.splits, nkv * chunks, requests);
+    {
         const size_t bytes = four::simt_floats(d) * sizeof(float);
         auto run = [&](auto kernel) {
             cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);

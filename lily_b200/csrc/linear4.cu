@@ -149,38 +149,47 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) product_few_kernel(const Pr
     }
 }
 
-// Up to eight tokens in float32: a warp eight rows, a lane 32 columns of one of them at a time, all products and sums in float32.  grid (rows / 64)
-constexpr int F32_TOKENS = 8;
+// Up to eight tokens in float32: a block eight rows, its eight warps an eighth of the columns' tiles each; a lane eight columns of a row at a time, all products and sums in
+// float32, a word's eight of them before their scale.  grid (rows / 8)
+constexpr int F32_TOKENS = 8, F32_WARPS = 8;
 template <int TOKENS>
-__global__ void __launch_bounds__(256) product_f32_kernel(const ProductArgs a, int group) {
+__global__ void __launch_bounds__(32 * F32_WARPS) product_f32_kernel(const ProductArgs a, int group_shift) {
+    __shared__ float sum_s[F32_WARPS][TOKENS][8];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int row0 = blockIdx.x * 64 + warp * 8, row = row0 + g, tile_row = row0 / 128;
-    pdl_enter_small();
-    if (row0 >= a.n) return;
+    const int row0 = blockIdx.x * 8, tile_row = row0 / 128;
     const uint8_t* codes = a.codes + ((size_t)tile_row * a.tiles * 128 + row0 % 128) * 64 + lane * 16;
-    const int per_tile = 128 / group;
-    const size_t held0 = (size_t)tile_row * a.tiles * per_tile * 128 + row0 % 128 + g;
+    const size_t held0 = (size_t)tile_row * (a.tiles * 128 >> group_shift) * 128 + row0 % 128 + g;
+    uint4 v = make_uint4(0, 0, 0, 0), next = v;
+    if (warp < a.tiles) v = weights16(codes + (size_t)warp * 128 * 64);
+    pdl_launch_dependents();
+    pdl_wait();
     float total[TOKENS];
 #pragma unroll
     for (int i = 0; i < TOKENS; ++i) total[i] = 0.f;
-    for (int kt = 0; kt < a.tiles; ++kt) {
-        const uint4 v = weights16(codes + (size_t)kt * 128 * 64);
+    for (int kt = warp; kt < a.tiles; kt += F32_WARPS, v = next) {
+        if (kt + F32_WARPS < a.tiles) next = weights16(codes + (size_t)(kt + F32_WARPS) * 128 * 64);
         const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+        float s[4], z[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int col = kt * 128 + 32 * w;
+            const size_t at = held0 + (size_t)(col >> group_shift) * 128;
+            s[w] = col < a.k ? __bfloat162float(a.scales[at]) : 0.f;
+            z[w] = 8388608.f + (a.zeros && col < a.k ? (float)a.zeros[at] : 8.f);
+        }
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const int col = kt * 128 + 32 * w + 8 * t;
             if (col >= a.k) continue;
-            const size_t at = held0 + (size_t)((kt * 128 + 32 * w) / group) * 128;
-            const float s = __bfloat162float(a.scales[at]), z = a.zeros ? (float)a.zeros[at] : 8.f;
             float c[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) c[e] = ((float)(words[w] >> (4 * e) & 15u) - z) * s;
+            for (int e = 0; e < 8; ++e) c[e] = __uint_as_float((words[w] >> (4 * e) & 15u) | 0x4B000000u) - z[w];         // (2^23 + code: exact)
 #pragma unroll
             for (int i = 0; i < TOKENS; ++i) {
                 if (i >= a.m) break;
                 const float4 *p = reinterpret_cast<const float4*>((const float*)a.x + (size_t)i * a.k + col), x0 = p[0], x1 = p[1];
-                total[i] = fmaf(c[0], x0.x, fmaf(c[1], x0.y, fmaf(c[2], x0.z, fmaf(c[3], x0.w, total[i]))));
-                total[i] = fmaf(c[4], x1.x, fmaf(c[5], x1.y, fmaf(c[6], x1.z, fmaf(c[7], x1.w, total[i]))));
+                const float first = fmaf(c[0], x0.x, fmaf(c[1], x0.y, fmaf(c[2], x0.z, c[3] * x0.w))), second = fmaf(c[4], x1.x, fmaf(c[5], x1.y, fmaf(c[6], x1.z, c[7] * x1.w)));
+                total[i] = fmaf(s[w], first + second, total[i]);
             }
         }
     }
@@ -188,7 +197,15 @@ __global__ void __launch_bounds__(256) product_f32_kernel(const ProductArgs a, i
     for (int i = 0; i < TOKENS; ++i) {
         total[i] += __shfl_xor_sync(0xffffffffu, total[i], 1);
         total[i] += __shfl_xor_sync(0xffffffffu, total[i], 2);
-        if (i < a.m && t == 0 && row < a.n) ((float*)a.out)[(size_t)i * a.n + row] = total[i] + (a.bias ? ((const float*)a.bias)[row] : 0.f);
+        if (t == 0) sum_s[warp][i][g] = total[i];
+    }
+    __syncthreads();
+    if (threadIdx.x < TOKENS * 8) {
+        const int i = threadIdx.x / 8, r = threadIdx.x % 8;
+        float y = 0.f;
+#pragma unroll
+        for (int w = 0; w < F32_WARPS; ++w) y += sum_s[w][i][r];
+        if (i < a.m && row0 + r < a.n) ((float*)a.out)[(size_t)i * a.n + row0 + r] = y + (a.bias ? ((const float*)a.bias)[row0 + r] : 0.f);
     }
 }
 
@@ -237,9 +254,11 @@ LILY_API int lily_linear4(const void* x, int dtype, const void* codes, const voi
     LILY_REQUIRE(((uintptr_t)x | (uintptr_t)codes) % 16 == 0, "linear4: tensors on boundaries of sixteen bytes");
     const four::ProductArgs a{x, (const uint8_t*)codes, (const __nv_bfloat16*)scales, (const uint8_t*)zeros, bias, bias_f32, out, out_f32, m, n, k, (k + 127) / 128};
     if (dtype == kF32) {
-        const dim3 grid((n + 63) / 64);
-        if (m == 1) launch_pdl(four::product_f32_kernel<1>, grid, dim3(256), 0, stream, a, group);
-        else launch_pdl(four::product_f32_kernel<four::F32_TOKENS>, grid, dim3(256), 0, stream, a, group);
+        const dim3 grid((n + 7) / 8), block(32 * four::F32_WARPS);
+        const int shift = group == 32 ? 5 : group == 64 ? 6 : 7;
+        if (m == 1) launch_pdl(four::product_f32_kernel<1>, grid, block, 0, stream, a, shift);
+        else if (m <= 4) launch_pdl(four::product_f32_kernel<4>, grid, block, 0, stream, a, shift);
+        else launch_pdl(four::product_f32_kernel<four::F32_TOKENS>, grid, block, 0, stream, a, shift);
     } else {
         const dim3 grid((n + four::FEW_ROWS - 1) / four::FEW_ROWS), block(32 * four::FEW_WARPS);
 #define FEW(NT)                                                                                          \
