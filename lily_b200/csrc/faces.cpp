@@ -48,6 +48,7 @@ struct Entries {
     int (*key_weights_tc_takes)(int, int, int, int, float);
     // numbers held in four bits
     int (*linear4)(const void*, int, const void*, const void*, const void*, const void*, int, void*, int, int, int, int, int, void*);
+    int (*linear4_many)(const void*, const void*, const void*, const void*, const void*, int, void*, int, int, int, int, int, void*);
     int (*weights4)(const void*, const void*, const void*, void*, int, int, int, int, void*);
     int (*write4)(const void*, int, int, const void*, const void*, int, double, const float*, const float*, int, const int*, int, const int*, const int*, int, int, void*, int, void*, int, int,
                   int, int, int, void*);
@@ -411,9 +412,9 @@ Matrix4 matrix4(const char* what, PyObject* const* p) {
     return w;
 }
 
-// x, codes, scales, zeros, n, k, group, bias, whether the result is float32 whatever x is
+// x, codes, scales, zeros, n, k, group, bias, whether the result is float32 whatever x is, tokens from which on tcgen05 multiplies
 PyObject* linear4(PyObject*, PyObject* const* p, Py_ssize_t count) {
-    return guarded(count, 9, [&]() -> PyObject* {
+    return guarded(count, 10, [&]() -> PyObject* {
         const Tensor& x = tensor(p[0]);
         const Matrix4 w = matrix4("linear4", p + 1);
         const Tensor* bias = maybe(p[7]);
@@ -422,6 +423,11 @@ PyObject* linear4(PyObject*, PyObject* const* p, Py_ssize_t count) {
         if (bias && (bias->dim() != 1 || bias->numel() != w.n || (code_of(*bias) == BF16 && code == F32))) refuse("linear4: a bias of ", w.n, " numbers, got ", words(*bias));
         here({&x, &w.codes, &w.scales, w.zeros, bias});
         Tensor out = at::empty({x.size(0), (int64_t)w.n}, x.options().dtype(wide ? at::kFloat : at::kBFloat16));
+        if (code == BF16 && x.size(0) >= number(p[9])) {
+            done("lily_linear4_many", call(entry.linear4_many, x.const_data_ptr(), w.codes.const_data_ptr(), w.scales.const_data_ptr(), w.zeros ? w.zeros->const_data_ptr() : nullptr,
+                                           bias ? bias->const_data_ptr() : nullptr, bias ? (int)(code_of(*bias) == F32) : 0, out.data_ptr(), wide, narrow(x.size(0)), w.n, w.k, w.group, stream()));
+            return THPVariable_Wrap(std::move(out));
+        }
         done("lily_linear4", call(entry.linear4, x.const_data_ptr(), code, w.codes.const_data_ptr(), w.scales.const_data_ptr(), w.zeros ? w.zeros->const_data_ptr() : nullptr,
                                   bias ? bias->const_data_ptr() : nullptr, bias ? (int)(code_of(*bias) == F32) : 0, out.data_ptr(), wide, narrow(x.size(0)), w.n, w.k, w.group, stream()));
         return THPVariable_Wrap(std::move(out));
@@ -530,15 +536,16 @@ PyObject* attention_decode4(PyObject*, PyObject* const* p, Py_ssize_t count) {
 
 // the addresses of the entries for numbers held in four bits, in their order
 PyObject* bind4(PyObject*, PyObject* const* p, Py_ssize_t count) {
-    return guarded(count, 6, [&]() -> PyObject* {
-        void* at[6];
-        for (int i = 0; i < 6; ++i) at[i] = (void*)(uintptr_t)whole(p[i]);
+    return guarded(count, 7, [&]() -> PyObject* {
+        void* at[7];
+        for (int i = 0; i < 7; ++i) at[i] = (void*)(uintptr_t)whole(p[i]);
         entry.linear4 = (decltype(entry.linear4))at[0];
         entry.weights4 = (decltype(entry.weights4))at[1];
         entry.write4 = (decltype(entry.write4))at[2];
         entry.values4 = (decltype(entry.values4))at[3];
         entry.decode4_floats = (decltype(entry.decode4_floats))at[4];
         entry.decode4 = (decltype(entry.decode4))at[5];
+        entry.linear4_many = (decltype(entry.linear4_many))at[6];
         Py_RETURN_NONE;
     });
 }

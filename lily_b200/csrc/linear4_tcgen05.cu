@@ -1,0 +1,350 @@
+// Products with 4-bit weights for more than a few tokens, on tcgen05: Y^T = W X^T, weights on the 128 rows of a tile, up to 256 tokens on its columns.
+//
+// A block has 128 rows of W and a range of its columns, in steps of 128:
+//   warp 0     brings the step's codes (8 KB, contiguous), scales and zero points by bulk copies and its tokens [tokens, 128] by TMA into a ring of stages;
+//   warps 2-17 make the codes bfloat16 numbers, (code - zero) exactly and then its product with the scale, rounded once, in the swizzled layout of an operand: eight warps the even steps,
+//              eight the odd ones;
+//   warp 1     multiplies: eight 128 x tokens x 16 products a step into one accumulator in tensor memory.
+// The blocks of a cluster share out a row tile's columns and add their accumulators up through shared memory, each for its share of the tokens.
+// The weights are rounded to bfloat16 because an operand of the tensor cores has one scale for all its columns; their products and sums are float32 throughout.
+//
+// Every wait is bounded: one that runs out leaves its code in a status word (lily_linear4_status) and NaN in the block's outputs.
+#include "four.cuh"
+#include "tcgen05.cuh"
+
+#include <cooperative_groups.h>
+
+namespace lily {
+namespace four {
+namespace many {
+
+constexpr int ROWS = 128, STEP = 128;
+constexpr int CODES = ROWS * STEP / 2;
+constexpr int OPERAND = ROWS * STEP * 2;                 // two halves of 64 columns, rows of 128 bytes
+constexpr int OPERANDS = 4;                              // at most; two where many tokens leave no room
+constexpr int WORKERS = 8, GROUPS = 2, THREADS = 32 * (2 + GROUPS * WORKERS);      // warps that make an operand, groups of them that take steps in turn
+constexpr int MOST_TOKENS = 256, MOST_SPLITS = 8;
+constexpr uint32_t SPIN_LIMIT = 1u << 17;                // polls of up to ten microseconds each: a second before a wait gives up
+
+__device__ int g_status = 0;                             // 0; else (code << 24 | block) of the first wait that gave up
+
+struct Args {
+    const uint8_t* codes;
+    const uint8_t* scales;                               // bytes of bfloat16 numbers
+    const uint8_t* zeros;                                // or null: 8
+    const void* bias;
+    int bias_f32;
+    void* out;
+    int out_f32;
+    int m, n, k, tiles;                                  // tiles of 128 columns
+    int tokens;                                          // columns of the accumulator, a multiple of 16
+    int stages, splits, operands;
+};
+
+// Asks once, asleep for up to ten microseconds: a warp that polls takes turns away from those that work.
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity), "r"(10000u) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* lost, int code) {
+    bool come = false;
+    uint32_t i = 0;
+    for (; i < SPIN_LIMIT && !come; ++i) {
+        come = try_wait(bar, parity);
+        if ((i & 15u) == 15u && *lost) break;
+    }
+    come = __all_sync(0xffffffffu, come);                // (the whole warp goes on, or none of it)
+    if (!come && !*lost) {
+        *lost = 1;
+        atomicCAS(&g_status, 0, (code << 24) | (int)((blockIdx.x + blockIdx.y * gridDim.x) & 0xFFFFFF));
+    }
+    return come;
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// Bytes i of two words of codes 0..15, one code a byte, as a pair of bfloat16 numbers code 2^-133 (the lowest subnormal ones; the bytes above them are the codes' signs, zero).
+template <int I>
+__device__ __forceinline__ uint32_t tiny_pair(uint32_t even, uint32_t odd) {
+    uint32_t r;                                          // (the intrinsic leaves out the selector's bits for signs)
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(even), "r"(odd), "n"(0xC480 + 0x1111 * I));
+    return r;
+}
+
+// What a stage holds: codes, scales (up to four groups of 128), zero points, tokens (two halves).
+__host__ __device__ constexpr int SCALES_AT() { return CODES; }
+__host__ __device__ constexpr int ZEROS_AT() { return CODES + 4 * 256; }
+__host__ __device__ constexpr int TOKENS_AT() { return CODES + 4 * 256 + 4 * 128 + 512; }       // (a multiple of 1024 for the swizzle)
+__host__ __device__ inline int stage_bytes(int tokens) { return TOKENS_AT() + tokens * 256; }
+
+// grid (row tiles x splits, token tiles), cluster (splits)
+template <int PER_STEP>                                  // groups of a step: 1, 2 or 4
+__global__ void __launch_bounds__(THREADS, 1) product_many_kernel(const __grid_constant__ CUtensorMap map_x, const Args a) {
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + (-tc5::smem_u32(smem_raw) & 1023u);      // (an offset, so that it stays an address of shared memory)
+    __shared__ __align__(8) uint64_t bars[2 * 8 + 2 * OPERANDS + 1];
+    __shared__ uint32_t tmem_s;
+    __shared__ int lost_s, given_up_s;                   // a wait of this block ran out, of another one of the cluster
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = blockIdx.x % a.splits, row_tile = blockIdx.x / a.splits, token0 = blockIdx.y * a.tokens;
+    const int kt0 = (int)((long long)a.tiles * rank / a.splits), steps = (int)((long long)a.tiles * (rank + 1) / a.splits) - kt0;
+    const int stage = stage_bytes(a.tokens);
+    unsigned char* operands = smem;                      // [operands][OPERAND]
+    unsigned char* ring = smem + a.operands * OPERAND;
+    const uint32_t full0 = tc5::smem_u32(&bars[0]), empty0 = tc5::smem_u32(&bars[8]), made0 = tc5::smem_u32(&bars[16]), freed0 = tc5::smem_u32(&bars[16 + OPERANDS]),
+                   ready = tc5::smem_u32(&bars[16 + 2 * OPERANDS]);
+    volatile int* lost = &lost_s;
+    uint32_t columns = 32;
+    while ((int)columns < a.tokens) columns *= 2;
+
+    if (threadIdx.x == 0) {
+        lost_s = given_up_s = 0;
+        for (int s = 0; s < a.stages; ++s) {
+            tc5::mbar_init(full0 + 8 * s, 1);
+            tc5::mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int s = 0; s < OPERANDS; ++s) {
+            tc5::mbar_init(made0 + 8 * s, WORKERS);
+            tc5::mbar_init(freed0 + 8 * s, 1);
+        }
+        tc5::mbar_init(ready, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tc5::smem_u32(&tmem_s)), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    tc5::tc_fence_before();
+    __syncthreads();
+    tc5::tc_fence_after();
+    const uint32_t tmem = tmem_s;
+    pdl_launch_dependents();
+
+    if (warp == 0) {
+        const uint32_t held = 256u * PER_STEP, bytes = CODES + held + (a.zeros ? held / 2 : 0) + (uint32_t)a.tokens * 256;
+        const uint8_t* codes = a.codes + ((size_t)row_tile * a.tiles + kt0) * CODES;
+        const uint8_t* scales = a.scales + ((size_t)row_tile * a.tiles + kt0) * held;
+        const uint8_t* zeros = a.zeros ? a.zeros + ((size_t)row_tile * a.tiles + kt0) * (held / 2) : nullptr;
+        auto weights = [&](int it, int s) {
+            const uint32_t at = tc5::smem_u32(ring + (size_t)s * stage), bar = full0 + 8 * s;
+            tc5::mbar_expect_tx(bar, bytes);
+            bulk_copy(at, codes + (size_t)it * CODES, CODES, bar);
+            bulk_copy(at + SCALES_AT(), scales + (size_t)it * held, held, bar);
+            if (zeros) bulk_copy(at + ZEROS_AT(), zeros + (size_t)it * (held / 2), held / 2, bar);
+        };
+        auto tokens = [&](int it, int s) {
+            const uint32_t at = tc5::smem_u32(ring + (size_t)s * stage) + TOKENS_AT(), bar = full0 + 8 * s;
+            tc5::tma_load_2d(at, &map_x, bar, (kt0 + it) * STEP, token0);
+            tc5::tma_load_2d(at + a.tokens * 128, &map_x, bar, (kt0 + it) * STEP + 64, token0);
+        };
+        // the first stages' weights are nobody's results: on their way before the kernel ahead has ended
+        const int early = min(a.stages, steps);
+        if (tc5::elect_one())
+            for (int it = 0; it < early; ++it) weights(it, it);
+        __syncwarp();
+        pdl_wait();
+        if (tc5::elect_one())
+            for (int it = 0; it < early; ++it) tokens(it, it);
+        __syncwarp();
+        int it = early;
+        for (int s = 0, turn = 0; it < steps; ++it) {
+            if (!wait(empty0 + 8 * s, turn, lost, 1)) break;
+            if (tc5::elect_one()) {
+                weights(it, s);
+                tokens(it, s);
+            }
+            __syncwarp();
+            if (++s == a.stages) s = 0, turn ^= 1;
+        }
+        if (*lost)                                       // copies already issued still land here: give each a bounded wait
+            for (int j = max(0, it - a.stages); j < it; ++j)
+                for (uint32_t i = 0; i < (1u << 20) && !tc5::mbar_try_wait(full0 + 8 * (j % a.stages), (j / a.stages) & 1); ++i) {}
+    } else if (warp == 1) {
+        // kind::f16, bfloat16 a and b (k-major), float32 d, 128 rows
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(a.tokens >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+        bool ok = true;
+        for (int it = 0, s = 0, turn = 0, o = 0, o_turn = 0; it < steps; ++it) {
+            ok = wait(full0 + 8 * s, turn, lost, 2) && wait(made0 + 8 * o, o_turn, lost, 3);
+            if (!ok) break;
+            tc5::tc_fence_after();
+            const uint32_t w = tc5::smem_u32(operands + o * OPERAND), x = tc5::smem_u32(ring + (size_t)s * stage) + TOKENS_AT();
+            if (tc5::elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < STEP / 16; ++kk) {
+                    const uint64_t da = tc5::desc_k_major(w + (kk / 4) * (OPERAND / 2)) + (uint64_t)((kk % 4) * 2);
+                    const uint64_t db = tc5::desc_k_major(x + (kk / 4) * (a.tokens * 128)) + (uint64_t)((kk % 4) * 2);
+                    tc5::umma(tmem, da, db, idesc, (it | kk) != 0 ? 1u : 0u);
+                }
+                tc5::umma_commit(empty0 + 8 * s);
+                tc5::umma_commit(freed0 + 8 * o);
+                if (it == steps - 1) tc5::umma_commit(ready);
+            }
+            __syncwarp();
+            if (++s == a.stages) s = 0, turn ^= 1;
+            if (++o == a.operands) o = 0, o_turn ^= 1;
+        }
+    } else {
+        // A thread a row's piece of sixteen bytes, twice a step: a word of each 32 columns.  Of eight neighbouring threads four have a row and four the row four further, whose
+        // swizzled pieces lie in the other banks.
+        const int group = (warp - 2) / WORKERS, worker = (threadIdx.x - 64) % (32 * WORKERS), t = worker & 3, row0 = (worker >> 5 << 3) | (worker >> 3 & 3) | (worker & 4);
+        const __nv_bfloat162 up = __halves2bfloat162(__ushort_as_bfloat16(0x7F00), __ushort_as_bfloat16(0x7F00));                 // 2^127
+        int s = group, turn = 0, o = group, o_turn = 1;  // (there are two stages at least, and an even number of operands)
+        for (int it = group; it < steps; it += GROUPS) {
+            if (!wait(full0 + 8 * s, turn, lost, 4)) break;
+            const unsigned char* in = ring + (size_t)s * stage;
+            uint4 raw[2];
+            uint32_t scale[2][PER_STEP], zero[2][PER_STEP];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int row = half * 64 + row0;
+                raw[half] = *reinterpret_cast<const uint4*>(in + row * 64 + t * 16);
+#pragma unroll
+                for (int i = 0; i < PER_STEP; ++i) {
+                    scale[half][i] = *reinterpret_cast<const unsigned short*>(in + SCALES_AT() + (i * 128 + row) * 2);
+                    zero[half][i] = a.zeros ? in[ZEROS_AT() + i * 128 + row] : 8u;
+                }
+            }
+            if (it >= a.operands && !wait(freed0 + 8 * o, o_turn, lost, 5)) break;
+            unsigned char* to = operands + o * OPERAND;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int row = half * 64 + row0;
+                const uint32_t words[4] = {raw[half].x, raw[half].y, raw[half].z, raw[half].w};
+#pragma unroll
+                for (int i = 0; i < PER_STEP; ++i) {
+                    // (code - zero) 2^-6 in one operation, exactly; its product with 2^6 scale rounded once
+                    const __nv_bfloat162 down = __bfloat162bfloat162(__float2bfloat16_rn((__uint_as_float(0x4B000000u | zero[half][i]) - 8388608.f) * -0.015625f));
+                    float f = __uint_as_float(scale[half][i] << 16) * 64.f;
+                    if ((kt0 + it) * STEP + i * (STEP / PER_STEP) >= a.k) f = 0.f;      // (what stands behind the last column may be no number)
+                    const __nv_bfloat162 by = __bfloat162bfloat162(__float2bfloat16_rn(f));
+                    auto number = [&](uint32_t tiny) { return bits(__hmul2(__hfma2(two(tiny), up, down), by)); };
+#pragma unroll
+                    for (int v = 0; v < 4 / PER_STEP; ++v) {
+                        const int w = i * (4 / PER_STEP) + v;
+                        const uint32_t even = words[w] & 0x0F0F0F0Fu, odd = words[w] >> 4 & 0x0F0F0F0Fu;
+                        const uint4 numbers = make_uint4(number(tiny_pair<0>(even, odd)), number(tiny_pair<1>(even, odd)), number(tiny_pair<2>(even, odd)), number(tiny_pair<3>(even, odd)));
+                        const int piece = (w & 1) * 4 + t;
+                        *reinterpret_cast<uint4*>(to + (w >> 1) * (OPERAND / 2) + row * 128 + ((piece ^ (row & 7)) << 4)) = numbers;
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tc5::mbar_arrive(made0 + 8 * o);
+            s += GROUPS;
+            if (s >= a.stages) s -= a.stages, turn ^= 1;
+            o += GROUPS;
+            if (o >= a.operands) o -= a.operands, o_turn ^= 1;
+        }
+        // the accumulator to shared memory, where the ring was: [tokens][128]
+        const bool ok = wait(ready, 0, lost, 6);
+        tc5::tc_fence_after();
+        float* sums = reinterpret_cast<float*>(smem);
+        const int quarter = warp & 3, first = (warp - 2) >> 2;      // (a warp reads its quarter of the lanes)
+        for (int c = first * 32; c < a.tokens; c += 32 * (GROUPS * WORKERS / 4)) {
+            float v[32] = {};
+            if (ok) {
+                tc5::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
+                tc5::tmem_wait_ld();
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                if (c + e < a.tokens) sums[(c + e) * ROWS + quarter * 32 + lane] = v[e];
+        }
+        tc5::tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 1) {
+        tc5::tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(columns) : "memory");
+    }
+    const auto cluster = cooperative_groups::this_cluster();
+    if (a.splits > 1) {
+        cluster.sync();
+        if (lost_s && threadIdx.x < a.splits) *cluster.map_shared_rank(&given_up_s, threadIdx.x) = 1;
+        cluster.sync();
+    }
+    const float* sums = reinterpret_cast<const float*>(smem);
+    const bool given_up = lost_s || given_up_s;
+    for (int i = threadIdx.x; i < (a.tokens - rank + a.splits - 1) / a.splits * ROWS; i += THREADS) {
+        const int token = rank + i / ROWS * a.splits, r = i % ROWS, row = row_tile * ROWS + r, y = token0 + token;
+        if (y >= a.m || row >= a.n) continue;
+        float v = 0.f;
+        if (a.splits == 1) v = sums[token * ROWS + r];
+        else {
+            float part[MOST_SPLITS];
+#pragma unroll
+            for (int z = 0; z < MOST_SPLITS; ++z) part[z] = z < a.splits ? *cluster.map_shared_rank(sums + token * ROWS + r, z) : 0.f;
+#pragma unroll
+            for (int z = 0; z < MOST_SPLITS; ++z) v += part[z];
+        }
+        if (a.bias) v += a.bias_f32 ? ((const float*)a.bias)[row] : __bfloat162float(((const __nv_bfloat16*)a.bias)[row]);
+        if (given_up) v = __int_as_float(0x7fffffff);
+        const size_t to = (size_t)y * a.n + row;
+        if (a.out_f32) ((float*)a.out)[to] = v;
+        else ((__nv_bfloat16*)a.out)[to] = __float2bfloat16_rn(v);
+    }
+    if (a.splits > 1) cluster.sync();                    // nobody leaves while its memory is read
+}
+
+}  // namespace many
+}  // namespace four
+}  // namespace lily
+
+using namespace lily;
+
+// 0, or the code of a wait that gave up since the word was last read (synchronises, and clears it).
+LILY_API int lily_linear4_status() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, four::many::g_status, sizeof(int)) != cudaSuccess) return -1;
+    if (v) cudaMemcpyToSymbol(four::many::g_status, &zero, sizeof(int));
+    return v;
+}
+
+LILY_API int lily_linear4_many(const void* x, const void* codes, const void* scales, const void* zeros, const void* bias, int bias_f32, void* out, int out_f32, int m, int n, int k, int group,
+                               cudaStream_t stream) {
+    using namespace four::many;
+    if (m == 0 || n == 0) return 0;
+    LILY_REQUIRE(n > 0 && k > 0 && (group == 32 || group == 64 || group == 128) && k % group == 0 && n <= INT32_MAX - 256 && k <= INT32_MAX - 256, "linear4: a matrix [%d, %d] in groups of %d", n, k,
+                 group);
+    LILY_REQUIRE(m > 0 && ((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales | (uintptr_t)zeros) % 16 == 0, "linear4: tensors on boundaries of sixteen bytes");
+    const int token_tiles = (m + MOST_TOKENS - 1) / MOST_TOKENS, row_tiles = (n + ROWS - 1) / ROWS;
+    Args a{(const uint8_t*)codes, (const uint8_t*)scales, (const uint8_t*)zeros, bias, bias_f32, out, out_f32, m, n, k, (k + STEP - 1) / STEP};
+    a.tokens = ((m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
+    // columns shared out while there are SMs without a row tile, no fewer than two steps a block
+    a.splits = 1;
+    while (a.splits < MOST_SPLITS && 2ll * a.splits * row_tiles * token_tiles <= sm_count() && a.tiles >= 4 * a.splits) a.splits *= 2;
+    // four operands in shared memory, so that nobody waits for a product, where that leaves three stages
+    const int stage = stage_bytes(a.tokens), room = 224 * 1024;
+    a.operands = room - OPERANDS * OPERAND >= 3 * stage ? OPERANDS : 2;
+    a.stages = min(min(6, (room - a.operands * OPERAND) / stage), max(2, (a.tiles + a.splits - 1) / a.splits));
+    const int bytes = max(a.operands * OPERAND + a.stages * stage, a.tokens * ROWS * 4) + 1024;
+    LILY_REQUIRE(a.stages >= 2 && row_tiles <= INT32_MAX / 8 && token_tiles <= 65535, "linear4: %d tokens, %d rows", m, n);
+    tc5::EncodeTiled encode = tc5::encoder();
+    LILY_REQUIRE(encode != nullptr, "linear4: no encoder of tensor maps");
+    CUtensorMap map;
+    const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)m}, strides[1] = {(cuuint64_t)k * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)a.tokens}, steps[2] = {1, 1};
+    const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    LILY_REQUIRE(rc == CUDA_SUCCESS, "linear4: tensor map: error %d", (int)rc);
+    auto kernel = group == 128 ? product_many_kernel<1> : group == 64 ? product_many_kernel<2> : product_many_kernel<4>;
+    LILY_REQUIRE(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess, "linear4: cannot get %d bytes of shared memory", bytes);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(row_tiles * a.splits, token_tiles);
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = a.splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kernel, map, a);
+    LILY_CHECK_LAUNCH("linear4");
+    return 0;
+}

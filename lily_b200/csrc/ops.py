@@ -102,6 +102,7 @@ _SIGNATURES = {
     "lily_apply_penalties": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_top_logprobs": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_cache4_values": [_vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _vp],
+    "lily_linear4_status": [],
     "lily_sample": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
 }
 
@@ -1213,7 +1214,7 @@ def _faces():
                  "lily_key_weights", "lily_key_weights_floats", "lily_key_weights_tc", "lily_key_weights_tc_floats", "lily_key_weights_tc_takes")
         address = lambda n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value
         module.bind(KernelError, *[address(n) for n in names])
-        module.bind4(*[address(n) for n in ("lily_linear4", "lily_weights4", "lily_qk_norm_rope_write4", "lily_cache4_values", "lily_attention_decode4_floats", "lily_attention_decode4")])
+        module.bind4(*[address(n) for n in ("lily_linear4", "lily_weights4", "lily_qk_norm_rope_write4", "lily_cache4_values", "lily_attention_decode4_floats", "lily_attention_decode4", "lily_linear4_many")])
         _module = module
     return _module
 
@@ -1400,14 +1401,21 @@ def weights4(w: Weight4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     return out
 
 
+LINEAR4_MANY = 512            # tokens up to which a product makes numbers of its codes on the way
+
+
+def linear4_status() -> int:
+    """0, or the code of a bounded wait that gave up in the tcgen05 kernel of ``linear4`` since the code was last read (synchronises, and clears it); what its block was to give is NaN."""
+    return int(library().lily_linear4_status())
+
+
 def linear4(x: torch.Tensor, w: Weight4, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``x [M, K] . W^T (+ bias)`` [M, N] for a matrix held in four bits, in the dtype of ``x`` (or float32: ``out_dtype``)."""
-    few = 16 if x.dtype == torch.bfloat16 else 8
     if out_dtype not in (None, x.dtype, torch.float32):
         raise KernelError(f"linear4: the result is {x.dtype} or float32, not {out_dtype}")
-    if x.dim() == 2 and x.shape[0] > few:
+    if x.dim() == 2 and x.shape[0] > (LINEAR4_MANY if x.dtype == torch.bfloat16 else 8):
         return linear(x, weights4(w, x.dtype), bias, out_dtype)
-    out = (_module or _faces()).linear4(x, *w, bias, out_dtype == torch.float32)
+    out = (_module or _faces()).linear4(x, *w, bias, out_dtype == torch.float32, 17)
     launches["count"] += 1
     return out
 
