@@ -1,9 +1,9 @@
 // Products with 4-bit weights for more than a few tokens, on tcgen05: Y^T = W X^T, weights on the 128 rows of a tile, up to 256 tokens on its columns.
 //
 // A block has 128 rows of W and a range of its columns, in steps of 128:
-//   warp 0     brings the step's codes (8 KB, contiguous), scales and zero points by bulk copies and its tokens [tokens, 128] by TMA into a ring of stages;
-//   warps 2-17 make the codes bfloat16 numbers, (code - zero) exactly and then its product with the scale, rounded once, in the swizzled layout of an operand: eight warps the even steps,
-//              eight the odd ones;
+//   warp 0     brings the step's codes (8 KB) and its tokens [tokens, 128] by TMA, its scales and zero points by bulk copies, into a ring of stages;
+//   warps 2-9  make the codes bfloat16 numbers, (code - zero) exactly and then its product with the scale, rounded once, and put them into tensor memory as the products' first
+//              operand (a thread a row; four warps the even steps, four the odd ones): through shared memory they would be written and read at the bandwidth that bounds the products;
 //   warp 1     multiplies: eight 128 x tokens x 16 products a step into one accumulator in tensor memory.
 // The blocks of a cluster share out a row tile's columns and add their accumulators up through shared memory, each for its share of the tokens.
 // The weights are rounded to bfloat16 because an operand of the tensor cores has one scale for all its columns; their products and sums are float32 throughout.
@@ -20,16 +20,15 @@ namespace many {
 
 constexpr int ROWS = 128, STEP = 128;
 constexpr int CODES = ROWS * STEP / 2;
-constexpr int OPERAND = ROWS * STEP * 2;                 // two halves of 64 columns, rows of 128 bytes
-constexpr int OPERANDS = 4;                              // at most; two where many tokens leave no room
-constexpr int WORKERS = 8, GROUPS = 2, THREADS = 32 * (2 + GROUPS * WORKERS);      // warps that make an operand, groups of them that take steps in turn
+constexpr int OPERAND = STEP / 2;                        // columns of tensor memory of a step's weights
+constexpr int OPERANDS = 4;                              // at most
+constexpr int GROUPS = 2, WORKERS = 4, THREADS = 32 * (2 + GROUPS * WORKERS);      // groups of warps that take steps in turn, a warp a quarter of the rows
 constexpr int MOST_TOKENS = 256, MOST_SPLITS = 8;
 constexpr uint32_t SPIN_LIMIT = 1u << 17;                // polls of up to ten microseconds each: a second before a wait gives up
 
 __device__ int g_status = 0;                             // 0; else (code << 24 | block) of the first wait that gave up
 
 struct Args {
-    const uint8_t* codes;
     const uint8_t* scales;                               // bytes of bfloat16 numbers
     const uint8_t* zeros;                                // or null: 8
     const void* bias;
@@ -39,6 +38,7 @@ struct Args {
     int m, n, k, tiles;                                  // tiles of 128 columns
     int tokens;                                          // columns of the accumulator, a multiple of 16
     int stages, splits, operands;
+    int columns;                                         // of tensor memory: the accumulator's, then the operands'
 };
 
 // Asks once, asleep for up to ten microseconds: a warp that polls takes turns away from those that work.
@@ -80,7 +80,7 @@ __host__ __device__ inline int stage_bytes(int tokens) { return TOKENS_AT() + to
 
 // grid (row tiles x splits, token tiles), cluster (splits)
 template <int PER_STEP>                                  // groups of a step: 1, 2 or 4
-__global__ void __launch_bounds__(THREADS, 1) product_many_kernel(const __grid_constant__ CUtensorMap map_x, const Args a) {
+__global__ void __launch_bounds__(THREADS, 2) product_many_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const Args a) {
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + (-tc5::smem_u32(smem_raw) & 1023u);      // (an offset, so that it stays an address of shared memory)
     __shared__ __align__(8) uint64_t bars[2 * 8 + 2 * OPERANDS + 1];
@@ -90,13 +90,11 @@ __global__ void __launch_bounds__(THREADS, 1) product_many_kernel(const __grid_c
     const int rank = blockIdx.x % a.splits, row_tile = blockIdx.x / a.splits, token0 = blockIdx.y * a.tokens;
     const int kt0 = (int)((long long)a.tiles * rank / a.splits), steps = (int)((long long)a.tiles * (rank + 1) / a.splits) - kt0;
     const int stage = stage_bytes(a.tokens);
-    unsigned char* operands = smem;                      // [operands][OPERAND]
-    unsigned char* ring = smem + a.operands * OPERAND;
+    unsigned char* ring = smem;
     const uint32_t full0 = tc5::smem_u32(&bars[0]), empty0 = tc5::smem_u32(&bars[8]), made0 = tc5::smem_u32(&bars[16]), freed0 = tc5::smem_u32(&bars[16 + OPERANDS]),
                    ready = tc5::smem_u32(&bars[16 + 2 * OPERANDS]);
     volatile int* lost = &lost_s;
-    uint32_t columns = 32;
-    while ((int)columns < a.tokens) columns *= 2;
+    const uint32_t columns = a.columns;
 
     if (threadIdx.x == 0) {
         lost_s = given_up_s = 0;
@@ -118,18 +116,18 @@ __global__ void __launch_bounds__(THREADS, 1) product_many_kernel(const __grid_c
     tc5::tc_fence_before();
     __syncthreads();
     tc5::tc_fence_after();
-    const uint32_t tmem = tmem_s;
+    const uint32_t tmem = tmem_s, operands = tmem + columns - a.operands * OPERAND;
     pdl_launch_dependents();
 
     if (warp == 0) {
         const uint32_t held = 256u * PER_STEP, bytes = CODES + held + (a.zeros ? held / 2 : 0) + (uint32_t)a.tokens * 256;
-        const uint8_t* codes = a.codes + ((size_t)row_tile * a.tiles + kt0) * CODES;
+        const int codes = (row_tile * a.tiles + kt0) * ROWS;
         const uint8_t* scales = a.scales + ((size_t)row_tile * a.tiles + kt0) * held;
         const uint8_t* zeros = a.zeros ? a.zeros + ((size_t)row_tile * a.tiles + kt0) * (held / 2) : nullptr;
         auto weights = [&](int it, int s) {
             const uint32_t at = tc5::smem_u32(ring + (size_t)s * stage), bar = full0 + 8 * s;
             tc5::mbar_expect_tx(bar, bytes);
-            bulk_copy(at, codes + (size_t)it * CODES, CODES, bar);
+            tc5::tma_load_2d(at, &map_w, bar, 0, codes + it * ROWS);
             bulk_copy(at + SCALES_AT(), scales + (size_t)it * held, held, bar);
             if (zeros) bulk_copy(at + ZEROS_AT(), zeros + (size_t)it * (held / 2), held / 2, bar);
         };
@@ -168,13 +166,12 @@ __global__ void __launch_bounds__(THREADS, 1) product_many_kernel(const __grid_c
             ok = wait(full0 + 8 * s, turn, lost, 2) && wait(made0 + 8 * o, o_turn, lost, 3);
             if (!ok) break;
             tc5::tc_fence_after();
-            const uint32_t w = tc5::smem_u32(operands + o * OPERAND), x = tc5::smem_u32(ring + (size_t)s * stage) + TOKENS_AT();
+            const uint32_t w = operands + o * OPERAND, x = tc5::smem_u32(ring + (size_t)s * stage) + TOKENS_AT();
             if (tc5::elect_one()) {
 #pragma unroll
                 for (int kk = 0; kk < STEP / 16; ++kk) {
-                    const uint64_t da = tc5::desc_k_major(w + (kk / 4) * (OPERAND / 2)) + (uint64_t)((kk % 4) * 2);
                     const uint64_t db = tc5::desc_k_major(x + (kk / 4) * (a.tokens * 128)) + (uint64_t)((kk % 4) * 2);
-                    tc5::umma(tmem, da, db, idesc, (it | kk) != 0 ? 1u : 0u);
+                    tc5::umma_ts(tmem, w + kk * 8, db, idesc, (it | kk) != 0 ? 1u : 0u);
                 }
                 tc5::umma_commit(empty0 + 8 * s);
                 tc5::umma_commit(freed0 + 8 * o);
@@ -185,57 +182,57 @@ __global__ void __launch_bounds__(THREADS, 1) product_many_kernel(const __grid_c
             if (++o == a.operands) o = 0, o_turn ^= 1;
         }
     } else {
-        // A thread a row's piece of sixteen bytes, twice a step: a word of each 32 columns.  Of eight neighbouring threads four have a row and four the row four further, whose
-        // swizzled pieces lie in the other banks.
-        const int group = (warp - 2) / WORKERS, worker = (threadIdx.x - 64) % (32 * WORKERS), t = worker & 3, row0 = (worker >> 5 << 3) | (worker >> 3 & 3) | (worker & 4);
+        // A thread a row of the step: pieces of sixteen bytes, which the copy has swizzled so that eight threads' lie in all banks, with a word of each 32 columns.
+        const int group = (warp - 2) / WORKERS, row = (warp & 3) * 32 + lane;
         const __nv_bfloat162 up = __halves2bfloat162(__ushort_as_bfloat16(0x7F00), __ushort_as_bfloat16(0x7F00));                 // 2^127
-        int s = group, turn = 0, o = group, o_turn = 1;  // (there are two stages at least, and an even number of operands)
+        int s = group, turn = 0, o = group, o_turn = 1;  // (there are two stages and two operands at least)
         for (int it = group; it < steps; it += GROUPS) {
             if (!wait(full0 + 8 * s, turn, lost, 4)) break;
             const unsigned char* in = ring + (size_t)s * stage;
-            uint4 raw[2];
-            uint32_t scale[2][PER_STEP], zero[2][PER_STEP];
+            uint4 raw[4];
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int row = half * 64 + row0;
-                raw[half] = *reinterpret_cast<const uint4*>(in + row * 64 + t * 16);
+            for (int t = 0; t < 4; ++t) raw[t] = *reinterpret_cast<const uint4*>(in + row * 64 + ((t ^ (row >> 1 & 3)) << 4));
+            uint32_t scale[PER_STEP], zero[PER_STEP];
 #pragma unroll
-                for (int i = 0; i < PER_STEP; ++i) {
-                    scale[half][i] = *reinterpret_cast<const unsigned short*>(in + SCALES_AT() + (i * 128 + row) * 2);
-                    zero[half][i] = a.zeros ? in[ZEROS_AT() + i * 128 + row] : 8u;
-                }
+            for (int i = 0; i < PER_STEP; ++i) {
+                scale[i] = *reinterpret_cast<const unsigned short*>(in + SCALES_AT() + (i * 128 + row) * 2);
+                zero[i] = a.zeros ? in[ZEROS_AT() + i * 128 + row] : 8u;
             }
             if (it >= a.operands && !wait(freed0 + 8 * o, o_turn, lost, 5)) break;
-            unsigned char* to = operands + o * OPERAND;
+            tc5::tc_fence_after();
+            const uint32_t to = operands + o * OPERAND + ((uint32_t)((warp & 3) * 32) << 16);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-                const int row = half * 64 + row0;
-                const uint32_t words[4] = {raw[half].x, raw[half].y, raw[half].z, raw[half].w};
+                uint32_t numbers[32];                    // columns 64 half + (0..63), in pairs
 #pragma unroll
-                for (int i = 0; i < PER_STEP; ++i) {
+                for (int v = 0; v < 2; ++v) {
+                    const int w = 2 * half + v, i = w * PER_STEP / 4;
                     // (code - zero) 2^-6 in one operation, exactly; its product with 2^6 scale rounded once
-                    const __nv_bfloat162 down = __bfloat162bfloat162(__float2bfloat16_rn((__uint_as_float(0x4B000000u | zero[half][i]) - 8388608.f) * -0.015625f));
-                    float f = __uint_as_float(scale[half][i] << 16) * 64.f;
-                    if ((kt0 + it) * STEP + i * (STEP / PER_STEP) >= a.k) f = 0.f;      // (what stands behind the last column may be no number)
+                    const __nv_bfloat162 down = __bfloat162bfloat162(__float2bfloat16_rn((__uint_as_float(0x4B000000u | zero[i]) - 8388608.f) * -0.015625f));
+                    float f = __uint_as_float(scale[i] << 16) * 64.f;
+                    if ((kt0 + it) * STEP + 32 * w >= a.k) f = 0.f;      // (what stands behind the last column may be no number)
                     const __nv_bfloat162 by = __bfloat162bfloat162(__float2bfloat16_rn(f));
                     auto number = [&](uint32_t tiny) { return bits(__hmul2(__hfma2(two(tiny), up, down), by)); };
 #pragma unroll
-                    for (int v = 0; v < 4 / PER_STEP; ++v) {
-                        const int w = i * (4 / PER_STEP) + v;
-                        const uint32_t even = words[w] & 0x0F0F0F0Fu, odd = words[w] >> 4 & 0x0F0F0F0Fu;
-                        const uint4 numbers = make_uint4(number(tiny_pair<0>(even, odd)), number(tiny_pair<1>(even, odd)), number(tiny_pair<2>(even, odd)), number(tiny_pair<3>(even, odd)));
-                        const int piece = (w & 1) * 4 + t;
-                        *reinterpret_cast<uint4*>(to + (w >> 1) * (OPERAND / 2) + row * 128 + ((piece ^ (row & 7)) << 4)) = numbers;
+                    for (int t = 0; t < 4; ++t) {
+                        const uint32_t word = w == 0 ? raw[t].x : w == 1 ? raw[t].y : w == 2 ? raw[t].z : raw[t].w;
+                        const uint32_t even = word & 0x0F0F0F0Fu, odd = word >> 4 & 0x0F0F0F0Fu;
+                        numbers[16 * v + 4 * t] = number(tiny_pair<0>(even, odd));
+                        numbers[16 * v + 4 * t + 1] = number(tiny_pair<1>(even, odd));
+                        numbers[16 * v + 4 * t + 2] = number(tiny_pair<2>(even, odd));
+                        numbers[16 * v + 4 * t + 3] = number(tiny_pair<3>(even, odd));
                     }
                 }
+                tc5::tmem_st32(to + 32 * half, reinterpret_cast<const float*>(numbers));
             }
-            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            tc5::tmem_wait_st();
+            tc5::tc_fence_before();
             __syncwarp();
             if (lane == 0) tc5::mbar_arrive(made0 + 8 * o);
             s += GROUPS;
-            if (s >= a.stages) s -= a.stages, turn ^= 1;
+            while (s >= a.stages) s -= a.stages, turn ^= 1;
             o += GROUPS;
-            if (o >= a.operands) o -= a.operands, o_turn ^= 1;
+            while (o >= a.operands) o -= a.operands, o_turn ^= 1;
         }
         // the accumulator to shared memory, where the ring was: [tokens][128]
         const bool ok = wait(ready, 0, lost, 6);
@@ -310,17 +307,19 @@ LILY_API int lily_linear4_many(const void* x, const void* codes, const void* sca
                  group);
     LILY_REQUIRE(m > 0 && ((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales | (uintptr_t)zeros) % 16 == 0, "linear4: tensors on boundaries of sixteen bytes");
     const int token_tiles = (m + MOST_TOKENS - 1) / MOST_TOKENS, row_tiles = (n + ROWS - 1) / ROWS;
-    Args a{(const uint8_t*)codes, (const uint8_t*)scales, (const uint8_t*)zeros, bias, bias_f32, out, out_f32, m, n, k, (k + STEP - 1) / STEP};
+    Args a{(const uint8_t*)scales, (const uint8_t*)zeros, bias, bias_f32, out, out_f32, m, n, k, (k + STEP - 1) / STEP};
     a.tokens = ((m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
-    // columns shared out while there are SMs without a row tile, no fewer than two steps a block
+    // columns shared out while there is room for more blocks (two a SM up to 128 tokens), no fewer than two steps a block
     a.splits = 1;
-    while (a.splits < MOST_SPLITS && 2ll * a.splits * row_tiles * token_tiles <= sm_count() && a.tiles >= 4 * a.splits) a.splits *= 2;
-    // four operands in shared memory, so that nobody waits for a product, where that leaves three stages
-    const int stage = stage_bytes(a.tokens), room = 224 * 1024;
-    a.operands = room - OPERANDS * OPERAND >= 3 * stage ? OPERANDS : 2;
-    a.stages = min(min(6, (room - a.operands * OPERAND) / stage), max(2, (a.tiles + a.splits - 1) / a.splits));
-    const int bytes = max(a.operands * OPERAND + a.stages * stage, a.tokens * ROWS * 4) + 1024;
-    LILY_REQUIRE(a.stages >= 2 && row_tiles <= INT32_MAX / 8 && token_tiles <= 65535, "linear4: %d tokens, %d rows", m, n);
+    while (a.splits < MOST_SPLITS && 2ll * a.splits * row_tiles * token_tiles <= (a.tokens <= 128 ? 2 : 1) * sm_count() && a.tiles >= 4 * a.splits) a.splits *= 2;
+    // tensor memory: half of it, so that two blocks share an SM, where that holds two operands at least beside the accumulator
+    const int accumulator = (a.tokens + 31) / 32 * 32;
+    a.columns = accumulator + 2 * OPERAND <= 256 ? 256 : 512;
+    a.operands = min(OPERANDS, (a.columns - accumulator) / OPERAND);
+    const int stage = stage_bytes(a.tokens), room = (a.columns == 256 ? 112 : 224) * 1024;
+    a.stages = min(min(6, room / stage), max(2, (a.tiles + a.splits - 1) / a.splits));
+    const int bytes = max(a.stages * stage, a.tokens * ROWS * 4) + 1024;
+    LILY_REQUIRE(a.stages >= 2 && (long long)row_tiles * a.tiles <= INT32_MAX / ROWS && token_tiles <= 65535, "linear4: %d tokens, a matrix [%d, %d]", m, n, k);
     tc5::EncodeTiled encode = tc5::encoder();
     LILY_REQUIRE(encode != nullptr, "linear4: no encoder of tensor maps");
     CUtensorMap map;
@@ -328,7 +327,12 @@ LILY_API int lily_linear4_many(const void* x, const void* codes, const void* sca
     const cuuint32_t box[2] = {64, (cuuint32_t)a.tokens}, steps[2] = {1, 1};
     const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    LILY_REQUIRE(rc == CUDA_SUCCESS, "linear4: tensor map: error %d", (int)rc);
+    CUtensorMap map_w;
+    const cuuint64_t w_dims[2] = {64, (cuuint64_t)row_tiles * a.tiles * ROWS}, w_strides[1] = {64};
+    const cuuint32_t w_box[2] = {64, ROWS};
+    const CUresult w_rc = encode(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), w_dims, w_strides, w_box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    LILY_REQUIRE(rc == CUDA_SUCCESS && w_rc == CUDA_SUCCESS, "linear4: tensor map: errors %d, %d", (int)rc, (int)w_rc);
     auto kernel = group == 128 ? product_many_kernel<1> : group == 64 ? product_many_kernel<2> : product_many_kernel<4>;
     LILY_REQUIRE(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess, "linear4: cannot get %d bytes of shared memory", bytes);
     cudaLaunchConfig_t cfg = {};
@@ -344,7 +348,7 @@ LILY_API int lily_linear4_many(const void* x, const void* codes, const void* sca
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    cudaLaunchKernelEx(&cfg, kernel, map, a);
+    cudaLaunchKernelEx(&cfg, kernel, map, map_w, a);
     LILY_CHECK_LAUNCH("linear4");
     return 0;
 }
