@@ -27,21 +27,26 @@ __device__ __forceinline__ uint4 weights16(const void* p) {          // weights 
 }
 __device__ __forceinline__ uint32_t minus(uint32_t a, uint32_t b) { return bits(__hsub2(two(a), two(b))); }
 
-constexpr int FEW_WARPS = 8, FEW_ROWS = 32;
+constexpr int FEW_WARPS = 8;
 
-// Up to 8 NT tokens: a block 32 rows, its warps an eighth of the columns' tiles each; weights on the rows of the products, tokens on their eight columns.  The first
-// weights are on their way before the kernel ahead has ended.  grid (rows / 32)
-template <int NT, int PER_GROUP>                                      // words of a lane (32 columns each) that share a scale: 1, 2 or 4
-__global__ void __launch_bounds__(32 * FEW_WARPS, 2) product_few_kernel(const ProductArgs a) {
-    constexpr int MT = FEW_ROWS / 16, GROUPS = 4 / PER_GROUP;
-    __shared__ float sum_s[FEW_WARPS][8 * NT][FEW_ROWS + 1];
+// Up to 8 NT tokens: blocks walk tiles of 16 MT rows, their warps an eighth of the columns' tiles each; weights on the rows of the products, tokens on their eight columns.  A warp's weights
+// are one stream, from one tile of rows to the next, which it asks for DEPTH steps ahead (the first ones before the kernel ahead has ended); tokens stay in the L1.
+template <int NT, int PER_GROUP, int MT>                              // PER_GROUP: words of a lane (32 columns each) that share a scale, 1, 2 or 4
+__global__ void __launch_bounds__(32 * FEW_WARPS, 2) product_few_kernel(const ProductArgs a, int row_tiles) {
+    constexpr int GROUPS = 4 / PER_GROUP, ROWS = 16 * MT, DEPTH = GROUPS == 1 ? 3 : 2;
+    __shared__ float sum_s[2][FEW_WARPS][8 * NT][ROWS + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int row0 = blockIdx.x * FEW_ROWS, tile_row = row0 / 128, in_tile = row0 % 128;
-    const uint8_t* codes = a.codes + ((size_t)tile_row * a.tiles * 128 + in_tile) * 64 + lane * 16;        // (a lane's sixteen bytes: row g, piece t)
-    const size_t groups = (size_t)a.tiles * GROUPS, held0 = (size_t)tile_row * groups * 128 + in_tile + g;
+    const size_t groups = (size_t)a.tiles * GROUPS;
+    const int steps = (a.tiles - warp + FEW_WARPS - 1) / FEW_WARPS;   // of this warp and a tile of rows
     struct Step { uint4 w[MT][2]; unsigned short s[MT][2][GROUPS]; unsigned char z[MT][2][GROUPS]; };
-    auto load = [&](int kt, Step& c) {
-        const uint8_t* p = codes + (size_t)kt * 128 * 64;
+    // what to ask for next
+    int ask_tile = blockIdx.x, ask_kt = warp;
+    auto ask = [&](Step& c) {
+        if (steps == 0 || ask_tile >= row_tiles) return;
+        const int row0 = ask_tile * ROWS, in_tile = row0 % 128;
+        const size_t tile_row = row0 / 128;
+        const uint8_t* p = a.codes + ((tile_row * a.tiles + ask_kt) * 128 + in_tile) * 64 + lane * 16;        // (a lane's sixteen bytes: row g, piece t)
+        const size_t held0 = (tile_row * groups + (size_t)ask_kt * GROUPS) * 128 + in_tile + g;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -49,26 +54,31 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) product_few_kernel(const Pr
                 c.w[mt][e] = weights16(p + (mt * 16 + e * 8) * 64);
 #pragma unroll
                 for (int i = 0; i < GROUPS; ++i) {
-                    const size_t at = held0 + ((size_t)kt * GROUPS + i) * 128 + mt * 16 + e * 8;
-                    const bool in = kt * 128 + i * (128 / GROUPS) < a.k;               // (what stands behind the last column may be no number)
+                    const size_t at = held0 + i * 128 + mt * 16 + e * 8;
+                    const bool in = ask_kt * 128 + i * (128 / GROUPS) < a.k;             // (what stands behind the last column may be no number)
                     c.s[mt][e][i] = in ? __ldg(reinterpret_cast<const unsigned short*>(a.scales) + at) : 0;
                     c.z[mt][e][i] = a.zeros ? __ldg(a.zeros + at) : 8;
                 }
             }
+        ask_kt += FEW_WARPS;
+        if (ask_kt >= a.tiles) ask_kt = warp, ask_tile += gridDim.x;
     };
-    Step cur, next;
-    if (warp < a.tiles) load(warp, cur);
+    Step ring[DEPTH];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) ask(ring[d]);
     pdl_launch_dependents();
     pdl_wait();
     float total[MT][NT][4];
+    auto clear = [&]() {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) total[mt][nt][e] = 0.f;
-    for (int kt = warp; kt < a.tiles; kt += FEW_WARPS) {
-        if (kt + FEW_WARPS < a.tiles) load(kt + FEW_WARPS, next);
+                for (int e = 0; e < 4; ++e) total[mt][nt][e] = 0.f;
+    };
+    clear();
+    auto work = [&](const Step& cur, int kt) {
         uint4 xv[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -81,17 +91,16 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) product_few_kernel(const Pr
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) {
             float sum[MT][NT][4];
+            uint32_t zero[MT][2];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) sum[mt][nt][e] = 0.f;
-            uint32_t zero[MT][2];
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) zero[mt][e] = (0x4300u | cur.z[mt][e][i]) * 0x10001u;
+            }
 #pragma unroll
             for (int v = 0; v < PER_GROUP; ++v) {
                 const int w = i * PER_GROUP + v;
@@ -127,25 +136,48 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) product_few_kernel(const Pr
                 }
             }
         }
-        cur = next;
+    };
+    int tile = blockIdx.x, buffer = 0;
+    // the warps' sums of a tile of rows together (one barrier a tile: sums of the next one go to the other buffer)
+    auto finish = [&]() {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum_s[buffer][warp][nt * 8 + 2 * t + (e & 1)][mt * 16 + g + (e >> 1) * 8] = total[mt][nt][e];
+        __syncthreads();
+        for (int i = threadIdx.x; i < 8 * NT * ROWS; i += 32 * FEW_WARPS) {
+            const int token = i / ROWS, r = i % ROWS, row = tile * ROWS + r;
+            if (token >= a.m || row >= a.n) continue;
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < FEW_WARPS; ++w) v += sum_s[buffer][w][token][r];
+            if (a.bias) v += a.bias_f32 ? ((const float*)a.bias)[row] : __bfloat162float(((const __nv_bfloat16*)a.bias)[row]);
+            const size_t at = (size_t)token * a.n + row;
+            if (a.out_f32) ((float*)a.out)[at] = v;
+            else ((__nv_bfloat16*)a.out)[at] = __float2bfloat16_rn(v);
+        }
+        buffer ^= 1;
+        tile += gridDim.x;
+        clear();
+    };
+    if (steps == 0) {                                                 // (fewer tiles of columns than warps)
+        while (tile < row_tiles) finish();
+        return;
     }
+    for (int kt = warp; tile < row_tiles;) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum_s[warp][nt * 8 + 2 * t + (e & 1)][mt * 16 + g + (e >> 1) * 8] = total[mt][nt][e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 8 * NT * FEW_ROWS; i += 32 * FEW_WARPS) {
-        const int token = i / FEW_ROWS, r = i % FEW_ROWS, row = row0 + r;
-        if (token >= a.m || row >= a.n) continue;
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < FEW_WARPS; ++w) v += sum_s[w][token][r];
-        if (a.bias) v += a.bias_f32 ? ((const float*)a.bias)[row] : __bfloat162float(((const __nv_bfloat16*)a.bias)[row]);
-        const size_t at = (size_t)token * a.n + row;
-        if (a.out_f32) ((float*)a.out)[at] = v;
-        else ((__nv_bfloat16*)a.out)[at] = __float2bfloat16_rn(v);
+        for (int d = 0; d < DEPTH; ++d) {
+            if (tile >= row_tiles) break;
+            work(ring[d], kt);
+            ask(ring[d]);
+            kt += FEW_WARPS;
+            if (kt >= a.tiles) {
+                kt = warp;
+                finish();
+            }
+        }
     }
 }
 
@@ -260,15 +292,23 @@ LILY_API int lily_linear4(const void* x, int dtype, const void* codes, const voi
         else if (m <= 4) launch_pdl(four::product_f32_kernel<4>, grid, block, 0, stream, a, shift);
         else launch_pdl(four::product_f32_kernel<four::F32_TOKENS>, grid, block, 0, stream, a, shift);
     } else {
-        const dim3 grid((n + four::FEW_ROWS - 1) / four::FEW_ROWS), block(32 * four::FEW_WARPS);
-#define FEW(NT)                                                                                          \
-    do {                                                                                                 \
-        if (group == 128) launch_pdl(four::product_few_kernel<NT, 4>, grid, block, 0, stream, a);        \
-        else if (group == 64) launch_pdl(four::product_few_kernel<NT, 2>, grid, block, 0, stream, a);    \
-        else launch_pdl(four::product_few_kernel<NT, 1>, grid, block, 0, stream, a);                     \
+        // 32 rows a block and turn, 16 where that leaves SMs without
+        const int mt = (n + 31) / 32 <= sm_count() ? 1 : 2, row_tiles = (n + 16 * mt - 1) / (16 * mt);
+        const dim3 grid(min(row_tiles, 2 * sm_count())), block(32 * four::FEW_WARPS);
+#define FEW_OF(NT, MT)                                                                                               \
+    do {                                                                                                             \
+        if (group == 128) launch_pdl(four::product_few_kernel<NT, 4, MT>, grid, block, 0, stream, a, row_tiles);     \
+        else if (group == 64) launch_pdl(four::product_few_kernel<NT, 2, MT>, grid, block, 0, stream, a, row_tiles); \
+        else launch_pdl(four::product_few_kernel<NT, 1, MT>, grid, block, 0, stream, a, row_tiles);                  \
+    } while (0)
+#define FEW(NT)                   \
+    do {                          \
+        if (mt == 1) FEW_OF(NT, 1); \
+        else FEW_OF(NT, 2);       \
     } while (0)
         if (m <= 8) FEW(1);
         else FEW(2);
+#undef FEW_OF
 #undef FEW
     }
     LILY_CHECK_LAUNCH("linear4");

@@ -1401,7 +1401,11 @@ def weights4(w: Weight4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     return out
 
 
-LINEAR4_MANY = 512            # tokens up to which a product makes numbers of its codes on the way
+def linear4_on_the_way(m: int, n: int, k: int) -> bool:
+    """Whether a bfloat16 product of ``m`` tokens makes numbers of its codes on the way (tcgen05, a tile of 256 tokens at a time) rather than bringing the whole matrix to numbers in memory for
+    ``linear``, which pays for many tokens.  Measured, us, on the way / numbers and ``linear``: 4,096 x 12,288 16 / 53 with 64 tokens, 31 / 58 with 256, 58 / 72 with 512, 97 / 87 with 768;
+    24,576 x 4,096 83 / 109 with 256, 132 / 127 with 512; 4,096 x 4,096 19 / 21 with 256, 26 / 23 with 384; 2,048 x 2,048 7.6 / 10 with 64, 10.3 / 10 with 128, 22 / 10 with 256."""
+    return m <= 128 or (m <= 256 and n * k >= 1 << 24) or (m <= 512 and n * k >= 3 << 24)
 
 
 def linear4_status() -> int:
@@ -1413,7 +1417,7 @@ def linear4(x: torch.Tensor, w: Weight4, bias: Optional[torch.Tensor] = None, ou
     """``x [M, K] . W^T (+ bias)`` [M, N] for a matrix held in four bits, in the dtype of ``x`` (or float32: ``out_dtype``)."""
     if out_dtype not in (None, x.dtype, torch.float32):
         raise KernelError(f"linear4: the result is {x.dtype} or float32, not {out_dtype}")
-    if x.dim() == 2 and x.shape[0] > (LINEAR4_MANY if x.dtype == torch.bfloat16 else 8):
+    if x.dim() == 2 and x.shape[0] > 8 and (x.dtype != torch.bfloat16 or not linear4_on_the_way(x.shape[0], w.n, w.k)):
         return linear(x, weights4(w, x.dtype), bias, out_dtype)
     out = (_module or _faces()).linear4(x, *w, bias, out_dtype == torch.float32, 17)
     launches["count"] += 1
