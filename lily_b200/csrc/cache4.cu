@@ -19,7 +19,7 @@ struct WriteArgs {
     int ld;
     const void* q_gain;
     const void* k_gain;
-    double eps;
+    double eps, by_d;                // 1 / d
     const float* cos_t;              // [table_rows, rd / 2]
     const float* sin_t;
     int table_rows;
@@ -68,39 +68,39 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) write_kernel(const WriteArgs
     float y[8];
     load8((const T*)a.qkv + (size_t)n * a.ld + (size_t)head * a.d + f, y);
     const W* gain = kind == 2 ? nullptr : (const W*)(kind ? a.k_gain : a.q_gain);
-    const int pos = a.positions[n], req = kind ? a.token_req[n] : 0;
-    double squares = 0.0;
+    const int pos = a.positions[n], req = kind ? a.token_req[n] : 0, half = a.rd / 2;
+    const bool known = pos >= 0 && pos < a.table_rows, turned = kind != 2 && f < a.rd;
+    const float *ct = a.cos_t + (size_t)(known ? pos : 0) * half, *st = a.sin_t + (size_t)(known ? pos : 0) * half;
+    float c[8], sn[8], g[8];                             // asked for ahead of the sums
+    if (WHOLE_PIECES && turned) {
+        load8(ct + (f < half ? f : f - half), c);
+        load8(st + (f < half ? f : f - half), sn);
+    }
+    if (gain) load8(gain + f, g);
+    if (__any_sync(0xffffffffu, gain != nullptr)) {
+        double squares = 0.0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) squares = fma((double)y[i], (double)y[i], squares);
-    if (l >= words) squares = 0.0;
-    if (words == 24)                                     // (a head over 24 of 32 lanes; the others bring nothing)
-        for (int o = 16; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
-    else
-        for (int o = words >> 1; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
-    if (gain) {
-        const float r = (float)(1.0 / sqrt(squares / (double)a.d + a.eps));
-        float g[8];
-        load8(gain + f, g);
+        for (int i = 0; i < 8; ++i) squares = fma((double)y[i], (double)y[i], squares);
+        if (l >= words) squares = 0.0;
+        // (a head of 192 features over 24 of 32 lanes: the others bring nothing)
+        for (int o = words == 24 ? 16 : words >> 1; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+        if (gain) {
+            const float r = (float)rsqrt(fma(squares, a.by_d, a.eps));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(__fmul_rn(y[i], r), g[i]);
+            for (int i = 0; i < 8; ++i) y[i] = __fmul_rn(__fmul_rn(y[i], r), g[i]);
+        }
     }
     float* row = turn_s[warp] + mine * a.d;
     if (l < words) store8(row + f, y);
     __syncwarp();
-    const int half = a.rd / 2;
-    if (kind != 2 && f < a.rd) {
-        const bool known = pos >= 0 && pos < a.table_rows;
+    if (turned) {
         const float nan = __int_as_float(0x7fffffff);
-        const float *ct = a.cos_t + (size_t)(known ? pos : 0) * half, *st = a.sin_t + (size_t)(known ? pos : 0) * half;
         if (WHOLE_PIECES) {                              // half a multiple of eight: a thread's features are of one half
-            const int j = f < half ? f : f - half;
-            float c[8], s[8], other[8];
-            load8(ct + j, c);
-            load8(st + j, s);
-            load8(row + (f < half ? f + half : j), other);
+            float other[8];
+            load8(row + (f < half ? f + half : f - half), other);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float first = __fmul_rn(y[i], c[i]), second = __fmul_rn(other[i], s[i]);
+                const float first = __fmul_rn(y[i], c[i]), second = __fmul_rn(other[i], sn[i]);
                 y[i] = !known ? nan : f < half ? __fsub_rn(first, second) : __fadd_rn(first, second);
             }
         } else {
@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) write_kernel(const WriteArgs
         }
     }
     if (kind == 0 && in) store8((T*)a.q_out + ((size_t)n * a.nq + head) * a.d + f, y);
+    if (__all_sync(0xffffffffu, kind == 0)) return;
     // eight neighbouring lanes hold a group of 64 features
     float most_v = y[0], least = y[0];
     bool fine = true;
@@ -157,14 +158,15 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) write_kernel(const WriteArgs
 
 // Pages as numbers, lowest + step code in one rounding: of every page that a block table names to [requests, width, 2, nkv, page_size, d] (``compact`` false), or of the pages
 // that portions of prompts see, one request's behind the other's, [pages, 2, nkv, page_size, d], with a block table of them and zeros behind a request's last place.
-// A thread a word of eight codes, bound by the numbers it writes.  grid (pages, requests, kv heads x 2)
-template <typename T>
-__global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__ kv, int pages, const int* __restrict__ block_table, int width, T* __restrict__ out, int nkv,
-                                                     int d, int page_size, const int* __restrict__ cu, const int* __restrict__ prefix, int* __restrict__ table_out,
-                                                     int table_width, int most_pages) {
+// Eight threads a place and kind, each with the words that lie side by side, one a group.  grid (pages, requests, kv heads x 2)
+template <typename T, int G>
+__global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__ kv, int pages, const int* __restrict__ block_table, int width, T* __restrict__ out, int nkv, int page_size,
+                                                     const int* __restrict__ cu, const int* __restrict__ prefix, int* __restrict__ table_out, int table_width, int most_pages) {
+    constexpr int D = G * GROUP;
     __shared__ int sum_s[8];
     pdl_enter_small();
-    const int r = blockIdx.y, at = blockIdx.x, head = blockIdx.z >> 1, value = blockIdx.z & 1, words = d / 8, groups = d / GROUP;
+    const int r = blockIdx.y, at = blockIdx.x, head = blockIdx.z >> 1, value = blockIdx.z & 1;
+    int page = at < width ? block_table[(size_t)r * width + at] : 0;
     size_t to = (size_t)r * width + at;
     int places = page_size;
     if (cu) {
@@ -174,29 +176,38 @@ __global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__
         if (at >= (total + page_size - 1) / page_size) return;
         places = min(page_size, total - at * page_size);
         int before = 0;
-        for (int i = threadIdx.x; i < r; i += 256) before += (places_of(i) + page_size - 1) / page_size;
-        for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-        if ((threadIdx.x & 31) == 0) sum_s[threadIdx.x >> 5] = before;
-        __syncthreads();
-        before = 0;
-        for (int w = 0; w < 8; ++w) before += sum_s[w];
+        if (r > 0) {
+            for (int i = threadIdx.x; i < r; i += 256) before += (places_of(i) + page_size - 1) / page_size;
+            before = __reduce_add_sync(0xffffffffu, before);
+            if ((threadIdx.x & 31) == 0) sum_s[threadIdx.x >> 5] = before;
+            __syncthreads();
+            before = 0;
+            for (int w = 0; w < 8; ++w) before += sum_s[w];
+        }
         to = (size_t)before + at;
         if (to >= (size_t)most_pages || at >= table_width) return;
         if (threadIdx.x == 0 && blockIdx.z == 0) table_out[(size_t)r * table_width + at] = (int)to;
     }
-    int page = at < width ? block_table[(size_t)r * width + at] : 0;
     if ((unsigned)page >= (unsigned)pages) page = 0;
-    const uint8_t* rows = kv + (((size_t)page * nkv + head) * 2 + value) * ((size_t)page_size * row_bytes(d));
-    const uint32_t* held = reinterpret_cast<const uint32_t*>(rows + (size_t)page_size * (d / 2));
-    T* dst = out + ((to * 2 + value) * nkv + head) * ((size_t)page_size * d);
-    for (int i = threadIdx.x; i < page_size * words; i += 256) {
-        const int slot = i / words, l = i - slot * words;
-        const uint32_t w = reinterpret_cast<const uint32_t*>(rows + (size_t)slot * (d / 2))[value ? value_word(l, groups) : key_word(l, groups)];
-        const uint32_t h = held[slot * groups + (l >> 3)];
-        float v[8];
+    const uint8_t* rows = kv + (((size_t)page * nkv + head) * 2 + value) * ((size_t)page_size * row_bytes(D));
+    const uint32_t *words = reinterpret_cast<const uint32_t*>(rows), *held = reinterpret_cast<const uint32_t*>(rows + (size_t)page_size * (D / 2));
+    T* dst = out + ((to * 2 + value) * nkv + head) * ((size_t)page_size * D);
+    const int i8 = threadIdx.x & 7;
+#pragma unroll 2
+    for (int slot = threadIdx.x >> 3; slot < page_size; slot += 32) {
+        uint32_t w[G], h[G];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = slot < places ? fmaf((float)(w >> (4 * e) & 15u), low(h), high(h)) : 0.f;
-        store8(dst + (size_t)slot * d + l * 8, v);
+        for (int e = 0; e < G; ++e) w[e] = words[(size_t)slot * (D / 8) + i8 * G + e], h[e] = held[slot * G + e];
+#pragma unroll
+        for (int e = 0; e < G; ++e) {
+            const int in = (i8 & 1) * G + e;              // a key's words of lane column i8 / 2: (j, h) one behind the other
+            const int l = value ? 8 * e + i8 : 8 * (in >> 1) + 4 * (in & 1) + (i8 >> 1), j = l >> 3;
+            const uint32_t of = G == 1 ? h[0] : G == 2 ? (j ? h[1] : h[0]) : G == 3 ? (j == 0 ? h[0] : j == 1 ? h[1] : h[G - 1]) : (j < 2 ? (j ? h[1] : h[0]) : (j == 2 ? h[2 % G] : h[G - 1]));
+            float v[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[c] = slot < places ? fmaf((float)(w[e] >> (4 * c) & 15u), low(of), high(of)) : 0.f;
+            store8(dst + (size_t)slot * D + l * 8, v);
+        }
     }
 }
 
@@ -224,7 +235,7 @@ LILY_API int lily_qk_norm_rope_write4(const void* qkv, int dtype, int ld, const 
     const bool pieces = rd % 16 == 0;
     for (int t0 = 0; t0 < tokens; t0 += 65535) {
         const int n = min(65535, tokens - t0), item = dtype == kBF16 ? 2 : 4;
-        const four::WriteArgs a{(const char*)qkv + (size_t)t0 * ld * item, ld, q_gain, k_gain, eps, cos_t, sin_t, table_rows, positions + t0, token_req + t0, block_table, requests, bt_stride,
+        const four::WriteArgs a{(const char*)qkv + (size_t)t0 * ld * item, ld, q_gain, k_gain, eps, 1.0 / d, cos_t, sin_t, table_rows, positions + t0, token_req + t0, block_table, requests, bt_stride,
                                 (uint8_t*)kv, pages, (char*)q_out + (size_t)t0 * nq * d * item, nq, nkv, d, rd, page_size, n};
         const dim3 grid((nq + 2 * nkv + per_block - 1) / per_block, n);
 #define LAUNCH(T, W)                                                                                                              \
@@ -251,11 +262,19 @@ LILY_API int lily_cache4_values(const void* kv, int pages, const int* block_tabl
     LILY_REQUIRE(((uintptr_t)kv | (uintptr_t)out) % 16 == 0, "cache4_values: tensors on boundaries of sixteen bytes");
     const dim3 grid(cu ? table_width : width, requests, 2 * nkv);
     if (grid.x == 0) return 0;
-    if (dtype == kF32)
-        launch_pdl(four::values_kernel<float>, grid, dim3(256), 0, stream, (const uint8_t*)kv, pages, block_table, width, (float*)out, nkv, d, page_size, cu, prefix, table_out, table_width, most_pages);
-    else
-        launch_pdl(four::values_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, (const uint8_t*)kv, pages, block_table, width, (__nv_bfloat16*)out, nkv, d, page_size, cu, prefix, table_out,
-                   table_width, most_pages);
+#define VALUES(T, G) \
+    launch_pdl(four::values_kernel<T, G>, grid, dim3(256), 0, stream, (const uint8_t*)kv, pages, block_table, width, (T*)out, nkv, page_size, cu, prefix, table_out, table_width, most_pages)
+#define VALUES_OF(T)                 \
+    do {                             \
+        if (d == 64) VALUES(T, 1);   \
+        else if (d == 128) VALUES(T, 2); \
+        else if (d == 192) VALUES(T, 3); \
+        else VALUES(T, 4);           \
+    } while (0)
+    if (dtype == kF32) VALUES_OF(float);
+    else VALUES_OF(__nv_bfloat16);
+#undef VALUES_OF
+#undef VALUES
     LILY_CHECK_LAUNCH("cache4_values");
     return 0;
 }

@@ -191,24 +191,37 @@ __global__ void __launch_bounds__(32 * F32_WARPS) product_f32_kernel(const Produ
     const int row0 = blockIdx.x * 8, tile_row = row0 / 128;
     const uint8_t* codes = a.codes + ((size_t)tile_row * a.tiles * 128 + row0 % 128) * 64 + lane * 16;
     const size_t held0 = (size_t)tile_row * (a.tiles * 128 >> group_shift) * 128 + row0 % 128 + g;
-    uint4 v = make_uint4(0, 0, 0, 0), next = v;
-    if (warp < a.tiles) v = weights16(codes + (size_t)warp * 128 * 64);
+    struct Step { uint4 v; unsigned short s[4]; unsigned char z[4]; };
+    auto ask = [&](int kt, Step& c) {
+        if (kt >= a.tiles) return;
+        c.v = weights16(codes + (size_t)kt * 128 * 64);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int col = kt * 128 + 32 * w;
+            const size_t at = held0 + (size_t)(col >> group_shift) * 128;
+            c.s[w] = col < a.k ? __ldg(reinterpret_cast<const unsigned short*>(a.scales) + at) : 0;
+            c.z[w] = a.zeros && col < a.k ? __ldg(a.zeros + at) : 8;
+        }
+    };
+    constexpr int DEPTH = 3;
+    Step ring[DEPTH];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) ask(warp + d * F32_WARPS, ring[d]);
     pdl_launch_dependents();
     pdl_wait();
     float total[TOKENS];
 #pragma unroll
     for (int i = 0; i < TOKENS; ++i) total[i] = 0.f;
-    for (int kt = warp; kt < a.tiles; kt += F32_WARPS, v = next) {
-        if (kt + F32_WARPS < a.tiles) next = weights16(codes + (size_t)(kt + F32_WARPS) * 128 * 64);
-        const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+    for (int kt0 = warp; kt0 < a.tiles; kt0 += DEPTH * F32_WARPS) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+        const int kt = kt0 + d * F32_WARPS;
+        if (kt >= a.tiles) break;
+        const uint32_t words[4] = {ring[d].v.x, ring[d].v.y, ring[d].v.z, ring[d].v.w};
         float s[4], z[4];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const int col = kt * 128 + 32 * w;
-            const size_t at = held0 + (size_t)(col >> group_shift) * 128;
-            s[w] = col < a.k ? __bfloat162float(a.scales[at]) : 0.f;
-            z[w] = 8388608.f + (a.zeros && col < a.k ? (float)a.zeros[at] : 8.f);
-        }
+        for (int w = 0; w < 4; ++w) s[w] = __uint_as_float((uint32_t)ring[d].s[w] << 16), z[w] = __uint_as_float(0x4B000000u | ring[d].z[w]);      // (2^23 + zero point)
+        ask(kt + DEPTH * F32_WARPS, ring[d]);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const int col = kt * 128 + 32 * w + 8 * t;
@@ -224,6 +237,7 @@ __global__ void __launch_bounds__(32 * F32_WARPS) product_f32_kernel(const Produ
                 total[i] = fmaf(s[w], first + second, total[i]);
             }
         }
+    }
     }
 #pragma unroll
     for (int i = 0; i < TOKENS; ++i) {
