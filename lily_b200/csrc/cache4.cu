@@ -54,6 +54,26 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
 
 constexpr int WRITE_WARPS = 4;
 
+// Eight codes min(15, max(0, rint((y - lowest) / step))) as a word.  The quotient by the step's reciprocal is within 2 10^-6 of the rounded one (two roundings of numbers up to 15 or so), so where no
+// code is that near to the border of two it gives the same; else, and where the reciprocal is not a number, they are divided.
+__device__ __forceinline__ uint32_t codes_of(const float (&y)[8], float lowest, float step) {
+    const float by = __frcp_rn(step);
+    uint32_t word = 0;
+    bool near = !(step > 1e-30f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float t = fminf(fmaxf(__fmul_rn(__fsub_rn(y[i], lowest), by), 0.f), 15.f), whole = t + 12582912.f;      // 1.5 2^23: the sum's last bits are the nearest whole number
+        near = near || fabsf(t - (whole - 12582912.f)) > 0.49999f;
+        word |= (__float_as_uint(whole) & 15u) << (4 * i);
+    }
+    if (near) {
+        word = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) word |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(y[i], lowest), step)), 0.f), 15.f) << (4 * i);
+    }
+    return word;
+}
+
 // A thread eight features, d / 8 threads a head, 32 / (d / 8) heads a warp.  grid (blocks of a token's heads, tokens)
 template <typename T, typename W, bool WHOLE_PIECES>
 __global__ void __launch_bounds__(32 * WRITE_WARPS) write_kernel(const WriteArgs a) {
@@ -138,14 +158,7 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) write_kernel(const WriteArgs
     if (at < 0 || at >= a.bt_stride || (unsigned)req >= (unsigned)a.requests) return;
     const int page = a.block_table[(size_t)req * a.bt_stride + at];
     if ((unsigned)page >= (unsigned)a.pages) return;
-    uint32_t word = 0;
-    if (fine && step > 0.f) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(y[i], lowest), step)), 0.f), 15.f);
-            word |= (uint32_t)c << (4 * i);
-        }
-    }
+    const uint32_t word = fine && step > 0.f ? codes_of(y, lowest, step) : 0u;
     const int groups = a.d / GROUP, slot = pos - at * a.page_size;
     uint8_t* rows = a.kv + (((size_t)page * a.nkv + (head - a.nq - (kind == 2 ? a.nkv : 0))) * 2 + (kind == 2)) * ((size_t)a.page_size * row_bytes(a.d));
     reinterpret_cast<uint32_t*>(rows + (size_t)slot * (a.d / 2))[kind == 1 ? key_word(l, groups) : value_word(l, groups)] = word;
@@ -154,6 +167,97 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) write_kernel(const WriteArgs
         reinterpret_cast<uint32_t*>(rows + (size_t)a.page_size * (a.d / 2))[slot * groups + (l >> 3)] =
             bits(fine ? __halves2bfloat162(step_b, low_b) : __halves2bfloat162(nan, nan));
     }
+}
+
+// The same where all features are turned and heads are 64, 128 or 256 features: a thread a word and its partners', d / 16 threads a head, which so needs no exchange but for sums and extremes, and half as
+// much work that is not its numbers'.  grid (blocks of a token's heads, tokens)
+template <typename T, typename W, int D>
+__global__ void __launch_bounds__(32 * WRITE_WARPS) write_turned_kernel(const WriteArgs a, const int page_shift) {
+    constexpr int THREADS = D / 16, HALF = D / 2, G = D / GROUP;
+    pdl_enter_small();
+    const int n = blockIdx.y, t = threadIdx.x % THREADS, asked = blockIdx.x * (32 * WRITE_WARPS / THREADS) + threadIdx.x / THREADS, most = a.nq + 2 * a.nkv, lane = threadIdx.x & 31;
+    const bool in = asked < most;
+    const int head = min(asked, most - 1), kind = head < a.nq ? 0 : head < a.nq + a.nkv ? 1 : 2;
+    const T* src = (const T*)a.qkv + (size_t)n * a.ld + (size_t)head * D + t * 8;
+    float x[8], y[8], c[8], s[8];
+    load8(src, x);
+    load8(src + HALF, y);
+    const int pos = a.positions[n], req = kind ? a.token_req[n] : 0;
+    const bool known = pos >= 0 && pos < a.table_rows;
+    if (kind != 2) {
+        load8(a.cos_t + (size_t)(known ? pos : 0) * HALF + t * 8, c);
+        load8(a.sin_t + (size_t)(known ? pos : 0) * HALF + t * 8, s);
+    }
+    const W* gain = kind == 2 ? nullptr : (const W*)(kind ? a.k_gain : a.q_gain);
+    if (__any_sync(0xffffffffu, gain != nullptr)) {
+        float gx[8], gy[8];
+        if (gain) load8(gain + t * 8, gx), load8(gain + HALF + t * 8, gy);
+        double squares = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) squares = fma((double)y[i], (double)y[i], fma((double)x[i], (double)x[i], squares));
+#pragma unroll
+        for (int o = THREADS / 2; o > 0; o >>= 1) squares += __shfl_xor_sync(0xffffffffu, squares, o);
+        if (gain) {
+            const float r = (float)rsqrt(fma(squares, 1.0 / D, a.eps));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], r), gx[i]), y[i] = __fmul_rn(__fmul_rn(y[i], r), gy[i]);
+        }
+    }
+    if (kind != 2) {
+        const float nan = __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float was = x[i];
+            x[i] = known ? __fsub_rn(__fmul_rn(was, c[i]), __fmul_rn(y[i], s[i])) : nan;
+            y[i] = known ? __fadd_rn(__fmul_rn(y[i], c[i]), __fmul_rn(was, s[i])) : nan;
+        }
+    }
+    if (kind == 0 && in) {
+        T* to = (T*)a.q_out + ((size_t)n * a.nq + head) * D + t * 8;
+        store8(to, x);
+        store8(to + HALF, y);
+    }
+    if (__all_sync(0xffffffffu, kind == 0)) return;
+    // extremes of the groups of 64 features: eight threads' words, or (64 features a head) both words of four
+    float most_x = x[0], least_x = x[0], most_y = y[0], least_y = y[0];
+    bool fine_x = true, fine_y = true;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        most_x = fmaxf(most_x, x[i]), least_x = fminf(least_x, x[i]), most_y = fmaxf(most_y, y[i]), least_y = fminf(least_y, y[i]);
+        fine_x = fine_x && isfinite(x[i]), fine_y = fine_y && isfinite(y[i]);
+    }
+    if (D == 64) {
+        most_x = most_y = fmaxf(most_x, most_y), least_x = least_y = fminf(least_x, least_y);
+        fine_x = fine_y = fine_x && fine_y;
+    }
+    constexpr int SPAN = D == 64 ? 4 : 8;
+#pragma unroll
+    for (int o = SPAN / 2; o > 0; o >>= 1) {
+        most_x = fmaxf(most_x, __shfl_xor_sync(0xffffffffu, most_x, o)), least_x = fminf(least_x, __shfl_xor_sync(0xffffffffu, least_x, o));
+        if (D != 64) most_y = fmaxf(most_y, __shfl_xor_sync(0xffffffffu, most_y, o)), least_y = fminf(least_y, __shfl_xor_sync(0xffffffffu, least_y, o));
+    }
+    if (D == 64) most_y = most_x, least_y = least_x;
+    constexpr uint32_t ALL = (1u << SPAN) - 1;
+    fine_x = (__ballot_sync(0xffffffffu, fine_x) >> (lane & ~(SPAN - 1)) & ALL) == ALL;
+    fine_y = D == 64 ? fine_x : (__ballot_sync(0xffffffffu, fine_y) >> (lane & ~(SPAN - 1)) & ALL) == ALL;
+    if (kind == 0 || !in) return;
+    const int at = pos < 0 ? -1 : page_shift >= 0 ? pos >> page_shift : pos / a.page_size;
+    if (at < 0 || at >= a.bt_stride || (unsigned)req >= (unsigned)a.requests) return;
+    const int page = a.block_table[(size_t)req * a.bt_stride + at];
+    if ((unsigned)page >= (unsigned)a.pages) return;
+    const int slot = pos - at * a.page_size;
+    uint8_t* rows = a.kv + (((size_t)page * a.nkv + (head - a.nq - (kind == 2 ? a.nkv : 0))) * 2 + (kind == 2)) * ((size_t)a.page_size * row_bytes(D));
+    uint32_t* words = reinterpret_cast<uint32_t*>(rows + (size_t)slot * (D / 2));
+    uint32_t* held = reinterpret_cast<uint32_t*>(rows + (size_t)a.page_size * (D / 2)) + slot * G;
+    auto put = [&](const float (&v)[8], int l, float most_v, float least, bool fine, bool says) {
+        const __nv_bfloat16 step_b = __float2bfloat16_rn(__fmul_rn(__fsub_rn(most_v, least), (float)(1.0 / 15.0))), low_b = __float2bfloat16_rn(least), nan = __float2bfloat16_rn(__int_as_float(0x7fffffff));
+        const float step = __bfloat162float(step_b), lowest = __bfloat162float(low_b);
+        fine = fine && isfinite(step) && isfinite(lowest);
+        words[kind == 1 ? key_word(l, G) : value_word(l, G)] = fine && step > 0.f ? codes_of(v, lowest, step) : 0u;
+        if (says) held[l >> 3] = bits(fine ? __halves2bfloat162(step_b, low_b) : __halves2bfloat162(nan, nan));
+    };
+    put(x, t, most_x, least_x, fine_x, (t & 7) == 0);
+    put(y, t + THREADS, most_y, least_y, fine_y, D != 64 && (t & 7) == 0);
 }
 
 // Pages as numbers, lowest + step code in one rounding: of every page that a block table names to [requests, width, 2, nkv, page_size, d] (``compact`` false), or of the pages
@@ -233,20 +337,28 @@ LILY_API int lily_qk_norm_rope_write4(const void* qkv, int dtype, int ld, const 
     LILY_REQUIRE(where % 16 == 0 && ld % 8 == 0, "qk_norm_rope_write4: tensors on boundaries of sixteen bytes");
     const int per_block = four::WRITE_WARPS * (32 / (d / 8));
     const bool pieces = rd % 16 == 0;
+    int shift = 0;
+    while (1 << shift < page_size) ++shift;
+    if (1 << shift != page_size) shift = -1;
     for (int t0 = 0; t0 < tokens; t0 += 65535) {
         const int n = min(65535, tokens - t0), item = dtype == kBF16 ? 2 : 4;
         const four::WriteArgs a{(const char*)qkv + (size_t)t0 * ld * item, ld, q_gain, k_gain, eps, 1.0 / d, cos_t, sin_t, table_rows, positions + t0, token_req + t0, block_table, requests, bt_stride,
                                 (uint8_t*)kv, pages, (char*)q_out + (size_t)t0 * nq * d * item, nq, nkv, d, rd, page_size, n};
-        const dim3 grid((nq + 2 * nkv + per_block - 1) / per_block, n);
+        const dim3 grid((nq + 2 * nkv + per_block - 1) / per_block, n), turned((nq + 2 * nkv + 2 * per_block - 1) / (2 * per_block), n);
+#define TURNED(T, W, D) launch_pdl(four::write_turned_kernel<T, W, D>, turned, dim3(32 * four::WRITE_WARPS), 0, stream, a, shift)
 #define LAUNCH(T, W)                                                                                                              \
     do {                                                                                                                          \
-        if (pieces) launch_pdl(four::write_kernel<T, W, true>, grid, dim3(32 * four::WRITE_WARPS), 0, stream, a);                  \
+        if (rd == d && d == 64) TURNED(T, W, 64);                                                                                  \
+        else if (rd == d && d == 128) TURNED(T, W, 128);                                                                           \
+        else if (rd == d && d == 256) TURNED(T, W, 256);                                                                           \
+        else if (pieces) launch_pdl(four::write_kernel<T, W, true>, grid, dim3(32 * four::WRITE_WARPS), 0, stream, a);                  \
         else launch_pdl(four::write_kernel<T, W, false>, grid, dim3(32 * four::WRITE_WARPS), 0, stream, a);                        \
     } while (0)
         if (dtype == kF32) LAUNCH(float, float);
         else if (gain_dtype == kBF16) LAUNCH(__nv_bfloat16, __nv_bfloat16);
         else LAUNCH(__nv_bfloat16, float);
 #undef LAUNCH
+#undef TURNED
         LILY_CHECK_LAUNCH("qk_norm_rope_write4");
     }
     return 0;
