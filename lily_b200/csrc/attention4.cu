@@ -20,9 +20,9 @@ struct DecodeArgs {
     const int* block_table;       // [requests, width]
     int width;
     const int* seq_lens;
-    float* part_o;                // [requests, nq, splits, d]
-    float* part_ml;               // [requests, nq, splits, 2]
-    int splits, nq, nkv, d, page_size, pages, longest;
+    float* part_o;                // [2 blocks, 8, d]: what blocks leave of pairs that they share
+    float* part_ml;               // [2 blocks, 8, 2]
+    int nq, nkv, d, page_size, pages, longest;
     int page_shift;               // tensor-core kernel: log2 of page_size
     int requests;
     float scale;
@@ -35,30 +35,6 @@ __device__ __forceinline__ int page_of(const DecodeArgs& a, int req, int j) {
     const int page = a.block_table[(size_t)req * a.width + j / a.page_size];
     return (unsigned)page < (unsigned)a.pages ? page : 0;
 }
-// The places of range `z` of a request: equal shares in steps of `step`.
-__device__ __forceinline__ void range_of(const DecodeArgs& a, int req, int z, int step, int& beg, int& end) {
-    const int n = places_of(a, req);
-    const int per = ((n + a.splits - 1) / a.splits + step - 1) / step * step;
-    beg = min(n, z * per);
-    end = min(n, beg + per);
-}
-
-// What a block found for its range, `heads` of them with (max in units of log2, sum, output not divided yet) in shared memory: to the scratch, or, where it is the only range,
-// divided and rounded to the output.
-template <typename T>
-__device__ __forceinline__ void leave(const DecodeArgs& a, int req, int head0, int heads, const float* m, const float* l, const float* o, int ld) {
-    for (int i = threadIdx.x; i < heads * a.d; i += blockDim.x) {
-        const int h = i / a.d, f = i - h * a.d;
-        const size_t row = (size_t)req * a.nq + head0 + h;
-        if (a.splits == 1) ((T*)a.out)[row * a.d + f] = from_float<T>(l[h] == 0.f ? 0.f : o[h * ld + f] / l[h]);
-        else {
-            const size_t at = row * a.splits + blockIdx.x;
-            a.part_o[at * a.d + f] = o[h * ld + f];
-            if (f == 0) a.part_ml[2 * at] = m[h], a.part_ml[2 * at + 1] = l[h];
-        }
-    }
-}
-
 // ---- bfloat16 on the tensor cores -------------------------------------------------------------------
 constexpr int KT = 32;                        // places a tile
 constexpr int WARPS = 4, STAGES = 2, BLOCKS = 2;      // warps a block, tiles in a warp's ring, blocks a SM
@@ -171,32 +147,20 @@ struct Cut {
     }
 };
 
-// Keys on the rows of the products (16 of them), query heads on their eight columns: S^T = K q^T, O^T = V^T P^T.  The warps of a block take the tiles of its share in turn, each through
-// a ring of its own that runs on from one pair to the next; they meet where a pair's part ends.
-template <int D>
-__global__ void __launch_bounds__(32 * WARPS, BLOCKS) decode_mma_kernel(const DecodeArgs a) {
-    using S = Tile<D>;
-    constexpr int G = S::G, LD = D + 4;
-    extern __shared__ __align__(16) unsigned char ring_s[];
-    __shared__ float m_s[WARPS][HEADS], l_s[WARPS][HEADS];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int group = a.nq / a.nkv, chunks = (group + HEADS - 1) / HEADS, pairs = a.nkv * chunks;
-    unsigned char* mine = ring_s + warp * STAGES * S::BYTES;
-    float* o_s = reinterpret_cast<float*>(ring_s + WARPS * STAGES * S::BYTES);      // [warps][heads][LD]
-    const uint32_t ring = mma16::smem_u32(mine);
-    pdl_wait();
-    pdl_launch_dependents();                                          // (the joining kernel may so read the lengths ahead of its own wait)
+// This block's share of the tiles, and where it begins.  Rows without places are zeroed on the way.
+template <typename T, int D>
+__device__ __forceinline__ void begin_share(const DecodeArgs& a, int pairs, int chunks, Place& at, int& share) {
+    const int lane = threadIdx.x & 31;
     int total = 0;
     for (int r = lane; r < a.requests; r += 32) total += tiles_of(a, r);
     total = __reduce_add_sync(0xffffffffu, total);
     const Cut cut(total * pairs, gridDim.x);
-    const int first = cut.begins(blockIdx.x), share = cut.per + ((int)blockIdx.x < cut.more);
-    // a request without places has zeros
+    const int first = cut.begins(blockIdx.x);
+    share = cut.per + ((int)blockIdx.x < cut.more);
     for (int r = blockIdx.x; r < a.requests; r += gridDim.x)
         if (places_of(a, r) == 0)
-            for (int i = threadIdx.x; i < a.nq * D / 8; i += 32 * WARPS) reinterpret_cast<uint4*>((__nv_bfloat16*)a.out + (size_t)r * a.nq * D)[i] = make_uint4(0, 0, 0, 0);
+            for (int i = threadIdx.x; i < a.nq * D; i += 32 * WARPS) ((T*)a.out)[(size_t)r * a.nq * D + i] = from_float<T>(0.f);
     if (share == 0) return;
-    Place at{};
     for (int r0 = 0, before = 0; r0 < a.requests; r0 += 32) {
         const int own = r0 + lane < a.requests ? tiles_of(a, r0 + lane) * pairs : 0;
         int run = own;                                                // of the requests up to this lane's
@@ -215,10 +179,62 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) decode_mma_kernel(const De
             at.tile = in - pair_no * at.tiles;
             at.kvh = chunks == 1 ? pair_no : pair_no / chunks;
             at.chunk = pair_no - at.kvh * chunks;
-            break;
+            return;
         }
         before += __shfl_sync(0xffffffffu, run, 31);
     }
+}
+
+__device__ __forceinline__ void put4(float* to, float4 v) { *reinterpret_cast<float4*>(to) = v; }
+__device__ __forceinline__ void put4(__nv_bfloat16* to, float4 v) { *reinterpret_cast<uint2*>(to) = make_uint2(bits(__floats2bfloat162_rn(v.x, v.y)), bits(__floats2bfloat162_rn(v.z, v.w))); }
+
+// The warps' (max in units of log2, sum, output) of a pair's part, in shared memory, together: divided and rounded to the output where the whole pair was here (``alone``), else to
+// the part's slot.
+template <typename T, int D>
+__device__ __forceinline__ void end_part(const DecodeArgs& a, int req, int head0, int heads, bool alone, bool second, const float (*m_s)[HEADS], const float (*l_s)[HEADS], const float* o_s,
+                                         int o_warp, int o_head) {
+    const size_t part = 2 * (size_t)blockIdx.x + second;
+    for (int i = threadIdx.x; i < heads * (D / 4); i += 32 * WARPS) {
+        const int h = i / (D / 4), f = 4 * (i - h * (D / 4));
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, m_s[w][h]);
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float by = m_s[w][h] == -INFINITY ? (l_s[w][h] == 0.f ? 0.f : 1.f) : ex2(m_s[w][h] - m);
+            const float4 x = *reinterpret_cast<const float4*>(o_s + w * o_warp + h * o_head + f);
+            if (by != 0.f) l = fmaf(by, l_s[w][h], l), v.x = fmaf(by, x.x, v.x), v.y = fmaf(by, x.y, v.y), v.z = fmaf(by, x.z, v.z), v.w = fmaf(by, x.w, v.w);
+        }
+        if (alone) {
+            const float by = l == 0.f ? 0.f : 1.f / l;
+            put4((T*)a.out + ((size_t)req * a.nq + head0 + h) * D + f, make_float4(v.x * by, v.y * by, v.z * by, v.w * by));
+        } else {
+            *reinterpret_cast<float4*>(a.part_o + (part * HEADS + h) * D + f) = v;
+            if (f == 0) *reinterpret_cast<float2*>(a.part_ml + (part * HEADS + h) * 2) = make_float2(m, l);
+        }
+    }
+}
+
+// Keys on the rows of the products (16 of them), query heads on their eight columns: S^T = K q^T, O^T = V^T P^T.  The warps of a block take the tiles of its share in turn, each through
+// a ring of its own that runs on from one pair to the next; they meet where a pair's part ends.
+template <int D>
+__global__ void __launch_bounds__(32 * WARPS, BLOCKS) decode_mma_kernel(const DecodeArgs a) {
+    using S = Tile<D>;
+    constexpr int G = S::G, LD = D + 4;
+    extern __shared__ __align__(16) unsigned char ring_s[];
+    __shared__ float m_s[WARPS][HEADS], l_s[WARPS][HEADS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = a.nq / a.nkv, chunks = (group + HEADS - 1) / HEADS, pairs = a.nkv * chunks;
+    unsigned char* mine = ring_s + warp * STAGES * S::BYTES;
+    float* o_s = reinterpret_cast<float*>(ring_s + WARPS * STAGES * S::BYTES);      // [warps][heads][LD]
+    const uint32_t ring = mma16::smem_u32(mine);
+    pdl_wait();
+    pdl_launch_dependents();                                          // (the joining kernel may so read the lengths ahead of its own wait)
+    Place at{};
+    int share = 0;
+    begin_share<__nv_bfloat16, D>(a, pairs, chunks, at, share);
+    if (share == 0) return;
     // the tile to ask for next, the `asked`-th of the share: this warp's own are `warp` and every fourth behind it
     Place ahead = at;
     int asked = warp, issued = 0;
@@ -410,29 +426,7 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) decode_mma_kernel(const De
         }
     }
     __syncthreads();
-    const bool alone = at.tile == 0 && ends - began == at.tiles;
-    const size_t part = 2 * (size_t)blockIdx.x + (began != 0);
-    for (int i = threadIdx.x; i < heads * (D / 4); i += 32 * WARPS) {
-        const int h = i / (D / 4), f = 4 * (i - h * (D / 4));
-        float m = -INFINITY, l = 0.f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, m_s[w][h]);
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-            const float by = m_s[w][h] == -INFINITY ? (l_s[w][h] == 0.f ? 0.f : 1.f) : ex2(m_s[w][h] - m);
-            const float4 x = *reinterpret_cast<const float4*>(o_s + (w * HEADS + h) * LD + f);
-            if (by != 0.f) l = fmaf(by, l_s[w][h], l), v.x = fmaf(by, x.x, v.x), v.y = fmaf(by, x.y, v.y), v.z = fmaf(by, x.z, v.z), v.w = fmaf(by, x.w, v.w);
-        }
-        if (alone) {
-            const float by = l == 0.f ? 0.f : 1.f / l;
-            *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)req * a.nq + head0 + h) * D + f) =
-                make_uint2(bits(__floats2bfloat162_rn(v.x * by, v.y * by)), bits(__floats2bfloat162_rn(v.z * by, v.w * by)));
-        } else {
-            *reinterpret_cast<float4*>(a.part_o + (part * HEADS + h) * D + f) = v;
-            if (f == 0) *reinterpret_cast<float2*>(a.part_ml + (part * HEADS + h) * 2) = make_float2(m, l);
-        }
-    }
+    end_part<__nv_bfloat16, D>(a, req, head0, heads, at.tile == 0 && ends - began == at.tiles, began != 0, m_s, l_s, o_s, HEADS * LD, LD);
     __syncthreads();                                                  // (the next part's sums go where these were)
     began = ends;
     if (began < share) at.next_pair(a, chunks);
@@ -441,10 +435,10 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) decode_mma_kernel(const De
 
 // The parts of a pair that several blocks have worked on: a block a pair.  grid (pairs of a request, requests)
 constexpr int JOIN_THREADS = 128;
-template <int D>
-__global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const DecodeArgs a, int blocks) {
-    const int req = blockIdx.y, group = a.nq / a.nkv, chunks = (group + HEADS - 1) / HEADS, pairs = a.nkv * chunks;
-    const int kvh = blockIdx.x / chunks, chunk = blockIdx.x - kvh * chunks, head0 = kvh * group + chunk * HEADS, heads = min(HEADS, group - chunk * HEADS);
+template <typename T, int D>
+__global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const DecodeArgs a, int blocks, int chunk_heads) {
+    const int req = blockIdx.y, group = a.nq / a.nkv, chunks = (group + chunk_heads - 1) / chunk_heads, pairs = a.nkv * chunks;
+    const int kvh = blockIdx.x / chunks, chunk = blockIdx.x - kvh * chunks, head0 = kvh * group + chunk * chunk_heads, heads = min(chunk_heads, group - chunk * chunk_heads);
     pdl_launch_dependents();
     const int tiles = tiles_of(a, req), lane = threadIdx.x & 31;
     int total = 0, before = 0;
@@ -476,108 +470,130 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const DecodeAr
             if (by != 0.f) l = fmaf(by, ml.y, l), o.x = fmaf(by, v.x, o.x), o.y = fmaf(by, v.y, o.y), o.z = fmaf(by, v.z, o.z), o.w = fmaf(by, v.w, o.w);
         }
         const float by = l == 0.f ? 0.f : 1.f / l;
-        *reinterpret_cast<uint2*>((__nv_bfloat16*)a.out + ((size_t)req * a.nq + head0 + h) * D + f) =
-            make_uint2(bits(__floats2bfloat162_rn(o.x * by, o.y * by)), bits(__floats2bfloat162_rn(o.z * by, o.w * by)));
+        put4((T*)a.out + ((size_t)req * a.nq + head0 + h) * D + f, make_float4(o.x * by, o.y * by, o.z * by, o.w * by));
     }
 }
 
-// ---- any page, float32 or bfloat16 queries, on the CUDA cores -----------------------------------------
-constexpr int SIMT_KT = 32, SIMT_THREADS = 128;
-
-inline size_t simt_floats(int d) { return (size_t)SIMT_KT * (d + 1) + (size_t)SIMT_KT * d + (size_t)2 * HEADS * d + HEADS * SIMT_KT + 3 * HEADS; }
-
-template <typename T>
-__global__ void __launch_bounds__(SIMT_THREADS) decode_simt_kernel(const DecodeArgs a) {
-    extern __shared__ float sm[];
-    const int d = a.d, ld = d + 1, groups = d / GROUP, words = d / 8;
-    float* k_s = sm;                                // [places][d + 1]
-    float* v_s = k_s + SIMT_KT * ld;                // [places][d]
-    float* q_s = v_s + SIMT_KT * d;                 // [heads][d]
-    float* o_s = q_s + HEADS * d;                   // [heads][d]
-    float* p_s = o_s + HEADS * d;                   // [heads][places]
-    float* m_s = p_s + HEADS * SIMT_KT;
-    float* l_s = m_s + HEADS;
-    float* f_s = l_s + HEADS;
-    const int tid = threadIdx.x;
-    const int group = a.nq / a.nkv, chunks = (group + HEADS - 1) / HEADS, kvh = blockIdx.y / chunks, chunk = blockIdx.y - kvh * chunks, req = blockIdx.z;
-    const int head0 = kvh * group + chunk * HEADS, heads = min(HEADS, group - chunk * HEADS);
-    pdl_enter_small();
-    int beg, end;
-    range_of(a, req, blockIdx.x, SIMT_KT, beg, end);
+// ---- float32, and any page, on the CUDA cores ----------------------------------------------------------
+// The same cut of the work.  A warp a tile at a time: a lane a place for the scores (its key's words out of global memory, the queries out of shared memory), then a lane a word of
+// eight features of the values, D / 8 lanes side by side and what is left of the warp on other places.  Everything is float32: x = lowest + step code in one rounding.
+template <typename T, int D, int HN>
+__global__ void __launch_bounds__(32 * WARPS) decode_cores_kernel(const DecodeArgs a) {
+    constexpr int G = D / GROUP, WORDS = D / 8, ROW = WORDS <= 8 ? 8 : WORDS <= 16 ? 16 : 32, AT_ONCE = 32 / ROW, LD = D + 4;
+    __shared__ __align__(16) float q_s[D][HN], o_s[WARPS][HN][LD];
+    __shared__ float p_s[WARPS][KT][HN], m_s[WARPS][HEADS], l_s[WARPS][HEADS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.nq / a.nkv, chunks = (group + HN - 1) / HN, pairs = a.nkv * chunks;
+    pdl_wait();
+    pdl_launch_dependents();
+    Place at{};
+    int share = 0;
+    begin_share<T, D>(a, pairs, chunks, at, share);
     const float scale = a.scale * LOG2E;
-    for (int i = tid; i < HEADS * d; i += SIMT_THREADS) {
-        q_s[i] = i / d < heads ? to_float(((const T*)a.q)[((size_t)req * a.nq + head0) * d + i]) * scale : 0.f;
-        o_s[i] = 0.f;
-    }
-    if (tid < HEADS) m_s[tid] = -INFINITY, l_s[tid] = 0.f;
-    const size_t rows = (size_t)a.page_size * row_bytes(d);
-    for (int key0 = beg; key0 < end; key0 += SIMT_KT) {
-        const int n = min(SIMT_KT, end - key0);
+    const size_t rows = (size_t)a.page_size * row_bytes(D);
+    for (int began = 0; began < share;) {
+        const int req = at.req, head0 = at.kvh * group + at.chunk * HN, heads = min(HN, group - at.chunk * HN), ends = min(share, began + at.tiles - at.tile);
+        for (int i = threadIdx.x; i < HN * D; i += 32 * WARPS) {
+            const int h = i / D, f = i - h * D;
+            q_s[f][h] = h < heads ? to_float(((const T*)a.q)[((size_t)req * a.nq + head0 + h) * D + f]) * scale : 0.f;
+        }
         __syncthreads();
-        for (int i = tid; i < n * words * 2; i += SIMT_THREADS) {
-            const int value = i >= n * words, x = value ? i - n * words : i, row = x / words, l = x - row * words;
-            const int j = key0 + row, slot = j % a.page_size;
-            const uint8_t* p = a.kv + (((size_t)page_of(a, req, j) * a.nkv + kvh) * 2 + value) * rows;
-            const uint32_t w = reinterpret_cast<const uint32_t*>(p + (size_t)slot * (d / 2))[value ? value_word(l, groups) : key_word(l, groups)];
-            const uint32_t h = reinterpret_cast<const uint32_t*>(p + (size_t)a.page_size * (d / 2))[slot * groups + (l >> 3)];
-            float* dst = (value ? v_s + row * d : k_s + row * ld) + 8 * l;
+        float most[HN], sum[HN], o[HN][8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = fmaf((float)(w >> (4 * e) & 15u), low(h), high(h));
+        for (int h = 0; h < HN; ++h) {
+            most[h] = -INFINITY, sum[h] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[h][e] = 0.f;
         }
-        __syncthreads();
-        for (int i = tid; i < HEADS * SIMT_KT; i += SIMT_THREADS) {
-            const int h = i / SIMT_KT, j = i - h * SIMT_KT;
-            float s = -INFINITY;
-            if (j < n && h < heads) {
-                float s0 = 0.f, s1 = 0.f;
-                for (int f = 0; f < d; f += 2) {
-                    s0 = fmaf(q_s[h * d + f], k_s[j * ld + f], s0);
-                    s1 = fmaf(q_s[h * d + f + 1], k_s[j * ld + f + 1], s1);
+        for (int next = began + warp; next < ends; next += WARPS) {
+            const int key0 = (at.tile + next - began) * KT, n = min(KT, at.places - key0), j = key0 + min(lane, n - 1);
+            const int slot = j % a.page_size;
+            const uint8_t* page = a.kv + ((size_t)page_of(a, req, j) * a.nkv + at.kvh) * (2 * rows);        // of this lane's place
+            float s[HN];
+            {
+                uint32_t w[WORDS];
+                const uint32_t* held = reinterpret_cast<const uint32_t*>(page + (size_t)a.page_size * (D / 2)) + slot * G;
+                if (rows % 16 == 0) {
+#pragma unroll
+                    for (int i = 0; i < WORDS; i += 4) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(page + (size_t)slot * (D / 2) + 4 * i);
+                        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+                    }
+                } else {                                              // (pages of one or two places)
+#pragma unroll
+                    for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const uint32_t*>(page + (size_t)slot * (D / 2))[i];
                 }
-                s = s0 + s1;
+#pragma unroll
+                for (int h = 0; h < HN; ++h) s[h] = 0.f;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const uint32_t hd = held[g];
+                    const float step = low(hd), lowest = high(hd);
+#pragma unroll
+                    for (int l = 0; l < 8; ++l) {
+                        const uint32_t word = w[(l & 3) * 2 * G + 2 * g + (l >> 2)];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float x = fmaf(__uint_as_float((word >> (4 * e) & 15u) | 0x4B000000u) - 8388608.f, step, lowest);
+                            const float* q = q_s[64 * g + 8 * l + e];
+#pragma unroll
+                            for (int h = 0; h < HN; ++h) s[h] = fmaf(q[h], x, s[h]);
+                        }
+                    }
+                }
             }
-            p_s[i] = s;
-        }
-        __syncthreads();
-        // a warp two heads, a lane a place
-        for (int h = tid >> 5; h < heads; h += SIMT_THREADS / 32) {
-            const int lane = tid & 31;
-            const float s = p_s[h * SIMT_KT + lane], m = fmaxf(m_s[h], warp_max(s)), z = m == -INFINITY ? 0.f : m;
-            const float p = lane < n ? exp2f(s - z) : 0.f, sum = warp_sum(p);
-            const float was = m_s[h], f = was == m ? 1.f : exp2f(was - z);
+#pragma unroll
+            for (int h = 0; h < HN; ++h) {
+                if (lane >= n) s[h] = -INFINITY;
+                const float m = fmaxf(most[h], warp_max(s[h])), z = m == -INFINITY ? 0.f : m;
+                const float f = most[h] == m ? 1.f : ex2(most[h] - z), p = ex2(s[h] - z);
+                most[h] = m;
+                sum[h] = fmaf(sum[h], f, p);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[h][e] *= f;
+                p_s[warp][lane][h] = p;
+            }
             __syncwarp();
-            p_s[h * SIMT_KT + lane] = p;
-            if (lane == 0) m_s[h] = m, l_s[h] = l_s[h] * f + sum, f_s[h] = f;
+            const int l = lane % ROW, sub = lane / ROW;
+            if (l < WORDS) {
+#pragma unroll 4
+                for (int i = sub; i < n; i += AT_ONCE) {
+                    const int jv = key0 + i, sv = jv % a.page_size;
+                    const uint8_t* pv = a.kv + ((size_t)page_of(a, req, jv) * a.nkv + at.kvh) * (2 * rows) + rows;
+                    const uint32_t word = reinterpret_cast<const uint32_t*>(pv + (size_t)sv * (D / 2))[value_word(l, G)];
+                    const uint32_t hd = reinterpret_cast<const uint32_t*>(pv + (size_t)a.page_size * (D / 2))[sv * G + (l >> 3)];
+                    const float step = low(hd), lowest = high(hd);
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = fmaf(__uint_as_float((word >> (4 * e) & 15u) | 0x4B000000u) - 8388608.f, step, lowest);
+#pragma unroll
+                    for (int h = 0; h < HN; ++h) {
+                        const float p = p_s[warp][i][h];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[h][e] = fmaf(p, x[e], o[h][e]);
+                    }
+                }
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int h = 0; h < HN; ++h) {
+            sum[h] = warp_sum(sum[h]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int x = ROW; x < 32; x <<= 1) o[h][e] += __shfl_xor_sync(0xffffffffu, o[h][e], x);
+            if (lane == 0) m_s[warp][h] = most[h], l_s[warp][h] = sum[h];
+            if (lane < WORDS) {
+                float4* to = reinterpret_cast<float4*>(o_s[warp][h] + 8 * lane);
+                to[0] = make_float4(o[h][0], o[h][1], o[h][2], o[h][3]);
+                to[1] = make_float4(o[h][4], o[h][5], o[h][6], o[h][7]);
+            }
         }
         __syncthreads();
-        for (int i = tid; i < heads * d; i += SIMT_THREADS) {
-            const int h = i / d, f = i - h * d;
-            float v = o_s[i] * f_s[h];
-            for (int j = 0; j < n; ++j) v = fmaf(p_s[h * SIMT_KT + j], v_s[j * d + f], v);
-            o_s[i] = v;
-        }
-    }
-    __syncthreads();
-    leave<T>(a, req, head0, heads, m_s, l_s, o_s, d);
-}
-
-// ---- what the ranges of a row left, joined ------------------------------------------------------------
-template <typename T>
-__global__ void __launch_bounds__(128) join_kernel(const DecodeArgs a) {
-    pdl_enter_small();
-    const size_t row = blockIdx.x;                  // request x query head
-    const float* ml = a.part_ml + row * a.splits * 2;
-    float m = -INFINITY;
-    for (int z = 0; z < a.splits; ++z) m = fmaxf(m, ml[2 * z]);
-    float l = 0.f;
-    for (int z = 0; z < a.splits; ++z) l += ml[2 * z] == -INFINITY ? ml[2 * z + 1] : exp2f(ml[2 * z] - m) * ml[2 * z + 1];
-    for (int f = threadIdx.x; f < a.d; f += 128) {
-        float v = 0.f;
-        for (int z = 0; z < a.splits; ++z) {
-            const float w = ml[2 * z] == -INFINITY ? (ml[2 * z + 1] == 0.f ? 0.f : 1.f) : exp2f(ml[2 * z] - m);
-            if (w != 0.f) v += w * a.part_o[(row * a.splits + z) * a.d + f];
-        }
-        ((T*)a.out)[row * a.d + f] = from_float<T>(l == 0.f ? 0.f : v / l);
+        end_part<T, D>(a, req, head0, heads, at.tile == 0 && ends - began == at.tiles, began != 0, m_s, l_s, &o_s[0][0][0], HN * LD, LD);
+        __syncthreads();
+        began = ends;
+        if (began < share) at.next_pair(a, chunks);
     }
 }
 
@@ -589,16 +605,20 @@ inline int log2_of(int page_size) {
 // The tensor-core kernel takes bfloat16 and pages of a power of two from 16 places on (a run of sixteen bytes of steps lies in one page).
 inline bool on_tensor_cores(int page_size, int dtype) { return dtype == kBF16 && page_size >= 16 && log2_of(page_size) >= 0; }
 
-// Ranges a row's places are cut into on the CUDA cores: as many as fill the device, none too short.
-inline int ranges_of(int requests, int nq, int nkv, int longest) {
-    const long long pairs = (long long)requests * nkv * ((nq / nkv + HEADS - 1) / HEADS);
-    const long long want = pairs > 0 ? 3 * sm_count() / pairs : 1, most = ((long long)longest + 2 * SIMT_KT - 1) / (2 * SIMT_KT);
-    return (int)max(1ll, min(min(want, most), 256ll));
+// Query heads of a pair on the CUDA cores.
+inline int cores_heads(int group) { return group <= 4 ? 4 : 8; }
+// Blocks: as many as are on the device at once, a tile a warp at least.
+inline int blocks_of(int requests, int nq, int nkv, int longest, int heads, int a_sm) {
+    const long long pairs = (long long)requests * nkv * ((nq / nkv + heads - 1) / heads), tiles = pairs * (((long long)longest + KT - 1) / KT);
+    return (int)max(1ll, min((long long)a_sm * sm_count(), (tiles + WARPS - 1) / WARPS));
 }
-// Blocks of the tensor-core kernel: as many as are on the device at once, a tile a warp at least.
-inline int blocks_of(int requests, int nq, int nkv, int d, int longest) {
-    const long long pairs = (long long)requests * nkv * ((nq / nkv + HEADS - 1) / HEADS), tiles = pairs * (((long long)longest + KT - 1) / KT);
-    return (int)max(1ll, min((long long)BLOCKS * sm_count(), (tiles + WARPS - 1) / WARPS));
+struct Plan { bool tensor_cores; int heads, blocks; };
+inline Plan plan_of(int requests, int nq, int nkv, int longest, int page_size, int dtype) {
+    Plan p{};
+    p.tensor_cores = on_tensor_cores(page_size, dtype);
+    p.heads = p.tensor_cores ? HEADS : cores_heads(nq / nkv);
+    p.blocks = blocks_of(requests, nq, nkv, longest, p.heads, p.tensor_cores ? BLOCKS : 3);
+    return p;
 }
 
 }  // namespace four
@@ -609,9 +629,7 @@ using namespace lily;
 // float32 of scratch that lily_attention_decode4 needs
 LILY_API size_t lily_attention_decode4_floats(int requests, int nq, int nkv, int d, int longest, int page_size, int dtype) {
     if (requests <= 0 || nkv <= 0 || nq <= 0 || nq % nkv || page_size <= 0) return 0;
-    if (four::on_tensor_cores(page_size, dtype)) return (size_t)2 * four::blocks_of(requests, nq, nkv, d, longest) * four::HEADS * (d + 2);
-    const int splits = four::ranges_of(requests, nq, nkv, longest);
-    return splits == 1 ? 0 : (size_t)requests * nq * splits * (d + 2);
+    return (size_t)2 * four::plan_of(requests, nq, nkv, longest, page_size, dtype).blocks * four::HEADS * (d + 2);
 }
 
 LILY_API int lily_attention_decode4(const void* q, const void* kv, void* out, const int* block_table, int width, const int* seq_lens, float* scratch, int requests, int longest, int nq,
@@ -624,55 +642,43 @@ LILY_API int lily_attention_decode4(const void* q, const void* kv, void* out, co
     LILY_REQUIRE(longest <= INT32_MAX - 1024, "attention_decode4: rows of %d places", longest);
     LILY_REQUIRE(((uintptr_t)q | (uintptr_t)kv | (uintptr_t)out) % 16 == 0, "attention_decode4: tensors on boundaries of sixteen bytes");
     LILY_REQUIRE(scale != 0.f && scale - scale == 0.f, "attention_decode4: a scale of %g", (double)scale);
-    const int chunks = (nq / nkv + four::HEADS - 1) / four::HEADS;
-    LILY_REQUIRE((long long)nkv * chunks <= 65535, "attention_decode4: %d kv heads", nkv);
+    const four::Plan plan = four::plan_of(requests, nq, nkv, longest, page_size, dtype);
+    const int chunks = (nq / nkv + plan.heads - 1) / plan.heads;
+    LILY_REQUIRE((long long)requests * nkv * chunks * ((longest + four::KT - 1) / four::KT) <= INT32_MAX, "attention_decode4: %d requests of up to %d places are too many for one call", requests, longest);
+    LILY_REQUIRE(scratch != nullptr && (uintptr_t)scratch % 16 == 0, "attention_decode4: the parts of %d blocks need scratch on a boundary of sixteen bytes", plan.blocks);
     four::DecodeArgs a{};
     a.q = q; a.kv = (const uint8_t*)kv; a.out = out; a.block_table = block_table; a.width = width; a.seq_lens = seq_lens;
-    const bool tensor_cores = four::on_tensor_cores(page_size, dtype);
-    a.requests = requests;
-    a.nq = nq; a.nkv = nkv; a.d = d; a.page_size = page_size; a.pages = pages; a.longest = longest; a.scale = scale;
-    if (tensor_cores) {
-        a.page_shift = four::log2_of(page_size);
-        LILY_REQUIRE((long long)requests * nkv * chunks * ((longest + four::KT - 1) / four::KT) <= INT32_MAX, "attention_decode4: %d requests of up to %d places are too many for one call", requests, longest);
-        const int blocks = four::blocks_of(requests, nq, nkv, d, longest);
-        LILY_REQUIRE(scratch != nullptr && (uintptr_t)scratch % 16 == 0, "attention_decode4: the parts of %d blocks need scratch on a boundary of sixteen bytes", blocks);
-        a.part_o = scratch;
-        a.part_ml = scratch + (size_t)2 * blocks * four::HEADS * d;
-#define DECODE(D)                                                                                                                     \
-    {                                                                                                                                 \
-        constexpr int bytes = four::WARPS * (four::STAGES * four::Tile<D>::BYTES + four::HEADS * (D + 4) * 4);                        \
-        cudaFuncSetAttribute(four::decode_mma_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);                         \
-        launch_pdl(four::decode_mma_kernel<D>, dim3(blocks), dim3(32 * four::WARPS), bytes, stream, a);                               \
-        LILY_CHECK_LAUNCH("attention_decode4");                                                                                       \
-        launch_pdl(four::join_parts_kernel<D>, dim3(nkv * chunks, requests), dim3(four::JOIN_THREADS), 0, stream, a, blocks); \
-    }
-        if (d == 64) DECODE(64)
-        else if (d == 128) DECODE(128)
-        else if (d == 192) DECODE(192)
-        else DECODE(256)
-#undef DECODE
-        LILY_CHECK_LAUNCH("attention_decode4 (join)");
-        return 0;
-    }
-    a.splits = four::ranges_of(requests, nq, nkv, longest);
+    a.requests = requests; a.nq = nq; a.nkv = nkv; a.d = d; a.page_size = page_size; a.pages = pages; a.longest = longest; a.scale = scale;
+    a.page_shift = four::log2_of(page_size);
     a.part_o = scratch;
-    a.part_ml = scratch + (size_t)requests * nq * a.splits * d;
-    LILY_REQUIRE(a.splits == 1 || scratch != nullptr, "attention_decode4: %d ranges need scratch", a.splits);
-    const dim3 grid(a.splits, nkv * chunks, requests);
-    {
-        const size_t bytes = four::simt_floats(d) * sizeof(float);
-        auto run = [&](auto kernel) {
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-            launch_pdl(kernel, grid, dim3(four::SIMT_THREADS), bytes, stream, a);
-        };
-        if (dtype == kF32) run(four::decode_simt_kernel<float>);
-        else run(four::decode_simt_kernel<__nv_bfloat16>);
-    }
-    LILY_CHECK_LAUNCH("attention_decode4");
-    if (a.splits > 1) {
-        if (dtype == kF32) launch_pdl(four::join_kernel<float>, dim3(requests * nq), dim3(128), 0, stream, a);
-        else launch_pdl(four::join_kernel<__nv_bfloat16>, dim3(requests * nq), dim3(128), 0, stream, a);
-        LILY_CHECK_LAUNCH("attention_decode4 (join)");
-    }
+    a.part_ml = scratch + (size_t)2 * plan.blocks * four::HEADS * d;
+    const dim3 block(32 * four::WARPS);
+#define JOIN(T, D)                                                                                                                                                 \
+    LILY_CHECK_LAUNCH("attention_decode4");                                                                                                                        \
+    launch_pdl(four::join_parts_kernel<T, D>, dim3(nkv * chunks, requests), dim3(four::JOIN_THREADS), 0, stream, a, plan.blocks, plan.heads)
+#define DECODE(D)                                                                                                                                                  \
+    do {                                                                                                                                                           \
+        if (plan.tensor_cores) {                                                                                                                                   \
+            constexpr int bytes = four::WARPS * (four::STAGES * four::Tile<D>::BYTES + four::HEADS * (D + 4) * 4);                                                 \
+            cudaFuncSetAttribute(four::decode_mma_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);                                                  \
+            launch_pdl(four::decode_mma_kernel<D>, dim3(plan.blocks), block, bytes, stream, a);                                                                    \
+            JOIN(__nv_bfloat16, D);                                                                                                                                \
+        } else if (dtype == kF32) {                                                                                                                                \
+            if (plan.heads == 4) launch_pdl(four::decode_cores_kernel<float, D, 4>, dim3(plan.blocks), block, 0, stream, a);                                       \
+            else launch_pdl(four::decode_cores_kernel<float, D, 8>, dim3(plan.blocks), block, 0, stream, a);                                                       \
+            JOIN(float, D);                                                                                                                                        \
+        } else {                                                                                                                                                   \
+            if (plan.heads == 4) launch_pdl(four::decode_cores_kernel<__nv_bfloat16, D, 4>, dim3(plan.blocks), block, 0, stream, a);                               \
+            else launch_pdl(four::decode_cores_kernel<__nv_bfloat16, D, 8>, dim3(plan.blocks), block, 0, stream, a);                                               \
+            JOIN(__nv_bfloat16, D);                                                                                                                                \
+        }                                                                                                                                                          \
+    } while (0)
+    if (d == 64) DECODE(64);
+    else if (d == 128) DECODE(128);
+    else if (d == 192) DECODE(192);
+    else DECODE(256);
+#undef DECODE
+#undef JOIN
+    LILY_CHECK_LAUNCH("attention_decode4 (join)");
     return 0;
 }

@@ -258,7 +258,7 @@ def decode_case(lengths, nq, nkv, d, page, dtype, seed=0, lean=0.5):
     return q.to(DEV), kv.to(DEV), table.to(DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV)
 
 
-HEADS = [(8, 2, 128, 64), (4, 4, 64, 16), (16, 1, 128, 16), (24, 2, 64, 128), (6, 1, 192, 32), (4, 1, 256, 64), (7, 1, 128, 64), (2, 1, 64, 4)]
+HEADS = [(8, 2, 128, 64), (4, 4, 64, 16), (16, 1, 128, 16), (24, 2, 64, 128), (6, 1, 192, 32), (4, 1, 256, 64), (7, 1, 128, 64), (2, 1, 64, 4), (3, 1, 64, 1), (2, 2, 128, 3), (10, 2, 192, 2)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
