@@ -151,18 +151,23 @@ struct Cut {
 template <typename T, int D>
 __device__ __forceinline__ void begin_share(const DecodeArgs& a, int pairs, int chunks, Place& at, int& share) {
     const int lane = threadIdx.x & 31;
-    int total = 0;
-    for (int r = lane; r < a.requests; r += 32) total += tiles_of(a, r);
+    auto length = [&](int r) { return r < a.requests ? places_of(a, r) : 0; };
+    const int own_length = length(lane);                              // (most steps have no more than 32 rows: one read each)
+    int total = (own_length + KT - 1) / KT;
+    for (int r = lane + 32; r < a.requests; r += 32) total += tiles_of(a, r);
     total = __reduce_add_sync(0xffffffffu, total);
     const Cut cut(total * pairs, gridDim.x);
     const int first = cut.begins(blockIdx.x);
     share = cut.per + ((int)blockIdx.x < cut.more);
-    for (int r = blockIdx.x; r < a.requests; r += gridDim.x)
-        if (places_of(a, r) == 0)
-            for (int i = threadIdx.x; i < a.nq * D; i += 32 * WARPS) ((T*)a.out)[(size_t)r * a.nq * D + i] = from_float<T>(0.f);
-    if (share == 0) return;
+    bool found = share == 0;
     for (int r0 = 0, before = 0; r0 < a.requests; r0 += 32) {
-        const int own = r0 + lane < a.requests ? tiles_of(a, r0 + lane) * pairs : 0;
+        const int n = r0 ? length(r0 + lane) : own_length, own = (n + KT - 1) / KT * pairs;
+        for (unsigned without = __ballot_sync(0xffffffffu, r0 + lane < a.requests && n == 0); without; without &= without - 1) {
+            const int r = r0 + __ffs(without) - 1;
+            if (r % (int)gridDim.x == (int)blockIdx.x)
+                for (int i = threadIdx.x; i < a.nq * D; i += 32 * WARPS) ((T*)a.out)[(size_t)r * a.nq * D + i] = from_float<T>(0.f);
+        }
+        if (found) continue;
         int run = own;                                                // of the requests up to this lane's
 #pragma unroll
         for (int x = 1; x < 32; x <<= 1) {
@@ -173,13 +178,13 @@ __device__ __forceinline__ void begin_share(const DecodeArgs& a, int pairs, int 
         if (beyond) {
             const int where = __ffs(beyond) - 1;
             at.req = r0 + where;
-            at.places = places_of(a, at.req);
+            at.places = __shfl_sync(0xffffffffu, n, where);
             at.tiles = (at.places + KT - 1) / KT;
             const int in = first - (before + __shfl_sync(0xffffffffu, run - own, where)), pair_no = in / at.tiles;
             at.tile = in - pair_no * at.tiles;
             at.kvh = chunks == 1 ? pair_no : pair_no / chunks;
             at.chunk = pair_no - at.kvh * chunks;
-            return;
+            found = true;
         }
         before += __shfl_sync(0xffffffffu, run, 31);
     }
@@ -455,19 +460,28 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const DecodeAr
     if (b0 == b1) return;
     for (int i = threadIdx.x; i < heads * (D / 4); i += JOIN_THREADS) {
         const int h = i / (D / 4), f = 4 * (i - h * (D / 4));
+        auto part_of = [&](int b) { return (2 * (size_t)b + (b == b0 ? behind : 0)) * HEADS + h; };
         float m = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int b = b0; b <= b1; ++b) {
-            const size_t part = 2 * (size_t)b + (b == b0 ? behind : 0);
-            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (part * HEADS + h) * 2);
-            const float4 v = *reinterpret_cast<const float4*>(a.part_o + (part * HEADS + h) * D + f);
-            const float next = fmaxf(m, ml.x), was = m == next ? 1.f : ex2(m - next);
-            const float by = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : ex2(ml.x - next);
+        for (int first = b0; first <= b1; first += 4) {               // four parts at a time
+            float2 ml[4];
+            float4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const size_t part = part_of(min(first + i, b1));
+                ml[i] = *reinterpret_cast<const float2*>(a.part_ml + part * 2);
+                v[i] = *reinterpret_cast<const float4*>(a.part_o + part * D + f);
+                if (first + i > b1) ml[i] = make_float2(-INFINITY, 0.f);
+            }
+            const float next = fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x)), was = m == next ? 1.f : ex2(m - next);
             m = next;
             l *= was;
             o.x *= was, o.y *= was, o.z *= was, o.w *= was;
-            if (by != 0.f) l = fmaf(by, ml.y, l), o.x = fmaf(by, v.x, o.x), o.y = fmaf(by, v.y, o.y), o.z = fmaf(by, v.z, o.z), o.w = fmaf(by, v.w, o.w);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float by = ml[i].x == -INFINITY ? (ml[i].y == 0.f ? 0.f : 1.f) : ex2(ml[i].x - m);
+                if (by != 0.f) l = fmaf(by, ml[i].y, l), o.x = fmaf(by, v[i].x, o.x), o.y = fmaf(by, v[i].y, o.y), o.z = fmaf(by, v[i].z, o.z), o.w = fmaf(by, v[i].w, o.w);
+            }
         }
         const float by = l == 0.f ? 0.f : 1.f / l;
         put4((T*)a.out + ((size_t)req * a.nq + head0 + h) * D + f, make_float4(o.x * by, o.y * by, o.z * by, o.w * by));
@@ -475,14 +489,25 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const DecodeAr
 }
 
 // ---- float32, and any page, on the CUDA cores ----------------------------------------------------------
-// The same cut of the work.  A warp a tile at a time: a lane a place for the scores (its key's words out of global memory, the queries out of shared memory), then a lane a word of
-// eight features of the values, D / 8 lanes side by side and what is left of the warp on other places.  Everything is float32: x = lowest + step code in one rounding.
+// The same cut of the work.  A warp a tile at a time, whose rows its lanes bring to shared memory, a place each: a lane a place for the scores, then a lane a word of eight features of the
+// values, D / 8 lanes side by side and what is left of the warp on other places.  Everything is float32: x = lowest + step code in one rounding.  A step has a few tiles a warp at
+// most, so it is short loops that count: unrolled ones (the scores' 128 features, 16 places' values) are fetched from memory as they run once, 20 us where these take 10.
+template <int D, int HN> struct CoresTile {
+    static constexpr int G = D / GROUP, ROW = D / 2 + 16, HELD = 32 * ROW * 2, P = HELD + 32 * 8 * G, BYTES = P + 32 * HN * 4;      // keys' and values' rows, steps, weights
+    static constexpr int LD = D + 4, Q = WARPS * BYTES, O = Q + D * HN * 4, ALL = O + WARPS * HN * LD * 4;
+};
+
 template <typename T, int D, int HN>
 __global__ void __launch_bounds__(32 * WARPS) decode_cores_kernel(const DecodeArgs a) {
-    constexpr int G = D / GROUP, WORDS = D / 8, ROW = WORDS <= 8 ? 8 : WORDS <= 16 ? 16 : 32, AT_ONCE = 32 / ROW, LD = D + 4;
-    __shared__ __align__(16) float q_s[D][HN], o_s[WARPS][HN][LD];
-    __shared__ float p_s[WARPS][KT][HN], m_s[WARPS][HEADS], l_s[WARPS][HEADS];
+    using S = CoresTile<D, HN>;
+    constexpr int G = S::G, WORDS = D / 8, ROW = WORDS <= 8 ? 8 : WORDS <= 16 ? 16 : 32, AT_ONCE = 32 / ROW, LD = S::LD;
+    extern __shared__ __align__(16) unsigned char cores_s[];
+    __shared__ float m_s[WARPS][HEADS], l_s[WARPS][HEADS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.nq / a.nkv, chunks = (group + HN - 1) / HN, pairs = a.nkv * chunks;
+    unsigned char* mine = cores_s + warp * S::BYTES;
+    float (*q_s)[HN] = reinterpret_cast<float (*)[HN]>(cores_s + S::Q);
+    float* o_s = reinterpret_cast<float*>(cores_s + S::O);            // [warps][heads][LD]
+    float (*p_s)[HN] = reinterpret_cast<float (*)[HN]>(mine + S::P);
     pdl_wait();
     pdl_launch_dependents();
     Place at{};
@@ -490,13 +515,13 @@ __global__ void __launch_bounds__(32 * WARPS) decode_cores_kernel(const DecodeAr
     begin_share<T, D>(a, pairs, chunks, at, share);
     const float scale = a.scale * LOG2E;
     const size_t rows = (size_t)a.page_size * row_bytes(D);
+    const bool pieces = rows % 16 == 0;                               // (not pages of one or two places)
     for (int began = 0; began < share;) {
         const int req = at.req, head0 = at.kvh * group + at.chunk * HN, heads = min(HN, group - at.chunk * HN), ends = min(share, began + at.tiles - at.tile);
         for (int i = threadIdx.x; i < HN * D; i += 32 * WARPS) {
             const int h = i / D, f = i - h * D;
             q_s[f][h] = h < heads ? to_float(((const T*)a.q)[((size_t)req * a.nq + head0 + h) * D + f]) * scale : 0.f;
         }
-        __syncthreads();
         float most[HN], sum[HN], o[HN][8];
 #pragma unroll
         for (int h = 0; h < HN; ++h) {
@@ -504,73 +529,67 @@ __global__ void __launch_bounds__(32 * WARPS) decode_cores_kernel(const DecodeAr
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[h][e] = 0.f;
         }
+        __syncthreads();
         for (int next = began + warp; next < ends; next += WARPS) {
-            const int key0 = (at.tile + next - began) * KT, n = min(KT, at.places - key0), j = key0 + min(lane, n - 1);
-            const int slot = j % a.page_size;
-            const uint8_t* page = a.kv + ((size_t)page_of(a, req, j) * a.nkv + at.kvh) * (2 * rows);        // of this lane's place
-            float s[HN];
-            {
-                uint32_t w[WORDS];
-                const uint32_t* held = reinterpret_cast<const uint32_t*>(page + (size_t)a.page_size * (D / 2)) + slot * G;
-                if (rows % 16 == 0) {
+            const int key0 = (at.tile + next - began) * KT, n = min(KT, at.places - key0);
+            if (lane < n) {
+                const int j = key0 + lane, slot = j % a.page_size;
+                const uint8_t* page = a.kv + ((size_t)page_of(a, req, j) * a.nkv + at.kvh) * (2 * rows);
+                const uint8_t *codes = page + (size_t)slot * (D / 2), *held = page + (size_t)a.page_size * (D / 2) + (size_t)slot * G * 4;
+                unsigned char* to = mine + lane * S::ROW;
 #pragma unroll
-                    for (int i = 0; i < WORDS; i += 4) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(page + (size_t)slot * (D / 2) + 4 * i);
-                        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
-                    }
-                } else {                                              // (pages of one or two places)
+                for (int kind = 0; kind < 2; ++kind) {
+                    if (pieces) {
 #pragma unroll
-                    for (int i = 0; i < WORDS; ++i) w[i] = reinterpret_cast<const uint32_t*>(page + (size_t)slot * (D / 2))[i];
+                        for (int i = 0; i < D / 32; ++i) reinterpret_cast<uint4*>(to + kind * 32 * S::ROW)[i] = reinterpret_cast<const uint4*>(codes + kind * rows)[i];
+                    } else
+                        for (int i = 0; i < WORDS; ++i) reinterpret_cast<uint32_t*>(to + kind * 32 * S::ROW)[i] = reinterpret_cast<const uint32_t*>(codes + kind * rows)[i];
+#pragma unroll
+                    for (int i = 0; i < G; ++i) reinterpret_cast<uint32_t*>(mine + S::HELD)[(kind * 32 + lane) * G + i] = reinterpret_cast<const uint32_t*>(held + kind * rows)[i];
                 }
+            }
+            __syncwarp();
+            float s[HN];
 #pragma unroll
-                for (int h = 0; h < HN; ++h) s[h] = 0.f;
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    const uint32_t hd = held[g];
+            for (int h = 0; h < HN; ++h) s[h] = lane < n ? 0.f : -INFINITY;
+            if (lane < n) {
+#pragma unroll 1
+                for (int at_word = 0; at_word < WORDS; ++at_word) {   // in the order they lie in
+                    const int in = at_word % (2 * G), f = 64 * (in >> 1) + 32 * (in & 1) + 8 * (at_word / (2 * G));
+                    const uint32_t word = reinterpret_cast<const uint32_t*>(mine + lane * S::ROW)[at_word], hd = reinterpret_cast<const uint32_t*>(mine + S::HELD)[lane * G + (in >> 1)];
                     const float step = low(hd), lowest = high(hd);
 #pragma unroll
-                    for (int l = 0; l < 8; ++l) {
-                        const uint32_t word = w[(l & 3) * 2 * G + 2 * g + (l >> 2)];
+                    for (int e = 0; e < 8; ++e) {
+                        const float x = fmaf(__uint_as_float((word >> (4 * e) & 15u) | 0x4B000000u) - 8388608.f, step, lowest);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float x = fmaf(__uint_as_float((word >> (4 * e) & 15u) | 0x4B000000u) - 8388608.f, step, lowest);
-                            const float* q = q_s[64 * g + 8 * l + e];
-#pragma unroll
-                            for (int h = 0; h < HN; ++h) s[h] = fmaf(q[h], x, s[h]);
-                        }
+                        for (int h = 0; h < HN; ++h) s[h] = fmaf(q_s[f + e][h], x, s[h]);
                     }
                 }
             }
 #pragma unroll
             for (int h = 0; h < HN; ++h) {
-                if (lane >= n) s[h] = -INFINITY;
                 const float m = fmaxf(most[h], warp_max(s[h])), z = m == -INFINITY ? 0.f : m;
                 const float f = most[h] == m ? 1.f : ex2(most[h] - z), p = ex2(s[h] - z);
                 most[h] = m;
                 sum[h] = fmaf(sum[h], f, p);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) o[h][e] *= f;
-                p_s[warp][lane][h] = p;
+                p_s[lane][h] = p;
             }
             __syncwarp();
-            const int l = lane % ROW, sub = lane / ROW;
-            if (l < WORDS) {
-#pragma unroll 4
-                for (int i = sub; i < n; i += AT_ONCE) {
-                    const int jv = key0 + i, sv = jv % a.page_size;
-                    const uint8_t* pv = a.kv + ((size_t)page_of(a, req, jv) * a.nkv + at.kvh) * (2 * rows) + rows;
-                    const uint32_t word = reinterpret_cast<const uint32_t*>(pv + (size_t)sv * (D / 2))[value_word(l, G)];
-                    const uint32_t hd = reinterpret_cast<const uint32_t*>(pv + (size_t)a.page_size * (D / 2))[sv * G + (l >> 3)];
-                    const float step = low(hd), lowest = high(hd);
-                    float x[8];
+            const int l = min(lane % ROW, WORDS - 1);                 // (d = 192: the last lanes follow the one ahead of them and are not looked at)
+#pragma unroll 1
+            for (int i = lane / ROW; i < n; i += AT_ONCE) {
+                const uint32_t word = reinterpret_cast<const uint32_t*>(mine + (32 + i) * S::ROW)[value_word(l, G)], hd = reinterpret_cast<const uint32_t*>(mine + S::HELD)[(32 + i) * G + (l >> 3)];
+                const float step = low(hd), lowest = high(hd);
+                float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = fmaf(__uint_as_float((word >> (4 * e) & 15u) | 0x4B000000u) - 8388608.f, step, lowest);
+                for (int e = 0; e < 8; ++e) x[e] = fmaf(__uint_as_float((word >> (4 * e) & 15u) | 0x4B000000u) - 8388608.f, step, lowest);
 #pragma unroll
-                    for (int h = 0; h < HN; ++h) {
-                        const float p = p_s[warp][i][h];
+                for (int h = 0; h < HN; ++h) {
+                    const float p = p_s[i][h];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) o[h][e] = fmaf(p, x[e], o[h][e]);
-                    }
+                    for (int e = 0; e < 8; ++e) o[h][e] = fmaf(p, x[e], o[h][e]);
                 }
             }
             __syncwarp();
@@ -584,13 +603,13 @@ __global__ void __launch_bounds__(32 * WARPS) decode_cores_kernel(const DecodeAr
                 for (int x = ROW; x < 32; x <<= 1) o[h][e] += __shfl_xor_sync(0xffffffffu, o[h][e], x);
             if (lane == 0) m_s[warp][h] = most[h], l_s[warp][h] = sum[h];
             if (lane < WORDS) {
-                float4* to = reinterpret_cast<float4*>(o_s[warp][h] + 8 * lane);
+                float4* to = reinterpret_cast<float4*>(o_s + (warp * HN + h) * LD + 8 * lane);
                 to[0] = make_float4(o[h][0], o[h][1], o[h][2], o[h][3]);
                 to[1] = make_float4(o[h][4], o[h][5], o[h][6], o[h][7]);
             }
         }
         __syncthreads();
-        end_part<T, D>(a, req, head0, heads, at.tile == 0 && ends - began == at.tiles, began != 0, m_s, l_s, &o_s[0][0][0], HN * LD, LD);
+        end_part<T, D>(a, req, head0, heads, at.tile == 0 && ends - began == at.tiles, began != 0, m_s, l_s, o_s, HN * LD, LD);
         __syncthreads();
         began = ends;
         if (began < share) at.next_pair(a, chunks);
@@ -656,6 +675,12 @@ LILY_API int lily_attention_decode4(const void* q, const void* kv, void* out, co
 #define JOIN(T, D)                                                                                                                                                 \
     LILY_CHECK_LAUNCH("attention_decode4");                                                                                                                        \
     launch_pdl(four::join_parts_kernel<T, D>, dim3(nkv * chunks, requests), dim3(four::JOIN_THREADS), 0, stream, a, plan.blocks, plan.heads)
+#define CORES(T, D, HN)                                                                                                                                            \
+    do {                                                                                                                                                           \
+        constexpr int bytes = four::CoresTile<D, HN>::ALL;                                                                                                         \
+        cudaFuncSetAttribute(four::decode_cores_kernel<T, D, HN>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);                                             \
+        launch_pdl(four::decode_cores_kernel<T, D, HN>, dim3(plan.blocks), block, bytes, stream, a);                                                               \
+    } while (0)
 #define DECODE(D)                                                                                                                                                  \
     do {                                                                                                                                                           \
         if (plan.tensor_cores) {                                                                                                                                   \
@@ -664,12 +689,12 @@ LILY_API int lily_attention_decode4(const void* q, const void* kv, void* out, co
             launch_pdl(four::decode_mma_kernel<D>, dim3(plan.blocks), block, bytes, stream, a);                                                                    \
             JOIN(__nv_bfloat16, D);                                                                                                                                \
         } else if (dtype == kF32) {                                                                                                                                \
-            if (plan.heads == 4) launch_pdl(four::decode_cores_kernel<float, D, 4>, dim3(plan.blocks), block, 0, stream, a);                                       \
-            else launch_pdl(four::decode_cores_kernel<float, D, 8>, dim3(plan.blocks), block, 0, stream, a);                                                       \
+            if (plan.heads == 4) CORES(float, D, 4);                                                                                                               \
+            else CORES(float, D, 8);                                                                                                                               \
             JOIN(float, D);                                                                                                                                        \
         } else {                                                                                                                                                   \
-            if (plan.heads == 4) launch_pdl(four::decode_cores_kernel<__nv_bfloat16, D, 4>, dim3(plan.blocks), block, 0, stream, a);                               \
-            else launch_pdl(four::decode_cores_kernel<__nv_bfloat16, D, 8>, dim3(plan.blocks), block, 0, stream, a);                                               \
+            if (plan.heads == 4) CORES(__nv_bfloat16, D, 4);                                                                                                       \
+            else CORES(__nv_bfloat16, D, 8);                                                                                                                       \
             JOIN(__nv_bfloat16, D);                                                                                                                                \
         }                                                                                                                                                          \
     } while (0)
@@ -678,6 +703,7 @@ LILY_API int lily_attention_decode4(const void* q, const void* kv, void* out, co
     else if (d == 192) DECODE(192);
     else DECODE(256);
 #undef DECODE
+#undef CORES
 #undef JOIN
     LILY_CHECK_LAUNCH("attention_decode4 (join)");
     return 0;

@@ -217,25 +217,25 @@ __global__ void __launch_bounds__(32 * F32_WARPS) product_f32_kernel(const Produ
     for (int d = 0; d < DEPTH; ++d) {
         const int kt = kt0 + d * F32_WARPS;
         if (kt >= a.tiles) break;
-        const uint32_t words[4] = {ring[d].v.x, ring[d].v.y, ring[d].v.z, ring[d].v.w};
+        uint32_t words[4] = {ring[d].v.x, ring[d].v.y, ring[d].v.z, ring[d].v.w};
         float s[4], z[4];
 #pragma unroll
         for (int w = 0; w < 4; ++w) s[w] = __uint_as_float((uint32_t)ring[d].s[w] << 16), z[w] = __uint_as_float(0x4B000000u | ring[d].z[w]);      // (2^23 + zero point)
         ask(kt + DEPTH * F32_WARPS, ring[d]);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const int col = kt * 128 + 32 * w + 8 * t;
-            if (col >= a.k) continue;
+#pragma unroll 1
+        for (int col = kt * 128 + 8 * t; col < min(a.k, kt * 128 + 128); col += 32) {      // (a short loop: its words in turn)
             float c[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) c[e] = __uint_as_float((words[w] >> (4 * e) & 15u) | 0x4B000000u) - z[w];         // (2^23 + code: exact)
+            for (int e = 0; e < 8; ++e) c[e] = __uint_as_float((words[0] >> (4 * e) & 15u) | 0x4B000000u) - z[0];         // (2^23 + code: exact)
 #pragma unroll
             for (int i = 0; i < TOKENS; ++i) {
                 if (i >= a.m) break;
                 const float4 *p = reinterpret_cast<const float4*>((const float*)a.x + (size_t)i * a.k + col), x0 = p[0], x1 = p[1];
                 const float first = fmaf(c[0], x0.x, fmaf(c[1], x0.y, fmaf(c[2], x0.z, c[3] * x0.w))), second = fmaf(c[4], x1.x, fmaf(c[5], x1.y, fmaf(c[6], x1.z, c[7] * x1.w)));
-                total[i] = fmaf(s[w], first + second, total[i]);
+                total[i] = fmaf(s[0], first + second, total[i]);
             }
+#pragma unroll
+            for (int w = 0; w < 3; ++w) words[w] = words[w + 1], s[w] = s[w + 1], z[w] = z[w + 1];
         }
     }
     }
