@@ -7,7 +7,9 @@ values at 1; page 0 is never handed out) and one block table per live request.  
 head is a contiguous ``[page_size, head_dim]`` tile.  Where the values have a head size of their own the tensor is
 ``[layers, pages + 1, kv_heads * page_size * (head_dim + v_head_dim)]``: a page's keys ``[kv_heads, page_size, head_dim]``
 followed by its values ``[kv_heads, page_size, v_head_dim]`` (the first form is this one with equal sizes); where the
-values are columns of the key rows themselves (``CacheNeed.values_in_keys``) a page is its keys alone.
+values are columns of the key rows themselves (``CacheNeed.values_in_keys``) a page is its keys alone.  Where a group holds them in
+four bits (``CacheNeed.four_bits``) the tensor is uint8 ``[layers, pages + 1, kv_heads, 2, page_size (head_dim / 2 + head_dim / 16)]``: codes, then
+two bfloat16 numbers for each position and 64 features.
 
 A request takes a slot when it is opened, grows page by page as its tokens arrive (all
 groups together, or not at all: ``OutOfPages``), gives pages of windowed groups back as the
@@ -46,7 +48,14 @@ class CacheGroup:
 def bytes_per_token(groups: Sequence[Tuple[CacheNeed, int]], dtype: torch.dtype) -> int:
     """Bytes of keys and values one token takes over all layers (model_runner.py:160-164)."""
     item = torch.empty((), dtype=dtype).element_size()
-    return sum(need.kv_heads * (need.head_dim + value_columns(need)) * layers * item for need, layers in groups)
+    return sum(need.kv_heads * layers * (four_bit_bytes(need) if need.four_bits else (need.head_dim + value_columns(need)) * item) for need, layers in groups)
+
+
+def four_bit_bytes(need: CacheNeed) -> int:
+    """Bytes of a position's key and value of one head in four bits."""
+    if need.window or need.values_in_keys or need.v_head_dim not in (None, need.head_dim) or need.head_dim % 64 or not 64 <= need.head_dim <= 256:
+        raise ValueError(f"four bits hold all keys and values of 64, 128, 192 or 256 features, not {need}")
+    return 2 * (need.head_dim // 2 + need.head_dim // 16)
 
 
 def value_columns(need: CacheNeed) -> int:
@@ -77,7 +86,9 @@ class KVCacheManager:
                 same = need.v_head_dim in (None, need.head_dim) and not need.values_in_keys
                 shape = (2, need.kv_heads, page_size, need.head_dim) if same else \
                     (need.kv_heads * page_size * (need.head_dim + value_columns(need)),)
-                data = torch.zeros((layers, num_pages + 1, *shape), dtype=dtype, device=device)
+                if need.four_bits:
+                    shape = (need.kv_heads, 2, page_size * four_bit_bytes(need) // 2)
+                data = torch.zeros((layers, num_pages + 1, *shape), dtype=torch.uint8 if need.four_bits else dtype, device=device)
             self.groups.append(CacheGroup(need, layers, GroupTables(num_pages, page_size, need.window, need.keep_first), data))
         self.state_needs = list(states)
         # states of one kind lie in one tensor [of that kind, slots, ...], so that a request's rows of all of them are zeroed at once

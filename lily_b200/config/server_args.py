@@ -1,9 +1,9 @@
 """Runtime arguments: every knob is a dataclass field with a matching ``--flag``.
 
 Names, meanings and defaults are those of CodeMan62/lily's lily/server_args.py:17-174
-for the fields this engine has (one GPU, no server, no quantization, no speculative
+for the fields this engine has (one GPU, no server, no speculative
 decoding); ``page_size`` is this engine's own (the reference's pool is token-granular,
-lily/mem_cache/allocator.py:37-38).
+lily/mem_cache/allocator.py:37-38), and so are ``kv_cache_dtype`` and ``quantization_group``.
 """
 
 from __future__ import annotations
@@ -21,6 +21,9 @@ class ServerArgs:
     model_path: str = ""
     dtype: str = "auto"                       # auto | bfloat16 | float32
     context_length: Optional[int] = None      # overrides max_position_embeddings
+    quantization: Optional[str] = None        # int4: the matrices of attention and gated feed-forwards are held in four bits (quantised while they are loaded)
+    quantization_group: int = 128             # columns that share a scale: 32, 64 or 128
+    kv_cache_dtype: str = "auto"              # int4: keys and values are cached in four bits; auto: in dtype
 
     # Memory
     mem_fraction_static: Optional[float] = None   # share of device memory for weights + KV pool
@@ -50,6 +53,12 @@ class ServerArgs:
             raise ValueError(f"Unknown schedule policy {self.schedule_policy!r}")
         if self.dtype not in ("auto", "bfloat16", "float32"):
             raise ValueError(f"Unknown dtype {self.dtype!r}; this engine serves bfloat16 and float32")
+        if self.quantization not in (None, "int4"):
+            raise ValueError(f"Unknown quantization {self.quantization!r}; this engine holds matrices in dtype or int4")
+        if self.quantization_group not in (32, 64, 128):
+            raise ValueError(f"quantization_group = {self.quantization_group!r}: 32, 64 or 128 columns share a scale")
+        if self.kv_cache_dtype not in ("auto", "int4"):
+            raise ValueError(f"Unknown kv_cache_dtype {self.kv_cache_dtype!r}; keys and values are cached in dtype (auto) or int4")
         if self.page_size < 1 or self.page_size & (self.page_size - 1):
             raise ValueError("page_size must be a power of two")
         for name in ("max_prefill_tokens", "chunked_prefill_size"):

@@ -24,6 +24,7 @@ constexpr int OPERAND = STEP / 2;                        // columns of tensor me
 constexpr int OPERANDS = 4;                              // at most
 constexpr int GROUPS = 2, WORKERS = 4, THREADS = 32 * (2 + GROUPS * WORKERS);      // groups of warps that take steps in turn, a warp a quarter of the rows
 constexpr int MOST_TOKENS = 256, MOST_SPLITS = 8;
+constexpr int MOST_BYTES = 225 * 1024;                   // of shared memory
 constexpr uint32_t SPIN_LIMIT = 1u << 17;                // polls of up to ten microseconds each: a second before a wait gives up
 
 __device__ int g_status = 0;                             // 0; else (code << 24 | block) of the first wait that gave up
@@ -85,7 +86,7 @@ __global__ void __launch_bounds__(THREADS, 2) product_many_kernel(const __grid_c
     unsigned char* smem = smem_raw + (-tc5::smem_u32(smem_raw) & 1023u);      // (an offset, so that it stays an address of shared memory)
     __shared__ __align__(8) uint64_t bars[2 * 8 + 2 * OPERANDS + 1];
     __shared__ uint32_t tmem_s;
-    __shared__ int lost_s, given_up_s;                   // a wait of this block ran out, of another one of the cluster
+    __shared__ int lost_s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = blockIdx.x % a.splits, row_tile = blockIdx.x / a.splits, token0 = blockIdx.y * a.tokens;
     const int kt0 = (int)((long long)a.tiles * rank / a.splits), steps = (int)((long long)a.tiles * (rank + 1) / a.splits) - kt0;
@@ -97,7 +98,7 @@ __global__ void __launch_bounds__(THREADS, 2) product_many_kernel(const __grid_c
     const uint32_t columns = a.columns;
 
     if (threadIdx.x == 0) {
-        lost_s = given_up_s = 0;
+        lost_s = 0;
         for (int s = 0; s < a.stages; ++s) {
             tc5::mbar_init(full0 + 8 * s, 1);
             tc5::mbar_init(empty0 + 8 * s, 1);
@@ -257,13 +258,15 @@ __global__ void __launch_bounds__(THREADS, 2) product_many_kernel(const __grid_c
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(columns) : "memory");
     }
     const auto cluster = cooperative_groups::this_cluster();
-    if (a.splits > 1) {
-        cluster.sync();
-        if (lost_s && threadIdx.x < a.splits) *cluster.map_shared_rank(&given_up_s, threadIdx.x) = 1;
-        cluster.sync();
-    }
+    if (a.splits > 1) cluster.sync();
     const float* sums = reinterpret_cast<const float*>(smem);
-    const bool given_up = lost_s || given_up_s;
+    bool given_up = lost_s;                              // a wait of this block ran out, or of another one of the cluster
+    if (a.splits > 1) {
+        int theirs = 0;
+#pragma unroll
+        for (int z = 0; z < MOST_SPLITS; ++z) theirs |= *cluster.map_shared_rank(&lost_s, min(z, a.splits - 1));
+        given_up = given_up || theirs;
+    }
     for (int i = threadIdx.x; i < (a.tokens - rank + a.splits - 1) / a.splits * ROWS; i += THREADS) {
         const int token = rank + i / ROWS * a.splits, r = i % ROWS, row = row_tile * ROWS + r, y = token0 + token;
         if (y >= a.m || row >= a.n) continue;
@@ -334,7 +337,8 @@ LILY_API int lily_linear4_many(const void* x, const void* codes, const void* sca
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     LILY_REQUIRE(rc == CUDA_SUCCESS && w_rc == CUDA_SUCCESS, "linear4: tensor map: errors %d, %d", (int)rc, (int)w_rc);
     auto kernel = group == 128 ? product_many_kernel<1> : group == 64 ? product_many_kernel<2> : product_many_kernel<4>;
-    LILY_REQUIRE(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess, "linear4: cannot get %d bytes of shared memory", bytes);
+    // (to one number, whatever the call needs: another thread's launch may lie between)
+    LILY_REQUIRE(bytes <= MOST_BYTES && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST_BYTES) == cudaSuccess, "linear4: cannot get %d bytes of shared memory", bytes);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(row_tiles * a.splits, token_tiles);
     cfg.blockDim = dim3(THREADS);

@@ -454,7 +454,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     bfloat16: up to 16 rows this package's kernel that streams the weights (``few_rows_take``), else cuBLAS, both with
     float32 accumulation; ``out_dtype=float32`` keeps the accumulator's precision (used for the logits).
     ``weight`` is at rest: the kernels for few rows (as ``linear_split`` and ``swiglu_skinny``) read its first tiles while the kernel
-    launched before may still run, so it must not be what that kernel of this package writes."""
+    launched before may still run, so it must not be what that kernel of this package writes.  A ``Weight4`` goes to ``linear4``."""
+    if isinstance(weight, Weight4):
+        return linear4(x, weight, bias if bias is None or x.dtype == torch.bfloat16 else bias.float(), out_dtype)
     _dev(x, weight, bias)
     m, k = x.shape
     n = weight.shape[0]
@@ -591,7 +593,7 @@ def linear_auto(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     """The product in whichever form is fastest for the shape: float32 partial sums from
     ``linear_split`` for a few tokens, else ``linear``'s [M, N].  For producers whose consumer is
     one of the kernels that take either form."""
-    if bias is None:
+    if bias is None and not isinstance(weight, Weight4):
         parts = linear_split(x, weight)
         if parts is not None:
             return parts
@@ -1397,7 +1399,7 @@ def weights4(w: Weight4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     if dtype not in (torch.float32, torch.bfloat16):
         raise KernelError(f"weights4: float32 or bfloat16, not {dtype}")
     out = (_module or _faces()).weights4(*w, dtype == torch.float32)
-    launches["count"] += 1
+    launches["count"] += 2                                       # the numbers; what lets them be a product's weights at once
     return out
 
 
@@ -1472,14 +1474,32 @@ def attention_decode4(q: torch.Tensor, kv_layer: torch.Tensor, block_table: torc
     return out
 
 
+class Prefill4Plan(NamedTuple):
+    """How portions over a cache held in four bits are cut: tiles of ``rows`` new tokens (``prefill_tiles``), and the pages that they see."""
+
+    rows: int
+    tile_req: torch.Tensor
+    tile_start: torch.Tensor
+    pages: int                    # of all portions
+    width: int                    # of the longest
+
+
+def plan_prefill4(dtype: torch.dtype, d: int, page_size: int, h_prefix_lens: Sequence[int], h_new_lens: Sequence[int], device) -> Prefill4Plan:
+    """The plan of ``attention_prefill4`` for portions of these lengths; a step's layers share one."""
+    pages = [-(-(p + n) // page_size) if n else 0 for p, n in zip(h_prefix_lens, h_new_lens)]
+    rows = prefill_tile_rows(dtype, d, page_size, sum(h_new_lens))
+    return Prefill4Plan(rows, *prefill_tiles(h_prefix_lens, h_new_lens, 0, rows, device), sum(pages), max(pages, default=0))
+
+
 def attention_prefill4(q: torch.Tensor, kv_layer: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor, prefix_lens: torch.Tensor, h_prefix_lens: Sequence[int],
-                       h_new_lens: Sequence[int], nq: int, nkv: int, d: int, page_size: int, scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                       h_new_lens: Sequence[int], nq: int, nkv: int, d: int, page_size: int, scale: float, out: Optional[torch.Tensor] = None,
+                       plan: Optional[Prefill4Plan] = None) -> torch.Tensor:
     """Causal attention of prompt portions over a cache held in four bits: each request's new tokens (rows ``cu_seqlens`` of ``q`` [tokens, nq * d]) over its cached prefix and themselves, whose keys are in
-    the cache already.  ``h_prefix_lens``, ``h_new_lens``: the lengths on the host, by which the work is cut.  The pages that the portions see are brought to numbers of ``q``'s dtype first, and
-    ``attention_prefill`` reads those."""
+    the cache already.  ``h_prefix_lens``, ``h_new_lens``: the lengths on the host, by which the work is cut (``plan``: ``plan_prefill4`` of them, made here where not given).  The pages that the
+    portions see are brought to numbers of ``q``'s dtype first, and ``attention_prefill`` reads those.  Rows of ``out`` that no portion has stay as they are."""
     _dev(q, kv_layer, block_table, cu_seqlens, prefix_lens, out)
     requests = len(h_new_lens)
-    if nkv < 1 or nq < 1 or nq % nkv or page_size < 1 or len(h_prefix_lens) != requests or any(int(n) < 0 or int(p) < 0 for n, p in zip(h_new_lens, h_prefix_lens)):
+    if nkv < 1 or nq < 1 or nq % nkv or page_size < 1 or len(h_prefix_lens) != requests or any(n < 0 or p < 0 for n, p in zip(h_new_lens, h_prefix_lens)):
         raise KernelError(f"attention_prefill4: portions of {tuple(h_new_lens)} behind {tuple(h_prefix_lens)}, {nq} query heads over {nkv} kv heads")
     if kv_layer.dtype != torch.uint8 or tuple(kv_layer.shape[1:]) != cache4_shape(nkv, page_size, d):
         raise KernelError(f"attention_prefill4: a cache layer is uint8 [pages, {', '.join(map(str, cache4_shape(nkv, page_size, d)))}], got {kv_layer.dtype} {tuple(kv_layer.shape)}")
@@ -1488,23 +1508,21 @@ def attention_prefill4(q: torch.Tensor, kv_layer: torch.Tensor, block_table: tor
         raise KernelError(f"attention_prefill4: queries are [tokens, {nq * d}], got {tuple(q.shape)} for {tokens} tokens")
     if cu_seqlens.numel() != requests + 1 or prefix_lens.numel() != requests or block_table.dim() != 2 or block_table.shape[0] != requests:
         raise KernelError(f"attention_prefill4: {requests} portions have a prefix and a row of the block table each and {requests + 1} offsets")
-    pages = [-(-(p + n) // page_size) if n else 0 for p, n in zip(h_prefix_lens, h_new_lens)]
-    if max(pages, default=0) > block_table.shape[1]:
-        raise KernelError(f"attention_prefill4: {max(pages)} pages of a request; the block table holds {block_table.shape[1]}")
     if out is None:
         out = torch.empty_like(q)
     elif out.shape != q.shape or out.dtype != q.dtype:
         raise KernelError("attention_prefill4: out has the shape and dtype of q")
     if tokens == 0:
         return out
-    width = max(pages)
-    values = torch.empty((sum(pages), 2, nkv, page_size, d), dtype=q.dtype, device=q.device)
-    table = torch.zeros((requests, width), dtype=torch.int32, device=q.device)
+    if plan is None:
+        plan = plan_prefill4(q.dtype, d, page_size, h_prefix_lens, h_new_lens, q.device)
+    if plan.width > block_table.shape[1]:
+        raise KernelError(f"attention_prefill4: {plan.width} pages of a request; the block table holds {block_table.shape[1]}")
+    values = torch.empty((plan.pages, 2, nkv, page_size, d), dtype=q.dtype, device=q.device)
+    table = torch.zeros((requests, plan.width), dtype=torch.int32, device=q.device)
     _call("lily_cache4_values", _p(kv_layer), kv_layer.shape[0], _i32(block_table, "block_table"), requests, block_table.shape[1], _p(values), _dt(q), nkv, d, page_size,
-          _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens"), _p(table), width, values.shape[0], _stream())
-    rows = prefill_tile_rows(q.dtype, d, page_size, tokens)
-    tile_req, tile_start = prefill_tiles(h_prefix_lens, h_new_lens, 0, rows, q.device)
-    attention_prefill(q, values, table, cu_seqlens, prefix_lens, tile_req, tile_start, out, nq, nkv, d, page_size, scale, tile_rows=rows)
+          _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens"), _p(table), plan.width, plan.pages, _stream())
+    attention_prefill(q, values, table, cu_seqlens, prefix_lens, plan.tile_req, plan.tile_start, out, nq, nkv, d, page_size, scale, tile_rows=plan.rows)
     return out
 
 

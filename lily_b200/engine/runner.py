@@ -206,7 +206,8 @@ class ModelRunner:
         if args.random_seed is not None:
             torch.manual_seed(args.random_seed)
         ctx = BuildContext(device=self.device, dtype=self.dtype, ops=ops, page_size=self.page_size,
-                           max_position=self.context_len)
+                           max_position=self.context_len, weight_group=args.quantization_group if args.quantization else None,
+                           cache4=args.kv_cache_dtype == "int4")
         t0 = time.time()
         self.model = AssembledModel(spec, ctx)
         moved = load_model_weights(self.model, source, self.dtype, self.device)

@@ -67,7 +67,7 @@ class AssembledModel:
                         raise ValueError(f"schedule position {pos} reads the cache of position {entry.reads}, "
                                          f"whose mixer {k} has none")
                     other = owners[k].cache_need()
-                    if (other.kv_heads, other.head_dim, other.v_head_dim) != (need.kv_heads, need.head_dim, need.v_head_dim):
+                    if (other.kv_heads, other.head_dim, other.v_head_dim, other.four_bits) != (need.kv_heads, need.head_dim, need.v_head_dim, need.four_bits):
                         raise ValueError(f"schedule position {pos} cannot read a cache of another shape")
                     caches.append((lent[0], lent[1], False))
                 else:
@@ -153,9 +153,10 @@ class AssembledModel:
         def visit(obj):
             nonlocal total
             for v in vars(obj).values():
-                if isinstance(v, torch.Tensor) and v.data_ptr() not in seen and not getattr(v, "_is_table", False):
-                    seen.add(v.data_ptr())
-                    total += v.numel() * v.element_size()
+                for t in v if isinstance(v, tuple) else (v,):              # (a matrix held in four bits is a tuple of its tensors and sizes)
+                    if isinstance(t, torch.Tensor) and t.data_ptr() not in seen and not getattr(t, "_is_table", False):
+                        seen.add(t.data_ptr())
+                        total += t.numel() * t.element_size()
             for inner in getattr(obj, "parts", ()) if isinstance(obj, FeedForward) else ():
                 visit(inner)                              # a feed-forward put together from others
         visit(self)

@@ -10,7 +10,8 @@ output projection, W_g reading the mixer's input; or one gate a head, ``head_gat
 matrix), keys and values of another run's cache (``own_kv`` False), q and k heads brought to unit root mean square without a
 gain (``qk_gain`` False; a rotation leaves a head's root mean square as it is, so it does not matter which of the two comes
 first), rotation of interleaved pairs (the rows of the q and k projections
-are reordered once at load time, see ``rope.pairing_order``), and the checkpoint's own tensor names.  How a step's attention is cut (key ranges, kernel forms, tile
+are reordered once at load time, see ``rope.pairing_order``), and the checkpoint's own tensor names.  With ``BuildContext.weight_group`` the matrices are held in four bits (``ops.Weight4``), with ``BuildContext.cache4`` the keys and values
+are.  How a step's attention is cut (key ranges, kernel forms, tile
 lists) is this part's own plan, made once a step from the batch's host fields by asking the kernels
 (``ops.plan_decode_attention``, ``ops.prefill_tile_rows``, ``ops.prefill_tiles``); the step function
 knows nothing of it.  Sizes, eps, scale, window and the position encoding are
@@ -99,6 +100,14 @@ class AttentionPlan:
 
 
 @dataclass
+class FourBitPlan:
+    """The same over a cache held in four bits: floats of scratch the decode rows want, and how the portions are cut (``ops.plan_prefill4``)."""
+
+    scratch_floats: int
+    portions: Any
+
+
+@dataclass
 class LayerCache:
     """The cache one run of a mixer reads and writes: its group and its layer's pages."""
 
@@ -133,6 +142,11 @@ class Attention(Mixer):
         self.row = None                       # columns of the product where its rows go on behind the heads
         if spec.conv_taps < 0 or (spec.conv_taps and spec.bias):
             raise ValueError("the short convolution has at least one tap and comes without biases")
+        if ctx.cache4 and (spec.window or spec.softcap or spec.sink or spec.talk or spec.v_norm or spec.v_share or spec.conv_taps or spec.head_gate or not spec.own_kv
+                           or spec.value_dim != spec.head_dim or spec.head_dim % 64 or spec.head_dim > 256):
+            raise ValueError("a cache held in four bits serves attention over all keys of 64, 128, 192 or 256 features, without cap, sink, convolution or shared, mixed or normed values")
+        if ctx.weight_group and (spec.hidden_size % ctx.weight_group or spec.num_heads * spec.value_dim % ctx.weight_group):
+            raise ValueError(f"matrices of {spec.hidden_size} and {spec.num_heads * spec.value_dim} columns do not come in groups of {ctx.weight_group}")
         self.conv_w = None
 
     @property
@@ -144,7 +158,7 @@ class Attention(Mixer):
     def cache_need(self) -> CacheNeed:
         s = self.spec
         return CacheNeed(s.num_kv_heads, s.head_dim, s.window, None if s.value_dim == s.head_dim else s.value_dim,
-                         keep_first=int(s.keep_first) if s.window else 0)
+                         keep_first=int(s.keep_first) if s.window else 0, four_bits=self.ctx.cache4)
 
     def state_need(self) -> Optional[StateNeed]:
         s = self.spec
@@ -235,6 +249,10 @@ class Attention(Mixer):
             self.k_gain = get(f"{p}.{s.name('k_norm')}")
             if self.q_gain.dtype != self.k_gain.dtype:
                 self.q_gain, self.k_gain = self.q_gain.float(), self.k_gain.float()
+        if self.ctx.weight_group:
+            for name in ("w_qkv", "w_o", "w_g"):
+                if getattr(self, name) is not None:
+                    setattr(self, name, self.ctx.ops.quantize_weight4(getattr(self, name), self.ctx.weight_group))
 
     # ---- one step ----------------------------------------------------------------
 
@@ -280,7 +298,35 @@ class Attention(Mixer):
             return AttentionPlan(decode, rows, tiles)
         return batch.plan(key, make)
 
+    def _forward_four_bits(self, x, batch, cache: LayerCache, write_cache: bool):
+        """One step over a cache held in four bits: norm + rotation + write, attention of the rows with one token and of the portions."""
+        s, ops, page, nd = self.spec, self.ctx.ops, self.ctx.page_size, batch.num_decode
+        if not write_cache:
+            raise ValueError("a cache held in four bits is read by the run that writes it")
+        table = batch.block_tables[cache.group]
+
+        def make(b):
+            floats = ops.decode4_scratch_floats(nd, s.num_heads, s.num_kv_heads, s.head_dim, b.max_decode_len, page, x.dtype) if nd else 0
+            portions = ops.plan_prefill4(x.dtype, s.head_dim, page, b.h_prefix_lens[nd:], b.h_new_lens[nd:], b.token_ids.device) if b.num_requests > nd else None
+            return FourBitPlan(floats, portions)
+        plan = batch.plan(("attention4", cache.group, s.num_heads, s.num_kv_heads, s.head_dim, x.dtype, page), make)
+        cos, sin = self.position.tables() if self.position is not None else (None, None)
+        q = ops.qk_norm_rope_write4(ops.linear(x, self.w_qkv, self.b_qkv), self.q_gain, self.k_gain, s.norm_eps, cos, sin, batch.positions, batch.token_req, table, cache.data,
+                                    s.num_heads, s.num_kv_heads, s.head_dim, self.position.rotary_dim if self.position is not None else 0, page)
+        out = torch.empty_like(q)
+        if nd:
+            ops.attention_decode4(q[:nd], cache.data, table[:nd], batch.seq_lens[:nd], batch.max_decode_len, s.num_heads, s.num_kv_heads, s.head_dim, page, self.scale,
+                                  out[:nd], batch.workspace.floats("attention_decode4", plan.scratch_floats))
+        if batch.num_requests > nd:
+            ops.attention_prefill4(q, cache.data, table[nd:], batch.cu_seqlens[nd:], batch.prefix_lens[nd:], batch.h_prefix_lens[nd:], batch.h_new_lens[nd:], s.num_heads,
+                                   s.num_kv_heads, s.head_dim, page, self.scale, out, plan.portions)
+        if s.out_gate:
+            ops.sigmoid_gate(out, ops.linear_auto(x, self.w_g))
+        return ops.linear_auto(out, self.w_o, self.b_o)
+
     def forward(self, x, batch, cache: LayerCache, state=None, write_cache: bool = True):
+        if self.ctx.cache4:
+            return self._forward_four_bits(x, batch, cache, write_cache)
         s, ops = self.spec, self.ctx.ops
         page = self.ctx.page_size
         dv = s.value_dim

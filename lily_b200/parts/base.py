@@ -79,6 +79,7 @@ class CacheNeed:
     values_in_keys: bool = False         # the values are columns of the key rows themselves (a cached latent that serves
                                          # as both): a page holds keys only
     keep_first: int = 0                  # with a window: the request's first positions stay visible (and cached) for good
+    four_bits: bool = False              # keys and values are held in four bits (``ops.cache4_shape``)
 
 
 @dataclass(frozen=True)
@@ -101,6 +102,8 @@ class BuildContext:
     ops: Any                           # lily_b200.csrc.ops (the kernels), or a stand-in in CPU tests
     page_size: int = 64
     max_position: int = 4096           # positions the position tables must cover
+    weight_group: Optional[int] = None # columns that share a scale where matrices are held in four bits (attention, gated feed-forwards); None: they are held in ``dtype``
+    cache4: bool = False               # keys and values are cached in four bits
 
 
 class Part:

@@ -9,6 +9,7 @@ few tokens the tcgen05 kernel applies SiLU*mul in its epilogue, so the ``[tokens
 intermediate never reaches memory.  Otherwise gate rows come first, then up rows.  For up to 8
 tokens (decode) one weight-streaming kernel forms both sums and SiLU*mul from either layout; the
 reference streams these products through its own kernel as well (lily/csrc/bf16_skinny.cu:45-96).
+With ``BuildContext.weight_group`` both matrices are held in four bits (``ops.Weight4``), gate rows ahead of up rows.
 """
 
 from __future__ import annotations
@@ -44,6 +45,9 @@ class SwiGLU(FeedForward):
         self.w_gate_up = None
         self.w_down = None
         self.block = None          # rows of gate / up alternate in runs of this many (None: all gate, then all up)
+        self.four_bits = bool(ctx.weight_group)
+        if self.four_bits and (spec.hidden_size % ctx.weight_group or spec.intermediate_size % ctx.weight_group):
+            raise ValueError(f"matrices of {spec.hidden_size} and {spec.intermediate_size} columns do not come in groups of {ctx.weight_group}")
 
     def tensors(self) -> Dict[str, TensorSpec]:
         h, i, p = self.spec.hidden_size, self.spec.intermediate_size, self.prefix
@@ -57,7 +61,7 @@ class SwiGLU(FeedForward):
         gate = get(f"{p}.{name('gate')}")
         h = self.spec.hidden_size
         self.w_gate_up = torch.empty((2 * i, h), dtype=gate.dtype, device=gate.device)
-        self.block = b = self.ctx.ops.gate_up_interleave(gate.dtype, i)
+        self.block = b = None if self.four_bits else self.ctx.ops.gate_up_interleave(gate.dtype, i)
         if b:
             runs = self.w_gate_up.view(i // b, 2, b, h)
             runs[:, 0].copy_(gate.view(i // b, b, h))
@@ -68,6 +72,9 @@ class SwiGLU(FeedForward):
             del gate
             self.w_gate_up[i:].copy_(get(f"{p}.{name('up')}"))
         self.w_down = get(f"{p}.{name('down')}").contiguous()
+        if self.four_bits:
+            self.w_gate_up = self.ctx.ops.quantize_weight4(self.w_gate_up, self.ctx.weight_group)
+            self.w_down = self.ctx.ops.quantize_weight4(self.w_down, self.ctx.weight_group)
 
     def forward(self, x, batch):
         ops = self.ctx.ops
@@ -75,7 +82,9 @@ class SwiGLU(FeedForward):
         how = {} if self.spec.activation == "silu" else {"activation": self.spec.activation}
         if self.spec.activation == "swish_clamped":
             how.update(limit=self.spec.limit, alpha=self.spec.alpha)
-        if ops.swiglu_skinny_need(x.shape[0], self.spec.intermediate_size, self.spec.hidden_size, x.dtype, self.block) is not None:
+        if self.four_bits:
+            act = ops.silu_mul(product(x, self.w_gate_up), x.dtype, **how)
+        elif ops.swiglu_skinny_need(x.shape[0], self.spec.intermediate_size, self.spec.hidden_size, x.dtype, self.block) is not None:
             # a few tokens: one kernel streams the fused matrix and applies the activation and the product to its own sums
             act = ops.swiglu_skinny(x, self.w_gate_up, self.block, **how)
         elif self.block and ops.gate_up_fused_pays(x.shape[0], self.w_gate_up.shape[0]) and ops.gemm_tc_takes(x, self.w_gate_up):
