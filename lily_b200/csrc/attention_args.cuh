@@ -1,6 +1,8 @@
 // Arguments shared by the attention kernels (CUDA-core and tensor-core files).
 #pragma once
 
+#include "common.cuh"
+
 namespace lily {
 
 struct AttnArgs {
@@ -57,6 +59,16 @@ struct AttnArgs {
     int score_stride, max_len;      // ... and the places a row has at most
     int stages;               // decode, tensor-core kernel: key/value tiles a block keeps in shared memory (0: the default, 2;
                               // 3: two blocks a SM instead of three, each with two tiles in flight; head sizes up to 128)
+    const unsigned* spans;    // mma.sync prefill: not null where queries and keys are half-precision numbers times powers of two (below)
 };
+
+// Queries and keys in half precision, whose eleven bits hold what four-bit codes, their steps and lowest values make of a key (bfloat16's eight would round it).  `spans` holds the largest magnitude of
+// the queries and of the keys, as bits of float32; each is multiplied by the power of two that brings the largest to 2^13 .. 2^14, so that nothing overflows and 2^-28 of it is still a normal number.
+__device__ __forceinline__ int span_exponent(unsigned bits) { return min(max(267 - (int)(bits >> 23), 1), 253); }
+__device__ __forceinline__ float span_multiplier(unsigned bits) { return __uint_as_float((unsigned)span_exponent(bits) << 23); }
+// What a product of such numbers is to be multiplied by.
+__device__ __forceinline__ float span_factor(const unsigned* spans) {
+    return __uint_as_float((unsigned)(254 - span_exponent(spans[0])) << 23) * __uint_as_float((unsigned)(254 - span_exponent(spans[1])) << 23);
+}
 
 }  // namespace lily

@@ -89,6 +89,10 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, u
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
                  : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
 }
+__device__ __forceinline__ void mma_half(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -131,7 +135,7 @@ constexpr int TILE_POLLS = 1 << 22;
 template <int D, int STAGES>
 __host__ __device__ constexpr size_t tma_bytes() { return 1024 + 2 * (size_t)STAGES * BN * D * 2 + 16 * D * 2 + 2 * D * 2; }
 
-template <int D, bool DECODE, int STAGES, bool CLUSTER, bool TMA>
+template <int D, bool DECODE, int STAGES, bool CLUSTER, bool TMA, bool HALF = false>
 __global__ void __launch_bounds__(THREADS, D <= 128 ? 3 : 1)
 attention_mma_kernel(const AttnArgs a, const int page_shift, const __grid_constant__ CUtensorMap map_kv) {
     constexpr int CH = D / 8;                  // 16-byte pieces per row
@@ -528,7 +532,7 @@ attention_mma_kernel(const AttnArgs a, const int page_shift, const __grid_consta
     // (the hardware's tanh, relative error about 2^-11: the weights are rounded to bfloat16 for the p . v product anyway;
     // the float32 path is the CUDA-core kernel's, which calls tanhf)
     const float cap = a.softcap, cap_in = cap > 0.f ? a.scale / cap : 0.f;
-    const float sl2 = (cap > 0.f ? 1.f : a.scale) * 1.4426950408889634f;
+    const float sl2 = (cap > 0.f ? 1.f : a.scale) * 1.4426950408889634f * (HALF ? span_factor(a.spans) : 1.f);
     auto tanh_fast = [](float v) { float r; asm("tanh.approx.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; };
 
     for (int t = 0; t < ntiles; ++t) {
@@ -585,8 +589,13 @@ attention_mma_kernel(const AttnArgs a, const int page_shift, const __grid_consta
                 uint32_t b0, b1, b2, b3;
                 const int krow = key0 + jp * 16 + (lane & 7) + ((lane >> 4) << 3);
                 ldmatrix_x4(smem_u32(kt + piece(krow, kk * 2 + ((lane >> 3) & 1))), b0, b1, b2, b3);
-                mma_bf16(s[2 * jp], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], b0, b1);
-                mma_bf16(s[2 * jp + 1], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], b2, b3);
+                if constexpr (HALF) {
+                    mma_half(s[2 * jp], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], b0, b1);
+                    mma_half(s[2 * jp + 1], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], b2, b3);
+                } else {
+                    mma_bf16(s[2 * jp], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], b0, b1);
+                    mma_bf16(s[2 * jp + 1], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], b2, b3);
+                }
             }
         }
 
@@ -868,7 +877,7 @@ static bool cluster_enabled() {
 }
 
 // Returns 0 on success, and in `merged` whether the kernel itself merged the splits into `out`.
-template <int D, bool DECODE, int STAGES, bool TMA = false>
+template <int D, bool DECODE, int STAGES, bool TMA = false, bool HALF = false>
 static int launch(const AttnArgs& a, dim3 grid, int page_shift, cudaStream_t stream, bool* merged, const CUtensorMap& map = CUtensorMap{}) {
     size_t smem = TMA ? tma_bytes<D, STAGES>() : stage_bytes<D, STAGES>(DECODE);
     // clusters pay when all of them are resident at once; over several rounds of blocks their placement costs
@@ -901,7 +910,7 @@ static int launch(const AttnArgs& a, dim3 grid, int page_shift, cudaStream_t str
             return 0;
         }
     }
-    auto kern = attention_mma_kernel<D, DECODE, STAGES, false, TMA>;
+    auto kern = attention_mma_kernel<D, DECODE, STAGES, false, TMA, HALF>;
     static bool configured = false;
     if (!configured) {
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -980,6 +989,13 @@ static int dispatch(const AttnArgs& a, dim3 grid, cudaStream_t stream, bool* mer
         if (a.d == 64) return launch<64, DECODE, DECODE ? 3 : 2>(a, grid, page_shift, stream, merged);
         return launch<128, DECODE, DECODE ? 3 : 2>(a, grid, page_shift, stream, merged);
     }
+    if constexpr (!DECODE)
+        if (a.spans) switch (a.d) {
+            case 64: return launch<64, false, 2, false, true>(a, grid, page_shift, stream, merged);
+            case 128: return launch<128, false, 2, false, true>(a, grid, page_shift, stream, merged);
+            case 192: return launch<192, false, 2, false, true>(a, grid, page_shift, stream, merged);
+            case 256: return launch<256, false, 2, false, true>(a, grid, page_shift, stream, merged);
+        }
     switch (a.d) {
         case 64: return launch<64, DECODE, ST>(a, grid, page_shift, stream, merged);
         case 128: return launch<128, DECODE, ST>(a, grid, page_shift, stream, merged);
@@ -1028,6 +1044,23 @@ LILY_API int lily_attention_prefill_mma(const void* q, const void* kv, void* out
     a.splits = 1; a.nq = nq; a.nkv = nkv; a.d = d; a.page_size = page_size; a.window = window; a.scale = scale;
     a.softcap = softcap; a.sink = sink; a.v_shift = v_shift;
     a.keep_first = window > 0 && keep_first > 0 ? keep_first : 0;
+    bool merged = false;
+    int rc = mma::dispatch<false>(a, dim3(tiles, nq), stream, &merged);
+    if (rc) return rc;
+    LILY_CHECK_LAUNCH("attention_prefill_mma");
+    return 0;
+}
+
+// The same over queries and keys in half precision (values stay bfloat16); spans: attention_args.cuh.
+LILY_API int lily_attention_prefill_mma_half(const void* q, const void* kv, void* out, const int* block_table, int bt_stride, const int* cu_seqlens, const int* prefix_lens, const int* tile_req,
+                                             const int* tile_start, int tiles, int nq, int nkv, int d, int page_size, float scale, const unsigned* spans, cudaStream_t stream) {
+    if (tiles == 0) return 0;
+    LILY_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0 && spans != nullptr, "attention_prefill: %d query heads over %d kv heads", nq, nkv);
+    LILY_REQUIRE(nq <= 65535 && page_size > 0, "attention_prefill: nq=%d page_size=%d", nq, page_size);
+    AttnArgs a{};
+    a.q = q; a.kv = kv; a.out = out; a.block_table = block_table; a.bt_stride = bt_stride; a.spans = spans;
+    a.cu_seqlens = cu_seqlens; a.prefix_lens = prefix_lens; a.tile_req = tile_req; a.tile_start = tile_start;
+    a.splits = 1; a.nq = nq; a.nkv = nkv; a.d = d; a.page_size = page_size; a.scale = scale;
     bool merged = false;
     int rc = mma::dispatch<false>(a, dim3(tiles, nq), stream, &merged);
     if (rc) return rc;

@@ -33,6 +33,7 @@
 // former and the latter are not stored.  Every wait on an mbarrier is bounded; a wait that runs out
 // sets a status word (lily_attention_tc_status), the roles leave their loops and the block frees
 // its tensor memory.
+#include "attention_args.cuh"
 #include "common.cuh"
 #include "tcgen05.cuh"
 
@@ -103,6 +104,7 @@ struct Params {
     float scale_log2;                     // softmax scale times log2(e) (log2(e) alone under a cap)
     int sink;                             // the softmax's denominator holds one more unit: a key of score 0 without a value
     size_t plane;                         // elements between the planes of `out` (grid z): plane z weighs the values of kv head (own + z) % nkv
+    const unsigned* spans;                // not null where queries and keys are half-precision numbers times powers of two (attention_args.cuh)
     float cap, cap_in;                    // cap > 0: scores become cap * tanh(score * cap_in), cap_in = scale / cap
 };
 
@@ -180,6 +182,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     // q and the cache come from the kernels before this one
     pdl_wait();
     pdl_launch_dependents();
+    const float scale_log2 = p.spans ? p.scale_log2 * span_factor(p.spans) : p.scale_log2;
 
     // the tiles were listed in order of position: the last ones, which see the most keys, go first
     const int tile = p.tiles - 1 - (int)blockIdx.y;
@@ -242,7 +245,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     } else if (warp == 1) {
         if (lane == 0) {
             // kind::f16: float32 accumulator, bfloat16 a and b, n = 128, m = 128; bit 16 makes b MN-major
-            const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+            const uint32_t idesc_s = (1u << 4) | (p.spans ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
             const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
             bool ok = mbar_wait(q_full, 0, abort_flag, 3);
             auto scores = [&](int i) {                   // S_i = Q K_i^T into accumulator i % 2
@@ -376,15 +379,15 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             const float m_new = fmaxf(m_used, row_max);
             if (j == 0) {
                 m_used = m_new;
-                if (p.sink && part == 0) l = ex2(-m_used * p.scale_log2);       // the unit, against the row's maximum
+                if (p.sink && part == 0) l = ex2(-m_used * scale_log2);       // the unit, against the row's maximum
             } else {
-                const bool grow = (m_new - m_used) * p.scale_log2 > GROW_LOG2;      // also when m_used is -inf
+                const bool grow = (m_new - m_used) * scale_log2 > GROW_LOG2;      // also when m_used is -inf
                 if (__any_sync(0xffffffffu, grow)) {
                     // O must hold every product up to tile j - 1 before its rows are rescaled
                     ok = mbar_wait(pv_done + 8 * ((j - 1) & 1), (uint32_t)(((j - 1) >> 1) & 1), abort_flag, 8);
                     if (!ok) break;
                     tc_fence_after();
-                    const float alpha = grow ? ex2((m_used - m_new) * p.scale_log2) : 1.f;
+                    const float alpha = grow ? ex2((m_used - m_new) * scale_log2) : 1.f;
                     if (grow) m_used = m_new;
                     l *= alpha;
 #pragma unroll 1
@@ -400,11 +403,11 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 }
             }
             FA_TOC(22 + (part & 1), row == 0);
-            const float mb = (m_used == -INFINITY ? 0.f : m_used) * p.scale_log2;
+            const float mb = (m_used == -INFINITY ? 0.f : m_used) * scale_log2;
             float sum4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < COLS; ++c) {
-                s[c] = ex2(fmaf(s[c], p.scale_log2, -mb));
+                s[c] = ex2(fmaf(s[c], scale_log2, -mb));
                 sum4[c & 3] += s[c];
             }
             l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
@@ -551,6 +554,7 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
 
     pdl_wait();
     pdl_launch_dependents();
+    const float scale_log2 = p.spans ? p.scale_log2 * span_factor(p.spans) : p.scale_log2;
 
     const int tile = p.tiles - 1 - (int)blockIdx.y;             // the last tiles, which see the most keys, go first
     const int head0 = blockIdx.x * NH2;
@@ -611,7 +615,7 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+            const uint32_t idesc_s = (1u << 4) | (p.spans ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
             const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
             bool ok = mbar_wait(q_full, 0, abort_flag, 3);
             auto scores = [&](int h, int i) {            // S_h(i) = Q_h K_i^T; the second head hands the K stage back
@@ -727,15 +731,15 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
             FA_TOC(10 + h, row == 0);
             if (j == 0) {
                 m_used = m_new;
-                if (p.sink) l = ex2(-m_used * p.scale_log2);
+                if (p.sink) l = ex2(-m_used * scale_log2);
             } else {
-                const bool grow = (m_new - m_used) * p.scale_log2 > GROW_LOG2;      // also when m_used is -inf
+                const bool grow = (m_new - m_used) * scale_log2 > GROW_LOG2;      // also when m_used is -inf
                 if (__any_sync(0xffffffffu, grow)) {
                     // O must hold every product up to tile j - 1 before its rows are rescaled
                     ok = mbar_wait(pv_done + 8 * h, (uint32_t)((j - 1) & 1), abort_flag, 8);
                     if (!ok) break;
                     tc_fence_after();
-                    const float alpha = grow ? ex2((m_used - m_new) * p.scale_log2) : 1.f;
+                    const float alpha = grow ? ex2((m_used - m_new) * scale_log2) : 1.f;
                     if (grow) m_used = m_new;
                     l *= alpha;
 #pragma unroll 1
@@ -752,7 +756,7 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
             }
             // second pass: P = exp2(s * scale - max) as bfloat16 pairs over the first 64 columns of S.  Piece c
             // lands on columns [16 c, 16 c + 16), all of them in pieces that this pass has read already.
-            const float mb = (m_used == -INFINITY ? 0.f : m_used) * p.scale_log2;
+            const float mb = (m_used == -INFINITY ? 0.f : m_used) * scale_log2;
             float sum4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
             for (int c = 0; c < BKV / 32; ++c) {
@@ -773,7 +777,7 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
                 }
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                    s[e] = ex2(fmaf(s[e], p.scale_log2, -mb));
+                    s[e] = ex2(fmaf(s[e], scale_log2, -mb));
                     sum4[e & 3] += s[e];
                 }
                 uint32_t packed[16];
@@ -872,16 +876,9 @@ LILY_API int lily_attention_tc_status() {
     return v;
 }
 
-// The arguments of lily_attention_prefill_mma with tiles of 128 rows, plus the number of pages of
-// the layer (`kv` is [num_pages, 2, nkv, page_size, d]) and of new tokens (`q` is [tokens, nq, d]);
-// heads_per_block 1 or 2 names the kernel, 0 leaves the choice to the launcher.  sink: the softmax's denominator holds one more
-// unit.  planes: plane z of `out` ([planes][tokens, nq, d]) holds every head's weights over the values of kv head (its own + z) % nkv,
-// all in one launch (2,000 tokens, 16 heads over 4 of 128: four launches of the mma.sync kernel 4 x 108 us, this one 112).
-LILY_API int lily_attention_prefill_tc(const void* q, const void* kv, void* out, const int* block_table, int bt_stride,
-                                       const int* cu_seqlens, const int* prefix_lens, const int* tile_req,
-                                       const int* tile_start, int tiles, int nq, int nkv, int d, int page_size, int window,
-                                       float scale, int tokens, int num_pages, int heads_per_block, float softcap,
-                                       int keep_first, int sink, int planes, cudaStream_t stream) {
+static int prefill_tc(const void* q, const void* kv, void* out, const int* block_table, int bt_stride, const int* cu_seqlens, const int* prefix_lens, const int* tile_req, const int* tile_start,
+                      int tiles, int nq, int nkv, int d, int page_size, int window, float scale, int tokens, int num_pages, int heads_per_block, float softcap, int keep_first, int sink, int planes,
+                      const unsigned* spans, cudaStream_t stream) {
     if (tiles == 0) return 0;
     LILY_REQUIRE(planes >= 1 && planes <= nkv, "attention_prefill_tc: %d planes of %d kv heads", planes, nkv);
     LILY_REQUIRE(lily_attention_prefill_tc_takes(d, page_size), "attention_prefill_tc: head size %d, page size %d (takes 64 or 128, and multiples of 64)",
@@ -913,6 +910,7 @@ LILY_API int lily_attention_prefill_tc(const void* q, const void* kv, void* out,
         LILY_REQUIRE(rc == CUDA_SUCCESS, "attention_prefill_tc: cuTensorMapEncodeTiled (cache) failed with %d", (int)rc);
     }
     fa::Params p{};
+    p.spans = spans;
     p.block_table = block_table; p.cu_seqlens = cu_seqlens; p.prefix_lens = prefix_lens; p.tile_req = tile_req;
     p.tile_start = tile_start; p.out = (__nv_bfloat16*)out; p.bt_stride = bt_stride; p.tiles = tiles; p.nq = nq; p.nkv = nkv;
     p.page_size = page_size; p.window = window; p.sink = sink; p.plane = (size_t)tokens * nq * d;
@@ -931,4 +929,26 @@ LILY_API int lily_attention_prefill_tc(const void* q, const void* kv, void* out,
     if (rc) return rc;
     LILY_CHECK_LAUNCH("attention_prefill_tc");
     return 0;
+}
+
+// The arguments of lily_attention_prefill_mma with tiles of 128 rows, plus the number of pages of
+// the layer (`kv` is [num_pages, 2, nkv, page_size, d]) and of new tokens (`q` is [tokens, nq, d]);
+// heads_per_block 1 or 2 names the kernel, 0 leaves the choice to the launcher.  sink: the softmax's denominator holds one more
+// unit.  planes: plane z of `out` ([planes][tokens, nq, d]) holds every head's weights over the values of kv head (its own + z) % nkv,
+// all in one launch (2,000 tokens, 16 heads over 4 of 128: four launches of the mma.sync kernel 4 x 108 us, this one 112).
+LILY_API int lily_attention_prefill_tc(const void* q, const void* kv, void* out, const int* block_table, int bt_stride,
+                                       const int* cu_seqlens, const int* prefix_lens, const int* tile_req,
+                                       const int* tile_start, int tiles, int nq, int nkv, int d, int page_size, int window,
+                                       float scale, int tokens, int num_pages, int heads_per_block, float softcap,
+                                       int keep_first, int sink, int planes, cudaStream_t stream) {
+    return prefill_tc(q, kv, out, block_table, bt_stride, cu_seqlens, prefix_lens, tile_req, tile_start, tiles, nq, nkv, d, page_size, window, scale, tokens, num_pages, heads_per_block, softcap,
+                      keep_first, sink, planes, nullptr, stream);
+}
+
+// The same over queries and keys in half precision (values stay bfloat16), without cap, window and sink; spans: attention_args.cuh.
+LILY_API int lily_attention_prefill_tc_half(const void* q, const void* kv, void* out, const int* block_table, int bt_stride, const int* cu_seqlens, const int* prefix_lens, const int* tile_req,
+                                            const int* tile_start, int tiles, int nq, int nkv, int d, int page_size, float scale, int tokens, int num_pages, const unsigned* spans,
+                                            cudaStream_t stream) {
+    LILY_REQUIRE(spans != nullptr, "attention_prefill_tc: half-precision queries come with their spans");
+    return prefill_tc(q, kv, out, block_table, bt_stride, cu_seqlens, prefix_lens, tile_req, tile_start, tiles, nq, nkv, d, page_size, 0, scale, tokens, num_pages, 0, 0.f, 0, 0, 1, spans, stream);
 }

@@ -9,7 +9,10 @@
 // A number next to the border of two codes is a whole step off where its last bit falls the other way, so a token's codes are made a function of its numbers
 // alone: the sum of squares is taken in 64 bits (squares of float32 numbers are exact there, and no order of adding them up shows in the root's 24 bits), and every other
 // operation is one IEEE operation, none contracted.  The same token gets the same codes in a prompt, alone, and from a statement in plain operations.
+#include "attention_args.cuh"
 #include "four.cuh"
+
+#include <cuda_fp16.h>
 
 namespace lily {
 namespace four {
@@ -50,6 +53,17 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
     *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+
+// Half-precision numbers where bfloat16 ones would lie.
+__device__ __forceinline__ void store_halves(void* p, const float (&v)[8], float by) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = __floats2half2_rn(v[2 * i] * by, v[2 * i + 1] * by);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 constexpr int WRITE_WARPS = 4;
@@ -262,10 +276,11 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) write_turned_kernel(const Wr
 
 // Pages as numbers, lowest + step code in one rounding: of every page that a block table names to [requests, width, 2, nkv, page_size, d] (``compact`` false), or of the pages
 // that portions of prompts see, one request's behind the other's, [pages, 2, nkv, page_size, d], with a block table of them and zeros behind a request's last place.
-// Eight threads a place and kind, each with the words that lie side by side, one a group.  grid (pages, requests, kv heads x 2)
+// Eight threads a place and kind, each with the words that lie side by side, one a group.  ``spans``: keys become half-precision numbers times a power of two (attention_args.cuh).
+// grid (pages, requests, kv heads x 2)
 template <typename T, int G>
 __global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__ kv, int pages, const int* __restrict__ block_table, int width, T* __restrict__ out, int nkv, int page_size,
-                                                     const int* __restrict__ cu, const int* __restrict__ prefix, int* __restrict__ table_out, int table_width, int most_pages) {
+                                                     const int* __restrict__ cu, const int* __restrict__ prefix, int* __restrict__ table_out, int table_width, int most_pages, const unsigned* __restrict__ spans) {
     constexpr int D = G * GROUP;
     __shared__ int sum_s[8];
     pdl_enter_small();
@@ -297,6 +312,8 @@ __global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__
     const uint32_t *words = reinterpret_cast<const uint32_t*>(rows), *held = reinterpret_cast<const uint32_t*>(rows + (size_t)page_size * (D / 2));
     T* dst = out + ((to * 2 + value) * nkv + head) * ((size_t)page_size * D);
     const int i8 = threadIdx.x & 7;
+    const bool halves = sizeof(T) == 2 && spans && !value;
+    const float by = halves ? span_multiplier(spans[1]) : 1.f;
 #pragma unroll 2
     for (int slot = threadIdx.x >> 3; slot < page_size; slot += 32) {
         uint32_t w[G], h[G];
@@ -310,9 +327,53 @@ __global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__
             float v[8];
 #pragma unroll
             for (int c = 0; c < 8; ++c) v[c] = slot < places ? fmaf((float)(w[e] >> (4 * c) & 15u), low(of), high(of)) : 0.f;
-            store8(dst + (size_t)slot * D + l * 8, v);
+            if (halves) store_halves(dst + (size_t)slot * D + l * 8, v, by);
+            else store8(dst + (size_t)slot * D + l * 8, v);
         }
     }
+}
+
+// The largest magnitudes of what portions attend with: of the queries (grid-wide, 16 bytes a thread), and a bound of the keys' from their steps and lowest values (lowest + 15 step, or lowest), as bits
+// that are compared as whole numbers.  What is no number counts for nothing.  blocks [0, query_blocks): queries; the others: a block a (page, request), all its heads
+__global__ void __launch_bounds__(256) spans_kernel(const __nv_bfloat16* __restrict__ q, size_t pieces, int query_blocks, const uint8_t* __restrict__ kv, int pages, const int* __restrict__ block_table,
+                                                    int width, int nkv, int d, int page_size, const int* __restrict__ cu, const int* __restrict__ prefix, int most, unsigned* __restrict__ spans) {
+    pdl_enter_small();
+    float m = 0.f;
+    auto take = [&](float v) {
+        v = fabsf(v);
+        if (v <= 3e38f) m = fmaxf(m, v);
+    };
+    const bool queries = (int)blockIdx.x < query_blocks;
+    if (queries) {
+        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (size_t)query_blocks * 256) {
+            const uint4 v = reinterpret_cast<const uint4*>(q)[i];
+            take(low(v.x)), take(high(v.x)), take(low(v.y)), take(high(v.y)), take(low(v.z)), take(high(v.z)), take(low(v.w)), take(high(v.w));
+        }
+    } else {
+        const int r = ((int)blockIdx.x - query_blocks) / most, at = ((int)blockIdx.x - query_blocks) % most, groups = d / GROUP;
+        const int total = cu[r + 1] > cu[r] ? prefix[r] + cu[r + 1] - cu[r] : 0, places = min(page_size, total - at * page_size);
+        if (places <= 0) return;
+        int page = at < width ? block_table[(size_t)r * width + at] : 0;
+        if ((unsigned)page >= (unsigned)pages) page = 0;
+        const size_t rows = (size_t)page_size * row_bytes(d);
+        for (int i = threadIdx.x; i < nkv * places * groups; i += 256) {
+            const int head = i / (places * groups), in = i - head * places * groups;
+            const uint32_t h = reinterpret_cast<const uint32_t*>(kv + ((size_t)page * nkv + head) * 2 * rows + (size_t)page_size * (d / 2))[in];
+            take(high(h)), take(fmaf(15.f, low(h), high(h)));
+        }
+    }
+    const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+    if ((threadIdx.x & 31) == 0 && bits) atomicMax(spans + (queries ? 0 : 1), bits);
+}
+
+// Queries in half precision.  A thread eight numbers.
+__global__ void __launch_bounds__(256) halves_kernel(const __nv_bfloat16* __restrict__ q, size_t pieces, __nv_bfloat16* __restrict__ out, const unsigned* __restrict__ spans) {
+    pdl_enter_small();
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= pieces) return;
+    float v[8];
+    load8(q + i * 8, v);
+    store_halves(out + i * 8, v, span_multiplier(spans[0]));
 }
 
 inline bool head_fits(int d) { return d >= GROUP && d <= 256 && d % GROUP == 0; }
@@ -364,10 +425,10 @@ LILY_API int lily_qk_norm_rope_write4(const void* qkv, int dtype, int ld, const 
     return 0;
 }
 
-// cu, prefix, table_out: null, or of a step's portions (offsets of their tokens, tokens cached ahead of them, a block table [requests, table_width] of the pages
+// spans: null, or the largest magnitudes of queries and keys, for keys in half precision (lily_spans4).  cu, prefix, table_out: null, or of a step's portions (offsets of their tokens, tokens cached ahead of them, a block table [requests, table_width] of the pages
 // written, of which there is room for `most_pages`).
 LILY_API int lily_cache4_values(const void* kv, int pages, const int* block_table, int requests, int width, void* out, int dtype, int nkv, int d, int page_size, const int* cu,
-                                const int* prefix, int* table_out, int table_width, int most_pages, cudaStream_t stream) {
+                                const int* prefix, int* table_out, int table_width, int most_pages, const unsigned* spans, cudaStream_t stream) {
     if (requests == 0 || width == 0) return 0;
     LILY_REQUIRE(four::head_fits(d), "cache4_values: heads of 64, 128, 192 or 256 features, not %d", d);
     LILY_REQUIRE(page_size > 0 && nkv > 0 && nkv <= 32767 && requests > 0 && requests <= 65535 && width > 0, "cache4_values: %d requests, %d kv heads, pages of %d places", requests, nkv, page_size);
@@ -375,7 +436,7 @@ LILY_API int lily_cache4_values(const void* kv, int pages, const int* block_tabl
     const dim3 grid(cu ? table_width : width, requests, 2 * nkv);
     if (grid.x == 0) return 0;
 #define VALUES(T, G) \
-    launch_pdl(four::values_kernel<T, G>, grid, dim3(256), 0, stream, (const uint8_t*)kv, pages, block_table, width, (T*)out, nkv, page_size, cu, prefix, table_out, table_width, most_pages)
+    launch_pdl(four::values_kernel<T, G>, grid, dim3(256), 0, stream, (const uint8_t*)kv, pages, block_table, width, (T*)out, nkv, page_size, cu, prefix, table_out, table_width, most_pages, spans)
 #define VALUES_OF(T)                 \
     do {                             \
         if (d == 64) VALUES(T, 1);   \
@@ -388,5 +449,22 @@ LILY_API int lily_cache4_values(const void* kv, int pages, const int* block_tabl
 #undef VALUES_OF
 #undef VALUES
     LILY_CHECK_LAUNCH("cache4_values");
+    return 0;
+}
+
+// What portions attend with in half precision: the largest magnitudes to `spans` (two words that are zero before), and the queries times a power of two to `out`.
+LILY_API int lily_spans4(const void* q, int tokens, int nq, const void* kv, int pages, const int* block_table, int requests, int width, int nkv, int d, int page_size, const int* cu, const int* prefix,
+                         int most_pages, unsigned* spans, void* out, cudaStream_t stream) {
+    if (tokens == 0 || requests == 0) return 0;
+    LILY_REQUIRE(four::head_fits(d) && page_size > 0 && nkv > 0 && nq > 0 && most_pages > 0 && (long long)requests * most_pages <= INT32_MAX / 2, "spans4: %d requests of up to %d pages", requests, most_pages);
+    LILY_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)kv) % 16 == 0, "spans4: tensors on boundaries of sixteen bytes");
+    const size_t pieces = (size_t)tokens * nq * (d / 8);
+    const int query_blocks = (int)min((size_t)(4 * sm_count()), (pieces + 255) / 256);
+    launch_pdl(four::spans_kernel, dim3(query_blocks + requests * most_pages), dim3(256), 0, stream, (const __nv_bfloat16*)q, pieces, query_blocks, (const uint8_t*)kv, pages, block_table, width, nkv, d,
+               page_size, cu, prefix, most_pages, spans);
+    LILY_CHECK_LAUNCH("spans4");
+    LILY_REQUIRE((pieces + 255) / 256 <= INT32_MAX, "spans4: %d tokens", tokens);
+    launch_pdl(four::halves_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, stream, (const __nv_bfloat16*)q, pieces, (__nv_bfloat16*)out, (const unsigned*)spans);
+    LILY_CHECK_LAUNCH("spans4");
     return 0;
 }

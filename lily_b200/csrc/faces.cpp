@@ -52,7 +52,7 @@ struct Entries {
     int (*weights4)(const void*, const void*, const void*, void*, int, int, int, int, void*);
     int (*write4)(const void*, int, int, const void*, const void*, int, double, const float*, const float*, int, const int*, int, const int*, const int*, int, int, void*, int, void*, int, int,
                   int, int, int, void*);
-    int (*values4)(const void*, int, const int*, int, int, void*, int, int, int, int, const int*, const int*, int*, int, int, void*);
+    int (*values4)(const void*, int, const int*, int, int, void*, int, int, int, int, const int*, const int*, int*, int, int, const unsigned*, void*);
     size_t (*decode4_floats)(int, int, int, int, int, int, int);
     int (*decode4)(const void*, const void*, void*, const int*, int, const int*, float*, int, int, int, int, int, int, int, float, int, void*);
 } entry;
@@ -496,7 +496,7 @@ PyObject* cache4_values(PyObject*, PyObject* const* p, Py_ssize_t count) {
         here({&kv, &table});
         Tensor out = at::empty({table.size(0), table.size(1), 2, (int64_t)nkv, (int64_t)page, (int64_t)d}, kv.options().dtype(wide ? at::kFloat : at::kBFloat16));
         done("lily_cache4_values", call(entry.values4, kv.const_data_ptr(), narrow(kv.size(0)), table.const_data_ptr<int>(), narrow(table.size(0)), narrow(table.size(1)), out.data_ptr(),
-                                        wide ? F32 : BF16, nkv, d, page, (const int*)nullptr, (const int*)nullptr, (int*)nullptr, 0, 0, stream()));
+                                        wide ? F32 : BF16, nkv, d, page, (const int*)nullptr, (const int*)nullptr, (int*)nullptr, 0, 0, (const unsigned*)nullptr, stream()));
         return THPVariable_Wrap(std::move(out));
     });
 }

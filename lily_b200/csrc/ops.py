@@ -101,7 +101,10 @@ _SIGNATURES = {
     "lily_argmax": [_vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_apply_penalties": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_top_logprobs": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
-    "lily_cache4_values": [_vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _vp],
+    "lily_cache4_values": [_vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _vp],
+    "lily_spans4": [_vp, _i, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp],
+    "lily_attention_prefill_tc_half": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _vp],
+    "lily_attention_prefill_mma_half": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp, _vp],
     "lily_linear4_status": [],
     "lily_sample": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
 }
@@ -1496,7 +1499,7 @@ def attention_prefill4(q: torch.Tensor, kv_layer: torch.Tensor, block_table: tor
                        plan: Optional[Prefill4Plan] = None) -> torch.Tensor:
     """Causal attention of prompt portions over a cache held in four bits: each request's new tokens (rows ``cu_seqlens`` of ``q`` [tokens, nq * d]) over its cached prefix and themselves, whose keys are in
     the cache already.  ``h_prefix_lens``, ``h_new_lens``: the lengths on the host, by which the work is cut (``plan``: ``plan_prefill4`` of them, made here where not given).  The pages that the
-    portions see are brought to numbers of ``q``'s dtype first, and ``attention_prefill`` reads those.  Rows of ``out`` that no portion has stay as they are."""
+    portions see are brought to numbers first, and the kernels of ``attention_prefill`` read those: float32, or values in bfloat16 with keys (and queries) in half precision, whose bits hold them.  Rows of ``out`` that no portion has stay as they are."""
     _dev(q, kv_layer, block_table, cu_seqlens, prefix_lens, out)
     requests = len(h_new_lens)
     if nkv < 1 or nq < 1 or nq % nkv or page_size < 1 or len(h_prefix_lens) != requests or any(n < 0 or p < 0 for n, p in zip(h_new_lens, h_prefix_lens)):
@@ -1518,11 +1521,28 @@ def attention_prefill4(q: torch.Tensor, kv_layer: torch.Tensor, block_table: tor
         plan = plan_prefill4(q.dtype, d, page_size, h_prefix_lens, h_new_lens, q.device)
     if plan.width > block_table.shape[1]:
         raise KernelError(f"attention_prefill4: {plan.width} pages of a request; the block table holds {block_table.shape[1]}")
+    if not 0 < scale < float("inf"):
+        raise KernelError(f"attention_prefill4: a scale of {scale}")
     values = torch.empty((plan.pages, 2, nkv, page_size, d), dtype=q.dtype, device=q.device)
-    table = torch.zeros((requests, plan.width), dtype=torch.int32, device=q.device)
+    words = torch.zeros((requests * plan.width + 2,), dtype=torch.int32, device=q.device)
+    spans, table = words[:2], words[2:].view(requests, plan.width)
+    # (the tensor-core kernels; others, of float32 and of pages that are no power of two, read the numbers themselves)
+    halves = uses_tensor_cores(q.dtype, d) and page_size & (page_size - 1) == 0
+    heads = q
+    if halves:
+        heads = torch.empty_like(q)
+        _call("lily_spans4", _p(q), q.shape[0], nq, _p(kv_layer), kv_layer.shape[0], _i32(block_table, "block_table"), requests, block_table.shape[1], nkv, d, page_size,
+              _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens"), plan.width, _p(spans), _p(heads), _stream())
     _call("lily_cache4_values", _p(kv_layer), kv_layer.shape[0], _i32(block_table, "block_table"), requests, block_table.shape[1], _p(values), _dt(q), nkv, d, page_size,
-          _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens"), _p(table), plan.width, plan.pages, _stream())
-    attention_prefill(q, values, table, cu_seqlens, prefix_lens, plan.tile_req, plan.tile_start, out, nq, nkv, d, page_size, scale, tile_rows=plan.rows)
+          _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens"), _p(table), plan.width, plan.pages, _p(spans) if halves else None, _stream())
+    if not halves:
+        attention_prefill(q, values, table, cu_seqlens, prefix_lens, plan.tile_req, plan.tile_start, out, nq, nkv, d, page_size, scale, tile_rows=plan.rows)
+        return out
+    common = (_p(heads), _p(values), _p(out), _p(table), plan.width, _p(cu_seqlens), _p(prefix_lens), _p(plan.tile_req), _p(plan.tile_start), plan.tile_req.numel(), nq, nkv, d, page_size, float(scale))
+    if plan.rows == int(library().lily_attention_prefill_tc_rows()):
+        _call("lily_attention_prefill_tc_half", *common, q.shape[0], plan.pages, _p(spans), _stream())
+    else:
+        _call("lily_attention_prefill_mma_half", *common, _p(spans), _stream())
     return out
 
 
