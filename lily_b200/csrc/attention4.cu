@@ -3,10 +3,12 @@
 // With x_jf = low_jg + step_jg c_jf (g the group of 64 features that f is in) a key's score and the output are
 //   q . k_j = sum_g step_jg (sum_f q_f c_jf) + low_jg sum_f q_f,
 //   o_f = sum_j (p_j step_jg) c_jf + sum_j p_j low_jg,
-// so codes go into tensor-core products as they are, 0..15 as bfloat16 numbers 128 + c, which cost one logical operation a pair and no conversion; steps meet the sums behind the
-// products (keys) or the weights ahead of them (values), and the 128 is taken off with sums of the queries and of the weights as they were rounded.
+// so codes go into tensor-core products as they are, 0..15, without a conversion.  Keys: four bits of a word, masked, are the half-precision number c 2^-24 (or 16 c 2^-24, which needs no shift either),
+// and products are exact; a head's queries are brought to 2^13 .. 2^14 by a power of two for it, so that they stay as they are.  Values: weights times steps may lie anywhere, which asks for bfloat16;
+// codes are numbers 16 + c there, and the 16 is taken off at the end with sums of the weights as they were rounded.  Steps meet the sums behind the products (keys) or the weights ahead of them (values).
 #include "four.cuh"
 #include "mma.cuh"
+#include <cuda_fp16.h>
 
 namespace lily {
 namespace four {
@@ -37,8 +39,15 @@ __device__ __forceinline__ int page_of(const DecodeArgs& a, int req, int j) {
 }
 // ---- bfloat16 on the tensor cores -------------------------------------------------------------------
 constexpr int KT = 32;                        // places a tile
-constexpr int WARPS = 4, STAGES = 2, BLOCKS = 2;      // warps a block, tiles in a warp's ring, blocks a SM
+constexpr int WARPS = 4, STAGES = 2;          // warps a block, tiles in a warp's ring
 constexpr int HEADS = 8;                      // query heads a block: the columns of a product
+
+// A pair's part ends where the warps of its block meet.  Where pairs are many, blocks are one warp, which meets nobody; their many parts would be slow to join where pairs are few, and heads above 128
+// have no registers for enough of them.  Measured with 32 query heads of 128 over 8, blocks of four warps (two a multiprocessor) against blocks of one (twelve): 32 rows of 1,024 places 18.3 us
+// against 18.7; 64 rows of 1,000 29.9 against 28, 128 of 500 38 against 29, 256 of 130 52 against 30.  (Heads of 256, 64 rows of 1,000: 50 against 59.)
+// Blocks of four warps (8 rows of 4,000 places, three a multiprocessor against two): heads of 64 have room for three, 12.9 us against 15.2; heads of 128 have not the registers, 20.6 against 18.8,
+// heads of 256 even less, 58 against 30.
+constexpr int blocks_a_sm(int d, int warps) { return warps == 1 ? 12 : d == 64 ? 3 : 2; }
 
 template <int D> struct Tile {
     static constexpr int G = D / GROUP, CODES = D / 2;
@@ -121,6 +130,14 @@ __device__ __forceinline__ uint32_t pair16(uint32_t w, int i) {
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(i == 0 ? w << 3 : w >> (4 * i - 3)), "r"(0x00780078u), "r"(0x41804180u));
     return r;
 }
+__device__ __forceinline__ uint32_t half_bits(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void mma_half(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 template <int N> __device__ __forceinline__ void words_of(const unsigned char* p, uint32_t (&w)[N]) {
     if constexpr (N % 4 == 0) {
 #pragma unroll
@@ -155,7 +172,7 @@ struct Cut {
 };
 
 // This block's share of the tiles, and where it begins.  Rows without places are zeroed on the way.
-template <typename T, int D>
+template <typename T, int D, int W>
 __device__ __forceinline__ void begin_share(const DecodeArgs& a, int pairs, int chunks, Place& at, int& share) {
     const int lane = threadIdx.x & 31;
     auto length = [&](int r) { return r < a.requests ? places_of(a, r) : 0; };
@@ -172,7 +189,7 @@ __device__ __forceinline__ void begin_share(const DecodeArgs& a, int pairs, int 
         for (unsigned without = __ballot_sync(0xffffffffu, r0 + lane < a.requests && n == 0); without; without &= without - 1) {
             const int r = r0 + __ffs(without) - 1;
             if (r % (int)gridDim.x == (int)blockIdx.x)
-                for (int i = threadIdx.x; i < a.nq * D; i += 32 * WARPS) ((T*)a.out)[(size_t)r * a.nq * D + i] = from_float<T>(0.f);
+                for (int i = threadIdx.x; i < a.nq * D; i += 32 * W) ((T*)a.out)[(size_t)r * a.nq * D + i] = from_float<T>(0.f);
         }
         if (found) continue;
         int run = own;                                                // of the requests up to this lane's
@@ -202,18 +219,18 @@ __device__ __forceinline__ void put4(__nv_bfloat16* to, float4 v) { *reinterpret
 
 // The warps' (max in units of log2, sum, output) of a pair's part, in shared memory, together: divided and rounded to the output where the whole pair was here (``alone``), else to
 // the part's slot.
-template <typename T, int D>
+template <typename T, int D, int W>
 __device__ __forceinline__ void end_part(const DecodeArgs& a, int req, int head0, int heads, bool alone, bool second, const float (*m_s)[HEADS], const float (*l_s)[HEADS], const float* o_s,
                                          int o_warp, int o_head) {
     const size_t part = 2 * (size_t)blockIdx.x + second;
-    for (int i = threadIdx.x; i < heads * (D / 4); i += 32 * WARPS) {
+    for (int i = threadIdx.x; i < heads * (D / 4); i += 32 * W) {
         const int h = i / (D / 4), f = 4 * (i - h * (D / 4));
         float m = -INFINITY, l = 0.f;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, m_s[w][h]);
+        for (int w = 0; w < W; ++w) m = fmaxf(m, m_s[w][h]);
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float by = m_s[w][h] == -INFINITY ? (l_s[w][h] == 0.f ? 0.f : 1.f) : ex2(m_s[w][h] - m);
             const float4 x = *reinterpret_cast<const float4*>(o_s + w * o_warp + h * o_head + f);
             if (by != 0.f) l = fmaf(by, l_s[w][h], l), v.x = fmaf(by, x.x, v.x), v.y = fmaf(by, x.y, v.y), v.z = fmaf(by, x.z, v.z), v.w = fmaf(by, x.w, v.w);
@@ -230,22 +247,22 @@ __device__ __forceinline__ void end_part(const DecodeArgs& a, int req, int head0
 
 // Keys on the rows of the products (16 of them), query heads on their eight columns: S^T = K q^T, O^T = V^T P^T.  The warps of a block take the tiles of its share in turn, each through
 // a ring of its own that runs on from one pair to the next; they meet where a pair's part ends.
-template <int D>
-__global__ void __launch_bounds__(32 * WARPS, BLOCKS) decode_mma_kernel(const DecodeArgs a) {
+template <int D, int W>
+__global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(const DecodeArgs a) {
     using S = Tile<D>;
     constexpr int G = S::G, LD = D + 4;
     extern __shared__ __align__(16) unsigned char ring_s[];
-    __shared__ float m_s[WARPS][HEADS], l_s[WARPS][HEADS];
+    __shared__ float m_s[W][HEADS], l_s[W][HEADS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int group = a.nq / a.nkv, chunks = (group + HEADS - 1) / HEADS, pairs = a.nkv * chunks;
     unsigned char* mine = ring_s + warp * STAGES * S::BYTES;
-    float* o_s = reinterpret_cast<float*>(ring_s + WARPS * STAGES * S::BYTES);      // [warps][heads][LD]
+    float* o_s = reinterpret_cast<float*>(ring_s + W * STAGES * S::BYTES);      // [warps][heads][LD]
     const uint32_t ring = mma16::smem_u32(mine);
     pdl_wait();
     pdl_launch_dependents();                                          // (the joining kernel may so read the lengths ahead of its own wait)
     Place at{};
     int share = 0;
-    begin_share<__nv_bfloat16, D>(a, pairs, chunks, at, share);
+    begin_share<__nv_bfloat16, D, W>(a, pairs, chunks, at, share);
     if (share == 0) return;
     // the tile to ask for next, the `asked`-th of the share: this warp's own are `warp` and every fourth behind it
     Place ahead = at;
@@ -260,8 +277,8 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) decode_mma_kernel(const De
             }
             fetch<D>(a, ahead, ring + issued % STAGES * S::BYTES);
             ++issued;
-            asked += WARPS;
-            ahead.tile += WARPS;
+            asked += W;
+            ahead.tile += W;
         }
         mma16::cp_async_commit();
     };
@@ -269,186 +286,207 @@ __global__ void __launch_bounds__(32 * WARPS, BLOCKS) decode_mma_kernel(const De
     for (int s = 0; s < STAGES - 1; ++s) ask();
     int next = warp, used = 0;                                        // this warp's next tile of the share; tiles taken out of the ring
     for (int began = 0; began < share;) {
-    const int req = at.req, head0 = at.kvh * group + at.chunk * HEADS, heads = min(HEADS, group - at.chunk * HEADS), ends = min(share, began + at.tiles - at.tile);
-    // the queries as the products' second operand, in the order of the keys' words, and their sums
-    uint32_t q[G][2][4];
-    float sums[G];
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-        float both = 0.f;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (g < heads) v = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + ((size_t)req * a.nq + head0 + g) * D + 64 * j + 32 * h + 8 * t);
-            if (a.scale < 0.f) v.x ^= 0x80008000u, v.y ^= 0x80008000u, v.z ^= 0x80008000u, v.w ^= 0x80008000u;
-            both += low(v.x) + high(v.x) + low(v.y) + high(v.y) + low(v.z) + high(v.z) + low(v.w) + high(v.w);
-            q[j][h][0] = __byte_perm(v.x, v.z, 0x5410);               // features 0 and 4, 1 and 5, 2 and 6, 3 and 7 of the eight
-            q[j][h][1] = __byte_perm(v.x, v.z, 0x7632);
-            q[j][h][2] = __byte_perm(v.y, v.w, 0x5410);
-            q[j][h][3] = __byte_perm(v.y, v.w, 0x7632);
-        }
-        both += __shfl_xor_sync(0xffffffffu, both, 1);
-        sums[j] = both + __shfl_xor_sync(0xffffffffu, both, 2);
-    }
-    float qs[G][2];                                                   // of heads 2 t and 2 t + 1
-#pragma unroll
-    for (int j = 0; j < G; ++j) qs[j][0] = __shfl_sync(0xffffffffu, sums[j], 8 * t), qs[j][1] = __shfl_sync(0xffffffffu, sums[j], 8 * t + 4);
-    const float scale = fabsf(a.scale) * LOG2E;
-    float o[G][4][4], most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, ones[G][4], lows[G][2];      // (scores and their maximum are kept unscaled)
-#pragma unroll
-    for (int j = 0; j < G; ++j) {
-        lows[j][0] = lows[j][1] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            ones[j][e] = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[j][i][e] = 0.f;
-        }
-    }
-    const uint32_t one[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-    const float margin = 8.f / scale;                                 // in units of scores
-    auto work = [&](const unsigned char* tile, const int left) {
-        float s[2][4];                                                // scores of keys g and g + 8, heads 2 t and 2 t + 1
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-            const int row = 16 * mt + g;
-            uint32_t w0[2 * G], w1[2 * G], h0[G], h1[G];
-            words_of<2 * G>(tile + S::KEYS + row * S::KEY_ROW + t * 8 * G, w0);
-            words_of<2 * G>(tile + S::KEYS + (row + 8) * S::KEY_ROW + t * 8 * G, w1);
-            words_of<G>(tile + S::KEY_HELD + row * 4 * G, h0);
-            words_of<G>(tile + S::KEY_HELD + (row + 8) * 4 * G, h1);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[mt][e] = 0.f;
+        const int req = at.req, head0 = at.kvh * group + at.chunk * HEADS, heads = min(HEADS, group - at.chunk * HEADS), ends = min(share, began + at.tiles - at.tile);
+        // the queries as the products' second operand, in the order of the keys' words, and their sums: brought by a power of two to 2^13 .. 2^14, a sixteenth of it where codes come as 16 c
+        uint32_t q[G][2][4];
+        float qs[G][2], scale[2], margin[2];                              // of heads 2 t and 2 t + 1: the sums and the softmax's factor in units of the products; 2^8 of weight as a difference of scores
+        {
+            uint4 v[G][2];
+            float most_q = 0.f, sums[G];
 #pragma unroll
             for (int j = 0; j < G; ++j) {
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                sums[j] = 0.f;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t x = w0[2 * j + h], y = w1[2 * j + h];
-                    const uint32_t a0[4] = {pair(x, 0), pair(y, 0), pair(x, 1), pair(y, 1)}, a1[4] = {pair(x, 2), pair(y, 2), pair(x, 3), pair(y, 3)};
-                    mma16::mma_bf16(c, a0, q[j][h][0], q[j][h][1]);
-                    mma16::mma_bf16(c, a1, q[j][h][2], q[j][h][3]);
+                    uint4& x = v[j][h];
+                    x = make_uint4(0, 0, 0, 0);
+                    if (g < heads) x = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + ((size_t)req * a.nq + head0 + g) * D + 64 * j + 32 * h + 8 * t);
+                    if (a.scale < 0.f) x.x ^= 0x80008000u, x.y ^= 0x80008000u, x.z ^= 0x80008000u, x.w ^= 0x80008000u;
+                    for (const uint32_t w : {x.x, x.y, x.z, x.w}) sums[j] += low(w) + high(w), most_q = fmaxf(most_q, fmaxf(fabsf(low(w)), fabsf(high(w))));
                 }
-                const float s0 = low(h0[j]), s1 = low(h1[j]), b0 = fmaf(s0, -128.f, high(h0[j])), b1 = fmaf(s1, -128.f, high(h1[j]));
-                s[mt][0] = fmaf(s0, c[0], fmaf(b0, qs[j][0], s[mt][0]));
-                s[mt][1] = fmaf(s0, c[1], fmaf(b0, qs[j][1], s[mt][1]));
-                s[mt][2] = fmaf(s1, c[2], fmaf(b1, qs[j][0], s[mt][2]));
-                s[mt][3] = fmaf(s1, c[3], fmaf(b1, qs[j][1], s[mt][3]));
+                sums[j] += __shfl_xor_sync(0xffffffffu, sums[j], 1);
+                sums[j] += __shfl_xor_sync(0xffffffffu, sums[j], 2);
             }
-            if (left < KT) {
-                if (row >= left) s[mt][0] = s[mt][1] = -INFINITY;
-                if (row + 8 >= left) s[mt][2] = s[mt][3] = -INFINITY;
+            most_q = fmaxf(most_q, __shfl_xor_sync(0xffffffffu, most_q, 1));
+            most_q = fmaxf(most_q, __shfl_xor_sync(0xffffffffu, most_q, 2));
+            const int exponent = (int)(__float_as_uint(most_q) >> 23);    // 2^(exponent - 127) is the largest query's size
+            const float by = __uint_as_float((uint32_t)min(max(267 - exponent, 1), 253) << 23), unit = by * 0x1p-24f;      // a product is the sum over queries times codes in units of 2^24 / by
+#pragma unroll
+            for (int j = 0; j < G; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {                             // features 0 and 4, 1 and 5, 2 and 6, 3 and 7 of the eight
+                    const uint4 x = v[j][h];
+                    const float less = by * 0.0625f;
+                    q[j][h][0] = half_bits(low(x.x) * by, low(x.z) * by);
+                    q[j][h][1] = half_bits(high(x.x) * less, high(x.z) * less);
+                    q[j][h][2] = half_bits(low(x.y) * by, low(x.w) * by);
+                    q[j][h][3] = half_bits(high(x.y) * less, high(x.w) * less);
+                }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float u = __shfl_sync(0xffffffffu, unit, 8 * t + 4 * e);
+#pragma unroll
+                for (int j = 0; j < G; ++j) qs[j][e] = __shfl_sync(0xffffffffu, sums[j], 8 * t + 4 * e) * u;
+                scale[e] = fabsf(a.scale) * LOG2E / u;
+                margin[e] = 8.f / scale[e];
             }
         }
-        float m0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])), m1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
-        // The maximum moves only where a score is 2^8 times its weight ahead (weights of up to 256 are as good as ones of up to 1), which after the first tile is rare.
-        if (__any_sync(0xffffffffu, m0 > most[0] + margin || m1 > most[1] + margin)) {
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, x));
-                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, x));
-            }
-            m0 = fmaxf(m0, most[0]);
-            m1 = fmaxf(m1, most[1]);
-            const float f0 = m0 == most[0] ? 1.f : ex2((most[0] - m0) * scale), f1 = m1 == most[1] ? 1.f : ex2((most[1] - m1) * scale);
-            most[0] = m0;
-            most[1] = m1;
-            sum[0] *= f0;
-            sum[1] *= f1;
-#pragma unroll
-            for (int j = 0; j < G; ++j) {
-                lows[j][0] *= f0;
-                lows[j][1] *= f1;
-                ones[j][0] *= f0;
-                ones[j][1] *= f1;
-#pragma unroll
-                for (int n = 0; n < 4; ++n) o[j][n][0] *= f0, o[j][n][1] *= f1, o[j][n][2] *= f0, o[j][n][3] *= f1;
-            }
-        }
-        const float z0 = most[0] == -INFINITY ? 0.f : -most[0] * scale, z1 = most[1] == -INFINITY ? 0.f : -most[1] * scale;      // (nobody has a score yet)
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt) {
-            const int row = 16 * mt;
-            float p[4];
-            p[0] = ex2(fmaf(s[mt][0], scale, z0));
-            p[1] = ex2(fmaf(s[mt][1], scale, z1));
-            p[2] = ex2(fmaf(s[mt][2], scale, z0));
-            p[3] = ex2(fmaf(s[mt][3], scale, z1));
-            sum[0] += p[0] + p[2];
-            sum[1] += p[1] + p[3];
-            uint32_t w[4][G], h0[G], h1[G];
-            words_of<G>(tile + S::VALUE_HELD + (row + g) * 4 * G, h0);
-            words_of<G>(tile + S::VALUE_HELD + (row + g + 8) * 4 * G, h1);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) words_of<G>(tile + S::VALUES + (row + 2 * t + (e & 1) + (e >> 1) * 8) * S::VALUE_ROW + g * 4 * G, w[e]);
-#pragma unroll
-            for (int j = 0; j < G; ++j) {
-                if (left < KT) {                                      // (what stands behind the last place may be no number)
-                    if (row + g >= left) h0[j] = 0;
-                    if (row + g + 8 >= left) h1[j] = 0;
-                }
-                lows[j][0] = fmaf(p[2], high(h1[j]), fmaf(p[0], high(h0[j]), lows[j][0]));
-                lows[j][1] = fmaf(p[3], high(h1[j]), fmaf(p[1], high(h0[j]), lows[j][1]));
-                // weights times steps, rounded to bfloat16 as the second operand asks
-                const float s0 = low(h0[j]), s1 = low(h1[j]);
-                const uint32_t b0 = transposed(bits(__floats2bfloat162_rn(p[0] * s0, p[1] * s0))), b1 = transposed(bits(__floats2bfloat162_rn(p[2] * s1, p[3] * s1)));
-                mma16::mma_bf16(ones[j], one, b0, b1);
-                const uint32_t x0 = __byte_perm(w[0][j], w[1][j], 0x5410), x1 = __byte_perm(w[0][j], w[1][j], 0x7632);
-                const uint32_t y0 = __byte_perm(w[2][j], w[3][j], 0x5410), y1 = __byte_perm(w[2][j], w[3][j], 0x7632);
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {                         // features 8 g + 2 n (rows g) and 8 g + 2 n + 1 (rows g + 8) of the group
-                    const uint32_t x = n < 2 ? x0 : x1, y = n < 2 ? y0 : y1;
-                    const int i0 = 2 * (n & 1);
-                    const uint32_t av[4] = {pair16(x, i0), pair16(x, i0 + 1), pair16(y, i0), pair16(y, i0 + 1)};
-                    mma16::mma_bf16(o[j][n], av, b0, b1);
-                }
-            }
-        }
-    };
-    for (; next < ends; next += WARPS, ++used) {
-        ask();
-        mma16::cp_async_wait<STAGES - 1>();
-        __syncwarp();
-        work(mine + used % STAGES * S::BYTES, at.places - (at.tile + next - began) * KT);
-        __syncwarp();
-    }
-    // the warps' sums together: finished, where the whole pair was here; else to the part's slot
-#pragma unroll
-    for (int x = 4; x < 32; x <<= 1) {
-        sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], x);
-        sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], x);
+        float o[G][4][4], most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, ones[G][4], lows[G][2];      // (scores and their maximum are kept unscaled)
 #pragma unroll
         for (int j = 0; j < G; ++j) {
-            lows[j][0] += __shfl_xor_sync(0xffffffffu, lows[j][0], x);
-            lows[j][1] += __shfl_xor_sync(0xffffffffu, lows[j][1], x);
+            lows[j][0] = lows[j][1] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                ones[j][e] = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[j][i][e] = 0.f;
+            }
         }
-    }
+        const uint32_t one[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        auto work = [&](const unsigned char* tile, const int left) {
+            float s[2][4];                                                // scores of keys g and g + 8, heads 2 t and 2 t + 1
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const int h = 2 * t + e;
-        if (h >= heads) continue;
-        if (g == 0) m_s[warp][h] = most[e] * scale, l_s[warp][h] = sum[e];
+            for (int mt = 0; mt < 2; ++mt) {
+                const int row = 16 * mt + g;
+                uint32_t w0[2 * G], w1[2 * G], h0[G], h1[G];
+                words_of<2 * G>(tile + S::KEYS + row * S::KEY_ROW + t * 8 * G, w0);
+                words_of<2 * G>(tile + S::KEYS + (row + 8) * S::KEY_ROW + t * 8 * G, w1);
+                words_of<G>(tile + S::KEY_HELD + row * 4 * G, h0);
+                words_of<G>(tile + S::KEY_HELD + (row + 8) * 4 * G, h1);
 #pragma unroll
-        for (int j = 0; j < G; ++j) {                                 // features 64 j + 8 g + (0..7)
-            float4* to = reinterpret_cast<float4*>(o_s + (warp * HEADS + h) * LD + 64 * j + 8 * g);
+                for (int e = 0; e < 4; ++e) s[mt][e] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                to[i] = make_float4(fmaf(-16.f, ones[j][e], o[j][2 * i][e] + lows[j][e]), fmaf(-16.f, ones[j][e], o[j][2 * i][e + 2] + lows[j][e]),
-                                    fmaf(-16.f, ones[j][e], o[j][2 * i + 1][e] + lows[j][e]), fmaf(-16.f, ones[j][e], o[j][2 * i + 1][e + 2] + lows[j][e]));
+                for (int j = 0; j < G; ++j) {
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t x = w0[2 * j + h], y = w1[2 * j + h], x8 = x >> 8, y8 = y >> 8;
+                        const uint32_t a0[4] = {x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u}, a1[4] = {x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u};
+                        mma_half(c, a0, q[j][h][0], q[j][h][1]);
+                        mma_half(c, a1, q[j][h][2], q[j][h][3]);
+                    }
+                    const float s0 = low(h0[j]), s1 = low(h1[j]), b0 = high(h0[j]), b1 = high(h1[j]);
+                    s[mt][0] = fmaf(s0, c[0], fmaf(b0, qs[j][0], s[mt][0]));
+                    s[mt][1] = fmaf(s0, c[1], fmaf(b0, qs[j][1], s[mt][1]));
+                    s[mt][2] = fmaf(s1, c[2], fmaf(b1, qs[j][0], s[mt][2]));
+                    s[mt][3] = fmaf(s1, c[3], fmaf(b1, qs[j][1], s[mt][3]));
+                }
+                if (left < KT) {
+                    if (row >= left) s[mt][0] = s[mt][1] = -INFINITY;
+                    if (row + 8 >= left) s[mt][2] = s[mt][3] = -INFINITY;
+                }
+            }
+            float m0 = fmaxf(fmaxf(s[0][0], s[0][2]), fmaxf(s[1][0], s[1][2])), m1 = fmaxf(fmaxf(s[0][1], s[0][3]), fmaxf(s[1][1], s[1][3]));
+            // The maximum moves only where a score is 2^8 times its weight ahead (weights of up to 256 are as good as ones of up to 1), which after the first tile is rare.
+            if (__any_sync(0xffffffffu, m0 > most[0] + margin[0] || m1 > most[1] + margin[1])) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) {
+                    m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, x));
+                    m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, x));
+                }
+                m0 = fmaxf(m0, most[0]);
+                m1 = fmaxf(m1, most[1]);
+                const float f0 = m0 == most[0] ? 1.f : ex2((most[0] - m0) * scale[0]), f1 = m1 == most[1] ? 1.f : ex2((most[1] - m1) * scale[1]);
+                most[0] = m0;
+                most[1] = m1;
+                sum[0] *= f0;
+                sum[1] *= f1;
+#pragma unroll
+                for (int j = 0; j < G; ++j) {
+                    lows[j][0] *= f0;
+                    lows[j][1] *= f1;
+                    ones[j][0] *= f0;
+                    ones[j][1] *= f1;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) o[j][n][0] *= f0, o[j][n][1] *= f1, o[j][n][2] *= f0, o[j][n][3] *= f1;
+                }
+            }
+            const float z0 = most[0] == -INFINITY ? 0.f : most[0], z1 = most[1] == -INFINITY ? 0.f : most[1];      // (nobody has a score yet)
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+                const int row = 16 * mt;
+                float p[4];
+                p[0] = ex2((s[mt][0] - z0) * scale[0]);      // (the difference first: a product of large scores would be off by more than it)
+                p[1] = ex2((s[mt][1] - z1) * scale[1]);
+                p[2] = ex2((s[mt][2] - z0) * scale[0]);
+                p[3] = ex2((s[mt][3] - z1) * scale[1]);
+                sum[0] += p[0] + p[2];
+                sum[1] += p[1] + p[3];
+                uint32_t w[4][G], h0[G], h1[G];
+                words_of<G>(tile + S::VALUE_HELD + (row + g) * 4 * G, h0);
+                words_of<G>(tile + S::VALUE_HELD + (row + g + 8) * 4 * G, h1);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) words_of<G>(tile + S::VALUES + (row + 2 * t + (e & 1) + (e >> 1) * 8) * S::VALUE_ROW + g * 4 * G, w[e]);
+#pragma unroll
+                for (int j = 0; j < G; ++j) {
+                    if (left < KT) {                                      // (what stands behind the last place may be no number)
+                        if (row + g >= left) h0[j] = 0;
+                        if (row + g + 8 >= left) h1[j] = 0;
+                    }
+                    lows[j][0] = fmaf(p[2], high(h1[j]), fmaf(p[0], high(h0[j]), lows[j][0]));
+                    lows[j][1] = fmaf(p[3], high(h1[j]), fmaf(p[1], high(h0[j]), lows[j][1]));
+                    // weights times steps, rounded to bfloat16 as the second operand asks
+                    const float s0 = low(h0[j]), s1 = low(h1[j]);
+                    const uint32_t b0 = transposed(bits(__floats2bfloat162_rn(p[0] * s0, p[1] * s0))), b1 = transposed(bits(__floats2bfloat162_rn(p[2] * s1, p[3] * s1)));
+                    mma16::mma_bf16(ones[j], one, b0, b1);
+                    const uint32_t x0 = __byte_perm(w[0][j], w[1][j], 0x5410), x1 = __byte_perm(w[0][j], w[1][j], 0x7632);
+                    const uint32_t y0 = __byte_perm(w[2][j], w[3][j], 0x5410), y1 = __byte_perm(w[2][j], w[3][j], 0x7632);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {                         // features 8 g + 2 n (rows g) and 8 g + 2 n + 1 (rows g + 8) of the group
+                        const uint32_t x = n < 2 ? x0 : x1, y = n < 2 ? y0 : y1;
+                        const int i0 = 2 * (n & 1);
+                        const uint32_t av[4] = {pair16(x, i0), pair16(x, i0 + 1), pair16(y, i0), pair16(y, i0 + 1)};
+                        mma16::mma_bf16(o[j][n], av, b0, b1);
+                    }
+                }
+            }
+        };
+        for (; next < ends; next += W, ++used) {
+            ask();
+            mma16::cp_async_wait<STAGES - 1>();
+            __syncwarp();
+            work(mine + used % STAGES * S::BYTES, at.places - (at.tile + next - began) * KT);
+            __syncwarp();
         }
-    }
-    __syncthreads();
-    end_part<__nv_bfloat16, D>(a, req, head0, heads, at.tile == 0 && ends - began == at.tiles, began != 0, m_s, l_s, o_s, HEADS * LD, LD);
-    __syncthreads();                                                  // (the next part's sums go where these were)
-    began = ends;
-    if (began < share) at.next_pair(a, chunks);
+        // the warps' sums together: finished, where the whole pair was here; else to the part's slot
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+            sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], x);
+            sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], x);
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                lows[j][0] += __shfl_xor_sync(0xffffffffu, lows[j][0], x);
+                lows[j][1] += __shfl_xor_sync(0xffffffffu, lows[j][1], x);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int h = 2 * t + e;
+            if (h >= heads) continue;
+            if (g == 0) m_s[warp][h] = most[e] * scale[e], l_s[warp][h] = sum[e];
+#pragma unroll
+            for (int j = 0; j < G; ++j) {                                 // features 64 j + 8 g + (0..7)
+                float4* to = reinterpret_cast<float4*>(o_s + (warp * HEADS + h) * LD + 64 * j + 8 * g);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    to[i] = make_float4(fmaf(-16.f, ones[j][e], o[j][2 * i][e] + lows[j][e]), fmaf(-16.f, ones[j][e], o[j][2 * i][e + 2] + lows[j][e]),
+                                        fmaf(-16.f, ones[j][e], o[j][2 * i + 1][e] + lows[j][e]), fmaf(-16.f, ones[j][e], o[j][2 * i + 1][e + 2] + lows[j][e]));
+            }
+        }
+        __syncthreads();
+        end_part<__nv_bfloat16, D, W>(a, req, head0, heads, at.tile == 0 && ends - began == at.tiles, began != 0, m_s, l_s, o_s, HEADS * LD, LD);
+        __syncthreads();                                                  // (the next part's sums go where these were)
+        began = ends;
+        if (began < share) at.next_pair(a, chunks);
     }
 }
 
-// The parts of a pair that several blocks have worked on: a block a pair.  grid (pairs of a request, requests)
-constexpr int JOIN_THREADS = 128;
-template <typename T, int D>
-__global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const DecodeArgs a, int blocks, int chunk_heads) {
+// The parts of a pair that several blocks have worked on.  A quarter of a block's threads takes every fourth part of a head (SLICES = 4), or every fourth head (SLICES = 1).
+// grid (pairs of a request, requests, blocks that a pair's heads are shared out to)
+template <typename T, int D, int SLICES>
+__global__ void __launch_bounds__(D) join_parts_kernel(const DecodeArgs a, int blocks, int chunk_heads) {
+    __shared__ float2 ml_s[SLICES];
+    __shared__ float4 o_s[SLICES][D / 4];
     const int req = blockIdx.y, group = a.nq / a.nkv, chunks = (group + chunk_heads - 1) / chunk_heads, pairs = a.nkv * chunks;
     const int kvh = blockIdx.x / chunks, chunk = blockIdx.x - kvh * chunks, head0 = kvh * group + chunk * chunk_heads, heads = min(chunk_heads, group - chunk * chunk_heads);
     pdl_launch_dependents();
@@ -465,21 +503,12 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const DecodeAr
     const int b0 = tiles ? cut.owner(lo) : 0, b1 = tiles ? cut.owner(lo + tiles - 1) : 0, behind = tiles && cut.begins(b0) != lo;
     pdl_wait();
     if (b0 == b1) return;
-    for (int i = threadIdx.x; i < heads * (D / 4); i += JOIN_THREADS) {
-        const int h = i / (D / 4), f = 4 * (i - h * (D / 4));
-        auto part_of = [&](int b) { return (2 * (size_t)b + (b == b0 ? behind : 0)) * HEADS + h; };
+    const int quarter = threadIdx.x / (D / 4), i4 = threadIdx.x % (D / 4);
+    const int slice = SLICES == 1 ? 0 : quarter;
+    for (int h = SLICES == 1 ? 4 * blockIdx.z + quarter : blockIdx.z; h < heads; h += (SLICES == 1 ? 4 : 1) * gridDim.z) {
         float m = -INFINITY, l = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int first = b0; first <= b1; first += 4) {               // four parts at a time
-            float2 ml[4];
-            float4 v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const size_t part = part_of(min(first + i, b1));
-                ml[i] = *reinterpret_cast<const float2*>(a.part_ml + part * 2);
-                v[i] = *reinterpret_cast<const float4*>(a.part_o + part * D + f);
-                if (first + i > b1) ml[i] = make_float2(-INFINITY, 0.f);
-            }
+        auto add = [&](const float2 (&ml)[4], const float4 (&v)[4]) {
             const float next = fmaxf(fmaxf(m, fmaxf(ml[0].x, ml[1].x)), fmaxf(ml[2].x, ml[3].x)), was = m == next ? 1.f : ex2(m - next);
             m = next;
             l *= was;
@@ -489,16 +518,41 @@ __global__ void __launch_bounds__(JOIN_THREADS) join_parts_kernel(const DecodeAr
                 const float by = ml[i].x == -INFINITY ? (ml[i].y == 0.f ? 0.f : 1.f) : ex2(ml[i].x - m);
                 if (by != 0.f) l = fmaf(by, ml[i].y, l), o.x = fmaf(by, v[i].x, o.x), o.y = fmaf(by, v[i].y, o.y), o.z = fmaf(by, v[i].z, o.z), o.w = fmaf(by, v[i].w, o.w);
             }
+        };
+        float2 ml[4];
+        float4 v[4];
+        for (int first = b0 + slice; first <= b1; first += 4 * SLICES) {      // four parts at a time
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int b = min(first + SLICES * i, b1);
+                const size_t part = (2 * (size_t)b + (b == b0 ? behind : 0)) * HEADS + h;
+                ml[i] = *reinterpret_cast<const float2*>(a.part_ml + part * 2);
+                v[i] = *reinterpret_cast<const float4*>(a.part_o + part * D + 4 * i4);
+                if (first + SLICES * i > b1) ml[i] = make_float2(-INFINITY, 0.f);
+            }
+            add(ml, v);
+        }
+        if constexpr (SLICES > 1) {
+            __syncthreads();                                          // (the head before has been read)
+            o_s[slice][i4] = o;
+            if (i4 == 0) ml_s[slice] = make_float2(m, l);
+            __syncthreads();
+            if (slice) continue;
+#pragma unroll
+            for (int i = 0; i < SLICES; ++i) ml[i] = ml_s[i], v[i] = o_s[i][i4];
+            m = -INFINITY, l = 0.f;
+            o = make_float4(0.f, 0.f, 0.f, 0.f);
+            add(ml, v);
         }
         const float by = l == 0.f ? 0.f : 1.f / l;
-        put4((T*)a.out + ((size_t)req * a.nq + head0 + h) * D + f, make_float4(o.x * by, o.y * by, o.z * by, o.w * by));
+        put4((T*)a.out + ((size_t)req * a.nq + head0 + h) * D + 4 * i4, make_float4(o.x * by, o.y * by, o.z * by, o.w * by));
     }
 }
 
 // ---- float32, and any page, on the CUDA cores ----------------------------------------------------------
 // The same cut of the work.  A warp a tile at a time, whose rows its lanes bring to shared memory, a place each: a lane a place for the scores, then a lane a word of eight features of the
 // values, D / 8 lanes side by side and what is left of the warp on other places.  Everything is float32: x = lowest + step code in one rounding.  A step has a few tiles a warp at
-// most, so it is short loops that count: unrolled ones (the scores' 128 features, 16 places' values) are fetched from memory as they run once, 20 us where these take 10.
+// most, so it is short loops that count: unrolled ones (the scores' 128 features, 16 places' values) are fetched from memory as they run once (3 rows of up to 2,900 places 20 to 22 us, where these took 18).
 template <int D, int HN> struct CoresTile {
     static constexpr int G = D / GROUP, ROW = D / 2 + 16, HELD = 32 * ROW * 2, P = HELD + 32 * 8 * G, BYTES = P + 32 * HN * 4;      // keys' and values' rows, steps, weights
     static constexpr int LD = D + 4, Q = WARPS * BYTES, O = Q + D * HN * 4, ALL = O + WARPS * HN * LD * 4;
@@ -519,7 +573,7 @@ __global__ void __launch_bounds__(32 * WARPS) decode_cores_kernel(const DecodeAr
     pdl_launch_dependents();
     Place at{};
     int share = 0;
-    begin_share<T, D>(a, pairs, chunks, at, share);
+    begin_share<T, D, WARPS>(a, pairs, chunks, at, share);
     const float scale = a.scale * LOG2E;
     const size_t rows = (size_t)a.page_size * row_bytes(D);
     const bool pieces = rows % 16 == 0;                               // (not pages of one or two places)
@@ -616,7 +670,7 @@ __global__ void __launch_bounds__(32 * WARPS) decode_cores_kernel(const DecodeAr
             }
         }
         __syncthreads();
-        end_part<T, D>(a, req, head0, heads, at.tile == 0 && ends - began == at.tiles, began != 0, m_s, l_s, o_s, HN * LD, LD);
+        end_part<T, D, WARPS>(a, req, head0, heads, at.tile == 0 && ends - began == at.tiles, began != 0, m_s, l_s, o_s, HN * LD, LD);
         __syncthreads();
         began = ends;
         if (began < share) at.next_pair(a, chunks);
@@ -634,16 +688,14 @@ inline bool on_tensor_cores(int page_size, int dtype) { return dtype == kBF16 &&
 // Query heads of a pair on the CUDA cores.
 inline int cores_heads(int group) { return group <= 4 ? 4 : 8; }
 // Blocks: as many as are on the device at once, a tile a warp at least.
-inline int blocks_of(int requests, int nq, int nkv, int longest, int heads, int a_sm) {
-    const long long pairs = (long long)requests * nkv * ((nq / nkv + heads - 1) / heads), tiles = pairs * (((long long)longest + KT - 1) / KT);
-    return (int)max(1ll, min((long long)a_sm * sm_count(), (tiles + WARPS - 1) / WARPS));
-}
-struct Plan { bool tensor_cores; int heads, blocks; };
-inline Plan plan_of(int requests, int nq, int nkv, int longest, int page_size, int dtype) {
+struct Plan { bool tensor_cores; int heads, warps, blocks; };
+inline Plan plan_of(int requests, int nq, int nkv, int d, int longest, int page_size, int dtype) {
     Plan p{};
     p.tensor_cores = on_tensor_cores(page_size, dtype);
     p.heads = p.tensor_cores ? HEADS : cores_heads(nq / nkv);
-    p.blocks = blocks_of(requests, nq, nkv, longest, p.heads, p.tensor_cores ? BLOCKS : 3);
+    const long long pairs = (long long)requests * nkv * ((nq / nkv + p.heads - 1) / p.heads), tiles = pairs * (((long long)longest + KT - 1) / KT);
+    p.warps = p.tensor_cores && d <= 128 && pairs >= 3ll * sm_count() ? 1 : WARPS;      // (at blocks_a_sm)
+    p.blocks = (int)max(1ll, min((long long)(p.tensor_cores ? blocks_a_sm(d, p.warps) : 3) * sm_count(), (tiles + p.warps - 1) / p.warps));
     return p;
 }
 
@@ -652,10 +704,21 @@ inline Plan plan_of(int requests, int nq, int nkv, int longest, int page_size, i
 
 using namespace lily;
 
+template <int D, int W> static void launch_mma_of(const four::DecodeArgs& a, const four::Plan& plan, cudaStream_t stream) {
+    constexpr int bytes = W * (four::STAGES * four::Tile<D>::BYTES + four::HEADS * (D + 4) * 4);
+    cudaFuncSetAttribute(four::decode_mma_kernel<D, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    launch_pdl(four::decode_mma_kernel<D, W>, dim3(plan.blocks), dim3(32 * W), bytes, stream, a);
+}
+template <int D> static void launch_mma(const four::DecodeArgs& a, const four::Plan& plan, cudaStream_t stream) {
+    if constexpr (D <= 128)
+        if (plan.warps == 1) return launch_mma_of<D, 1>(a, plan, stream);
+    launch_mma_of<D, four::WARPS>(a, plan, stream);
+}
+
 // float32 of scratch that lily_attention_decode4 needs
 LILY_API size_t lily_attention_decode4_floats(int requests, int nq, int nkv, int d, int longest, int page_size, int dtype) {
     if (requests <= 0 || nkv <= 0 || nq <= 0 || nq % nkv || page_size <= 0) return 0;
-    return (size_t)2 * four::plan_of(requests, nq, nkv, longest, page_size, dtype).blocks * four::HEADS * (d + 2);
+    return (size_t)2 * four::plan_of(requests, nq, nkv, d, longest, page_size, dtype).blocks * four::HEADS * (d + 2);
 }
 
 LILY_API int lily_attention_decode4(const void* q, const void* kv, void* out, const int* block_table, int width, const int* seq_lens, float* scratch, int requests, int longest, int nq,
@@ -668,7 +731,7 @@ LILY_API int lily_attention_decode4(const void* q, const void* kv, void* out, co
     LILY_REQUIRE(longest <= INT32_MAX - 1024, "attention_decode4: rows of %d places", longest);
     LILY_REQUIRE(((uintptr_t)q | (uintptr_t)kv | (uintptr_t)out) % 16 == 0, "attention_decode4: tensors on boundaries of sixteen bytes");
     LILY_REQUIRE(scale != 0.f && scale - scale == 0.f, "attention_decode4: a scale of %g", (double)scale);
-    const four::Plan plan = four::plan_of(requests, nq, nkv, longest, page_size, dtype);
+    const four::Plan plan = four::plan_of(requests, nq, nkv, d, longest, page_size, dtype);
     const int chunks = (nq / nkv + plan.heads - 1) / plan.heads;
     LILY_REQUIRE((long long)requests * nkv * chunks * ((longest + four::KT - 1) / four::KT) <= INT32_MAX, "attention_decode4: %d requests of up to %d places are too many for one call", requests, longest);
     LILY_REQUIRE(scratch != nullptr && (uintptr_t)scratch % 16 == 0, "attention_decode4: the parts of %d blocks need scratch on a boundary of sixteen bytes", plan.blocks);
@@ -679,9 +742,16 @@ LILY_API int lily_attention_decode4(const void* q, const void* kv, void* out, co
     a.part_o = scratch;
     a.part_ml = scratch + (size_t)2 * plan.blocks * four::HEADS * d;
     const dim3 block(32 * four::WARPS);
+    const long long all_pairs = (long long)requests * nkv * chunks;
+    // Few pairs have many parts each, which slices of a block join side by side, a block a head: one row of 8,192 places 11.1 us with them and 14.9 without, 4 rows of 4,096 12.4 and 13.1, 16 rows of
+    // 2,048 (128 pairs) 18.4 and 18.0, 256 rows of 130 many times more blocks and 85 against 31.
+    const bool sliced = 2 * all_pairs <= sm_count();
+    const int most_heads = min(plan.heads, nq / nkv);
+    const dim3 joins(nkv * chunks, requests, sliced ? most_heads : (most_heads + 3) / 4);
 #define JOIN(T, D)                                                                                                                                                 \
     LILY_CHECK_LAUNCH("attention_decode4");                                                                                                                        \
-    launch_pdl(four::join_parts_kernel<T, D>, dim3(nkv * chunks, requests), dim3(four::JOIN_THREADS), 0, stream, a, plan.blocks, plan.heads)
+    if (sliced) launch_pdl(four::join_parts_kernel<T, D, 4>, joins, dim3(D), 0, stream, a, plan.blocks, plan.heads);                                               \
+    else launch_pdl(four::join_parts_kernel<T, D, 1>, joins, dim3(D), 0, stream, a, plan.blocks, plan.heads)
 #define CORES(T, D, HN)                                                                                                                                            \
     do {                                                                                                                                                           \
         constexpr int bytes = four::CoresTile<D, HN>::ALL;                                                                                                         \
@@ -691,9 +761,7 @@ LILY_API int lily_attention_decode4(const void* q, const void* kv, void* out, co
 #define DECODE(D)                                                                                                                                                  \
     do {                                                                                                                                                           \
         if (plan.tensor_cores) {                                                                                                                                   \
-            constexpr int bytes = four::WARPS * (four::STAGES * four::Tile<D>::BYTES + four::HEADS * (D + 4) * 4);                                                 \
-            cudaFuncSetAttribute(four::decode_mma_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);                                                  \
-            launch_pdl(four::decode_mma_kernel<D>, dim3(plan.blocks), block, bytes, stream, a);                                                                    \
+            launch_mma<D>(a, plan, stream);                                                                                                                        \
             JOIN(__nv_bfloat16, D);                                                                                                                                \
         } else if (dtype == kF32) {                                                                                                                                \
             if (plan.heads == 4) CORES(float, D, 4);                                                                                                               \

@@ -278,6 +278,39 @@ def test_decode(dtype, nq, nkv, d, page, lengths):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,nq,nkv,d,page", [(75, 16, 8, 128, 64), (75, 36, 4, 64, 16), (230, 6, 2, 128, 32), (60, 16, 8, 256, 64), (60, 8, 8, 192, 128)])
+def test_decode_of_many_rows(dtype, rows, nq, nkv, d, page):
+    """More pairs of a row and a kv head than three a multiprocessor, of ragged rows, some of them empty."""
+    lengths = [(37 * r) % 211 if r % 9 else 0 for r in range(rows)]
+    lengths[rows // 2] = 1500
+    q, kv, table, seq = decode_case(lengths, nq, nkv, d, page, dtype)
+    want, by_codes, by_values = fb.attention(q, kv, table, [(1 if n else 0, n - 1 if n else 0) for n in lengths], nq, nkv, d, page, d ** -0.5)
+    got = ops().attention_decode4(q, kv, table, seq, max(lengths), nq, nkv, d, page, d ** -0.5)
+    within(got, want, attention_bound(by_codes, by_values, want, dtype))
+    assert torch.equal(got, ops().attention_decode4(q, kv, table, seq, max(lengths), nq, nkv, d, page, d ** -0.5))
+
+
+@pytest.mark.parametrize("lengths", [[9000], [3000, 7, 5000], [100] * 70])
+def test_decode_of_queries_of_any_size(lengths):
+    """Queries times a power of two with the scale divided by it give the same bits, a head's own power among others'; a head of zeros has its values' mean."""
+    nq, nkv, d, page = 16, 8, 128, 64
+    q, kv, table, seq = decode_case(lengths, nq, nkv, d, page, BF16)
+    run = lambda q, scale: ops().attention_decode4(q, kv, table, seq, max(lengths), nq, nkv, d, page, scale)
+    want = run(q, d ** -0.5)
+    for power in (-60, -9, 7, 60):
+        assert torch.equal(run(q * 2.0 ** power, d ** -0.5 * 2.0 ** -power), want)
+    heads = q.view(-1, nq, d).clone()
+    heads[:, 3] *= 2.0 ** 30
+    heads[:, 4] = 0
+    got, kept = run(heads.view_as(q), d ** -0.5).view(-1, nq, d), [h for h in range(nq) if h // 2 not in (1, 2)]      # (heads of one kv head move their maxima together)
+    assert torch.equal(got[:, kept], want.view(-1, nq, d)[:, kept]) and torch.isfinite(got).all()
+    mean, by_codes, by_values = fb.attention(heads.view_as(q), kv, table, [(1, n - 1) for n in lengths], nq, nkv, d, page, d ** -0.5)
+    bound = attention_bound(by_codes, by_values, mean, BF16)
+    at = lambda x: x.view(-1, nq, d)[:, 4]
+    within(got[:, 4], at(mean), at(bound))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_decode_of_far_apart_scores(dtype):
     """Scores from -400 to 400: one place has all the weight, wherever it lies."""
     nq, nkv, d, page, n = 4, 1, 128, 64, 900
