@@ -5,7 +5,9 @@
 //   o_f = sum_j (p_j step_jg) c_jf + sum_j p_j low_jg,
 // so codes go into tensor-core products as they are, 0..15, without a conversion.  Keys: four bits of a word, masked, are the half-precision number c 2^-24 (or 16 c 2^-24, which needs no shift either),
 // and products are exact; a head's queries are brought to 2^13 .. 2^14 by a power of two for it, so that they stay as they are.  Values: weights times steps may lie anywhere, which asks for bfloat16;
-// codes are numbers 16 + c there, and the 16 is taken off at the end with sums of the weights as they were rounded.  Steps meet the sums behind the products (keys) or the weights ahead of them (values).
+// codes are numbers 16 + c there, and 24 is taken off at the end with sums of the weights as they were rounded, for low + 8 step is summed in float32 beside it: what the rounding of a weight moves is so
+// c - 8 times it, no more than the value is from its group's middle (one row of 23 places 2.0e-3 from 64 bits, of which the output's own rounding is 1.7e-3; 3.1e-3 with low alone).  Steps meet the sums
+// behind the products (keys) or the weights ahead of them (values).
 #include "four.cuh"
 #include "mma.cuh"
 #include <cuda_fp16.h>
@@ -331,10 +333,10 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
                 margin[e] = 8.f / scale[e];
             }
         }
-        float o[G][4][4], most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, ones[G][4], lows[G][2];      // (scores and their maximum are kept unscaled)
+        float o[G][4][4], most[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f}, ones[G][4], mids[G][2];      // (scores and their maximum are kept unscaled)
 #pragma unroll
         for (int j = 0; j < G; ++j) {
-            lows[j][0] = lows[j][1] = 0.f;
+            mids[j][0] = mids[j][1] = 0.f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 ones[j][e] = 0.f;
@@ -393,8 +395,8 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
                 sum[1] *= f1;
 #pragma unroll
                 for (int j = 0; j < G; ++j) {
-                    lows[j][0] *= f0;
-                    lows[j][1] *= f1;
+                    mids[j][0] *= f0;
+                    mids[j][1] *= f1;
                     ones[j][0] *= f0;
                     ones[j][1] *= f1;
 #pragma unroll
@@ -423,10 +425,10 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
                         if (row + g >= left) h0[j] = 0;
                         if (row + g + 8 >= left) h1[j] = 0;
                     }
-                    lows[j][0] = fmaf(p[2], high(h1[j]), fmaf(p[0], high(h0[j]), lows[j][0]));
-                    lows[j][1] = fmaf(p[3], high(h1[j]), fmaf(p[1], high(h0[j]), lows[j][1]));
+                    const float s0 = low(h0[j]), s1 = low(h1[j]), mid0 = fmaf(8.f, s0, high(h0[j])), mid1 = fmaf(8.f, s1, high(h1[j]));
+                    mids[j][0] = fmaf(p[2], mid1, fmaf(p[0], mid0, mids[j][0]));
+                    mids[j][1] = fmaf(p[3], mid1, fmaf(p[1], mid0, mids[j][1]));
                     // weights times steps, rounded to bfloat16 as the second operand asks
-                    const float s0 = low(h0[j]), s1 = low(h1[j]);
                     const uint32_t b0 = transposed(bits(__floats2bfloat162_rn(p[0] * s0, p[1] * s0))), b1 = transposed(bits(__floats2bfloat162_rn(p[2] * s1, p[3] * s1)));
                     mma16::mma_bf16(ones[j], one, b0, b1);
                     const uint32_t x0 = __byte_perm(w[0][j], w[1][j], 0x5410), x1 = __byte_perm(w[0][j], w[1][j], 0x7632);
@@ -455,8 +457,8 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
             sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], x);
 #pragma unroll
             for (int j = 0; j < G; ++j) {
-                lows[j][0] += __shfl_xor_sync(0xffffffffu, lows[j][0], x);
-                lows[j][1] += __shfl_xor_sync(0xffffffffu, lows[j][1], x);
+                mids[j][0] += __shfl_xor_sync(0xffffffffu, mids[j][0], x);
+                mids[j][1] += __shfl_xor_sync(0xffffffffu, mids[j][1], x);
             }
         }
 #pragma unroll
@@ -469,8 +471,8 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
                 float4* to = reinterpret_cast<float4*>(o_s + (warp * HEADS + h) * LD + 64 * j + 8 * g);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    to[i] = make_float4(fmaf(-16.f, ones[j][e], o[j][2 * i][e] + lows[j][e]), fmaf(-16.f, ones[j][e], o[j][2 * i][e + 2] + lows[j][e]),
-                                        fmaf(-16.f, ones[j][e], o[j][2 * i + 1][e] + lows[j][e]), fmaf(-16.f, ones[j][e], o[j][2 * i + 1][e + 2] + lows[j][e]));
+                    to[i] = make_float4(fmaf(-24.f, ones[j][e], o[j][2 * i][e] + mids[j][e]), fmaf(-24.f, ones[j][e], o[j][2 * i][e + 2] + mids[j][e]),
+                                        fmaf(-24.f, ones[j][e], o[j][2 * i + 1][e] + mids[j][e]), fmaf(-24.f, ones[j][e], o[j][2 * i + 1][e + 2] + mids[j][e]));
             }
         }
         __syncthreads();
@@ -728,7 +730,7 @@ LILY_API int lily_attention_decode4(const void* q, const void* kv, void* out, co
     LILY_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0, "attention_decode4: %d query heads over %d kv heads", nq, nkv);
     LILY_REQUIRE(requests > 0 && requests <= 65535 && page_size > 0 && longest >= 0 && longest <= (long long)width * page_size && pages > 0, "attention_decode4: %d requests of up to %d places, %d pages of %d",
                  requests, longest, width, page_size);
-    LILY_REQUIRE(longest <= INT32_MAX - 1024, "attention_decode4: rows of %d places", longest);
+    LILY_REQUIRE(longest <= INT32_MAX - 1024 && (long long)page_size * four::row_bytes(d) <= INT32_MAX, "attention_decode4: rows of %d places, pages of %d", longest, page_size);
     LILY_REQUIRE(((uintptr_t)q | (uintptr_t)kv | (uintptr_t)out) % 16 == 0, "attention_decode4: tensors on boundaries of sixteen bytes");
     LILY_REQUIRE(scale != 0.f && scale - scale == 0.f, "attention_decode4: a scale of %g", (double)scale);
     const four::Plan plan = four::plan_of(requests, nq, nkv, d, longest, page_size, dtype);

@@ -59,16 +59,17 @@ struct AttnArgs {
     int score_stride, max_len;      // ... and the places a row has at most
     int stages;               // decode, tensor-core kernel: key/value tiles a block keeps in shared memory (0: the default, 2;
                               // 3: two blocks a SM instead of three, each with two tiles in flight; head sizes up to 128)
-    const unsigned* spans;    // mma.sync prefill: not null where queries and keys are half-precision numbers times powers of two (below)
+    const unsigned* spans;    // mma.sync prefill: not null where queries and keys are half-precision numbers times powers of two (below):
+    const float* units;       // [requests, nkv] of keys and [tokens, nq] of queries
 };
 
-// Queries and keys in half precision, whose eleven bits hold what four-bit codes, their steps and lowest values make of a key (bfloat16's eight would round it).  `spans` holds the largest magnitude of
-// the queries and of the keys, as bits of float32; each is multiplied by the power of two that brings the largest to 2^13 .. 2^14, so that nothing overflows and 2^-28 of it is still a normal number.
+// Queries and keys in half precision, whose eleven bits hold what four-bit codes, their steps and lowest values make of a key (bfloat16's eight would round it).  Each is multiplied by the power of two
+// that brings the largest magnitude to 2^13 .. 2^14, so that nothing overflows and 2^-28 of it is still a normal number: a token's query head by one of its own, and the keys of a request and kv head
+// by one together, so that no token's queries and no request's keys take bits from another's.  `spans` holds the keys' largest magnitudes, as bits of float32; `units` what a query head's power undoes.
 __device__ __forceinline__ int span_exponent(unsigned bits) { return min(max(267 - (int)(bits >> 23), 1), 253); }
 __device__ __forceinline__ float span_multiplier(unsigned bits) { return __uint_as_float((unsigned)span_exponent(bits) << 23); }
-// What a product of such numbers is to be multiplied by.
-__device__ __forceinline__ float span_factor(const unsigned* spans) {
-    return __uint_as_float((unsigned)(254 - span_exponent(spans[0])) << 23) * __uint_as_float((unsigned)(254 - span_exponent(spans[1])) << 23);
-}
+__device__ __forceinline__ float span_unit(unsigned bits) { return __uint_as_float((unsigned)(254 - span_exponent(bits)) << 23); }
+// What a row's products are multiplied by, in units of log2: a number that times a masked score, minus infinity, is minus infinity.
+__device__ __forceinline__ float span_scale(float scale_log2, float query_unit, unsigned keys) { return fminf(fmaxf(scale_log2 * (query_unit * span_unit(keys)), 1.2e-38f), 3e38f); }
 
 }  // namespace lily

@@ -532,7 +532,13 @@ attention_mma_kernel(const AttnArgs a, const int page_shift, const __grid_consta
     // (the hardware's tanh, relative error about 2^-11: the weights are rounded to bfloat16 for the p . v product anyway;
     // the float32 path is the CUDA-core kernel's, which calls tanhf)
     const float cap = a.softcap, cap_in = cap > 0.f ? a.scale / cap : 0.f;
-    const float sl2 = (cap > 0.f ? 1.f : a.scale) * 1.4426950408889634f * (HALF ? span_factor(a.spans) : 1.f);
+    const float sl2 = (cap > 0.f ? 1.f : a.scale) * 1.4426950408889634f;
+    float sl2_lo = sl2, sl2_hi = sl2;                   // of this thread's two rows
+    if constexpr (HALF) {
+        const unsigned keys = a.spans[(size_t)req * a.nkv + head0 / (a.nq / a.nkv)];
+        sl2_lo = span_scale(sl2, a.units[((size_t)tok0 + min(row_lo, nrows - 1)) * a.nq + head0], keys);
+        sl2_hi = span_scale(sl2, a.units[((size_t)tok0 + min(row_hi, nrows - 1)) * a.nq + head0], keys);
+    }
     auto tanh_fast = [](float v) { float r; asm("tanh.approx.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; };
 
     for (int t = 0; t < ntiles; ++t) {
@@ -633,7 +639,7 @@ attention_mma_kernel(const AttnArgs a, const int page_shift, const __grid_consta
         mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, 1));
         mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, 2));
         // running maxima are kept in scaled (log2) units: scale > 0, so the order is the same
-        const float mn_lo = fmaxf(m_lo, mx_lo * sl2), mn_hi = fmaxf(m_hi, mx_hi * sl2);
+        const float mn_lo = fmaxf(m_lo, mx_lo * sl2_lo), mn_hi = fmaxf(m_hi, mx_hi * sl2_hi);
         const float base_lo = mn_lo == -INFINITY ? 0.f : mn_lo, base_hi = mn_hi == -INFINITY ? 0.f : mn_hi;
         const float al_lo = exp2f(m_lo - base_lo), al_hi = exp2f(m_hi - base_hi);
         m_lo = mn_lo;
@@ -641,10 +647,10 @@ attention_mma_kernel(const AttnArgs a, const int page_shift, const __grid_consta
         float sum_lo = 0.f, sum_hi = 0.f;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            s[j][0] = exp2f(fmaf(s[j][0], sl2, -base_lo));
-            s[j][1] = exp2f(fmaf(s[j][1], sl2, -base_lo));
-            s[j][2] = exp2f(fmaf(s[j][2], sl2, -base_hi));
-            s[j][3] = exp2f(fmaf(s[j][3], sl2, -base_hi));
+            s[j][0] = exp2f(fmaf(s[j][0], sl2_lo, -base_lo));
+            s[j][1] = exp2f(fmaf(s[j][1], sl2_lo, -base_lo));
+            s[j][2] = exp2f(fmaf(s[j][2], sl2_hi, -base_hi));
+            s[j][3] = exp2f(fmaf(s[j][3], sl2_hi, -base_hi));
             sum_lo += s[j][0] + s[j][1];
             sum_hi += s[j][2] + s[j][3];
         }
@@ -1051,14 +1057,14 @@ LILY_API int lily_attention_prefill_mma(const void* q, const void* kv, void* out
     return 0;
 }
 
-// The same over queries and keys in half precision (values stay bfloat16); spans: attention_args.cuh.
+// The same over queries and keys in half precision (values stay bfloat16); spans, units: attention_args.cuh.
 LILY_API int lily_attention_prefill_mma_half(const void* q, const void* kv, void* out, const int* block_table, int bt_stride, const int* cu_seqlens, const int* prefix_lens, const int* tile_req,
-                                             const int* tile_start, int tiles, int nq, int nkv, int d, int page_size, float scale, const unsigned* spans, cudaStream_t stream) {
+                                             const int* tile_start, int tiles, int nq, int nkv, int d, int page_size, float scale, const unsigned* spans, const float* units, cudaStream_t stream) {
     if (tiles == 0) return 0;
-    LILY_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0 && spans != nullptr, "attention_prefill: %d query heads over %d kv heads", nq, nkv);
+    LILY_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0 && spans != nullptr && units != nullptr, "attention_prefill: %d query heads over %d kv heads", nq, nkv);
     LILY_REQUIRE(nq <= 65535 && page_size > 0, "attention_prefill: nq=%d page_size=%d", nq, page_size);
     AttnArgs a{};
-    a.q = q; a.kv = kv; a.out = out; a.block_table = block_table; a.bt_stride = bt_stride; a.spans = spans;
+    a.q = q; a.kv = kv; a.out = out; a.block_table = block_table; a.bt_stride = bt_stride; a.spans = spans; a.units = units;
     a.cu_seqlens = cu_seqlens; a.prefix_lens = prefix_lens; a.tile_req = tile_req; a.tile_start = tile_start;
     a.splits = 1; a.nq = nq; a.nkv = nkv; a.d = d; a.page_size = page_size; a.scale = scale;
     bool merged = false;

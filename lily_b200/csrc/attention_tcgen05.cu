@@ -104,9 +104,15 @@ struct Params {
     float scale_log2;                     // softmax scale times log2(e) (log2(e) alone under a cap)
     int sink;                             // the softmax's denominator holds one more unit: a key of score 0 without a value
     size_t plane;                         // elements between the planes of `out` (grid z): plane z weighs the values of kv head (own + z) % nkv
-    const unsigned* spans;                // not null where queries and keys are half-precision numbers times powers of two (attention_args.cuh)
+    const unsigned* spans;                // not null where queries and keys are half-precision numbers times powers of two (attention_args.cuh):
+    const float* units;                   // of the keys and of the queries
     float cap, cap_in;                    // cap > 0: scores become cap * tanh(score * cap_in), cap_in = scale / cap
 };
+// What a row's scores are multiplied by in units of log2.
+__device__ __forceinline__ float row_scale(const Params& p, int req, int token, int head) {
+    if (!p.spans) return p.scale_log2;
+    return span_scale(p.scale_log2, p.units[(size_t)token * p.nq + head], p.spans[(size_t)req * p.nkv + head / (p.nq / p.nkv)]);
+}
 
 // The hardware's tanh (relative error about 2^-11; the weights are rounded to bfloat16 for the p.v product).
 __device__ __forceinline__ float tanh_fast(float v) {
@@ -182,7 +188,6 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     // q and the cache come from the kernels before this one
     pdl_wait();
     pdl_launch_dependents();
-    const float scale_log2 = p.spans ? p.scale_log2 * span_factor(p.spans) : p.scale_log2;
 
     // the tiles were listed in order of position: the last ones, which see the most keys, go first
     const int tile = p.tiles - 1 - (int)blockIdx.y;
@@ -303,6 +308,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         const int row = quarter * 32 + lane;
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
         const int pos = pos0 + row;
+        const float scale_log2 = row_scale(p, req, q_begin + start + min(row, rows_valid - 1), head);
         float m_used = p.sink ? 0.f : -INFINITY, l = 0.f;
         bool ok = true;
         // The threads of a row hand each other one float per tile (the maximum of their keys; at the end
@@ -554,7 +560,6 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
 
     pdl_wait();
     pdl_launch_dependents();
-    const float scale_log2 = p.spans ? p.scale_log2 * span_factor(p.spans) : p.scale_log2;
 
     const int tile = p.tiles - 1 - (int)blockIdx.y;             // the last tiles, which see the most keys, go first
     const int head0 = blockIdx.x * NH2;
@@ -696,6 +701,7 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
         const uint32_t my_s = tmem + lane_addr + (uint32_t)(h * BKV), my_o = tmem_o + lane_addr + (uint32_t)(h * D);
         const int pos = pos0 + row;
+        const float scale_log2 = row_scale(p, req, q_begin + start + min(row, rows_valid - 1), head0 + h);
         float m_used = p.sink ? 0.f : -INFINITY, l = 0.f;
         bool ok = true;
         for (int j = 0; j < n && ok; ++j) {
@@ -878,7 +884,7 @@ LILY_API int lily_attention_tc_status() {
 
 static int prefill_tc(const void* q, const void* kv, void* out, const int* block_table, int bt_stride, const int* cu_seqlens, const int* prefix_lens, const int* tile_req, const int* tile_start,
                       int tiles, int nq, int nkv, int d, int page_size, int window, float scale, int tokens, int num_pages, int heads_per_block, float softcap, int keep_first, int sink, int planes,
-                      const unsigned* spans, cudaStream_t stream) {
+                      const unsigned* spans, const float* units, cudaStream_t stream) {
     if (tiles == 0) return 0;
     LILY_REQUIRE(planes >= 1 && planes <= nkv, "attention_prefill_tc: %d planes of %d kv heads", planes, nkv);
     LILY_REQUIRE(lily_attention_prefill_tc_takes(d, page_size), "attention_prefill_tc: head size %d, page size %d (takes 64 or 128, and multiples of 64)",
@@ -910,7 +916,7 @@ static int prefill_tc(const void* q, const void* kv, void* out, const int* block
         LILY_REQUIRE(rc == CUDA_SUCCESS, "attention_prefill_tc: cuTensorMapEncodeTiled (cache) failed with %d", (int)rc);
     }
     fa::Params p{};
-    p.spans = spans;
+    p.spans = spans; p.units = units;
     p.block_table = block_table; p.cu_seqlens = cu_seqlens; p.prefix_lens = prefix_lens; p.tile_req = tile_req;
     p.tile_start = tile_start; p.out = (__nv_bfloat16*)out; p.bt_stride = bt_stride; p.tiles = tiles; p.nq = nq; p.nkv = nkv;
     p.page_size = page_size; p.window = window; p.sink = sink; p.plane = (size_t)tokens * nq * d;
@@ -942,13 +948,13 @@ LILY_API int lily_attention_prefill_tc(const void* q, const void* kv, void* out,
                                        float scale, int tokens, int num_pages, int heads_per_block, float softcap,
                                        int keep_first, int sink, int planes, cudaStream_t stream) {
     return prefill_tc(q, kv, out, block_table, bt_stride, cu_seqlens, prefix_lens, tile_req, tile_start, tiles, nq, nkv, d, page_size, window, scale, tokens, num_pages, heads_per_block, softcap,
-                      keep_first, sink, planes, nullptr, stream);
+                      keep_first, sink, planes, nullptr, nullptr, stream);
 }
 
-// The same over queries and keys in half precision (values stay bfloat16), without cap, window and sink; spans: attention_args.cuh.
+// The same over queries and keys in half precision (values stay bfloat16), without cap, window and sink; spans, units: attention_args.cuh.
 LILY_API int lily_attention_prefill_tc_half(const void* q, const void* kv, void* out, const int* block_table, int bt_stride, const int* cu_seqlens, const int* prefix_lens, const int* tile_req,
                                             const int* tile_start, int tiles, int nq, int nkv, int d, int page_size, float scale, int tokens, int num_pages, const unsigned* spans,
-                                            cudaStream_t stream) {
-    LILY_REQUIRE(spans != nullptr, "attention_prefill_tc: half-precision queries come with their spans");
-    return prefill_tc(q, kv, out, block_table, bt_stride, cu_seqlens, prefix_lens, tile_req, tile_start, tiles, nq, nkv, d, page_size, 0, scale, tokens, num_pages, 0, 0.f, 0, 0, 1, spans, stream);
+                                            const float* units, cudaStream_t stream) {
+    LILY_REQUIRE(spans != nullptr && units != nullptr, "attention_prefill_tc: half-precision queries and keys come with their powers of two");
+    return prefill_tc(q, kv, out, block_table, bt_stride, cu_seqlens, prefix_lens, tile_req, tile_start, tiles, nq, nkv, d, page_size, 0, scale, tokens, num_pages, 0, 0.f, 0, 0, 1, spans, units, stream);
 }

@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__
     T* dst = out + ((to * 2 + value) * nkv + head) * ((size_t)page_size * D);
     const int i8 = threadIdx.x & 7;
     const bool halves = sizeof(T) == 2 && spans && !value;
-    const float by = halves ? span_multiplier(spans[1]) : 1.f;
+    const float by = halves ? span_multiplier(spans[(size_t)r * nkv + head]) : 1.f;
 #pragma unroll 2
     for (int slot = threadIdx.x >> 3; slot < page_size; slot += 32) {
         uint32_t w[G], h[G];
@@ -333,47 +333,50 @@ __global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__
     }
 }
 
-// The largest magnitudes of what portions attend with: of the queries (grid-wide, 16 bytes a thread), and a bound of the keys' from their steps and lowest values (lowest + 15 step, or lowest), as bits
-// that are compared as whole numbers.  What is no number counts for nothing.  blocks [0, query_blocks): queries; the others: a block a (page, request), all its heads
-__global__ void __launch_bounds__(256) spans_kernel(const __nv_bfloat16* __restrict__ q, size_t pieces, int query_blocks, const uint8_t* __restrict__ kv, int pages, const int* __restrict__ block_table,
-                                                    int width, int nkv, int d, int page_size, const int* __restrict__ cu, const int* __restrict__ prefix, int most, unsigned* __restrict__ spans) {
+// What portions attend with in half precision (attention_args.cuh).  blocks [0, query_blocks): queries, times the power of two of their token and head, eight numbers a thread and d / 8 threads a head;
+// the others, a block a (page, request) and a warp a kv head at a time: a bound of the keys' magnitudes from their steps and lowest values (lowest + 15 step, or lowest), as bits that are compared as
+// whole numbers.  What is no number counts for nothing.
+__global__ void __launch_bounds__(256) halves_kernel(const __nv_bfloat16* __restrict__ q, size_t heads, __nv_bfloat16* __restrict__ out, float* __restrict__ units, int query_blocks,
+                                                     const uint8_t* __restrict__ kv, int pages, const int* __restrict__ block_table, int width, int nkv, int d, int page_size,
+                                                     const int* __restrict__ cu, const int* __restrict__ prefix, int most, unsigned* __restrict__ spans) {
     pdl_enter_small();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float m = 0.f;
     auto take = [&](float v) {
         v = fabsf(v);
         if (v <= 3e38f) m = fmaxf(m, v);
     };
-    const bool queries = (int)blockIdx.x < query_blocks;
-    if (queries) {
-        for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (size_t)query_blocks * 256) {
-            const uint4 v = reinterpret_cast<const uint4*>(q)[i];
-            take(low(v.x)), take(high(v.x)), take(low(v.y)), take(high(v.y)), take(low(v.z)), take(high(v.z)), take(low(v.w)), take(high(v.w));
-        }
-    } else {
-        const int r = ((int)blockIdx.x - query_blocks) / most, at = ((int)blockIdx.x - query_blocks) % most, groups = d / GROUP;
-        const int total = cu[r + 1] > cu[r] ? prefix[r] + cu[r + 1] - cu[r] : 0, places = min(page_size, total - at * page_size);
-        if (places <= 0) return;
-        int page = at < width ? block_table[(size_t)r * width + at] : 0;
-        if ((unsigned)page >= (unsigned)pages) page = 0;
-        const size_t rows = (size_t)page_size * row_bytes(d);
-        for (int i = threadIdx.x; i < nkv * places * groups; i += 256) {
-            const int head = i / (places * groups), in = i - head * places * groups;
-            const uint32_t h = reinterpret_cast<const uint32_t*>(kv + ((size_t)page * nkv + head) * 2 * rows + (size_t)page_size * (d / 2))[in];
+    if ((int)blockIdx.x < query_blocks) {
+        const int words = d / 8, per_warp = 32 / words, mine = lane / words, l = lane - mine * words;      // (d = 192: lanes 24 to 31 have no word)
+        const size_t head = ((size_t)blockIdx.x * 8 + warp) * per_warp + mine;
+        const bool in = mine < per_warp && head < heads;
+        float v[8] = {};
+        if (in) load8(q + head * d + l * 8, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) take(v[i]);
+        for (int o = words == 24 ? 16 : words >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (!in) return;
+        store_halves(out + head * d + l * 8, v, span_multiplier(__float_as_uint(m)));
+        if (l == 0) units[head] = span_unit(__float_as_uint(m));
+        return;
+    }
+    const int r = ((int)blockIdx.x - query_blocks) / most, at = ((int)blockIdx.x - query_blocks) % most, groups = d / GROUP;
+    const int total = cu[r + 1] > cu[r] ? prefix[r] + cu[r + 1] - cu[r] : 0, places = min(page_size, total - at * page_size);
+    if (places <= 0) return;
+    int page = at < width ? block_table[(size_t)r * width + at] : 0;
+    if ((unsigned)page >= (unsigned)pages) page = 0;
+    const size_t rows = (size_t)page_size * row_bytes(d);
+    for (int head = warp; head < nkv; head += 8) {
+        const uint32_t* held = reinterpret_cast<const uint32_t*>(kv + ((size_t)page * nkv + head) * 2 * rows + (size_t)page_size * (d / 2));
+        m = 0.f;
+#pragma unroll 4
+        for (int i = lane; i < places * groups; i += 32) {
+            const uint32_t h = held[i];
             take(high(h)), take(fmaf(15.f, low(h), high(h)));
         }
+        const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+        if (lane == 0 && bits) atomicMax(spans + (size_t)r * nkv + head, bits);
     }
-    const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-    if ((threadIdx.x & 31) == 0 && bits) atomicMax(spans + (queries ? 0 : 1), bits);
-}
-
-// Queries in half precision.  A thread eight numbers.
-__global__ void __launch_bounds__(256) halves_kernel(const __nv_bfloat16* __restrict__ q, size_t pieces, __nv_bfloat16* __restrict__ out, const unsigned* __restrict__ spans) {
-    pdl_enter_small();
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= pieces) return;
-    float v[8];
-    load8(q + i * 8, v);
-    store_halves(out + i * 8, v, span_multiplier(spans[0]));
 }
 
 inline bool head_fits(int d) { return d >= GROUP && d <= 256 && d % GROUP == 0; }
@@ -425,7 +428,7 @@ LILY_API int lily_qk_norm_rope_write4(const void* qkv, int dtype, int ld, const 
     return 0;
 }
 
-// spans: null, or the largest magnitudes of queries and keys, for keys in half precision (lily_spans4).  cu, prefix, table_out: null, or of a step's portions (offsets of their tokens, tokens cached ahead of them, a block table [requests, table_width] of the pages
+// spans: null, or the largest magnitudes of keys, for keys in half precision (lily_halves4).  cu, prefix, table_out: null, or of a step's portions (offsets of their tokens, tokens cached ahead of them, a block table [requests, table_width] of the pages
 // written, of which there is room for `most_pages`).
 LILY_API int lily_cache4_values(const void* kv, int pages, const int* block_table, int requests, int width, void* out, int dtype, int nkv, int d, int page_size, const int* cu,
                                 const int* prefix, int* table_out, int table_width, int most_pages, const unsigned* spans, cudaStream_t stream) {
@@ -452,19 +455,17 @@ LILY_API int lily_cache4_values(const void* kv, int pages, const int* block_tabl
     return 0;
 }
 
-// What portions attend with in half precision: the largest magnitudes to `spans` (two words that are zero before), and the queries times a power of two to `out`.
-LILY_API int lily_spans4(const void* q, int tokens, int nq, const void* kv, int pages, const int* block_table, int requests, int width, int nkv, int d, int page_size, const int* cu, const int* prefix,
-                         int most_pages, unsigned* spans, void* out, cudaStream_t stream) {
+// What portions attend with in half precision (attention_args.cuh): the largest magnitudes of keys to `spans` [requests, nkv], which is zeros before, the queries times powers of two to `out`, what undoes
+// them to `units` [tokens, nq].
+LILY_API int lily_halves4(const void* q, int tokens, int nq, const void* kv, int pages, const int* block_table, int requests, int width, int nkv, int d, int page_size, const int* cu, const int* prefix,
+                          int most_pages, unsigned* spans, void* out, float* units, cudaStream_t stream) {
     if (tokens == 0 || requests == 0) return 0;
-    LILY_REQUIRE(four::head_fits(d) && page_size > 0 && nkv > 0 && nq > 0 && most_pages > 0 && (long long)requests * most_pages <= INT32_MAX / 2, "spans4: %d requests of up to %d pages", requests, most_pages);
-    LILY_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)kv) % 16 == 0, "spans4: tensors on boundaries of sixteen bytes");
-    const size_t pieces = (size_t)tokens * nq * (d / 8);
-    const int query_blocks = (int)min((size_t)(4 * sm_count()), (pieces + 255) / 256);
-    launch_pdl(four::spans_kernel, dim3(query_blocks + requests * most_pages), dim3(256), 0, stream, (const __nv_bfloat16*)q, pieces, query_blocks, (const uint8_t*)kv, pages, block_table, width, nkv, d,
-               page_size, cu, prefix, most_pages, spans);
-    LILY_CHECK_LAUNCH("spans4");
-    LILY_REQUIRE((pieces + 255) / 256 <= INT32_MAX, "spans4: %d tokens", tokens);
-    launch_pdl(four::halves_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, stream, (const __nv_bfloat16*)q, pieces, (__nv_bfloat16*)out, (const unsigned*)spans);
-    LILY_CHECK_LAUNCH("spans4");
+    LILY_REQUIRE(four::head_fits(d) && page_size > 0 && nkv > 0 && nq > 0 && most_pages > 0 && (long long)requests * most_pages <= INT32_MAX / 2, "halves4: %d requests of up to %d pages", requests, most_pages);
+    LILY_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)kv) % 16 == 0, "halves4: tensors on boundaries of sixteen bytes");
+    const size_t heads = (size_t)tokens * nq, a_block = 8 * (32 / (d / 8)), query_blocks = (heads + a_block - 1) / a_block;
+    LILY_REQUIRE(query_blocks <= INT32_MAX / 2, "halves4: %d tokens", tokens);
+    launch_pdl(four::halves_kernel, dim3((unsigned)query_blocks + requests * most_pages), dim3(256), 0, stream, (const __nv_bfloat16*)q, heads, (__nv_bfloat16*)out, units, (int)query_blocks,
+               (const uint8_t*)kv, pages, block_table, width, nkv, d, page_size, cu, prefix, most_pages, spans);
+    LILY_CHECK_LAUNCH("halves4");
     return 0;
 }

@@ -102,9 +102,9 @@ _SIGNATURES = {
     "lily_apply_penalties": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_top_logprobs": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_cache4_values": [_vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _vp],
-    "lily_spans4": [_vp, _i, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp],
-    "lily_attention_prefill_tc_half": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _vp],
-    "lily_attention_prefill_mma_half": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp, _vp],
+    "lily_halves4": [_vp, _i, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp],
+    "lily_attention_prefill_tc_half": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _vp, _vp],
+    "lily_attention_prefill_mma_half": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp],
     "lily_linear4_status": [],
     "lily_sample": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
 }
@@ -1519,20 +1519,25 @@ def attention_prefill4(q: torch.Tensor, kv_layer: torch.Tensor, block_table: tor
         return out
     if plan is None:
         plan = plan_prefill4(q.dtype, d, page_size, h_prefix_lens, h_new_lens, q.device)
+    else:
+        _dev(plan.tile_req, plan.tile_start)
+        pages = [-(-(p + n) // page_size) if n else 0 for p, n in zip(h_prefix_lens, h_new_lens)]
+        if (plan.pages, plan.width) != (sum(pages), max(pages)) or plan.rows != prefill_tile_rows(q.dtype, d, page_size, tokens) or plan.tile_req.numel() != sum(-(-n // plan.rows) for n in h_new_lens):
+            raise KernelError(f"attention_prefill4: the plan is not one of portions of {tuple(h_new_lens)} behind {tuple(h_prefix_lens)}")
     if plan.width > block_table.shape[1]:
         raise KernelError(f"attention_prefill4: {plan.width} pages of a request; the block table holds {block_table.shape[1]}")
     if not 0 < scale < float("inf"):
         raise KernelError(f"attention_prefill4: a scale of {scale}")
     values = torch.empty((plan.pages, 2, nkv, page_size, d), dtype=q.dtype, device=q.device)
-    words = torch.zeros((requests * plan.width + 2,), dtype=torch.int32, device=q.device)
-    spans, table = words[:2], words[2:].view(requests, plan.width)
+    words = torch.zeros((requests * (nkv + plan.width),), dtype=torch.int32, device=q.device)
+    spans, table = words[:requests * nkv], words[requests * nkv:].view(requests, plan.width)
     # (the tensor-core kernels; others, of float32 and of pages that are no power of two, read the numbers themselves)
     halves = uses_tensor_cores(q.dtype, d) and page_size & (page_size - 1) == 0
     heads = q
     if halves:
-        heads = torch.empty_like(q)
-        _call("lily_spans4", _p(q), q.shape[0], nq, _p(kv_layer), kv_layer.shape[0], _i32(block_table, "block_table"), requests, block_table.shape[1], nkv, d, page_size,
-              _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens"), plan.width, _p(spans), _p(heads), _stream())
+        heads, units = torch.empty_like(q), torch.empty((q.shape[0], nq), dtype=torch.float32, device=q.device)
+        _call("lily_halves4", _p(q), q.shape[0], nq, _p(kv_layer), kv_layer.shape[0], _i32(block_table, "block_table"), requests, block_table.shape[1], nkv, d, page_size,
+              _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens"), plan.width, _p(spans), _p(heads), _p(units), _stream())
     _call("lily_cache4_values", _p(kv_layer), kv_layer.shape[0], _i32(block_table, "block_table"), requests, block_table.shape[1], _p(values), _dt(q), nkv, d, page_size,
           _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens"), _p(table), plan.width, plan.pages, _p(spans) if halves else None, _stream())
     if not halves:
@@ -1540,9 +1545,9 @@ def attention_prefill4(q: torch.Tensor, kv_layer: torch.Tensor, block_table: tor
         return out
     common = (_p(heads), _p(values), _p(out), _p(table), plan.width, _p(cu_seqlens), _p(prefix_lens), _p(plan.tile_req), _p(plan.tile_start), plan.tile_req.numel(), nq, nkv, d, page_size, float(scale))
     if plan.rows == int(library().lily_attention_prefill_tc_rows()):
-        _call("lily_attention_prefill_tc_half", *common, q.shape[0], plan.pages, _p(spans), _stream())
+        _call("lily_attention_prefill_tc_half", *common, q.shape[0], plan.pages, _p(spans), _p(units), _stream())
     else:
-        _call("lily_attention_prefill_mma_half", *common, _p(spans), _stream())
+        _call("lily_attention_prefill_mma_half", *common, _p(spans), _p(units), _stream())
     return out
 
 

@@ -73,7 +73,7 @@ def turn(x, gain, eps, cos, sin, rot):
 
 
 def attention(q, kv, table, spans, nq, nkv, d, page, scale):
-    """Causal attention in 64 bits of ``spans`` [(new, cached)], rows of q in their order: (outputs, bounds of what one rounding of the weights times steps, and of a value, moves them by)
+    """Causal attention in 64 bits of ``spans`` [(new, cached)], rows of q in their order: (outputs, bounds of what one rounding of the weights times steps, around the middle code 8, and of a value, moves them by)
     [tokens, nq * d].  A request without places has a row of zeros where it brings one token (``new`` 0)."""
     group, q = nq // nkv, q.double().view(-1, nq, d)
     out, by_codes, by_values = torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(q)
@@ -91,7 +91,7 @@ def attention(q, kv, table, spans, nq, nkv, d, page, scale):
                     e = (q[t0:t0 + n, h] @ k.T * scale).masked_fill(hidden, -math.inf)
                     p = torch.softmax(e, -1)
                     out[t0:t0 + n, h] = p @ v
-                    by_codes[t0:t0 + n, h] = p @ (vs * vc)
+                    by_codes[t0:t0 + n, h] = p @ (vs * (vc - 8).abs())
                     by_values[t0:t0 + n, h] = p @ v.abs()
         t0 += rows
     return tuple(t.view(-1, nq * d) for t in (out, by_codes, by_values))

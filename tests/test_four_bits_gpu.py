@@ -236,7 +236,7 @@ def test_values(dtype, nkv, d, page):
 # ---- attention ----
 
 def attention_bound(by_codes, by_values, want, dtype):
-    """bfloat16: a rounding of each weight times its step (2^-8 of that part of the sum), of the result, and, for portions, of keys and values (``cached``); float32 sums: scores of up to some 30 with
+    """bfloat16: a rounding of each weight times its step (sum w (c - 8) + p (low + 8 step), where p stays float32: a relative 2^-8 of w moves that part alone), of the result, and, for portions, of keys and values (``cached``); float32 sums: scores of up to some 30 with
     errors of 2^-16, which are the relative errors of weights."""
     if dtype == F32:
         return 2.0 ** -14 * by_values + HALF[F32] * want.abs()
@@ -366,6 +366,80 @@ def test_portions(dtype, nq, nkv, d, page, new, cached):
         # keys rounded to bfloat16 move scores of |q| |k| d^-1/2 (up to some 4 |q_f k_f| sums) by 2^-8 of sum |q_f k_f| / sqrt(d), at most 2^-8 * 2 sqrt(d) here; weights and values are rounded too
         bound = bound + HALF[BF16] * (2 * 2 * d ** 0.5 + 2) * by_values
     within(got, want, bound)
+
+
+def portions_case(new, cached, nq, nkv, d, page, seed=4):
+    lengths = [p + n for p, n in zip(cached, new)]
+    _, kv, table, _ = decode_case(lengths, nq, nkv, d, page, BF16, seed=seed, lean=0.0)
+    q = torch.randn(sum(new), nq * d, generator=torch.Generator().manual_seed(seed)).to(BF16).to(DEV)
+    cu = torch.tensor([0, *torch.tensor(new).cumsum(0).tolist()], dtype=torch.int32, device=DEV)
+    pre = torch.tensor(cached, dtype=torch.int32, device=DEV)
+    return q, kv, lambda q, kv, out=None, plan=None: ops().attention_prefill4(q, kv, table, cu, pre, cached, new, nq, nkv, d, page, d ** -0.5, out, plan), table
+
+
+# both tensor-core kernels: many tokens and few, pages that the one takes and that only the other takes
+WHO = [([700, 900, 600], [0, 130, 0], 8, 4, 128, 64), ([40, 1, 70], [3, 200, 0], 6, 2, 128, 16), ([30, 50, 9], [0, 20, 64], 4, 2, 192, 32), ([500, 700, 800], [10, 0, 100], 4, 4, 64, 64)]
+
+
+@pytest.mark.parametrize("new,cached,nq,nkv,d,page", WHO)
+def test_portions_keep_to_themselves(new, cached, nq, nkv, d, page):
+    """Queries and keys of any size, and what is no number, change nothing in other requests' rows, in other tokens' rows above, or in other kv heads."""
+    q, kv, run, table = portions_case(new, cached, nq, nkv, d, page)
+    clean = run(q, kv)
+    a, b = new[0], new[0] + new[1]
+    for large in (3e38, 1e30, math.inf, math.nan):
+        other = q.clone()
+        other[a:b] = large                                     # a whole request
+        assert torch.equal(run(other, kv)[:a], clean[:a]) and torch.equal(run(other, kv)[b:], clean[b:])
+        other = q.clone()
+        other[a - 1, d:2 * d] = large                          # one token's head
+        got, kept = run(other, kv), torch.ones(a, nq, dtype=torch.bool, device=DEV)
+        kept[a - 1, 1] = False
+        assert torch.equal(got[:a].view(a, nq, d)[kept], clean[:a].view(a, nq, d)[kept]) and torch.equal(got[a:], clean[a:])
+    # a key of the second request, in its kv head 1, whose lowest values are huge
+    keys = kv.clone()
+    held = torch.tensor([[1.0, 2.0 ** 100]] * (d // 64), dtype=BF16, device=DEV)
+    fb.write_row(keys[table[1, 0], 1, 0], 0, page, d, False, torch.zeros(d, dtype=torch.uint8, device=DEV), held)
+    got = run(q, keys)
+    assert torch.equal(got[:a], clean[:a]) and torch.equal(got[b:], clean[b:])
+    heads = slice(0, nq // nkv)
+    assert torch.equal(got[a:b].view(-1, nq, d)[:, heads], clean[a:b].view(-1, nq, d)[:, heads])
+    # rows behind the last portion
+    room = torch.cat([q, torch.full((37, nq * d), 3e38, dtype=BF16, device=DEV)])
+    out = torch.full_like(room, 7.0)
+    run(room, kv, out)
+    assert torch.equal(out[:len(q)], clean) and bool((out[len(q):] == 7.0).all())
+
+
+@pytest.mark.parametrize("new,cached,nq,nkv,d,page", WHO)
+def test_portions_of_queries_of_any_size(new, cached, nq, nkv, d, page):
+    """A query head times a power of two, the keys divided by it, give the same bits; a head of zeros has the mean of the values it sees."""
+    q, kv, run, table = portions_case(new, cached, nq, nkv, d, page)
+    clean = run(q, kv)
+    for power in (-40, 25):
+        moved = kv.clone()
+        held = moved[:, :, 0, page * d // 2:].contiguous().view(BF16)
+        moved[:, :, 0, page * d // 2:] = (held * 2.0 ** -power).view(torch.uint8)
+        assert torch.equal(run(q * 2.0 ** power, moved), clean)
+    nothing = q.clone()
+    nothing[3] = 0
+    got = run(nothing, kv)
+    want, by_codes, by_values = fb.attention(nothing, kv, table, list(zip(new, cached)), nq, nkv, d, page, d ** -0.5)
+    # (weights and values are rounded: 2^-8 of the values' magnitudes each)
+    within(got[3], want[3], HALF[BF16] * (2 * by_values[3] + want[3].abs()) + 2.0 ** -12 * by_values[3] + 1e-30)
+    assert torch.equal(got[:3], clean[:3]) and torch.equal(got[4:], clean[4:])
+
+
+def test_portions_refuse_a_plan_of_others():
+    new, cached, nq, nkv, d, page = [40, 1, 70], [3, 200, 0], 6, 2, 128, 16
+    q, kv, run, _ = portions_case(new, cached, nq, nkv, d, page)
+    clean, plan = run(q, kv), lambda *a: ops().plan_prefill4(BF16, d, page, *a, q.device)
+    assert torch.equal(run(q, kv, None, plan(cached, new)), clean)
+    for other in (plan([0, 0, 0], [0, 0, 0]), plan(cached, [41, 1, 69]), plan([3, 216, 0], new), plan([19, 200, 0], new), ops().plan_prefill4(F32, d, page, cached, new, q.device)):
+        if other.rows == plan(cached, new).rows and other.tile_req.numel() == plan(cached, new).tile_req.numel() and (other.pages, other.width) == plan(cached, new)[3:]:
+            continue                                           # (lengths that are cut the same way)
+        with pytest.raises(ops().KernelError, match="plan"):
+            run(q, kv, None, other)
 
 
 # ---- streams, graphs, large offsets, together ----
