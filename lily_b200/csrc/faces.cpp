@@ -1,4 +1,4 @@
-// Python faces in C++ of the operators of a cache held to a budget: checks of arguments, what is allocated, the launch.
+// Python faces in C++ of the operators of a cache held to a budget and of those on numbers held in four bits: checks of arguments, what is allocated, the launch.
 //
 // A small call of these is over on the device in 3 to 6 us, and a face in Python, some seventy looks at its tensors and thirty numbers
 // through ctypes, takes 13 to 15 us of the host; here it is 5 to 6.  The kernels stay what they are, C entries over raw pointers in a library
@@ -12,6 +12,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -20,6 +21,7 @@
 #include <cstdint>
 #include <sstream>
 #include <string>
+#include <tuple>
 #include <vector>
 
 namespace {
@@ -55,6 +57,9 @@ struct Entries {
     int (*values4)(const void*, int, const int*, int, int, void*, int, int, int, int, const int*, const int*, int*, int, int, const unsigned*, void*);
     size_t (*decode4_floats)(int, int, int, int, int, int, int);
     int (*decode4)(const void*, const void*, void*, const int*, int, const int*, float*, int, int, int, int, int, int, int, float, int, void*);
+    int (*halves4)(const void*, int, int, const void*, int, const int*, int, int, int, int, int, const int*, const int*, int, unsigned*, size_t, void*, float*, void*);
+    int (*prefill_tc_half)(const void*, const void*, void*, const int*, int, const int*, const int*, const int*, const int*, int, int, int, int, int, float, int, int, const unsigned*, const float*, void*);
+    int (*prefill_mma_half)(const void*, const void*, void*, const int*, int, const int*, const int*, const int*, const int*, int, int, int, int, int, float, const unsigned*, const float*, void*);
 } entry;
 
 // ---- words ----
@@ -534,11 +539,115 @@ PyObject* attention_decode4(PyObject*, PyObject* const* p, Py_ssize_t count) {
     });
 }
 
+// How portions are cut: (request, offset) of each tile of ``rows`` new tokens in the order of the keys that it sees, and the pages that portions see.
+struct Cut4 { Tensor req, start; int64_t pages, width; };
+Cut4 cut4(const char* what, const std::vector<int>& prefix, const std::vector<int>& fresh, int page, int rows, int device) {
+    if (prefix.size() != fresh.size() || page < 1 || rows < 1) refuse(what, ": ", fresh.size(), " portions behind ", prefix.size(), " lengths, pages of ", page, " places");
+    std::vector<std::tuple<int64_t, int, int>> tiles;
+    Cut4 c{{}, {}, 0, 0};
+    for (size_t r = 0; r < fresh.size(); ++r) {
+        if (fresh[r] < 0 || prefix[r] < 0) refuse(what, ": a portion of ", fresh[r], " tokens behind ", prefix[r]);
+        if (fresh[r] == 0) continue;
+        const int64_t pages = ((int64_t)prefix[r] + fresh[r] + page - 1) / page;
+        c.pages += pages;
+        c.width = std::max(c.width, pages);
+        for (int64_t at = 0; at < fresh[r]; at += rows) tiles.emplace_back(prefix[r] + at, (int)r, (int)at);
+    }
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) refuse(what, ": a captured call's plan is made ahead of the capture");
+    std::sort(tiles.begin(), tiles.end());
+    const int64_t n = (int64_t)tiles.size();
+    Tensor host = at::empty({2, n}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
+    int* at = host.data_ptr<int>();
+    for (int64_t i = 0; i < n; ++i) at[i] = std::get<1>(tiles[i]), at[n + i] = std::get<2>(tiles[i]);
+    const Tensor both = host.to(at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)device), /*non_blocking=*/true);
+    c.req = both.select(0, 0);
+    c.start = both.select(0, 1);
+    return c;
+}
+
+// lengths of prefixes, of portions, page_size, rows of a tile, the device's index -> (requests, offsets, pages, width)
+PyObject* plan4(PyObject*, PyObject* const* p, Py_ssize_t count) {
+    return guarded(count, 5, [&]() -> PyObject* {
+        Cut4 c = cut4("plan_prefill4", lengths(p[0]), lengths(p[1]), number(p[2]), number(p[3]), number(p[4]));
+        return Py_BuildValue("(NNLL)", THPVariable_Wrap(std::move(c.req)), THPVariable_Wrap(std::move(c.start)), (long long)c.pages, (long long)c.width);
+    });
+}
+
+// q, kv_layer, block_table, cu_seqlens, prefix_lens, lengths of prefixes, of portions, nq, nkv, d, page_size, scale, out, a plan's (rows, requests, offsets, pages, width) or None, rows of a tile, the
+// kernel: 0 neither, 1 mma.sync, 2 tcgen05 -> out; for 0 (out, requests, offsets, pages, width), nothing launched
+PyObject* attention_prefill4(PyObject*, PyObject* const* p, Py_ssize_t count) {
+    return guarded(count, 16, [&]() -> PyObject* {
+        const char* what = "attention_prefill4";
+        const Tensor &q = tensor(p[0]), &kv = tensor(p[1]), &table = tensor(p[2]), &cu = tensor(p[3]), &prefix = tensor(p[4]);
+        const std::vector<int> cached = lengths(p[5]), fresh = lengths(p[6]);
+        const int nq = number(p[7]), nkv = number(p[8]), d = number(p[9]), page = number(p[10]), rows = number(p[14]), kernel = number(p[15]);
+        const float scale = real(p[11]);
+        const Tensor* given = maybe(p[12]);
+        const int64_t requests = (int64_t)fresh.size();
+        if (nkv < 1 || nq < 1 || nq % nkv || page < 1 || (int64_t)cached.size() != requests)
+            refuse(what, ": ", requests, " portions behind ", cached.size(), " lengths, ", nq, " query heads over ", nkv, " kv heads, pages of ", page, " places");
+        layer4_fits(what, kv, nkv, page, d);
+        code_of(q);
+        int64_t tokens = 0;
+        for (size_t r = 0; r < fresh.size(); ++r) {
+            if (fresh[r] < 0 || cached[r] < 0) refuse(what, ": a portion of ", fresh[r], " tokens behind ", cached[r]);
+            tokens += fresh[r];
+        }
+        if (q.dim() != 2 || q.size(1) != (int64_t)nq * d || q.size(0) < tokens) refuse(what, ": queries are [tokens, ", (int64_t)nq * d, "], got ", words(q), " for ", tokens, " tokens");
+        if (cu.numel() != requests + 1 || prefix.numel() != requests) refuse(what, ": ", requests, " portions have a prefix each and ", requests + 1, " offsets");
+        const int *offsets = ints(cu, "cu_seqlens"), *behind = ints(prefix, "prefix_lens");
+        const int width = requests ? table_width(what, table, requests) : 0;
+        if (given && (given->scalar_type() != q.scalar_type() || given->sizes() != q.sizes())) refuse(what, ": out has the shape and dtype of q");
+        if (!(scale > 0.f) || scale > 3.4e38f) refuse(what, ": a scale of ", scale);
+        here({&q, &kv, &table, &cu, &prefix, given});
+        Cut4 c;
+        if (p[13] == Py_None) c = cut4(what, cached, fresh, page, rows, q.get_device());
+        else {
+            if (!PyTuple_Check(p[13]) || PyTuple_GET_SIZE(p[13]) != 5) refuse(what, ": a plan is what plan_prefill4 gives");
+            c = {tensor(PyTuple_GET_ITEM(p[13], 1)), tensor(PyTuple_GET_ITEM(p[13], 2)), whole(PyTuple_GET_ITEM(p[13], 3)), whole(PyTuple_GET_ITEM(p[13], 4))};
+            int64_t pages = 0, most = 0, tiles = 0;
+            for (size_t r = 0; r < fresh.size(); ++r) {
+                const int64_t own = fresh[r] ? ((int64_t)cached[r] + fresh[r] + page - 1) / page : 0;
+                pages += own;
+                most = std::max(most, own);
+                tiles += ((int64_t)fresh[r] + rows - 1) / rows;
+            }
+            if (whole(PyTuple_GET_ITEM(p[13], 0)) != rows || c.pages != pages || c.width != most || c.req.numel() != tiles || c.start.numel() != tiles)
+                refuse(what, ": the plan is not one of these portions (", tiles, " tiles of ", rows, " tokens, ", pages, " pages)");
+            ints(c.req, "a plan's requests"), ints(c.start, "a plan's offsets");
+            here({&c.req, &c.start});
+        }
+        if (c.width > width) refuse(what, ": ", c.width, " pages of a request; the block table holds ", width);
+        Tensor out = given ? *given : at::empty_like(q);
+        if (kernel == 0) return Py_BuildValue("(NNNLL)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(c.req)), THPVariable_Wrap(std::move(c.start)), (long long)c.pages, (long long)c.width);
+        if (!is(q, at::kBFloat16)) refuse(what, ": these kernels take bfloat16");
+        if (tokens == 0) return THPVariable_Wrap(std::move(out));
+        // the keys' spans and the block table of the numbers, zeros; the numbers of the pages; queries in half precision and what undoes their powers of two
+        const int64_t spans_n = requests * nkv, words_n = spans_n + requests * c.width;
+        Tensor zeroed = at::empty({words_n}, q.options().dtype(at::kInt)), values = at::empty({c.pages, 2, (int64_t)nkv, (int64_t)page, (int64_t)d}, q.options());
+        Tensor heads = at::empty_like(q), units = at::empty({q.size(0), (int64_t)nq}, q.options().dtype(at::kFloat));
+        unsigned* spans = (unsigned*)zeroed.data_ptr<int>();
+        int* numbers = zeroed.data_ptr<int>() + spans_n;
+        const int *bt = table.const_data_ptr<int>(), *tile_req = c.req.const_data_ptr<int>(), *tile_start = c.start.const_data_ptr<int>();
+        const int n = narrow(q.size(0)), pages = narrow(c.pages), wide = narrow(c.width), r = narrow(requests), tiles = narrow(c.req.numel()), held = narrow(kv.size(0));
+        done("lily_halves4", call(entry.halves4, q.const_data_ptr(), n, nq, kv.const_data_ptr(), held, bt, r, width, nkv, d, page, offsets, behind, wide, spans, (size_t)words_n * 4, heads.data_ptr(),
+                                  units.data_ptr<float>(), stream()));
+        done("lily_cache4_values", call(entry.values4, kv.const_data_ptr(), held, bt, r, width, values.data_ptr(), BF16, nkv, d, page, offsets, behind, numbers, wide, pages, (const unsigned*)spans, stream()));
+        if (kernel == 2)
+            done("lily_attention_prefill_tc_half", call(entry.prefill_tc_half, heads.const_data_ptr(), values.const_data_ptr(), out.data_ptr(), (const int*)numbers, wide, offsets, behind, tile_req, tile_start,
+                                                        tiles, nq, nkv, d, page, scale, n, pages, (const unsigned*)spans, units.const_data_ptr<float>(), stream()));
+        else
+            done("lily_attention_prefill_mma_half", call(entry.prefill_mma_half, heads.const_data_ptr(), values.const_data_ptr(), out.data_ptr(), (const int*)numbers, wide, offsets, behind, tile_req,
+                                                         tile_start, tiles, nq, nkv, d, page, scale, (const unsigned*)spans, units.const_data_ptr<float>(), stream()));
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
 // the addresses of the entries for numbers held in four bits, in their order
 PyObject* bind4(PyObject*, PyObject* const* p, Py_ssize_t count) {
-    return guarded(count, 7, [&]() -> PyObject* {
-        void* at[7];
-        for (int i = 0; i < 7; ++i) at[i] = (void*)(uintptr_t)whole(p[i]);
+    return guarded(count, 10, [&]() -> PyObject* {
+        void* at[10];
+        for (int i = 0; i < 10; ++i) at[i] = (void*)(uintptr_t)whole(p[i]);
         entry.linear4 = (decltype(entry.linear4))at[0];
         entry.weights4 = (decltype(entry.weights4))at[1];
         entry.write4 = (decltype(entry.write4))at[2];
@@ -546,13 +655,16 @@ PyObject* bind4(PyObject*, PyObject* const* p, Py_ssize_t count) {
         entry.decode4_floats = (decltype(entry.decode4_floats))at[4];
         entry.decode4 = (decltype(entry.decode4))at[5];
         entry.linear4_many = (decltype(entry.linear4_many))at[6];
+        entry.halves4 = (decltype(entry.halves4))at[7];
+        entry.prefill_tc_half = (decltype(entry.prefill_tc_half))at[8];
+        entry.prefill_mma_half = (decltype(entry.prefill_mma_half))at[9];
         Py_RETURN_NONE;
     });
 }
 
 #define FACE(name) {#name, (PyCFunction)(void (*)())name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FACE(axes_rope_write), FACE(attention_decode_weighed), FACE(select_keys), FACE(move_keys), FACE(key_weights_scratch_floats), FACE(attention_key_weights),
-                         FACE(bind), FACE(linear4), FACE(weights4), FACE(qk_norm_rope_write4), FACE(cache4_values), FACE(attention_decode4), FACE(bind4), {nullptr, nullptr, 0, nullptr}};
+                         FACE(bind), FACE(linear4), FACE(weights4), FACE(qk_norm_rope_write4), FACE(cache4_values), FACE(attention_decode4), FACE(plan4), FACE(attention_prefill4), FACE(bind4), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "lily_faces", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

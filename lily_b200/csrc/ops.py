@@ -102,9 +102,6 @@ _SIGNATURES = {
     "lily_apply_penalties": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_top_logprobs": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_cache4_values": [_vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _vp],
-    "lily_halves4": [_vp, _i, _i, _vp, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp],
-    "lily_attention_prefill_tc_half": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _vp, _vp],
-    "lily_attention_prefill_mma_half": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp],
     "lily_linear4_status": [],
     "lily_sample": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
 }
@@ -1219,7 +1216,8 @@ def _faces():
                  "lily_key_weights", "lily_key_weights_floats", "lily_key_weights_tc", "lily_key_weights_tc_floats", "lily_key_weights_tc_takes")
         address = lambda n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value
         module.bind(KernelError, *[address(n) for n in names])
-        module.bind4(*[address(n) for n in ("lily_linear4", "lily_weights4", "lily_qk_norm_rope_write4", "lily_cache4_values", "lily_attention_decode4_floats", "lily_attention_decode4", "lily_linear4_many")])
+        module.bind4(*[address(n) for n in ("lily_linear4", "lily_weights4", "lily_qk_norm_rope_write4", "lily_cache4_values", "lily_attention_decode4_floats", "lily_attention_decode4", "lily_linear4_many", "lily_halves4",
+                                               "lily_attention_prefill_tc_half", "lily_attention_prefill_mma_half")])
         _module = module
     return _module
 
@@ -1488,10 +1486,10 @@ class Prefill4Plan(NamedTuple):
 
 
 def plan_prefill4(dtype: torch.dtype, d: int, page_size: int, h_prefix_lens: Sequence[int], h_new_lens: Sequence[int], device) -> Prefill4Plan:
-    """The plan of ``attention_prefill4`` for portions of these lengths; a step's layers share one."""
-    pages = [-(-(p + n) // page_size) if n else 0 for p, n in zip(h_prefix_lens, h_new_lens)]
+    """The plan of ``attention_prefill4`` for portions of these lengths; a step's layers share one, and a captured call's is made ahead of the capture."""
+    device = torch.device(device)
     rows = prefill_tile_rows(dtype, d, page_size, sum(h_new_lens))
-    return Prefill4Plan(rows, *prefill_tiles(h_prefix_lens, h_new_lens, 0, rows, device), sum(pages), max(pages, default=0))
+    return Prefill4Plan(rows, *(_module or _faces()).plan4(h_prefix_lens, h_new_lens, page_size, rows, torch.cuda.current_device() if device.index is None else device.index))
 
 
 def attention_prefill4(q: torch.Tensor, kv_layer: torch.Tensor, block_table: torch.Tensor, cu_seqlens: torch.Tensor, prefix_lens: torch.Tensor, h_prefix_lens: Sequence[int],
@@ -1500,54 +1498,22 @@ def attention_prefill4(q: torch.Tensor, kv_layer: torch.Tensor, block_table: tor
     """Causal attention of prompt portions over a cache held in four bits: each request's new tokens (rows ``cu_seqlens`` of ``q`` [tokens, nq * d]) over its cached prefix and themselves, whose keys are in
     the cache already.  ``h_prefix_lens``, ``h_new_lens``: the lengths on the host, by which the work is cut (``plan``: ``plan_prefill4`` of them, made here where not given).  The pages that the
     portions see are brought to numbers first, and the kernels of ``attention_prefill`` read those: float32, or values in bfloat16 with keys (and queries) in half precision, whose bits hold them.  Rows of ``out`` that no portion has stay as they are."""
-    _dev(q, kv_layer, block_table, cu_seqlens, prefix_lens, out)
-    requests = len(h_new_lens)
-    if nkv < 1 or nq < 1 or nq % nkv or page_size < 1 or len(h_prefix_lens) != requests or any(n < 0 or p < 0 for n, p in zip(h_new_lens, h_prefix_lens)):
-        raise KernelError(f"attention_prefill4: portions of {tuple(h_new_lens)} behind {tuple(h_prefix_lens)}, {nq} query heads over {nkv} kv heads")
-    if kv_layer.dtype != torch.uint8 or tuple(kv_layer.shape[1:]) != cache4_shape(nkv, page_size, d):
-        raise KernelError(f"attention_prefill4: a cache layer is uint8 [pages, {', '.join(map(str, cache4_shape(nkv, page_size, d)))}], got {kv_layer.dtype} {tuple(kv_layer.shape)}")
-    tokens = sum(h_new_lens)
-    if q.dim() != 2 or q.shape[1] != nq * d or q.shape[0] < tokens:
-        raise KernelError(f"attention_prefill4: queries are [tokens, {nq * d}], got {tuple(q.shape)} for {tokens} tokens")
-    if cu_seqlens.numel() != requests + 1 or prefix_lens.numel() != requests or block_table.dim() != 2 or block_table.shape[0] != requests:
-        raise KernelError(f"attention_prefill4: {requests} portions have a prefix and a row of the block table each and {requests + 1} offsets")
-    if out is None:
-        out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype:
-        raise KernelError("attention_prefill4: out has the shape and dtype of q")
-    if tokens == 0:
-        return out
-    if plan is None:
-        plan = plan_prefill4(q.dtype, d, page_size, h_prefix_lens, h_new_lens, q.device)
-    else:
-        _dev(plan.tile_req, plan.tile_start)
-        pages = [-(-(p + n) // page_size) if n else 0 for p, n in zip(h_prefix_lens, h_new_lens)]
-        if (plan.pages, plan.width) != (sum(pages), max(pages)) or plan.rows != prefill_tile_rows(q.dtype, d, page_size, tokens) or plan.tile_req.numel() != sum(-(-n // plan.rows) for n in h_new_lens):
-            raise KernelError(f"attention_prefill4: the plan is not one of portions of {tuple(h_new_lens)} behind {tuple(h_prefix_lens)}")
-    if plan.width > block_table.shape[1]:
-        raise KernelError(f"attention_prefill4: {plan.width} pages of a request; the block table holds {block_table.shape[1]}")
-    if not 0 < scale < float("inf"):
-        raise KernelError(f"attention_prefill4: a scale of {scale}")
-    values = torch.empty((plan.pages, 2, nkv, page_size, d), dtype=q.dtype, device=q.device)
-    words = torch.zeros((requests * (nkv + plan.width),), dtype=torch.int32, device=q.device)
-    spans, table = words[:requests * nkv], words[requests * nkv:].view(requests, plan.width)
+    tokens, face = sum(h_new_lens), _module or _faces()
+    rows = prefill_tile_rows(q.dtype, d, page_size, tokens)
     # (the tensor-core kernels; others, of float32 and of pages that are no power of two, read the numbers themselves)
     halves = uses_tensor_cores(q.dtype, d) and page_size & (page_size - 1) == 0
-    heads = q
-    if halves:
-        heads, units = torch.empty_like(q), torch.empty((q.shape[0], nq), dtype=torch.float32, device=q.device)
-        _call("lily_halves4", _p(q), q.shape[0], nq, _p(kv_layer), kv_layer.shape[0], _i32(block_table, "block_table"), requests, block_table.shape[1], nkv, d, page_size,
-              _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens"), plan.width, _p(spans), _p(heads), _p(units), _stream())
-    _call("lily_cache4_values", _p(kv_layer), kv_layer.shape[0], _i32(block_table, "block_table"), requests, block_table.shape[1], _p(values), _dt(q), nkv, d, page_size,
-          _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens"), _p(table), plan.width, plan.pages, _p(spans) if halves else None, _stream())
-    if not halves:
-        attention_prefill(q, values, table, cu_seqlens, prefix_lens, plan.tile_req, plan.tile_start, out, nq, nkv, d, page_size, scale, tile_rows=plan.rows)
+    kernel = 0 if not halves else 2 if rows == int(library().lily_attention_prefill_tc_rows()) else 1
+    done = face.attention_prefill4(q, kv_layer, block_table, cu_seqlens, prefix_lens, h_prefix_lens, h_new_lens, nq, nkv, d, page_size, scale, out, plan, rows, kernel)
+    if kernel:
+        launches["count"] += 4 if tokens else 0
+        return done
+    out, tile_req, tile_start, pages, width = done
+    if tokens == 0:
         return out
-    common = (_p(heads), _p(values), _p(out), _p(table), plan.width, _p(cu_seqlens), _p(prefix_lens), _p(plan.tile_req), _p(plan.tile_start), plan.tile_req.numel(), nq, nkv, d, page_size, float(scale))
-    if plan.rows == int(library().lily_attention_prefill_tc_rows()):
-        _call("lily_attention_prefill_tc_half", *common, q.shape[0], plan.pages, _p(spans), _p(units), _stream())
-    else:
-        _call("lily_attention_prefill_mma_half", *common, _p(spans), _p(units), _stream())
+    values, table = torch.empty((pages, 2, nkv, page_size, d), dtype=q.dtype, device=q.device), torch.zeros((len(h_new_lens), width), dtype=torch.int32, device=q.device)
+    _call("lily_cache4_values", _p(kv_layer), kv_layer.shape[0], _i32(block_table, "block_table"), len(h_new_lens), block_table.shape[1], _p(values), _dt(q), nkv, d, page_size,
+          _i32(cu_seqlens, "cu_seqlens"), _i32(prefix_lens, "prefix_lens"), _p(table), width, pages, None, _stream())
+    attention_prefill(q, values, table, cu_seqlens, prefix_lens, tile_req, tile_start, out, nq, nkv, d, page_size, scale, tile_rows=rows)
     return out
 
 

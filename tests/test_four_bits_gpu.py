@@ -442,6 +442,29 @@ def test_portions_refuse_a_plan_of_others():
             run(q, kv, None, other)
 
 
+@pytest.mark.parametrize("page", [16, 64])
+def test_portions_in_a_graph(page):
+    """A captured call has its plan made ahead, and is refused without one; what is replayed follows the queries and the cache."""
+    new, cached, nq, nkv, d = [130, 1, 70], [3, 200, 0], 8, 2, 128
+    q, kv, run, _ = portions_case(new, cached, nq, nkv, d, page)
+    plan, out, stream = ops().plan_prefill4(BF16, d, page, cached, new, q.device), torch.zeros_like(q), torch.cuda.Stream()
+    want = [run(x, kv) for x in (q, q.flip(0).contiguous())]
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            with pytest.raises(ops().KernelError, match="ahead of the capture"):
+                run(q, kv, out)
+            run(q, kv, out, plan)
+        graph.replay()
+        stream.synchronize()
+        assert torch.equal(out, want[0])
+        q.copy_(q.flip(0).contiguous())
+        graph.replay()
+        stream.synchronize()
+        assert torch.equal(out, want[1])
+
+
 # ---- streams, graphs, large offsets, together ----
 
 def test_on_another_stream_and_in_a_graph():
