@@ -36,8 +36,8 @@ class KeyBudget:
         if cache.device is None:
             raise ValueError("a cache without device tensors has nothing to evict")
         for g in cache.groups:
-            if g.need.window is not None or g.need.values_in_keys or g.need.v_head_dim not in (None, g.need.head_dim):
-                raise ValueError("a budget is for caches of all keys, with keys and values of one head size")
+            if g.need.window is not None or g.need.values_in_keys or g.need.v_head_dim not in (None, g.need.head_dim) or g.need.four_bits:
+                raise ValueError("a budget is for caches of all keys, with keys and values of one head size, not held in four bits")
         if cache.state_needs:
             raise ValueError("a mixer with a state of its own does not live on cached keys alone")
         if ops is None:

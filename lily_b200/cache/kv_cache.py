@@ -88,6 +88,8 @@ class KVCacheManager:
                     (need.kv_heads * page_size * (need.head_dim + value_columns(need)),)
                 if need.four_bits:
                     shape = (need.kv_heads, 2, page_size * four_bit_bytes(need) // 2)
+                    if layers > 1 and (num_pages + 1) * need.kv_heads * page_size * four_bit_bytes(need) % 16:
+                        raise ValueError(f"pages of {page_size} places of {need.kv_heads} heads of {need.head_dim} in four bits: {num_pages} of them do not end on a boundary of sixteen bytes")
                 data = torch.zeros((layers, num_pages + 1, *shape), dtype=torch.uint8 if need.four_bits else dtype, device=device)
             self.groups.append(CacheGroup(need, layers, GroupTables(num_pages, page_size, need.window, need.keep_first), data))
         self.state_needs = list(states)

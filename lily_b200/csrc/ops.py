@@ -1444,7 +1444,7 @@ def qk_norm_rope_write4(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_gai
     """``qk_norm_rope_write`` into a cache held in four bits (``kv_layer`` uint8 [pages, *cache4_shape]): per-head RMSNorm of q and k (when gains are given), rotation by the tables, q to ``q_out``
     [tokens, nq * d], k and v, 64 features at a time, as codes round((x - lowest) / step) with step = (max - min) / 15.  A token's codes depend on its own numbers alone, to the bit.
     A group that holds what is not finite reads as NaN.  ``qkv`` [tokens, (nq + 2 nkv) d] float32 or bfloat16.  A position outside the tables gives NaN; what has a position or a request outside
-    the block table is not written."""
+    the block table is not written; no two tokens of a call have one place."""
     q = (_module or _faces()).qk_norm_rope_write4(qkv, q_gain, k_gain, eps, cos, sin, positions, token_req, block_table, kv_layer, nq, nkv, d, rotary_dim, page_size, q_out)
     launches["count"] += 1
     return q

@@ -7,7 +7,10 @@ import pytest
 import torch
 
 import four_bits as fb
+import godotar_models
 import kernel_refs
+from harness import make_runner
+from lily_b200.cache.key_budget import KeyBudget
 from lily_b200.cache.kv_cache import KVCacheManager, bytes_per_token
 from lily_b200.config.server_args import ServerArgs
 from lily_b200.csrc import ops
@@ -161,6 +164,23 @@ def test_cache_in_four_bits():
                 CacheNeed(1, 128, values_in_keys=True, four_bits=True)):
         with pytest.raises(ValueError):
             bytes_per_token([(bad, 1)], torch.bfloat16)
+
+
+def test_what_goes_with_a_cache_in_four_bits():
+    """Layers that begin on boundaries of sixteen bytes; no budget of places, whose keys are moved as numbers."""
+    make = lambda need, layers, page, pages: KVCacheManager([(need, layers)], [], page_size=page, num_pages=pages, max_requests=2, max_context=8, device=torch.device("cpu"))
+    need = CacheNeed(1, 64, four_bits=True)
+    make(need, 1, 1, 4), make(need, 3, 1, 5), make(need, 3, 2, 4)
+    with pytest.raises(ValueError, match="sixteen"):
+        make(need, 3, 1, 4)
+    with pytest.raises(ValueError, match="four bits"):
+        KeyBudget(make(need, 1, 2, 4), keep=4, first=1, recent=1, slack=1, ops=kernel_refs)
+
+
+def test_architectures_that_cache_something_else_are_refused(tmp_path):
+    path = godotar_models.write_model_dir(str(tmp_path / "m"), godotar_models.WIDE, godotar_models.make_weights(godotar_models.WIDE, 3))
+    with pytest.raises(ValueError, match="four bits"):
+        make_runner(path, kv_cache_dtype="int4")
 
 
 @pytest.mark.parametrize("more", [dict(window=32), dict(softcap=30.0), dict(v_head_dim=128), dict(head_dim=32), dict(sink=True), dict(talk=True), dict(v_norm=True), dict(conv_taps=2),
