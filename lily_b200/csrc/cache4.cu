@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__
             const uint32_t of = G == 1 ? h[0] : G == 2 ? (j ? h[1] : h[0]) : G == 3 ? (j == 0 ? h[0] : j == 1 ? h[1] : h[G - 1]) : (j < 2 ? (j ? h[1] : h[0]) : (j == 2 ? h[2 % G] : h[G - 1]));
             float v[8];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) v[c] = slot < places ? fmaf((float)(w[e] >> (4 * c) & 15u), low(of), high(of)) : 0.f;
+            for (int c = 0; c < 8; ++c) v[c] = slot < places ? fmaf(__uint_as_float((w[e] >> (4 * c) & 15u) | 0x4B000000u) - 8388608.f, low(of), high(of)) : 0.f;
             if (halves) store_halves(dst + (size_t)slot * D + l * 8, v, by);
             else store8(dst + (size_t)slot * D + l * 8, v);
         }
@@ -350,10 +350,21 @@ __global__ void __launch_bounds__(256) halves_kernel(const __nv_bfloat16* __rest
         const int words = d / 8, per_warp = 32 / words, mine = lane / words, l = lane - mine * words;      // (d = 192: lanes 24 to 31 have no word)
         const size_t head = ((size_t)blockIdx.x * 8 + warp) * per_warp + mine;
         const bool in = mine < per_warp && head < heads;
-        float v[8] = {};
-        if (in) load8(q + head * d + l * 8, v);
+        uint4 raw = make_uint4(0, 0, 0, 0);
+        if (in) raw = *reinterpret_cast<const uint4*>(q + head * d + l * 8);
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) take(v[i]);
+        for (int i = 0; i < 4; ++i) v[2 * i] = low(w[i]), v[2 * i + 1] = high(w[i]);
+        uint32_t most_w = 0;                                          // magnitudes as whole numbers, two at a time; those of infinities and of what is no number are the largest
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most_w = __vmaxu2(most_w, w[i] & 0x7fff7fffu);
+        m = __uint_as_float(max(most_w & 0xffffu, most_w >> 16) << 16);
+        if (!(m <= 3e38f)) {
+            m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) take(v[i]);
+        }
         for (int o = words == 24 ? 16 : words >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         if (!in) return;
         store_halves(out + head * d + l * 8, v, span_multiplier(__float_as_uint(m)));

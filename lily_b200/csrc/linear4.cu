@@ -252,26 +252,43 @@ __global__ void __launch_bounds__(32 * F32_WARPS, 2) product_f32_kernel(const Pr
     }
 }
 
-// The weights as numbers [n, k] (float32: exact; bfloat16: rounded once).  A thread a word of eight codes.
+// The weights as numbers [n, k] (float32: exact; bfloat16: rounded once).  A warp eight rows of a tile, a lane sixteen bytes of codes, four words of eight.  In bfloat16 code - zero is exact and its product
+// with the scale one rounding, of two numbers an operation.  6,144 x 4,096 in bfloat16 10.6 us with the empty kernel behind it, 0.9 of what its bytes take (a word a thread 14.4, number by number besides 16.8).
+// grid (tiles of columns / 8, rows / 8)
 template <typename T>
-__global__ void __launch_bounds__(256) weights_kernel(const ProductArgs a, int group) {
+__global__ void __launch_bounds__(256) weights_kernel(const ProductArgs a, int group_shift) {
     pdl_enter_small();
-    const int words = a.k / 8, row = blockIdx.y * 8 + (threadIdx.x >> 5);
-    const int per_tile = 128 / group;
-    if (row >= a.n) return;
-    for (int l = blockIdx.x * 32 + (threadIdx.x & 31); l < words; l += gridDim.x * 32) {
-        const int kt = l >> 4, in = l & 15;                           // word `in` of the tile: columns 8 in + (0..7)
-        const uint32_t w = reinterpret_cast<const uint32_t*>(a.codes + (((size_t)(row / 128) * a.tiles + kt) * 128 + row % 128) * 64)[(in & 3) * 4 + (in >> 2)];
-        const size_t at = ((size_t)(row / 128) * a.tiles * per_tile + (size_t)l * 8 / group) * 128 + row % 128;
-        const float s = __bfloat162float(a.scales[at]), z = a.zeros ? (float)a.zeros[at] : 8.f;
-        T* dst = (T*)a.out + (size_t)row * a.k + (size_t)l * 8;
-        float v[8];
+    const int lane = threadIdx.x & 31, t = lane & 3, row = blockIdx.y * 8 + (lane >> 2), kt = blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (kt >= a.tiles || row >= a.n) return;
+    const uint4 codes = weights16(a.codes + (((size_t)(row / 128) * a.tiles + kt) * 128 + row % 128) * 64 + t * 16);
+    const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
+    const size_t held0 = (size_t)(row / 128) * (a.tiles * 128 >> group_shift) * 128 + row % 128;
+    __nv_bfloat16 scales[4];
+    uint32_t zeros[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = ((float)(w >> (4 * e) & 15u) - z) * s;
-        if constexpr (sizeof(T) == 2)
-            *reinterpret_cast<uint4*>(dst) = make_uint4(bits(__floats2bfloat162_rn(v[0], v[1])), bits(__floats2bfloat162_rn(v[2], v[3])), bits(__floats2bfloat162_rn(v[4], v[5])),
-                                                        bits(__floats2bfloat162_rn(v[6], v[7])));
-        else {
+    for (int w = 0; w < 4; ++w) {
+        const int col = kt * 128 + 32 * w;
+        const size_t at = held0 + (size_t)(col >> group_shift) * 128;
+        scales[w] = col < a.k ? a.scales[at] : __ushort_as_bfloat16(0);
+        zeros[w] = a.zeros && col < a.k ? a.zeros[at] : 8u;
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int col = kt * 128 + 32 * w + 8 * t;
+        if (col >= a.k) break;
+        T* dst = (T*)a.out + (size_t)row * a.k + col;
+        if constexpr (sizeof(T) == 2) {
+            const uint32_t z = (0x4300u | zeros[w]) * 0x10001u;       // 128 + zero, twice
+            const __nv_bfloat162 s = __halves2bfloat162(scales[w], scales[w]);
+            uint32_t p[4];                                            // numbers i and i + 4
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = bits(__hmul2(two(minus(pair(words[w], i), z)), s));
+            *reinterpret_cast<uint4*>(dst) = make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410), __byte_perm(p[0], p[1], 0x7632), __byte_perm(p[2], p[3], 0x7632));
+        } else {
+            const float s = __bfloat162float(scales[w]), z = __uint_as_float(0x4B000000u | zeros[w]);      // (2^23 + zero)
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = (__uint_as_float((words[w] >> (4 * e) & 15u) | 0x4B000000u) - z) * s;
             reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
             reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
         }
@@ -336,9 +353,10 @@ LILY_API int lily_weights4(const void* codes, const void* scales, const void* ze
     const four::ProductArgs a{nullptr, (const uint8_t*)codes, (const __nv_bfloat16*)scales, (const uint8_t*)zeros, nullptr, 0, out, 0, 0, n, k, (k + 127) / 128};
     const int rows = (n + 7) / 8;
     LILY_REQUIRE(rows <= 65535, "weights4: %d rows", n);
-    const dim3 grid((k / 8 + 127) / 128, rows);
-    if (dtype == kF32) launch_pdl(four::weights_kernel<float>, grid, dim3(256), 0, stream, a, group);
-    else launch_pdl(four::weights_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, a, group);
+    const dim3 grid((a.tiles + 7) / 8, rows);
+    const int shift = group == 32 ? 5 : group == 64 ? 6 : 7;
+    if (dtype == kF32) launch_pdl(four::weights_kernel<float>, grid, dim3(256), 0, stream, a, shift);
+    else launch_pdl(four::weights_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, a, shift);
     LILY_CHECK_LAUNCH("weights4");
     four::at_rest_kernel<<<1, 32, 0, stream>>>();
     LILY_CHECK_LAUNCH("weights4");
