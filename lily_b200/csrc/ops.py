@@ -1406,9 +1406,10 @@ def weights4(w: Weight4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
 
 def linear4_on_the_way(m: int, n: int, k: int) -> bool:
     """Whether a bfloat16 product of ``m`` tokens makes numbers of its codes on the way (tcgen05, a tile of 256 tokens at a time) rather than bringing the whole matrix to numbers in memory for
-    ``linear``, which pays for many tokens.  Measured, us, on the way / numbers and ``linear``: 4,096 x 12,288 16 / 53 with 64 tokens, 31 / 58 with 256, 58 / 72 with 512, 97 / 87 with 768;
-    24,576 x 4,096 83 / 109 with 256, 132 / 127 with 512; 4,096 x 4,096 19 / 21 with 256, 26 / 23 with 384; 2,048 x 2,048 7.6 / 10 with 64, 10.3 / 10 with 128, 22 / 10 with 256."""
-    return m <= 128 or (m <= 256 and n * k >= 1 << 24) or (m <= 512 and n * k >= 3 << 24)
+    ``linear``, which pays for many tokens.  Measured, us, on the way / numbers and ``linear``: 2,048 x 2,048 7.6 / 9.0 with 64 tokens, 9.7 / 8.6 with 128; 4,096 x 4,096 13.4 / 15.7 with 128, 16.1 / 16.0
+    with 192; 6,144 x 4,096 17.8 / 19.8 with 128, 30.6 / 22.6 with 256; 12,288 x 4,096 40.8 / 43.2 with 256, 68 / 49 with 384; 4,096 x 12,288 31 / 47 with 256, 55 / 60 with 512, 102 / 77 with 768."""
+    size = n * k
+    return m <= 64 or (m <= 128 and size >= 1 << 23) or (size >= 3 << 24 and m <= (512 if k >= 2 * n else 256))
 
 
 def linear4_status() -> int:

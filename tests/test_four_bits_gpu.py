@@ -50,6 +50,20 @@ def test_product(dtype, m, n, k, group, zeros):
     within(got, want, product_bound(x, w, want, dtype, dtype, dtype == BF16 and m > 16))
 
 
+@pytest.mark.parametrize("m", [17, 65, 128, 129, 256, 257, 300, 600])
+@pytest.mark.parametrize("n,k,group,zeros", [(130, 160, 32, True), (300, 1088, 64, False), (64, 4096, 128, True)])
+def test_product_on_the_way(m, n, k, group, zeros):
+    """The tcgen05 kernel itself, whichever side of the line sizes are."""
+    g = torch.Generator().manual_seed(m + n)
+    codes, scales, z = fb.make_matrix(n, k, group, zeros, g, DEV)
+    x = torch.randn(m, k, generator=g).to(BF16).to(DEV)
+    w = fb.matrix_values(codes, scales, z)
+    want = x.double() @ w.t()
+    got = ops()._faces().linear4(x, *ops().pack_weight4(codes, scales, z), None, False, 17)
+    within(got, want, product_bound(x, w, want, BF16, BF16, True))
+    assert ops().linear4_status() == 0
+
+
 @pytest.mark.parametrize("dtype,m,out", [(BF16, 5, BF16), (BF16, 5, F32), (BF16, 40, BF16), (BF16, 40, F32), (F32, 5, F32), (F32, 40, F32)])
 @pytest.mark.parametrize("bias_dtype", [None, BF16, F32])
 def test_product_with_bias_and_wide_result(dtype, m, out, bias_dtype):
