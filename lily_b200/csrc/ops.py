@@ -1406,10 +1406,10 @@ def weights4(w: Weight4, dtype: torch.dtype = torch.float32) -> torch.Tensor:
 
 def linear4_on_the_way(m: int, n: int, k: int) -> bool:
     """Whether a bfloat16 product of ``m`` tokens makes numbers of its codes on the way (tcgen05, a tile of 256 tokens at a time) rather than bringing the whole matrix to numbers in memory for
-    ``linear``, which pays for many tokens.  Measured, us, on the way / numbers and ``linear``: 2,048 x 2,048 7.6 / 9.0 with 64 tokens, 9.7 / 8.6 with 128; 4,096 x 4,096 13.4 / 15.7 with 128, 16.1 / 16.0
-    with 192; 6,144 x 4,096 17.8 / 19.8 with 128, 30.6 / 22.6 with 256; 12,288 x 4,096 40.8 / 43.2 with 256, 68 / 49 with 384; 4,096 x 12,288 31 / 47 with 256, 55 / 60 with 512, 102 / 77 with 768."""
-    size = n * k
-    return m <= 64 or (m <= 128 and size >= 1 << 23) or (size >= 3 << 24 and m <= (512 if k >= 2 * n else 256))
+    ``linear``, which pays for many tokens.  Measured on the device, us, on the way / numbers and ``linear``: 4,096 x 12,288 28 / 47 with 256 tokens, 45 / 60 with 512, 92 / 77 with 768; 24,576 x 4,096
+    62 / 90, 109 / 111, 144 / 139; 6,144 x 4,096 20 / 22, 30 / 30, 32 / 37 (1,024: 59 / 45); 12,288 x 4,096 30 / 43, 59 / 55, 69 / 70; 2,048 x 6,144 17 / 17, 18 / 20, 26 / 23; 2,048 x 2,048 7 / 8 with 64,
+    11 / 9 with 256, 13 / 10 with 512.  Up to 256 tokens the one launch is taken for small matrices too: what it may lose on the device, 2 us, is less than the 10 us of the host that three more take."""
+    return m <= 256 or (m <= 512 and n * k >= 1 << 24)
 
 
 def linear4_status() -> int:
