@@ -31,6 +31,7 @@ constexpr int FEW_WARPS = 8;
 
 // Up to 8 NT tokens: blocks walk tiles of 16 MT rows, their warps an eighth of the columns' tiles each; weights on the rows of the products, tokens on their eight columns.  A warp's weights
 // are one stream, from one tile of rows to the next, which it asks for DEPTH steps ahead (the first ones before the kernel ahead has ended); tokens stay in the L1.
+// What bounds it: logical operations and subtractions on the codes, of which a pair of codes takes two and a half (8 tokens, 24,576 x 4,096: 16.2 us, 3.2 TB/s of weights, the logic unit 55 % busy).
 template <int NT, int PER_GROUP, int MT>                              // PER_GROUP: words of a lane (32 columns each) that share a scale, 1, 2 or 4
 __global__ void __launch_bounds__(32 * FEW_WARPS, 2) product_few_kernel(const ProductArgs a, int row_tiles) {
     constexpr int GROUPS = 4 / PER_GROUP, ROWS = 16 * MT, DEPTH = GROUPS == 1 ? 3 : 2;
@@ -324,8 +325,9 @@ LILY_API int lily_linear4(const void* x, int dtype, const void* codes, const voi
         else if (m <= 4) launch_pdl(four::product_f32_kernel<4>, grid, block, 0, stream, a, shift);
         else launch_pdl(four::product_f32_kernel<four::F32_TOKENS>, grid, block, 0, stream, a, shift);
     } else {
-        // 32 rows a block and turn, 16 where that leaves SMs without
-        const int mt = (n + 31) / 32 <= sm_count() ? 1 : 2, row_tiles = (n + 16 * mt - 1) / (16 * mt);
+        // Up to eight tokens 32 rows a block and turn (24,576 x 4,096 with eight 16.2 us, 18.2 with 16 rows; 6,144 x 4,096 with four 5.9 and 7.2), 16 where that leaves SMs without (4,096 x 4,096 with one
+        // token 3.9 us, 5.3 with 32 rows).  From nine on 16, by the registers (12,288 x 4,096 with sixteen 15.0 us, 18.5 with 32; 4,096 x 12,288 14.4 and 26.3; 6,144 x 4,096 9.9 and 9.5).
+        const int mt = m > 8 || (n + 31) / 32 <= sm_count() ? 1 : 2, row_tiles = (n + 16 * mt - 1) / (16 * mt);
         const dim3 grid(min(row_tiles, 2 * sm_count())), block(32 * four::FEW_WARPS);
 #define FEW_OF(NT, MT)                                                                                               \
     do {                                                                                                             \
@@ -333,15 +335,10 @@ LILY_API int lily_linear4(const void* x, int dtype, const void* codes, const voi
         else if (group == 64) launch_pdl(four::product_few_kernel<NT, 2, MT>, grid, block, 0, stream, a, row_tiles); \
         else launch_pdl(four::product_few_kernel<NT, 1, MT>, grid, block, 0, stream, a, row_tiles);                  \
     } while (0)
-#define FEW(NT)                   \
-    do {                          \
-        if (mt == 1) FEW_OF(NT, 1); \
-        else FEW_OF(NT, 2);       \
-    } while (0)
-        if (m <= 8) FEW(1);
-        else FEW(2);
+        if (m > 8) FEW_OF(2, 1);
+        else if (mt == 1) FEW_OF(1, 1);
+        else FEW_OF(1, 2);
 #undef FEW_OF
-#undef FEW
     }
     LILY_CHECK_LAUNCH("linear4");
     return 0;
