@@ -11,6 +11,7 @@
 #include "four.cuh"
 #include "mma.cuh"
 #include <cuda_fp16.h>
+#include <type_traits>
 
 namespace lily {
 namespace four {
@@ -345,7 +346,10 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
             }
         }
         const uint32_t one[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-        auto work = [&](const unsigned char* tile, const int left) {
+        // Masks only where a request ends, elsewhere they took a select a score and a step (8 rows of 8,192 places 26.0 us, 26.5 with them).  Heads above 128 keep one form: two are more code than short
+        // rows fetch in time (heads of 256, 128 rows of 500 58 us, 65 with two).
+        auto work = [&](auto whole, const unsigned char* tile, const int left) {
+            constexpr bool WHOLE = decltype(whole)::value;
             float s[2][4];                                                // scores of keys g and g + 8, heads 2 t and 2 t + 1
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
@@ -373,7 +377,7 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
                     s[mt][2] = fmaf(s1, c[2], fmaf(b1, qs[j][0], s[mt][2]));
                     s[mt][3] = fmaf(s1, c[3], fmaf(b1, qs[j][1], s[mt][3]));
                 }
-                if (left < KT) {
+                if (!WHOLE) {
                     if (row >= left) s[mt][0] = s[mt][1] = -INFINITY;
                     if (row + 8 >= left) s[mt][2] = s[mt][3] = -INFINITY;
                 }
@@ -421,7 +425,7 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
                 for (int e = 0; e < 4; ++e) words_of<G>(tile + S::VALUES + (row + 2 * t + (e & 1) + (e >> 1) * 8) * S::VALUE_ROW + g * 4 * G, w[e]);
 #pragma unroll
                 for (int j = 0; j < G; ++j) {
-                    if (left < KT) {                                      // (what stands behind the last place may be no number)
+                    if (!WHOLE) {                                      // (what stands behind the last place may be no number)
                         if (row + g >= left) h0[j] = 0;
                         if (row + g + 8 >= left) h1[j] = 0;
                     }
@@ -447,7 +451,10 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
             ask();
             mma16::cp_async_wait<STAGES - 1>();
             __syncwarp();
-            work(mine + used % STAGES * S::BYTES, at.places - (at.tile + next - began) * KT);
+            const unsigned char* tile = mine + used % STAGES * S::BYTES;
+            const int left = at.places - (at.tile + next - began) * KT;
+            if (D <= 128 && left >= KT) work(std::true_type(), tile, left);
+            else work(std::false_type(), tile, left);
             __syncwarp();
         }
         // the warps' sums together: finished, where the whole pair was here; else to the part's slot

@@ -50,6 +50,22 @@ def test_product(dtype, m, n, k, group, zeros):
     within(got, want, product_bound(x, w, want, dtype, dtype, dtype == BF16 and m > 16))
 
 
+@pytest.mark.parametrize("m,out", [(300, BF16), (300, F32), (600, BF16), (600, F32)])
+@pytest.mark.parametrize("bias_dtype", [BF16, F32])
+def test_many_tokens_with_bias_and_wide_result(m, out, bias_dtype):
+    """Through numbers in memory, by ``linear4`` and by ``linear``."""
+    g = torch.Generator().manual_seed(m)
+    codes, scales, z = fb.make_matrix(300, 256, 64, True, g, DEV)
+    x, bias = torch.randn(m, 256, generator=g).to(BF16).to(DEV), torch.randn(300, generator=g).to(bias_dtype).to(DEV)
+    w, w4 = fb.matrix_values(codes, scales, z), ops().pack_weight4(codes, scales, z)
+    want = x.double() @ w.t() + bias.double()
+    for product in (ops().linear4, ops().linear):
+        got = product(x, w4, bias, out_dtype=out)
+        assert got.dtype == out
+        # (the library may round sums to bfloat16 ahead of the bias: one rounding more)
+        within(got, want, product_bound(x, w, want, BF16, out, True) + HALF[BF16] * ((want - bias.double()).abs() + bias.double().abs()))
+
+
 @pytest.mark.parametrize("m", [17, 65, 128, 129, 256, 257, 300, 600])
 @pytest.mark.parametrize("n,k,group,zeros", [(130, 160, 32, True), (300, 1088, 64, False), (64, 4096, 128, True)])
 def test_product_on_the_way(m, n, k, group, zeros):
