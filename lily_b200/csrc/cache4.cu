@@ -410,7 +410,7 @@ LILY_API int lily_qk_norm_rope_write4(const void* qkv, int dtype, int ld, const 
                                       void* q_out, int nq, int nkv, int d, int rd, int page_size, cudaStream_t stream) {
     if (tokens == 0) return 0;
     LILY_REQUIRE(four::head_fits(d), "qk_norm_rope_write4: heads of 64, 128, 192 or 256 features, not %d", d);
-    LILY_REQUIRE(rd >= 0 && rd <= d && rd % 2 == 0 && (rd == 0 || (cos_t && sin_t)), "qk_norm_rope_write4: rotary_dim %d does not fit head_dim %d", rd, d);
+    LILY_REQUIRE(rd >= 0 && rd <= d && rd % 2 == 0 && (rd == 0 || (cos_t && sin_t && table_rows > 0)), "qk_norm_rope_write4: rotary_dim %d does not fit head_dim %d, or tables of %d positions", rd, d, table_rows);
     LILY_REQUIRE(page_size > 0 && tokens > 0 && tokens <= 65535 * 32, "qk_norm_rope_write4: %d tokens, pages of %d places", tokens, page_size);
     LILY_REQUIRE(nq >= 0 && nkv >= 0 && nq + nkv > 0 && ld >= (nq + 2 * nkv) * d, "qk_norm_rope_write4: rows of %d numbers", ld);
     LILY_REQUIRE((q_gain == nullptr) == (k_gain == nullptr), "qk_norm_rope_write4: q and k gains come together");

@@ -468,7 +468,7 @@ PyObject* qk_norm_rope_write4(PyObject*, PyObject* const* p, Py_ssize_t count) {
         const int64_t n = qkv.size(0);
         const int code = code_of(qkv);
         if (rd < 0 || rd > d || rd % 2 || (rd && (!cos || !sin))) refuse(what, ": rotary_dim ", rd, " does not fit head_dim ", d, ", or has no tables");
-        if (rd && (!is(*cos, at::kFloat) || !is(*sin, at::kFloat) || cos->dim() != 2 || cos->size(1) != rd / 2 || sin->sizes() != cos->sizes()))
+        if (rd && (!is(*cos, at::kFloat) || !is(*sin, at::kFloat) || cos->dim() != 2 || cos->size(0) < 1 || cos->size(1) != rd / 2 || sin->sizes() != cos->sizes()))
             refuse(what, ": rotation tables are float32 [positions, rotary_dim / 2]");
         if (positions.numel() != n || req.numel() != n || table.dim() != 2 || table.size(1) < 1) refuse(what, ": ", n, " tokens have a position and a request each, and there is a block table");
         int gain = F32;

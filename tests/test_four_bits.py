@@ -112,7 +112,13 @@ DECODE = "pppp" "i" "pp" "iiiiiii" "f" "ip"          # q, kv, out, table, width,
 LINEAR = "pi" "pppp" "i" "p" "iiiii" "p"             # x, dtype, codes, scales, zeros, bias, bias_f32, out, out_f32, m, n, k, group, stream
 
 
+WRITE = "pii" "pp" "id" "pp" "i" "p" "i" "pp" "ii" "p" "i" "p" "iiiii" "p"      # qkv, dtype, ld, gains, their dtype, eps, tables, rows, positions, tokens, token_req, table, requests, width, kv, pages, q_out, nq, nkv, d, rd, page, stream
+
+
 @pytest.mark.parametrize("name,kinds,args,said", [
+    ("lily_qk_norm_rope_write4", WRITE, (16, 1, 256, 0, 0, 0, 1e-6, 16, 16, 0, 16, 1, 16, 16, 1, 1, 16, 2, 16, 2, 1, 64, 64, 16, 0), "tables of 0 positions"),
+    ("lily_qk_norm_rope_write4", WRITE, (16, 1, 256, 16, 0, 0, 1e-6, 16, 16, 8, 16, 1, 16, 16, 1, 1, 16, 2, 16, 2, 1, 64, 64, 16, 0), "gains come together"),
+    ("lily_qk_norm_rope_write4", WRITE, (16, 1, 256, 0, 0, 0, 1e-6, 16, 16, 8, 16, 1, 16, 16, 1, 1, 24, 2, 16, 2, 1, 64, 64, 16, 0), "sixteen bytes"),
     ("lily_attention_decode4", DECODE, (16, 16, 16, 16, 1, 16, 16, 1, 16, 3, 2, 64, 16, 2, 0.1, 1, 0), "query heads over"),
     ("lily_attention_decode4", DECODE, (16, 16, 16, 16, 1, 16, 16, 1, 16, 2, 0, 64, 16, 2, 0.1, 1, 0), "query heads over"),
     ("lily_attention_decode4", DECODE, (16, 16, 16, 16, 1, 16, 16, 1, 16, 2, 2, 80, 16, 2, 0.1, 1, 0), "not 80"),
