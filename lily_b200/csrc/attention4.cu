@@ -696,7 +696,7 @@ inline bool on_tensor_cores(int page_size, int dtype) { return dtype == kBF16 &&
 
 // Query heads of a pair on the CUDA cores.
 inline int cores_heads(int group) { return group <= 4 ? 4 : 8; }
-// Blocks: as many as are on the device at once, a tile a warp at least.
+// Blocks: as many as are on the device at once, where there is work for them.
 struct Plan { bool tensor_cores; int heads, warps, blocks; };
 inline Plan plan_of(int requests, int nq, int nkv, int d, int longest, int page_size, int dtype) {
     Plan p{};
@@ -704,7 +704,10 @@ inline Plan plan_of(int requests, int nq, int nkv, int d, int longest, int page_
     p.heads = p.tensor_cores ? HEADS : cores_heads(nq / nkv);
     const long long pairs = (long long)requests * nkv * ((nq / nkv + p.heads - 1) / p.heads), tiles = pairs * (((long long)longest + KT - 1) / KT);
     p.warps = p.tensor_cores && d <= 128 && pairs >= 3ll * sm_count() ? 1 : WARPS;      // (at blocks_a_sm)
-    p.blocks = (int)max(1ll, min((long long)(p.tensor_cores ? blocks_a_sm(d, p.warps) : 3) * sm_count(), (tiles + p.warps - 1) / p.warps));
+    // Two tiles a block at least, of four warps, but no two pairs in a block while there are blocks: a pair's end is some 2 us that the next one waits for.  Against a tile a warp: 8 rows of one place
+    // 4.6 us for 10.6 (float32 6.9 for 21.1), of 130 8.1 and 8.2, two of 300 6.0 and 7.9, float32 3 rows of 150 to 2,900 10.2 and 15.5 (of 2,000 18.6 and 17.4); a tile a block: 8 rows of 60 6.1 for 4.9.
+    const long long wanted = p.warps == 1 ? tiles : max(pairs, (tiles + 1) / 2);
+    p.blocks = (int)max(1ll, min((long long)(p.tensor_cores ? blocks_a_sm(d, p.warps) : 3) * sm_count(), wanted));
     return p;
 }
 
