@@ -391,11 +391,15 @@ __global__ void __launch_bounds__(256) halves_kernel(const __nv_bfloat16* __rest
     }
 }
 
-// (a kernel and not a memset, which the one behind it waits for in full: portions of 2,048 tokens 70.5 us in a graph, 74.2 with a memset)
-__global__ void __launch_bounds__(256) zero_kernel(unsigned* __restrict__ words, int n) {
+// Zeros to the spans and the block table, and the portions' tiles, which come with the launch: a copy of them would have 2,048 tokens wait 6 us.  (A kernel and not a memset, which the one behind it waits for
+// in full: portions of 2,048 tokens 70.5 us in a graph, 74.2 with a memset.)
+constexpr int MOST_TILES = 480;
+struct Tiles { int n, of[2 * MOST_TILES]; };
+__global__ void __launch_bounds__(256) zero_kernel(unsigned* __restrict__ words, int n, int* __restrict__ tiles_out, const __grid_constant__ Tiles tiles) {
     pdl_enter_small();
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i < n) words[i] = 0u;
+    if (i < 2 * tiles.n) tiles_out[i] = tiles.of[i];
 }
 
 inline bool head_fits(int d) { return d >= GROUP && d <= 256 && d % GROUP == 0; }
@@ -475,16 +479,21 @@ LILY_API int lily_cache4_values(const void* kv, int pages, const int* block_tabl
 }
 
 // What portions attend with in half precision (attention_args.cuh): the largest magnitudes of keys to `spans` [requests, nkv] (`zeroed` bytes from there on are set to zero first), the queries times powers
-// of two to `out`, what undoes them to `units` [tokens, nq].
+// of two to `out`, what undoes them to `units` [tokens, nq].  tiles: up to lily_halves4_tiles() of the portions' tiles, numbers of the host (requests, then offsets), which go to `tiles_out`.
+LILY_API int lily_halves4_tiles() { return four::MOST_TILES; }
 LILY_API int lily_halves4(const void* q, int tokens, int nq, const void* kv, int pages, const int* block_table, int requests, int width, int nkv, int d, int page_size, const int* cu, const int* prefix,
-                          int most_pages, unsigned* spans, size_t zeroed, void* out, float* units, cudaStream_t stream) {
+                          int most_pages, unsigned* spans, size_t zeroed, const int* tiles, int tile_count, int* tiles_out, void* out, float* units, cudaStream_t stream) {
     if (tokens == 0 || requests == 0) return 0;
     LILY_REQUIRE(four::head_fits(d) && page_size > 0 && nkv > 0 && nq > 0 && most_pages > 0 && (long long)requests * most_pages <= INT32_MAX / 2, "halves4: %d requests of up to %d pages", requests, most_pages);
     LILY_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)kv) % 16 == 0, "halves4: tensors on boundaries of sixteen bytes");
     const size_t heads = (size_t)tokens * nq, a_block = 8 * (32 / (d / 8)), query_blocks = (heads + a_block - 1) / a_block;
     LILY_REQUIRE(query_blocks <= INT32_MAX / 2, "halves4: %d tokens", tokens);
     LILY_REQUIRE(zeroed >= (size_t)requests * nkv * sizeof(unsigned) && zeroed % 4 == 0 && zeroed <= INT32_MAX, "halves4: %zu bytes of spans and tables", zeroed);
-    launch_pdl(four::zero_kernel, dim3((unsigned)((zeroed / 4 + 255) / 256)), dim3(256), 0, stream, spans, (int)(zeroed / 4));
+    LILY_REQUIRE(tile_count >= 0 && tile_count <= four::MOST_TILES && (tile_count == 0 || (tiles && tiles_out)), "halves4: %d tiles", tile_count);
+    four::Tiles with;
+    with.n = tile_count;
+    for (int i = 0; i < 2 * tile_count; ++i) with.of[i] = tiles[i];
+    launch_pdl(four::zero_kernel, dim3((unsigned)((max((int)(zeroed / 4), 2 * tile_count) + 255) / 256)), dim3(256), 0, stream, spans, (int)(zeroed / 4), tiles_out, with);
     LILY_CHECK_LAUNCH("halves4");
     launch_pdl(four::halves_kernel, dim3((unsigned)query_blocks + requests * most_pages), dim3(256), 0, stream, (const __nv_bfloat16*)q, heads, (__nv_bfloat16*)out, units, (int)query_blocks,
                (const uint8_t*)kv, pages, block_table, width, nkv, d, page_size, cu, prefix, most_pages, spans);

@@ -57,7 +57,8 @@ struct Entries {
     int (*values4)(const void*, int, const int*, int, int, void*, int, int, int, int, const int*, const int*, int*, int, int, const unsigned*, void*);
     size_t (*decode4_floats)(int, int, int, int, int, int, int);
     int (*decode4)(const void*, const void*, void*, const int*, int, const int*, float*, int, int, int, int, int, int, int, float, int, void*);
-    int (*halves4)(const void*, int, int, const void*, int, const int*, int, int, int, int, int, const int*, const int*, int, unsigned*, size_t, void*, float*, void*);
+    int (*halves4)(const void*, int, int, const void*, int, const int*, int, int, int, int, int, const int*, const int*, int, unsigned*, size_t, const int*, int, int*, void*, float*, void*);
+    int (*halves4_tiles)();
     int (*prefill_tc_half)(const void*, const void*, void*, const int*, int, const int*, const int*, const int*, const int*, int, int, int, int, int, float, int, int, const unsigned*, const float*, void*);
     int (*prefill_mma_half)(const void*, const void*, void*, const int*, int, const int*, const int*, const int*, const int*, int, int, int, int, int, float, const unsigned*, const float*, void*);
 } entry;
@@ -539,12 +540,12 @@ PyObject* attention_decode4(PyObject*, PyObject* const* p, Py_ssize_t count) {
     });
 }
 
-// How portions are cut: (request, offset) of each tile of ``rows`` new tokens in the order of the keys that it sees, and the pages that portions see.
-struct Cut4 { Tensor req, start; int64_t pages, width; };
-Cut4 cut4(const char* what, const std::vector<int>& prefix, const std::vector<int>& fresh, int page, int rows, int device) {
+// How portions are cut: the requests, then the offsets, of tiles of ``rows`` new tokens in the order of the keys that they see, and the pages that portions see.
+struct Cut4 { std::vector<int> tiles; int64_t pages, width; Tensor both; };
+Cut4 cut4(const char* what, const std::vector<int>& prefix, const std::vector<int>& fresh, int page, int rows) {
     if (prefix.size() != fresh.size() || page < 1 || rows < 1) refuse(what, ": ", fresh.size(), " portions behind ", prefix.size(), " lengths, pages of ", page, " places");
     std::vector<std::tuple<int64_t, int, int>> tiles;
-    Cut4 c{{}, {}, 0, 0};
+    Cut4 c{{}, 0, 0, {}};
     for (size_t r = 0; r < fresh.size(); ++r) {
         if (fresh[r] < 0 || prefix[r] < 0) refuse(what, ": a portion of ", fresh[r], " tokens behind ", prefix[r]);
         if (fresh[r] == 0) continue;
@@ -553,23 +554,26 @@ Cut4 cut4(const char* what, const std::vector<int>& prefix, const std::vector<in
         c.width = std::max(c.width, pages);
         for (int64_t at = 0; at < fresh[r]; at += rows) tiles.emplace_back(prefix[r] + at, (int)r, (int)at);
     }
-    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) refuse(what, ": a captured call's plan is made ahead of the capture");
     std::sort(tiles.begin(), tiles.end());
-    const int64_t n = (int64_t)tiles.size();
-    Tensor host = at::empty({2, n}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
-    int* at = host.data_ptr<int>();
-    for (int64_t i = 0; i < n; ++i) at[i] = std::get<1>(tiles[i]), at[n + i] = std::get<2>(tiles[i]);
-    const Tensor both = host.to(at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)device), /*non_blocking=*/true);
-    c.req = both.select(0, 0);
-    c.start = both.select(0, 1);
+    const size_t n = tiles.size();
+    c.tiles.resize(2 * n);
+    for (size_t i = 0; i < n; ++i) c.tiles[i] = std::get<1>(tiles[i]), c.tiles[n + i] = std::get<2>(tiles[i]);
     return c;
+}
+// ... on the device: both[0] the requests, both[1] the offsets.
+void cut_to(const char* what, Cut4& c, int device) {
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) refuse(what, ": a captured call's plan is made ahead of the capture");
+    Tensor host = at::empty({2, (int64_t)c.tiles.size() / 2}, at::TensorOptions().dtype(at::kInt).pinned_memory(true));
+    std::copy(c.tiles.begin(), c.tiles.end(), host.data_ptr<int>());
+    c.both = host.to(at::TensorOptions().dtype(at::kInt).device(at::kCUDA, (c10::DeviceIndex)device), /*non_blocking=*/true);
 }
 
 // lengths of prefixes, of portions, page_size, rows of a tile, the device's index -> (requests, offsets, pages, width)
 PyObject* plan4(PyObject*, PyObject* const* p, Py_ssize_t count) {
     return guarded(count, 5, [&]() -> PyObject* {
-        Cut4 c = cut4("plan_prefill4", lengths(p[0]), lengths(p[1]), number(p[2]), number(p[3]), number(p[4]));
-        return Py_BuildValue("(NNLL)", THPVariable_Wrap(std::move(c.req)), THPVariable_Wrap(std::move(c.start)), (long long)c.pages, (long long)c.width);
+        Cut4 c = cut4("plan_prefill4", lengths(p[0]), lengths(p[1]), number(p[2]), number(p[3]));
+        cut_to("plan_prefill4", c, number(p[4]));
+        return Py_BuildValue("(NNLL)", THPVariable_Wrap(c.both.select(0, 0)), THPVariable_Wrap(c.both.select(0, 1)), (long long)c.pages, (long long)c.width);
     });
 }
 
@@ -600,54 +604,66 @@ PyObject* attention_prefill4(PyObject*, PyObject* const* p, Py_ssize_t count) {
         if (given && (given->scalar_type() != q.scalar_type() || given->sizes() != q.sizes())) refuse(what, ": out has the shape and dtype of q");
         if (!(scale > 0.f) || scale > 3.4e38f) refuse(what, ": a scale of ", scale);
         here({&q, &kv, &table, &cu, &prefix, given});
-        Cut4 c;
-        if (p[13] == Py_None) c = cut4(what, cached, fresh, page, rows, q.get_device());
-        else {
+        if (entry.halves4_tiles == nullptr) refuse("the kernels are not bound");
+        Cut4 c{{}, 0, 0, {}};
+        Tensor req, start;                               // a plan's tiles; those of a call without one go with its first launch where they are few
+        int64_t tiles = 0;
+        if (p[13] == Py_None) {
+            c = cut4(what, cached, fresh, page, rows);
+            tiles = (int64_t)c.tiles.size() / 2;
+            if (kernel == 0 || tiles > entry.halves4_tiles()) {
+                cut_to(what, c, q.get_device());
+                req = c.both.select(0, 0), start = c.both.select(0, 1);
+                c.tiles.clear();
+            }
+        } else {
             if (!PyTuple_Check(p[13]) || PyTuple_GET_SIZE(p[13]) != 5) refuse(what, ": a plan is what plan_prefill4 gives");
-            c = {tensor(PyTuple_GET_ITEM(p[13], 1)), tensor(PyTuple_GET_ITEM(p[13], 2)), whole(PyTuple_GET_ITEM(p[13], 3)), whole(PyTuple_GET_ITEM(p[13], 4))};
-            int64_t pages = 0, most = 0, tiles = 0;
+            req = tensor(PyTuple_GET_ITEM(p[13], 1)), start = tensor(PyTuple_GET_ITEM(p[13], 2)), c.pages = whole(PyTuple_GET_ITEM(p[13], 3)), c.width = whole(PyTuple_GET_ITEM(p[13], 4));
+            int64_t pages = 0, most = 0;
             for (size_t r = 0; r < fresh.size(); ++r) {
                 const int64_t own = fresh[r] ? ((int64_t)cached[r] + fresh[r] + page - 1) / page : 0;
                 pages += own;
                 most = std::max(most, own);
                 tiles += ((int64_t)fresh[r] + rows - 1) / rows;
             }
-            if (whole(PyTuple_GET_ITEM(p[13], 0)) != rows || c.pages != pages || c.width != most || c.req.numel() != tiles || c.start.numel() != tiles)
+            if (whole(PyTuple_GET_ITEM(p[13], 0)) != rows || c.pages != pages || c.width != most || req.numel() != tiles || start.numel() != tiles)
                 refuse(what, ": the plan is not one of these portions (", tiles, " tiles of ", rows, " tokens, ", pages, " pages)");
-            ints(c.req, "a plan's requests"), ints(c.start, "a plan's offsets");
-            here({&c.req, &c.start});
+            ints(req, "a plan's requests"), ints(start, "a plan's offsets");
+            here({&req, &start});
         }
         if (c.width > width) refuse(what, ": ", c.width, " pages of a request; the block table holds ", width);
         Tensor out = given ? *given : at::empty_like(q);
-        if (kernel == 0) return Py_BuildValue("(NNNLL)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(c.req)), THPVariable_Wrap(std::move(c.start)), (long long)c.pages, (long long)c.width);
+        if (kernel == 0) return Py_BuildValue("(NNNLL)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(req)), THPVariable_Wrap(std::move(start)), (long long)c.pages, (long long)c.width);
         if (!is(q, at::kBFloat16)) refuse(what, ": these kernels take bfloat16");
         if (tokens == 0) return THPVariable_Wrap(std::move(out));
         // the keys' spans and the block table of the numbers, zeros; the numbers of the pages; queries in half precision and what undoes their powers of two
         const int64_t spans_n = requests * nkv, words_n = spans_n + requests * c.width;
-        Tensor zeroed = at::empty({words_n}, q.options().dtype(at::kInt)), values = at::empty({c.pages, 2, (int64_t)nkv, (int64_t)page, (int64_t)d}, q.options());
+        Tensor zeroed = at::empty({words_n + (int64_t)c.tiles.size()}, q.options().dtype(at::kInt)), values = at::empty({c.pages, 2, (int64_t)nkv, (int64_t)page, (int64_t)d}, q.options());
         Tensor heads = at::empty_like(q), units = at::empty({q.size(0), (int64_t)nq}, q.options().dtype(at::kFloat));
         unsigned* spans = (unsigned*)zeroed.data_ptr<int>();
         int* numbers = zeroed.data_ptr<int>() + spans_n;
-        const int *bt = table.const_data_ptr<int>(), *tile_req = c.req.const_data_ptr<int>(), *tile_start = c.start.const_data_ptr<int>();
-        const int n = narrow(q.size(0)), pages = narrow(c.pages), wide = narrow(c.width), r = narrow(requests), tiles = narrow(c.req.numel()), held = narrow(kv.size(0));
-        done("lily_halves4", call(entry.halves4, q.const_data_ptr(), n, nq, kv.const_data_ptr(), held, bt, r, width, nkv, d, page, offsets, behind, wide, spans, (size_t)words_n * 4, heads.data_ptr(),
+        const int* bt = table.const_data_ptr<int>();
+        const int n = narrow(q.size(0)), pages = narrow(c.pages), wide = narrow(c.width), r = narrow(requests), tiles_n = narrow(tiles), held = narrow(kv.size(0));
+        int* own = c.tiles.empty() ? nullptr : numbers + requests * c.width;
+        const int *tile_req = own ? own : req.const_data_ptr<int>(), *tile_start = own ? own + tiles_n : start.const_data_ptr<int>();
+        done("lily_halves4", call(entry.halves4, q.const_data_ptr(), n, nq, kv.const_data_ptr(), held, bt, r, width, nkv, d, page, offsets, behind, wide, spans, (size_t)words_n * 4, (const int*)c.tiles.data(), own ? tiles_n : 0, own, heads.data_ptr(),
                                   units.data_ptr<float>(), stream()));
         done("lily_cache4_values", call(entry.values4, kv.const_data_ptr(), held, bt, r, width, values.data_ptr(), BF16, nkv, d, page, offsets, behind, numbers, wide, pages, (const unsigned*)spans, stream()));
         if (kernel == 2)
             done("lily_attention_prefill_tc_half", call(entry.prefill_tc_half, heads.const_data_ptr(), values.const_data_ptr(), out.data_ptr(), (const int*)numbers, wide, offsets, behind, tile_req, tile_start,
-                                                        tiles, nq, nkv, d, page, scale, n, pages, (const unsigned*)spans, units.const_data_ptr<float>(), stream()));
+                                                        tiles_n, nq, nkv, d, page, scale, n, pages, (const unsigned*)spans, units.const_data_ptr<float>(), stream()));
         else
             done("lily_attention_prefill_mma_half", call(entry.prefill_mma_half, heads.const_data_ptr(), values.const_data_ptr(), out.data_ptr(), (const int*)numbers, wide, offsets, behind, tile_req,
-                                                         tile_start, tiles, nq, nkv, d, page, scale, (const unsigned*)spans, units.const_data_ptr<float>(), stream()));
+                                                         tile_start, tiles_n, nq, nkv, d, page, scale, (const unsigned*)spans, units.const_data_ptr<float>(), stream()));
         return THPVariable_Wrap(std::move(out));
     });
 }
 
 // the addresses of the entries for numbers held in four bits, in their order
 PyObject* bind4(PyObject*, PyObject* const* p, Py_ssize_t count) {
-    return guarded(count, 10, [&]() -> PyObject* {
-        void* at[10];
-        for (int i = 0; i < 10; ++i) at[i] = (void*)(uintptr_t)whole(p[i]);
+    return guarded(count, 11, [&]() -> PyObject* {
+        void* at[11];
+        for (int i = 0; i < 11; ++i) at[i] = (void*)(uintptr_t)whole(p[i]);
         entry.linear4 = (decltype(entry.linear4))at[0];
         entry.weights4 = (decltype(entry.weights4))at[1];
         entry.write4 = (decltype(entry.write4))at[2];
@@ -658,6 +674,7 @@ PyObject* bind4(PyObject*, PyObject* const* p, Py_ssize_t count) {
         entry.halves4 = (decltype(entry.halves4))at[7];
         entry.prefill_tc_half = (decltype(entry.prefill_tc_half))at[8];
         entry.prefill_mma_half = (decltype(entry.prefill_mma_half))at[9];
+        entry.halves4_tiles = (decltype(entry.halves4_tiles))at[10];
         Py_RETURN_NONE;
     });
 }

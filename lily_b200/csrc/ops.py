@@ -1217,7 +1217,7 @@ def _faces():
         address = lambda n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value
         module.bind(KernelError, *[address(n) for n in names])
         module.bind4(*[address(n) for n in ("lily_linear4", "lily_weights4", "lily_qk_norm_rope_write4", "lily_cache4_values", "lily_attention_decode4_floats", "lily_attention_decode4", "lily_linear4_many", "lily_halves4",
-                                               "lily_attention_prefill_tc_half", "lily_attention_prefill_mma_half")])
+                                               "lily_attention_prefill_tc_half", "lily_attention_prefill_mma_half", "lily_halves4_tiles")])
         _module = module
     return _module
 
@@ -1487,7 +1487,7 @@ class Prefill4Plan(NamedTuple):
 
 
 def plan_prefill4(dtype: torch.dtype, d: int, page_size: int, h_prefix_lens: Sequence[int], h_new_lens: Sequence[int], device) -> Prefill4Plan:
-    """The plan of ``attention_prefill4`` for portions of these lengths; a step's layers share one, and a captured call's is made ahead of the capture."""
+    """The plan of ``attention_prefill4`` for portions of these lengths; a step's layers share one, and that of a captured call of many tiles or in float32 is made ahead of the capture."""
     device = torch.device(device)
     rows = prefill_tile_rows(dtype, d, page_size, sum(h_new_lens))
     return Prefill4Plan(rows, *(_module or _faces()).plan4(h_prefix_lens, h_new_lens, page_size, rows, torch.cuda.current_device() if device.index is None else device.index))

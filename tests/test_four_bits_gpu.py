@@ -472,19 +472,19 @@ def test_portions_refuse_a_plan_of_others():
             run(q, kv, None, other)
 
 
-@pytest.mark.parametrize("page", [16, 64])
-def test_portions_in_a_graph(page):
-    """A captured call has its plan made ahead, and is refused without one; what is replayed follows the queries and the cache."""
+@pytest.mark.parametrize("page,planned", [(16, False), (16, True), (64, False), (64, True)])
+def test_portions_in_a_graph(page, planned):
+    """A captured call, its tiles a plan's or going with the launch; what is replayed follows the queries and the cache.  In float32 tiles are copied, so a call without a plan is refused."""
     new, cached, nq, nkv, d = [130, 1, 70], [3, 200, 0], 8, 2, 128
     q, kv, run, _ = portions_case(new, cached, nq, nkv, d, page)
-    plan, out, stream = ops().plan_prefill4(BF16, d, page, cached, new, q.device), torch.zeros_like(q), torch.cuda.Stream()
-    want = [run(x, kv) for x in (q, q.flip(0).contiguous())]
+    plan, out, stream = ops().plan_prefill4(BF16, d, page, cached, new, q.device) if planned else None, torch.zeros_like(q), torch.cuda.Stream()
+    want, wide = [run(x, kv) for x in (q, q.flip(0).contiguous())], q.float()
     torch.cuda.synchronize()
     with torch.cuda.stream(stream):
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=stream):
             with pytest.raises(ops().KernelError, match="ahead of the capture"):
-                run(q, kv, out)
+                run(wide, kv)
             run(q, kv, out, plan)
         graph.replay()
         stream.synchronize()
@@ -493,6 +493,17 @@ def test_portions_in_a_graph(page):
         graph.replay()
         stream.synchronize()
         assert torch.equal(out, want[1])
+
+
+def test_portions_of_many_tiles():
+    """More tiles than go with a launch: the same bits by a plan and without one, each request's as alone."""
+    new, cached, nq, nkv, d, page = [1 + r % 3 for r in range(520)], [r % 40 for r in range(520)], 2, 1, 64, 16
+    q, kv, run, table = portions_case(new, cached, nq, nkv, d, page)
+    got = run(q, kv)
+    assert torch.equal(run(q, kv, None, ops().plan_prefill4(BF16, d, page, cached, new, q.device)), got)
+    want, by_codes, by_values = fb.attention(q, kv, table, list(zip(new, cached)), nq, nkv, d, page, d ** -0.5)
+    # (test_portions says why: keys, weights and values are rounded)
+    within(got, want, attention_bound(by_codes, by_values, want, BF16) + HALF[BF16] * (2 * 2 * d ** 0.5 + 2) * by_values)
 
 
 # ---- streams, graphs, large offsets, together ----
