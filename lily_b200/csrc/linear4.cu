@@ -308,13 +308,13 @@ using namespace lily;
 static bool weights_fit(int n, int k, int group) { return n > 0 && k > 0 && (group == 32 || group == 64 || group == 128) && k % group == 0 && n <= INT32_MAX - 256 && k <= INT32_MAX - 256; }
 
 // Tokens that the kernels for few of them take.
-LILY_API int lily_linear4_few(int dtype) { return dtype == kBF16 ? 16 : four::F32_TOKENS; }
+static int few_tokens(int dtype) { return dtype == kBF16 ? 16 : four::F32_TOKENS; }
 
 LILY_API int lily_linear4(const void* x, int dtype, const void* codes, const void* scales, const void* zeros, const void* bias, int bias_f32, void* out, int out_f32, int m, int n, int k,
                           int group, cudaStream_t stream) {
     if (m == 0 || n == 0) return 0;
     LILY_REQUIRE(weights_fit(n, k, group), "linear4: a matrix [%d, %d] in groups of %d", n, k, group);
-    LILY_REQUIRE(m > 0 && m <= lily_linear4_few(dtype), "linear4: %d tokens", m);
+    LILY_REQUIRE(m > 0 && m <= few_tokens(dtype), "linear4: %d tokens", m);
     LILY_REQUIRE(dtype == kBF16 || (out_f32 && (!bias || bias_f32)), "linear4: float32 tokens keep float32");
     LILY_REQUIRE(((uintptr_t)x | (uintptr_t)codes) % 16 == 0, "linear4: tensors on boundaries of sixteen bytes");
     const four::ProductArgs a{x, (const uint8_t*)codes, (const __nv_bfloat16*)scales, (const uint8_t*)zeros, bias, bias_f32, out, out_f32, m, n, k, (k + 127) / 128};

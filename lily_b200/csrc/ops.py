@@ -191,8 +191,6 @@ def library():
         lib.lily_mlstm_chunk_floats.restype = _sz
         lib.lily_attention_decode4_floats.argtypes = [_i, _i, _i, _i, _i, _i, _i]
         lib.lily_attention_decode4_floats.restype = _sz
-        lib.lily_linear4_few.argtypes = [_i]
-        lib.lily_linear4_few.restype = _i
         _lib = lib
     return _lib
 
