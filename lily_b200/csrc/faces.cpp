@@ -51,6 +51,7 @@ struct Entries {
     // numbers held in four bits
     int (*linear4)(const void*, int, const void*, const void*, const void*, const void*, int, void*, int, int, int, int, int, void*);
     int (*linear4_many)(const void*, const void*, const void*, const void*, const void*, int, void*, int, int, int, int, int, void*);
+    int (*linear4_many_within)(const void*, const void*, const void*, const void*, const void*, int, void*, int, int, int, int, int, int, void*);
     int (*weights4)(const void*, const void*, const void*, void*, int, int, int, int, void*);
     int (*write4)(const void*, int, int, const void*, const void*, int, double, const float*, const float*, int, const int*, int, const int*, const int*, int, int, void*, int, void*, int, int,
                   int, int, int, void*);
@@ -418,9 +419,9 @@ Matrix4 matrix4(const char* what, PyObject* const* p) {
     return w;
 }
 
-// x, codes, scales, zeros, n, k, group, bias, whether the result is float32 whatever x is, tokens from which on tcgen05 multiplies
+// x, codes, scales, zeros, n, k, group, bias, whether the result is float32 whatever x is, tokens from which on tcgen05 multiplies(, how often its waits ask)
 PyObject* linear4(PyObject*, PyObject* const* p, Py_ssize_t count) {
-    return guarded(count, 10, [&]() -> PyObject* {
+    return guarded(count == 11 ? 10 : count, 10, [&]() -> PyObject* {
         const Tensor& x = tensor(p[0]);
         const Matrix4 w = matrix4("linear4", p + 1);
         const Tensor* bias = maybe(p[7]);
@@ -430,7 +431,11 @@ PyObject* linear4(PyObject*, PyObject* const* p, Py_ssize_t count) {
         here({&x, &w.codes, &w.scales, w.zeros, bias});
         Tensor out = at::empty({x.size(0), (int64_t)w.n}, x.options().dtype(wide ? at::kFloat : at::kBFloat16));
         if (code == BF16 && x.size(0) >= number(p[9])) {
-            done("lily_linear4_many", call(entry.linear4_many, x.const_data_ptr(), w.codes.const_data_ptr(), w.scales.const_data_ptr(), w.zeros ? w.zeros->const_data_ptr() : nullptr,
+            if (count == 11)
+                done("lily_linear4_many", call(entry.linear4_many_within, x.const_data_ptr(), w.codes.const_data_ptr(), w.scales.const_data_ptr(), w.zeros ? w.zeros->const_data_ptr() : nullptr,
+                                               bias ? bias->const_data_ptr() : nullptr, bias ? (int)(code_of(*bias) == F32) : 0, out.data_ptr(), wide, narrow(x.size(0)), w.n, w.k, w.group,
+                                               number(p[10]), stream()));
+            else done("lily_linear4_many", call(entry.linear4_many, x.const_data_ptr(), w.codes.const_data_ptr(), w.scales.const_data_ptr(), w.zeros ? w.zeros->const_data_ptr() : nullptr,
                                            bias ? bias->const_data_ptr() : nullptr, bias ? (int)(code_of(*bias) == F32) : 0, out.data_ptr(), wide, narrow(x.size(0)), w.n, w.k, w.group, stream()));
             return THPVariable_Wrap(std::move(out));
         }
@@ -661,9 +666,9 @@ PyObject* attention_prefill4(PyObject*, PyObject* const* p, Py_ssize_t count) {
 
 // the addresses of the entries for numbers held in four bits, in their order
 PyObject* bind4(PyObject*, PyObject* const* p, Py_ssize_t count) {
-    return guarded(count, 11, [&]() -> PyObject* {
-        void* at[11];
-        for (int i = 0; i < 11; ++i) at[i] = (void*)(uintptr_t)whole(p[i]);
+    return guarded(count, 12, [&]() -> PyObject* {
+        void* at[12];
+        for (int i = 0; i < 12; ++i) at[i] = (void*)(uintptr_t)whole(p[i]);
         entry.linear4 = (decltype(entry.linear4))at[0];
         entry.weights4 = (decltype(entry.weights4))at[1];
         entry.write4 = (decltype(entry.write4))at[2];
@@ -675,6 +680,7 @@ PyObject* bind4(PyObject*, PyObject* const* p, Py_ssize_t count) {
         entry.prefill_tc_half = (decltype(entry.prefill_tc_half))at[8];
         entry.prefill_mma_half = (decltype(entry.prefill_mma_half))at[9];
         entry.halves4_tiles = (decltype(entry.halves4_tiles))at[10];
+        entry.linear4_many_within = (decltype(entry.linear4_many_within))at[11];
         Py_RETURN_NONE;
     });
 }

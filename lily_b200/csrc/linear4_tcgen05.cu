@@ -11,14 +11,17 @@
 // What bounds it: a step takes a block some 0.5 us, which its eight warps spend on the codes, two blocks a SM side by side (45 tokens, 4,096 x 12,288 in groups of 64 with zero points: 15.6 us, 1.9 TB/s of weights,
 // the tensor pipe 15 % busy); through shared memory the weights took 20.8.  Filling and joining take 3 us.
 //
-// Every wait is bounded: one that runs out leaves its code in a status word (lily_linear4_status) and NaN in the block's outputs.
+// Every wait is bounded: one that runs out leaves its code in a word of the host's memory (lily_linear4_status) and NaN in the outputs of its cluster.  The block then
+// waits, a bounded time again, for what it has on its way, copies and products, before it frees its tensor memory and leaves.
 #include "four.cuh"
 #include "tcgen05.cuh"
 
+#include <atomic>
 #include <cooperative_groups.h>
 #include <type_traits>
 
 namespace lily {
+int* new_host_word();
 namespace four {
 namespace many {
 
@@ -29,9 +32,8 @@ constexpr int OPERANDS = 4;                              // at most
 constexpr int GROUPS = 2, WORKERS = 4, THREADS = 32 * (2 + GROUPS * WORKERS);      // groups of warps that take steps in turn, a warp a quarter of the rows
 constexpr int MOST_TOKENS = 256, MOST_SPLITS = 8;
 constexpr int MOST_BYTES = 225 * 1024;                   // of shared memory
-constexpr uint32_t SPIN_LIMIT = 1u << 17;                // polls of up to ten microseconds each: a second before a wait gives up
-
-__device__ int g_status = 0;                             // 0; else (code << 24 | block) of the first wait that gave up
+constexpr int POLLS = 1 << 17;                           // of up to ten microseconds each: a second before a wait gives up
+constexpr int LAST_POLLS = 1 << 16;                      // ... and of the waits of a block that has given up for what it has on its way
 
 struct Args {
     const uint8_t* scales;                               // bytes of bfloat16 numbers
@@ -44,6 +46,8 @@ struct Args {
     int tokens;                                          // columns of the accumulator, a multiple of 16
     int stages, splits, operands;
     int columns;                                         // of tensor memory: the accumulator's, then the operands'
+    int polls;                                           // how often a wait asks before it gives up
+    int* lost;                                           // a word of the host's where it says so: (code << 24 | block)
 };
 
 // Asks once, asleep for up to ten microseconds: a warp that polls takes turns away from those that work.
@@ -52,19 +56,24 @@ __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
     asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.b32 %0, 1, 0, p;\n}\n" : "=r"(ok) : "r"(bar), "r"(parity), "r"(10000u) : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* lost, int code) {
+struct Waits { volatile int* lost; int* word; int polls; };
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, const Waits& w, int code) {
     bool come = false;
-    uint32_t i = 0;
-    for (; i < SPIN_LIMIT && !come; ++i) {
+    for (int i = 0; i < w.polls && !come; ++i) {
         come = try_wait(bar, parity);
-        if ((i & 15u) == 15u && *lost) break;
+        if ((i & 15) == 15 && *w.lost) break;
     }
     come = __all_sync(0xffffffffu, come);                // (the whole warp goes on, or none of it)
-    if (!come && !*lost) {
-        *lost = 1;
-        atomicCAS(&g_status, 0, (code << 24) | (int)((blockIdx.x + blockIdx.y * gridDim.x) & 0xFFFFFF));
+    if (!come && !*w.lost) {
+        *w.lost = 1;
+        *(volatile int*)w.word = (code << 24) | (int)((blockIdx.x + blockIdx.y * gridDim.x) & 0xFFFFFF);
+        __threadfence_system();
     }
     return come;
+}
+// What is on its way when a block has given up.
+__device__ __forceinline__ void last_wait(uint32_t bar, uint32_t parity) {
+    for (int i = 0; i < LAST_POLLS && !try_wait(bar, parity); ++i) {}
 }
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
@@ -99,6 +108,8 @@ __global__ void __launch_bounds__(THREADS, 2) product_many_kernel(const __grid_c
     const uint32_t full0 = tc5::smem_u32(&bars[0]), empty0 = tc5::smem_u32(&bars[8]), made0 = tc5::smem_u32(&bars[16]), freed0 = tc5::smem_u32(&bars[16 + OPERANDS]),
                    ready = tc5::smem_u32(&bars[16 + 2 * OPERANDS]);
     volatile int* lost = &lost_s;
+    const Waits waits{lost, a.lost, a.polls};
+    int issued = 0;                                      // warp 0: steps whose copies are on their way or have come
     const uint32_t columns = a.columns;
 
     if (threadIdx.x == 0) {
@@ -152,7 +163,7 @@ __global__ void __launch_bounds__(THREADS, 2) product_many_kernel(const __grid_c
         __syncwarp();
         int it = early;
         for (int s = 0, turn = 0; it < steps; ++it) {
-            if (!wait(empty0 + 8 * s, turn, lost, 1)) break;
+            if (!wait(empty0 + 8 * s, turn, waits, 1)) break;
             if (tc5::elect_one()) {
                 weights(it, s);
                 tokens(it, s);
@@ -160,15 +171,13 @@ __global__ void __launch_bounds__(THREADS, 2) product_many_kernel(const __grid_c
             __syncwarp();
             if (++s == a.stages) s = 0, turn ^= 1;
         }
-        if (*lost)                                       // copies already issued still land here: give each a bounded wait
-            for (int j = max(0, it - a.stages); j < it; ++j)
-                for (uint32_t i = 0; i < (1u << 20) && !tc5::mbar_try_wait(full0 + 8 * (j % a.stages), (j / a.stages) & 1); ++i) {}
+        issued = it;
     } else if (warp == 1) {
         // kind::f16, bfloat16 a and b (k-major), float32 d, 128 rows
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(a.tokens >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
         bool ok = true;
         for (int it = 0, s = 0, turn = 0, o = 0, o_turn = 0; it < steps; ++it) {
-            ok = wait(full0 + 8 * s, turn, lost, 2) && wait(made0 + 8 * o, o_turn, lost, 3);
+            ok = wait(full0 + 8 * s, turn, waits, 2) && wait(made0 + 8 * o, o_turn, waits, 3);
             if (!ok) break;
             tc5::tc_fence_after();
             const uint32_t w = operands + o * OPERAND, x = tc5::smem_u32(ring + (size_t)s * stage) + TOKENS_AT();
@@ -186,13 +195,18 @@ __global__ void __launch_bounds__(THREADS, 2) product_many_kernel(const __grid_c
             if (++s == a.stages) s = 0, turn ^= 1;
             if (++o == a.operands) o = 0, o_turn ^= 1;
         }
+        if (!ok) {                                       // products on their way read shared and tensor memory: they end first
+            if (tc5::elect_one()) tc5::umma_commit(ready);
+            __syncwarp();
+            last_wait(ready, 0);
+        }
     } else {
         // A thread a row of the step: pieces of sixteen bytes, which the copy has swizzled so that eight threads' lie in all banks, with a word of each 32 columns.
         const int group = (warp - 2) / WORKERS, row = (warp & 3) * 32 + lane;
         const __nv_bfloat162 up = __halves2bfloat162(__ushort_as_bfloat16(0x7F00), __ushort_as_bfloat16(0x7F00));                 // 2^127
         int s = group, turn = 0, o = group, o_turn = 1;  // (there are two stages and two operands at least)
         for (int it = group; it < steps; it += GROUPS) {
-            if (!wait(full0 + 8 * s, turn, lost, 4)) break;
+            if (!wait(full0 + 8 * s, turn, waits, 4)) break;
             const unsigned char* in = ring + (size_t)s * stage;
             uint4 raw[4];
 #pragma unroll
@@ -203,7 +217,7 @@ __global__ void __launch_bounds__(THREADS, 2) product_many_kernel(const __grid_c
                 scale[i] = *reinterpret_cast<const unsigned short*>(in + SCALES_AT() + (i * 128 + row) * 2);
                 zero[i] = a.zeros ? in[ZEROS_AT() + i * 128 + row] : 8u;
             }
-            if (it >= a.operands && !wait(freed0 + 8 * o, o_turn, lost, 5)) break;
+            if (it >= a.operands && !wait(freed0 + 8 * o, o_turn, waits, 5)) break;
             tc5::tc_fence_after();
             const uint32_t to = operands + o * OPERAND + ((uint32_t)((warp & 3) * 32) << 16);
 #pragma unroll
@@ -240,16 +254,14 @@ __global__ void __launch_bounds__(THREADS, 2) product_many_kernel(const __grid_c
             while (o >= a.operands) o -= a.operands, o_turn ^= 1;
         }
         // the accumulator to shared memory, where the ring was: [tokens][128]
-        const bool ok = wait(ready, 0, lost, 6);
+        const bool ok = wait(ready, 0, waits, 6) && !__any_sync(0xffffffffu, *lost);
         tc5::tc_fence_after();
         float* sums = reinterpret_cast<float*>(smem);
         const int quarter = warp & 3, first = (warp - 2) >> 2;      // (a warp reads its quarter of the lanes)
-        for (int c = first * 32; c < a.tokens; c += 32 * (GROUPS * WORKERS / 4)) {
-            float v[32] = {};
-            if (ok) {
-                tc5::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
-                tc5::tmem_wait_ld();
-            }
+        for (int c = first * 32; ok && c < a.tokens; c += 32 * (GROUPS * WORKERS / 4)) {
+            float v[32];
+            tc5::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + c, v);
+            tc5::tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e)
                 if (c + e < a.tokens) sums[(c + e) * ROWS + quarter * 32 + lane] = v[e];
@@ -257,6 +269,8 @@ __global__ void __launch_bounds__(THREADS, 2) product_many_kernel(const __grid_c
         tc5::tc_fence_before();
     }
     __syncthreads();
+    if (warp == 0 && lost_s)                             // (whoever gave up, also behind the loader's last step)
+        for (int j = max(0, issued - a.stages); j < issued; ++j) last_wait(full0 + 8 * (j % a.stages), (j / a.stages) & 1);
     if (warp == 1) {
         tc5::tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(columns) : "memory");
@@ -328,24 +342,41 @@ __global__ void __launch_bounds__(THREADS, 2) product_many_kernel(const __grid_c
 
 using namespace lily;
 
-// 0, or the code of a wait that gave up since the word was last read (synchronises, and clears it).
-LILY_API int lily_linear4_status() {
-    int v = 0, zero = 0;
-    if (cudaMemcpyFromSymbol(&v, four::many::g_status, sizeof(int)) != cudaSuccess) return -1;
-    if (v) cudaMemcpyToSymbol(four::many::g_status, &zero, sizeof(int));
+// The host's word in which the kernel says that a wait ran out; made with the first launch.
+static std::atomic<int*> g_lost_word{nullptr};
+static int* lost_word() {
+    static int* word = [] {
+        int* p = new_host_word();
+        g_lost_word = p;
+        return p;
+    }();
+    return word;
+}
+
+// 0, or (code << 24 | block) of a bounded wait that gave up since the last call; clears it.  `wait`: behind all work of the device; else as far as the host knows (the kernels it has waited for).
+LILY_API int lily_linear4_status(int wait) {
+    if (wait && cudaDeviceSynchronize() != cudaSuccess) return -1;
+    volatile int* word = g_lost_word;
+    const int v = word ? *word : 0;
+    if (v != 0) *word = 0;
     return v;
 }
 
-LILY_API int lily_linear4_many(const void* x, const void* codes, const void* scales, const void* zeros, const void* bias, int bias_f32, void* out, int out_f32, int m, int n, int k, int group,
-                               cudaStream_t stream) {
+// polls: how often a wait of the kernel asks before it gives up.
+LILY_API int lily_linear4_many_within(const void* x, const void* codes, const void* scales, const void* zeros, const void* bias, int bias_f32, void* out, int out_f32, int m, int n, int k,
+                                      int group, int polls, cudaStream_t stream) {
     using namespace four::many;
     if (m == 0 || n == 0) return 0;
     LILY_REQUIRE(n > 0 && k > 0 && (group == 32 || group == 64 || group == 128) && k % group == 0 && n <= INT32_MAX - 256 && k <= INT32_MAX - 256, "linear4: a matrix [%d, %d] in groups of %d", n, k,
                  group);
+    LILY_REQUIRE(polls >= 0, "linear4: %d polls", polls);
     LILY_REQUIRE(m > 0 && ((uintptr_t)x | (uintptr_t)codes | (uintptr_t)scales | (uintptr_t)zeros) % 16 == 0, "linear4: tensors on boundaries of sixteen bytes");
     const int token_tiles = (m + MOST_TOKENS - 1) / MOST_TOKENS, row_tiles = (n + ROWS - 1) / ROWS;
     Args a{(const uint8_t*)scales, (const uint8_t*)zeros, bias, bias_f32, out, out_f32, m, n, k, (k + STEP - 1) / STEP};
     a.tokens = ((m + token_tiles - 1) / token_tiles + 15) / 16 * 16;
+    a.polls = polls;
+    a.lost = lost_word();
+    LILY_REQUIRE(a.lost != nullptr, "linear4: no word of the host's memory");
     // columns shared out while there is room for more blocks (two a SM up to 128 tokens), no fewer than two steps a block
     a.splits = 1;
     // (a block a SM: eight parts of the device do not all have room for two clusters of eight, and a second round of them doubles the time: 256 tokens, 2,048 x 2,048 in 11.2 us by four, 21.4 by eight)
@@ -391,4 +422,9 @@ LILY_API int lily_linear4_many(const void* x, const void* codes, const void* sca
     cudaLaunchKernelEx(&cfg, kernel, map, map_w, a);
     LILY_CHECK_LAUNCH("linear4");
     return 0;
+}
+
+LILY_API int lily_linear4_many(const void* x, const void* codes, const void* scales, const void* zeros, const void* bias, int bias_f32, void* out, int out_f32, int m, int n, int k, int group,
+                               cudaStream_t stream) {
+    return lily_linear4_many_within(x, codes, scales, zeros, bias, bias_f32, out, out_f32, m, n, k, group, four::many::POLLS, stream);
 }

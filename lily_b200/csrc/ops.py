@@ -102,7 +102,7 @@ _SIGNATURES = {
     "lily_apply_penalties": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_top_logprobs": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_cache4_values": [_vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _vp],
-    "lily_linear4_status": [],
+    "lily_linear4_status": [_i],
     "lily_sample": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
 }
 
@@ -1215,7 +1215,7 @@ def _faces():
         address = lambda n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value
         module.bind(KernelError, *[address(n) for n in names])
         module.bind4(*[address(n) for n in ("lily_linear4", "lily_weights4", "lily_qk_norm_rope_write4", "lily_cache4_values", "lily_attention_decode4_floats", "lily_attention_decode4", "lily_linear4_many", "lily_halves4",
-                                               "lily_attention_prefill_tc_half", "lily_attention_prefill_mma_half", "lily_halves4_tiles")])
+                                               "lily_attention_prefill_tc_half", "lily_attention_prefill_mma_half", "lily_halves4_tiles", "lily_linear4_many_within")])
         _module = module
     return _module
 
@@ -1410,9 +1410,18 @@ def linear4_on_the_way(m: int, n: int, k: int) -> bool:
     return m <= 256 or (m <= 512 and n * k >= 1 << 24)
 
 
+LINEAR4_POLLS: Optional[int] = None      # how often a wait of the tcgen05 kernel of ``linear4`` asks before it gives up (None: some second's worth)
+
+
 def linear4_status() -> int:
-    """0, or the code of a bounded wait that gave up in the tcgen05 kernel of ``linear4`` since the code was last read (synchronises, and clears it); what its block was to give is NaN."""
-    return int(library().lily_linear4_status())
+    """0, or a code of a bounded wait that gave up in the tcgen05 kernel of ``linear4`` since the code was last read (synchronises, and clears it).  What the cluster with that wait was to give, a
+    tile's rows of all its tokens, is NaN; other calls are not touched."""
+    return int(library().lily_linear4_status(1))
+
+
+def linear4_lost() -> int:
+    """``linear4_status`` for the kernels that the host has waited for; waits for nothing."""
+    return int(library().lily_linear4_status(0))
 
 
 def linear4(x: torch.Tensor, w: Weight4, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
@@ -1421,7 +1430,7 @@ def linear4(x: torch.Tensor, w: Weight4, bias: Optional[torch.Tensor] = None, ou
         raise KernelError(f"linear4: the result is {x.dtype} or float32, not {out_dtype}")
     if x.dim() == 2 and x.shape[0] > 8 and (x.dtype != torch.bfloat16 or not linear4_on_the_way(x.shape[0], w.n, w.k)):
         return linear(x, weights4(w, x.dtype), bias, out_dtype)
-    out = (_module or _faces()).linear4(x, *w, bias, out_dtype == torch.float32, 17)
+    out = (_module or _faces()).linear4(x, *w, bias, out_dtype == torch.float32, 17, *(() if LINEAR4_POLLS is None else (LINEAR4_POLLS,)))
     launches["count"] += 1
     return out
 
