@@ -28,6 +28,7 @@ class Lost:
 
 DECODE = Lost()                  # decode attention (ops.attention_decode_lost)
 KEY_WEIGHTS = Lost()             # column sums of prompt portions (ops.key_weights_lost)
+LINEAR4 = Lost()                 # products with 4-bit weights on tcgen05 (ops.linear4_lost)
 
 
 class Listener:
@@ -48,4 +49,4 @@ class Listener:
             raise RuntimeError(f"column sums of a portion: a wait was given up (code {KEY_WEIGHTS.row >> 24}, block {KEY_WEIGHTS.row & 0xFFFFFF}); the portion's weights are void")
 
 
-__all__ = ["DECODE", "KEY_WEIGHTS", "Listener", "Lost"]
+__all__ = ["DECODE", "KEY_WEIGHTS", "LINEAR4", "Listener", "Lost"]

@@ -25,7 +25,7 @@ from lily_b200.cache.kv_cache import KVCacheManager, OutOfPages, bytes_per_token
 from lily_b200.config.model_config import read_model_dir
 from lily_b200.config.registry import architecture_names, resolve_architecture
 from lily_b200.config.server_args import ServerArgs
-from lily_b200.csrc.waits import DECODE as _LOST
+from lily_b200.csrc.waits import DECODE as _LOST, LINEAR4 as _LOST4
 from lily_b200.engine import check
 from lily_b200.engine.batch import FUTURE, Lane, StepBatch, StepEntry, Workspace, build_step_batch, order_entries, rows_are_even, wire_array
 from lily_b200.engine.profiler import DecodeProfiler
@@ -246,7 +246,7 @@ class ModelRunner:
         self.future_tokens = torch.zeros(self.max_requests + 1, dtype=torch.int32, device=self.device)
         self._last_rows: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None
         self.seq_lens: Dict[int, int] = {}
-        self._lost_heard = _LOST.count
+        self._lost_heard, self._lost4_heard = _LOST.count, _LOST4.count
         self._ring = _PinnedRing() if self.device.type == "cuda" else None
         self.profiler = DecodeProfiler.from_env() if self.device.type == "cuda" else None
         self.steps_run = 0
@@ -310,11 +310,14 @@ class ModelRunner:
 
     def check_waits(self) -> None:
         """Raises when a kernel that the host has waited for gave up a wait of its own, so that its step's results are no results.  (A read of
-        a word in the host's memory.)"""
-        lost = getattr(self.model.ctx.ops, "attention_decode_lost", None)       # (stand-ins for the kernels wait for nothing)
+        a word in the host's memory for each kind of kernel.)"""
+        lost, lost4 = (getattr(self.model.ctx.ops, name, None) for name in ("attention_decode_lost", "linear4_lost"))       # (stand-ins for the kernels wait for nothing)
         heard = _LOST.heard(lost) if lost is not None else self._lost_heard
-        if heard != self._lost_heard:
-            self._lost_heard = heard
+        heard4 = _LOST4.heard(lost4) if lost4 is not None else self._lost4_heard
+        (was, was4), (self._lost_heard, self._lost4_heard) = (self._lost_heard, self._lost4_heard), (heard, heard4)
+        if heard4 != was4:
+            raise RuntimeError(f"product with 4-bit weights: a wait was given up (code {_LOST4.row >> 24}, block {_LOST4.row & 0xFFFFFF}); the step's tokens are void")
+        if heard != was:
             raise RuntimeError(f"decode attention: a tile of keys did not arrive in time (row {_LOST.row - 1} of its step); the step's tokens are void")
 
     # ---- one step --------------------------------------------------------------------
