@@ -59,13 +59,17 @@ struct AttnArgs {
     int score_stride, max_len;      // ... and the places a row has at most
     int stages;               // decode, tensor-core kernel: key/value tiles a block keeps in shared memory (0: the default, 2;
                               // 3: two blocks a SM instead of three, each with two tiles in flight; head sizes up to 128)
-    const unsigned* spans;    // mma.sync prefill: not null where queries and keys are half-precision numbers times powers of two (below):
-    const float* units;       // [requests, nkv] of keys and [tokens, nq] of queries
+    const unsigned* spans;    // mma.sync prefill: not null where queries, keys and values are half-precision numbers times powers of two (below):
+    const unsigned* value_spans;      // [requests, nkv] of keys, of values,
+    const float* units;       // and [tokens, nq] of queries
 };
 
-// Queries and keys in half precision, whose eleven bits hold what four-bit codes, their steps and lowest values make of a key (bfloat16's eight would round it).  Each is multiplied by the power of two
-// that brings the largest magnitude to 2^13 .. 2^14, so that nothing overflows and 2^-28 of it is still a normal number: a token's query head by one of its own, and the keys of a request and kv head
-// by one together, so that no token's queries and no request's keys take bits from another's.  `spans` holds the keys' largest magnitudes, as bits of float32; `units` what a query head's power undoes.
+// Queries, keys and values in half precision, whose eleven bits hold what four-bit codes, their steps and lowest values make of a number (bfloat16's eight would round it).  Each is multiplied by the power
+// of two that brings the largest magnitude to 2^13 .. 2^14, so that nothing overflows and 2^-28 of it is still a normal number: a token's query head by one of its own, the keys and the values of a request
+// and kv head by one together each, so that no token's queries and no request's keys and values take bits from another's.  (A key or value that is 2^28 times another one of its request and kv head does
+// take bits from it.)  `spans` holds the largest magnitudes, as bits of float32; `units` what a query head's power undoes.  The softmax's weights, which multiply the values, are half-precision numbers
+// times 2^14 or less: their least ones lose bits from 2^-28 of the largest one on.
+constexpr float WEIGHT_LOG2 = 14.f;       // of the largest weight (65,504 is the type's largest number)
 __device__ __forceinline__ int span_exponent(unsigned bits) { return min(max(267 - (int)(bits >> 23), 1), 253); }
 __device__ __forceinline__ float span_multiplier(unsigned bits) { return __uint_as_float((unsigned)span_exponent(bits) << 23); }
 __device__ __forceinline__ float span_unit(unsigned bits) { return __uint_as_float((unsigned)(254 - span_exponent(bits)) << 23); }

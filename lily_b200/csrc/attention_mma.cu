@@ -99,6 +99,10 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&v);
@@ -638,19 +642,21 @@ attention_mma_kernel(const AttnArgs a, const int page_shift, const __grid_consta
         mx_lo = fmaxf(mx_lo, __shfl_xor_sync(0xffffffffu, mx_lo, 2));
         mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, 1));
         mx_hi = fmaxf(mx_hi, __shfl_xor_sync(0xffffffffu, mx_hi, 2));
-        // running maxima are kept in scaled (log2) units: scale > 0, so the order is the same
-        const float mn_lo = fmaxf(m_lo, mx_lo * sl2_lo), mn_hi = fmaxf(m_hi, mx_hi * sl2_hi);
+        // running maxima are kept in scaled (log2) units: scale > 0, so the order is the same (HALF: unscaled, and differences are taken first, since what a large rounded product is off by would have a
+        // weight overflow)
+        const float mn_lo = fmaxf(m_lo, HALF ? mx_lo : mx_lo * sl2_lo), mn_hi = fmaxf(m_hi, HALF ? mx_hi : mx_hi * sl2_hi);
         const float base_lo = mn_lo == -INFINITY ? 0.f : mn_lo, base_hi = mn_hi == -INFINITY ? 0.f : mn_hi;
-        const float al_lo = exp2f(m_lo - base_lo), al_hi = exp2f(m_hi - base_hi);
+        const float al_lo = exp2f(HALF ? (m_lo - base_lo) * sl2_lo : m_lo - base_lo), al_hi = exp2f(HALF ? (m_hi - base_hi) * sl2_hi : m_hi - base_hi);
         m_lo = mn_lo;
         m_hi = mn_hi;
         float sum_lo = 0.f, sum_hi = 0.f;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            s[j][0] = exp2f(fmaf(s[j][0], sl2_lo, -base_lo));
-            s[j][1] = exp2f(fmaf(s[j][1], sl2_lo, -base_lo));
-            s[j][2] = exp2f(fmaf(s[j][2], sl2_hi, -base_hi));
-            s[j][3] = exp2f(fmaf(s[j][3], sl2_hi, -base_hi));
+            auto weight = [](float x, float scale, float base) { return exp2f(HALF ? fmaf(x - base, scale, WEIGHT_LOG2) : fmaf(x, scale, -base)); };
+            s[j][0] = weight(s[j][0], sl2_lo, base_lo);
+            s[j][1] = weight(s[j][1], sl2_lo, base_lo);
+            s[j][2] = weight(s[j][2], sl2_hi, base_hi);
+            s[j][3] = weight(s[j][3], sl2_hi, base_hi);
             sum_lo += s[j][0] + s[j][1];
             sum_hi += s[j][2] + s[j][3];
         }
@@ -667,17 +673,23 @@ attention_mma_kernel(const AttnArgs a, const int page_shift, const __grid_consta
         // ---- o += p . v -------------------------------------------------------------------------
 #pragma unroll
         for (int kb16 = 0; kb16 < NT / 2; ++kb16) {
-            const uint32_t a0 = pack_bf16(s[2 * kb16][0], s[2 * kb16][1]);
-            const uint32_t a1 = pack_bf16(s[2 * kb16][2], s[2 * kb16][3]);
-            const uint32_t a2 = pack_bf16(s[2 * kb16 + 1][0], s[2 * kb16 + 1][1]);
-            const uint32_t a3 = pack_bf16(s[2 * kb16 + 1][2], s[2 * kb16 + 1][3]);
+            auto pair = [](float x, float y) { return HALF ? pack_half(x, y) : pack_bf16(x, y); };
+            const uint32_t a0 = pair(s[2 * kb16][0], s[2 * kb16][1]);
+            const uint32_t a1 = pair(s[2 * kb16][2], s[2 * kb16][3]);
+            const uint32_t a2 = pair(s[2 * kb16 + 1][0], s[2 * kb16 + 1][1]);
+            const uint32_t a3 = pair(s[2 * kb16 + 1][2], s[2 * kb16 + 1][3]);
             const int vrow = key0 + kb16 * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
 #pragma unroll
             for (int jp = 0; jp < D / 16; ++jp) {
                 uint32_t b0, b1, b2, b3;
                 ldmatrix_x4_trans(smem_u32(vt + piece(vrow, jp * 2 + (lane >> 4))), b0, b1, b2, b3);
-                mma_bf16(o[2 * jp], a0, a1, a2, a3, b0, b1);
-                mma_bf16(o[2 * jp + 1], a0, a1, a2, a3, b2, b3);
+                if constexpr (HALF) {
+                    mma_half(o[2 * jp], a0, a1, a2, a3, b0, b1);
+                    mma_half(o[2 * jp + 1], a0, a1, a2, a3, b2, b3);
+                } else {
+                    mma_bf16(o[2 * jp], a0, a1, a2, a3, b0, b1);
+                    mma_bf16(o[2 * jp + 1], a0, a1, a2, a3, b2, b3);
+                }
             }
         }
         if (TMA && t + STAGES < ntiles) {
@@ -699,15 +711,21 @@ attention_mma_kernel(const AttnArgs a, const int page_shift, const __grid_consta
     if (!DECODE) {
         __nv_bfloat16* out = (__nv_bfloat16*)a.out;
         const float inv_lo = l_lo > 0.f ? 1.f / l_lo : 0.f, inv_hi = l_hi > 0.f ? 1.f / l_hi : 0.f;
+        if constexpr (HALF) {
+            const float unit = span_unit(a.value_spans[(size_t)req * a.nkv + head0 / (a.nq / a.nkv)]);
+#pragma unroll
+            for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][0] * inv_lo * unit, o[j][1] = o[j][1] * inv_lo * unit, o[j][2] = o[j][2] * inv_hi * unit, o[j][3] = o[j][3] * inv_hi * unit;
+        }
+        const float by_lo = HALF ? 1.f : inv_lo, by_hi = HALF ? 1.f : inv_hi;
 #pragma unroll
         for (int j = 0; j < D / 8; ++j) {
             const int col = j * 8 + 2 * c;
             if (row_lo < nrows)
                 *reinterpret_cast<uint32_t*>(out + ((size_t)(tok0 + row_lo) * a.nq + head0) * D + col) =
-                    pack_bf16(o[j][0] * inv_lo, o[j][1] * inv_lo);
+                    pack_bf16(o[j][0] * by_lo, o[j][1] * by_lo);
             if (row_hi < nrows)
                 *reinterpret_cast<uint32_t*>(out + ((size_t)(tok0 + row_hi) * a.nq + head0) * D + col) =
-                    pack_bf16(o[j][2] * inv_hi, o[j][3] * inv_hi);
+                    pack_bf16(o[j][2] * by_hi, o[j][3] * by_hi);
         }
         return;
     }
@@ -1057,14 +1075,15 @@ LILY_API int lily_attention_prefill_mma(const void* q, const void* kv, void* out
     return 0;
 }
 
-// The same over queries and keys in half precision (values stay bfloat16); spans, units: attention_args.cuh.
+// The same over queries, keys and values in half precision; spans, value_spans, units: attention_args.cuh.
 LILY_API int lily_attention_prefill_mma_half(const void* q, const void* kv, void* out, const int* block_table, int bt_stride, const int* cu_seqlens, const int* prefix_lens, const int* tile_req,
-                                             const int* tile_start, int tiles, int nq, int nkv, int d, int page_size, float scale, const unsigned* spans, const float* units, cudaStream_t stream) {
+                                             const int* tile_start, int tiles, int nq, int nkv, int d, int page_size, float scale, const unsigned* spans, const unsigned* value_spans, const float* units,
+                                             cudaStream_t stream) {
     if (tiles == 0) return 0;
-    LILY_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0 && spans != nullptr && units != nullptr, "attention_prefill: %d query heads over %d kv heads", nq, nkv);
+    LILY_REQUIRE(nq > 0 && nkv > 0 && nq % nkv == 0 && spans != nullptr && value_spans != nullptr && units != nullptr, "attention_prefill: %d query heads over %d kv heads", nq, nkv);
     LILY_REQUIRE(nq <= 65535 && page_size > 0, "attention_prefill: nq=%d page_size=%d", nq, page_size);
     AttnArgs a{};
-    a.q = q; a.kv = kv; a.out = out; a.block_table = block_table; a.bt_stride = bt_stride; a.spans = spans; a.units = units;
+    a.q = q; a.kv = kv; a.out = out; a.block_table = block_table; a.bt_stride = bt_stride; a.spans = spans; a.value_spans = value_spans; a.units = units;
     a.cu_seqlens = cu_seqlens; a.prefix_lens = prefix_lens; a.tile_req = tile_req; a.tile_start = tile_start;
     a.splits = 1; a.nq = nq; a.nkv = nkv; a.d = d; a.page_size = page_size; a.scale = scale;
     bool merged = false;

@@ -37,6 +37,8 @@
 #include "common.cuh"
 #include "tcgen05.cuh"
 
+#include <cuda_fp16.h>
+
 #include <cstdlib>
 
 namespace lily {
@@ -75,7 +77,8 @@ constexpr int off_p(int d) { return (1 + 2 * STAGES) * tile_bytes(d); }
 constexpr int off_bars(int d) { return off_p(d) + (P_TMEM ? 0 : SBUF) * P_TILE; }
 constexpr int off_misc(int d) { return off_bars(d) + 8 * NUM_BARS + 8; }
 constexpr int off_xch(int d) { return off_misc(d) + 16; }
-constexpr int smem_one(int d) { return off_xch(d) + 2 * PARTS * BQ * 4; }
+constexpr int off_tags(int d) { return off_xch(d) + 2 * PARTS * BQ * 4; }       // HALF: a byte a word
+constexpr int smem_one(int d, bool half) { return off_tags(d) + (half ? 2 * PARTS * BQ : 0); }
 constexpr uint32_t SPIN_LIMIT = 1u << 24;
 constexpr float GROW_LOG2 = 8.f;          // the reference maximum moves when the true one is 2^8 ahead
 
@@ -104,14 +107,34 @@ struct Params {
     float scale_log2;                     // softmax scale times log2(e) (log2(e) alone under a cap)
     int sink;                             // the softmax's denominator holds one more unit: a key of score 0 without a value
     size_t plane;                         // elements between the planes of `out` (grid z): plane z weighs the values of kv head (own + z) % nkv
-    const unsigned* spans;                // not null where queries and keys are half-precision numbers times powers of two (attention_args.cuh):
-    const float* units;                   // of the keys and of the queries
+    const unsigned* spans;                // not null where queries, keys, weights and values are half-precision numbers times powers of two (attention_args.cuh; the kernels' HALF):
+    const unsigned* value_spans;          // of the keys, of the values
+    const float* units;                   // and of the queries
     float cap, cap_in;                    // cap > 0: scores become cap * tanh(score * cap_in), cap_in = scale / cap
 };
 // What a row's scores are multiplied by in units of log2.
+template <bool HALF>
 __device__ __forceinline__ float row_scale(const Params& p, int req, int token, int head) {
-    if (!p.spans) return p.scale_log2;
+    if (!HALF) return p.scale_log2;
     return span_scale(p.scale_log2, p.units[(size_t)token * p.nq + head], p.spans[(size_t)req * p.nkv + head / (p.nq / p.nkv)]);
+}
+// A pair of weights as the second product takes them, and the exponents of N scores above their row's maximum `most` (`mb`: that times the scale).  HALF: the difference is taken first, since what a large
+// rounded product is off by would have a weight overflow; two operations for two scores, as without.
+template <bool HALF>
+__device__ __forceinline__ uint32_t weights2(float x, float y) {
+    if (!HALF) return pack2(x, y);
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <bool HALF>
+__device__ __forceinline__ void exponents2(float& x, float& y, float scale_log2, float mb, float most) {
+    if (!HALF) {
+        x = fmaf(x, scale_log2, -mb);
+        y = fmaf(y, scale_log2, -mb);
+        return;
+    }
+    asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%0, %1};\nmov.b64 b, {%2, %2};\nmov.b64 c, {%3, %3};\nmov.b64 d, {%4, %4};\nadd.rn.f32x2 a, a, b;\nfma.rn.f32x2 a, a, c, d;\nmov.b64 {%0, %1}, a;\n}\n"
+        : "+f"(x), "+f"(y) : "f"(-most), "f"(scale_log2), "f"(WEIGHT_LOG2 - GROW_LOG2));
 }
 
 // The hardware's tanh (relative error about 2^-11; the weights are rounded to bfloat16 for the p.v product).
@@ -130,7 +153,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     atomicCAS(&g_status, 0, (code << 24) | (int)((blockIdx.x + blockIdx.y * gridDim.x) & 0xFFFFFF));
     return false;
 }
-template <int D>
+template <int D, bool HALF>
 __global__ void __launch_bounds__(THREADS, 1)
 attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, const Params p) {
     static_assert(D == 64 || D == 128, "head sizes 64 and 128");
@@ -173,6 +196,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     for (int i = threadIdx.x; i < PARTS * BQ; i += THREADS) {    // exchange slots start with the tag before their first
         reinterpret_cast<uint32_t*>(xch)[i] = 3u;                                 // parity 0: tags 1, 3, 1, ...
         reinterpret_cast<uint32_t*>(xch)[PARTS * BQ + i] = 0u;                    // parity 1: tags 2, 0, 2, ...
+        if (HALF) smem[off_tags(D) + i] = 3, smem[off_tags(D) + PARTS * BQ + i] = 0;
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_base_s)), "r"(512) : "memory");
@@ -250,8 +274,9 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     } else if (warp == 1) {
         if (lane == 0) {
             // kind::f16: float32 accumulator, bfloat16 a and b, n = 128, m = 128; bit 16 makes b MN-major
-            const uint32_t idesc_s = (1u << 4) | (p.spans ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
-            const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+            constexpr uint32_t TYPES = HALF ? 0u : (1u << 7) | (1u << 10);      // half precision, or bfloat16
+            const uint32_t idesc_s = (1u << 4) | TYPES | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+            const uint32_t idesc_o = (1u << 4) | TYPES | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
             bool ok = mbar_wait(q_full, 0, abort_flag, 3);
             auto scores = [&](int i) {                   // S_i = Q K_i^T into accumulator i % 2
                 const int s = i % STAGES;
@@ -308,7 +333,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         const int row = quarter * 32 + lane;
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
         const int pos = pos0 + row;
-        const float scale_log2 = row_scale(p, req, q_begin + start + min(row, rows_valid - 1), head);
+        const float scale_log2 = row_scale<HALF>(p, req, q_begin + start + min(row, rows_valid - 1), head), unit = HALF ? span_unit(p.value_spans[(size_t)req * p.nkv + head / (p.nq / p.nkv)]) : 1.f;
         float m_used = p.sink ? 0.f : -INFINITY, l = 0.f;
         bool ok = true;
         // The threads of a row hand each other one float per tile (the maximum of their keys; at the end
@@ -316,11 +341,18 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         // tag, so a reader knows the word is this tile's without a barrier that an aborted partner
         // would never reach.  Slots alternate with the tile's parity; every thread drops the same two
         // bits of its own value, so all agree on the result.  `combine` folds the values in part order.
+        // HALF: the tag has a byte of its own and the word all its bits, since what a large maximum loses
+        // by two of them would have a weight overflow.
         volatile uint32_t* xw = reinterpret_cast<volatile uint32_t*>(xch);
+        volatile unsigned char* tags = smem + off_tags(D);
         auto exchange = [&](int seq, float mine, bool sum, float& result) {
             const uint32_t tag = (uint32_t)(seq + 1) & 3u;
-            const uint32_t bits = __float_as_uint(mine) & ~3u;
-            xw[((seq & 1) * PARTS + part) * BQ + row] = bits | tag;
+            const uint32_t bits = __float_as_uint(mine) & (HALF ? ~0u : ~3u);
+            xw[((seq & 1) * PARTS + part) * BQ + row] = HALF ? bits : bits | tag;
+            if (HALF) {
+                __threadfence_block();
+                tags[((seq & 1) * PARTS + part) * BQ + row] = (unsigned char)tag;
+            }
             float acc = sum ? 0.f : -INFINITY;
 #pragma unroll
             for (int q = 0; q < PARTS; ++q) {
@@ -329,9 +361,10 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                     volatile uint32_t* from = xw + ((seq & 1) * PARTS + q) * BQ + row;
                     bool got = false;
                     for (uint32_t i = 0; i < SPIN_LIMIT; ++i) {
-                        const uint32_t w = *from;
+                        const uint32_t w = HALF ? tags[from - xw] : *from;
                         if ((w & 3u) == tag) {
-                            v = __uint_as_float(w & ~3u);
+                            if (HALF) __threadfence_block();
+                            v = __uint_as_float(HALF ? *from : w & ~3u);
                             got = true;
                             break;
                         }
@@ -409,11 +442,12 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 }
             }
             FA_TOC(22 + (part & 1), row == 0);
-            const float mb = (m_used == -INFINITY ? 0.f : m_used) * scale_log2;
+            const float most = m_used == -INFINITY ? 0.f : m_used, mb = most * scale_log2;
             float sum4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < COLS; ++c) {
-                s[c] = ex2(fmaf(s[c], scale_log2, -mb));
+                if (c % 2 == 0) exponents2<HALF>(s[c], s[c + 1], scale_log2, mb, most);
+                s[c] = ex2(s[c]);
                 sum4[c & 3] += s[c];
             }
             l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
@@ -425,7 +459,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 // S product whose result was just read.
                 uint32_t packed[COLS / 2];
 #pragma unroll
-                for (int c = 0; c < COLS / 2; ++c) packed[c] = pack2(s[2 * c], s[2 * c + 1]);
+                for (int c = 0; c < COLS / 2; ++c) packed[c] = weights2<HALF>(s[2 * c], s[2 * c + 1]);
                 if (COLS == 64) tmem_st32(tmem + lane_addr + (uint32_t)(b * BKV + part * (COLS / 2)), reinterpret_cast<const float*>(packed));
                 else tmem_st16(tmem + lane_addr + (uint32_t)(b * BKV + part * (COLS / 2)), reinterpret_cast<const float*>(packed));
                 FA_TOC(24 + (part & 1), row == 0);
@@ -445,7 +479,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 for (int c = 0; c < COLS / 8; ++c) {
                     const float* v = s + c * 8;
                     *reinterpret_cast<uint4*>(prow + (((c0 + c) ^ (row & 7)) << 4)) =
-                        make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+                        make_uint4(weights2<HALF>(v[0], v[1]), weights2<HALF>(v[2], v[3]), weights2<HALF>(v[4], v[5]), weights2<HALF>(v[6], v[7]));
                 }
                 asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // the tensor cores read P through the async proxy
             }
@@ -472,11 +506,15 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                 tmem_ld32(tmem_o + lane_addr + (uint32_t)(part * OCOLS + c * 32), o);
                 tmem_wait_ld();
                 if (row < rows_valid) {
+                    if (HALF)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = o[e] * inv * unit;
+                    const float by = HALF ? 1.f : inv;
 #pragma unroll
                     for (int v = 0; v < 4; ++v)
                         *reinterpret_cast<uint4*>(dst + c * 32 + v * 8) =
-                            make_uint4(pack2(o[v * 8] * inv, o[v * 8 + 1] * inv), pack2(o[v * 8 + 2] * inv, o[v * 8 + 3] * inv),
-                                       pack2(o[v * 8 + 4] * inv, o[v * 8 + 5] * inv), pack2(o[v * 8 + 6] * inv, o[v * 8 + 7] * inv));
+                            make_uint4(pack2(o[v * 8] * by, o[v * 8 + 1] * by), pack2(o[v * 8 + 2] * by, o[v * 8 + 3] * by),
+                                       pack2(o[v * 8 + 4] * by, o[v * 8 + 5] * by), pack2(o[v * 8 + 6] * by, o[v * 8 + 7] * by));
                 }
             }
         }
@@ -512,7 +550,7 @@ constexpr int off2_bars(int d) { return off2_v(d) + KV2 * tile_bytes(d); }
 constexpr int off2_misc(int d) { return off2_bars(d) + 8 * NUM_BARS2 + 8; }
 constexpr int smem_two(int d) { return off2_misc(d) + 16; }
 
-template <int D>
+template <int D, bool HALF>
 __global__ void __launch_bounds__(THREADS2, 1)
 attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, const Params p) {
     static_assert(D == 64 || D == 128, "head sizes 64 and 128");
@@ -620,8 +658,9 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            const uint32_t idesc_s = (1u << 4) | (p.spans ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
-            const uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+            constexpr uint32_t TYPES = HALF ? 0u : (1u << 7) | (1u << 10);      // half precision, or bfloat16
+            const uint32_t idesc_s = (1u << 4) | TYPES | ((uint32_t)(BKV >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+            const uint32_t idesc_o = (1u << 4) | TYPES | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
             bool ok = mbar_wait(q_full, 0, abort_flag, 3);
             auto scores = [&](int h, int i) {            // S_h(i) = Q_h K_i^T; the second head hands the K stage back
                 const int s = i % KV2;
@@ -701,7 +740,7 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
         const uint32_t my_s = tmem + lane_addr + (uint32_t)(h * BKV), my_o = tmem_o + lane_addr + (uint32_t)(h * D);
         const int pos = pos0 + row;
-        const float scale_log2 = row_scale(p, req, q_begin + start + min(row, rows_valid - 1), head0 + h);
+        const float scale_log2 = row_scale<HALF>(p, req, q_begin + start + min(row, rows_valid - 1), head0 + h), unit = HALF ? span_unit(p.value_spans[(size_t)req * p.nkv + head0 / (p.nq / p.nkv)]) : 1.f;
         float m_used = p.sink ? 0.f : -INFINITY, l = 0.f;
         bool ok = true;
         for (int j = 0; j < n && ok; ++j) {
@@ -762,7 +801,7 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
             }
             // second pass: P = exp2(s * scale - max) as bfloat16 pairs over the first 64 columns of S.  Piece c
             // lands on columns [16 c, 16 c + 16), all of them in pieces that this pass has read already.
-            const float mb = (m_used == -INFINITY ? 0.f : m_used) * scale_log2;
+            const float most = m_used == -INFINITY ? 0.f : m_used, mb = most * scale_log2;
             float sum4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
             for (int c = 0; c < BKV / 32; ++c) {
@@ -783,12 +822,13 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
                 }
 #pragma unroll
                 for (int e = 0; e < 32; ++e) {
-                    s[e] = ex2(fmaf(s[e], scale_log2, -mb));
+                    if (e % 2 == 0) exponents2<HALF>(s[e], s[e + 1], scale_log2, mb, most);
+                    s[e] = ex2(s[e]);
                     sum4[e & 3] += s[e];
                 }
                 uint32_t packed[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) packed[e] = pack2(s[2 * e], s[2 * e + 1]);
+                for (int e = 0; e < 16; ++e) packed[e] = weights2<HALF>(s[2 * e], s[2 * e + 1]);
                 tmem_st16(my_s + (uint32_t)(c * 16), reinterpret_cast<const float*>(packed));
             }
             l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
@@ -809,11 +849,15 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
                 tmem_ld32(my_o + (uint32_t)(c * 32), o);
                 tmem_wait_ld();
                 if (row < rows_valid) {
+                    if (HALF)
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = o[e] * inv * unit;
+                    const float by = HALF ? 1.f : inv;
 #pragma unroll
                     for (int v = 0; v < 4; ++v)
                         *reinterpret_cast<uint4*>(dst + c * 32 + v * 8) =
-                            make_uint4(pack2(o[v * 8] * inv, o[v * 8 + 1] * inv), pack2(o[v * 8 + 2] * inv, o[v * 8 + 3] * inv),
-                                       pack2(o[v * 8 + 4] * inv, o[v * 8 + 5] * inv), pack2(o[v * 8 + 6] * inv, o[v * 8 + 7] * inv));
+                            make_uint4(pack2(o[v * 8] * by, o[v * 8 + 1] * by), pack2(o[v * 8 + 2] * by, o[v * 8 + 3] * by),
+                                       pack2(o[v * 8 + 4] * by, o[v * 8 + 5] * by), pack2(o[v * 8 + 6] * by, o[v * 8 + 7] * by));
                 }
             }
         }
@@ -829,23 +873,23 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
 // ---- host side --------------------------------------------------------------------------------
 
 // Launches the kernel of head size D with one head or two heads a block (the shared memory limits are raised once).
-template <int D>
+template <int D, bool HALF = false>
 static int launch(bool two, int nq, int tiles, int planes, cudaStream_t stream, const CUtensorMap& map_q, const CUtensorMap& map_kv, const Params& p) {
     static bool configured = false;
     if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(attention_prefill_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_one(D));
+        cudaError_t e = cudaFuncSetAttribute(attention_prefill_tc_kernel<D, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_one(D, HALF));
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(attention_prefill_tc2_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_two(D));
+            e = cudaFuncSetAttribute(attention_prefill_tc2_kernel<D, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_two(D));
         if (e != cudaSuccess) {
-            set_error("attention_prefill_tc: cannot get %d bytes of shared memory: %s", smem_one(D), cudaGetErrorString(e));
+            set_error("attention_prefill_tc: cannot get %d bytes of shared memory: %s", smem_one(D, HALF), cudaGetErrorString(e));
             return 2;
         }
         configured = true;
     }
     if (two)
-        launch_pdl(attention_prefill_tc2_kernel<D>, dim3(nq / 2, tiles, planes), dim3(THREADS2), (size_t)smem_two(D), stream, map_q, map_kv, p);
+        launch_pdl(attention_prefill_tc2_kernel<D, HALF>, dim3(nq / 2, tiles, planes), dim3(THREADS2), (size_t)smem_two(D), stream, map_q, map_kv, p);
     else
-        launch_pdl(attention_prefill_tc_kernel<D>, dim3(nq, tiles, planes), dim3(THREADS), (size_t)smem_one(D), stream, map_q, map_kv, p);
+        launch_pdl(attention_prefill_tc_kernel<D, HALF>, dim3(nq, tiles, planes), dim3(THREADS), (size_t)smem_one(D, HALF), stream, map_q, map_kv, p);
     return 0;
 }
 
@@ -884,7 +928,7 @@ LILY_API int lily_attention_tc_status() {
 
 static int prefill_tc(const void* q, const void* kv, void* out, const int* block_table, int bt_stride, const int* cu_seqlens, const int* prefix_lens, const int* tile_req, const int* tile_start,
                       int tiles, int nq, int nkv, int d, int page_size, int window, float scale, int tokens, int num_pages, int heads_per_block, float softcap, int keep_first, int sink, int planes,
-                      const unsigned* spans, const float* units, cudaStream_t stream) {
+                      const unsigned* spans, const unsigned* value_spans, const float* units, cudaStream_t stream) {
     if (tiles == 0) return 0;
     LILY_REQUIRE(planes >= 1 && planes <= nkv, "attention_prefill_tc: %d planes of %d kv heads", planes, nkv);
     LILY_REQUIRE(lily_attention_prefill_tc_takes(d, page_size), "attention_prefill_tc: head size %d, page size %d (takes 64 or 128, and multiples of 64)",
@@ -916,7 +960,7 @@ static int prefill_tc(const void* q, const void* kv, void* out, const int* block
         LILY_REQUIRE(rc == CUDA_SUCCESS, "attention_prefill_tc: cuTensorMapEncodeTiled (cache) failed with %d", (int)rc);
     }
     fa::Params p{};
-    p.spans = spans; p.units = units;
+    p.spans = spans; p.value_spans = value_spans; p.units = units;
     p.block_table = block_table; p.cu_seqlens = cu_seqlens; p.prefix_lens = prefix_lens; p.tile_req = tile_req;
     p.tile_start = tile_start; p.out = (__nv_bfloat16*)out; p.bt_stride = bt_stride; p.tiles = tiles; p.nq = nq; p.nkv = nkv;
     p.page_size = page_size; p.window = window; p.sink = sink; p.plane = (size_t)tokens * nq * d;
@@ -931,7 +975,8 @@ static int prefill_tc(const void* q, const void* kv, void* out, const int* block
     LILY_REQUIRE(heads_per_block >= 0 && heads_per_block <= 2 && (heads_per_block != 2 || even),
                  "attention_prefill_tc: %d heads a block with %d query heads per kv head", heads_per_block, nq / nkv);
     const bool two = heads_per_block == 2 || (heads_per_block == 0 && even && (long)tiles * planes * (nq / 2) >= sms);
-    const int rc = d == 64 ? fa::launch<64>(two, nq, tiles, planes, stream, map_q, map_kv, p) : fa::launch<128>(two, nq, tiles, planes, stream, map_q, map_kv, p);
+    const int rc = spans ? d == 64 ? fa::launch<64, true>(two, nq, tiles, planes, stream, map_q, map_kv, p) : fa::launch<128, true>(two, nq, tiles, planes, stream, map_q, map_kv, p)
+                         : d == 64 ? fa::launch<64>(two, nq, tiles, planes, stream, map_q, map_kv, p) : fa::launch<128>(two, nq, tiles, planes, stream, map_q, map_kv, p);
     if (rc) return rc;
     LILY_CHECK_LAUNCH("attention_prefill_tc");
     return 0;
@@ -948,13 +993,13 @@ LILY_API int lily_attention_prefill_tc(const void* q, const void* kv, void* out,
                                        float scale, int tokens, int num_pages, int heads_per_block, float softcap,
                                        int keep_first, int sink, int planes, cudaStream_t stream) {
     return prefill_tc(q, kv, out, block_table, bt_stride, cu_seqlens, prefix_lens, tile_req, tile_start, tiles, nq, nkv, d, page_size, window, scale, tokens, num_pages, heads_per_block, softcap,
-                      keep_first, sink, planes, nullptr, nullptr, stream);
+                      keep_first, sink, planes, nullptr, nullptr, nullptr, stream);
 }
 
-// The same over queries and keys in half precision (values stay bfloat16), without cap, window and sink; spans, units: attention_args.cuh.
+// The same over queries, keys and values in half precision, without cap, window and sink; spans, value_spans, units: attention_args.cuh.
 LILY_API int lily_attention_prefill_tc_half(const void* q, const void* kv, void* out, const int* block_table, int bt_stride, const int* cu_seqlens, const int* prefix_lens, const int* tile_req,
                                             const int* tile_start, int tiles, int nq, int nkv, int d, int page_size, float scale, int tokens, int num_pages, const unsigned* spans,
-                                            const float* units, cudaStream_t stream) {
-    LILY_REQUIRE(spans != nullptr && units != nullptr, "attention_prefill_tc: half-precision queries and keys come with their powers of two");
-    return prefill_tc(q, kv, out, block_table, bt_stride, cu_seqlens, prefix_lens, tile_req, tile_start, tiles, nq, nkv, d, page_size, 0, scale, tokens, num_pages, 0, 0.f, 0, 0, 1, spans, units, stream);
+                                            const unsigned* value_spans, const float* units, cudaStream_t stream) {
+    LILY_REQUIRE(spans != nullptr && value_spans != nullptr && units != nullptr, "attention_prefill_tc: half-precision queries, keys and values come with their powers of two");
+    return prefill_tc(q, kv, out, block_table, bt_stride, cu_seqlens, prefix_lens, tile_req, tile_start, tiles, nq, nkv, d, page_size, 0, scale, tokens, num_pages, 0, 0.f, 0, 0, 1, spans, value_spans, units, stream);
 }

@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) write_turned_kernel(const Wr
 
 // Pages as numbers, lowest + step code in one rounding: of every page that a block table names to [requests, width, 2, nkv, page_size, d] (``compact`` false), or of the pages
 // that portions of prompts see, one request's behind the other's, [pages, 2, nkv, page_size, d], with a block table of them and zeros behind a request's last place.
-// Eight threads a place and kind, each with the words that lie side by side, one a group.  ``spans``: keys become half-precision numbers times a power of two (attention_args.cuh).
+// Eight threads a place and kind, each with the words that lie side by side, one a group.  ``spans`` [2 (keys, values), requests, nkv]: half-precision numbers times powers of two (attention_args.cuh).
 // grid (pages, requests, kv heads x 2)
 template <typename T, int G>
 __global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__ kv, int pages, const int* __restrict__ block_table, int width, T* __restrict__ out, int nkv, int page_size,
@@ -313,8 +313,8 @@ __global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__
     const uint32_t *words = reinterpret_cast<const uint32_t*>(rows), *held = reinterpret_cast<const uint32_t*>(rows + (size_t)page_size * (D / 2));
     T* dst = out + ((to * 2 + value) * nkv + head) * ((size_t)page_size * D);
     const int i8 = threadIdx.x & 7;
-    const bool halves = sizeof(T) == 2 && spans && !value;
-    const float by = halves ? span_multiplier(spans[(size_t)r * nkv + head]) : 1.f;
+    const bool halves = sizeof(T) == 2 && spans;
+    const float by = halves ? span_multiplier(spans[((size_t)value * gridDim.y + r) * nkv + head]) : 1.f;
 #pragma unroll 2
     for (int slot = threadIdx.x >> 3; slot < page_size; slot += 32) {
         uint32_t w[G], h[G];
@@ -335,11 +335,11 @@ __global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__
 }
 
 // What portions attend with in half precision (attention_args.cuh).  blocks [0, query_blocks): queries, times the power of two of their token and head, eight numbers a thread and d / 8 threads a head;
-// the others, a block a (page, request) and a warp a kv head at a time: a bound of the keys' magnitudes from their steps and lowest values (lowest + 15 step, or lowest), as bits that are compared as
-// whole numbers.  What is no number counts for nothing.
+// the others, a block a (page, request) and a warp a kv head and kind at a time: a bound of the keys' or values' magnitudes from their steps and lowest values (lowest + 15 step, or lowest), as bits that
+// are compared as whole numbers.  What is no number counts for nothing.
 __global__ void __launch_bounds__(256) halves_kernel(const __nv_bfloat16* __restrict__ q, size_t heads, __nv_bfloat16* __restrict__ out, float* __restrict__ units, int query_blocks,
                                                      const uint8_t* __restrict__ kv, int pages, const int* __restrict__ block_table, int width, int nkv, int d, int page_size,
-                                                     const int* __restrict__ cu, const int* __restrict__ prefix, int most, unsigned* __restrict__ spans) {
+                                                     const int* __restrict__ cu, const int* __restrict__ prefix, int requests, int most, unsigned* __restrict__ spans) {
     pdl_enter_small();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float m = 0.f;
@@ -378,8 +378,8 @@ __global__ void __launch_bounds__(256) halves_kernel(const __nv_bfloat16* __rest
     int page = at < width ? block_table[(size_t)r * width + at] : 0;
     if ((unsigned)page >= (unsigned)pages) page = 0;
     const size_t rows = (size_t)page_size * row_bytes(d);
-    for (int head = warp; head < nkv; head += 8) {
-        const uint32_t* held = reinterpret_cast<const uint32_t*>(kv + ((size_t)page * nkv + head) * 2 * rows + (size_t)page_size * (d / 2));
+    for (int which = warp; which < 2 * nkv; which += 8) {            // (head, kind)
+        const uint32_t* held = reinterpret_cast<const uint32_t*>(kv + ((size_t)page * nkv * 2 + which) * rows + (size_t)page_size * (d / 2));
         m = 0.f;
 #pragma unroll 4
         for (int i = lane; i < places * groups; i += 32) {
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(256) halves_kernel(const __nv_bfloat16* __rest
             take(high(h)), take(fmaf(15.f, low(h), high(h)));
         }
         const unsigned bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
-        if (lane == 0 && bits) atomicMax(spans + (size_t)r * nkv + head, bits);
+        if (lane == 0 && bits) atomicMax(spans + ((size_t)(which & 1) * requests + r) * nkv + (which >> 1), bits);
     }
 }
 
@@ -451,7 +451,7 @@ LILY_API int lily_qk_norm_rope_write4(const void* qkv, int dtype, int ld, const 
     return 0;
 }
 
-// spans: null, or the largest magnitudes of keys, for keys in half precision (lily_halves4).  cu, prefix, table_out: null, or of a step's portions (offsets of their tokens, tokens cached ahead of them, a block
+// spans: null, or the largest magnitudes of keys and values, for numbers in half precision (lily_halves4).  cu, prefix, table_out: null, or of a step's portions (offsets of their tokens, tokens cached ahead of them, a block
 // table [requests, table_width] of the pages written, of which there is room for `most_pages`).
 LILY_API int lily_cache4_values(const void* kv, int pages, const int* block_table, int requests, int width, void* out, int dtype, int nkv, int d, int page_size, const int* cu,
                                 const int* prefix, int* table_out, int table_width, int most_pages, const unsigned* spans, cudaStream_t stream) {
@@ -478,7 +478,7 @@ LILY_API int lily_cache4_values(const void* kv, int pages, const int* block_tabl
     return 0;
 }
 
-// What portions attend with in half precision (attention_args.cuh): the largest magnitudes of keys to `spans` [requests, nkv] (`zeroed` bytes from there on are set to zero first), the queries times powers
+// What portions attend with in half precision (attention_args.cuh): the largest magnitudes of keys and values to `spans` [2, requests, nkv] (`zeroed` bytes from there on are set to zero first), the queries times powers
 // of two to `out`, what undoes them to `units` [tokens, nq].  tiles: up to lily_halves4_tiles() of the portions' tiles, numbers of the host (requests, then offsets), which go to `tiles_out`.
 LILY_API int lily_halves4_tiles() { return four::MOST_TILES; }
 LILY_API int lily_halves4(const void* q, int tokens, int nq, const void* kv, int pages, const int* block_table, int requests, int width, int nkv, int d, int page_size, const int* cu, const int* prefix,
@@ -488,7 +488,7 @@ LILY_API int lily_halves4(const void* q, int tokens, int nq, const void* kv, int
     LILY_REQUIRE(((uintptr_t)q | (uintptr_t)out | (uintptr_t)kv) % 16 == 0, "halves4: tensors on boundaries of sixteen bytes");
     const size_t heads = (size_t)tokens * nq, a_block = 8 * (32 / (d / 8)), query_blocks = (heads + a_block - 1) / a_block;
     LILY_REQUIRE(query_blocks <= INT32_MAX / 2, "halves4: %d tokens", tokens);
-    LILY_REQUIRE(zeroed >= (size_t)requests * nkv * sizeof(unsigned) && zeroed % 4 == 0 && zeroed <= INT32_MAX, "halves4: %zu bytes of spans and tables", zeroed);
+    LILY_REQUIRE(zeroed >= (size_t)2 * requests * nkv * sizeof(unsigned) && zeroed % 4 == 0 && zeroed <= INT32_MAX, "halves4: %zu bytes of spans and tables", zeroed);
     LILY_REQUIRE(tile_count >= 0 && tile_count <= four::MOST_TILES && (tile_count == 0 || (tiles && tiles_out)), "halves4: %d tiles", tile_count);
     four::Tiles with;
     with.n = tile_count;
@@ -496,7 +496,7 @@ LILY_API int lily_halves4(const void* q, int tokens, int nq, const void* kv, int
     launch_pdl(four::zero_kernel, dim3((unsigned)((max((int)(zeroed / 4), 2 * tile_count) + 255) / 256)), dim3(256), 0, stream, spans, (int)(zeroed / 4), tiles_out, with);
     LILY_CHECK_LAUNCH("halves4");
     launch_pdl(four::halves_kernel, dim3((unsigned)query_blocks + requests * most_pages), dim3(256), 0, stream, (const __nv_bfloat16*)q, heads, (__nv_bfloat16*)out, units, (int)query_blocks,
-               (const uint8_t*)kv, pages, block_table, width, nkv, d, page_size, cu, prefix, most_pages, spans);
+               (const uint8_t*)kv, pages, block_table, width, nkv, d, page_size, cu, prefix, requests, most_pages, spans);
     LILY_CHECK_LAUNCH("halves4");
     return 0;
 }

@@ -60,8 +60,8 @@ struct Entries {
     int (*decode4)(const void*, const void*, void*, const int*, int, const int*, float*, int, int, int, int, int, int, int, float, int, void*);
     int (*halves4)(const void*, int, int, const void*, int, const int*, int, int, int, int, int, const int*, const int*, int, unsigned*, size_t, const int*, int, int*, void*, float*, void*);
     int (*halves4_tiles)();
-    int (*prefill_tc_half)(const void*, const void*, void*, const int*, int, const int*, const int*, const int*, const int*, int, int, int, int, int, float, int, int, const unsigned*, const float*, void*);
-    int (*prefill_mma_half)(const void*, const void*, void*, const int*, int, const int*, const int*, const int*, const int*, int, int, int, int, int, float, const unsigned*, const float*, void*);
+    int (*prefill_tc_half)(const void*, const void*, void*, const int*, int, const int*, const int*, const int*, const int*, int, int, int, int, int, float, int, int, const unsigned*, const unsigned*, const float*, void*);
+    int (*prefill_mma_half)(const void*, const void*, void*, const int*, int, const int*, const int*, const int*, const int*, int, int, int, int, int, float, const unsigned*, const unsigned*, const float*, void*);
 } entry;
 
 // ---- words ----
@@ -641,11 +641,12 @@ PyObject* attention_prefill4(PyObject*, PyObject* const* p, Py_ssize_t count) {
         if (kernel == 0) return Py_BuildValue("(NNNLL)", THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(req)), THPVariable_Wrap(std::move(start)), (long long)c.pages, (long long)c.width);
         if (!is(q, at::kBFloat16)) refuse(what, ": these kernels take bfloat16");
         if (tokens == 0) return THPVariable_Wrap(std::move(out));
-        // the keys' spans and the block table of the numbers, zeros; the numbers of the pages; queries in half precision and what undoes their powers of two
-        const int64_t spans_n = requests * nkv, words_n = spans_n + requests * c.width;
+        // the keys' and the values' spans and the block table of the numbers, zeros; the numbers of the pages; queries in half precision and what undoes their powers of two
+        const int64_t spans_n = 2 * requests * nkv, words_n = spans_n + requests * c.width;
         Tensor zeroed = at::empty({words_n + (int64_t)c.tiles.size()}, q.options().dtype(at::kInt)), values = at::empty({c.pages, 2, (int64_t)nkv, (int64_t)page, (int64_t)d}, q.options());
         Tensor heads = at::empty_like(q), units = at::empty({q.size(0), (int64_t)nq}, q.options().dtype(at::kFloat));
         unsigned* spans = (unsigned*)zeroed.data_ptr<int>();
+        const unsigned* value_spans = spans + requests * nkv;
         int* numbers = zeroed.data_ptr<int>() + spans_n;
         const int* bt = table.const_data_ptr<int>();
         const int n = narrow(q.size(0)), pages = narrow(c.pages), wide = narrow(c.width), r = narrow(requests), tiles_n = narrow(tiles), held = narrow(kv.size(0));
@@ -656,10 +657,10 @@ PyObject* attention_prefill4(PyObject*, PyObject* const* p, Py_ssize_t count) {
         done("lily_cache4_values", call(entry.values4, kv.const_data_ptr(), held, bt, r, width, values.data_ptr(), BF16, nkv, d, page, offsets, behind, numbers, wide, pages, (const unsigned*)spans, stream()));
         if (kernel == 2)
             done("lily_attention_prefill_tc_half", call(entry.prefill_tc_half, heads.const_data_ptr(), values.const_data_ptr(), out.data_ptr(), (const int*)numbers, wide, offsets, behind, tile_req, tile_start,
-                                                        tiles_n, nq, nkv, d, page, scale, n, pages, (const unsigned*)spans, units.const_data_ptr<float>(), stream()));
+                                                        tiles_n, nq, nkv, d, page, scale, n, pages, (const unsigned*)spans, value_spans, units.const_data_ptr<float>(), stream()));
         else
             done("lily_attention_prefill_mma_half", call(entry.prefill_mma_half, heads.const_data_ptr(), values.const_data_ptr(), out.data_ptr(), (const int*)numbers, wide, offsets, behind, tile_req,
-                                                         tile_start, tiles_n, nq, nkv, d, page, scale, (const unsigned*)spans, units.const_data_ptr<float>(), stream()));
+                                                         tile_start, tiles_n, nq, nkv, d, page, scale, (const unsigned*)spans, value_spans, units.const_data_ptr<float>(), stream()));
         return THPVariable_Wrap(std::move(out));
     });
 }
