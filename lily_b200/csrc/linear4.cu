@@ -255,11 +255,11 @@ __global__ void __launch_bounds__(32 * F32_WARPS, 2) product_f32_kernel(const Pr
 
 // The weights as numbers [n, k] (float32: exact; bfloat16: rounded once).  A warp eight rows of a tile, a lane sixteen bytes of codes, four words of eight.  In bfloat16 code - zero is exact and its product
 // with the scale one rounding, of two numbers an operation.  6,144 x 4,096 in bfloat16 10.6 us with the empty kernel behind it, 0.9 of what its bytes take (a word a thread 14.4, number by number besides 16.8).
-// grid (tiles of columns / 8, rows / 8)
+// grid (tiles of columns / 8, rows / 8 from row0 on)
 template <typename T>
-__global__ void __launch_bounds__(256) weights_kernel(const ProductArgs a, int group_shift) {
+__global__ void __launch_bounds__(256) weights_kernel(const ProductArgs a, int group_shift, int row0) {
     pdl_enter_small();
-    const int lane = threadIdx.x & 31, t = lane & 3, row = blockIdx.y * 8 + (lane >> 2), kt = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, t = lane & 3, row = row0 + blockIdx.y * 8 + (lane >> 2), kt = blockIdx.x * 8 + (threadIdx.x >> 5);
     if (kt >= a.tiles || row >= a.n) return;
     const uint4 codes = weights16(a.codes + (((size_t)(row / 128) * a.tiles + kt) * 128 + row % 128) * 64 + t * 16);
     const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
@@ -348,13 +348,14 @@ LILY_API int lily_weights4(const void* codes, const void* scales, const void* ze
     LILY_REQUIRE(weights_fit(n, k, group), "weights4: a matrix [%d, %d] in groups of %d", n, k, group);
     LILY_REQUIRE(((uintptr_t)out | (uintptr_t)codes) % 16 == 0, "weights4: tensors on boundaries of sixteen bytes");
     const four::ProductArgs a{nullptr, (const uint8_t*)codes, (const __nv_bfloat16*)scales, (const uint8_t*)zeros, nullptr, 0, out, 0, 0, n, k, (k + 127) / 128};
-    const int rows = (n + 7) / 8;
-    LILY_REQUIRE(rows <= 65535, "weights4: %d rows", n);
-    const dim3 grid((a.tiles + 7) / 8, rows);
     const int shift = group == 32 ? 5 : group == 64 ? 6 : 7;
-    if (dtype == kF32) launch_pdl(four::weights_kernel<float>, grid, dim3(256), 0, stream, a, shift);
-    else launch_pdl(four::weights_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, a, shift);
-    LILY_CHECK_LAUNCH("weights4");
+    constexpr int MOST = 65535 * 8;                                   // rows of a launch
+    for (int row0 = 0; row0 < n; row0 += min(MOST, n - row0)) {
+        const dim3 grid((a.tiles + 7) / 8, (min(MOST, n - row0) + 7) / 8);
+        if (dtype == kF32) launch_pdl(four::weights_kernel<float>, grid, dim3(256), 0, stream, a, shift, row0);
+        else launch_pdl(four::weights_kernel<__nv_bfloat16>, grid, dim3(256), 0, stream, a, shift, row0);
+        LILY_CHECK_LAUNCH("weights4");
+    }
     four::at_rest_kernel<<<1, 32, 0, stream>>>();
     LILY_CHECK_LAUNCH("weights4");
     return 0;
