@@ -310,6 +310,8 @@ static bool weights_fit(int n, int k, int group) { return n > 0 && k > 0 && (gro
 // Tokens that the kernels for few of them take.
 static int few_tokens(int dtype) { return dtype == kBF16 ? 16 : four::F32_TOKENS; }
 
+LILY_API int lily_linear4_few_tokens(int dtype) { return few_tokens(dtype); }
+
 LILY_API int lily_linear4(const void* x, int dtype, const void* codes, const void* scales, const void* zeros, const void* bias, int bias_f32, void* out, int out_f32, int m, int n, int k,
                           int group, cudaStream_t stream) {
     if (m == 0 || n == 0) return 0;

@@ -102,6 +102,7 @@ _SIGNATURES = {
     "lily_apply_penalties": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_top_logprobs": [_vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
     "lily_cache4_values": [_vp, _i, _vp, _i, _i, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _vp, _vp],
+    "lily_linear4_few_tokens": [_i],
     "lily_linear4_status": [_i],
     "lily_sample": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp],
 }
@@ -1424,13 +1425,20 @@ def linear4_lost() -> int:
     return int(library().lily_linear4_status(0))
 
 
+@functools.lru_cache(maxsize=None)
+def linear4_few_tokens(dtype: torch.dtype) -> int:
+    """Tokens that the kernels for few of them take: from one more on tcgen05 multiplies (bfloat16), or the matrix is brought to numbers."""
+    return int(library().lily_linear4_few_tokens(_BF16 if dtype == torch.bfloat16 else _F32))
+
+
 def linear4(x: torch.Tensor, w: Weight4, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``x [M, K] . W^T (+ bias)`` [M, N] for a matrix held in four bits, in the dtype of ``x`` (or float32: ``out_dtype``)."""
     if out_dtype not in (None, x.dtype, torch.float32):
         raise KernelError(f"linear4: the result is {x.dtype} or float32, not {out_dtype}")
-    if x.dim() == 2 and x.shape[0] > 8 and (x.dtype != torch.bfloat16 or not linear4_on_the_way(x.shape[0], w.n, w.k)):
+    few = linear4_few_tokens(x.dtype)
+    if x.dim() == 2 and x.shape[0] > few and (x.dtype != torch.bfloat16 or not linear4_on_the_way(x.shape[0], w.n, w.k)):
         return linear(x, weights4(w, x.dtype), bias, out_dtype)
-    out = (_module or _faces()).linear4(x, *w, bias, out_dtype == torch.float32, 17, *(() if LINEAR4_POLLS is None else (LINEAR4_POLLS,)))
+    out = (_module or _faces()).linear4(x, *w, bias, out_dtype == torch.float32, few + 1, *(() if LINEAR4_POLLS is None else (LINEAR4_POLLS,)))
     launches["count"] += 1
     return out
 
