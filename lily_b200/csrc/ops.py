@@ -590,9 +590,12 @@ def linear_split(x: torch.Tensor, weight: torch.Tensor, splits: Optional[int] = 
 
 def linear_auto(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The product in whichever form is fastest for the shape: float32 partial sums from
-    ``linear_split`` for a few tokens, else ``linear``'s [M, N].  For producers whose consumer is
+    ``linear_split`` for a few tokens (a ``Weight4``: the sum alone, float32 [1, M, N]), else ``linear``'s [M, N].  For producers whose consumer is
     one of the kernels that take either form."""
-    if bias is None and not isinstance(weight, Weight4):
+    if bias is None and isinstance(weight, Weight4):
+        if x.dtype == torch.bfloat16 and x.shape[0] <= linear4_few_tokens(x.dtype):
+            return linear4(x, weight, out_dtype=torch.float32).unsqueeze(0)
+    elif bias is None:
         parts = linear_split(x, weight)
         if parts is not None:
             return parts
