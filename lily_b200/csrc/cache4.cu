@@ -89,7 +89,7 @@ __device__ __forceinline__ uint32_t codes_of(const float (&y)[8], float lowest, 
 }
 
 // A thread eight features, d / 8 threads a head, 32 / (d / 8) heads a warp.  grid (blocks of a token's heads, tokens)
-template <typename T, typename W, bool WHOLE_PIECES>
+template <typename T, typename W, typename Q, bool WHOLE_PIECES>
 __global__ void __launch_bounds__(32 * WRITE_WARPS) write_kernel(const WriteArgs a) {
     __shared__ __align__(16) float turn_s[WRITE_WARPS][256];
     pdl_enter_small();
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) write_kernel(const WriteArgs
             }
         }
     }
-    if (kind == 0 && in) store8((T*)a.q_out + ((size_t)n * a.nq + head) * a.d + f, y);
+    if (kind == 0 && in) store8((Q*)a.q_out + ((size_t)n * a.nq + head) * a.d + f, y);
     if (__all_sync(0xffffffffu, kind == 0)) return;
     // eight neighbouring lanes hold a group of 64 features
     float most_v = y[0], least = y[0];
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) write_kernel(const WriteArgs
 // The same where all features are turned and heads are 64, 128 or 256 features: a thread a word and its partners', d / 16 threads a head, which so needs no exchange but for sums and extremes, and half as
 // much work that is not its numbers'.  1,500 tokens of 32 heads over 8 of 128, with the pages as numbers behind: 16.8 us, 23.6 by the kernel above (8 tokens 5.5 and 5.8); what bounds it is instructions,
 // 0.58 a cycle and scheduler, over blocks of one token.  grid (blocks of a token's heads, tokens)
-template <typename T, typename W, int D>
+template <typename T, typename W, typename Q, int D>
 __global__ void __launch_bounds__(32 * WRITE_WARPS) write_turned_kernel(const WriteArgs a, const int page_shift) {
     constexpr int THREADS = D / 16, HALF = D / 2, G = D / GROUP;
     pdl_enter_small();
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) write_turned_kernel(const Wr
         }
     }
     if (kind == 0 && in) {
-        T* to = (T*)a.q_out + ((size_t)n * a.nq + head) * D + t * 8;
+        Q* to = (Q*)a.q_out + ((size_t)n * a.nq + head) * D + t * 8;
         store8(to, x);
         store8(to + HALF, y);
     }
@@ -402,6 +402,8 @@ __global__ void __launch_bounds__(256) zero_kernel(unsigned* __restrict__ words,
     if (i < 2 * tiles.n) tiles_out[i] = tiles.of[i];
 }
 
+constexpr int F32_TO_BF16 = 2;               // a dtype of heads: float32 ones, whose queries leave as bfloat16
+
 inline bool head_fits(int d) { return d >= GROUP && d <= 256 && d % GROUP == 0; }
 
 }  // namespace four
@@ -418,8 +420,8 @@ LILY_API int lily_qk_norm_rope_write4(const void* qkv, int dtype, int ld, const 
     LILY_REQUIRE(page_size > 0 && tokens > 0 && tokens <= 65535 * 32, "qk_norm_rope_write4: %d tokens, pages of %d places", tokens, page_size);
     LILY_REQUIRE(nq >= 0 && nkv >= 0 && nq + nkv > 0 && ld >= (nq + 2 * nkv) * d, "qk_norm_rope_write4: rows of %d numbers", ld);
     LILY_REQUIRE((q_gain == nullptr) == (k_gain == nullptr), "qk_norm_rope_write4: q and k gains come together");
-    LILY_REQUIRE(dtype == kF32 || (dtype == kBF16), "qk_norm_rope_write4: dtype %d", dtype);
-    LILY_REQUIRE(dtype == kBF16 || gain_dtype == kF32 || !q_gain, "qk_norm_rope_write4: float32 heads keep float32 gains");
+    LILY_REQUIRE(dtype == kF32 || dtype == kBF16 || dtype == four::F32_TO_BF16, "qk_norm_rope_write4: dtype %d", dtype);
+    LILY_REQUIRE(dtype != kF32 || gain_dtype == kF32 || !q_gain, "qk_norm_rope_write4: float32 heads keep float32 gains");
     const uintptr_t where = (uintptr_t)qkv | (uintptr_t)kv | (uintptr_t)q_out | (uintptr_t)q_gain | (uintptr_t)k_gain | (uintptr_t)cos_t | (uintptr_t)sin_t;
     LILY_REQUIRE(where % 16 == 0 && ld % 8 == 0, "qk_norm_rope_write4: tensors on boundaries of sixteen bytes");
     const int per_block = four::WRITE_WARPS * (32 / (d / 8));
@@ -428,22 +430,24 @@ LILY_API int lily_qk_norm_rope_write4(const void* qkv, int dtype, int ld, const 
     while (1 << shift < page_size) ++shift;
     if (1 << shift != page_size) shift = -1;
     for (int t0 = 0; t0 < tokens; t0 += 65535) {
-        const int n = min(65535, tokens - t0), item = dtype == kBF16 ? 2 : 4;
+        const int n = min(65535, tokens - t0), item = dtype == kBF16 ? 2 : 4, q_item = dtype == kF32 ? 4 : 2;
         const four::WriteArgs a{(const char*)qkv + (size_t)t0 * ld * item, ld, q_gain, k_gain, eps, 1.0 / d, cos_t, sin_t, table_rows, positions + t0, token_req + t0, block_table, requests, bt_stride,
-                                (uint8_t*)kv, pages, (char*)q_out + (size_t)t0 * nq * d * item, nq, nkv, d, rd, page_size, n};
+                                (uint8_t*)kv, pages, (char*)q_out + (size_t)t0 * nq * d * q_item, nq, nkv, d, rd, page_size, n};
         const dim3 grid((nq + 2 * nkv + per_block - 1) / per_block, n), turned((nq + 2 * nkv + 2 * per_block - 1) / (2 * per_block), n);
-#define TURNED(T, W, D) launch_pdl(four::write_turned_kernel<T, W, D>, turned, dim3(32 * four::WRITE_WARPS), 0, stream, a, shift)
-#define LAUNCH(T, W)                                                                                                              \
+#define TURNED(T, W, Q, D) launch_pdl(four::write_turned_kernel<T, W, Q, D>, turned, dim3(32 * four::WRITE_WARPS), 0, stream, a, shift)
+#define LAUNCH(T, W, Q)                                                                                                           \
     do {                                                                                                                          \
-        if (rd == d && d == 64) TURNED(T, W, 64);                                                                                  \
-        else if (rd == d && d == 128) TURNED(T, W, 128);                                                                           \
-        else if (rd == d && d == 256) TURNED(T, W, 256);                                                                           \
-        else if (pieces) launch_pdl(four::write_kernel<T, W, true>, grid, dim3(32 * four::WRITE_WARPS), 0, stream, a);                  \
-        else launch_pdl(four::write_kernel<T, W, false>, grid, dim3(32 * four::WRITE_WARPS), 0, stream, a);                        \
+        if (rd == d && d == 64) TURNED(T, W, Q, 64);                                                                                  \
+        else if (rd == d && d == 128) TURNED(T, W, Q, 128);                                                                           \
+        else if (rd == d && d == 256) TURNED(T, W, Q, 256);                                                                           \
+        else if (pieces) launch_pdl(four::write_kernel<T, W, Q, true>, grid, dim3(32 * four::WRITE_WARPS), 0, stream, a);                  \
+        else launch_pdl(four::write_kernel<T, W, Q, false>, grid, dim3(32 * four::WRITE_WARPS), 0, stream, a);                        \
     } while (0)
-        if (dtype == kF32) LAUNCH(float, float);
-        else if (gain_dtype == kBF16) LAUNCH(__nv_bfloat16, __nv_bfloat16);
-        else LAUNCH(__nv_bfloat16, float);
+        if (dtype == kF32) LAUNCH(float, float, float);
+        else if (dtype == four::F32_TO_BF16 && gain_dtype == kBF16) LAUNCH(float, __nv_bfloat16, __nv_bfloat16);
+        else if (dtype == four::F32_TO_BF16) LAUNCH(float, float, __nv_bfloat16);
+        else if (gain_dtype == kBF16) LAUNCH(__nv_bfloat16, __nv_bfloat16, __nv_bfloat16);
+        else LAUNCH(__nv_bfloat16, float, __nv_bfloat16);
 #undef LAUNCH
 #undef TURNED
         LILY_CHECK_LAUNCH("qk_norm_rope_write4");

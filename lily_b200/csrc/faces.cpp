@@ -483,12 +483,13 @@ PyObject* qk_norm_rope_write4(PyObject*, PyObject* const* p, Py_ssize_t count) {
                 refuse(what, ": q and k gains come together, with one dtype and head_dim numbers each");
             gain = code_of(*q_gain);
         }
-        if (given && (given->scalar_type() != qkv.scalar_type() || given->numel() != n * nq * d)) refuse(what, ": q_out is [tokens, nq * d] in the dtype of qkv");
+        const bool rounded = given && code == F32 && is(*given, at::kBFloat16);
+        if (given && ((given->scalar_type() != qkv.scalar_type() && !rounded) || given->numel() != n * nq * d)) refuse(what, ": q_out is [tokens, nq * d] in the dtype of qkv, or bfloat16");
         const int *at = ints(positions, "positions"), *of = ints(req, "token_req"), *bt = ints(table, "block_table");
         here({&qkv, q_gain, k_gain, cos, sin, &positions, &req, &table, &kv, given});
         Tensor q = given ? *given : at::empty({n, (int64_t)nq * d}, qkv.options());
         done("lily_qk_norm_rope_write4",
-             call(entry.write4, qkv.const_data_ptr(), code, narrow(ld), q_gain ? q_gain->const_data_ptr() : nullptr, k_gain ? k_gain->const_data_ptr() : nullptr, gain, eps,
+             call(entry.write4, qkv.const_data_ptr(), rounded ? 2 : code, narrow(ld), q_gain ? q_gain->const_data_ptr() : nullptr, k_gain ? k_gain->const_data_ptr() : nullptr, gain, eps,
                   rd ? cos->const_data_ptr<float>() : nullptr, rd ? sin->const_data_ptr<float>() : nullptr, rd ? narrow(cos->size(0)) : 0, at, narrow(n), of, bt, narrow(table.size(0)),
                   narrow(table.size(1)), kv.data_ptr(), narrow(kv.size(0)), q.data_ptr(), nq, nkv, d, rd, page, stream()));
         return THPVariable_Wrap(std::move(q));

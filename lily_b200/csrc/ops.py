@@ -602,6 +602,12 @@ def linear_auto(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     return linear(x, weight, bias)
 
 
+def linear_unrounded(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``linear`` whose float32 sums are kept where a kernel for a few tokens forms them."""
+    few = x.dtype == torch.bfloat16 and (x.shape[0] <= linear4_few_tokens(x.dtype) if isinstance(weight, Weight4) else few_rows_take(x, weight))
+    return linear(x, weight, bias, torch.float32 if few else None)
+
+
 def swiglu_skinny_need(tokens: int, intermediate: int, hidden: int, dtype: torch.dtype,
                        block: Optional[int] = None, whenever_possible: bool = False) -> Optional[Tuple[int, int]]:
     """None where ``swiglu_skinny`` does not take the shape (more than 8 tokens, not bfloat16, K not a multiple of 64): the caller
@@ -1462,7 +1468,7 @@ def qk_norm_rope_write4(qkv: torch.Tensor, q_gain: Optional[torch.Tensor], k_gai
                         page_size: int, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``qk_norm_rope_write`` into a cache held in four bits (``kv_layer`` uint8 [pages, *cache4_shape]): per-head RMSNorm of q and k (when gains are given), rotation by the tables, q to ``q_out``
     [tokens, nq * d], k and v, 64 features at a time, as codes round((x - lowest) / step) with step = (max - min) / 15.  A token's codes depend on its own numbers alone, to the bit.
-    A group that holds what is not finite reads as NaN.  ``qkv`` [tokens, (nq + 2 nkv) d] float32 or bfloat16.  A position outside the tables gives NaN; what has a position or a request outside
+    A group that holds what is not finite reads as NaN.  ``qkv`` [tokens, (nq + 2 nkv) d] float32 or bfloat16; queries leave in its dtype, or, of float32 heads, in a ``q_out`` of bfloat16.  A position outside the tables gives NaN; what has a position or a request outside
     the block table is not written; no two tokens of a call have one place."""
     q = (_module or _faces()).qk_norm_rope_write4(qkv, q_gain, k_gain, eps, cos, sin, positions, token_req, block_table, kv_layer, nq, nkv, d, rotary_dim, page_size, q_out)
     launches["count"] += 1

@@ -311,8 +311,9 @@ class Attention(Mixer):
             return FourBitPlan(floats, portions)
         plan = batch.plan(("attention4", cache.group, s.num_heads, s.num_kv_heads, s.head_dim, x.dtype, page), make)
         cos, sin = self.position.tables() if self.position is not None else (None, None)
-        q = ops.qk_norm_rope_write4(ops.linear(x, self.w_qkv, self.b_qkv), self.q_gain, self.k_gain, s.norm_eps, cos, sin, batch.positions, batch.token_req, table, cache.data,
-                                    s.num_heads, s.num_kv_heads, s.head_dim, self.position.rotary_dim if self.position is not None else 0, page)
+        q = torch.empty((x.shape[0], s.num_heads * s.head_dim), dtype=x.dtype, device=x.device)
+        ops.qk_norm_rope_write4(ops.linear_unrounded(x, self.w_qkv, self.b_qkv), self.q_gain, self.k_gain, s.norm_eps, cos, sin, batch.positions, batch.token_req, table, cache.data,
+                                    s.num_heads, s.num_kv_heads, s.head_dim, self.position.rotary_dim if self.position is not None else 0, page, q)
         out = torch.empty_like(q)
         if nd:
             ops.attention_decode4(q[:nd], cache.data, table[:nd], batch.seq_lens[:nd], batch.max_decode_len, s.num_heads, s.num_kv_heads, s.head_dim, page, self.scale,

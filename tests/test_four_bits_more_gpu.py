@@ -61,3 +61,44 @@ def test_a_few_tokens_gate_is_rounded_once(m, group):
     out = part.forward(x, None)
     assert out.dtype == F32
     within(out.sum(0) if out.dim() == 3 else out, act.double() @ down.t(), 2.0 ** -18 * (act.double().abs() @ down.abs().t()))
+
+
+@pytest.mark.parametrize("gain_dtype", [BF16, F32])
+@pytest.mark.parametrize("nq,nkv,d,rot,page", [(4, 2, 128, 128, 16), (6, 2, 64, 64, 64), (2, 1, 192, 96, 16), (4, 1, 256, 256, 32), (5, 1, 128, 36, 1), (2, 2, 128, 0, 64)])
+@pytest.mark.parametrize("norm", [True, False])
+def test_write_of_float32_heads_with_bfloat16_queries(gain_dtype, nq, nkv, d, rot, page, norm):
+    """Codes to the bit those of the plain statement on the float32 heads, queries with one rounding."""
+    from test_four_bits_gpu import run_write, same_bytes, write_case, written
+    c = write_case(F32, nq, nkv, d, rot, page, [3, 1, 20], [5, 70, 0], norm, gain_dtype, nq * d)
+    want_q, want_kv = written(c, nq, nkv, d, rot, page, 1e-6)
+    given = torch.empty(24, nq * d, dtype=BF16, device=DEV)
+    q, kv = run_write(c, nq, nkv, d, rot, page, 1e-6, q_out=given)
+    assert q.dtype == BF16 and torch.equal(q, want_q.to(BF16)) and torch.equal(given.cpu(), q)
+    assert same_bytes(kv, want_kv, page, d)
+
+
+def test_queries_of_another_type_are_refused():
+    from test_four_bits_gpu import run_write, write_case
+    c = write_case(BF16, 2, 1, 64, 64, 16, [3], [0], False, BF16, 1)
+    with pytest.raises(ops().KernelError, match="q_out"):
+        run_write(c, 2, 1, 64, 64, 16, 1e-6, q_out=torch.empty(3, 128, dtype=F32, device=DEV))
+    c = write_case(F32, 2, 1, 64, 64, 16, [3], [0], False, F32, 1)
+    with pytest.raises(ops().KernelError, match="q_out"):
+        run_write(c, 2, 1, 64, 64, 16, 1e-6, q_out=torch.empty(3, 128, dtype=torch.float16, device=DEV))
+
+
+@pytest.mark.parametrize("m", [1, 8, 16, 17])
+@pytest.mark.parametrize("quantised", [True, False])
+def test_heads_of_a_few_tokens_are_not_rounded_ahead_of_their_norm(m, quantised):
+    """What goes into the norm and the cache: float32 sums, within 2^-18 of the magnitudes, of up to 16 tokens; bfloat16 behind that, as ever."""
+    o, g, n, k = ops(), torch.Generator().manual_seed(m), 384, 256
+    w = (torch.randn(n, k, generator=g) / 16).to(BF16).to(DEV)
+    held = o.quantize_weight4(w, 128) if quantised else w
+    full = o.weights4(held, F32).double() if quantised else w.double()
+    x, bias = torch.randn(m, k, generator=g).to(BF16).to(DEV), torch.randn(n, generator=g).to(BF16).to(DEV)
+    for b in (None, bias):
+        got = o.linear_unrounded(x, held, b)
+        assert got.dtype == (F32 if m <= 16 else BF16)
+        if m <= 16:
+            want = x.double() @ full.t() + (0 if b is None else b.double())
+            within(got, want, 2.0 ** -18 * (x.double().abs() @ full.abs().t()) + 2.0 ** -23 * want.abs())
