@@ -212,6 +212,8 @@ class ModelRunner:
         self.model = AssembledModel(spec, ctx)
         if ctx.cache4 and not all(need.four_bits for need, _ in self.model.cache_groups):
             raise ValueError(f"kv_cache_dtype = int4: {spec.architecture} caches what four bits do not hold")
+        if ctx.weight_group and not self.model.four_bits:
+            raise ValueError(f"quantization = {args.quantization}: {spec.architecture} has neither the attention nor the gated feed-forwards whose matrices are held in four bits")
         moved = load_model_weights(self.model, source, self.dtype, self.device)
         self.weight_bytes = moved
         logger.info("loaded %s in %.1f s (%.2f GB on the device)", spec.architecture, time.time() - t0, moved / 1e9)

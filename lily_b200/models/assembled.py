@@ -147,25 +147,31 @@ class AssembledModel:
         self.step_vectors = {name: get(name).float().contiguous() for name in self.step_rows}      # added in float32
         self.head = self.embed if self.spec.head_name is None else get(self.spec.head_name).contiguous()
 
-    def weight_bytes(self) -> int:
-        seen, total = set(), 0
+    def _all_parts(self):
+        for b in self.blocks:
+            for part in b.parts:
+                yield part
+                if isinstance(part, FeedForward):
+                    yield from getattr(part, "parts", ())            # a feed-forward put together from others
+        yield self.final_norm
+        if self.embed_norm is not None:
+            yield self.embed_norm
 
-        def visit(obj):
-            nonlocal total
+    @property
+    def four_bits(self) -> bool:
+        """Whether any part holds its matrices in four bits."""
+        return any(getattr(part, "four_bits", False) for part in self._all_parts())
+
+    def weight_bytes(self, four_bits: bool = False) -> int:
+        """Bytes of the weights as they are held; ``four_bits``: of the matrices alone that are held in four bits."""
+        seen, total = set(), 0
+        for obj in (self, *self._all_parts()):
             for v in vars(obj).values():
-                for t in v if isinstance(v, tuple) else (v,):              # (a matrix held in four bits is a tuple of its tensors and sizes)
+                # (a matrix held in four bits is a tuple of its tensors and sizes)
+                for t in v if isinstance(v, tuple) else () if four_bits else (v,):
                     if isinstance(t, torch.Tensor) and t.data_ptr() not in seen and not getattr(t, "_is_table", False):
                         seen.add(t.data_ptr())
                         total += t.numel() * t.element_size()
-            for inner in getattr(obj, "parts", ()) if isinstance(obj, FeedForward) else ():
-                visit(inner)                              # a feed-forward put together from others
-        visit(self)
-        for b in self.blocks:
-            for part in b.parts:
-                visit(part)
-        visit(self.final_norm)
-        if self.embed_norm is not None:
-            visit(self.embed_norm)
         return total
 
     # ---- one step ------------------------------------------------------------------

@@ -147,6 +147,7 @@ class Attention(Mixer):
             raise ValueError("a cache held in four bits serves attention over all keys of 64, 128, 192 or 256 features, without cap, sink, convolution or shared, mixed or normed values")
         if ctx.weight_group and (spec.hidden_size % ctx.weight_group or spec.num_heads * spec.value_dim % ctx.weight_group):
             raise ValueError(f"matrices of {spec.hidden_size} and {spec.num_heads * spec.value_dim} columns do not come in groups of {ctx.weight_group}")
+        self.four_bits = bool(ctx.weight_group)
         self.conv_w = None
 
     @property

@@ -108,6 +108,7 @@ class BuildContext:
 
 class Part:
     kind: str = ""
+    four_bits: bool = False            # its matrices are held in four bits (``BuildContext.weight_group``)
 
     def tensors(self) -> Dict[str, TensorSpec]:
         return {}

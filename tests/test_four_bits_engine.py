@@ -3,6 +3,7 @@
 import pytest
 
 import kernel_refs
+import nafazen_models
 import tiny_models
 from harness import make_runner, model_dir
 from lily_b200.engine.scheduler import Scheduler
@@ -41,3 +42,12 @@ def test_every_runner_hears_of_a_4_bit_product_that_gave_up(model, monkeypatch):
             r.check_waits()
         r.check_waits()
     make_runner(path).check_waits()
+
+
+@pytest.mark.parametrize("cfg", [nafazen_models.SHARP, dict(nafazen_models.WIDE, layers=[dict(layer, mlp=nafazen_models.moe(ff=64, experts=8, top=4, shared=None)) for layer in nafazen_models.WIDE["layers"]])])
+def test_architectures_without_such_matrices_are_refused(cfg, tmp_path):
+    """Four bits hold the matrices of attention and gated feed-forwards: a model that has neither would be served in its dtype without a word."""
+    path = nafazen_models.write_model_dir(str(tmp_path / "m"), cfg, nafazen_models.make_weights(cfg, 3))
+    make_runner(path)
+    with pytest.raises(ValueError, match="quantization = int4: .* held in four bits"):
+        make_runner(path, quantization="int4", quantization_group=32)
