@@ -215,8 +215,13 @@ class ModelRunner:
         if ctx.weight_group and not self.model.four_bits:
             raise ValueError(f"quantization = {args.quantization}: {spec.architecture} has neither the attention nor the gated feed-forwards whose matrices are held in four bits")
         moved = load_model_weights(self.model, source, self.dtype, self.device)
-        self.weight_bytes = moved
-        logger.info("loaded %s in %.1f s (%.2f GB on the device)", spec.architecture, time.time() - t0, moved / 1e9)
+        # bytes on the device: what was moved, or, where matrices became four bits on the way, what they are held in
+        self.weight_bytes = self.model.weight_bytes() if ctx.weight_group else moved
+        logger.info("loaded %s in %.1f s (%.2f GB on the device)", spec.architecture, time.time() - t0, self.weight_bytes / 1e9)
+        if ctx.weight_group:
+            held = self.model.weight_bytes(four_bits=True)
+            logger.info("quantization = %s: %.2f GB of them are matrices of attention and gated feed-forwards in four bits, %.2f GB (embedding, head and what else there is) stay as they were",
+                        args.quantization, held / 1e9, (self.weight_bytes - held) / 1e9)
 
         groups = self.model.cache_groups
         if args.max_total_tokens is not None:

@@ -1,5 +1,7 @@
 """The engine around matrices and caches in four bits, what can be looked at without a GPU."""
 
+import logging
+
 import pytest
 
 import kernel_refs
@@ -51,3 +53,22 @@ def test_architectures_without_such_matrices_are_refused(cfg, tmp_path):
     make_runner(path)
     with pytest.raises(ValueError, match="quantization = int4: .* held in four bits"):
         make_runner(path, quantization="int4", quantization_group=32)
+
+
+def test_the_load_report_is_what_the_device_holds(tmp_path, monkeypatch, caplog):
+    """Bytes of a quantised model are those it is held in, not those of the checkpoint, and the log says how many of them are in four bits."""
+    from lily_b200.csrc import ops
+    monkeypatch.setattr(kernel_refs, "quantize_weight4", ops.quantize_weight4, raising=False)
+    cfg = dict(tiny_models.TINY_QWEN3, hidden_size=128, head_dim=64, intermediate_size=256)
+    path, weights = model_dir(cfg, 3, str(tmp_path))
+    full = make_runner(path)
+    caplog.set_level(logging.INFO)
+    four = make_runner(path, quantization="int4", quantization_group=64)
+    names = [n for n in weights if any(f"{x}_proj.weight" in n for x in ("q", "k", "v", "o", "gate", "up", "down"))]
+    numbers = sum(weights[n].numel() for n in names)
+    held = four.model.weight_bytes(four_bits=True)
+    # codes in whole tiles of 128 rows and columns, a bfloat16 scale a group: these matrices' sizes are whole tiles once q, k and v, and gate and up, are stacked
+    assert held == numbers // 2 + numbers // 64 * 2
+    assert full.weight_bytes == sum(w.numel() * 4 for w in weights.values()) and four.weight_bytes == full.weight_bytes - numbers * 4 + held
+    said = [r.getMessage() for r in caplog.records if "four bits" in r.getMessage()]
+    assert len(said) == 1 and f"{held / 1e9:.2f} GB" in said[0]
