@@ -69,6 +69,8 @@ class AssembledModel:
                     other = owners[k].cache_need()
                     if (other.kv_heads, other.head_dim, other.v_head_dim, other.four_bits) != (need.kv_heads, need.head_dim, need.v_head_dim, need.four_bits):
                         raise ValueError(f"schedule position {pos} cannot read a cache of another shape")
+                    if need.four_bits:
+                        raise ValueError(f"schedule position {pos} reads the cache of position {entry.reads}: a cache held in four bits is read by the run that writes it")
                     caches.append((lent[0], lent[1], False))
                 else:
                     need = dataclasses.replace(need, window=kept[pos, k][0], keep_first=kept[pos, k][1])

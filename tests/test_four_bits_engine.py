@@ -3,12 +3,18 @@
 import logging
 
 import pytest
+import torch
 
 import kernel_refs
 import nafazen_models
 import tiny_models
 from harness import make_runner, model_dir
 from lily_b200.engine.scheduler import Scheduler
+from lily_b200.models.assembled import AssembledModel
+from lily_b200.parts.attention import AttentionSpec
+from lily_b200.parts.base import BlockSpec, BuildContext, ModelSpec, ScheduleEntry
+from lily_b200.parts.mlp import SwiGLUSpec
+from lily_b200.parts.norm import RMSNormSpec
 from lily_b200.sampling.params import SamplingParams
 
 
@@ -72,3 +78,14 @@ def test_the_load_report_is_what_the_device_holds(tmp_path, monkeypatch, caplog)
     assert full.weight_bytes == sum(w.numel() * 4 for w in weights.values()) and four.weight_bytes == full.weight_bytes - numbers * 4 + held
     said = [r.getMessage() for r in caplog.records if "four bits" in r.getMessage()]
     assert len(said) == 1 and f"{held / 1e9:.2f} GB" in said[0]
+
+
+def test_runs_that_read_another_runs_4_bit_cache_are_refused():
+    """When the model is put together, and not by its first step."""
+    block = BlockSpec(prefix="l", mixer=AttentionSpec(64, 2, 1, 64), feed_forward=SwiGLUSpec(64, 128), norm_in=RMSNormSpec(64, 1e-6), norm_post=RMSNormSpec(64, 1e-6))
+    build = lambda schedule, cache4: AssembledModel(ModelSpec(architecture="toy", vocab_size=32, hidden_size=64, blocks=[block], schedule=schedule, final_norm=RMSNormSpec(64, 1e-6), head_name=None,
+                                                              max_position=64, eos_token_ids=[]), BuildContext(torch.device("cpu"), torch.float32, kernel_refs, cache4=cache4))
+    lent = [ScheduleEntry(0), ScheduleEntry(0, reads=0)]
+    build(lent, False), build([ScheduleEntry(0), ScheduleEntry(0)], True)
+    with pytest.raises(ValueError, match="read by the run that writes it"):
+        build(lent, True)
