@@ -10,6 +10,7 @@
 // behind the products (keys) or the weights ahead of them (values).
 #include "four.cuh"
 #include "mma.cuh"
+#include <algorithm>
 #include <cuda_fp16.h>
 #include <type_traits>
 
@@ -696,6 +697,18 @@ inline bool on_tensor_cores(int page_size, int dtype) { return dtype == kBF16 &&
 
 // Query heads of a pair on the CUDA cores.
 inline int cores_heads(int group) { return group <= 4 ? 4 : 8; }
+// Blocks of the kernel on the CUDA cores that a multiprocessor holds: three by their registers, and by shared memory (228 KB, of which a block takes 1 KB of its own) two where eight heads of 256 features are
+// a pair.  With a third more than it holds, shares that are cut evenly would run in two rounds: 8 float32 rows of 2,000 places, 16 query heads of
+// 256 over 2, 29.6 us, 40.3 with three.
+template <int D> constexpr int cores_a_sm(bool eight) {
+    const int room = 228 * 1024, fixed = 1024 + 512;
+    return std::min(3, room / ((int)(eight ? CoresTile<D, 8>::ALL : CoresTile<D, 4>::ALL) + fixed));
+}
+static_assert(cores_a_sm<256>(true) == 2 && cores_a_sm<256>(false) == 3 && cores_a_sm<192>(true) == 3, "");
+inline int cores_blocks(int d, int heads) {
+    const bool eight = heads == 8;
+    return d == 64 ? cores_a_sm<64>(eight) : d == 128 ? cores_a_sm<128>(eight) : d == 192 ? cores_a_sm<192>(eight) : cores_a_sm<256>(eight);
+}
 // Blocks: as many as are on the device at once, where there is work for them.
 struct Plan { bool tensor_cores; int heads, warps, blocks; };
 inline Plan plan_of(int requests, int nq, int nkv, int d, int longest, int page_size, int dtype) {
@@ -707,7 +720,7 @@ inline Plan plan_of(int requests, int nq, int nkv, int d, int longest, int page_
     // Two tiles a block at least, of four warps, but no two pairs in a block while there are blocks: a pair's end is some 2 us that the next one waits for.  Against a tile a warp: 8 rows of one place
     // 4.6 us for 10.6 (float32 6.9 for 21.1), of 130 8.1 and 8.2, two of 300 6.0 and 7.9, float32 3 rows of 150 to 2,900 10.2 and 15.5 (of 2,000 18.6 and 17.4); a tile a block: 8 rows of 60 6.1 for 4.9.
     const long long wanted = p.warps == 1 ? tiles : max(pairs, (tiles + 1) / 2);
-    p.blocks = (int)max(1ll, min((long long)(p.tensor_cores ? blocks_a_sm(d, p.warps) : 3) * sm_count(), wanted));
+    p.blocks = (int)max(1ll, min((long long)(p.tensor_cores ? blocks_a_sm(d, p.warps) : cores_blocks(d, p.heads)) * sm_count(), wanted));
     return p;
 }
 

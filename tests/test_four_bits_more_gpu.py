@@ -102,3 +102,13 @@ def test_heads_of_a_few_tokens_are_not_rounded_ahead_of_their_norm(m, quantised)
         if m <= 16:
             want = x.double() @ full.t() + (0 if b is None else b.double())
             within(got, want, 2.0 ** -18 * (x.double().abs() @ full.abs().t()) + 2.0 ** -23 * want.abs())
+
+
+# ---- how decode rows are cut ----
+
+@pytest.mark.parametrize("dtype,page", [(F32, 64), (BF16, 8)])
+@pytest.mark.parametrize("nq,d,most", [(8, 256, 2), (4, 256, 3), (8, 192, 3), (8, 128, 3)])
+def test_blocks_on_cuda_cores_are_no_more_than_the_device_holds(dtype, page, nq, d, most):
+    """What a block has in shared memory (86,528 bytes where eight heads of 256 features are a pair, so that a multiprocessor's 233,472 hold two), looked at by the scratch that blocks leave parts in."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert ops().decode4_scratch_floats(4, nq, 1, d, 200_000, page, dtype) == 2 * most * sms * 8 * (d + 2)
