@@ -719,6 +719,8 @@ inline Plan plan_of(int requests, int nq, int nkv, int d, int longest, int page_
     p.warps = p.tensor_cores && d <= 128 && pairs >= 3ll * sm_count() ? 1 : WARPS;      // (at blocks_a_sm)
     // Two tiles a block at least, of four warps, but no two pairs in a block while there are blocks: a pair's end is some 2 us that the next one waits for.  Against a tile a warp: 8 rows of one place
     // 4.6 us for 10.6 (float32 6.9 for 21.1), of 130 8.1 and 8.2, two of 300 6.0 and 7.9, float32 3 rows of 150 to 2,900 10.2 and 15.5 (of 2,000 18.6 and 17.4); a tile a block: 8 rows of 60 6.1 for 4.9.
+    // (The lengths that count are the longest there may be.  A captured step is made for rows of thousands of places, so short rows there are cut a tile a block: 8 rows of 60 places 7.0 us, where a call that
+    // says 60 takes 4.8; of 1, 130 and 400 places 5.1, 8.8 and 9.5 us, within 0.3 of theirs.  Blocks counted on the device from the rows at hand took 5.8 for the first, and 0.1 to 0.6 us more of all others.)
     const long long wanted = p.warps == 1 ? tiles : max(pairs, (tiles + 1) / 2);
     p.blocks = (int)max(1ll, min((long long)(p.tensor_cores ? blocks_a_sm(d, p.warps) : cores_blocks(d, p.heads)) * sm_count(), wanted));
     return p;

@@ -112,3 +112,19 @@ def test_blocks_on_cuda_cores_are_no_more_than_the_device_holds(dtype, page, nq,
     """What a block has in shared memory (86,528 bytes where eight heads of 256 features are a pair, so that a multiprocessor's 233,472 hold two), looked at by the scratch that blocks leave parts in."""
     sms = torch.cuda.get_device_properties(0).multi_processor_count
     assert ops().decode4_scratch_floats(4, nq, 1, d, 200_000, page, dtype) == 2 * most * sms * 8 * (d + 2)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("nq,nkv,d,page", [(16, 4, 128, 64), (8, 2, 64, 16), (8, 1, 256, 64), (6, 2, 128, 8)])
+@pytest.mark.parametrize("lengths", [[1] * 8, [60] * 8, [0, 64, 0, 17], [5], [64, 3, 32], [40] * 70, [1000, 3, 90]])
+def test_the_longest_row_that_may_come(dtype, nq, nkv, d, page, lengths):
+    """A captured step is made for rows of thousands of places, and gives rows of any length as near as a call that is made for them."""
+    q, kv, table, seq = decode_case(lengths, nq, nkv, d, page, dtype)
+    run = lambda table, longest: ops().attention_decode4(q, kv, table, seq, longest, nq, nkv, d, page, d ** -0.5)
+    want, by_codes, by_values = fb.attention(q, kv, table, [(1 if n else 0, n - 1 if n else 0) for n in lengths], nq, nkv, d, page, d ** -0.5)
+    within(run(table, max(lengths)), want, attention_bound(by_codes, by_values, want, dtype))
+    for longest in (8192, 131072):
+        wide = torch.zeros(len(lengths), longest // page, dtype=torch.int32, device=DEV)
+        wide[:, :table.shape[1]] = table
+        got = run(wide, longest)
+        within(got, want, attention_bound(by_codes, by_values, want, dtype))
