@@ -298,40 +298,42 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
             uint4 v[G][2];
             float most_q = 0.f, sums[G];
 #pragma unroll
-            for (int j = 0; j < G; ++j) {
-                sums[j] = 0.f;
+            for (int j = 0; j < G; ++j)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     uint4& x = v[j][h];
                     x = make_uint4(0, 0, 0, 0);
                     if (g < heads) x = *reinterpret_cast<const uint4*>((const __nv_bfloat16*)a.q + ((size_t)req * a.nq + head0 + g) * D + 64 * j + 32 * h + 8 * t);
                     if (a.scale < 0.f) x.x ^= 0x80008000u, x.y ^= 0x80008000u, x.z ^= 0x80008000u, x.w ^= 0x80008000u;
-                    for (const uint32_t w : {x.x, x.y, x.z, x.w}) sums[j] += low(w) + high(w), most_q = fmaxf(most_q, fmaxf(fabsf(low(w)), fabsf(high(w))));
+                    for (const uint32_t w : {x.x, x.y, x.z, x.w}) most_q = fmaxf(most_q, fmaxf(fabsf(low(w)), fabsf(high(w))));
                 }
-                sums[j] += __shfl_xor_sync(0xffffffffu, sums[j], 1);
-                sums[j] += __shfl_xor_sync(0xffffffffu, sums[j], 2);
-            }
             most_q = fmaxf(most_q, __shfl_xor_sync(0xffffffffu, most_q, 1));
             most_q = fmaxf(most_q, __shfl_xor_sync(0xffffffffu, most_q, 2));
             const int exponent = (int)(__float_as_uint(most_q) >> 23);    // 2^(exponent - 127) is the largest query's size
             const float by = __uint_as_float((uint32_t)min(max(267 - exponent, 1), 253) << 23), unit = by * 0x1p-24f;      // a product is the sum over queries times codes in units of 2^24 / by
 #pragma unroll
-            for (int j = 0; j < G; ++j)
+            for (int j = 0; j < G; ++j) {
+                sums[j] = 0.f;                                            // (of queries times their power, so that large ones' is a number)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {                             // features 0 and 4, 1 and 5, 2 and 6, 3 and 7 of the eight
                     const uint4 x = v[j][h];
                     const float less = by * 0.0625f;
+                    for (const uint32_t w : {x.x, x.y, x.z, x.w}) sums[j] += low(w) * by + high(w) * by;
                     q[j][h][0] = half_bits(low(x.x) * by, low(x.z) * by);
                     q[j][h][1] = half_bits(high(x.x) * less, high(x.z) * less);
                     q[j][h][2] = half_bits(low(x.y) * by, low(x.w) * by);
                     q[j][h][3] = half_bits(high(x.y) * less, high(x.w) * less);
                 }
+                sums[j] += __shfl_xor_sync(0xffffffffu, sums[j], 1);
+                sums[j] += __shfl_xor_sync(0xffffffffu, sums[j], 2);
+            }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float u = __shfl_sync(0xffffffffu, unit, 8 * t + 4 * e);
 #pragma unroll
-                for (int j = 0; j < G; ++j) qs[j][e] = __shfl_sync(0xffffffffu, sums[j], 8 * t + 4 * e) * u;
-                scale[e] = fabsf(a.scale) * LOG2E / u;
+                for (int j = 0; j < G; ++j) qs[j][e] = __shfl_sync(0xffffffffu, sums[j], 8 * t + 4 * e) * 0x1p-24f;
+                // (queries from some 2^92 on: two scores that differ at all differ by more than any softmax sees at 2^100 as well, which keeps what it multiplies a number)
+                scale[e] = fminf(fabsf(a.scale) * LOG2E / u, 0x1p100f);
                 margin[e] = 8.f / scale[e];
             }
         }

@@ -128,3 +128,30 @@ def test_the_longest_row_that_may_come(dtype, nq, nkv, d, page, lengths):
         wide[:, :table.shape[1]] = table
         got = run(wide, longest)
         within(got, want, attention_bound(by_codes, by_values, want, dtype))
+
+
+@pytest.mark.parametrize("power", [60, 90, 100, 110, 118, 120, 122, 124, 125])
+@pytest.mark.parametrize("nq,nkv,d,page", [(4, 1, 128, 64), (8, 2, 64, 16), (4, 1, 256, 64)])
+def test_decode_of_queries_near_the_largest_numbers(nq, nkv, d, page, power):
+    """Scores of up to 2^127: every head has the value of its best place, wherever that is, as far as float32 scores tell it from the next (errors of 2^-18 of sum |q_f k_f|)."""
+    lengths = [900, 40, 0, 333]
+    q, kv, table, seq = decode_case(lengths, nq, nkv, d, page, BF16, seed=power)
+    q = (q.float().clamp(-3.9, 3.9) * 2.0 ** power).to(BF16)
+    got = ops().attention_decode4(q, kv, table, seq, 900, nq, nkv, d, page, d ** -0.5).view(-1, nq, d)
+    assert bool(torch.isfinite(got).all()) and bool((got[2] == 0).all())
+    seen = 0
+    for r, n in enumerate(lengths):
+        if not n:
+            continue
+        pages = table[r].long()[:-(-n // page)]
+        for h in range(nq):
+            k, v = (lo + s * c for c, s, lo in ([t.reshape(-1, d)[:n] for t in fb.read_rows(kv[pages, h // (nq // nkv), i], page, d, bool(i))] for i in range(2)))
+            x = q.view(-1, nq, d)[r, h].double()
+            e, error = k @ x, 2.0 ** -18 * (k.abs() @ x.abs()).max()
+            top = e.topk(2)
+            if float(top.values[0] - top.values[1]) > 2 * float(error):
+                seen += 1
+                want = v[top.indices[0]]
+                # the value through the second product: codes less the middle one, and its step, exact; the output's rounding and that of a weight of one
+                within(got[r, h], want, HALF[BF16] * want.abs() + 2.0 ** -7 * want.abs() + 2.0 ** -12 * v.abs().max())
+    assert seen >= nq * 3 // 2
