@@ -4,10 +4,11 @@
 //   q . k_j = sum_g step_jg (sum_f q_f c_jf) + low_jg sum_f q_f,
 //   o_f = sum_j (p_j step_jg) c_jf + sum_j p_j low_jg,
 // so codes go into tensor-core products as they are, 0..15, without a conversion.  Keys: four bits of a word, masked, are the half-precision number c 2^-24 (or 16 c 2^-24, which needs no shift either),
-// and products are exact; a head's queries are brought to 2^13 .. 2^14 by a power of two for it, so that they stay as they are.  Values: weights times steps may lie anywhere, which asks for bfloat16;
-// codes are numbers 16 + c there, and 24 is taken off at the end with sums of the weights as they were rounded, for low + 8 step is summed in float32 beside it: what the rounding of a weight moves is so
-// c - 8 times it, no more than the value is from its group's middle (one row of 23 places 2.0e-3 from 64 bits, of which the output's own rounding is 1.7e-3; 3.1e-3 with low alone).  Steps meet the sums
-// behind the products (keys) or the weights ahead of them (values).
+// and products are exact; a head's queries are brought to 2^13 .. 2^14 by a power of two for it, so that they stay as they are.  Values: weights times steps are
+// half-precision numbers too, steps times a power of two that brings the largest of them to 2^6 .. 2^7 (a warp's own, lowered where a larger one comes; weights are up to 2^8), so that a weight keeps eleven
+// bits down to 2^-28 of the largest: with bfloat16's eight the outputs were 1.8e-3 from 64 bits, where their own rounding is 1.6e-3.  Codes are numbers 16 + c there, and 24 is taken off at the end with sums
+// of the weights as they were rounded, for low + 8 step is summed in float32 beside it: what the rounding of a weight moves is so c - 8 times it, no more than the value is from its group's middle.  Steps
+// meet the sums behind the products (keys) or the weights ahead of them (values).
 #include "four.cuh"
 #include "mma.cuh"
 #include <algorithm>
@@ -127,11 +128,11 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
-// Codes i of the halves of a word as bfloat16 numbers 16 + code.  The values' sums are long ones, and tensor cores cut what they add to an accumulator off: what is taken off again at the end is to be
-// no more than it must (with 128 + code, for which i = 0 needs no shift, rows of 1,000 places and more were 2.2e-3 from 64 bits, rows of 100,000 more).
+// Codes i of the halves of a word as half-precision numbers 16 + code.  The values' sums are long ones, and tensor cores cut what they add to an accumulator off: what is taken off again at the end is to be
+// no more than it must (with 128 + code rows of 1,000 places and more were 2.2e-3 from 64 bits, rows of 100,000 more).
 __device__ __forceinline__ uint32_t pair16(uint32_t w, int i) {
     uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(i == 0 ? w << 3 : w >> (4 * i - 3)), "r"(0x00780078u), "r"(0x41804180u));
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(i < 2 ? w << (6 - 4 * i) : w >> (4 * i - 6)), "r"(0x03C003C0u), "r"(0x4C004C00u));
     return r;
 }
 __device__ __forceinline__ uint32_t half_bits(float x, float y) {
@@ -348,7 +349,11 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
                 for (int i = 0; i < 4; ++i) o[j][i][e] = 0.f;
             }
         }
-        const uint32_t one[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        const uint32_t one[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+        // the largest step's exponent so far, and the power of two for steps: its own is 2^6 (an exponent is one of 0 to 254, a power one of 2^-121 to 2^126)
+        uint32_t largest = 7;
+        auto power = [](uint32_t exponent) { return __uint_as_float((260u - exponent) << 23); };
+        float up = power(largest);
         // Masks only where a request ends, elsewhere they took a select a score and a step (8 rows of 8,192 places 26.0 us, 26.5 with them).  Heads above 128 keep one form: two are more code than short
         // rows fetch in time (heads of 256, 128 rows of 500 58 us, 65 with two).
         auto work = [&](auto whole, const unsigned char* tile, const int left) {
@@ -410,6 +415,29 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
                     for (int n = 0; n < 4; ++n) o[j][n][0] *= f0, o[j][n][1] *= f1, o[j][n][2] *= f0, o[j][n][3] *= f1;
                 }
             }
+            {
+                uint32_t steps[G], e = 0;                                 // of a place a lane
+                words_of<G>(tile + S::VALUE_HELD + lane * 4 * G, steps);
+#pragma unroll
+                for (int j = 0; j < G; ++j) {
+                    const uint32_t own = steps[j] >> 7 & 0xffu;
+                    if ((WHOLE || lane < left) && own < 255u) e = max(e, own);
+                }
+                e = __reduce_max_sync(0xffffffffu, e);
+                if (e > largest) {                                        // sums so far in units of the new power
+                    const float f = __uint_as_float(max(127 + (int)largest - (int)e, 0) << 23);
+                    largest = e;
+                    up = power(e);
+#pragma unroll
+                    for (int j = 0; j < G; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            ones[j][i] *= f;
+#pragma unroll
+                            for (int n = 0; n < 4; ++n) o[j][n][i] *= f;
+                        }
+                }
+            }
             const float z0 = most[0] == -INFINITY ? 0.f : most[0], z1 = most[1] == -INFINITY ? 0.f : most[1];      // (nobody has a score yet)
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt) {
@@ -435,9 +463,10 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
                     const float s0 = low(h0[j]), s1 = low(h1[j]), mid0 = fmaf(8.f, s0, high(h0[j])), mid1 = fmaf(8.f, s1, high(h1[j]));
                     mids[j][0] = fmaf(p[2], mid1, fmaf(p[0], mid0, mids[j][0]));
                     mids[j][1] = fmaf(p[3], mid1, fmaf(p[1], mid0, mids[j][1]));
-                    // weights times steps, rounded to bfloat16 as the second operand asks
-                    const uint32_t b0 = transposed(bits(__floats2bfloat162_rn(p[0] * s0, p[1] * s0))), b1 = transposed(bits(__floats2bfloat162_rn(p[2] * s1, p[3] * s1)));
-                    mma16::mma_bf16(ones[j], one, b0, b1);
+                    // weights times steps, rounded to half precision as the second operand asks
+                    const float up0 = s0 * up, up1 = s1 * up;
+                    const uint32_t b0 = transposed(half_bits(p[0] * up0, p[1] * up0)), b1 = transposed(half_bits(p[2] * up1, p[3] * up1));
+                    mma_half(ones[j], one, b0, b1);
                     const uint32_t x0 = __byte_perm(w[0][j], w[1][j], 0x5410), x1 = __byte_perm(w[0][j], w[1][j], 0x7632);
                     const uint32_t y0 = __byte_perm(w[2][j], w[3][j], 0x5410), y1 = __byte_perm(w[2][j], w[3][j], 0x7632);
 #pragma unroll
@@ -445,7 +474,7 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
                         const uint32_t x = n < 2 ? x0 : x1, y = n < 2 ? y0 : y1;
                         const int i0 = 2 * (n & 1);
                         const uint32_t av[4] = {pair16(x, i0), pair16(x, i0 + 1), pair16(y, i0), pair16(y, i0 + 1)};
-                        mma16::mma_bf16(o[j][n], av, b0, b1);
+                        mma_half(o[j][n], av, b0, b1);
                     }
                 }
             }
@@ -479,10 +508,12 @@ __global__ void __launch_bounds__(32 * W, blocks_a_sm(D, W)) decode_mma_kernel(c
 #pragma unroll
             for (int j = 0; j < G; ++j) {                                 // features 64 j + 8 g + (0..7)
                 float4* to = reinterpret_cast<float4*>(o_s + (warp * HEADS + h) * LD + 64 * j + 8 * g);
+                auto less = [&](float v) { return fmaf(-24.f, ones[j][e], v); };
+                const float down = __uint_as_float((largest - 6u) << 23);      // what `up` undoes
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    to[i] = make_float4(fmaf(-24.f, ones[j][e], o[j][2 * i][e] + mids[j][e]), fmaf(-24.f, ones[j][e], o[j][2 * i][e + 2] + mids[j][e]),
-                                        fmaf(-24.f, ones[j][e], o[j][2 * i + 1][e] + mids[j][e]), fmaf(-24.f, ones[j][e], o[j][2 * i + 1][e + 2] + mids[j][e]));
+                    to[i] = make_float4(fmaf(less(o[j][2 * i][e]), down, mids[j][e]), fmaf(less(o[j][2 * i][e + 2]), down, mids[j][e]), fmaf(less(o[j][2 * i + 1][e]), down, mids[j][e]),
+                                        fmaf(less(o[j][2 * i + 1][e + 2]), down, mids[j][e]));
             }
         }
         __syncthreads();

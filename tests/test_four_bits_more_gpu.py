@@ -155,3 +155,52 @@ def test_decode_of_queries_near_the_largest_numbers(nq, nkv, d, page, power):
                 # the value through the second product: codes less the middle one, and its step, exact; the output's rounding and that of a weight of one
                 within(got[r, h], want, HALF[BF16] * want.abs() + 2.0 ** -7 * want.abs() + 2.0 ** -12 * v.abs().max())
     assert seen >= nq * 3 // 2
+
+
+# ---- weights times steps in half precision ----
+
+def decode_bound(by_codes, by_values, want, largest):
+    """A weight times a step rounded to half precision moves c - 8 of it (2^-11), a subnormal one (2^-24 where the largest is 2^6 or more; codes are up to 31 there, and a row's weights 2^13 at most together,
+    its largest being 2^8) no more than 2^-14 of the largest value altogether; float32 sums 2^-12; the output's rounding."""
+    return 2.0 ** -11 * by_codes + HALF[BF16] * want.abs() + 2.0 ** -12 * by_values + 2.0 ** -14 * largest + 1e-30
+
+
+@pytest.mark.parametrize("nq,nkv,d,page", [(8, 2, 128, 64), (4, 4, 64, 16), (16, 1, 128, 16), (24, 2, 64, 128), (6, 1, 192, 32), (4, 1, 256, 64)])
+@pytest.mark.parametrize("lengths", [[1], [23], [63, 64, 65], [300, 0, 1, 16, 257], [2500], [100] * 70])
+def test_decode_is_as_near_as_its_outputs_rounding(nq, nkv, d, page, lengths):
+    """All outputs together: no further off than the 64-bit ones' own rounding to bfloat16, r of their norm, and what weights in half precision add, 2^-11 at most and independent of it: sqrt(r^2 + 2^-22),
+    a twentieth more for the rounding of numbers that are a little off.  (r itself is 1.6e-3 as a rule and is taken from the numbers: a row of one place has each of its values in all of its heads, and 128
+    numbers twelve times over have r = 2.2e-3.  Weights in bfloat16 would add 1.6e-3 to long rows.)"""
+    q, kv, table, seq = decode_case(lengths, nq, nkv, d, page, BF16, seed=3, lean=0.0)
+    want, by_codes, by_values = fb.attention(q, kv, table, [(1 if n else 0, n - 1 if n else 0) for n in lengths], nq, nkv, d, page, d ** -0.5)
+    got = ops().attention_decode4(q, kv, table, seq, max(lengths), nq, nkv, d, page, d ** -0.5)
+    within(got, want, decode_bound(by_codes, by_values, want, 0.0 * want))
+    r = float((want.to(BF16).double() - want).norm())
+    assert float((got.double() - want).norm()) <= 1.05 * (r ** 2 + 2.0 ** -22 * float(want.norm()) ** 2) ** 0.5 + 1e-30
+
+
+@pytest.mark.parametrize("nq,nkv,d,page", [(8, 2, 128, 64), (4, 4, 64, 16), (4, 1, 256, 64)])
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed"])
+@pytest.mark.parametrize("low,high", [(-12, 12), (-60, 60), (-110, -90), (60, 110)])
+def test_decode_over_values_of_all_sizes(nq, nkv, d, page, order, low, high):
+    """Values whose sizes grow along the row, so that the power of two for steps is lowered again and again, or fall, or jump: sums so far follow, and nothing overflows."""
+    n = 1300
+    q, kv, table, seq = decode_case([n], nq, nkv, d, page, BF16, seed=9, lean=0.0)
+    power = torch.linspace(low, high, n).round()
+    power = power if order == "rising" else power.flip(0) if order == "falling" else power[torch.randperm(n, generator=torch.Generator().manual_seed(1))]
+    held = kv[:, :, 1, page * d // 2:].contiguous().view(BF16).view(-1, nkv, page, d // 64, 2)
+    for j in range(n):
+        held[table[0, j // page].long(), :, j % page] *= 2.0 ** float(power[j])
+    kv[:, :, 1, page * d // 2:] = held.reshape(-1, nkv, page * d // 32).view(torch.uint8).view(-1, nkv, page * d // 16)
+    want, by_codes, by_values = fb.attention(q, kv, table, [(1, n - 1)], nq, nkv, d, page, d ** -0.5)
+    largest = torch.full_like(want, 0.0)
+    pages = table[0].long()[:-(-n // page)]
+    for kvh in range(nkv):
+        c, s, lo = (t.reshape(-1, d)[:n] for t in fb.read_rows(kv[pages, kvh, 1], page, d, True))
+        v = (lo + s * c).abs().amax()
+        largest.view(-1, nq, d)[:, kvh * (nq // nkv):(kvh + 1) * (nq // nkv)] = v / n
+    for longest in (n, 8192):
+        wide = torch.zeros(1, -(-longest // page), dtype=torch.int32, device=DEV)
+        wide[:, :table.shape[1]] = table
+        got = ops().attention_decode4(q, kv, wide, seq, longest, nq, nkv, d, page, d ** -0.5)
+        within(got, want, decode_bound(by_codes, by_values, want, largest))
