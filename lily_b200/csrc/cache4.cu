@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(32 * WRITE_WARPS) write_turned_kernel(const Wr
 // that portions of prompts see, one request's behind the other's, [pages, 2, nkv, page_size, d], with a block table of them and zeros behind a request's last place.
 // Eight threads a place and kind, each with the words that lie side by side, one a group.  ``spans`` [2 (keys, values), requests, nkv]: half-precision numbers times powers of two (attention_args.cuh).
 // grid (pages, requests, kv heads x 2)
-template <typename T, int G>
+template <typename T, int G, bool HALVES>
 __global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__ kv, int pages, const int* __restrict__ block_table, int width, T* __restrict__ out, int nkv, int page_size,
                                                      const int* __restrict__ cu, const int* __restrict__ prefix, int* __restrict__ table_out, int table_width, int most_pages, const unsigned* __restrict__ spans) {
     constexpr int D = G * GROUP;
@@ -313,8 +313,7 @@ __global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__
     const uint32_t *words = reinterpret_cast<const uint32_t*>(rows), *held = reinterpret_cast<const uint32_t*>(rows + (size_t)page_size * (D / 2));
     T* dst = out + ((to * 2 + value) * nkv + head) * ((size_t)page_size * D);
     const int i8 = threadIdx.x & 7;
-    const bool halves = sizeof(T) == 2 && spans;
-    const float by = halves ? span_multiplier(spans[((size_t)value * gridDim.y + r) * nkv + head]) : 1.f;
+    const float by = HALVES ? span_multiplier(spans[((size_t)value * gridDim.y + r) * nkv + head]) : 1.f;
 #pragma unroll 2
     for (int slot = threadIdx.x >> 3; slot < page_size; slot += 32) {
         uint32_t w[G], h[G];
@@ -328,7 +327,7 @@ __global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__
             float v[8];
 #pragma unroll
             for (int c = 0; c < 8; ++c) v[c] = slot < places ? fmaf(__uint_as_float((w[e] >> (4 * c) & 15u) | 0x4B000000u) - 8388608.f, low(of), high(of)) : 0.f;
-            if (halves) store_halves(dst + (size_t)slot * D + l * 8, v, by);
+            if (HALVES) store_halves(dst + (size_t)slot * D + l * 8, v, by);
             else store8(dst + (size_t)slot * D + l * 8, v);
         }
     }
@@ -465,17 +464,19 @@ LILY_API int lily_cache4_values(const void* kv, int pages, const int* block_tabl
     LILY_REQUIRE(((uintptr_t)kv | (uintptr_t)out) % 16 == 0, "cache4_values: tensors on boundaries of sixteen bytes");
     const dim3 grid(cu ? table_width : width, requests, 2 * nkv);
     if (grid.x == 0) return 0;
-#define VALUES(T, G) \
-    launch_pdl(four::values_kernel<T, G>, grid, dim3(256), 0, stream, (const uint8_t*)kv, pages, block_table, width, (T*)out, nkv, page_size, cu, prefix, table_out, table_width, most_pages, spans)
-#define VALUES_OF(T)                 \
-    do {                             \
-        if (d == 64) VALUES(T, 1);   \
-        else if (d == 128) VALUES(T, 2); \
-        else if (d == 192) VALUES(T, 3); \
-        else VALUES(T, 4);           \
+#define VALUES(T, G, HALVES) \
+    launch_pdl(four::values_kernel<T, G, HALVES>, grid, dim3(256), 0, stream, (const uint8_t*)kv, pages, block_table, width, (T*)out, nkv, page_size, cu, prefix, table_out, table_width, most_pages, spans)
+#define VALUES_OF(T, HALVES)                 \
+    do {                                     \
+        if (d == 64) VALUES(T, 1, HALVES);   \
+        else if (d == 128) VALUES(T, 2, HALVES); \
+        else if (d == 192) VALUES(T, 3, HALVES); \
+        else VALUES(T, 4, HALVES);           \
     } while (0)
-    if (dtype == kF32) VALUES_OF(float);
-    else VALUES_OF(__nv_bfloat16);
+    LILY_REQUIRE(!spans || dtype == kBF16, "cache4_values: numbers in half precision lie where bfloat16 ones would");
+    if (dtype == kF32) VALUES_OF(float, false);
+    else if (spans) VALUES_OF(__nv_bfloat16, true);
+    else VALUES_OF(__nv_bfloat16, false);
 #undef VALUES_OF
 #undef VALUES
     LILY_CHECK_LAUNCH("cache4_values");
