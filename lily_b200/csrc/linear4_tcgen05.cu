@@ -58,12 +58,12 @@ __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
 }
 struct Waits { volatile int* lost; int* word; int polls; };
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, const Waits& w, int code) {
-    bool come = false;
-    for (int i = 0; i < w.polls && !come; ++i) {
-        come = try_wait(bar, parity);
+    bool come = try_wait(bar, parity);
+    for (int i = 1; !come && i < w.polls; ++i) {
         if ((i & 15) == 15 && *w.lost) break;
+        come = try_wait(bar, parity);
     }
-    come = __all_sync(0xffffffffu, come);                // (the whole warp goes on, or none of it)
+    come = __all_sync(0xffffffffu, come && w.polls > 0);      // (the whole warp goes on, or none of it)
     if (!come && !*w.lost) {
         *w.lost = 1;
         *(volatile int*)w.word = (code << 24) | (int)((blockIdx.x + blockIdx.y * gridDim.x) & 0xFFFFFF);
