@@ -1441,7 +1441,8 @@ def linear4_few_tokens(dtype: torch.dtype) -> int:
 
 
 def linear4(x: torch.Tensor, w: Weight4, bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    """``x [M, K] . W^T (+ bias)`` [M, N] for a matrix held in four bits, in the dtype of ``x`` (or float32: ``out_dtype``)."""
+    """``x [M, K] . W^T (+ bias)`` [M, N] for a matrix held in four bits, in the dtype of ``x`` (or float32: ``out_dtype``).  Weights are exact for up to ``linear4_few_tokens`` tokens and in float32, and rounded
+    once to bfloat16 for more tokens of that dtype."""
     if out_dtype not in (None, x.dtype, torch.float32):
         raise KernelError(f"linear4: the result is {x.dtype} or float32, not {out_dtype}")
     few = linear4_few_tokens(x.dtype)
@@ -1522,7 +1523,7 @@ def attention_prefill4(q: torch.Tensor, kv_layer: torch.Tensor, block_table: tor
                        plan: Optional[Prefill4Plan] = None) -> torch.Tensor:
     """Causal attention of prompt portions over a cache held in four bits: each request's new tokens (rows ``cu_seqlens`` of ``q`` [tokens, nq * d]) over its cached prefix and themselves, whose keys are in
     the cache already.  ``h_prefix_lens``, ``h_new_lens``: the lengths on the host, by which the work is cut (``plan``: ``plan_prefill4`` of them, made here where not given).  The pages that the
-    portions see are brought to numbers first, and the kernels of ``attention_prefill`` read those: float32, or half precision, whose bits hold them, as are the queries and the softmax's weights then (bfloat16 where neither tensor-core kernel takes the pages).  Rows of ``out`` that no portion has stay as they are."""
+    portions see are brought to numbers first, and the kernels of ``attention_prefill`` read those: float32, or half precision, whose bits hold them, as are the queries and the softmax's weights then (bfloat16 where neither tensor-core kernel takes the pages); keys or values of a request and kv head lose bits beside one 2^28 times as large.  Rows of ``out`` that no portion has stay as they are."""
     tokens, face = sum(h_new_lens), _module or _faces()
     rows = prefill_tile_rows(q.dtype, d, page_size, tokens)
     # (the tensor-core kernels; others, of float32 and of pages that are no power of two, read the numbers themselves)
