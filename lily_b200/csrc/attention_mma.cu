@@ -539,9 +539,10 @@ attention_mma_kernel(const AttnArgs a, const int page_shift, const __grid_consta
     const float sl2 = (cap > 0.f ? 1.f : a.scale) * 1.4426950408889634f;
     float sl2_lo = sl2, sl2_hi = sl2;                   // of this thread's two rows
     if constexpr (HALF) {
+        // (rows that the tile has not take its last one's power; token 0's where the request has none on the device)
         const unsigned keys = a.spans[(size_t)req * a.nkv + head0 / (a.nq / a.nkv)];
-        sl2_lo = span_scale(sl2, a.units[((size_t)tok0 + min(row_lo, nrows - 1)) * a.nq + head0], keys);
-        sl2_hi = span_scale(sl2, a.units[((size_t)tok0 + min(row_hi, nrows - 1)) * a.nq + head0], keys);
+        sl2_lo = span_scale(sl2, a.units[(size_t)max(tok0 + min(row_lo, nrows - 1), 0) * a.nq + head0], keys);
+        sl2_hi = span_scale(sl2, a.units[(size_t)max(tok0 + min(row_hi, nrows - 1), 0) * a.nq + head0], keys);
     }
     auto tanh_fast = [](float v) { float r; asm("tanh.approx.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; };
 

@@ -112,7 +112,7 @@ struct Params {
     const float* units;                   // and of the queries
     float cap, cap_in;                    // cap > 0: scores become cap * tanh(score * cap_in), cap_in = scale / cap
 };
-// What a row's scores are multiplied by in units of log2.
+// What a row's scores are multiplied by in units of log2.  (`token`: rows that the tile has not take its last one's; 0 where the request has none on the device.)
 template <bool HALF>
 __device__ __forceinline__ float row_scale(const Params& p, int req, int token, int head) {
     if (!HALF) return p.scale_log2;
@@ -333,7 +333,7 @@ attention_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         const int row = quarter * 32 + lane;
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
         const int pos = pos0 + row;
-        const float scale_log2 = row_scale<HALF>(p, req, q_begin + start + min(row, rows_valid - 1), head), unit = HALF ? span_unit(p.value_spans[(size_t)req * p.nkv + head / (p.nq / p.nkv)]) : 1.f;
+        const float scale_log2 = row_scale<HALF>(p, req, max(q_begin + start + min(row, rows_valid - 1), 0), head), unit = HALF ? span_unit(p.value_spans[(size_t)req * p.nkv + head / (p.nq / p.nkv)]) : 1.f;
         float m_used = p.sink ? 0.f : -INFINITY, l = 0.f;
         bool ok = true;
         // The threads of a row hand each other one float per tile (the maximum of their keys; at the end
@@ -740,7 +740,7 @@ attention_prefill_tc2_kernel(const __grid_constant__ CUtensorMap map_q, const __
         const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
         const uint32_t my_s = tmem + lane_addr + (uint32_t)(h * BKV), my_o = tmem_o + lane_addr + (uint32_t)(h * D);
         const int pos = pos0 + row;
-        const float scale_log2 = row_scale<HALF>(p, req, q_begin + start + min(row, rows_valid - 1), head0 + h), unit = HALF ? span_unit(p.value_spans[(size_t)req * p.nkv + head0 / (p.nq / p.nkv)]) : 1.f;
+        const float scale_log2 = row_scale<HALF>(p, req, max(q_begin + start + min(row, rows_valid - 1), 0), head0 + h), unit = HALF ? span_unit(p.value_spans[(size_t)req * p.nkv + head0 / (p.nq / p.nkv)]) : 1.f;
         float m_used = p.sink ? 0.f : -INFINITY, l = 0.f;
         bool ok = true;
         for (int j = 0; j < n && ok; ++j) {

@@ -1522,7 +1522,7 @@ def attention_prefill4(q: torch.Tensor, kv_layer: torch.Tensor, block_table: tor
                        h_new_lens: Sequence[int], nq: int, nkv: int, d: int, page_size: int, scale: float, out: Optional[torch.Tensor] = None,
                        plan: Optional[Prefill4Plan] = None) -> torch.Tensor:
     """Causal attention of prompt portions over a cache held in four bits: each request's new tokens (rows ``cu_seqlens`` of ``q`` [tokens, nq * d]) over its cached prefix and themselves, whose keys are in
-    the cache already.  ``h_prefix_lens``, ``h_new_lens``: the lengths on the host, by which the work is cut (``plan``: ``plan_prefill4`` of them, made here where not given).  The pages that the
+    the cache already.  ``h_prefix_lens``, ``h_new_lens``: the lengths on the host, by which the work is cut (``plan``: ``plan_prefill4`` of them, made here where not given); those on the device may be shorter, not longer.  The pages that the
     portions see are brought to numbers first, and the kernels of ``attention_prefill`` read those: float32, or half precision, whose bits hold them, as are the queries and the softmax's weights then (bfloat16 where neither tensor-core kernel takes the pages); keys or values of a request and kv head lose bits beside one 2^28 times as large.  Rows of ``out`` that no portion has stay as they are."""
     tokens, face = sum(h_new_lens), _module or _faces()
     rows = prefill_tile_rows(q.dtype, d, page_size, tokens)

@@ -71,3 +71,20 @@ def test_large_scores(nq, nkv, d, page, new):
         assert int(sure.sum()) > new // 8
         near = (got[sure, h].double() - v[top.indices[sure, 0]]).abs() - (2.0 ** -8 + 2.0 ** -10) * v[top.indices[sure, 0]].abs()
         assert bool((near <= 1e-30).all())
+
+
+@pytest.mark.parametrize("nq,nkv,d,page,new", [(8, 2, 128, 64, [300, 700, 260]), (6, 2, 128, 16, [70, 130, 9]), (4, 4, 64, 64, [900, 40, 300])])
+def test_portions_that_are_shorter_on_the_device(nq, nkv, d, page, new):
+    """A call that is cut for longer portions than there are, as a captured one may be when it is replayed: tiles without rows write nothing, a request without tokens takes nothing from the others, and rows
+    behind the last one stay as they are."""
+    for short in ([0, *new[1:]], [1, max(new[1] - 50, 2), 0], [new[0], 0, 0], [0, 0, 5]):
+        cached = [0, 30, 65]
+        _, kv, table, _ = decode_case([p + n for p, n in zip(cached, new)], nq, nkv, d, page, BF16, seed=12, lean=0.0)
+        q = torch.randn(sum(new), nq * d, generator=torch.Generator().manual_seed(13)).to(BF16).to(DEV)
+        tensors = lambda lens: (torch.tensor([0, *torch.tensor(lens).cumsum(0).tolist()], dtype=torch.int32, device=DEV), torch.tensor(cached, dtype=torch.int32, device=DEV))
+        out = torch.full_like(q, 7.0)
+        ops().attention_prefill4(q, kv, table, *tensors(short), cached, new, nq, nkv, d, page, d ** -0.5, out)
+        torch.cuda.synchronize()
+        want, bound = fp.want(q, kv, table, list(zip(short, cached)), nq, nkv, d, page, d ** -0.5)
+        n = sum(short)
+        assert bool(((out[:n].double() - want[:n]).abs() <= bound[:n]).all()) and bool((out[n:] == 7.0).all())
